@@ -622,6 +622,70 @@ int vdsl_op_gemm_w8a8_packed_noalloc(vdsl_queue q, int64_t M, int64_t N, int64_t
                                      vdsl_buffer y, int32_t out_dtype, int32_t relu,
                                      vdsl_buffer acc_out);
 
+/* ========================================================================================== */
+/* Op class 6: what makes an MLP a model of tokens (no reference code): the embedding, layer  */
+/* norm between residual blocks, and the output layer with its cross entropy.                 */
+/* ========================================================================================== */
+/* out[i] = scale * table[ids[i]] (one f32 product per element, rounded once); zeros where ids[i] is
+ * outside [0, vocab).  table: F32 or BF16 [vocab][dim]; ids: I32 [n]; out: F32 or BF16 [n][dim]. */
+int vdsl_op_embedding_fwd(vdsl_queue q, int64_t n, int64_t dim, int64_t vocab, int32_t table_dtype,
+                          vdsl_buffer table, vdsl_buffer ids, float scale, int32_t out_dtype,
+                          vdsl_buffer out);
+/* The table's gradient: dtable[v] (F32 [vocab][dim], every row written) = scale * the f32 sum of dy[i]
+ * (F32 or BF16 [n][dim]) over the i with ids[i] = v, 0 where there is none; ids outside [0, vocab) add
+ * to nothing.  The same bits on every call.  workspace: vdsl_embedding_bwd_workspace_bytes() bytes of
+ * any contents (two calls that overlap in time need two); it may be NULL when that is 0. */
+int vdsl_embedding_bwd_workspace_bytes(int64_t n, int64_t vocab, int64_t dim, size_t* bytes);
+int vdsl_op_embedding_bwd(vdsl_queue q, int64_t n, int64_t dim, int64_t vocab, vdsl_buffer ids,
+                          int32_t dy_dtype, vdsl_buffer dy, float scale, vdsl_buffer dtable,
+                          vdsl_buffer workspace);
+
+/* Layer norm of each row: h = (x - mean) * rstd with mean = sum(x) / cols and
+ * rstd = 1 / sqrt(sum((x - mean)^2) / cols + eps), y = h * gamma + beta, all in f32, y rounded once.
+ * x, y: F32 or BF16 [rows][cols] (y may be x when the types agree); gamma, beta: F32 or BF16 [cols],
+ * of one type param_dtype, NULL for 1 and 0; mean, rstd: F32 [rows] for the backward pass, or NULL. */
+int vdsl_op_layer_norm_fwd(vdsl_queue q, int64_t rows, int64_t cols, int32_t x_dtype, vdsl_buffer x,
+                           int32_t param_dtype, vdsl_buffer gamma, vdsl_buffer beta, float eps,
+                           int32_t y_dtype, vdsl_buffer y, vdsl_buffer mean, vdsl_buffer rstd);
+/* Its backward pass from x and the forward pass's mean and rstd: with g = dy * gamma,
+ * dx = rstd * (g - mean(g) - h * mean(g * h)), dgamma = sum over rows of dy * h, dbeta = sum over rows
+ * of dy.  dy, x, dx: F32 or BF16 [rows][cols] (dx may be dy when the types agree); gamma as above, or
+ * NULL; dgamma, dbeta: F32 [cols], each may be NULL.  The same bits on every call.  workspace:
+ * vdsl_layer_norm_bwd_workspace_bytes() bytes of any contents (two calls that overlap in time need two);
+ * it may be NULL when dgamma and dbeta both are. */
+int vdsl_layer_norm_bwd_workspace_bytes(int64_t rows, int64_t cols, size_t* bytes);
+int vdsl_op_layer_norm_bwd(vdsl_queue q, int64_t rows, int64_t cols, int32_t dy_dtype, vdsl_buffer dy,
+                           int32_t x_dtype, vdsl_buffer x, int32_t param_dtype, vdsl_buffer gamma,
+                           vdsl_buffer mean, vdsl_buffer rstd, int32_t dx_dtype, vdsl_buffer dx,
+                           vdsl_buffer dgamma, vdsl_buffer dbeta, vdsl_buffer workspace);
+
+/* The output layer over a vocabulary with its softmax cross entropy: z = x w^T (x BF16 [n][dim],
+ * w BF16 [vocab][dim], f32 accumulate, never stored), lse[i] = log sum_v exp(z[i][v]),
+ * row_loss[i] = lse[i] - z[i][labels[i]], 0 where labels[i] (I32 [n]) is outside [0, vocab): such a row
+ * does not count; loss (F32 [1]) = sum of row_loss / number of rows that count (0 if none does).
+ * row_loss, lse: F32 [n], each may be NULL.  dim >= 8.  A row whose logits hold a NaN or +inf has a NaN
+ * lse and loss.  workspace: vdsl_linear_xent_workspace_bytes(n, vocab, dim, 0, 0) bytes. */
+int vdsl_linear_xent_workspace_bytes(int64_t n, int64_t vocab, int64_t dim, int64_t piece,
+                                     int32_t backward, size_t* bytes);
+int vdsl_op_linear_xent_fwd(vdsl_queue q, int64_t n, int64_t dim, int64_t vocab, vdsl_buffer x,
+                            vdsl_buffer w, vdsl_buffer labels, vdsl_buffer loss, vdsl_buffer row_loss,
+                            vdsl_buffer lse, vdsl_buffer workspace);
+/* The same with the gradients of grad_scale * loss: G = softmax(z) - onehot(label) (0 for a row that
+ * does not count), dx (F32 or BF16 [n][dim]) = grad_scale / count * G w and dw (F32 or BF16
+ * [vocab][dim], every row written) = grad_scale / count * G^T x.  G is rounded to bf16 for these products,
+ * as every gradient that a bf16 GEMM of this library takes; they accumulate in f32 and are rounded once.
+ * The vocabulary is worked on in pieces of `piece` columns (rounded up to a multiple of 256, the pieces
+ * then made alike): the workspace holds 2 n piece bytes for one of them, and more pieces take more
+ * operations (all but one form their logits twice).  piece 0: as many columns as 2 n piece <= 1 GiB allows.
+ * The same bits on every call with the same piece.  workspace:
+ * vdsl_linear_xent_workspace_bytes(n, vocab, dim, piece, 1) bytes of any contents (two calls that overlap
+ * in time need two). */
+int vdsl_op_linear_xent_fwd_bwd(vdsl_queue q, int64_t n, int64_t dim, int64_t vocab, vdsl_buffer x,
+                                vdsl_buffer w, vdsl_buffer labels, int64_t piece, float grad_scale,
+                                vdsl_buffer loss, vdsl_buffer row_loss, vdsl_buffer lse,
+                                int32_t dx_dtype, vdsl_buffer dx, int32_t dw_dtype, vdsl_buffer dw,
+                                vdsl_buffer workspace);
+
 /* ---- failure injection (tests of error paths, host-side only) ----------------------------- */
 /* After `n` more successful buffer allocations, the next one fails with VDSL_ERR_OUT_OF_MEMORY
  * (n < 0 disables).  While n is 0, queues and recordings get no scratch memory either (which fails

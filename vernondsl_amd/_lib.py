@@ -163,6 +163,17 @@ PROTOTYPES = {
     "vdsl_op_pack_w8a8_weights": (C.c_int, [_vp, _i64, _i64, _vp, _vp]),
     "vdsl_gemm_w8a8_packed_workspace_bytes": (C.c_int, [_i64, _i64, _i64, C.POINTER(_sz)]),
     "vdsl_op_gemm_w8a8_packed": (C.c_int, [_vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _vp, _vp]),
+    "vdsl_op_embedding_fwd": (C.c_int, [_vp, _i64, _i64, _i64, _i32, _vp, _vp, C.c_float, _i32, _vp]),
+    "vdsl_embedding_bwd_workspace_bytes": (C.c_int, [_i64, _i64, _i64, C.POINTER(_sz)]),
+    "vdsl_op_embedding_bwd": (C.c_int, [_vp, _i64, _i64, _i64, _vp, _i32, _vp, C.c_float, _vp, _vp]),
+    "vdsl_op_layer_norm_fwd": (C.c_int, [_vp, _i64, _i64, _i32, _vp, _i32, _vp, _vp, C.c_float, _i32, _vp, _vp, _vp]),
+    "vdsl_layer_norm_bwd_workspace_bytes": (C.c_int, [_i64, _i64, C.POINTER(_sz)]),
+    "vdsl_op_layer_norm_bwd": (C.c_int, [_vp, _i64, _i64, _i32, _vp, _i32, _vp, _i32, _vp, _vp, _vp, _i32, _vp, _vp, _vp,
+                                         _vp]),
+    "vdsl_linear_xent_workspace_bytes": (C.c_int, [_i64, _i64, _i64, _i64, _i32, C.POINTER(_sz)]),
+    "vdsl_op_linear_xent_fwd": (C.c_int, [_vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "vdsl_op_linear_xent_fwd_bwd": (C.c_int, [_vp, _i64, _i64, _i64, _vp, _vp, _vp, _i64, C.c_float, _vp, _vp, _vp, _i32, _vp,
+                                              _i32, _vp, _vp]),
     "vdsl_debug_fail_alloc_after": (C.c_int, [_i64]),
     "vdsl_debug_gemm_config": (C.c_int, [_i32]),
     "vdsl_debug_w8a8_packed_plan": (C.c_int, [_i32, _i32]),

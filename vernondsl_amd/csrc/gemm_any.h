@@ -50,21 +50,22 @@ struct AnyOperand {
   int k_of[C];         // the chunk's first K value within a stage
   int lds[C];
 
-  __device__ __forceinline__ AnyOperand(const uint16_t* p, int rows, int K, int r0) {
+  // ld: elements from one stored row to the next; the tensor is allocated in whole stored rows.
+  __device__ __forceinline__ AnyOperand(const uint16_t* p, int rows, int K, int r0, int64_t ld) {
     base = reinterpret_cast<const char*>(p);
-    size = static_cast<int64_t>(rows) * K;
+    size = (KM ? K : rows) * ld;
     last = size - 8;
-    kstep = KM ? rows : 1;
+    kstep = KM ? ld : 1;
 #pragma unroll
     for (int i = 0; i < C; ++i) {
       const int c = static_cast<int>(threadIdx.x) + NT * i, row = c / CPR, chunk = c % CPR;
       lds[i] = row * LDS_ROW + chunk * 16;
       if constexpr (KM) {
         k_of[i] = row;
-        at[i] = static_cast<int64_t>(row) * rows + (r0 + 8 * chunk < rows ? r0 + 8 * chunk : 0);
+        at[i] = row * ld + (r0 + 8 * chunk < rows ? r0 + 8 * chunk : 0);
       } else {
         k_of[i] = 8 * chunk;
-        at[i] = static_cast<int64_t>(r0 + row < rows ? r0 + row : rows - 1) * K + 8 * chunk;
+        at[i] = (r0 + row < rows ? r0 + row : rows - 1) * ld + 8 * chunk;
       }
     }
   }
@@ -109,14 +110,16 @@ __device__ __forceinline__ bf16x8 any_fragment(const char* area, int row0, int f
   }
 }
 
+// lda, ldb: elements between stored rows (negative: dense).
 template <class Cfg>
 __device__ __forceinline__ void any_mainloop(const uint16_t* __restrict__ A, const uint16_t* __restrict__ B, int M, int N, int K,
-                                             int m0, int n0, char* smem, f32x16 (&acc)[Cfg::FM][Cfg::FN]) {
+                                             int m0, int n0, char* smem, f32x16 (&acc)[Cfg::FM][Cfg::FN], int64_t lda = -1,
+                                             int64_t ldb = -1) {
   constexpr int FM = Cfg::FM, FN = Cfg::FN;
   const int wave = threadIdx.x >> 6;
   const int wr = (wave / Cfg::WGN) * Cfg::WTM, wc = (wave % Cfg::WGN) * Cfg::WTN;
-  const AnyOperand<Cfg::AKM, Cfg::BM, Cfg::NT, Cfg::CA, Cfg::A_ROW> a(A, M, K, m0);
-  const AnyOperand<Cfg::BKM, Cfg::BN, Cfg::NT, Cfg::CB, Cfg::B_ROW> b(B, N, K, n0);
+  const AnyOperand<Cfg::AKM, Cfg::BM, Cfg::NT, Cfg::CA, Cfg::A_ROW> a(A, M, K, m0, lda < 0 ? (Cfg::AKM ? M : K) : lda);
+  const AnyOperand<Cfg::BKM, Cfg::BN, Cfg::NT, Cfg::CB, Cfg::B_ROW> b(B, N, K, n0, ldb < 0 ? (Cfg::BKM ? N : K) : ldb);
 #pragma unroll
   for (int i = 0; i < FM; ++i)
 #pragma unroll

@@ -394,3 +394,122 @@ def gemm_w8a8_packed_noalloc(q: Queue, xq: Tensor, x_scale: Tensor, wp: Tensor, 
     _expect(acc_out, (M, N), "i32", "acc_out")
     call("vdsl_op_gemm_w8a8_packed_noalloc", q.handle, M, N, K, xq.handle, x_scale.handle, wp.handle,
          w_scale.handle, y.handle, y.dtype, int(bool(relu)), _h(acc_out))
+
+
+# ---- op class 6: what makes an MLP a model of tokens -------------------------------------------------
+def embedding_fwd(q: Queue, table: Tensor, ids: Tensor, out: Tensor, scale: float = 1.0):
+    """out [n][dim] = scale * table [vocab][dim][ids[i]] (f32 or bf16 each; ids i32 [n]); zeros where an
+    id is outside the table."""
+    vocab, dim = table.shape
+    (n,) = ids.shape
+    _expect(ids, (n,), "i32", "ids")
+    if out.shape != (n, dim):
+        raise ValueError(f"out: shape {out.shape}, expected {(n, dim)}")
+    call("vdsl_op_embedding_fwd", q.handle, n, dim, vocab, table.dtype, table.handle, ids.handle, scale, out.dtype, out.handle)
+
+
+def embedding_bwd_workspace_bytes(n, vocab, dim) -> int:
+    b = C.c_size_t()
+    call("vdsl_embedding_bwd_workspace_bytes", n, vocab, dim, C.byref(b))
+    return b.value
+
+
+def embedding_bwd(q: Queue, ids: Tensor, dy: Tensor, dtable: Tensor, scale: float = 1.0, workspace=None):
+    """dtable (f32 [vocab][dim], every row written) = scale * the sum of dy [n][dim] over each row's tokens.
+    workspace: embedding_bwd_workspace_bytes(n, vocab, dim) bytes."""
+    vocab, dim = dtable.shape
+    (n,) = ids.shape
+    _expect(ids, (n,), "i32", "ids")
+    if dy.shape != (n, dim):
+        raise ValueError(f"dy: shape {dy.shape}, expected {(n, dim)}")
+    _expect(dtable, (vocab, dim), "f32", "dtable")
+    call("vdsl_op_embedding_bwd", q.handle, n, dim, vocab, ids.handle, dy.dtype, dy.handle, scale, dtable.handle, _h(workspace))
+
+
+def _norm_params(cols, *params) -> int:
+    """The one dtype of gamma and beta, each [cols] or None."""
+    dt = _lib.F32
+    given = [p for p in params if p is not None]
+    for p in given:
+        dt = given[0].dtype
+        _expect(p, (cols,), dt, "gamma / beta")
+    return dt
+
+
+def layer_norm_fwd(q: Queue, x: Tensor, gamma, beta, y: Tensor, mean=None, rstd=None, eps: float = 1e-5):
+    """y = (x - mean) * rstd * gamma + beta over the rows of x [rows][cols]; gamma, beta [cols] or None
+    (1 and 0); mean and rstd (f32 [rows], optional) are kept for layer_norm_bwd."""
+    rows, cols = x.shape
+    if y.shape != (rows, cols):
+        raise ValueError(f"y: shape {y.shape}, expected {(rows, cols)}")
+    _expect(mean, (rows,), "f32", "mean")
+    _expect(rstd, (rows,), "f32", "rstd")
+    pdt = _norm_params(cols, gamma, beta)
+    call("vdsl_op_layer_norm_fwd", q.handle, rows, cols, x.dtype, x.handle, pdt, _h(gamma), _h(beta), eps, y.dtype, y.handle,
+         _h(mean), _h(rstd))
+
+
+def layer_norm_bwd_workspace_bytes(rows, cols) -> int:
+    b = C.c_size_t()
+    call("vdsl_layer_norm_bwd_workspace_bytes", rows, cols, C.byref(b))
+    return b.value
+
+
+def layer_norm_bwd(q: Queue, dy: Tensor, x: Tensor, gamma, mean: Tensor, rstd: Tensor, dx: Tensor, dgamma=None, dbeta=None,
+                   workspace=None):
+    """dx [rows][cols], dgamma and dbeta (f32 [cols], optional) from dy, x and the forward pass's mean and
+    rstd.  workspace: layer_norm_bwd_workspace_bytes(rows, cols) bytes, where dgamma or dbeta is wanted."""
+    rows, cols = x.shape
+    if dy.shape != (rows, cols):
+        raise ValueError(f"dy: shape {dy.shape}, expected {(rows, cols)}")
+    if dx.shape != (rows, cols):
+        raise ValueError(f"dx: shape {dx.shape}, expected {(rows, cols)}")
+    _expect(mean, (rows,), "f32", "mean")
+    _expect(rstd, (rows,), "f32", "rstd")
+    _expect(dgamma, (cols,), "f32", "dgamma")
+    _expect(dbeta, (cols,), "f32", "dbeta")
+    pdt = _norm_params(cols, gamma)
+    call("vdsl_op_layer_norm_bwd", q.handle, rows, cols, dy.dtype, dy.handle, x.dtype, x.handle, pdt, _h(gamma), mean.handle,
+         rstd.handle, dx.dtype, dx.handle, _h(dgamma), _h(dbeta), _h(workspace))
+
+
+def linear_xent_workspace_bytes(n, vocab, dim, piece=0, backward=True) -> int:
+    b = C.c_size_t()
+    call("vdsl_linear_xent_workspace_bytes", n, vocab, dim, piece, int(bool(backward)), C.byref(b))
+    return b.value
+
+
+def _xent_operands(x, w, labels, loss, row_loss, lse):
+    n, dim = x.shape
+    vocab = w.shape[0]
+    _expect(x, (n, dim), "bf16", "x")
+    _expect(w, (vocab, dim), "bf16", "w")
+    _expect(labels, (n,), "i32", "labels")
+    _expect(loss, (1,), "f32", "loss")
+    _expect(row_loss, (n,), "f32", "row_loss")
+    _expect(lse, (n,), "f32", "lse")
+    return n, dim, vocab
+
+
+def linear_xent_fwd(q: Queue, x: Tensor, w: Tensor, labels: Tensor, loss: Tensor, row_loss=None, lse=None, workspace=None):
+    """loss = the mean over the rows of x (bf16 [n][dim]) that count of logsumexp(x w^T) - (x w^T)[label], w
+    bf16 [vocab][dim]; a row whose label (i32 [n]) is outside [0, vocab) does not count.  row_loss and lse
+    (f32 [n], optional): the rows' losses and log sums.  workspace:
+    linear_xent_workspace_bytes(n, vocab, dim, backward=False) bytes."""
+    n, dim, vocab = _xent_operands(x, w, labels, loss, row_loss, lse)
+    call("vdsl_op_linear_xent_fwd", q.handle, n, dim, vocab, x.handle, w.handle, labels.handle, loss.handle, _h(row_loss), _h(lse),
+         _h(workspace))
+
+
+def linear_xent_fwd_bwd(q: Queue, x: Tensor, w: Tensor, labels: Tensor, loss: Tensor, dx: Tensor, dw: Tensor, row_loss=None,
+                        lse=None, piece: int = 0, grad_scale: float = 1.0, workspace=None):
+    """linear_xent_fwd with the gradients of grad_scale * loss: dx [n][dim] and dw [vocab][dim], f32 or bf16
+    each.  piece: columns of the vocabulary worked on at a time (0: the library's choice); workspace:
+    linear_xent_workspace_bytes(n, vocab, dim, piece) bytes."""
+    n, dim, vocab = _xent_operands(x, w, labels, loss, row_loss, lse)
+    if dx.shape != (n, dim):
+        raise ValueError(f"dx: shape {dx.shape}, expected {(n, dim)}")
+    if dw.shape != (vocab, dim):
+        raise ValueError(f"dw: shape {dw.shape}, expected {(vocab, dim)}")
+    call("vdsl_op_linear_xent_fwd_bwd", q.handle, n, dim, vocab, x.handle, w.handle, labels.handle, piece, grad_scale, loss.handle,
+         _h(row_loss), _h(lse), dx.dtype, dx.handle, dw.dtype, dw.handle, _h(workspace))

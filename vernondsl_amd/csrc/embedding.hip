@@ -16,7 +16,10 @@
 namespace vdsl {
 namespace {
 
-// L lanes per output row (a power of two), KU units of U elements each; blockIdx.y: strips of L KU units.
+// A value that is the same for all lanes of a wave, as a scalar.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// 2^log_l lanes per output row, KU units of U elements each; blockIdx.y: strips of columns.
 template <int TT, int OT, int U, int KU>
 __global__ __launch_bounds__(256) void embedding_fwd_kernel(const void* __restrict__ table, const int32_t* __restrict__ ids,
                                                             void* __restrict__ out, int64_t n, int64_t dim, int64_t vocab,
@@ -26,97 +29,374 @@ __global__ __launch_bounds__(256) void embedding_fwd_kernel(const void* __restri
   if (i >= n) return;
   const int32_t id = ids[i];
   const bool valid = id >= 0 && id < vocab;
+  const int64_t row = valid ? id : 0;
   const int64_t c0 = (static_cast<int64_t>(blockIdx.y) * KU * lanes + (threadIdx.x & (lanes - 1))) * U;
   float v[KU][U];
 #pragma unroll
-  for (int k = 0; k < KU; ++k) {
-    const int64_t c = c0 + static_cast<int64_t>(k) * lanes * U;
-    load_unit<TT, U>(table, static_cast<int64_t>(id) * dim + c, valid ? dim - c : 0, v[k]);
-  }
+  for (int k = 0; k < KU; ++k) load_whole<TT, U>(table, row * dim + UnitAt<U>(c0 + static_cast<int64_t>(k) * lanes * U, dim).c, v[k]);
 #pragma unroll
   for (int k = 0; k < KU; ++k) {
-    const int64_t c = c0 + static_cast<int64_t>(k) * lanes * U;
+    const UnitAt<U> at(c0 + static_cast<int64_t>(k) * lanes * U, dim);
 #pragma unroll
     for (int j = 0; j < U; ++j) v[k][j] = valid ? v[k][j] * scale : 0.0f;
-    store_unit<OT, U>(out, i * dim + c, dim - c, v[k]);
+    if (at.any()) store_whole<OT, U>(out, i * dim + at.c, v[k]);
   }
 }
 
-// The positions sorted by token: position i goes to place #{j : id_j < id_i} + #{j < i : id_j = id_i}.
-// A block ranks 64 positions, one a lane, its 16 waves a share of all ids each.  Ids are compared as
-// unsigned numbers, so those that are no row come last.
-__global__ __launch_bounds__(1024) void embedding_rank_kernel(const int32_t* __restrict__ ids, int64_t n,
-                                                              uint32_t* __restrict__ sorted, int32_t* __restrict__ order) {
+__global__ __launch_bounds__(256) void embedding_zero_kernel(uint16_t* __restrict__ p, int64_t n) {
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256) p[i] = 0;
+}
+
+// ---- positions sorted by token -------------------------------------------------------------------
+// Every row's places [x, y) among the sorted positions, none at first (null: not wanted).
+__device__ __forceinline__ void clear_places(int2* __restrict__ places, int64_t vocab) {
+  if (!places) return;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.x;
+  for (int64_t v = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; v < vocab; v += step) places[v] = make_int2(0, 0);
+}
+
+// Up to kRankTile positions: position i goes to place #{j : id_j < id_i} + #{j < i : id_j = id_i}.  A block
+// ranks 64 positions, one a lane, its 16 waves a share of the ids each.  Ids are compared as unsigned
+// numbers, so those that are no row come last.  More positions are ranked so in tiles, and a second kernel
+// adds to an element's rank what the other tiles have before it, a binary search in each: 16384 positions
+// 28 us ranked against all ids, 10 so (radix passes 24).
+constexpr int kRankTile = 1024;
+
+__global__ __launch_bounds__(1024) void embedding_rank_kernel(const int32_t* __restrict__ ids, int n, uint32_t* __restrict__ sorted,
+                                                              int32_t* __restrict__ order, int2* __restrict__ places, int64_t vocab) {
+  clear_places(places, vocab);
   __shared__ int part[16][64];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 64 + lane;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const int i0 = static_cast<int>(blockIdx.x) * 64, i = i0 + lane, tile = i0 / kRankTile * kRankTile;
   const uint32_t key = i < n ? static_cast<uint32_t>(ids[i]) : 0;
-  const int64_t share = (n + 15) / 16, j0 = wave * share, j1 = j0 + share < n ? j0 + share : n;
+  constexpr int kShare = kRankTile / 16;
+  const int j0 = tile + wave * kShare, j1 = min(j0 + kShare, n);
   int rank = 0;
-  for (int64_t j = j0; j < j1; ++j) {
-    const uint32_t other = static_cast<uint32_t>(ids[j]);
-    rank += other < key || (other == key && j < i);
+  if (j0 == i0) {  // the ids at the block's own positions
+    for (int j = j0; j < j1; ++j) {
+      const uint32_t other = static_cast<uint32_t>(ids[j]);
+      rank += other < key || (other == key && j < i);
+    }
+  } else if (j0 < i0) {  // before them
+#pragma unroll 16
+    for (int j = j0; j < j1; ++j) rank += static_cast<uint32_t>(ids[j]) <= key;
+  } else {
+#pragma unroll 16
+    for (int j = j0; j < j1; ++j) rank += static_cast<uint32_t>(ids[j]) < key;
   }
   part[wave][lane] = rank;
   __syncthreads();
   if (wave != 0 || i >= n) return;
-  rank = 0;
+  rank = tile;
 #pragma unroll
   for (int w = 0; w < 16; ++w) rank += part[w][lane];
   sorted[rank] = key;
-  order[rank] = static_cast<int32_t>(i);
+  order[rank] = i;
 }
+static_assert(kRankTile / 16 == 64, "a wave's share of the ids is a block's positions, or lies on one side of them");
 
-// dtable rows: a block takes 2^(8 - log_l) R consecutive rows, 2^log_l lanes to a row, each NV units of 4
-// columns; blockIdx.y: strips of columns.  The rows' shares of the sorted positions come from binary searches.
-constexpr int kRowsPerSlot = 4;
-
-template <int DYT, int NV>
-__global__ __launch_bounds__(256) void embedding_bwd_kernel(const uint32_t* __restrict__ sorted, const int32_t* __restrict__ order,
-                                                            const void* __restrict__ dy, float* __restrict__ dtable, int64_t n,
-                                                            int64_t dim, int64_t vocab, float scale, int log_l) {
-  __shared__ int first[256 + 1];
-  const int slots = 256 >> log_l, lanes = 1 << log_l, rows = slots * kRowsPerSlot;
-  const int64_t v0 = static_cast<int64_t>(blockIdx.x) * rows;
-  for (int r = threadIdx.x; r <= rows; r += 256) {  // the first place whose token is not below row v0 + r
-    const uint64_t v = static_cast<uint64_t>(v0 + r < vocab ? v0 + r : vocab);
-    int lo = 0, hi = static_cast<int>(n);
+__global__ __launch_bounds__(1024) void embedding_merge_kernel(const uint32_t* __restrict__ tiles, const int32_t* __restrict__ from, int n,
+                                                               uint32_t* __restrict__ sorted, int32_t* __restrict__ order) {
+  __shared__ int part[16][64];
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const int e0 = static_cast<int>(blockIdx.x) * 64, e = e0 + lane, mine = e0 / kRankTile;
+  const uint32_t key = tiles[e < n ? e : n - 1];
+  int rank = 0;
+  for (int t = wave; t * kRankTile < n; t += 16) {
+    if (t == mine) continue;
+    // equal tokens of an earlier tile come first
+    const uint64_t bound = static_cast<uint64_t>(key) + (t < mine ? 1 : 0);
+    int lo = 0, hi = min(kRankTile, n - t * kRankTile);
     while (lo < hi) {
-      const int mid = lo + ((hi - lo) >> 1);
-      if (sorted[mid] < v) lo = mid + 1;
+      const int mid = (lo + hi) >> 1;
+      if (tiles[t * kRankTile + mid] < bound) lo = mid + 1;
       else hi = mid;
     }
-    first[r] = lo;
+    rank += lo;
+  }
+  part[wave][lane] = rank;
+  __syncthreads();
+  if (wave != 0 || e >= n) return;
+  rank = e - mine * kRankTile;
+#pragma unroll
+  for (int w = 0; w < 16; ++w) rank += part[w][lane];
+  sorted[rank] = key;
+  order[rank] = from[e];
+}
+
+// Many: a radix sort from the lowest of the tokens' 8-bit digits up, each pass stable.  The positions lie
+// in tiles; hist[pass][tile][digit] counts a pass's digits in each tile of its input.  The first pass's
+// counts come from a kernel of their own, a later pass's from the pass before, which adds to them where
+// it puts a position (whole numbers: their order changes nothing).
+constexpr int kDigits = 256;
+
+__device__ __forceinline__ uint32_t token_key(int32_t id, uint32_t vocab) {  // those that are no row last
+  return static_cast<uint32_t>(id) < vocab ? static_cast<uint32_t>(id) : vocab;
+}
+
+__global__ __launch_bounds__(256) void embedding_count_kernel(const int32_t* __restrict__ ids, int n, uint32_t vocab, int tile,
+                                                              int* __restrict__ hist, int passes, int2* __restrict__ places) {
+  __shared__ int count[kDigits];
+  clear_places(places, vocab);
+  count[threadIdx.x] = 0;
+  __syncthreads();
+  const int i0 = static_cast<int>(blockIdx.x) * tile, i1 = min(i0 + tile, n);
+  for (int i = i0 + static_cast<int>(threadIdx.x); i < i1; i += 256) atomicAdd(&count[token_key(ids[i], vocab) & 255u], 1);
+  __syncthreads();
+  const size_t at = static_cast<size_t>(blockIdx.x) * kDigits + threadIdx.x, pass = static_cast<size_t>(gridDim.x) * kDigits;
+  hist[at] = count[threadIdx.x];
+  for (int p = 1; p < passes; ++p) hist[p * pass + at] = 0;
+}
+
+// One pass, a tile per block, a quarter of it per wave.  keys null: the first pass, which takes the ids.
+__global__ __launch_bounds__(256) void embedding_radix_kernel(const int32_t* __restrict__ ids, const uint32_t* __restrict__ keys,
+                                                              const int32_t* __restrict__ from, int n, uint32_t vocab, int tile,
+                                                              int shift, const int* __restrict__ hist, int* __restrict__ next_hist,
+                                                              uint32_t* __restrict__ out_keys, int32_t* __restrict__ out_order) {
+  __shared__ int place[4][kDigits];  // the next place of a digit for each wave
+  __shared__ int wave_total[4];
+  const int b = threadIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int i0 = static_cast<int>(blockIdx.x) * tile, i1 = min(i0 + tile, n);
+  const int quarter = tile / 4, w0 = min(i0 + wave * quarter, i1), w1 = min(w0 + quarter, i1);
+  int before = 0, total = 0;
+#pragma unroll 8
+  for (int t = 0; t < static_cast<int>(gridDim.x); ++t) {
+    const int c = hist[static_cast<size_t>(t) * kDigits + b];
+    total += c;
+    before += t < static_cast<int>(blockIdx.x) ? c : 0;
+  }
+  int scan = total;  // of the digits below: within the wave, then of the waves before
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int up = __shfl_up(scan, d, 64);
+    if (lane >= d) scan += up;
+  }
+  if (lane == 63) wave_total[wave] = scan;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) place[w][b] = 0;
+  __syncthreads();
+  int start = scan - total + before;
+  for (int w = 0; w < wave; ++w) start += wave_total[w];
+  const auto key_at = [&](int i) { return keys ? keys[i] : token_key(ids[i], vocab); };
+  for (int i = w0 + lane; i < w1; i += 64) atomicAdd(&place[wave][(key_at(i) >> shift) & 255u], 1);
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const int c = place[w][b];
+    place[w][b] = start;
+    start += c;
   }
   __syncthreads();
-  const int64_t c0 = (static_cast<int64_t>(blockIdx.y) * NV * lanes + (threadIdx.x & (lanes - 1))) * 4;
-  for (int k = 0; k < kRowsPerSlot; ++k) {
-    const int r = k * slots + static_cast<int>(threadIdx.x >> log_l);
-    const int64_t v = v0 + r;
-    if (v >= vocab) return;
-    float acc[NV][4];
+  volatile int* const mine = place[wave];  // this wave's alone: its LDS accesses keep their order
+  for (int c0 = w0; c0 < w1; c0 += 64) {
+    const int i = c0 + lane;
+    const bool in = i < w1;
+    const uint32_t key = in ? key_at(i) : 0;
+    const uint32_t digit = (key >> shift) & 255u;
+    uint64_t same = __ballot(in);
 #pragma unroll
-    for (int u = 0; u < NV; ++u)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[u][j] = 0.0f;
-    for (int e = first[r]; e < first[r + 1]; ++e) {
-      const int64_t i = order[e];
-#pragma unroll
-      for (int u = 0; u < NV; ++u) {
-        const int64_t c = c0 + static_cast<int64_t>(u) * lanes * 4;
-        float d[4];
-        load_unit<DYT, 4>(dy, i * dim + c, dim - c, d);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[u][j] += d[j];
-      }
+    for (int bit = 0; bit < 8; ++bit) {
+      const bool set = (digit >> bit) & 1u;
+      const uint64_t ones = __ballot(set);
+      same &= set ? ones : ~ones;
     }
+    const int below = __popcll(same & ((uint64_t{1} << lane) - 1));
+    if (in) {
+      const int at = mine[digit] + below;
+      if ((same >> lane) >> 1 == 0) mine[digit] = at + 1;  // the last lane of this digit
+      out_keys[at] = key;
+      out_order[at] = keys ? from[i] : i;
+      if (next_hist) atomicAdd(&next_hist[static_cast<size_t>(at / tile) * kDigits + ((key >> (shift + 8)) & 255u)], 1);
+    }
+  }
+}
+
+// ---- the rows' sums ------------------------------------------------------------------------------
+// The first of the n sorted places whose token is not below v.
+__device__ __forceinline__ int lower_bound(const uint32_t* sorted, int n, uint32_t v) {
+  int lo = 0, hi = n;
+  while (lo < hi) {
+    const int mid = lo + ((hi - lo) >> 1);
+    if (sorted[mid] < v) lo = mid + 1;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// A wave of the following kernels works on one row at a time (several waves share a wide one), so where a
+// row is and which positions it sums is the same for all of its lanes and stays in scalar registers.
+
+// The columns of a lane: NV units of U, 2^log_l units apart.
+template <int U, int NV>
+struct LaneColumns {
+  uint32_t c[NV];
+  bool any[NV];
+  __device__ __forceinline__ LaneColumns(int log_l, int64_t dim) {
 #pragma unroll
     for (int u = 0; u < NV; ++u) {
-      const int64_t c = c0 + static_cast<int64_t>(u) * lanes * 4;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[u][j] *= scale;
-      store_unit<VDSL_F32, 4>(dtable, v * dim + c, dim - c, acc[u]);
+      const int64_t unit = ((static_cast<int64_t>(blockIdx.y) * NV + u) << log_l) + (threadIdx.x & ((1 << log_l) - 1));
+      const UnitAt<U> at(unit * U, dim);
+      c[u] = static_cast<uint32_t>(at.c);
+      any[u] = at.any();
     }
+  }
+};
+
+// A unit as it is loaded, so that the loads in flight take no more registers than they bring.
+template <int DT, int U>
+struct RawUnit;
+template <int DT>
+struct RawUnit<DT, 1> {
+  float v;
+  __device__ __forceinline__ void load(const char* row, uint32_t c) { v = load_elem<DT>(row, c); }
+  __device__ __forceinline__ void add_to(float (&acc)[1]) const { acc[0] += v; }
+};
+template <>
+struct RawUnit<VDSL_F32, 4> {
+  f32x4 v;
+  __device__ __forceinline__ void load(const char* row, uint32_t c) { v = reinterpret_cast<const F32x4At4*>(row + size_t{4} * c)->v; }
+  __device__ __forceinline__ void add_to(float (&acc)[4]) const {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[j] += v[j];
+  }
+};
+template <>
+struct RawUnit<VDSL_BF16, 4> {
+  u32x2 v;
+  __device__ __forceinline__ void load(const char* row, uint32_t c) { v = reinterpret_cast<const U32x2At2*>(row + size_t{2} * c)->v; }
+  __device__ __forceinline__ void add_to(float (&acc)[4]) const {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      acc[2 * j] += __uint_as_float(v[j] << 16);
+      acc[2 * j + 1] += __uint_as_float(v[j] & 0xFFFF0000u);
+    }
+  }
+};
+
+// acc += the E rows index[k] of p, in that order, their loads issued together.
+template <int DT, int U, int NV, int E>
+__device__ __forceinline__ void add_rows(const void* __restrict__ p, int64_t dim, const LaneColumns<U, NV>& at, float (&acc)[NV][U],
+                                         const int* index) {
+  RawUnit<DT, U> d[E][NV];
+#pragma unroll
+  for (int k = 0; k < E; ++k) {
+    const char* const row = static_cast<const char*>(p) + index[k] * dim * (DT == VDSL_F32 ? 4 : 2);
+#pragma unroll
+    for (int u = 0; u < NV; ++u) d[k][u].load(row, at.c[u]);
+  }
+#pragma unroll
+  for (int k = 0; k < E; ++k)
+#pragma unroll
+    for (int u = 0; u < NV; ++u) d[k][u].add_to(acc[u]);
+}
+
+// acc += rows row(e) of p for e in [e0, e1), in order, E at a time; the next E are looked up before these
+// are waited for.
+template <int DT, int U, int NV, int E, class Row>
+__device__ __forceinline__ void add_range(const void* __restrict__ p, int64_t dim, const LaneColumns<U, NV>& at, int e0, int e1,
+                                          float (&acc)[NV][U], Row&& row) {
+  if (e0 >= e1) return;
+  int index[E], next[E];
+#pragma unroll
+  for (int k = 0; k < E; ++k) index[k] = uniform(row(min(e0 + k, e1 - 1)));
+  int e = e0;
+  for (; e + E <= e1; e += E) {
+#pragma unroll
+    for (int k = 0; k < E; ++k) next[k] = uniform(row(min(e + E + k, e1 - 1)));
+    add_rows<DT, U, NV, E>(p, dim, at, acc, index);
+#pragma unroll
+    for (int k = 0; k < E; ++k) index[k] = next[k];
+  }
+  int left = e1 - e;
+  if (E > 4 && left >= 4) {
+    add_rows<DT, U, NV, 4>(p, dim, at, acc, index);
+    left -= 4;
+#pragma unroll
+    for (int k = 0; k + 4 < E; ++k) index[k] = index[k + 4];
+  }
+  if (E > 2 && left >= 2) {
+    add_rows<DT, U, NV, 2>(p, dim, at, acc, index);
+    left -= 2;
+    index[0] = index[2 % E];
+  }
+  if (left) add_rows<DT, U, NV, 1>(p, dim, at, acc, index);
+}
+
+// Rows of this type that fit 8 NV registers, the loads in flight of a lane that shares its CU with many.
+template <int DT>
+constexpr int kInFlight = DT == VDSL_F32 ? 2 : 4;
+
+// Where the positions are many: each row's places, and the sums of the chunks of sorted places that hold one
+// token only (a frequent token's places are then added chunk by chunk, by many blocks).  Blocks below
+// `place_blocks` do the former.
+template <int DYT, int U, int NV>
+__global__ __launch_bounds__(256) void embedding_chunk_kernel(const uint32_t* __restrict__ sorted, const int32_t* __restrict__ order,
+                                                              const void* __restrict__ dy, int n, int64_t dim, int64_t vocab,
+                                                              int chunk, int log_l, int place_blocks, int2* __restrict__ places,
+                                                              float* __restrict__ partials) {
+  if (static_cast<int>(blockIdx.x) < place_blocks) {
+    const int64_t e = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    if (blockIdx.y != 0 || e >= n) return;
+    const uint32_t token = sorted[e];
+    if (token >= vocab) return;
+    if (e == 0 || sorted[e - 1] != token) places[token].x = static_cast<int>(e);
+    if (e == n - 1 || sorted[e + 1] != token) places[token].y = static_cast<int>(e) + 1;
+    return;
+  }
+  const int k = ((static_cast<int>(blockIdx.x) - place_blocks) << (8 - log_l)) + uniform(threadIdx.x >> log_l);
+  const int e0 = k * chunk;
+  if (k >= n / chunk) return;
+  const uint32_t token = sorted[e0];
+  if (token >= vocab || sorted[e0 + chunk - 1] != token) return;
+  const LaneColumns<U, NV> at(log_l, dim);
+  float acc[NV][U] = {};
+  add_range<DYT, U, NV, 2 * kInFlight<DYT>>(dy, dim, at, e0, e0 + chunk, acc, [&](int e) { return order[e]; });
+#pragma unroll
+  for (int u = 0; u < NV; ++u)
+    if (at.any[u]) store_whole<VDSL_F32, U>(partials, k * dim + at.c[u], acc[u]);
+}
+
+// dtable rows: 2^log_l lanes (64 to 256) to a row, each NV units of U columns; blockIdx.y: strips of columns.  CHUNKS:
+// the rows' places and the chunks' sums come from embedding_chunk_kernel; otherwise the sorted tokens (at
+// most kFewPositions) are searched in LDS.
+constexpr int kFewPositions = 512;
+
+template <int DYT, int U, int NV, bool CHUNKS>
+__global__ __launch_bounds__(256) void embedding_bwd_kernel(const uint32_t* __restrict__ sorted, const int32_t* __restrict__ order,
+                                                            const void* __restrict__ dy, const int2* __restrict__ places,
+                                                            const float* __restrict__ partials, int chunk,
+                                                            float* __restrict__ dtable, int n, int64_t dim, int64_t vocab,
+                                                            float scale, int log_l) {
+  const int64_t v = (static_cast<int64_t>(blockIdx.x) << (8 - log_l)) + uniform(threadIdx.x >> log_l);
+  int e0 = 0, e1 = 0;
+  if constexpr (CHUNKS) {
+    if (v >= vocab) return;
+    const int2 place = places[v];
+    e0 = place.x;
+    e1 = place.y;
+  } else {
+    __shared__ uint32_t tokens[kFewPositions];
+    for (int e = threadIdx.x; e < n; e += 256) tokens[e] = sorted[e];
+    __syncthreads();
+    if (v >= vocab) return;
+    e0 = uniform(lower_bound(tokens, n, static_cast<uint32_t>(v)));
+    e1 = uniform(lower_bound(tokens, n, static_cast<uint32_t>(v) + 1));
+  }
+  const LaneColumns<U, NV> at(log_l, dim);
+  const auto term = [&](int e) { return order[e]; };
+  float acc[NV][U] = {};
+  if (CHUNKS && e1 - e0 >= 2 * chunk) {  // whole chunks lie inside: the places around them, and their sums between
+    const int k0 = (e0 + chunk - 1) / chunk, k1 = e1 / chunk;
+    add_range<DYT, U, NV, kInFlight<DYT>>(dy, dim, at, e0, k0 * chunk, acc, term);
+    add_range<VDSL_F32, U, NV, 2>(partials, dim, at, k0, k1, acc, [&](int h) { return h; });
+    e0 = k1 * chunk;
+  }
+  add_range<DYT, U, NV, kInFlight<DYT>>(dy, dim, at, e0, e1, acc, term);
+#pragma unroll
+  for (int u = 0; u < NV; ++u) {
+#pragma unroll
+    for (int j = 0; j < U; ++j) acc[u][j] *= scale;
+    if (at.any[u]) store_whole<VDSL_F32, U>(dtable, v * dim + at.c[u], acc[u]);
   }
 }
 
@@ -132,6 +412,7 @@ int lanes_log2(int64_t units) {
 int check_extents(int64_t n, int64_t dim, int64_t vocab) {
   if (n < 0 || dim < 0 || vocab < 0) return fail(VDSL_ERR_INVALID_ARG, "negative shape");
   if (n > 0x7fffffff || vocab > 0x7fffffff) return fail(VDSL_ERR_UNSUPPORTED, "embedding: too many tokens or table rows");
+  if (dim > 0x1fffffff) return fail(VDSL_ERR_UNSUPPORTED, "embedding: rows too wide");
   return VDSL_OK;
 }
 
@@ -150,6 +431,11 @@ extern "C" int vdsl_op_embedding_fwd(vdsl_queue q, int64_t n, int64_t dim, int64
   VDSL_TRY(check_buffer(q, out, nbytes(n, dim, dtype_size(out_dtype)), "out", true));
   if (out == table) return fail(VDSL_ERR_INVALID_ARG, "embedding_fwd: out must not be the table");
   if (n == 0 || dim == 0) return VDSL_OK;
+  if (vocab == 0) {  // no id is a row
+    hipLaunchKernelGGL(embedding_zero_kernel, dim3(1024), dim3(256), 0, q->stream, static_cast<uint16_t*>(out->ptr),
+                       n * dim * static_cast<int64_t>(dtype_size(out_dtype) / 2));
+    return check_launch("embedding_zero_kernel");
+  }
   const auto go = [&](auto tt, auto ot, auto unit, auto ku) {
     constexpr int TT = decltype(tt)::value, OT = decltype(ot)::value, U = decltype(unit)::value, KU = decltype(ku)::value;
     const int64_t units = (dim + U - 1) / U;
@@ -160,55 +446,151 @@ extern "C" int vdsl_op_embedding_fwd(vdsl_queue q, int64_t n, int64_t dim, int64
                        q->stream, table->ptr, static_cast<const int32_t*>(ids->ptr), out->ptr, n, dim, vocab, scale, l);
     return check_launch("embedding_fwd_kernel");
   };
+  // A lane takes 4 units where that leaves enough waves to fill the card, so that their loads are in flight together.
+  const bool many = n * dim >= int64_t{1} << 22;
+  const auto pick = [&](auto tt, auto ot) {
+    constexpr int U = decltype(tt)::value == VDSL_BF16 && decltype(ot)::value == VDSL_BF16 ? 8 : 4;
+    if (dim < U) return go(tt, ot, std::integral_constant<int, 1>{}, std::integral_constant<int, 1>{});
+    if (many) return go(tt, ot, std::integral_constant<int, U>{}, std::integral_constant<int, 16 / U>{});
+    return go(tt, ot, std::integral_constant<int, U>{}, std::integral_constant<int, 1>{});
+  };
   using F = std::integral_constant<int, VDSL_F32>;
   using B = std::integral_constant<int, VDSL_BF16>;
-  using K = std::integral_constant<int, 1>;
-  using U4 = std::integral_constant<int, 4>;
-  using U8 = std::integral_constant<int, 8>;
-  if (table_dtype == VDSL_F32 && out_dtype == VDSL_F32) return go(F{}, F{}, U4{}, K{});
-  if (table_dtype == VDSL_F32) return go(F{}, B{}, U4{}, K{});
-  if (out_dtype == VDSL_F32) return go(B{}, F{}, U4{}, K{});
-  return go(B{}, B{}, U8{}, K{});
+  if (table_dtype == VDSL_F32) return out_dtype == VDSL_F32 ? pick(F{}, F{}) : pick(F{}, B{});
+  return out_dtype == VDSL_F32 ? pick(B{}, F{}) : pick(B{}, B{});
 }
+
+namespace vdsl {
+namespace {
+// How the gradient of n positions is laid out.
+struct GradPlan {
+  bool radix;        // the sort: radix passes, or ranks
+  int passes, tile;  // of the radix sort
+  int64_t tiles;
+  int chunk;         // places per chunk; 0: none
+  size_t sorted = 0, order = 0, keys2 = 0, order2 = 0, hist = 0, places = 0, partials = 0, bytes = 0;
+};
+
+int grad_plan(int64_t n, int64_t vocab, int64_t dim, GradPlan& p) {
+  VDSL_TRY(check_extents(n, dim, vocab));
+  p.radix = n > 16384;
+  p.passes = vocab < 256 ? 1 : vocab < 65536 ? 2 : vocab < (1 << 24) ? 3 : 4;
+  p.tile = static_cast<int>(std::max<int64_t>(1024, ((n + 255) / 256 + 1023) / 1024 * 1024));
+  p.tiles = (n + p.tile - 1) / p.tile;
+  p.chunk = n <= kFewPositions ? 0 : n <= 32768 ? 16 : n <= 262144 ? 64 : 256;
+  size_t at = 0;
+  bool fits = true;
+  const auto take = [&](int64_t a, int64_t b) {
+    const size_t from = at, size = nbytes(a, b);
+    if (size == kSizeOverflow || __builtin_add_overflow(at, size, &at) || at > kSizeOverflow - 512) fits = false;
+    else at = (at + 255) / 256 * 256;
+    return from;
+  };
+  p.sorted = take(n, 4);
+  p.order = take(n, 4);
+  if (n > kRankTile) {
+    p.keys2 = take(n, 4);
+    p.order2 = take(n, 4);
+  }
+  if (p.radix) {
+    p.hist = take(p.passes * p.tiles, 4 * kDigits);
+  }
+  if (p.chunk) {
+    p.places = take(vocab, 8);
+    p.partials = take(n / p.chunk, nbytes(dim, 4) == kSizeOverflow ? -1 : dim * 4);
+  }
+  p.bytes = at;
+  return fits ? VDSL_OK : fail(VDSL_ERR_SHAPE, "embedding_bwd: the workspace's size overflows");
+}
+}  // namespace
+}  // namespace vdsl
 
 extern "C" int vdsl_embedding_bwd_workspace_bytes(int64_t n, int64_t vocab, int64_t dim, size_t* bytes) {
   if (!bytes) return fail(VDSL_ERR_INVALID_ARG, "bytes is null");
-  VDSL_TRY(check_extents(n, dim, vocab));
-  *bytes = static_cast<size_t>(n) * 8;
+  GradPlan p;
+  VDSL_TRY(grad_plan(n, vocab, dim, p));
+  *bytes = p.bytes;
   return VDSL_OK;
 }
 
 extern "C" int vdsl_op_embedding_bwd(vdsl_queue q, int64_t n, int64_t dim, int64_t vocab, vdsl_buffer ids, int32_t dy_dtype,
                                      vdsl_buffer dy, float scale, vdsl_buffer dtable, vdsl_buffer workspace) {
   VDSL_TRY(enter_queue(q));
-  VDSL_TRY(check_extents(n, dim, vocab));
+  GradPlan p;
+  VDSL_TRY(grad_plan(n, vocab, dim, p));
   if (!float_type(dy_dtype)) return fail(VDSL_ERR_UNSUPPORTED, "embedding_bwd supports f32 and bf16");
   VDSL_TRY(check_buffer(q, ids, nbytes(n, 4), "ids", false));
   VDSL_TRY(check_buffer(q, dy, nbytes(n, dim, dtype_size(dy_dtype)), "dy", false));
   VDSL_TRY(check_buffer(q, dtable, nbytes(vocab, dim, 4), "dtable", true));
-  size_t need = 0;
-  VDSL_TRY(vdsl_embedding_bwd_workspace_bytes(n, vocab, dim, &need));
-  if (need) VDSL_TRY(check_buffer(q, workspace, need, "workspace", true));
+  if (p.bytes) VDSL_TRY(check_buffer(q, workspace, p.bytes, "workspace", true));
+  if (dtable == dy) return fail(VDSL_ERR_INVALID_ARG, "embedding_bwd: dtable must not be dy");
   if (vocab == 0 || dim == 0) return VDSL_OK;
-  uint32_t* sorted = n ? static_cast<uint32_t*>(workspace->ptr) : nullptr;
-  int32_t* order = reinterpret_cast<int32_t*>(sorted) + n;
-  if (n) {
-    hipLaunchKernelGGL(embedding_rank_kernel, dim3(static_cast<unsigned>((n + 63) / 64)), dim3(1024), 0, q->stream,
-                       static_cast<const int32_t*>(ids->ptr), n, sorted, order);
+  const hipStream_t s = q->stream;
+  // A wave per row of up to 1024 columns (1, 2 or 4 units a lane), 2 or 4 waves for a wider one.
+  const int unit = dim < 4 ? 1 : 4;
+  const int64_t units = (dim + unit - 1) / unit;
+  const int nv = units <= 64 ? 1 : units <= 128 ? 2 : 4;
+  const int l = std::max(6, lanes_log2((units + nv - 1) / nv));
+  const int64_t strips = (units + (int64_t{nv} << l) - 1) / (int64_t{nv} << l);
+  if (strips > 65535) return fail(VDSL_ERR_UNSUPPORTED, "embedding_bwd: rows too wide");
+  char* const ws = p.bytes ? static_cast<char*>(workspace->ptr) : nullptr;
+  const int32_t* id = static_cast<const int32_t*>(ids->ptr);
+  uint32_t* const sorted = reinterpret_cast<uint32_t*>(ws + p.sorted);
+  int32_t* const order = reinterpret_cast<int32_t*>(ws + p.order);
+  const int count = static_cast<int>(n);
+  int2* const places = p.chunk ? reinterpret_cast<int2*>(ws + p.places) : nullptr;
+  uint32_t* const keys2 = reinterpret_cast<uint32_t*>(ws + p.keys2);
+  int32_t* const order2 = reinterpret_cast<int32_t*>(ws + p.order2);
+  if (p.radix) {
+    int* const hist = reinterpret_cast<int*>(ws + p.hist);
+    const dim3 tiles(static_cast<unsigned>(p.tiles));
+    hipLaunchKernelGGL(embedding_count_kernel, tiles, dim3(256), 0, s, id, count, static_cast<uint32_t>(vocab), p.tile, hist, p.passes,
+                       places);
+    VDSL_TRY(check_launch("embedding_count_kernel"));
+    for (int k = 0; k < p.passes; ++k) {  // the last pass ends in sorted and order
+      const bool second = (p.passes - 1 - k) & 1, from_second = !second;
+      int* const h = hist + static_cast<size_t>(k) * p.tiles * kDigits;
+      hipLaunchKernelGGL(embedding_radix_kernel, tiles, dim3(256), 0, s, id, k == 0 ? nullptr : from_second ? keys2 : sorted,
+                         from_second ? order2 : order, count, static_cast<uint32_t>(vocab), p.tile, 8 * k, h,
+                         k + 1 < p.passes ? h + p.tiles * kDigits : nullptr, second ? keys2 : sorted, second ? order2 : order);
+      VDSL_TRY(check_launch("embedding_radix_kernel"));
+    }
+  } else if (n) {
+    const dim3 blocks(static_cast<unsigned>((n + 63) / 64));
+    const bool merge = n > kRankTile;
+    hipLaunchKernelGGL(embedding_rank_kernel, blocks, dim3(1024), 0, s, id, count, merge ? keys2 : sorted, merge ? order2 : order, places,
+                       vocab);
     VDSL_TRY(check_launch("embedding_rank_kernel"));
+    if (merge) {
+      hipLaunchKernelGGL(embedding_merge_kernel, blocks, dim3(1024), 0, s, keys2, order2, count, sorted, order);
+      VDSL_TRY(check_launch("embedding_merge_kernel"));
+    }
   }
-  constexpr int NV = 4;
-  const int64_t units = (dim + 3) / 4;
-  const int l = lanes_log2((units + NV - 1) / NV);
-  const int64_t rows = int64_t{256 >> l} * kRowsPerSlot;
-  const int64_t by = (units + (int64_t{NV} << l) - 1) / (int64_t{NV} << l);
-  if (by > 65535) return fail(VDSL_ERR_UNSUPPORTED, "embedding_bwd: rows too wide");
-  const dim3 grid(static_cast<unsigned>((vocab + rows - 1) / rows), static_cast<unsigned>(by));
-  if (dy_dtype == VDSL_F32)
-    hipLaunchKernelGGL((embedding_bwd_kernel<VDSL_F32, NV>), grid, dim3(256), 0, q->stream, sorted, order, dy->ptr,
-                       static_cast<float*>(dtable->ptr), n, dim, vocab, scale, l);
-  else
-    hipLaunchKernelGGL((embedding_bwd_kernel<VDSL_BF16, NV>), grid, dim3(256), 0, q->stream, sorted, order, dy->ptr,
-                       static_cast<float*>(dtable->ptr), n, dim, vocab, scale, l);
-  return check_launch("embedding_bwd_kernel");
+  float* const partials = reinterpret_cast<float*>(ws + p.partials);
+  const auto go = [&](auto dyt, auto u, auto units_a_lane) {
+    constexpr int DYT = decltype(dyt)::value, U = decltype(u)::value, NV = decltype(units_a_lane)::value;
+    const int64_t rows = 256 >> l;
+    const dim3 grid(static_cast<unsigned>((vocab + rows - 1) / rows), static_cast<unsigned>(strips));
+    if (!p.chunk) {
+      hipLaunchKernelGGL((embedding_bwd_kernel<DYT, U, NV, false>), grid, dim3(256), 0, s, sorted, order, dy->ptr, nullptr, nullptr, 0,
+                         static_cast<float*>(dtable->ptr), count, dim, vocab, scale, l);
+      return check_launch("embedding_bwd_kernel");
+    }
+    const int64_t place_blocks = (n + 255) / 256, chunk_blocks = (n / p.chunk + (256 >> l) - 1) >> (8 - l);
+    hipLaunchKernelGGL((embedding_chunk_kernel<DYT, U, NV>), dim3(static_cast<unsigned>(place_blocks + chunk_blocks), static_cast<unsigned>(strips)),
+                       dim3(256), 0, s, sorted, order, dy->ptr, count, dim, vocab, p.chunk, l, static_cast<int>(place_blocks), places,
+                       partials);
+    VDSL_TRY(check_launch("embedding_chunk_kernel"));
+    hipLaunchKernelGGL((embedding_bwd_kernel<DYT, U, NV, true>), grid, dim3(256), 0, s, sorted, order, dy->ptr, places, partials, p.chunk,
+                       static_cast<float*>(dtable->ptr), count, dim, vocab, scale, l);
+    return check_launch("embedding_bwd_kernel");
+  };
+  const auto pick = [&](auto dyt) {
+    using One = std::integral_constant<int, 1>;
+    using Four = std::integral_constant<int, 4>;
+    if (unit == 1) return go(dyt, One{}, One{});
+    return nv == 1 ? go(dyt, Four{}, One{}) : nv == 2 ? go(dyt, Four{}, std::integral_constant<int, 2>{}) : go(dyt, Four{}, Four{});
+  };
+  if (dy_dtype == VDSL_F32) return pick(std::integral_constant<int, VDSL_F32>{});
+  return pick(std::integral_constant<int, VDSL_BF16>{});
 }

@@ -61,9 +61,11 @@ __device__ __forceinline__ void load_params(const void* __restrict__ p, int dt, 
                                             float (&v)[S::kUnits][S::kUnit]) {
 #pragma unroll
   for (int k = 0; k < S::kUnits; ++k) {
-    const int64_t c = (int64_t{k} * S::kLanes + t) * S::kUnit;
-    if (p) {
-      load_unit<S::kUnit>(dt, p, c, cols - c, v[k]);
+    const UnitAt<S::kUnit> at((int64_t{k} * S::kLanes + t) * S::kUnit, cols);
+    if (p && dt == VDSL_F32) {
+      load_whole<VDSL_F32, S::kUnit>(p, at.c, v[k]);
+    } else if (p) {
+      load_whole<VDSL_BF16, S::kUnit>(p, at.c, v[k]);
     } else {
 #pragma unroll
       for (int j = 0; j < S::kUnit; ++j) v[k][j] = none;
@@ -76,8 +78,8 @@ __device__ __forceinline__ void load_row(const void* __restrict__ p, int64_t row
                                          float (&v)[S::kUnits][S::kUnit]) {
 #pragma unroll
   for (int k = 0; k < S::kUnits; ++k) {
-    const int64_t c = (int64_t{k} * S::kLanes + t) * S::kUnit;
-    load_unit<DT, S::kUnit>(p, row * cols + c, cols - c, v[k]);
+    const UnitAt<S::kUnit> at((int64_t{k} * S::kLanes + t) * S::kUnit, cols);
+    load_whole<DT, S::kUnit>(p, row * cols + at.c, v[k]);
   }
 }
 
@@ -105,20 +107,22 @@ __global__ __launch_bounds__(S::kThreads) void layer_norm_fwd_rows(const void* x
     if (row + step < rows) load_row<S, XT>(x, row + step, cols, t, next);
     float s[1] = {0.0f};
 #pragma unroll
-    for (int k = 0; k < NV; ++k)
+    for (int k = 0; k < NV; ++k) {
+      const UnitAt<U> at((int64_t{k} * S::kLanes + t) * U, cols);
 #pragma unroll
-      for (int j = 0; j < U; ++j) s[0] += v[k][j];
+      for (int j = 0; j < U; ++j) s[0] += j >= at.skip ? v[k][j] : 0.0f;
+    }
     row_sums<S::kLanes>(s, 0);
     const float mean = s[0] * inv_cols;
     // the sum of squares about the mean: no cancellation, however large the mean
     float q[1] = {0.0f};
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int64_t left = cols - (int64_t{k} * S::kLanes + t) * U;
+      const UnitAt<U> at((int64_t{k} * S::kLanes + t) * U, cols);
 #pragma unroll
       for (int j = 0; j < U; ++j) {
-        v[k][j] = j < left ? v[k][j] - mean : 0.0f;
-        q[0] += v[k][j] * v[k][j];
+        v[k][j] -= mean;
+        q[0] += j >= at.skip ? v[k][j] * v[k][j] : 0.0f;
       }
     }
     row_sums<S::kLanes>(q, 1);
@@ -129,11 +133,11 @@ __global__ __launch_bounds__(S::kThreads) void layer_norm_fwd_rows(const void* x
     }
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int64_t c = (int64_t{k} * S::kLanes + t) * U;
+      const UnitAt<U> at((int64_t{k} * S::kLanes + t) * U, cols);
       float o[U];
 #pragma unroll
       for (int j = 0; j < U; ++j) o[j] = v[k][j] * rstd * ga[k][j] + be[k][j];
-      store_unit<U>(y_dt, y, row * cols + c, cols - c, o);
+      if (at.any()) store_whole<U>(y_dt, y, row * cols + at.c, o);
     }
   }
 }
@@ -148,7 +152,7 @@ __global__ __launch_bounds__(1024) void layer_norm_fwd_stream(const void* x, int
   float s[1] = {0.0f};
   for (int64_t c = 4 * threadIdx.x; c < cols; c += 4096) {
     float v[4];
-    load_unit<4>(x_dt, x, base + c, cols - c, v);
+    load_some(x_dt, x, base + c, cols - c, v);
     s[0] += (v[0] + v[1]) + (v[2] + v[3]);
   }
   row_sums<1024>(s, 0);
@@ -156,7 +160,7 @@ __global__ __launch_bounds__(1024) void layer_norm_fwd_stream(const void* x, int
   float q[1] = {0.0f};
   for (int64_t c = 4 * threadIdx.x; c < cols; c += 4096) {
     float v[4];
-    load_unit<4>(x_dt, x, base + c, cols - c, v);
+    load_some(x_dt, x, base + c, cols - c, v);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const float d = c + j < cols ? v[j] - mean : 0.0f;
@@ -171,12 +175,12 @@ __global__ __launch_bounds__(1024) void layer_norm_fwd_stream(const void* x, int
   }
   for (int64_t c = 4 * threadIdx.x; c < cols; c += 4096) {
     float v[4], ga[4] = {1.0f, 1.0f, 1.0f, 1.0f}, be[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    load_unit<4>(x_dt, x, base + c, cols - c, v);
-    if (gamma) load_unit<4>(param_dt, gamma, c, cols - c, ga);
-    if (beta) load_unit<4>(param_dt, beta, c, cols - c, be);
+    load_some(x_dt, x, base + c, cols - c, v);
+    if (gamma) load_some(param_dt, gamma, c, cols - c, ga);
+    if (beta) load_some(param_dt, beta, c, cols - c, be);
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] = (v[j] - mean) * rstd * ga[j] + be[j];
-    store_unit<4>(y_dt, y, base + c, cols - c, v);
+    store_some(y_dt, y, base + c, cols - c, v);
   }
 }
 
@@ -212,10 +216,9 @@ __global__ __launch_bounds__(S::kThreads) void layer_norm_bwd_rows(const void* d
     const float r = nrstd;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int64_t left = cols - (int64_t{k} * S::kLanes + t) * U;
 #pragma unroll
       for (int j = 0; j < U; ++j) {
-        h[k][j] = j < left ? (nx[k][j] - nmean) * r : 0.0f;
+        h[k][j] = (nx[k][j] - nmean) * r;
         d[k][j] = ny[k][j];
       }
     }
@@ -227,25 +230,27 @@ __global__ __launch_bounds__(S::kThreads) void layer_norm_bwd_rows(const void* d
     }
     float s[2] = {0.0f, 0.0f};
 #pragma unroll
-    for (int k = 0; k < NV; ++k)
+    for (int k = 0; k < NV; ++k) {
+      const UnitAt<U> at((int64_t{k} * S::kLanes + t) * U, cols);
 #pragma unroll
       for (int j = 0; j < U; ++j) {
         dg[k][j] += d[k][j] * h[k][j];
         db[k][j] += d[k][j];
         d[k][j] *= ga[k][j];
-        s[0] += d[k][j];
-        s[1] += d[k][j] * h[k][j];
+        s[0] += j >= at.skip ? d[k][j] : 0.0f;
+        s[1] += j >= at.skip ? d[k][j] * h[k][j] : 0.0f;
       }
+    }
     row_sums<S::kLanes>(s, parity);
     parity ^= 1;
     const float m1 = s[0] * inv_cols, m2 = s[1] * inv_cols;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int64_t c = (int64_t{k} * S::kLanes + t) * U;
+      const UnitAt<U> at((int64_t{k} * S::kLanes + t) * U, cols);
       float o[U];
 #pragma unroll
       for (int j = 0; j < U; ++j) o[j] = r * ((d[k][j] - m1) - h[k][j] * m2);
-      store_unit<U>(dx_dt, dx, row * cols + c, cols - c, o);
+      if (at.any()) store_whole<U>(dx_dt, dx, row * cols + at.c, o);
     }
   }
   if (!partials) return;
@@ -275,9 +280,10 @@ __global__ __launch_bounds__(S::kThreads) void layer_norm_bwd_rows(const void* d
   float* const out = partials + static_cast<int64_t>(blockIdx.x) * 2 * cols;
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
-    const int64_t c = (int64_t{k} * S::kLanes + t) * U;
-    store_unit<VDSL_F32, U>(out, c, cols - c, dg[k]);
-    store_unit<VDSL_F32, U>(out, cols + c, cols - c, db[k]);
+    const UnitAt<U> at((int64_t{k} * S::kLanes + t) * U, cols);
+    if (!at.any()) continue;
+    store_whole<VDSL_F32, U>(out, at.c, dg[k]);
+    store_whole<VDSL_F32, U>(out, cols + at.c, db[k]);
   }
 }
 
@@ -292,9 +298,9 @@ __global__ __launch_bounds__(1024) void layer_norm_bwd_stream(const void* dy, in
   for (int pass = 0; pass < 2; ++pass) {
     for (int64_t c = 4 * threadIdx.x; c < cols; c += 4096) {
       float h[4], d[4], ga[4] = {1.0f, 1.0f, 1.0f, 1.0f};
-      load_unit<4>(x_dt, x, base + c, cols - c, h);
-      load_unit<4>(dy_dt, dy, base + c, cols - c, d);
-      if (gamma) load_unit<4>(param_dt, gamma, c, cols - c, ga);
+      load_some(x_dt, x, base + c, cols - c, h);
+      load_some(dy_dt, dy, base + c, cols - c, d);
+      if (gamma) load_some(param_dt, gamma, c, cols - c, ga);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         h[j] = c + j < cols ? (h[j] - m) * r : 0.0f;
@@ -303,7 +309,7 @@ __global__ __launch_bounds__(1024) void layer_norm_bwd_stream(const void* dy, in
         s[1] += d[j] * h[j];
         h[j] = r * ((d[j] - m1) - h[j] * m2);
       }
-      if (pass) store_unit<4>(dx_dt, dx, base + c, cols - c, h);
+      if (pass) store_some(dx_dt, dx, base + c, cols - c, h);
     }
     if (pass) return;
     row_sums<1024>(s, 0);
@@ -323,8 +329,8 @@ __global__ __launch_bounds__(256) void layer_norm_bwd_columns(const void* __rest
   float dg[4] = {0.0f, 0.0f, 0.0f, 0.0f}, db[4] = {0.0f, 0.0f, 0.0f, 0.0f};
   for (int64_t row = blockIdx.y; row < rows; row += gridDim.y) {
     float h[4], d[4];
-    load_unit<4>(x_dt, x, row * cols + c, cols - c, h);
-    load_unit<4>(dy_dt, dy, row * cols + c, cols - c, d);
+    load_some(x_dt, x, row * cols + c, cols - c, h);
+    load_some(dy_dt, dy, row * cols + c, cols - c, d);
     const float m = mean[row], r = rstd[row];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -333,8 +339,8 @@ __global__ __launch_bounds__(256) void layer_norm_bwd_columns(const void* __rest
     }
   }
   float* const out = partials + static_cast<int64_t>(blockIdx.y) * 2 * cols;
-  store_unit<VDSL_F32, 4>(out, c, cols - c, dg);
-  store_unit<VDSL_F32, 4>(out, cols + c, cols - c, db);
+  store_some(VDSL_F32, out, c, cols - c, dg);
+  store_some(VDSL_F32, out, cols + c, cols - c, db);
 }
 
 // dgamma and dbeta: the column sums of the n partial rows, each wave of a block a share of them, added in
@@ -366,6 +372,7 @@ __global__ __launch_bounds__(1024) void layer_norm_bwd_finish(const float* __res
 // Calls go(RowShape) for rows of `cols` columns in units of U, or wide() where no shape holds one.
 template <int U, class Go, class Wide>
 int row_shape(int64_t cols, Go&& go, Wide&& wide) {
+  if (cols < U) return go(RowShape<64, 1, 1>{});
   if (cols <= 64 * U) return go(RowShape<64, U, 1>{});
   if (cols <= 512) return go(RowShape<64, U, 512 / 64 / U>{});
   if (cols <= 1024) return go(RowShape<64, U, 1024 / 64 / U>{});

@@ -24,77 +24,99 @@ __device__ __forceinline__ float load_elem(const void* __restrict__ p, int64_t i
   else return bf16_to_f32(static_cast<const uint16_t*>(p)[i]);
 }
 
-// Elements [e, e + U) of p, those from the n-th on as 0 and never read (n may be zero or negative).
+// Elements [e, e + U) of p, U 1, 4 or 8, and their store, rounded once to p's type.
 template <int DT, int U>
-__device__ __forceinline__ void load_unit(const void* __restrict__ p, int64_t e, int64_t n, float (&v)[U]) {
-  static_assert(U == 4 || U == 8, "units of 4 or 8 elements");
-  if (n >= U) {
-    if constexpr (DT == VDSL_F32) {
+__device__ __forceinline__ void load_whole(const void* __restrict__ p, int64_t e, float (&v)[U]) {
+  if constexpr (U == 1) {
+    v[0] = load_elem<DT>(p, e);
+  } else if constexpr (DT == VDSL_F32) {
 #pragma unroll
-      for (int h = 0; h < U / 4; ++h) {
-        const f32x4 x = reinterpret_cast<const F32x4At4*>(static_cast<const float*>(p) + e + 4 * h)->v;
+    for (int h = 0; h < U / 4; ++h) {
+      const f32x4 x = reinterpret_cast<const F32x4At4*>(static_cast<const float*>(p) + e + 4 * h)->v;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[4 * h + j] = x[j];
-      }
-    } else if constexpr (U == 8) {
-      const u32x4 x = reinterpret_cast<const U32x4At2*>(static_cast<const uint16_t*>(p) + e)->v;
+      for (int j = 0; j < 4; ++j) v[4 * h + j] = x[j];
+    }
+  } else if constexpr (U == 8) {
+    const u32x4 x = reinterpret_cast<const U32x4At2*>(static_cast<const uint16_t*>(p) + e)->v;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        v[2 * j] = __uint_as_float(x[j] << 16);
-        v[2 * j + 1] = __uint_as_float(x[j] & 0xFFFF0000u);
-      }
-    } else {
-      const u32x2 x = reinterpret_cast<const U32x2At2*>(static_cast<const uint16_t*>(p) + e)->v;
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        v[2 * j] = __uint_as_float(x[j] << 16);
-        v[2 * j + 1] = __uint_as_float(x[j] & 0xFFFF0000u);
-      }
+    for (int j = 0; j < 4; ++j) {
+      v[2 * j] = __uint_as_float(x[j] << 16);
+      v[2 * j + 1] = __uint_as_float(x[j] & 0xFFFF0000u);
     }
   } else {
+    const u32x2 x = reinterpret_cast<const U32x2At2*>(static_cast<const uint16_t*>(p) + e)->v;
 #pragma unroll
-    for (int j = 0; j < U; ++j) v[j] = j < n ? load_elem<DT>(p, e + j) : 0.0f;
+    for (int j = 0; j < 2; ++j) {
+      v[2 * j] = __uint_as_float(x[j] << 16);
+      v[2 * j + 1] = __uint_as_float(x[j] & 0xFFFF0000u);
+    }
   }
 }
-
-// The first n of v (at most U) to elements [e, e + n) of p, rounded once to its type.
 template <int DT, int U>
-__device__ __forceinline__ void store_unit(void* __restrict__ p, int64_t e, int64_t n, const float (&v)[U]) {
-  if (n >= U) {
-    if constexpr (DT == VDSL_F32) {
+__device__ __forceinline__ void store_whole(void* __restrict__ p, int64_t e, const float (&v)[U]) {
+  if constexpr (U == 1) {
+    if constexpr (DT == VDSL_F32) static_cast<float*>(p)[e] = v[0];
+    else static_cast<uint16_t*>(p)[e] = f32_to_bf16(v[0]);
+  } else if constexpr (DT == VDSL_F32) {
 #pragma unroll
-      for (int h = 0; h < U / 4; ++h) {
-        const f32x4 x = {v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]};
-        reinterpret_cast<F32x4At4*>(static_cast<float*>(p) + e + 4 * h)->v = x;
-      }
-    } else if constexpr (U == 8) {
-      const u32x4 x = {pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])};
-      reinterpret_cast<U32x4At2*>(static_cast<uint16_t*>(p) + e)->v = x;
-    } else {
-      const u32x2 x = {pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
-      reinterpret_cast<U32x2At2*>(static_cast<uint16_t*>(p) + e)->v = x;
+    for (int h = 0; h < U / 4; ++h) {
+      const f32x4 x = {v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]};
+      reinterpret_cast<F32x4At4*>(static_cast<float*>(p) + e + 4 * h)->v = x;
     }
+  } else if constexpr (U == 8) {
+    const u32x4 x = {pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])};
+    reinterpret_cast<U32x4At2*>(static_cast<uint16_t*>(p) + e)->v = x;
+  } else {
+    const u32x2 x = {pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+    reinterpret_cast<U32x2At2*>(static_cast<uint16_t*>(p) + e)->v = x;
+  }
+}
+template <int U>
+__device__ __forceinline__ void store_whole(int dt, void* __restrict__ p, int64_t e, const float (&v)[U]) {
+  if (dt == VDSL_F32) store_whole<VDSL_F32, U>(p, e, v);
+  else store_whole<VDSL_BF16, U>(p, e, v);
+}
+
+// A lane's unit of U columns from column c on, in a row of at least U: a unit that would pass the row's end
+// is moved back to end there, so every access is whole and no load has a branch around it (which would
+// wait for that load before the next is issued).  Its first `skip` elements belong to the unit before
+// (all of them for a unit past the end): a sum leaves them out; a store may repeat them, its lane having
+// computed the same values.
+template <int U>
+struct UnitAt {
+  int64_t c;
+  int skip;
+  __device__ __forceinline__ UnitAt(int64_t col, int64_t cols) {
+    const int64_t over = col + U - cols;
+    c = over > 0 ? cols - U : col;
+    skip = over <= 0 ? 0 : over < U ? static_cast<int>(over) : U;
+  }
+  __device__ __forceinline__ bool any() const { return skip < U; }
+};
+
+// For accesses that are few: elements [e, e + 4) of p, of type dt (the same for every lane), those from the
+// n-th on as 0 and never read (n may be zero or negative); and the store of the first n of v.
+__device__ __forceinline__ void load_some(int dt, const void* __restrict__ p, int64_t e, int64_t n, float (&v)[4]) {
+  if (n >= 4) {
+    if (dt == VDSL_F32) load_whole<VDSL_F32, 4>(p, e, v);
+    else load_whole<VDSL_BF16, 4>(p, e, v);
   } else {
 #pragma unroll
-    for (int j = 0; j < U; ++j) {
+    for (int j = 0; j < 4; ++j) v[j] = j < n ? (dt == VDSL_F32 ? load_elem<VDSL_F32>(p, e + j) : load_elem<VDSL_BF16>(p, e + j)) : 0.0f;
+  }
+}
+__device__ __forceinline__ void store_some(int dt, void* __restrict__ p, int64_t e, int64_t n, const float (&v)[4]) {
+  if (n >= 4) {
+    store_whole<4>(dt, p, e, v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
       if (j < n) {
-        if constexpr (DT == VDSL_F32) static_cast<float*>(p)[e + j] = v[j];
+        if (dt == VDSL_F32) static_cast<float*>(p)[e + j] = v[j];
         else static_cast<uint16_t*>(p)[e + j] = f32_to_bf16(v[j]);
       }
     }
   }
-}
-
-// The same with the type as an argument that every lane shares.
-template <int U>
-__device__ __forceinline__ void load_unit(int dt, const void* __restrict__ p, int64_t e, int64_t n, float (&v)[U]) {
-  if (dt == VDSL_F32) load_unit<VDSL_F32, U>(p, e, n, v);
-  else load_unit<VDSL_BF16, U>(p, e, n, v);
-}
-template <int U>
-__device__ __forceinline__ void store_unit(int dt, void* __restrict__ p, int64_t e, int64_t n, const float (&v)[U]) {
-  if (dt == VDSL_F32) store_unit<VDSL_F32, U>(p, e, n, v);
-  else store_unit<VDSL_BF16, U>(p, e, n, v);
 }
 
 // A wave's sum through DPP, every lane getting it: a butterfly inside each row of 16 lanes, then the

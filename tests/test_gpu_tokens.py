@@ -398,6 +398,14 @@ def test_linear_xent_large_tiles(q, own):
     check_xent(q, own, *xent_input(r, 1000, 512, 5003), piece=2048)
 
 
+@pytest.mark.parametrize("n,dim,vocab,piece,gt", [(2100, 64, 5501, 0, "bf16"), (2048, 128, 6144, 0, "f32"), (2305, 192, 11000, 5632, "f32"),
+                                                  (520, 320, 16500, 0, "bf16"), (2081, 64, 11264, 5632, "bf16")])
+def test_linear_xent_256_tiles(q, own, n, dim, vocab, piece, gt):
+    """Sizes that take the tiles of 256 x 256: ragged rows, vocabularies and last pieces, one stage of dim and
+    several, rows that are and are not a multiple of a stage."""
+    check_xent(q, own, *xent_input(np.random.default_rng(n), n, dim, vocab), piece=piece, gt=gt)
+
+
 def test_linear_xent_grad_scale_and_calls_agree(q, own):
     r = np.random.default_rng(9)
     x, w, labels = xent_input(r, 70, 96, 900)

@@ -10,9 +10,9 @@
 // units of log2 (z log2 e), and leaves the maximum and the sum of 2^(z - maximum) of each row over each
 // group of columns, from which lse follows.  The gradient needs all of z once lse is known: the last piece
 // of the vocabulary leaves 16-bit codes of z for that, the others form their logits again.  A code is the
-// distance below its group's maximum in steps of 2^-11 of an octave, so exp of it is off by at most
-// 2^(2^-12) - 1 = 1.7e-4 relative (1e-4 root mean square) wherever it is more than 2^-32 of that maximum
-// (below, it counts as 0), a sixteenth of what the rounding of G to bf16 moves it by: a bf16 code
+// distance below its group's maximum in steps of 32 / 65535 octaves, so exp of it is off by at most 1.7e-4
+// relative (1e-4 root mean square) wherever it is more than 2^-32 of that maximum (below, it counts as 0), a
+// sixteenth of what the rounding of G to bf16 moves it by: a bf16 code
 // would double that rounding.  G is rounded to bf16 as every gradient between ops is, and before its
 // division by count: the label's entry then lies in [-1, 0), where a rounding is at most 2^-9 of 1.
 // Where the vocabulary is one piece that is 6 n vocab dim operations, else up to 8 n vocab dim.
@@ -21,18 +21,20 @@
 #include <type_traits>
 
 #include "gemm_any.h"
+#include "gemm_wide.h"
 
 namespace vdsl {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr float kCodeSteps = 2048.0f;  // per octave
+constexpr float kCodeOctaves = 32.0f;
 constexpr uint32_t kCodeZero = 65535;  // 2^-32 of the group's maximum or less
 
 enum { kLogitStats = 0, kLogitCodes = 1, kLogitGrad = 2 };
 
-__device__ __forceinline__ uint16_t code_of(float below) {  // octaves below the group's maximum
-  return static_cast<uint16_t>(fminf(__builtin_fmaf(below, kCodeSteps, 0.5f), 65535.0f));
+// Two codes from two distances below the group's maximum as shares of kCodeOctaves (a NaN: 0, its row is one).
+__device__ __forceinline__ uint32_t codes_of(float a, float b) {
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pknorm_u16(a, b));
 }
 
 // Butterflies over the 32 lanes that hold a row of an accumulator.
@@ -104,7 +106,7 @@ __device__ __forceinline__ void logits_epilogue(const LogitArgs& p, const f32x16
           const int col = acc_col<Cfg>(n0, j);
           if (counts && col < p.cols && p.v0 + col == label) p.zlabel[row] = v[j];
           if constexpr (MODE == kLogitCodes)
-            if (in && col < p.cols) p.g[row * p.ldg + col] = code_of(base - v[j]);
+            if (in && col < p.cols) p.g[row * p.ldg + col] = static_cast<uint16_t>(codes_of((base - v[j]) * (1.0f / kCodeOctaves), 0.0f));
         }
       }
     }
@@ -119,6 +121,101 @@ __global__ __launch_bounds__(Cfg::NT) void xent_logits_any(LogitArgs p) {
   f32x16 acc[Cfg::FM][Cfg::FN];
   any_mainloop<Cfg>(p.x, p.w, p.n, p.cols, p.dim, tm * Cfg::BM, tn * Cfg::BN, smem, acc);
   logits_epilogue<Cfg, MODE>(p, acc, tm * Cfg::BM, tn * Cfg::BN);
+}
+
+// The same for tiles of gemm_wide.h, the vocabulary as C's rows: a lane has a token's logits of half of 128
+// columns, so the token's maximum and sum over them need one exchange with the lane of the other half, and
+// 16-byte stores leave the codes or G.  A group is 128 columns.
+template <int MODE, bool EDGE>
+__device__ __forceinline__ void logits_epilogue_wide(const LogitArgs& p, const f32x16 (&acc)[4][4], int c0, int row0) {
+  const int half = (threadIdx.x & 63) >> 5;
+  const int group = p.group0 + c0 / 128;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    __builtin_amdgcn_sched_barrier(0);
+    const int row = row0 + 32 * j + static_cast<int>(threadIdx.x & 31);
+    const bool in = row < p.n;
+    const int label = in ? p.labels[row] : -1;
+    const bool counts = label >= 0 && label < p.vocab;
+    const int at = label - p.v0 - c0;  // among the wave's columns
+    const bool here = counts && at >= 0 && at < 128 && at % 8 / 4 == half;
+    const bool any_label = __any(here);
+    float z[4][16];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        z[i][r] = wide_value(acc[i][j][r]);
+        if (EDGE && c0 + 32 * i + 8 * (r >> 2) + 4 * half + (r & 3) >= p.cols) z[i][r] = -INFINITY;
+      }
+    float base;  // exp2's argument is z log2 e - base
+    if constexpr (MODE == kLogitGrad) {
+      base = in ? p.lse[row] : 0.0f;
+    } else {
+      float top = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, z[i][r]);
+      top = fmaxf(top, __shfl_xor(top, 32, 64)) * kLog2e;
+      base = top == -INFINITY ? 0.0f : top;
+      float s[4] = {};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r & 3] += __builtin_amdgcn_exp2f(__builtin_fmaf(z[i][r], kLog2e, -base));
+      float sum = (s[0] + s[1]) + (s[2] + s[3]);
+      sum += __shfl_xor(sum, 32, 64);
+      if (in && half == 0) p.stats[static_cast<int64_t>(row) * p.groups + group] = make_float2(top, sum);
+      if (any_label) {
+        float zl = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) zl = at == 32 * i + 8 * (r >> 2) + 4 * half + (r & 3) ? z[i][r] : zl;
+        if (here) p.zlabel[row] = zl * kLog2e;
+      }
+    }
+    if constexpr (MODE != kLogitStats) {
+      uint16_t* const out = p.g + row * p.ldg + c0 + 8 * half;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (MODE == kLogitCodes) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) z[i][r] = __builtin_fmaf(z[i][r], -kLog2e / kCodeOctaves, base * (1.0f / kCodeOctaves));
+        } else {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) z[i][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[i][r], kLog2e, -base));
+          if (any_label) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) z[i][r] -= here && at == 32 * i + 8 * (r >> 2) + 4 * half + (r & 3) ? 1.0f : 0.0f;
+          }
+        }
+#pragma unroll
+        for (int q = 0; q < 4; q += 2) {
+          uint32_t word[4];
+#pragma unroll
+          for (int h = 0; h < 4; ++h) {
+            const float a = z[i][4 * q + 2 * h], b = z[i][4 * q + 2 * h + 1];
+            word[h] = MODE == kLogitCodes ? codes_of(a, b) : pack_bf16x2(counts ? a : 0.0f, counts ? b : 0.0f);
+          }
+          const u32x4 eight = wide_exchange(word[0], word[1], word[2], word[3]);
+          if (in && (!EDGE || c0 + 32 * i + 8 * (q + half) < p.ldg)) *reinterpret_cast<u32x4*>(out + 32 * i + 8 * q) = eight;
+        }
+      }
+    }
+  }
+}
+
+template <int MODE>
+__global__ __launch_bounds__(WideCfg::NT, 1) void xent_logits_wide(LogitArgs p) {
+  __shared__ __attribute__((aligned(1024))) char smem[WideCfg::LDS_BYTES];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  wide_gemm<false, false>(p.w, p.x, p.cols, p.n, p.dim, p.dim, p.dim, false, smem, [&](const f32x16 (&acc)[4][4], int m0, int n0) {
+    const int c0 = m0 + 128 * (wave >> 1), row0 = n0 + 128 * (wave & 1);  // of the wave
+    if (c0 + 128 <= p.cols) logits_epilogue_wide<MODE, false>(p, acc, c0, row0);
+    else if (c0 < p.cols) logits_epilogue_wide<MODE, true>(p, acc, c0, row0);
+  });
 }
 
 __device__ __forceinline__ float block_sum_256(float v, float* area) {
@@ -143,14 +240,20 @@ struct RowArgs {
   float* row_loss;  // of the workspace
   float* row_loss_out;  // may be null
   uint16_t* g;      // codes in, G out, [n][ldg]; null: none
-  int cols, vocab, v0, group0, groups, group_cols;
+  int n, cols, vocab, v0, group0, groups, group_cols;
   int64_t ldg;
 };
 
-// A block per row: lse and the row's loss from the groups' maxima and sums, then G from the codes.
+// A block per row: lse and the row's loss from the groups' maxima and sums, then G from the codes.  Rows of G
+// past n are zeros.
 __global__ __launch_bounds__(256) void xent_rows_kernel(RowArgs p) {
   __shared__ float area[2][4];
   const int64_t row = blockIdx.x;
+  if (row >= p.n) {
+    u32x4* const g = reinterpret_cast<u32x4*>(p.g + row * p.ldg);
+    for (int c = 8 * static_cast<int>(threadIdx.x); c < p.ldg; c += 2048) g[c / 8] = u32x4{0u, 0u, 0u, 0u};
+    return;
+  }
   const float2* const st = p.stats + row * p.groups;
   float top = -INFINITY;
   for (int t = threadIdx.x; t < p.groups; t += 256) top = fmaxf(top, st[t].x);
@@ -171,23 +274,29 @@ __global__ __launch_bounds__(256) void xent_rows_kernel(RowArgs p) {
     if (p.row_loss_out) p.row_loss_out[row] = loss;
   }
   if (!p.g) return;
-  uint16_t* const g = p.g + row * p.ldg;
-  for (int64_t c = 2 * threadIdx.x; c < p.ldg; c += 512) {
-    const uint32_t two = *reinterpret_cast<const uint32_t*>(g + c);
-    float v[2];
+  u32x4* const g = reinterpret_cast<u32x4*>(p.g + row * p.ldg);
+  for (int c = 8 * static_cast<int>(threadIdx.x); c < p.ldg; c += 2048) {
+    u32x4 two = g[c / 8];
+    if (counts) {
+      const float below = st[p.group0 + (c < p.cols ? c : p.cols - 1) / p.group_cols].x - lse;
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int col = static_cast<int>(c) + k;
-      const uint32_t u = k ? two >> 16 : two & 0xFFFFu;
-      float e = 0.0f;
-      if (counts && col < p.cols) {
-        if (u != kCodeZero) e = __builtin_amdgcn_exp2f((st[p.group0 + col / p.group_cols].x - lse) - u * (1.0f / kCodeSteps));
-        if (!(lse == lse)) e = lse;  // NaN in the row: in all of its gradient
-        if (p.v0 + col == label) e = __builtin_amdgcn_exp2f(zl - lse) - 1.0f;
+      for (int k = 0; k < 4; ++k) {
+        float v[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t u = h ? two[k] >> 16 : two[k] & 0xFFFFu;
+          const int col = c + 2 * k + h;
+          v[h] = u != kCodeZero ? __builtin_amdgcn_exp2f(__builtin_fmaf(static_cast<float>(u), -kCodeOctaves / 65535.0f, below)) : 0.0f;
+          if (!(lse == lse)) v[h] = lse;  // NaN in the row: in all of its gradient
+          if (p.v0 + col == label) v[h] = __builtin_amdgcn_exp2f(zl - lse) - 1.0f;
+          if (col >= p.cols) v[h] = 0.0f;
+        }
+        two[k] = pack_bf16x2(v[0], v[1]);
       }
-      v[k] = e;
+    } else {
+      two = u32x4{0u, 0u, 0u, 0u};
     }
-    *reinterpret_cast<uint32_t*>(g + c) = pack_bf16x2(v[0], v[1]);
+    g[c / 8] = two;
   }
 }
 
@@ -273,16 +382,87 @@ __global__ __launch_bounds__(Cfg::NT) void xent_grad_any(GradArgs p) {
   grad_epilogue<Cfg>(p, acc, tm * Cfg::BM, tn * Cfg::BN);
 }
 
+// The gradients' products on tiles of gemm_wide.h: out[n][m] from A(m, k) and B(n, k), so that a lane has
+// neighbouring elements of a row of out.
+struct WideGradArgs {
+  const uint16_t *a, *b;
+  int m, n, k;         // m, n: of out
+  int n_alloc;         // of B, where it is K-major: columns that are allocated
+  int64_t lda, ldb;
+  float* sum;          // as GradArgs, [n][m]
+  bool first, last;
+  const float* inv;
+  void* out;
+  int out_dt;
+};
+
+// WHOLE: the product is all of the sum, rounded to bf16; otherwise any of the forms.
+template <bool BKM, bool WHOLE>
+__global__ __launch_bounds__(WideCfg::NT, 1) void xent_grad_wide(WideGradArgs p) {
+  __shared__ __attribute__((aligned(1024))) char smem[WideCfg::LDS_BYTES];
+  const int half = (threadIdx.x & 63) >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const float inv = p.inv[0];
+  wide_gemm<true, BKM>(p.a, p.b, p.m, BKM ? p.n_alloc : p.n, p.k, p.lda, p.ldb, BKM, smem, [&](const f32x16 (&acc)[4][4], int m0, int n0) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int row = n0 + 128 * (wave & 1) + 32 * j + static_cast<int>(threadIdx.x & 31);
+      const int c0 = m0 + 128 * (wave >> 1);
+      const int64_t out = static_cast<int64_t>(row) * p.m + c0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        __builtin_amdgcn_sched_barrier(0);
+        float v[16];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) v[r] = wide_value(acc[i][j][r]);
+        if constexpr (WHOLE) {
+#pragma unroll
+          for (int q = 0; q < 4; q += 2) {
+            uint32_t word[4];
+#pragma unroll
+            for (int h = 0; h < 4; ++h) word[h] = pack_bf16x2(v[4 * q + 2 * h] * inv, v[4 * q + 2 * h + 1] * inv);
+            const u32x4 eight = wide_exchange(word[0], word[1], word[2], word[3]);
+            const int c = 32 * i + 8 * (q + half);
+            if (row < p.n && c0 + c < p.m) *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(p.out) + out + c) = eight;
+          }
+        } else {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int c = 32 * i + 8 * q + 4 * half;
+            if (row >= p.n || c0 + c >= p.m) continue;
+            f32x4 s = {v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
+            if (!p.first) s += *reinterpret_cast<const f32x4*>(p.sum + out + c);
+            if (!p.last)
+              *reinterpret_cast<f32x4*>(p.sum + out + c) = s;
+            else if (p.out_dt == VDSL_F32)
+              *reinterpret_cast<f32x4*>(static_cast<float*>(p.out) + out + c) = s * inv;
+            else
+              *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + out + c) =
+                  make_uint2(pack_bf16x2(s[0] * inv, s[1] * inv), pack_bf16x2(s[2] * inv, s[3] * inv));
+          }
+        }
+      }
+    }
+  });
+}
+
 // ---- host ----------------------------------------------------------------------------------------
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Whether a product takes tiles of 128 x 128 or of 64 x 64.
 bool big_tiles(int64_t m, int64_t n) { return ceil_div(m, 64) * ceil_div(n, 64) >= 1024; }
 
+// Whether the products take gemm_wide.h's tiles: whole stages of dim, offsets of 256 rows that fit 32 bits, and
+// tiles for the card's 256 CUs.
+bool wide_runs(int64_t n, int64_t cols, int64_t dim) {
+  return dim % 64 == 0 && dim < (1 << 22) && cols < (1 << 22) && ceil_div(n, 256) * ceil_div(cols, 256) >= 192;
+}
+
 // How a call is laid out: the pieces and the workspace.
 struct Plan {
   int64_t piece = 0, pieces = 0;      // columns of a piece (the last may have fewer)
+  bool wide = false;                  // gemm_wide.h's tiles, else gemm_any.h's
   int64_t group_cols = 0, groups = 0;
+  int64_t g_rows = 0;                 // rows of G, those past n zeros
   int64_t ldg = 0;
   size_t stats = 0, zlabel = 0, lse = 0, row_loss = 0, inv = 0, g = 0, sum = 0, bytes = 0;
 };
@@ -299,9 +479,11 @@ int make_plan(int64_t n, int64_t vocab, int64_t dim, int64_t piece, bool backwar
   p.pieces = ceil_div(vocab, std::min(vocab, ceil_div(piece, 256) * 256));
   p.piece = p.pieces == 1 ? vocab : ceil_div(ceil_div(vocab, p.pieces), 256) * 256;
   p.pieces = ceil_div(vocab, p.piece);
-  p.group_cols = big_tiles(n, p.piece) ? 64 : 32;
+  p.wide = wide_runs(n, p.piece, dim);
+  p.group_cols = p.wide ? 128 : big_tiles(n, p.piece) ? 64 : 32;
   p.groups = (p.pieces - 1) * ceil_div(p.piece, p.group_cols) + ceil_div(vocab - (p.pieces - 1) * p.piece, p.group_cols);
-  p.ldg = ceil_div(p.piece, 8) * 8;
+  p.ldg = ceil_div(p.piece, p.wide ? 256 : 8) * (p.wide ? 256 : 8);
+  p.g_rows = p.wide ? ceil_div(n, 64) * 64 : n;
   size_t at = 0;
   bool fits = true;
   const auto take = [&](int64_t a, int64_t b) {
@@ -316,7 +498,7 @@ int make_plan(int64_t n, int64_t vocab, int64_t dim, int64_t piece, bool backwar
   p.row_loss = take(n, 4);
   p.inv = take(1, 4);
   if (backward) {
-    p.g = take(n, p.ldg * 2);
+    p.g = take(p.g_rows, p.ldg * 2);
     if (p.pieces > 1) p.sum = take(n, dim * 4);
   }
   p.bytes = at;
@@ -332,7 +514,13 @@ int with_tiles(int64_t m, int64_t n, bool big, const char* name, Go&& go) {
 }
 
 template <int MODE>
-int launch_logits(const LogitArgs& a, bool big, hipStream_t s) {
+int launch_logits(const LogitArgs& a, const Plan& plan, hipStream_t s) {
+  if (plan.wide) {
+    const unsigned blocks = wide_blocks(ceil_div(a.n, 256) * ceil_div(a.cols, 256));
+    hipLaunchKernelGGL(xent_logits_wide<MODE>, dim3(blocks), dim3(WideCfg::NT), 0, s, a);
+    return check_launch("xent_logits_wide");
+  }
+  const bool big = plan.group_cols == 64;
   using Big = AnyConfig<128, 128, 2, 2, false, false>;
   using Small = AnyConfig<64, 64, 2, 2, false, false>;
   return with_tiles(a.n, a.cols, big, "xent_logits_any", [&](unsigned tiles) {
@@ -350,6 +538,16 @@ int launch_grad(const GradArgs& a, hipStream_t s) {
     if (big) hipLaunchKernelGGL(xent_grad_any<Big>, dim3(tiles), dim3(Big::NT), 0, s, a);
     else hipLaunchKernelGGL(xent_grad_any<Small>, dim3(tiles), dim3(Small::NT), 0, s, a);
   });
+}
+
+template <bool BKM>
+int launch_grad_wide(const WideGradArgs& a, int64_t n, hipStream_t s) {
+  const unsigned blocks = wide_blocks(ceil_div(a.m, 256) * ceil_div(n, 256));
+  if (a.first && a.last && a.out_dt == VDSL_BF16)
+    hipLaunchKernelGGL((xent_grad_wide<BKM, true>), dim3(blocks), dim3(WideCfg::NT), 0, s, a);
+  else
+    hipLaunchKernelGGL((xent_grad_wide<BKM, false>), dim3(blocks), dim3(WideCfg::NT), 0, s, a);
+  return check_launch("xent_grad_wide");
 }
 
 int run_xent(vdsl_queue q, int64_t n, int64_t dim, int64_t vocab, vdsl_buffer x, vdsl_buffer w, vdsl_buffer labels, int64_t piece,
@@ -379,7 +577,6 @@ int run_xent(vdsl_queue q, int64_t n, int64_t dim, int64_t vocab, vdsl_buffer x,
   float* const inv = reinterpret_cast<float*>(ws + plan.inv);
   float* const each = reinterpret_cast<float*>(ws + plan.row_loss);
   uint16_t* const g = backward ? reinterpret_cast<uint16_t*>(ws + plan.g) : nullptr;
-  const bool big = plan.group_cols == 64;
   LogitArgs la{};
   la.x = static_cast<const uint16_t*>(x->ptr);
   la.labels = lab;
@@ -402,8 +599,8 @@ int run_xent(vdsl_queue q, int64_t n, int64_t dim, int64_t vocab, vdsl_buffer x,
   if (n > 0) {
     for (int64_t k = 0; k < plan.pieces; ++k) {
       set_piece(k);
-      if (backward && k == plan.pieces - 1) VDSL_TRY(launch_logits<kLogitCodes>(la, big, s));
-      else VDSL_TRY(launch_logits<kLogitStats>(la, big, s));
+      if (backward && k == plan.pieces - 1) VDSL_TRY(launch_logits<kLogitCodes>(la, plan, s));
+      else VDSL_TRY(launch_logits<kLogitStats>(la, plan, s));
     }
     RowArgs ra{};
     ra.labels = lab;
@@ -414,6 +611,7 @@ int run_xent(vdsl_queue q, int64_t n, int64_t dim, int64_t vocab, vdsl_buffer x,
     ra.row_loss = each;
     ra.row_loss_out = row_loss ? static_cast<float*>(row_loss->ptr) : nullptr;
     ra.g = g;
+    ra.n = la.n;
     ra.cols = la.cols;
     ra.vocab = la.vocab;
     ra.v0 = la.v0;
@@ -421,7 +619,7 @@ int run_xent(vdsl_queue q, int64_t n, int64_t dim, int64_t vocab, vdsl_buffer x,
     ra.groups = la.groups;
     ra.group_cols = static_cast<int>(plan.group_cols);
     ra.ldg = plan.ldg;
-    hipLaunchKernelGGL(xent_rows_kernel, dim3(static_cast<unsigned>(n)), dim3(256), 0, s, ra);
+    hipLaunchKernelGGL(xent_rows_kernel, dim3(static_cast<unsigned>(backward ? plan.g_rows : n)), dim3(256), 0, s, ra);
     VDSL_TRY(check_launch("xent_rows_kernel"));
   }
   hipLaunchKernelGGL(xent_mean_kernel, dim3(1), dim3(1024), 0, s, each, lab, n, static_cast<int>(vocab), grad_scale,
@@ -437,7 +635,19 @@ int run_xent(vdsl_queue q, int64_t n, int64_t dim, int64_t vocab, vdsl_buffer x,
   for (int64_t t = 0; t < plan.pieces; ++t) {
     const int64_t k = plan.pieces - 1 - t;
     set_piece(k);
-    if (t > 0) VDSL_TRY(launch_logits<kLogitGrad>(la, big, s));
+    if (t > 0) VDSL_TRY(launch_logits<kLogitGrad>(la, plan, s));
+    float* const sum = plan.pieces > 1 ? reinterpret_cast<float*>(ws + plan.sum) : nullptr;
+    void* const dw_piece = static_cast<char*>(dw->ptr) + static_cast<int64_t>(la.v0) * dim * static_cast<int64_t>(dtype_size(dw_dtype));
+    if (plan.wide) {
+      // dx^T = w^T G^T over the piece, dw^T = x^T G
+      WideGradArgs x_args{la.w, g,        la.dim, la.n,        la.cols, 0,       dim,       plan.ldg, sum,
+                          t == 0, t == plan.pieces - 1, inv, dx->ptr, dx_dtype};
+      VDSL_TRY(launch_grad_wide<false>(x_args, n, s));
+      WideGradArgs w_args{la.x, g, la.dim, la.cols, la.n, static_cast<int>(plan.ldg), dim, plan.ldg, nullptr, true, true, inv,
+                          dw_piece, dw_dtype};
+      VDSL_TRY(launch_grad_wide<true>(w_args, plan.ldg, s));
+      continue;
+    }
     GradArgs ga{};
     ga.inv = inv;
     ga.a = g;  // dx += G w
@@ -449,7 +659,7 @@ int run_xent(vdsl_queue q, int64_t n, int64_t dim, int64_t vocab, vdsl_buffer x,
     ga.k = la.cols;
     ga.first = t == 0;
     ga.last = t == plan.pieces - 1;
-    ga.sum = plan.pieces > 1 ? reinterpret_cast<float*>(ws + plan.sum) : nullptr;
+    ga.sum = sum;
     ga.out = dx->ptr;
     ga.out_dt = dx_dtype;
     VDSL_TRY((launch_grad<false, true>(ga, s)));
@@ -462,7 +672,7 @@ int run_xent(vdsl_queue q, int64_t n, int64_t dim, int64_t vocab, vdsl_buffer x,
     ga.k = la.n;
     ga.first = ga.last = true;
     ga.sum = nullptr;
-    ga.out = static_cast<char*>(dw->ptr) + static_cast<int64_t>(la.v0) * dim * static_cast<int64_t>(dtype_size(dw_dtype));
+    ga.out = dw_piece;
     ga.out_dt = dw_dtype;
     VDSL_TRY((launch_grad<true, true>(ga, s)));
   }

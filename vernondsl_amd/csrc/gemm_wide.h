@@ -3,7 +3,7 @@
 //
 // Why four waves: a wave of 128 x 128 reads 8 fragments for 16 MFMAs, one of 128 x 64 (gemm_dma.h's eight
 // waves a tile) 6 for 8.  Per 16 K values a CU then reads 32 KiB of LDS and writes 16 for 512 cycles of
-// MFMAs, three quarters of what LDS moves in them (128 bytes a cycle) instead of all of it.  The price is
+// MFMAs instead of 48 and 16.  The price is
 // one wave to a SIMD: nothing else runs while it waits, so every fragment read and copy is placed between
 // two MFMAs by hand (sched_barrier), and the accumulators take all 256 accumulation registers.
 //
@@ -19,8 +19,12 @@
 //             fragments of t + 1 and copies
 // From that barrier to the next, B(t + 2) goes to the slot of A(t) and then A(t + 3) to that of B(t), whose last
 // fragments every wave has read by then.  The wait leaves A(t + 2) in flight: the copies never drain, and
-// have half a stage or more to land (with two slots of both operands, which drain at each barrier, 1154, 1256
-// and 1226 TFLOP/s for the three products of n = 8192, dim = 4096, vocab = 32768; FIGURES here).
+// have half a stage or more to land.  The stages of a block's next tile follow those of the present one in
+// the ring, so its first copies are in flight during the epilogue.
+//
+// 8192 x 4096 x 32768 (B row-major, A K-major), us on one card: eight waves with 64-byte stages 1821; these
+// tiles with 32-value stages 1814, with two slots of both operands that drain at each barrier 1750, with the
+// ring 1597 (the MFMA units busy 82% of the cycles at the 1.64 GHz that the power limit leaves).
 //
 // Edges: rows past M or N repeat the last one (row-major) or the last 8 columns (K-major): they reach no
 // stored output.  K is taken in whole stages: a row-major operand holds them whole (K a multiple of 64, or

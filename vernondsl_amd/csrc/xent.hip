@@ -21,7 +21,9 @@
 #include <type_traits>
 
 #include "gemm_any.h"
+#include "gemm_ring.h"
 #include "gemm_wide.h"
+#include "rowunit.h"
 
 namespace vdsl {
 namespace {
@@ -37,18 +39,6 @@ __device__ __forceinline__ uint32_t codes_of(float a, float b) {
   return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pknorm_u16(a, b));
 }
 
-// Butterflies over the 32 lanes that hold a row of an accumulator.
-__device__ __forceinline__ float half_max(float v) {
-#pragma unroll
-  for (int m = 16; m >= 1; m >>= 1) v = fmaxf(v, __shfl_xor(v, m, 64));
-  return v;
-}
-__device__ __forceinline__ float half_sum(float v) {
-#pragma unroll
-  for (int m = 16; m >= 1; m >>= 1) v += __shfl_xor(v, m, 64);
-  return v;
-}
-
 struct LogitArgs {
   const uint16_t* x;       // [n][dim]
   const uint16_t* w;       // the piece's rows, [cols][dim]
@@ -61,91 +51,34 @@ struct LogitArgs {
   int v0;                  // the piece's first column
   int group0, groups;      // its first group, and all groups
   int64_t ldg;
+  int g0;                  // the first of the columns whose codes are wanted, G's first
 };
 
-// MODE kLogitStats: stats and zlabel; kLogitCodes: also the codes; kLogitGrad: G from lse.
-template <class Cfg, int MODE>
-__device__ __forceinline__ void logits_epilogue(const LogitArgs& p, const f32x16 (&acc)[Cfg::FM][Cfg::FN], int m0, int n0) {
-  const int lane = threadIdx.x & 63;
-  const int wcol = acc_col<Cfg>(n0, 0) - (lane & 31);  // the wave's first column: a group is a wave's columns
-  const int group = p.group0 + wcol / Cfg::WTN;
-#pragma unroll
-  for (int i = 0; i < Cfg::FM; ++i)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int row = acc_row<Cfg>(m0, i, r);
-      const bool in = row < p.n;
-      const int label = in ? p.labels[row] : -1;
-      const bool counts = label >= 0 && label < p.vocab;
-      float v[Cfg::FN];
-#pragma unroll
-      for (int j = 0; j < Cfg::FN; ++j) v[j] = acc_col<Cfg>(n0, j) < p.cols ? acc[i][j][r] * kLog2e : -INFINITY;
-      if constexpr (MODE == kLogitGrad) {
-        const float lse = in ? p.lse[row] : 0.0f;
-#pragma unroll
-        for (int j = 0; j < Cfg::FN; ++j) {
-          const int col = acc_col<Cfg>(n0, j);
-          float g = __builtin_amdgcn_exp2f(v[j] - lse);
-          if (p.v0 + col == label) g -= 1.0f;
-          if (!counts || col >= p.cols) g = 0.0f;
-          if (in && col < p.ldg) p.g[row * p.ldg + col] = f32_to_bf16(g);
-        }
-      } else {
-        float top = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < Cfg::FN; ++j) top = fmaxf(top, v[j]);
-        top = half_max(top);
-        const float base = top == -INFINITY ? 0.0f : top;  // a group of -inf only: a sum of 0
-        float s = 0.0f;
-#pragma unroll
-        for (int j = 0; j < Cfg::FN; ++j) s += __builtin_amdgcn_exp2f(v[j] - base);
-        s = half_sum(s);
-        if (in && wcol < p.cols && (lane & 31) == 0) p.stats[static_cast<int64_t>(row) * p.groups + group] = make_float2(top, s);
-#pragma unroll
-        for (int j = 0; j < Cfg::FN; ++j) {
-          const int col = acc_col<Cfg>(n0, j);
-          if (counts && col < p.cols && p.v0 + col == label) p.zlabel[row] = v[j];
-          if constexpr (MODE == kLogitCodes)
-            if (in && col < p.cols) p.g[row * p.ldg + col] = static_cast<uint16_t>(codes_of((base - v[j]) * (1.0f / kCodeOctaves), 0.0f));
-        }
-      }
-    }
-}
-
-template <class Cfg, int MODE>
-__global__ __launch_bounds__(Cfg::NT) void xent_logits_any(LogitArgs p) {
-  __shared__ __attribute__((aligned(16))) char smem[Cfg::LDS_BYTES];
-  const int tiles_m = (p.n + Cfg::BM - 1) / Cfg::BM, tiles_n = (p.cols + Cfg::BN - 1) / Cfg::BN;
-  int tm, tn;
-  tile_coords(xcd_remap(blockIdx.x, gridDim.x), tiles_m, tiles_n, tm, tn);
-  f32x16 acc[Cfg::FM][Cfg::FN];
-  any_mainloop<Cfg>(p.x, p.w, p.n, p.cols, p.dim, tm * Cfg::BM, tn * Cfg::BN, smem, acc);
-  logits_epilogue<Cfg, MODE>(p, acc, tm * Cfg::BM, tn * Cfg::BN);
-}
-
-// The same for tiles of gemm_wide.h, the vocabulary as C's rows: a lane has a token's logits of half of 128
-// columns, so the token's maximum and sum over them need one exchange with the lane of the other half, and
-// 16-byte stores leave the codes or G.  A group is 128 columns.
-template <int MODE, bool EDGE>
-__device__ __forceinline__ void logits_epilogue_wide(const LogitArgs& p, const f32x16 (&acc)[4][4], int c0, int row0) {
+// What a wave does with its tile of logits, 32 FM columns of the vocabulary (one group) from c0 on by 32 FN
+// tokens from row0 on.  The vocabulary is C's row side, so a lane has a token's logits of half of the columns:
+// the token's maximum and sum need one exchange with the lane of the other half, and four neighbours (eight
+// after another exchange) are stored together.  value(i, j, r): the accumulator's element; EDGE: some of the
+// columns are not there.  MODE kLogitStats: stats and zlabel; kLogitCodes: also the codes; kLogitGrad: G from lse.
+template <int FM, int FN, int MODE, bool EDGE, class Value>
+__device__ __forceinline__ void logits_epilogue(const LogitArgs& p, int c0, int row0, Value&& value) {
   const int half = (threadIdx.x & 63) >> 5;
-  const int group = p.group0 + c0 / 128;
+  const int group = p.group0 + c0 / (32 * FM);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
+  for (int j = 0; j < FN; ++j) {
     __builtin_amdgcn_sched_barrier(0);
     const int row = row0 + 32 * j + static_cast<int>(threadIdx.x & 31);
     const bool in = row < p.n;
     const int label = in ? p.labels[row] : -1;
     const bool counts = label >= 0 && label < p.vocab;
     const int at = label - p.v0 - c0;  // among the wave's columns
-    const bool here = counts && at >= 0 && at < 128 && at % 8 / 4 == half;
+    const bool here = counts && at >= 0 && at < 32 * FM && at % 8 / 4 == half;
     const bool any_label = __any(here);
-    float z[4][16];
+    float z[FM][16];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < FM; ++i)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        z[i][r] = wide_value(acc[i][j][r]);
+        z[i][r] = value(i, j, r);
         if (EDGE && c0 + 32 * i + 8 * (r >> 2) + 4 * half + (r & 3) >= p.cols) z[i][r] = -INFINITY;
       }
     float base;  // exp2's argument is z log2 e - base
@@ -154,14 +87,14 @@ __device__ __forceinline__ void logits_epilogue_wide(const LogitArgs& p, const f
     } else {
       float top = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < FM; ++i)
 #pragma unroll
         for (int r = 0; r < 16; ++r) top = fmaxf(top, z[i][r]);
       top = fmaxf(top, __shfl_xor(top, 32, 64)) * kLog2e;
-      base = top == -INFINITY ? 0.0f : top;
+      base = top == -INFINITY ? 0.0f : top;  // a group of -inf only: a sum of 0
       float s[4] = {};
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < FM; ++i)
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r & 3] += __builtin_amdgcn_exp2f(__builtin_fmaf(z[i][r], kLog2e, -base));
       float sum = (s[0] + s[1]) + (s[2] + s[3]);
@@ -170,16 +103,16 @@ __device__ __forceinline__ void logits_epilogue_wide(const LogitArgs& p, const f
       if (any_label) {
         float zl = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < FM; ++i)
 #pragma unroll
           for (int r = 0; r < 16; ++r) zl = at == 32 * i + 8 * (r >> 2) + 4 * half + (r & 3) ? z[i][r] : zl;
         if (here) p.zlabel[row] = zl * kLog2e;
       }
     }
     if constexpr (MODE != kLogitStats) {
-      uint16_t* const out = p.g + row * p.ldg + c0 + 8 * half;
+      uint16_t* const out = p.g + row * p.ldg + (c0 - p.g0) + 8 * half;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < FM; ++i) {
         if constexpr (MODE == kLogitCodes) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) z[i][r] = __builtin_fmaf(z[i][r], -kLog2e / kCodeOctaves, base * (1.0f / kCodeOctaves));
@@ -200,11 +133,22 @@ __device__ __forceinline__ void logits_epilogue_wide(const LogitArgs& p, const f
             word[h] = MODE == kLogitCodes ? codes_of(a, b) : pack_bf16x2(counts ? a : 0.0f, counts ? b : 0.0f);
           }
           const u32x4 eight = wide_exchange(word[0], word[1], word[2], word[3]);
-          if (in && (!EDGE || c0 + 32 * i + 8 * (q + half) < p.ldg)) *reinterpret_cast<u32x4*>(out + 32 * i + 8 * q) = eight;
+          if (in && (!EDGE || c0 - p.g0 + 32 * i + 8 * (q + half) < p.ldg)) *reinterpret_cast<u32x4*>(out + 32 * i + 8 * q) = eight;
         }
       }
     }
   }
+}
+
+template <int FM, int FN, int MODE, class Value>
+__device__ __forceinline__ void logits_tile(const LogitArgs& p, int c0, int row0, Value&& value) {
+  if (c0 >= p.cols) return;
+  if (MODE == kLogitCodes && c0 < p.g0) {  // a column of a piece whose logits are formed again
+    logits_epilogue<FM, FN, kLogitStats, false>(p, c0, row0, value);  // whole: pieces are multiples of 256
+    return;
+  }
+  if (c0 + 32 * FM <= p.cols) logits_epilogue<FM, FN, MODE, false>(p, c0, row0, value);
+  else logits_epilogue<FM, FN, MODE, true>(p, c0, row0, value);
 }
 
 template <int MODE>
@@ -212,10 +156,76 @@ __global__ __launch_bounds__(WideCfg::NT, 1) void xent_logits_wide(LogitArgs p) 
   __shared__ __attribute__((aligned(1024))) char smem[WideCfg::LDS_BYTES];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   wide_gemm<false, false>(p.w, p.x, p.cols, p.n, p.dim, p.dim, p.dim, false, smem, [&](const f32x16 (&acc)[4][4], int m0, int n0) {
-    const int c0 = m0 + 128 * (wave >> 1), row0 = n0 + 128 * (wave & 1);  // of the wave
-    if (c0 + 128 <= p.cols) logits_epilogue_wide<MODE, false>(p, acc, c0, row0);
-    else if (c0 < p.cols) logits_epilogue_wide<MODE, true>(p, acc, c0, row0);
+    logits_tile<4, 4, MODE>(p, m0 + 128 * (wave >> 1), n0 + 128 * (wave & 1),
+                            [&](int i, int j, int r) { return wide_value(acc[i][j][r]); });
   });
+}
+
+// inv: the gradients' factor, grad_scale over the number of rows that count, and that number's bits (1 if none does).
+// area: LDS (the block's only array: with a second one the compiler waits for every copy before each read of the first).
+__device__ __forceinline__ void count_rows(const int32_t* __restrict__ labels, int n, int vocab, float grad_scale, float* inv, char* area) {
+  int* const part = reinterpret_cast<int*>(area);
+  int k = 0;
+#pragma unroll 8
+  for (int i = threadIdx.x; i < n; i += blockDim.x) k += labels[i] >= 0 && labels[i] < vocab;
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) k += __shfl_xor(k, m, 64);
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = k;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  for (unsigned w = 1; w < blockDim.x / 64; ++w) k += part[w];
+  inv[0] = static_cast<float>(static_cast<double>(grad_scale) / (k > 0 ? k : 1));
+  inv[1] = __int_as_float(k > 0 ? k : 1);
+}
+
+// The main loops of the smaller tiles: gemm_ring.h's where rows are whole 16-byte units (dim % 8 == 0), else
+// gemm_any.h's.  Stages in the ring: as many as leave two blocks a CU (one of 128 x 128).
+template <int BM, int BN, int WGM, int WGN, int NS, bool AKM, bool BKM>
+struct RingLoop : RingConfig<BM, BN, WGM, WGN, NS, AKM, BKM> {
+  using Cfg = RingConfig<BM, BN, WGM, WGN, NS, AKM, BKM>;
+  __device__ static __forceinline__ void run(const uint16_t* a, const uint16_t* b, int m, int n, int, int kb, int ke, int m0, int n0,
+                                             char* smem, f32x16 (&acc)[Cfg::FM][Cfg::FN], int64_t lda, int64_t ldb) {
+    ring_mainloop<Cfg>(a, b, m, n, kb, ke, m0, n0, smem, acc, lda, ldb);
+  }
+};
+template <int BM, int BN, int WGM, int WGN, bool AKM, bool BKM>
+struct AnyLoop : AnyConfig<BM, BN, WGM, WGN, AKM, BKM> {
+  using Cfg = AnyConfig<BM, BN, WGM, WGN, AKM, BKM>;
+  __device__ static __forceinline__ void run(const uint16_t* a, const uint16_t* b, int m, int n, int k, int kb, int ke, int m0, int n0,
+                                             char* smem, f32x16 (&acc)[Cfg::FM][Cfg::FN], int64_t lda, int64_t ldb) {
+    any_mainloop_range<Cfg>(a, b, m, n, k, kb, ke, m0, n0, smem, acc, lda, ldb);
+  }
+};
+template <int BM_, int BN_, int WGM_, int WGN_, int NS>
+struct Tile {
+  static constexpr int BM = BM_, BN = BN_, WGM = WGM_, WGN = WGN_, NT = 64 * WGM_ * WGN_;
+  template <bool RING, bool AKM, bool BKM>
+  using Loop = std::conditional_t<RING, RingLoop<BM_, BN_, WGM_, WGN_, NS, AKM, BKM>, AnyLoop<BM_, BN_, WGM_, WGN_, AKM, BKM>>;
+  __host__ __device__ static int64_t tiles(int64_t m, int64_t n) { return ((m + BM - 1) / BM) * ((n + BN - 1) / BN); }
+};
+using Tile64x32 = Tile<64, 32, 2, 1, 6>;    // the logits of up to 32 rows
+using Tile128x32 = Tile<128, 32, 4, 1, 4>;  // their dx
+using Tile64 = Tile<64, 64, 2, 2, 5>;
+using Tile128x64 = Tile<128, 64, 2, 2, 3>;
+using Tile128 = Tile<128, 128, 2, 2, 5>;
+
+// Products of few tiles, of rows that are no whole stages, or of odd lengths.  The launch has a block more than
+// tiles: the last one counts the rows.
+template <class Cfg, int MODE>
+__global__ __launch_bounds__(Cfg::NT) void xent_logits_any(LogitArgs p, float grad_scale, float* inv) {
+  __shared__ __attribute__((aligned(1024))) char smem[Cfg::LDS_BYTES];
+  const int tiles_m = (p.cols + Cfg::BM - 1) / Cfg::BM, tiles_n = (p.n + Cfg::BN - 1) / Cfg::BN, tiles = tiles_m * tiles_n;
+  if (static_cast<int>(blockIdx.x) == tiles) {
+    count_rows(p.labels, p.n, p.vocab, grad_scale, inv, smem);
+    return;
+  }
+  int tm, tn;
+  tile_coords(xcd_remap(blockIdx.x, tiles), tiles_m, tiles_n, tm, tn);
+  f32x16 acc[Cfg::FM][Cfg::FN];
+  Cfg::run(p.w, p.x, p.cols, p.n, p.dim, 0, p.dim, tm * Cfg::BM, tn * Cfg::BN, smem, acc, p.dim, p.dim);
+  const int wave = threadIdx.x >> 6;
+  logits_tile<Cfg::FM, Cfg::FN, MODE>(p, tm * Cfg::BM + wave / Cfg::WGN * Cfg::WTM, tn * Cfg::BN + wave % Cfg::WGN * Cfg::WTN,
+                                      [&](int i, int j, int r) { return acc[i][j][r]; });
 }
 
 __device__ __forceinline__ float block_sum_256(float v, float* area) {
@@ -255,6 +265,16 @@ __global__ __launch_bounds__(256) void xent_rows_kernel(RowArgs p) {
     return;
   }
   const float2* const st = p.stats + row * p.groups;
+  constexpr int kAhead = 4;  // of this lane's units of 8 codes, loaded before lse is known
+  const u32x4* const codes = reinterpret_cast<const u32x4*>(p.g + row * p.ldg);
+  u32x4 ahead[kAhead];
+  if (p.g) {
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int c = 8 * static_cast<int>(threadIdx.x) + 2048 * k;
+      ahead[k] = codes[(c < p.ldg ? c : 0) / 8];
+    }
+  }
   float top = -INFINITY;
   for (int t = threadIdx.x; t < p.groups; t += 256) top = fmaxf(top, st[t].x);
   top = block_max_256(top, area[0]);
@@ -275,8 +295,8 @@ __global__ __launch_bounds__(256) void xent_rows_kernel(RowArgs p) {
   }
   if (!p.g) return;
   u32x4* const g = reinterpret_cast<u32x4*>(p.g + row * p.ldg);
-  for (int c = 8 * static_cast<int>(threadIdx.x); c < p.ldg; c += 2048) {
-    u32x4 two = g[c / 8];
+  const auto to_gradient = [&](int c, u32x4 two) {
+    if (c >= p.ldg) return;
     if (counts) {
       const float below = st[p.group0 + (c < p.cols ? c : p.cols - 1) / p.group_cols].x - lse;
 #pragma unroll
@@ -297,6 +317,15 @@ __global__ __launch_bounds__(256) void xent_rows_kernel(RowArgs p) {
       two = u32x4{0u, 0u, 0u, 0u};
     }
     g[c / 8] = two;
+  };
+  const int c0 = 8 * static_cast<int>(threadIdx.x);
+#pragma unroll
+  for (int k = 0; k < kAhead; ++k) to_gradient(c0 + 2048 * k, ahead[k]);
+  for (int c = c0 + 2048 * kAhead; c < p.ldg; c += 2048 * kAhead) {
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) ahead[k] = codes[(c + 2048 * k < p.ldg ? c + 2048 * k : 0) / 8];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) to_gradient(c + 2048 * k, ahead[k]);
   }
 }
 
@@ -330,56 +359,125 @@ __global__ __launch_bounds__(1024) void xent_mean_kernel(const float* __restrict
   const double c = k > 0 ? static_cast<double>(k) : 1.0;
   loss[0] = static_cast<float>(s / c);
   inv[0] = static_cast<float>(static_cast<double>(grad_scale) / c);
+  inv[1] = __int_as_float(static_cast<int>(c));
 }
 
 __global__ __launch_bounds__(256) void xent_zero_kernel(uint16_t* __restrict__ p, int64_t n) {
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256) p[i] = 0;
 }
 
+// A gradient's product, transposed: out[n][m] = inv sum_k A(m, k) B(n, k), A K-major, so that a lane has
+// neighbouring elements of a row of out.  k may be split, and there may be pieces: then the products go to
+// sum, [split][n][m] in f32, and a last kernel adds the splits.
 struct GradArgs {
   const uint16_t *a, *b;
   int m, n, k;
-  int64_t lda, ldb;    // negative: dense
-  float* sum;          // [m][n] f32, the pieces' sum; null: this product is all of it
-  bool first, last;    // of the pieces: sum holds nothing yet; the result is whole
+  int64_t lda, ldb;
+  float* sum;          // null: this product is all of it
+  bool first;          // of the pieces: sum holds nothing yet
+  int splits;
   const float* inv;    // the factor of the result
-  void* out;           // [m][n] of out_dt
+  void* out;           // [n][m] of out_dt
   int out_dt;
 };
 
 template <class Cfg>
-__device__ __forceinline__ void grad_epilogue(const GradArgs& p, const f32x16 (&acc)[Cfg::FM][Cfg::FN], int m0, int n0) {
+__device__ __forceinline__ void grad_tile(const GradArgs& p, int block, char* smem) {
+  const int tiles_m = (p.m + Cfg::BM - 1) / Cfg::BM, tiles_n = (p.n + Cfg::BN - 1) / Cfg::BN, tiles = tiles_m * tiles_n;
+  const int split = block / tiles;
+  int tm, tn;
+  tile_coords(block - split * tiles, tiles_m, tiles_n, tm, tn);
+  const int m0 = tm * Cfg::BM, n0 = tn * Cfg::BN;
+  const int stages = (p.k + 63) / 64;
+  const int kb = 64 * static_cast<int>(static_cast<int64_t>(stages) * split / p.splits);
+  const int ke = min(p.k, 64 * static_cast<int>(static_cast<int64_t>(stages) * (split + 1) / p.splits));
+  f32x16 acc[Cfg::FM][Cfg::FN];
+  if (kb < ke) {  // block-uniform
+    Cfg::run(p.a, p.b, p.m, p.n, p.k, kb, ke, m0, n0, smem, acc, p.lda, p.ldb);
+  } else {
+#pragma unroll
+    for (int i = 0; i < Cfg::FM; ++i)
+#pragma unroll
+      for (int j = 0; j < Cfg::FN; ++j) acc[i][j] = MfmaBf16::zero();
+  }
+  const int half = (threadIdx.x & 63) >> 5, wave = threadIdx.x >> 6;
   const float inv = p.inv[0];
+  float* const sum = p.sum ? p.sum + static_cast<int64_t>(split) * p.n * p.m : nullptr;
 #pragma unroll
-  for (int i = 0; i < Cfg::FM; ++i)
+  for (int j = 0; j < Cfg::FN; ++j) {
+    const int row = n0 + wave % Cfg::WGN * Cfg::WTN + 32 * j + static_cast<int>(threadIdx.x & 31);
+    if (row >= p.n) continue;
 #pragma unroll
-    for (int j = 0; j < Cfg::FN; ++j)
+    for (int i = 0; i < Cfg::FM; ++i)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int row = acc_row<Cfg>(m0, i, r), col = acc_col<Cfg>(n0, j);
-        if (row >= p.m || col >= p.n) continue;
-        const int64_t o = static_cast<int64_t>(row) * p.n + col;
-        float v = acc[i][j][r];
-        if (!p.first) v += p.sum[o];
-        if (!p.last) {
-          p.sum[o] = v;
+      for (int q = 0; q < 4; ++q) {
+        const int col = m0 + wave / Cfg::WGN * Cfg::WTM + 32 * i + 8 * q + 4 * half;
+        const int64_t o = static_cast<int64_t>(row) * p.m + col;
+        float v[4] = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+        if (sum) {
+          if (!p.first) {
+            float before[4];
+            load_some(VDSL_F32, sum, o, p.m - col, before);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] += before[e];
+          }
+          store_some(VDSL_F32, sum, o, p.m - col, v);
         } else {
-          v *= inv;
-          if (p.out_dt == VDSL_F32) static_cast<float*>(p.out)[o] = v;
-          else static_cast<uint16_t*>(p.out)[o] = f32_to_bf16(v);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] *= inv;
+          store_some(p.out_dt, p.out, o, p.m - col, v);
         }
       }
+  }
 }
 
-template <class Cfg>
-__global__ __launch_bounds__(Cfg::NT) void xent_grad_any(GradArgs p) {
-  __shared__ __attribute__((aligned(16))) char smem[Cfg::LDS_BYTES];
-  const int tiles_m = (p.m + Cfg::BM - 1) / Cfg::BM, tiles_n = (p.n + Cfg::BN - 1) / Cfg::BN;
-  int tm, tn;
-  tile_coords(xcd_remap(blockIdx.x, gridDim.x), tiles_m, tiles_n, tm, tn);
-  f32x16 acc[Cfg::FM][Cfg::FN];
-  any_mainloop<Cfg>(p.a, p.b, p.m, p.n, p.k, tm * Cfg::BM, tn * Cfg::BN, smem, acc, p.lda, p.ldb);
-  grad_epilogue<Cfg>(p, acc, tm * Cfg::BM, tn * Cfg::BN);
+__device__ __forceinline__ void mean_loss(const float* __restrict__ row_loss, int64_t n, const float* __restrict__ inv,
+                                          float* __restrict__ loss, char* area) {
+  double* const sums = reinterpret_cast<double*>(area);
+  double s = 0.0;
+#pragma unroll 8
+  for (int64_t i = threadIdx.x; i < n; i += blockDim.x) s += row_loss[i];
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) s += __shfl_xor(s, m, 64);
+  if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  for (unsigned w = 1; w < blockDim.x / 64; ++w) s += sums[w];
+  loss[0] = static_cast<float>(s / __float_as_int(inv[1]));
+}
+
+// Both gradients of a piece in one launch, dx's blocks first (they have the longer sums); loss, if not null:
+// one more block, which forms the mean loss.
+template <class Tx, class Tw, bool RING>
+__global__ __launch_bounds__(Tw::NT) void xent_grads_any(GradArgs dx, GradArgs dw, int dx_blocks, int dw_blocks,
+                                                            const float* row_loss, float* loss) {
+  using ForDx = typename Tx::template Loop<RING, true, false>;
+  static_assert(Tx::NT == Tw::NT, "one launch");
+  using ForDw = typename Tw::template Loop<RING, true, true>;
+  __shared__ __attribute__((aligned(1024))) char smem[ForDx::LDS_BYTES > ForDw::LDS_BYTES ? ForDx::LDS_BYTES : ForDw::LDS_BYTES];
+  const int block = static_cast<int>(blockIdx.x);
+  if (block < dx_blocks) grad_tile<ForDx>(dx, block, smem);
+  else if (block < dx_blocks + dw_blocks) grad_tile<ForDw>(dw, block - dx_blocks, smem);
+  else mean_loss(row_loss, dx.n, dx.inv, loss, smem);
+}
+
+// out = inv times the sum of the splits, four elements a lane.
+__global__ __launch_bounds__(64) void xent_join_kernel(const float* __restrict__ sum, int splits, int64_t n, const float* __restrict__ inv,
+                                                        void* __restrict__ out, int out_dt) {
+  const int64_t e = (static_cast<int64_t>(blockIdx.x) * 64 + threadIdx.x) * 4;
+  if (e >= n) return;
+  float s[4] = {};
+#pragma unroll 8
+  for (int k = 0; k < splits; ++k) {
+    float v[4];
+    load_some(VDSL_F32, sum, k * n + e, n - e, v);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s[j] += v[j];
+  }
+  const float f = inv[0];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) s[j] *= f;
+  store_some(out_dt, out, e, n - e, s);
 }
 
 // The gradients' products on tiles of gemm_wide.h: out[n][m] from A(m, k) and B(n, k), so that a lane has
@@ -389,8 +487,8 @@ struct WideGradArgs {
   int m, n, k;         // m, n: of out
   int n_alloc;         // of B, where it is K-major: columns that are allocated
   int64_t lda, ldb;
-  float* sum;          // as GradArgs, [n][m]
-  bool first, last;
+  float* sum;          // [n][m] f32, the pieces' sum
+  bool first, last;    // of the pieces: sum holds nothing yet; the result is whole
   const float* inv;
   void* out;
   int out_dt;
@@ -448,8 +546,18 @@ __global__ __launch_bounds__(WideCfg::NT, 1) void xent_grad_wide(WideGradArgs p)
 // ---- host ----------------------------------------------------------------------------------------
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Whether a product takes tiles of 128 x 128 or of 64 x 64.
-bool big_tiles(int64_t m, int64_t n) { return ceil_div(m, 64) * ceil_div(n, 64) >= 1024; }
+enum Tiling { kTiles64x32, kTiles128x32, kTiles64, kTiles128x64, kTiles128, kTilesWide };
+
+// The tile of an m x n product on gemm_any.h.  A CU takes in operands at about 55 bytes a nanosecond, so a launch
+// lasts as long as its busiest CU's: rounds of tiles over the 256 CUs times the tile's rows and columns.
+// 300 x 5003 x 1000 14.8 us in tiles of 64 x 64 (two rounds).
+Tiling any_tiles(int64_t m, int64_t n) {
+  const auto cost = [&](int64_t bm, int64_t bn) { return ceil_div(ceil_div(m, bm) * ceil_div(n, bn), 256) * (bm + bn); };
+  const int64_t a = cost(64, 64), b = cost(128, 64), c = cost(128, 128);
+  return a <= b && a <= c ? kTiles64 : b <= c ? kTiles128x64 : kTiles128;
+}
+int64_t rows_of(Tiling t) { return t == kTiles64x32 || t == kTiles64 ? 64 : 128; }
+int64_t cols_of(Tiling t) { return t == kTiles64x32 || t == kTiles128x32 ? 32 : t == kTiles128 ? 128 : 64; }
 
 // Whether the products take gemm_wide.h's tiles: whole stages of dim, offsets of 256 rows that fit 32 bits, and
 // tiles for the card's 256 CUs.
@@ -457,14 +565,20 @@ bool wide_runs(int64_t n, int64_t cols, int64_t dim) {
   return dim % 64 == 0 && dim < (1 << 22) && cols < (1 << 22) && ceil_div(n, 256) * ceil_div(cols, 256) >= 192;
 }
 
-// How a call is laid out: the pieces and the workspace.
+// Whether the smaller tiles take gemm_ring.h: rows of dim elements are whole 16-byte units, and the offsets of 128
+// rows fit 32 bits (G's rows are whole units of at most a vocabulary).
+bool ring_runs(int64_t dim) { return dim % 8 == 0 && dim < (1 << 23); }
+
+// How a call is laid out: the pieces, the tiles and the workspace.
 struct Plan {
-  int64_t piece = 0, pieces = 0;      // columns of a piece (the last may have fewer)
-  bool wide = false;                  // gemm_wide.h's tiles, else gemm_any.h's
+  int64_t piece = 0, pieces = 0;  // columns of a piece (the last may have fewer)
+  // of all logits, of a piece's formed again, of dw (and dx where it has no other), of dx
+  Tiling logits = kTiles64, again = kTiles64, grads = kTiles64, dx = kTiles64;
   int64_t group_cols = 0, groups = 0;
-  int64_t g_rows = 0;                 // rows of G, those past n zeros
-  int64_t ldg = 0;
-  size_t stats = 0, zlabel = 0, lse = 0, row_loss = 0, inv = 0, g = 0, sum = 0, bytes = 0;
+  int64_t g_rows = 0, ldg = 0;    // of G; its rows past n are zeros
+  int splits = 1;                 // of the sums over a piece's columns for dx
+  bool sum = false;               // whether dx is formed by way of f32 sums
+  size_t at_stats = 0, at_zlabel = 0, at_lse = 0, at_row_loss = 0, at_inv = 0, at_g = 0, at_sum = 0, bytes = 0;
 };
 
 constexpr int64_t kPieceBytes = int64_t{1} << 30;  // of codes, where the caller leaves the piece to the library
@@ -479,65 +593,87 @@ int make_plan(int64_t n, int64_t vocab, int64_t dim, int64_t piece, bool backwar
   p.pieces = ceil_div(vocab, std::min(vocab, ceil_div(piece, 256) * 256));
   p.piece = p.pieces == 1 ? vocab : ceil_div(ceil_div(vocab, p.pieces), 256) * 256;
   p.pieces = ceil_div(vocab, p.piece);
-  p.wide = wide_runs(n, p.piece, dim);
-  p.group_cols = p.wide ? 128 : big_tiles(n, p.piece) ? 64 : 32;
-  p.groups = (p.pieces - 1) * ceil_div(p.piece, p.group_cols) + ceil_div(vocab - (p.pieces - 1) * p.piece, p.group_cols);
-  p.ldg = ceil_div(p.piece, p.wide ? 256 : 8) * (p.wide ? 256 : 8);
-  p.g_rows = p.wide ? ceil_div(n, 64) * 64 : n;
+  const bool wide = wide_runs(n, p.piece, dim);
+  const bool few = n <= 32;
+  p.logits = wide ? kTilesWide : few ? kTiles64x32 : any_tiles(vocab, n);
+  p.again = wide ? kTilesWide : few ? kTiles64x32 : any_tiles(p.piece, n);
+  p.grads = wide ? kTilesWide : any_tiles(dim, p.piece);
+  p.dx = few ? kTiles128x32 : p.grads;
+  p.group_cols = wide ? 128 : rows_of(p.logits) / 2;
+  p.groups = ceil_div(vocab, p.group_cols);  // pieces are whole groups
+  const int64_t unit = wide ? 256 : 8;
+  p.ldg = ceil_div(p.piece, unit) * unit;
+  p.g_rows = wide ? ceil_div(n, 64) * 64 : n;
+  p.sum = p.pieces > 1;
+  if (!wide) {
+    // dx has few tiles and long sums: splits of about as many stages as dw's sums have, four at least, up to two
+    // blocks a CU, and few enough to be added in two rounds of loads
+    const int64_t tiles = std::max<int64_t>(1, ceil_div(dim, rows_of(p.dx)) * ceil_div(n, cols_of(p.dx)));
+    const int64_t stages = ceil_div(p.piece, 64), like_dw = ceil_div(stages, std::max<int64_t>(4, ceil_div(n, 64)));
+    p.splits = static_cast<int>(std::max<int64_t>(1, std::min(std::min(512 / tiles, like_dw), int64_t{16})));
+    p.sum = p.sum || p.splits > 1;
+  }
   size_t at = 0;
   bool fits = true;
-  const auto take = [&](int64_t a, int64_t b) {
-    const size_t from = at, size = nbytes(a, b);
+  const auto take = [&](int64_t a, int64_t b, int64_t c) {
+    const size_t from = at, size = nbytes(a, b, c);
     if (size == kSizeOverflow || __builtin_add_overflow(at, size, &at) || at > kSizeOverflow - 512) fits = false;
     else at = (at + 255) / 256 * 256;
     return from;
   };
-  p.stats = take(n, p.groups * 8);
-  p.zlabel = take(n, 4);
-  p.lse = take(n, 4);
-  p.row_loss = take(n, 4);
-  p.inv = take(1, 4);
+  p.at_stats = take(n, p.groups, 8);
+  p.at_zlabel = take(n, 4, 1);
+  p.at_lse = take(n, 4, 1);
+  p.at_row_loss = take(n, 4, 1);
+  p.at_inv = take(2, 4, 1);
   if (backward) {
-    p.g = take(p.g_rows, p.ldg * 2);
-    if (p.pieces > 1) p.sum = take(n, dim * 4);
+    p.at_g = take(p.g_rows, p.ldg, 2);
+    if (p.sum) p.at_sum = take(n, dim, 4 * p.splits);
   }
   p.bytes = at;
   return fits ? VDSL_OK : fail(VDSL_ERR_SHAPE, "linear_xent: the workspace's size overflows");
 }
 
-template <class Go>
-int with_tiles(int64_t m, int64_t n, bool big, const char* name, Go&& go) {
-  const int64_t b = big ? 128 : 64, tiles = ceil_div(m, b) * ceil_div(n, b);
-  if (tiles > 0x7fffffff) return fail(VDSL_ERR_UNSUPPORTED, std::string(name) + ": too many tiles");
-  go(static_cast<unsigned>(tiles));
-  return check_launch(name);
+template <class Cfg, int MODE>
+int launch_logits_on(const LogitArgs& a, float grad_scale, float* inv, hipStream_t s) {
+  const int64_t tiles = ceil_div(a.cols, Cfg::BM) * ceil_div(a.n, Cfg::BN);
+  if (tiles >= 0x7fffffff) return fail(VDSL_ERR_UNSUPPORTED, "linear_xent: too many tiles");
+  hipLaunchKernelGGL((xent_logits_any<Cfg, MODE>), dim3(static_cast<unsigned>(tiles + 1)), dim3(Cfg::NT), 0, s, a, grad_scale, inv);
+  return check_launch("xent_logits_any");
+}
+template <class T, int MODE>
+int launch_logits_any(const LogitArgs& a, float grad_scale, float* inv, hipStream_t s) {
+  if (ring_runs(a.dim)) return launch_logits_on<typename T::template Loop<true, false, false>, MODE>(a, grad_scale, inv, s);
+  return launch_logits_on<typename T::template Loop<false, false, false>, MODE>(a, grad_scale, inv, s);
 }
 
 template <int MODE>
-int launch_logits(const LogitArgs& a, const Plan& plan, hipStream_t s) {
-  if (plan.wide) {
-    const unsigned blocks = wide_blocks(ceil_div(a.n, 256) * ceil_div(a.cols, 256));
-    hipLaunchKernelGGL(xent_logits_wide<MODE>, dim3(blocks), dim3(WideCfg::NT), 0, s, a);
-    return check_launch("xent_logits_wide");
+int launch_logits(const LogitArgs& a, Tiling tiling, float grad_scale, float* inv, hipStream_t s) {
+  switch (tiling) {
+    case kTilesWide:
+      hipLaunchKernelGGL(xent_logits_wide<MODE>, dim3(wide_blocks(ceil_div(a.n, 256) * ceil_div(a.cols, 256))), dim3(WideCfg::NT), 0, s, a);
+      return check_launch("xent_logits_wide");
+    case kTiles128: return launch_logits_any<Tile128, MODE>(a, grad_scale, inv, s);
+    case kTiles128x64: return launch_logits_any<Tile128x64, MODE>(a, grad_scale, inv, s);
+    case kTiles64x32: return launch_logits_any<Tile64x32, MODE>(a, grad_scale, inv, s);
+    default: return launch_logits_any<Tile64, MODE>(a, grad_scale, inv, s);
   }
-  const bool big = plan.group_cols == 64;
-  using Big = AnyConfig<128, 128, 2, 2, false, false>;
-  using Small = AnyConfig<64, 64, 2, 2, false, false>;
-  return with_tiles(a.n, a.cols, big, "xent_logits_any", [&](unsigned tiles) {
-    if (big) hipLaunchKernelGGL((xent_logits_any<Big, MODE>), dim3(tiles), dim3(Big::NT), 0, s, a);
-    else hipLaunchKernelGGL((xent_logits_any<Small, MODE>), dim3(tiles), dim3(Small::NT), 0, s, a);
-  });
 }
 
-template <bool AKM, bool BKM>
-int launch_grad(const GradArgs& a, hipStream_t s) {
-  using Big = AnyConfig<128, 128, 2, 2, AKM, BKM>;
-  using Small = AnyConfig<64, 64, 2, 2, AKM, BKM>;
-  const bool big = big_tiles(a.m, a.n);
-  return with_tiles(a.m, a.n, big, "xent_grad_any", [&](unsigned tiles) {
-    if (big) hipLaunchKernelGGL(xent_grad_any<Big>, dim3(tiles), dim3(Big::NT), 0, s, a);
-    else hipLaunchKernelGGL(xent_grad_any<Small>, dim3(tiles), dim3(Small::NT), 0, s, a);
-  });
+template <class Tx, class Tw>
+int launch_grads_on(const GradArgs& dx, const GradArgs& dw, const float* row_loss, float* loss, hipStream_t s) {
+  const int64_t bx = Tx::tiles(dx.m, dx.n) * dx.splits, bw = Tw::tiles(dw.m, dw.n);
+  if (bx + bw >= 0x7fffffff) return fail(VDSL_ERR_UNSUPPORTED, "linear_xent: too many tiles");
+  const dim3 grid(static_cast<unsigned>(bx + bw + (loss ? 1 : 0)));
+  const int x = static_cast<int>(bx), w = static_cast<int>(bw);
+  if (ring_runs(dx.m)) hipLaunchKernelGGL((xent_grads_any<Tx, Tw, true>), grid, dim3(Tw::NT), 0, s, dx, dw, x, w, row_loss, loss);
+  else hipLaunchKernelGGL((xent_grads_any<Tx, Tw, false>), grid, dim3(Tw::NT), 0, s, dx, dw, x, w, row_loss, loss);
+  return check_launch("xent_grads_any");
+}
+template <class Tw>
+int launch_grads_any(const GradArgs& dx, const GradArgs& dw, Tiling dx_tiling, const float* row_loss, float* loss, hipStream_t s) {
+  if (dx_tiling == kTiles128x32) return launch_grads_on<Tile128x32, Tw>(dx, dw, row_loss, loss, s);
+  return launch_grads_on<Tw, Tw>(dx, dw, row_loss, loss, s);
 }
 
 template <bool BKM>
@@ -568,115 +704,96 @@ int run_xent(vdsl_queue q, int64_t n, int64_t dim, int64_t vocab, vdsl_buffer x,
   if (backward) {
     VDSL_TRY(check_buffer(q, dx, nbytes(n, dim, dtype_size(dx_dtype)), "dx", true));
     VDSL_TRY(check_buffer(q, dw, nbytes(vocab, dim, dtype_size(dw_dtype)), "dw", true));
-    if (dx == x || dx == w || dw == x || dw == w) return fail(VDSL_ERR_INVALID_ARG, "linear_xent_fwd_bwd: a gradient must not overwrite x or w");
+    if (dx == x || dx == w || dw == x || dw == w || dx == dw)
+      return fail(VDSL_ERR_INVALID_ARG, "linear_xent_fwd_bwd: a gradient must not share a buffer with x, w or the other one");
   }
   VDSL_TRY(check_buffer(q, workspace, plan.bytes, "workspace", true));
   const hipStream_t s = q->stream;
   char* const ws = static_cast<char*>(workspace->ptr);
   const int32_t* lab = static_cast<const int32_t*>(labels->ptr);
-  float* const inv = reinterpret_cast<float*>(ws + plan.inv);
-  float* const each = reinterpret_cast<float*>(ws + plan.row_loss);
-  uint16_t* const g = backward ? reinterpret_cast<uint16_t*>(ws + plan.g) : nullptr;
+  float* const inv = reinterpret_cast<float*>(ws + plan.at_inv);
+  float* const each = reinterpret_cast<float*>(ws + plan.at_row_loss);
+  float* const loss_out = static_cast<float*>(loss->ptr);
+  uint16_t* const g = backward ? reinterpret_cast<uint16_t*>(ws + plan.at_g) : nullptr;
+  const int64_t last_piece = (plan.pieces - 1) * plan.piece;
   LogitArgs la{};
   la.x = static_cast<const uint16_t*>(x->ptr);
+  la.w = static_cast<const uint16_t*>(w->ptr);
   la.labels = lab;
-  la.stats = reinterpret_cast<float2*>(ws + plan.stats);
-  la.zlabel = reinterpret_cast<float*>(ws + plan.zlabel);
+  la.stats = reinterpret_cast<float2*>(ws + plan.at_stats);
+  la.zlabel = reinterpret_cast<float*>(ws + plan.at_zlabel);
   la.g = g;
-  la.lse = reinterpret_cast<const float*>(ws + plan.lse);
+  la.lse = reinterpret_cast<const float*>(ws + plan.at_lse);
   la.n = static_cast<int>(n);
+  la.cols = la.vocab = static_cast<int>(vocab);
   la.dim = static_cast<int>(dim);
-  la.vocab = static_cast<int>(vocab);
   la.groups = static_cast<int>(plan.groups);
   la.ldg = plan.ldg;
-  const auto set_piece = [&](int64_t k) {
-    const int64_t v0 = k * plan.piece;
-    la.w = static_cast<const uint16_t*>(w->ptr) + v0 * dim;
-    la.v0 = static_cast<int>(v0);
-    la.cols = static_cast<int>(std::min(plan.piece, vocab - v0));
-    la.group0 = static_cast<int>(k * ceil_div(plan.piece, plan.group_cols));
-  };
+  la.g0 = static_cast<int>(last_piece);
   if (n > 0) {
-    for (int64_t k = 0; k < plan.pieces; ++k) {
-      set_piece(k);
-      if (backward && k == plan.pieces - 1) VDSL_TRY(launch_logits<kLogitCodes>(la, plan, s));
-      else VDSL_TRY(launch_logits<kLogitStats>(la, plan, s));
-    }
+    if (backward) VDSL_TRY(launch_logits<kLogitCodes>(la, plan.logits, grad_scale, inv, s));
+    else VDSL_TRY(launch_logits<kLogitStats>(la, plan.logits, grad_scale, inv, s));
     RowArgs ra{};
     ra.labels = lab;
     ra.stats = la.stats;
     ra.zlabel = la.zlabel;
-    ra.lse_octaves = reinterpret_cast<float*>(ws + plan.lse);
+    ra.lse_octaves = reinterpret_cast<float*>(ws + plan.at_lse);
     ra.lse = lse ? static_cast<float*>(lse->ptr) : nullptr;
     ra.row_loss = each;
     ra.row_loss_out = row_loss ? static_cast<float*>(row_loss->ptr) : nullptr;
     ra.g = g;
     ra.n = la.n;
-    ra.cols = la.cols;
+    ra.cols = static_cast<int>(vocab - last_piece);
     ra.vocab = la.vocab;
-    ra.v0 = la.v0;
-    ra.group0 = la.group0;
+    ra.v0 = static_cast<int>(last_piece);
+    ra.group0 = static_cast<int>(last_piece / plan.group_cols);
     ra.groups = la.groups;
     ra.group_cols = static_cast<int>(plan.group_cols);
     ra.ldg = plan.ldg;
     hipLaunchKernelGGL(xent_rows_kernel, dim3(static_cast<unsigned>(backward ? plan.g_rows : n)), dim3(256), 0, s, ra);
     VDSL_TRY(check_launch("xent_rows_kernel"));
   }
-  hipLaunchKernelGGL(xent_mean_kernel, dim3(1), dim3(1024), 0, s, each, lab, n, static_cast<int>(vocab), grad_scale,
-                     static_cast<float*>(loss->ptr), inv);
-  VDSL_TRY(check_launch("xent_mean_kernel"));
+  if (!backward || n == 0 || plan.grads == kTilesWide) {
+    hipLaunchKernelGGL(xent_mean_kernel, dim3(1), dim3(1024), 0, s, each, lab, n, la.vocab, grad_scale, loss_out, inv);
+    VDSL_TRY(check_launch("xent_mean_kernel"));
+  }
   if (!backward) return VDSL_OK;
   if (n == 0) {
     hipLaunchKernelGGL(xent_zero_kernel, dim3(2048), dim3(256), 0, s, static_cast<uint16_t*>(dw->ptr),
                        vocab * dim * static_cast<int64_t>(dtype_size(dw_dtype) / 2));
     return check_launch("xent_zero_kernel");
   }
+  float* const sum = plan.sum ? reinterpret_cast<float*>(ws + plan.at_sum) : nullptr;
+  la.g0 = 0;
   // The piece whose codes are held comes first, then those whose logits are formed again.
   for (int64_t t = 0; t < plan.pieces; ++t) {
-    const int64_t k = plan.pieces - 1 - t;
-    set_piece(k);
-    if (t > 0) VDSL_TRY(launch_logits<kLogitGrad>(la, plan, s));
-    float* const sum = plan.pieces > 1 ? reinterpret_cast<float*>(ws + plan.sum) : nullptr;
-    void* const dw_piece = static_cast<char*>(dw->ptr) + static_cast<int64_t>(la.v0) * dim * static_cast<int64_t>(dtype_size(dw_dtype));
-    if (plan.wide) {
-      // dx^T = w^T G^T over the piece, dw^T = x^T G
-      WideGradArgs x_args{la.w, g,        la.dim, la.n,        la.cols, 0,       dim,       plan.ldg, sum,
-                          t == 0, t == plan.pieces - 1, inv, dx->ptr, dx_dtype};
-      VDSL_TRY(launch_grad_wide<false>(x_args, n, s));
-      WideGradArgs w_args{la.x, g, la.dim, la.cols, la.n, static_cast<int>(plan.ldg), dim, plan.ldg, nullptr, true, true, inv,
-                          dw_piece, dw_dtype};
-      VDSL_TRY(launch_grad_wide<true>(w_args, plan.ldg, s));
+    const int64_t v0 = last_piece - t * plan.piece;
+    la.w = static_cast<const uint16_t*>(w->ptr) + v0 * dim;
+    la.v0 = static_cast<int>(v0);
+    la.cols = static_cast<int>(std::min(plan.piece, vocab - v0));
+    if (t > 0) VDSL_TRY(launch_logits<kLogitGrad>(la, plan.again, grad_scale, inv, s));
+    void* const dw_piece = static_cast<char*>(dw->ptr) + v0 * dim * static_cast<int64_t>(dtype_size(dw_dtype));
+    if (plan.grads == kTilesWide) {
+      const WideGradArgs for_dx{la.w, g,      la.dim, la.n,   la.cols, 0, dim, plan.ldg, sum, t == 0, t == plan.pieces - 1,
+                                inv,  dx->ptr, dx_dtype};
+      VDSL_TRY(launch_grad_wide<false>(for_dx, n, s));
+      const WideGradArgs for_dw{la.x, g,        la.dim, la.cols, la.n, static_cast<int>(plan.ldg), dim, plan.ldg, nullptr, true, true,
+                                inv,  dw_piece, dw_dtype};
+      VDSL_TRY(launch_grad_wide<true>(for_dw, plan.ldg, s));
       continue;
     }
-    GradArgs ga{};
-    ga.inv = inv;
-    ga.a = g;  // dx += G w
-    ga.lda = plan.ldg;
-    ga.b = la.w;
-    ga.ldb = -1;
-    ga.m = la.n;
-    ga.n = la.dim;
-    ga.k = la.cols;
-    ga.first = t == 0;
-    ga.last = t == plan.pieces - 1;
-    ga.sum = sum;
-    ga.out = dx->ptr;
-    ga.out_dt = dx_dtype;
-    VDSL_TRY((launch_grad<false, true>(ga, s)));
-    ga.a = g;  // dw of the piece = G^T x
-    ga.lda = plan.ldg;
-    ga.b = la.x;
-    ga.ldb = -1;
-    ga.m = la.cols;
-    ga.n = la.dim;
-    ga.k = la.n;
-    ga.first = ga.last = true;
-    ga.sum = nullptr;
-    ga.out = dw_piece;
-    ga.out_dt = dw_dtype;
-    VDSL_TRY((launch_grad<true, true>(ga, s)));
+    const GradArgs for_dx{la.w, g, la.dim, la.n, la.cols, dim, plan.ldg, sum, t == 0, plan.splits, inv, dx->ptr, dx_dtype};
+    const GradArgs for_dw{la.x, g, la.dim, la.cols, la.n, dim, plan.ldg, nullptr, true, 1, inv, dw_piece, dw_dtype};
+    float* const mean = t == 0 ? loss_out : nullptr;
+    if (plan.grads == kTiles128) VDSL_TRY(launch_grads_any<Tile128>(for_dx, for_dw, plan.dx, each, mean, s));
+    else if (plan.grads == kTiles128x64) VDSL_TRY(launch_grads_any<Tile128x64>(for_dx, for_dw, plan.dx, each, mean, s));
+    else VDSL_TRY(launch_grads_any<Tile64>(for_dx, for_dw, plan.dx, each, mean, s));
   }
-  return VDSL_OK;
+  if (plan.grads == kTilesWide || !sum) return VDSL_OK;
+  const int64_t blocks = ceil_div(n * dim, 256);
+  if (blocks > 0x7fffffff) return fail(VDSL_ERR_UNSUPPORTED, "linear_xent: dx too large");
+  hipLaunchKernelGGL(xent_join_kernel, dim3(static_cast<unsigned>(blocks)), dim3(64), 0, s, sum, plan.splits, n * dim, inv, dx->ptr, dx_dtype);
+  return check_launch("xent_join_kernel");
 }
 
 }  // namespace

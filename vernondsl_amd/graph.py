@@ -22,6 +22,10 @@ Backward rules (y = act(x W^T), W stored [out][in]):
     dx   = g W          -> vdsl_op_gemm_bf16(A = g [B][out], B = W [out][in], trans_b = 0)
     MSE: loss and dL/dy = 2 (y - t) / n (bf16, plus transpose) from one fused op.
     y = a + b: dL/da = dL/db = dL/dy.
+    embedding: dL/dtable = the sum of dL/dy over each row's tokens (vdsl_op_embedding_bwd).
+    layer_norm: dL/dx, dL/dgamma, dL/dbeta from dL/dy (f32 or bf16), x and the forward pass's mean and rstd.
+    linear_cross_entropy (the output layer with its loss, logits never stored): dL/dx and dL/dW from the
+    loss op itself (vdsl_op_linear_xent_fwd_bwd); W may be the embedding's table (tied weights).
     A value read by several ops (a residual input, a weight tied across layers): dL/dv is the f32
     sum of the terms its readers give (an add op per extra term); fusions that would apply a term
     before the sum is complete (GELU' in the dL/dx GEMM, the loss in the last GEMM) are skipped
@@ -165,6 +169,46 @@ class Graph:
         self._op("add", [a, b], [y])
         return y
 
+    def embedding(self, table: Value, ids: Value, scale: float = 1.0, out_dtype: str = "f32", name=None) -> Value:
+        """y[i] = scale * table[ids[i]]; table [vocab][dim] f32 or bf16, ids [n] i32 (zeros where an id is
+        outside the table)."""
+        if table.dtype not in ("f32", "bf16") or out_dtype not in ("f32", "bf16"):
+            raise TypeError("embedding takes an f32 or bf16 table and stores f32 or bf16")
+        if ids.dtype != "i32" or len(ids.shape) != 1 or len(table.shape) != 2:
+            raise TypeError("embedding takes a table [vocab][dim] and i32 ids [n]")
+        y = self._value(name or self._fresh("embedding"), (ids.shape[0], table.shape[1]), out_dtype, requires_grad=table.requires_grad)
+        self._op("embedding", [table, ids], [y], scale=float(scale))
+        return y
+
+    def layer_norm(self, x: Value, gamma: Value, beta: Value | None = None, eps: float = 1e-5, out_dtype: str = "bf16",
+                   name=None) -> Value:
+        """y = (x - mean) * rstd * gamma + beta over the rows of x [rows][cols] (f32 or bf16); gamma, beta [cols]
+        of one type."""
+        if x.dtype not in ("f32", "bf16") or out_dtype not in ("f32", "bf16"):
+            raise TypeError("layer_norm takes and stores f32 and bf16 tensors")
+        for p in (gamma, beta):
+            if p is not None and (p.shape != x.shape[1:] or p.dtype != gamma.dtype or p.dtype not in ("f32", "bf16")):
+                raise TypeError(f"layer_norm: {p.name} must be [{x.shape[1]}], f32 or bf16, gamma and beta of one type")
+        needs = x.requires_grad or gamma.requires_grad or (beta is not None and beta.requires_grad)
+        y = self._value(name or self._fresh("layer_norm"), x.shape, out_dtype, requires_grad=needs)
+        mean = self._value(self._fresh("mean"), x.shape[:1], "f32")  # kept for the backward pass
+        rstd = self._value(self._fresh("rstd"), x.shape[:1], "f32")
+        self._op("layer_norm", [x, gamma] + ([beta] if beta is not None else []), [y, mean, rstd], eps=float(eps))
+        return y
+
+    def linear_cross_entropy(self, x: Value, w: Value, labels: Value, piece: int = 0, name="loss") -> Value:
+        """The output layer over a vocabulary and its softmax cross entropy, without storing the logits: the mean over
+        the rows whose label is in [0, vocab) of logsumexp(x W^T) - (x W^T)[label].  x [n][dim] and w [vocab][dim] bf16,
+        labels [n] i32; piece: columns of the vocabulary worked on at a time in the backward pass (0: the library's
+        choice)."""
+        if x.dtype != "bf16" or w.dtype != "bf16" or labels.dtype != "i32":
+            raise TypeError("linear_cross_entropy takes bf16 activations and weights and i32 labels")
+        if x.shape[1] != w.shape[1] or labels.shape != x.shape[:1]:
+            raise ValueError(f"linear_cross_entropy: x {x.shape}, W {w.shape} and labels {labels.shape} do not fit")
+        loss = self._value(name, (1,), "f32", requires_grad=x.requires_grad or w.requires_grad)
+        self._op("linear_xent", [x, w, labels], [loss], piece=int(piece))
+        return loss
+
     def mse_loss(self, y: Value, t: Value, name="loss") -> Value:
         if y.dtype != "f32" or t.dtype != "f32" or y.shape != t.shape:
             raise TypeError("mse_loss takes two f32 tensors of one shape")
@@ -203,8 +247,8 @@ class Graph:
     # ---- autodiff --------------------------------------------------------------------------------
     def backward(self, loss: Value) -> dict:
         """Appends the backward ops of `loss` and returns {param name: f32 gradient Value}."""
-        if loss.producer is None or loss.producer.kind != "mse":
-            raise ValueError("backward() starts from an mse_loss value")
+        if loss.producer is None or loss.producer.kind not in ("mse", "linear_xent"):
+            raise ValueError("backward() starts from an mse_loss or a linear_cross_entropy value")
         fwd_ops = list(self.ops)
         uses: dict[str, int] = {}  # forward reads of each value: more than one means summed gradients
         for op in fwd_ops:
@@ -212,32 +256,42 @@ class Graph:
                 uses[v.name] = uses.get(v.name, 0) + 1
         # gradient of each activation: ("bf16", g, g_t) or ("f32", g)
         grad: dict[str, tuple] = {}
-        y, _ = loss.producer.inputs
-        dy = self._value(self._fresh("d_" + y.name), y.shape, "bf16", "grad")
-        dy_t = self._value(self._fresh("dT_" + y.name), y.shape[::-1], "bf16", "grad")
-        self._transposed.add(dy_t.name)
-        part = self._value(self._fresh("mse_partials"), (max(1, kernels.mse_partials_count(*y.shape)),), "f32", "scratch")
-        loss.producer.outputs += [dy, dy_t, part]  # the forward MSE op also emits dL/dy
-        grad[y.name] = ("bf16", dy, dy_t)
-        lin = y.producer
-        if (self.fuse_mse and lin is not None and lin.kind == "linear" and lin.attrs["act"] == "none"
-                and uses[y.name] == 1 and lin.attrs.get("packed") is not None and y.dtype == "f32"
-                and y.shape[0] % 128 == 0 and y.shape[1] % 256 == 0):
-            # the linear op and the loss become one op: the GEMM's epilogue forms the loss and dL/dy
-            mse_op = loss.producer
-            self.ops.remove(mse_op)
-            lin.kind = "linear_mse"
-            lin.inputs.append(mse_op.inputs[1])
-            lin.outputs += [loss, dy, dy_t, part]
-            for v in (loss, dy, dy_t, part):
-                v.producer = lin
-            if not self.keep_y:  # the fused op does not store y: nothing holds it
-                self.elided.add(y.name)
-        contrib: dict[str, list] = {}  # param name -> its gradient's terms, one per linear op reading it
+        contrib: dict[str, list] = {}  # param name -> its gradient's terms, one per op reading it
+        if loss.producer.kind == "linear_xent":
+            x, w, _ = loss.producer.inputs
+            dx = self._value(self._fresh("d_" + x.name), x.shape, "f32", "grad")
+            dw = self._value("grad_" + w.name if uses[w.name] == 1 else self._fresh("dterm_" + w.name), w.shape, "f32", "grad")
+            loss.producer.outputs += [dx, dw]  # the forward op also emits both gradients
+            dx.producer = dw.producer = loss.producer
+            grad[x.name] = ("f32", dx)
+            if w.requires_grad:
+                contrib[w.name] = [dw]
+        else:
+            y, _ = loss.producer.inputs
+            dy = self._value(self._fresh("d_" + y.name), y.shape, "bf16", "grad")
+            dy_t = self._value(self._fresh("dT_" + y.name), y.shape[::-1], "bf16", "grad")
+            self._transposed.add(dy_t.name)
+            part = self._value(self._fresh("mse_partials"), (max(1, kernels.mse_partials_count(*y.shape)),), "f32", "scratch")
+            loss.producer.outputs += [dy, dy_t, part]  # the forward MSE op also emits dL/dy
+            grad[y.name] = ("bf16", dy, dy_t)
+            lin = y.producer
+            if (self.fuse_mse and lin is not None and lin.kind == "linear" and lin.attrs["act"] == "none"
+                    and uses[y.name] == 1 and lin.attrs.get("packed") is not None and y.dtype == "f32"
+                    and y.shape[0] % 128 == 0 and y.shape[1] % 256 == 0):
+                # the linear op and the loss become one op: the GEMM's epilogue forms the loss and dL/dy
+                mse_op = loss.producer
+                self.ops.remove(mse_op)
+                lin.kind = "linear_mse"
+                lin.inputs.append(mse_op.inputs[1])
+                lin.outputs += [loss, dy, dy_t, part]
+                for v in (loss, dy, dy_t, part):
+                    v.producer = lin
+                if not self.keep_y:  # the fused op does not store y: nothing holds it
+                    self.elided.add(y.name)
         for op in reversed(fwd_ops):
-            if op.kind == "mse":
+            if op.kind in ("mse", "linear_xent"):
                 continue
-            if op.kind not in ("linear", "linear_mse", "add"):
+            if op.kind not in ("linear", "linear_mse", "add", "embedding", "layer_norm"):
                 raise NotImplementedError(f"no backward rule for {op.kind}")
             y = op.outputs[0]
             if y.name not in grad:
@@ -246,6 +300,21 @@ class Graph:
                 for x in op.inputs:
                     if x.requires_grad or (x.producer is not None and x.kind == "activation" and _needs(x, self)):
                         self._accumulate(grad, x, grad[y.name])
+                continue
+            if op.kind == "embedding":
+                table, ids = op.inputs
+                if table.requires_grad:
+                    dt = self._param_term(table, uses, contrib)
+                    self._op("embedding_bwd", [ids, grad[y.name][1]], [dt], scale=op.attrs["scale"])
+                continue
+            if op.kind == "layer_norm":
+                x, gamma = op.inputs[:2]
+                dx = self._value(self._fresh("d_" + x.name), x.shape, "f32", "grad")
+                dp = [self._param_term(p, uses, contrib) if p.requires_grad else None for p in op.inputs[1:]]
+                self._op("layer_norm_bwd", [grad[y.name][1], x, gamma, op.outputs[1], op.outputs[2]], [dx] + [d for d in dp if d is not None],
+                         dgamma=dp[0], dbeta=dp[1] if len(dp) > 1 else None)
+                if x.requires_grad or (x.producer is not None and x.kind == "activation" and _needs(x, self)):
+                    self._accumulate(grad, x, ("f32", dx))
                 continue
             x, w = op.inputs[:2]
             g = grad[y.name]
@@ -333,6 +402,12 @@ class Graph:
         if self.k_major_grads:
             self._elide_unread_transposes()
         return param_grads
+
+    def _param_term(self, p: Value, uses: dict, contrib: dict) -> Value:
+        """The f32 value of one op's term of param p's gradient: the gradient itself where no other op reads p."""
+        d = self._value("grad_" + p.name if uses[p.name] == 1 else self._fresh("dterm_" + p.name), p.shape, "f32", "grad")
+        contrib.setdefault(p.name, []).append(d)
+        return d
 
     def _accumulate(self, grad: dict, x: Value, g: tuple):
         """Adds the gradient term g to dL/dx: the first term is kept as it is; a second one (x read
@@ -427,6 +502,13 @@ class Executable:
             if op.kind == "w8a8_packed":
                 xq, _, wp, _ = op.inputs
                 ws = max(ws, kernels.gemm_w8a8_packed_workspace_bytes(xq.shape[0], wp.shape[0], xq.shape[1]))
+            if op.kind == "embedding_bwd":
+                ws = max(ws, kernels.embedding_bwd_workspace_bytes(op.inputs[0].shape[0], *op.outputs[0].shape))
+            if op.kind == "layer_norm_bwd":
+                ws = max(ws, kernels.layer_norm_bwd_workspace_bytes(*op.inputs[1].shape))
+            if op.kind == "linear_xent":
+                (n, dim), vocab, backward = op.inputs[0].shape, op.inputs[1].shape[0], len(op.outputs) > 1
+                ws = max(ws, kernels.linear_xent_workspace_bytes(n, vocab, dim, op.attrs["piece"] if backward else 0, backward))
         outs = g.host_outputs()
         try:
             for v in g.values.values():
@@ -508,6 +590,9 @@ class Executable:
         if op.kind == "gemm_mul_bwd":
             (M, K), N = ins[0].shape, ins[1].shape[0]
             return f"gemm x stored GELU' (packed B) {M}x{N}x{K}"
+        if op.kind == "linear_xent":
+            (M, K), N = ins[0].shape, ins[1].shape[0]
+            return f"linear + cross entropy{' and both gradients' if len(outs) > 1 else ''} {M}x{N}x{K}"
         if op.kind in ("w8a8", "w8a8_packed"):
             (M, K), N = ins[0].shape, ins[2].shape[0]
             return f"{op.kind} {'relu' if op.attrs['relu'] else 'no relu'} {M}x{N}x{K}"
@@ -518,6 +603,8 @@ class Executable:
         ins = op.inputs
         if op.kind in ("linear", "gemm_gelu_bwd", "gemm_mul_bwd", "linear_mse"):
             return 2 * ins[0].shape[0] * ins[0].shape[1] * ins[1].shape[0]
+        if op.kind == "linear_xent":
+            return (6 if len(op.outputs) > 1 else 2) * ins[0].shape[0] * ins[0].shape[1] * ins[1].shape[0]
         if op.kind == "gemm":
             a, b = ins
             M, K = (a.shape[1], a.shape[0]) if op.attrs["trans_a"] else a.shape
@@ -554,6 +641,20 @@ class Executable:
                 kernels.mse_fwd_bwd(q, ins[0], ins[1], loss, outs[1], outs[2], outs[3])
             else:
                 raise RuntimeError("mse without backward: call Graph.backward() or use the loss op's fused form")
+        elif op.kind == "linear_xent":
+            if len(outs) > 1:
+                kernels.linear_xent_fwd_bwd(q, *ins, outs[0], outs[1], outs[2], piece=op.attrs["piece"], workspace=self.workspace)
+            else:
+                kernels.linear_xent_fwd(q, *ins, outs[0], workspace=self.workspace)
+        elif op.kind == "embedding":
+            kernels.embedding_fwd(q, ins[0], ins[1], outs[0], op.attrs["scale"])
+        elif op.kind == "embedding_bwd":
+            kernels.embedding_bwd(q, ins[0], ins[1], outs[0], op.attrs["scale"], self.workspace)
+        elif op.kind == "layer_norm":
+            kernels.layer_norm_fwd(q, ins[0], ins[1], ins[2] if len(ins) > 2 else None, *outs, eps=op.attrs["eps"])
+        elif op.kind == "layer_norm_bwd":
+            dp = [None if op.attrs[k] is None else T[op.attrs[k].name] for k in ("dgamma", "dbeta")]
+            kernels.layer_norm_bwd(q, *ins, outs[0], *dp, workspace=self.workspace)
         elif op.kind == "gelu_bwd":
             kernels.gelu_bwd(q, ins[0], ins[1], outs[0], outs[1])
         elif op.kind == "relu_bwd":
@@ -620,7 +721,7 @@ class Step:
         self.graph.destroy()
 
 
-# ---- the two workload graphs ------------------------------------------------------------------------
+# ---- the workload graphs ------------------------------------------------------------------------
 def mlp_train_graph(batch=2048, d_in=4096, hidden=4096, d_out=4096, prepare_transposes=True,
                     fuse_gelu_backward=True, pack_weights=True, fuse_mse=True, keep_y=True, store_gelu_deriv=True,
                     k_major_grads=True):
@@ -650,3 +751,25 @@ def w8a8_infer_graph(batch=512, widths=(8192, 8192, 8192, 8192, 1024)):
         last = li == len(widths) - 2
         h = g.quant_linear(h, wq, ws, relu=not last, name="Y" if last else f"H{li}")
     return g
+
+
+def token_mlp_train_graph(tokens=2048, vocab=32768, dim=1024, hidden=4096, layers=2, tied=True, piece=0):
+    """A training step of a model of tokens whose blocks are MLPs: ids -> embedding (scaled by sqrt(dim), an f32
+    residual stream) -> [h + W2 gelu(W1 norm(h))] per layer -> norm -> output layer and cross entropy against the labels,
+    and back to every parameter.  tied: the output layer's weights are the embedding's table.  Ids and labels outside
+    [0, vocab) are padding."""
+    g = Graph(prepare_transposes=True, fuse_gelu_backward=True, pack_weights=True, store_gelu_deriv=True, k_major_grads=True)
+    ids, labels = g.input("ids", (tokens,), "i32"), g.input("labels", (tokens,), "i32")
+    table = g.param("E", (vocab, dim), "bf16")
+
+    def norm(x, name):
+        return g.layer_norm(x, g.param(name + "_gamma", (dim,), "f32"), g.param(name + "_beta", (dim,), "f32"))
+
+    h = g.embedding(table, ids, scale=float(dim) ** 0.5, out_dtype="f32")
+    for k in range(layers):
+        u = g.linear(norm(h, f"norm{k}"), g.param(f"W{k}_up", (hidden, dim), "bf16"), act="gelu")
+        h = g.add(h, g.linear(u, g.param(f"W{k}_down", (dim, hidden), "bf16"), out_dtype="f32"))
+    out = table if tied else g.param("W_out", (vocab, dim), "bf16")
+    loss = g.linear_cross_entropy(norm(h, "norm_out"), out, labels, piece)
+    grads = g.backward(loss)
+    return g, grads

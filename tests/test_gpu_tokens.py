@@ -457,6 +457,61 @@ def test_linear_xent_nan_and_inf_stay_in_their_rows(q, own):
     assert np.array_equal(np.isnan(dx.numpy(q)).all(1), bad) and np.array_equal(np.isnan(dx.numpy(q)).any(1), bad)
 
 
+def test_linear_xent_row_of_minus_infinity(q, own):
+    """A row whose logits all are -inf has no softmax: NaN in its loss and its gradient, whole or in pieces, and no
+    other row's."""
+    r = np.random.default_rng(14)
+    x, w, labels = xent_input(r, 50, 64, 700)
+    labels[:] = np.arange(50) % 700
+    w[:, 5] = np.abs(w[:, 5]) + 1.0
+    x[7, 5] = -np.inf
+    tx, tw, tl = own.put(x, "bf16"), own.put(bf16(w), "bf16"), own.put(labels, "i32")
+    bad = np.arange(50) == 7
+    for piece in (0, 256):
+        loss, each, dx, dw = (own.empty(s, "f32") for s in ((1,), (50,), (50, 64), (700, 64)))
+        kernels.linear_xent_fwd_bwd(q, tx, tw, tl, loss, dx, dw, row_loss=each, piece=piece,
+                                    workspace=own.scratch(kernels.linear_xent_workspace_bytes(50, 700, 64, piece=piece)))
+        assert np.array_equal(np.isnan(each.numpy(q)), bad)
+        assert np.array_equal(np.isnan(dx.numpy(q)).all(1), bad) and np.array_equal(np.isnan(dx.numpy(q)).any(1), bad)
+
+
+def test_linear_xent_piece_of_any_size(q, own):
+    r = np.random.default_rng(15)
+    x, w, labels = xent_input(r, 20, 24, 300)
+    whole = check_xent(q, own, x, w, labels)
+    for piece in (300, 301, 2 ** 62, 2 ** 63 - 1):
+        for a, b in zip(whole, check_xent(q, own, x, w, labels, piece=piece)):
+            assert np.array_equal(a, b)
+
+
+# long sums for the weights' gradient in few tiles
+@pytest.mark.parametrize("n,dim,vocab,piece", [(2000, 72, 300, 0), (1500, 71, 130, 0), (1100, 64, 700, 256)])
+def test_linear_xent_many_rows_few_logits(q, own, n, dim, vocab, piece):
+    check_xent(q, own, *xent_input(np.random.default_rng(n), n, dim, vocab), piece=piece)
+
+
+def test_linear_xent_rows_past_a_launch(q, own):
+    """More rows than one dimension of a launch holds blocks for.  Rows repeat with a period, so 64 bits of a period give
+    every row's loss and gradient."""
+    r = np.random.default_rng(16)
+    period, dim, vocab = 1024, 8, 24
+    n = (1 << 24) + period
+    x, w, labels = xent_input(r, period, dim, vocab)
+    tx, tw, tl = own.put(np.tile(x, (n // period, 1)), "bf16"), own.put(w, "bf16"), own.put(np.tile(labels, n // period), "i32")
+    loss, each, dx, dw = own.empty((1,), "f32"), own.empty((n,), "f32"), own.empty((n, dim), "f32"), own.empty((vocab, dim), "f32")
+    kernels.linear_xent_fwd_bwd(q, tx, tw, tl, loss, dx, dw, row_loss=each,
+                                workspace=own.scratch(kernels.linear_xent_workspace_bytes(n, vocab, dim)))
+    x, w = x.astype(np.float64), w.astype(np.float64)
+    wloss, weach, _, g, counts = xent(x, w, labels)
+    _, ee, eg = xent_tolerances(x, w, labels)
+    inv = 1.0 / (counts.sum() * (n // period))
+    assert np.all(np.abs(each.numpy(q).reshape(-1, period) - weach) <= ee)
+    assert abs(loss.numpy(q)[0] - wloss) <= ee.sum() / counts.sum() + 2 * U * abs(wloss)
+    tol = (eg @ np.abs(w) + (vocab + 8) * U * (np.abs(g) @ np.abs(w))) * inv
+    want = g @ w * inv
+    assert np.all(np.abs(dx.numpy(q).reshape(-1, period, dim) - want) <= tol + U * (np.abs(want) + tol))
+
+
 def test_linear_xent_against_differences(q, own):
     """The gradients against central differences of the 64-bit loss along a direction (see the layer norm's)."""
     r = np.random.default_rng(13)

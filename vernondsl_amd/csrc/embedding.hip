@@ -25,7 +25,7 @@ __global__ __launch_bounds__(256) void embedding_fwd_kernel(const void* __restri
                                                             void* __restrict__ out, int64_t n, int64_t dim, int64_t vocab,
                                                             float scale, int log_l) {
   const int lanes = 1 << log_l;
-  const int64_t i = (static_cast<int64_t>(blockIdx.x) << (8 - log_l)) + (threadIdx.x >> log_l);
+  const int64_t i = (block_index() << (8 - log_l)) + (threadIdx.x >> log_l);
   if (i >= n) return;
   const int32_t id = ids[i];
   const bool valid = id >= 0 && id < vocab;
@@ -367,7 +367,7 @@ __global__ __launch_bounds__(256) void embedding_bwd_kernel(const uint32_t* __re
                                                             const float* __restrict__ partials, int chunk,
                                                             float* __restrict__ dtable, int n, int64_t dim, int64_t vocab,
                                                             float scale, int log_l) {
-  const int64_t v = (static_cast<int64_t>(blockIdx.x) << (8 - log_l)) + uniform(threadIdx.x >> log_l);
+  const int64_t v = (block_index() << (8 - log_l)) + uniform(threadIdx.x >> log_l);
   int e0 = 0, e1 = 0;
   if constexpr (CHUNKS) {
     if (v >= vocab) return;
@@ -411,7 +411,8 @@ int lanes_log2(int64_t units) {
 
 int check_extents(int64_t n, int64_t dim, int64_t vocab) {
   if (n < 0 || dim < 0 || vocab < 0) return fail(VDSL_ERR_INVALID_ARG, "negative shape");
-  if (n > 0x7fffffff || vocab > 0x7fffffff) return fail(VDSL_ERR_UNSUPPORTED, "embedding: too many tokens or table rows");
+  // positions are ints that may run a tile or a chunk past n, and embedding_chunk_kernel's lanes stay below 2^32
+  if (n > 0x7f000000 || vocab > 0x7fffffff) return fail(VDSL_ERR_UNSUPPORTED, "embedding: too many tokens or table rows");
   if (dim > 0x1fffffff) return fail(VDSL_ERR_UNSUPPORTED, "embedding: rows too wide");
   return VDSL_OK;
 }
@@ -442,8 +443,8 @@ extern "C" int vdsl_op_embedding_fwd(vdsl_queue q, int64_t n, int64_t dim, int64
     const int l = lanes_log2(units);
     const int64_t bx = (n + (256 >> l) - 1) >> (8 - l), by = (units + (int64_t{KU} << l) - 1) / (int64_t{KU} << l);
     if (by > 65535) return fail(VDSL_ERR_UNSUPPORTED, "embedding_fwd: rows too wide");
-    hipLaunchKernelGGL((embedding_fwd_kernel<TT, OT, U, KU>), dim3(static_cast<unsigned>(bx), static_cast<unsigned>(by)), dim3(256), 0,
-                       q->stream, table->ptr, static_cast<const int32_t*>(ids->ptr), out->ptr, n, dim, vocab, scale, l);
+    hipLaunchKernelGGL((embedding_fwd_kernel<TT, OT, U, KU>), block_grid(bx, by), dim3(256), 0, q->stream, table->ptr,
+                       static_cast<const int32_t*>(ids->ptr), out->ptr, n, dim, vocab, scale, l);
     return check_launch("embedding_fwd_kernel");
   };
   // A lane takes 4 units where that leaves enough waves to fill the card, so that their loads are in flight together.
@@ -570,7 +571,7 @@ extern "C" int vdsl_op_embedding_bwd(vdsl_queue q, int64_t n, int64_t dim, int64
   const auto go = [&](auto dyt, auto u, auto units_a_lane) {
     constexpr int DYT = decltype(dyt)::value, U = decltype(u)::value, NV = decltype(units_a_lane)::value;
     const int64_t rows = 256 >> l;
-    const dim3 grid(static_cast<unsigned>((vocab + rows - 1) / rows), static_cast<unsigned>(strips));
+    const dim3 grid = block_grid((vocab + rows - 1) / rows, strips);
     if (!p.chunk) {
       hipLaunchKernelGGL((embedding_bwd_kernel<DYT, U, NV, false>), grid, dim3(256), 0, s, sorted, order, dy->ptr, nullptr, nullptr, 0,
                          static_cast<float*>(dtable->ptr), count, dim, vocab, scale, l);

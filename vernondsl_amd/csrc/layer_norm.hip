@@ -147,8 +147,9 @@ __global__ __launch_bounds__(S::kThreads) void layer_norm_fwd_rows(const void* x
 __global__ __launch_bounds__(1024) void layer_norm_fwd_stream(const void* x, int x_dt, const void* __restrict__ gamma,
                                                               const void* __restrict__ beta, int param_dt, void* y, int y_dt,
                                                               float* __restrict__ mean_out, float* __restrict__ rstd_out,
-                                                              int64_t cols, float eps) {
-  const int64_t row = blockIdx.x, base = row * cols;
+                                                              int64_t rows, int64_t cols, float eps) {
+  const int64_t row = block_index(), base = row * cols;
+  if (row >= rows) return;
   float s[1] = {0.0f};
   for (int64_t c = 4 * threadIdx.x; c < cols; c += 4096) {
     float v[4];
@@ -290,8 +291,9 @@ __global__ __launch_bounds__(S::kThreads) void layer_norm_bwd_rows(const void* d
 __global__ __launch_bounds__(1024) void layer_norm_bwd_stream(const void* dy, int dy_dt, const void* __restrict__ x, int x_dt,
                                                               const void* __restrict__ gamma, int param_dt,
                                                               const float* __restrict__ mean, const float* __restrict__ rstd,
-                                                              void* dx, int dx_dt, int64_t cols) {
-  const int64_t row = blockIdx.x, base = row * cols;
+                                                              void* dx, int dx_dt, int64_t rows, int64_t cols) {
+  const int64_t row = block_index(), base = row * cols;
+  if (row >= rows) return;
   const float m = mean[row], r = rstd[row];
   float s[2] = {0.0f, 0.0f};
   float m1 = 0.0f, m2 = 0.0f;
@@ -350,7 +352,7 @@ __global__ __launch_bounds__(1024) void layer_norm_bwd_finish(const float* __res
                                                               float* __restrict__ dgamma, float* __restrict__ dbeta) {
   __shared__ double part[16][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 64 + lane;
+  const int64_t i = block_index() * 64 + lane;
   double s = 0.0;
   if (i < 2 * cols) {
 #pragma unroll 8
@@ -422,8 +424,8 @@ extern "C" int vdsl_op_layer_norm_fwd(vdsl_queue q, int64_t rows, int64_t cols, 
     return check_launch("layer_norm_fwd_rows");
   };
   const auto wide = [&] {
-    hipLaunchKernelGGL(layer_norm_fwd_stream, dim3(static_cast<unsigned>(rows)), dim3(1024), 0, q->stream, x->ptr, x_dtype, g, b,
-                       param_dtype, y->ptr, y_dtype, mo, ro, cols, eps);
+    hipLaunchKernelGGL(layer_norm_fwd_stream, block_grid(rows), dim3(1024), 0, q->stream, x->ptr, x_dtype, g, b,
+                       param_dtype, y->ptr, y_dtype, mo, ro, rows, cols, eps);
     return check_launch("layer_norm_fwd_stream");
   };
   using F = std::integral_constant<int, VDSL_F32>;
@@ -490,8 +492,8 @@ extern "C" int vdsl_op_layer_norm_bwd(vdsl_queue q, int64_t rows, int64_t cols, 
                          0, q->stream, dy->ptr, dy_dtype, x->ptr, x_dtype, mi, ri, part, rows, cols);
       VDSL_TRY(check_launch("layer_norm_bwd_columns"));
     }
-    hipLaunchKernelGGL(layer_norm_bwd_stream, dim3(static_cast<unsigned>(rows)), dim3(1024), 0, q->stream, dy->ptr, dy_dtype, x->ptr,
-                       x_dtype, g, param_dtype, mi, ri, dx->ptr, dx_dtype, cols);
+    hipLaunchKernelGGL(layer_norm_bwd_stream, block_grid(rows), dim3(1024), 0, q->stream, dy->ptr, dy_dtype, x->ptr,
+                       x_dtype, g, param_dtype, mi, ri, dx->ptr, dx_dtype, rows, cols);
     return check_launch("layer_norm_bwd_stream");
   };
   using F = std::integral_constant<int, VDSL_F32>;
@@ -508,7 +510,7 @@ extern "C" int vdsl_op_layer_norm_bwd(vdsl_queue q, int64_t rows, int64_t cols, 
   if (!params) return VDSL_OK;
   const int64_t blocks = (2 * cols + 63) / 64;
   if (blocks > 0x7fffffff) return fail(VDSL_ERR_UNSUPPORTED, "layer_norm_bwd: too many columns");
-  hipLaunchKernelGGL(layer_norm_bwd_finish, dim3(static_cast<unsigned>(blocks)), dim3(1024), 0, q->stream, part, partial_rows, cols,
+  hipLaunchKernelGGL(layer_norm_bwd_finish, block_grid(blocks), dim3(1024), 0, q->stream, part, partial_rows, cols,
                      dgamma ? static_cast<float*>(dgamma->ptr) : nullptr, dbeta ? static_cast<float*>(dbeta->ptr) : nullptr);
   return check_launch("layer_norm_bwd_finish");
 }

@@ -1,5 +1,5 @@
 // Units of consecutive elements of a dense row, for kernels that give a lane several units of a row of
-// any length: F32 or BF16 memory, f32 registers.  A row of an odd number of elements starts anywhere,
+// any length (F32 or BF16 memory, f32 registers), and grids of any number of blocks.  A row of an odd number of elements starts anywhere,
 // so the vector accesses ask for no more than the element's alignment.
 #pragma once
 
@@ -17,6 +17,14 @@ struct __attribute__((packed, aligned(2))) U32x2At2 {
 struct __attribute__((packed, aligned(4))) F32x4At4 {
   f32x4 v;
 };
+
+// A grid of `blocks` blocks of up to 1024 lanes (times y): a launch takes fewer than 2^32 lanes along x, so x holds
+// 2^21 blocks and z what that leaves.  The last of z may hold more: a kernel returns from those past its own.
+inline dim3 block_grid(int64_t blocks, int64_t y = 1) {
+  const int64_t x = blocks < (1 << 21) ? blocks : (1 << 21);
+  return dim3(static_cast<unsigned>(x), static_cast<unsigned>(y), static_cast<unsigned>((blocks + x - 1) / x));
+}
+__device__ __forceinline__ int64_t block_index() { return static_cast<int64_t>(blockIdx.z) * gridDim.x + blockIdx.x; }
 
 template <int DT>
 __device__ __forceinline__ float load_elem(const void* __restrict__ p, int64_t i) {

@@ -215,12 +215,13 @@ template <class Cfg, int MODE>
 __global__ __launch_bounds__(Cfg::NT) void xent_logits_any(LogitArgs p, float grad_scale, float* inv) {
   __shared__ __attribute__((aligned(1024))) char smem[Cfg::LDS_BYTES];
   const int tiles_m = (p.cols + Cfg::BM - 1) / Cfg::BM, tiles_n = (p.n + Cfg::BN - 1) / Cfg::BN, tiles = tiles_m * tiles_n;
-  if (static_cast<int>(blockIdx.x) == tiles) {
-    count_rows(p.labels, p.n, p.vocab, grad_scale, inv, smem);
+  const int64_t block = block_index();
+  if (block >= tiles) {
+    if (block == tiles) count_rows(p.labels, p.n, p.vocab, grad_scale, inv, smem);
     return;
   }
   int tm, tn;
-  tile_coords(xcd_remap(blockIdx.x, tiles), tiles_m, tiles_n, tm, tn);
+  tile_coords(xcd_remap(static_cast<int>(block), tiles), tiles_m, tiles_n, tm, tn);
   f32x16 acc[Cfg::FM][Cfg::FN];
   Cfg::run(p.w, p.x, p.cols, p.n, p.dim, 0, p.dim, tm * Cfg::BM, tn * Cfg::BN, smem, acc, p.dim, p.dim);
   const int wave = threadIdx.x >> 6;
@@ -251,15 +252,16 @@ struct RowArgs {
   float* row_loss_out;  // may be null
   uint16_t* g;      // codes in, G out, [n][ldg]; null: none
   int n, cols, vocab, v0, group0, groups, group_cols;
-  int64_t ldg;
+  int64_t ldg, g_rows;
 };
 
 // A block per row: lse and the row's loss from the groups' maxima and sums, then G from the codes.  Rows of G
 // past n are zeros.
 __global__ __launch_bounds__(256) void xent_rows_kernel(RowArgs p) {
   __shared__ float area[2][4];
-  const int64_t row = blockIdx.x;
+  const int64_t row = block_index();
   if (row >= p.n) {
+    if (row >= p.g_rows) return;
     u32x4* const g = reinterpret_cast<u32x4*>(p.g + row * p.ldg);
     for (int c = 8 * static_cast<int>(threadIdx.x); c < p.ldg; c += 2048) g[c / 8] = u32x4{0u, 0u, 0u, 0u};
     return;
@@ -298,6 +300,7 @@ __global__ __launch_bounds__(256) void xent_rows_kernel(RowArgs p) {
   const auto to_gradient = [&](int c, u32x4 two) {
     if (c >= p.ldg) return;
     if (counts) {
+      const bool none = !(lse > -INFINITY);  // a NaN in the row, or nothing above -inf: NaN in all of its gradient
       const float below = st[p.group0 + (c < p.cols ? c : p.cols - 1) / p.group_cols].x - lse;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -307,7 +310,7 @@ __global__ __launch_bounds__(256) void xent_rows_kernel(RowArgs p) {
           const uint32_t u = h ? two[k] >> 16 : two[k] & 0xFFFFu;
           const int col = c + 2 * k + h;
           v[h] = u != kCodeZero ? __builtin_amdgcn_exp2f(__builtin_fmaf(static_cast<float>(u), -kCodeOctaves / 65535.0f, below)) : 0.0f;
-          if (!(lse == lse)) v[h] = lse;  // NaN in the row: in all of its gradient
+          if (none) v[h] = NAN;
           if (p.v0 + col == label) v[h] = __builtin_amdgcn_exp2f(zl - lse) - 1.0f;
           if (col >= p.cols) v[h] = 0.0f;
         }
@@ -449,35 +452,43 @@ __device__ __forceinline__ void mean_loss(const float* __restrict__ row_loss, in
 // Both gradients of a piece in one launch, dx's blocks first (they have the longer sums); loss, if not null:
 // one more block, which forms the mean loss.
 template <class Tx, class Tw, bool RING>
-__global__ __launch_bounds__(Tw::NT) void xent_grads_any(GradArgs dx, GradArgs dw, int dx_blocks, int dw_blocks,
+__global__ __launch_bounds__(Tw::NT) void xent_grads_any(GradArgs dx, GradArgs dw, int64_t dx_blocks, int64_t dw_blocks,
                                                             const float* row_loss, float* loss) {
   using ForDx = typename Tx::template Loop<RING, true, false>;
   static_assert(Tx::NT == Tw::NT, "one launch");
   using ForDw = typename Tw::template Loop<RING, true, true>;
   __shared__ __attribute__((aligned(1024))) char smem[ForDx::LDS_BYTES > ForDw::LDS_BYTES ? ForDx::LDS_BYTES : ForDw::LDS_BYTES];
-  const int block = static_cast<int>(blockIdx.x);
-  if (block < dx_blocks) grad_tile<ForDx>(dx, block, smem);
-  else if (block < dx_blocks + dw_blocks) grad_tile<ForDw>(dw, block - dx_blocks, smem);
-  else mean_loss(row_loss, dx.n, dx.inv, loss, smem);
+  const int64_t block = block_index();
+  if (block < dx_blocks) grad_tile<ForDx>(dx, static_cast<int>(block), smem);
+  else if (block < dx_blocks + dw_blocks) grad_tile<ForDw>(dw, static_cast<int>(block - dx_blocks), smem);
+  else if (loss && block == dx_blocks + dw_blocks) mean_loss(row_loss, dx.n, dx.inv, loss, smem);
 }
 
-// out = inv times the sum of the splits, four elements a lane.
-__global__ __launch_bounds__(64) void xent_join_kernel(const float* __restrict__ sum, int splits, int64_t n, const float* __restrict__ inv,
-                                                        void* __restrict__ out, int out_dt) {
-  const int64_t e = (static_cast<int64_t>(blockIdx.x) * 64 + threadIdx.x) * 4;
-  if (e >= n) return;
+// out = inv times the sum of the splits, four elements a lane, of one or two gradients.
+struct Join {
+  const float* sum;
+  int splits, out_dt;
+  int64_t n;  // elements, 0: nothing to do
+  void* out;
+};
+__global__ __launch_bounds__(64) void xent_join_kernel(Join dx, Join dw, int64_t dx_blocks, const float* __restrict__ inv) {
+  int64_t block = block_index();
+  const Join p = block < dx_blocks ? dx : dw;
+  if (block >= dx_blocks) block -= dx_blocks;
+  const int64_t e = (block * 64 + threadIdx.x) * 4;
+  if (e >= p.n) return;
   float s[4] = {};
 #pragma unroll 8
-  for (int k = 0; k < splits; ++k) {
+  for (int k = 0; k < p.splits; ++k) {
     float v[4];
-    load_some(VDSL_F32, sum, k * n + e, n - e, v);
+    load_some(VDSL_F32, p.sum, k * p.n + e, p.n - e, v);
 #pragma unroll
     for (int j = 0; j < 4; ++j) s[j] += v[j];
   }
   const float f = inv[0];
 #pragma unroll
   for (int j = 0; j < 4; ++j) s[j] *= f;
-  store_some(out_dt, out, e, n - e, s);
+  store_some(p.out_dt, p.out, e, p.n - e, s);
 }
 
 // The gradients' products on tiles of gemm_wide.h: out[n][m] from A(m, k) and B(n, k), so that a lane has
@@ -487,8 +498,9 @@ struct WideGradArgs {
   int m, n, k;         // m, n: of out
   int n_alloc;         // of B, where it is K-major: columns that are allocated
   int64_t lda, ldb;
-  float* sum;          // [n][m] f32, the pieces' sum
-  bool first, last;    // of the pieces: sum holds nothing yet; the result is whole
+  float* sum;          // [splits][n][m] f32, the pieces' sum
+  bool first, last;    // of the pieces: sum holds nothing yet; the result is whole (never with splits)
+  int splits;          // of k, blockIdx.y's
   const float* inv;
   void* out;
   int out_dt;
@@ -500,7 +512,13 @@ __global__ __launch_bounds__(WideCfg::NT, 1) void xent_grad_wide(WideGradArgs p)
   __shared__ __attribute__((aligned(1024))) char smem[WideCfg::LDS_BYTES];
   const int half = (threadIdx.x & 63) >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const float inv = p.inv[0];
-  wide_gemm<true, BKM>(p.a, p.b, p.m, BKM ? p.n_alloc : p.n, p.k, p.lda, p.ldb, BKM, smem, [&](const f32x16 (&acc)[4][4], int m0, int n0) {
+  const int64_t stages = (p.k + 63) / 64;
+  const int kb = 64 * static_cast<int>(stages * blockIdx.y / p.splits);
+  const int ke = min(p.k, 64 * static_cast<int>(stages * (blockIdx.y + 1) / p.splits));
+  const uint16_t *const a = p.a + kb * p.lda, *const b = p.b + (BKM ? kb * p.ldb : kb);
+  float* const sum = p.sum + static_cast<int64_t>(blockIdx.y) * p.n * p.m;
+  const int cols = BKM ? p.n_alloc : p.n;
+  wide_gemm<true, BKM>(a, b, p.m, cols, ke - kb, p.lda, p.ldb, BKM, smem, [&](const f32x16 (&acc)[4][4], int m0, int n0) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int row = n0 + 128 * (wave & 1) + 32 * j + static_cast<int>(threadIdx.x & 31);
@@ -528,9 +546,9 @@ __global__ __launch_bounds__(WideCfg::NT, 1) void xent_grad_wide(WideGradArgs p)
             const int c = 32 * i + 8 * q + 4 * half;
             if (row >= p.n || c0 + c >= p.m) continue;
             f32x4 s = {v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
-            if (!p.first) s += *reinterpret_cast<const f32x4*>(p.sum + out + c);
+            if (!p.first) s += *reinterpret_cast<const f32x4*>(sum + out + c);
             if (!p.last)
-              *reinterpret_cast<f32x4*>(p.sum + out + c) = s;
+              *reinterpret_cast<f32x4*>(sum + out + c) = s;
             else if (p.out_dt == VDSL_F32)
               *reinterpret_cast<f32x4*>(static_cast<float*>(p.out) + out + c) = s * inv;
             else
@@ -576,10 +594,26 @@ struct Plan {
   Tiling logits = kTiles64, again = kTiles64, grads = kTiles64, dx = kTiles64;
   int64_t group_cols = 0, groups = 0;
   int64_t g_rows = 0, ldg = 0;    // of G; its rows past n are zeros
-  int splits = 1;                 // of the sums over a piece's columns for dx
-  bool sum = false;               // whether dx is formed by way of f32 sums
-  size_t at_stats = 0, at_zlabel = 0, at_lse = 0, at_row_loss = 0, at_inv = 0, at_g = 0, at_sum = 0, bytes = 0;
+  int splits = 1, dw_splits = 1;  // of the sums over a piece's columns for dx, over the rows for dw
+  bool sum = false;               // whether dx is formed by way of f32 sums (dw: where it has splits)
+  size_t at_stats = 0, at_zlabel = 0, at_lse = 0, at_row_loss = 0, at_inv = 0, at_g = 0, at_sum = 0, at_dw_sum = 0, bytes = 0;
 };
+
+// The splits of the k of an m x n product on 256 x 256 tiles: as many as make its time least, rounds of a block on
+// each CU times their stages (1.6 us each) and what writing and adding the f32 sums takes (at 5 TB/s, and a launch).
+int wide_splits(int64_t n, int64_t m, int64_t k) {
+  const int64_t tiles = ceil_div(n, 256) * ceil_div(m, 256), stages = ceil_div(k, 64);
+  int best = 1;
+  double least = 0.0;
+  for (int s = 1; s <= 16 && stages >= 4 * s; ++s) {
+    const double us = 1.6 * static_cast<double>(ceil_div(tiles * s, 256) * ceil_div(stages, s)) +
+                      (s > 1 ? 6.0 + static_cast<double>(n) * static_cast<double>(m) * 8.0 * s / 5e6 : 0.0);
+    if (s > 1 && us >= least) continue;
+    best = s;
+    least = us;
+  }
+  return best;
+}
 
 constexpr int64_t kPieceBytes = int64_t{1} << 30;  // of codes, where the caller leaves the piece to the library
 
@@ -589,6 +623,7 @@ int make_plan(int64_t n, int64_t vocab, int64_t dim, int64_t piece, bool backwar
   if (dim < 8) return fail(VDSL_ERR_UNSUPPORTED, "linear_xent: dim must be at least 8");
   if (n > 0x7fffff00 || vocab > 0x7fffff00 || dim > 0x3fffff00) return fail(VDSL_ERR_UNSUPPORTED, "linear_xent: extents too large");
   if (!backward) piece = vocab;
+  else if (piece > vocab) piece = vocab;
   else if (piece == 0) piece = std::max<int64_t>(256, kPieceBytes / 2 / std::max<int64_t>(n, 1));
   p.pieces = ceil_div(vocab, std::min(vocab, ceil_div(piece, 256) * 256));
   p.piece = p.pieces == 1 ? vocab : ceil_div(ceil_div(vocab, p.pieces), 256) * 256;
@@ -604,15 +639,18 @@ int make_plan(int64_t n, int64_t vocab, int64_t dim, int64_t piece, bool backwar
   const int64_t unit = wide ? 256 : 8;
   p.ldg = ceil_div(p.piece, unit) * unit;
   p.g_rows = wide ? ceil_div(n, 64) * 64 : n;
-  p.sum = p.pieces > 1;
-  if (!wide) {
-    // dx has few tiles and long sums: splits of about as many stages as dw's sums have, four at least, up to two
-    // blocks a CU, and few enough to be added in two rounds of loads
-    const int64_t tiles = std::max<int64_t>(1, ceil_div(dim, rows_of(p.dx)) * ceil_div(n, cols_of(p.dx)));
-    const int64_t stages = ceil_div(p.piece, 64), like_dw = ceil_div(stages, std::max<int64_t>(4, ceil_div(n, 64)));
-    p.splits = static_cast<int>(std::max<int64_t>(1, std::min(std::min(512 / tiles, like_dw), int64_t{16})));
-    p.sum = p.sum || p.splits > 1;
+  if (wide) {
+    p.splits = wide_splits(n, dim, p.piece);
+    p.dw_splits = wide_splits(p.piece, dim, n);
+  } else {
+    // One launch: splits of about as many stages as two blocks a CU come to, five at least.
+    const auto tiles = [&](Tiling t, int64_t rows) { return ceil_div(dim, rows_of(t)) * ceil_div(rows, cols_of(t)); };
+    const int64_t x_stages = ceil_div(p.piece, 64), w_stages = ceil_div(n, 64);
+    const int64_t share = std::max<int64_t>(5, ceil_div(tiles(p.dx, n) * x_stages + tiles(p.grads, p.piece) * w_stages, 512));
+    p.splits = static_cast<int>(std::clamp<int64_t>(ceil_div(x_stages, share), 1, 64));
+    p.dw_splits = static_cast<int>(std::clamp<int64_t>(ceil_div(w_stages, share), 1, 64));
   }
+  p.sum = p.pieces > 1 || p.splits > 1;
   size_t at = 0;
   bool fits = true;
   const auto take = [&](int64_t a, int64_t b, int64_t c) {
@@ -629,6 +667,7 @@ int make_plan(int64_t n, int64_t vocab, int64_t dim, int64_t piece, bool backwar
   if (backward) {
     p.at_g = take(p.g_rows, p.ldg, 2);
     if (p.sum) p.at_sum = take(n, dim, 4 * p.splits);
+    if (p.dw_splits > 1) p.at_dw_sum = take(p.piece, dim, 4 * p.dw_splits);
   }
   p.bytes = at;
   return fits ? VDSL_OK : fail(VDSL_ERR_SHAPE, "linear_xent: the workspace's size overflows");
@@ -638,7 +677,7 @@ template <class Cfg, int MODE>
 int launch_logits_on(const LogitArgs& a, float grad_scale, float* inv, hipStream_t s) {
   const int64_t tiles = ceil_div(a.cols, Cfg::BM) * ceil_div(a.n, Cfg::BN);
   if (tiles >= 0x7fffffff) return fail(VDSL_ERR_UNSUPPORTED, "linear_xent: too many tiles");
-  hipLaunchKernelGGL((xent_logits_any<Cfg, MODE>), dim3(static_cast<unsigned>(tiles + 1)), dim3(Cfg::NT), 0, s, a, grad_scale, inv);
+  hipLaunchKernelGGL((xent_logits_any<Cfg, MODE>), block_grid(tiles + 1), dim3(Cfg::NT), 0, s, a, grad_scale, inv);
   return check_launch("xent_logits_any");
 }
 template <class T, int MODE>
@@ -662,10 +701,9 @@ int launch_logits(const LogitArgs& a, Tiling tiling, float grad_scale, float* in
 
 template <class Tx, class Tw>
 int launch_grads_on(const GradArgs& dx, const GradArgs& dw, const float* row_loss, float* loss, hipStream_t s) {
-  const int64_t bx = Tx::tiles(dx.m, dx.n) * dx.splits, bw = Tw::tiles(dw.m, dw.n);
-  if (bx + bw >= 0x7fffffff) return fail(VDSL_ERR_UNSUPPORTED, "linear_xent: too many tiles");
-  const dim3 grid(static_cast<unsigned>(bx + bw + (loss ? 1 : 0)));
-  const int x = static_cast<int>(bx), w = static_cast<int>(bw);
+  const int64_t x = Tx::tiles(dx.m, dx.n) * dx.splits, w = Tw::tiles(dw.m, dw.n) * dw.splits;
+  if (x > 0x7fffffff || w > 0x7fffffff) return fail(VDSL_ERR_UNSUPPORTED, "linear_xent: too many tiles");
+  const dim3 grid = block_grid(x + w + (loss ? 1 : 0));
   if (ring_runs(dx.m)) hipLaunchKernelGGL((xent_grads_any<Tx, Tw, true>), grid, dim3(Tw::NT), 0, s, dx, dw, x, w, row_loss, loss);
   else hipLaunchKernelGGL((xent_grads_any<Tx, Tw, false>), grid, dim3(Tw::NT), 0, s, dx, dw, x, w, row_loss, loss);
   return check_launch("xent_grads_any");
@@ -678,11 +716,11 @@ int launch_grads_any(const GradArgs& dx, const GradArgs& dw, Tiling dx_tiling, c
 
 template <bool BKM>
 int launch_grad_wide(const WideGradArgs& a, int64_t n, hipStream_t s) {
-  const unsigned blocks = wide_blocks(ceil_div(a.m, 256) * ceil_div(n, 256));
+  const dim3 grid(wide_blocks(ceil_div(a.m, 256) * ceil_div(n, 256)), static_cast<unsigned>(a.splits));
   if (a.first && a.last && a.out_dt == VDSL_BF16)
-    hipLaunchKernelGGL((xent_grad_wide<BKM, true>), dim3(blocks), dim3(WideCfg::NT), 0, s, a);
+    hipLaunchKernelGGL((xent_grad_wide<BKM, true>), grid, dim3(WideCfg::NT), 0, s, a);
   else
-    hipLaunchKernelGGL((xent_grad_wide<BKM, false>), dim3(blocks), dim3(WideCfg::NT), 0, s, a);
+    hipLaunchKernelGGL((xent_grad_wide<BKM, false>), grid, dim3(WideCfg::NT), 0, s, a);
   return check_launch("xent_grad_wide");
 }
 
@@ -750,7 +788,8 @@ int run_xent(vdsl_queue q, int64_t n, int64_t dim, int64_t vocab, vdsl_buffer x,
     ra.groups = la.groups;
     ra.group_cols = static_cast<int>(plan.group_cols);
     ra.ldg = plan.ldg;
-    hipLaunchKernelGGL(xent_rows_kernel, dim3(static_cast<unsigned>(backward ? plan.g_rows : n)), dim3(256), 0, s, ra);
+    ra.g_rows = backward ? plan.g_rows : n;
+    hipLaunchKernelGGL(xent_rows_kernel, block_grid(ra.g_rows), dim3(256), 0, s, ra);
     VDSL_TRY(check_launch("xent_rows_kernel"));
   }
   if (!backward || n == 0 || plan.grads == kTilesWide) {
@@ -764,6 +803,7 @@ int run_xent(vdsl_queue q, int64_t n, int64_t dim, int64_t vocab, vdsl_buffer x,
     return check_launch("xent_zero_kernel");
   }
   float* const sum = plan.sum ? reinterpret_cast<float*>(ws + plan.at_sum) : nullptr;
+  float* const dw_sum = plan.dw_splits > 1 ? reinterpret_cast<float*>(ws + plan.at_dw_sum) : nullptr;
   la.g0 = 0;
   // The piece whose codes are held comes first, then those whose logits are formed again.
   for (int64_t t = 0; t < plan.pieces; ++t) {
@@ -771,29 +811,34 @@ int run_xent(vdsl_queue q, int64_t n, int64_t dim, int64_t vocab, vdsl_buffer x,
     la.w = static_cast<const uint16_t*>(w->ptr) + v0 * dim;
     la.v0 = static_cast<int>(v0);
     la.cols = static_cast<int>(std::min(plan.piece, vocab - v0));
+    const bool last = t == plan.pieces - 1;
     if (t > 0) VDSL_TRY(launch_logits<kLogitGrad>(la, plan.again, grad_scale, inv, s));
     void* const dw_piece = static_cast<char*>(dw->ptr) + v0 * dim * static_cast<int64_t>(dtype_size(dw_dtype));
     if (plan.grads == kTilesWide) {
-      const WideGradArgs for_dx{la.w, g,      la.dim, la.n,   la.cols, 0, dim, plan.ldg, sum, t == 0, t == plan.pieces - 1,
-                                inv,  dx->ptr, dx_dtype};
+      const WideGradArgs for_dx{la.w, g,      la.dim, la.n,   la.cols, 0, dim, plan.ldg, sum, t == 0, last && plan.splits == 1,
+                                plan.splits, inv, dx->ptr, dx_dtype};
       VDSL_TRY(launch_grad_wide<false>(for_dx, n, s));
-      const WideGradArgs for_dw{la.x, g,        la.dim, la.cols, la.n, static_cast<int>(plan.ldg), dim, plan.ldg, nullptr, true, true,
-                                inv,  dw_piece, dw_dtype};
+      const WideGradArgs for_dw{la.x, g,        la.dim, la.cols, la.n, static_cast<int>(plan.ldg), dim, plan.ldg, dw_sum, true, !dw_sum,
+                                plan.dw_splits, inv, dw_piece, dw_dtype};
       VDSL_TRY(launch_grad_wide<true>(for_dw, plan.ldg, s));
-      continue;
+    } else {
+      const GradArgs for_dx{la.w, g, la.dim, la.n, la.cols, dim, plan.ldg, sum, t == 0, plan.splits, inv, dx->ptr, dx_dtype};
+      const GradArgs for_dw{la.x, g, la.dim, la.cols, la.n, dim, plan.ldg, dw_sum, true, plan.dw_splits, inv, dw_piece, dw_dtype};
+      float* const mean = t == 0 ? loss_out : nullptr;
+      if (plan.grads == kTiles128) VDSL_TRY(launch_grads_any<Tile128>(for_dx, for_dw, plan.dx, each, mean, s));
+      else if (plan.grads == kTiles128x64) VDSL_TRY(launch_grads_any<Tile128x64>(for_dx, for_dw, plan.dx, each, mean, s));
+      else VDSL_TRY(launch_grads_any<Tile64>(for_dx, for_dw, plan.dx, each, mean, s));
     }
-    const GradArgs for_dx{la.w, g, la.dim, la.n, la.cols, dim, plan.ldg, sum, t == 0, plan.splits, inv, dx->ptr, dx_dtype};
-    const GradArgs for_dw{la.x, g, la.dim, la.cols, la.n, dim, plan.ldg, nullptr, true, 1, inv, dw_piece, dw_dtype};
-    float* const mean = t == 0 ? loss_out : nullptr;
-    if (plan.grads == kTiles128) VDSL_TRY(launch_grads_any<Tile128>(for_dx, for_dw, plan.dx, each, mean, s));
-    else if (plan.grads == kTiles128x64) VDSL_TRY(launch_grads_any<Tile128x64>(for_dx, for_dw, plan.dx, each, mean, s));
-    else VDSL_TRY(launch_grads_any<Tile64>(for_dx, for_dw, plan.dx, each, mean, s));
+    // a wide dx without splits is whole with its last piece
+    const bool join_dx = last && sum && (plan.grads != kTilesWide || plan.splits > 1);
+    if (!join_dx && !dw_sum) continue;
+    const Join for_x{sum, plan.splits, dx_dtype, join_dx ? n * dim : 0, dx->ptr};
+    const Join for_w{dw_sum, plan.dw_splits, dw_dtype, dw_sum ? la.cols * dim : 0, dw_piece};
+    const int64_t x_blocks = ceil_div(for_x.n, 256);
+    hipLaunchKernelGGL(xent_join_kernel, block_grid(x_blocks + ceil_div(for_w.n, 256)), dim3(64), 0, s, for_x, for_w, x_blocks, inv);
+    VDSL_TRY(check_launch("xent_join_kernel"));
   }
-  if (plan.grads == kTilesWide || !sum) return VDSL_OK;
-  const int64_t blocks = ceil_div(n * dim, 256);
-  if (blocks > 0x7fffffff) return fail(VDSL_ERR_UNSUPPORTED, "linear_xent: dx too large");
-  hipLaunchKernelGGL(xent_join_kernel, dim3(static_cast<unsigned>(blocks)), dim3(64), 0, s, sum, plan.splits, n * dim, inv, dx->ptr, dx_dtype);
-  return check_launch("xent_join_kernel");
+  return VDSL_OK;
 }
 
 }  // namespace

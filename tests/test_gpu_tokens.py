@@ -484,6 +484,14 @@ def test_linear_xent_piece_of_any_size(q, own):
             assert np.array_equal(a, b)
 
 
+# gradients on 256 x 256 tiles, in splits: smaller tiles for the logits; f32; pieces; ragged rows and columns
+@pytest.mark.parametrize("n,dim,vocab,piece,gt", [(500, 1600, 16500, 0, "bf16"), (2048, 1152, 6144, 0, "f32"), (2305, 1024, 11000, 5632, "bf16"),
+                                                  (1100, 2112, 5701, 0, "bf16"), (2100, 1001, 6300, 0, "bf16"), (2100, 1003, 6300, 0, "f32"),
+                                                  (2100, 1000, 6300, 3328, "bf16")])
+def test_linear_xent_gradients_on_256_tiles(q, own, n, dim, vocab, piece, gt):
+    check_xent(q, own, *xent_input(np.random.default_rng(n), n, dim, vocab), piece=piece, gt=gt)
+
+
 # long sums for the weights' gradient in few tiles
 @pytest.mark.parametrize("n,dim,vocab,piece", [(2000, 72, 300, 0), (1500, 71, 130, 0), (1100, 64, 700, 256)])
 def test_linear_xent_many_rows_few_logits(q, own, n, dim, vocab, piece):

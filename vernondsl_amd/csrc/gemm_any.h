@@ -50,22 +50,21 @@ struct AnyOperand {
   int k_of[C];         // the chunk's first K value within a stage
   int lds[C];
 
-  // ld: elements from one stored row to the next; the tensor is allocated in whole stored rows.
-  __device__ __forceinline__ AnyOperand(const uint16_t* p, int rows, int K, int r0, int64_t ld) {
+  __device__ __forceinline__ AnyOperand(const uint16_t* p, int rows, int K, int r0) {
     base = reinterpret_cast<const char*>(p);
-    size = (KM ? K : rows) * ld;
+    size = static_cast<int64_t>(rows) * K;
     last = size - 8;
-    kstep = KM ? ld : 1;
+    kstep = KM ? rows : 1;
 #pragma unroll
     for (int i = 0; i < C; ++i) {
       const int c = static_cast<int>(threadIdx.x) + NT * i, row = c / CPR, chunk = c % CPR;
       lds[i] = row * LDS_ROW + chunk * 16;
       if constexpr (KM) {
         k_of[i] = row;
-        at[i] = row * ld + (r0 + 8 * chunk < rows ? r0 + 8 * chunk : 0);
+        at[i] = static_cast<int64_t>(row) * rows + (r0 + 8 * chunk < rows ? r0 + 8 * chunk : 0);
       } else {
         k_of[i] = 8 * chunk;
-        at[i] = (r0 + row < rows ? r0 + row : rows - 1) * ld + 8 * chunk;
+        at[i] = static_cast<int64_t>(r0 + row < rows ? r0 + row : rows - 1) * K + 8 * chunk;
       }
     }
   }
@@ -110,16 +109,14 @@ __device__ __forceinline__ bf16x8 any_fragment(const char* area, int row0, int f
   }
 }
 
-// lda, ldb: elements between stored rows (negative: dense).
 template <class Cfg>
 __device__ __forceinline__ void any_mainloop(const uint16_t* __restrict__ A, const uint16_t* __restrict__ B, int M, int N, int K,
-                                             int m0, int n0, char* smem, f32x16 (&acc)[Cfg::FM][Cfg::FN], int64_t lda = -1,
-                                             int64_t ldb = -1) {
+                                             int m0, int n0, char* smem, f32x16 (&acc)[Cfg::FM][Cfg::FN]) {
   constexpr int FM = Cfg::FM, FN = Cfg::FN;
   const int wave = threadIdx.x >> 6;
   const int wr = (wave / Cfg::WGN) * Cfg::WTM, wc = (wave % Cfg::WGN) * Cfg::WTN;
-  const AnyOperand<Cfg::AKM, Cfg::BM, Cfg::NT, Cfg::CA, Cfg::A_ROW> a(A, M, K, m0, lda < 0 ? (Cfg::AKM ? M : K) : lda);
-  const AnyOperand<Cfg::BKM, Cfg::BN, Cfg::NT, Cfg::CB, Cfg::B_ROW> b(B, N, K, n0, ldb < 0 ? (Cfg::BKM ? N : K) : ldb);
+  const AnyOperand<Cfg::AKM, Cfg::BM, Cfg::NT, Cfg::CA, Cfg::A_ROW> a(A, M, K, m0);
+  const AnyOperand<Cfg::BKM, Cfg::BN, Cfg::NT, Cfg::CB, Cfg::B_ROW> b(B, N, K, n0);
 #pragma unroll
   for (int i = 0; i < FM; ++i)
 #pragma unroll
@@ -169,63 +166,6 @@ __device__ __forceinline__ void any_mainloop(const uint16_t* __restrict__ A, con
   }
   if (kt < nk) VDSL_ANY_STEP(kt, 0, ra0, rb0, ra1, rb1);
 #undef VDSL_ANY_STEP
-}
-
-// The same for K values [kb, ke) of K, kb a multiple of 64, ke one or K.
-template <class Cfg>
-__device__ __forceinline__ void any_mainloop_range(const uint16_t* __restrict__ A, const uint16_t* __restrict__ B, int M, int N, int K,
-                                                   int kb, int ke, int m0, int n0, char* smem, f32x16 (&acc)[Cfg::FM][Cfg::FN],
-                                                   int64_t lda, int64_t ldb) {
-  constexpr int FM = Cfg::FM, FN = Cfg::FN, D = 4;  // stages whose loads are in flight
-  const int wave = threadIdx.x >> 6;
-  const int wr = (wave / Cfg::WGN) * Cfg::WTM, wc = (wave % Cfg::WGN) * Cfg::WTN;
-  const AnyOperand<Cfg::AKM, Cfg::BM, Cfg::NT, Cfg::CA, Cfg::A_ROW> a(A, M, K, m0, lda);
-  const AnyOperand<Cfg::BKM, Cfg::BN, Cfg::NT, Cfg::CB, Cfg::B_ROW> b(B, N, K, n0, ldb);
-#pragma unroll
-  for (int i = 0; i < FM; ++i)
-#pragma unroll
-    for (int j = 0; j < FN; ++j) acc[i][j] = MfmaBf16::zero();
-  u32x4 ra[D][Cfg::CA], rb[D][Cfg::CB];
-  const int nk = (ke - kb + Cfg::BK - 1) / Cfg::BK, k_last = kb + (nk - 1) * Cfg::BK;
-#pragma unroll
-  for (int s = 0; s < D; ++s) {
-    const int k = min(kb + s * Cfg::BK, k_last);
-    a.load(ra[s], k);
-    b.load(rb[s], k);
-  }
-  a.store(ra[0], kb, ke, smem);
-  b.store(rb[0], kb, ke, smem + Cfg::A_BYTES);
-  __syncthreads();
-  for (int kt = 0; kt < nk; kt += D) {
-#pragma unroll
-    for (int s = 0; s < D; ++s) {
-      if (kt + s < nk) {  // block-uniform
-        // set s is in LDS: it takes the stage D further on, while the stage in LDS is computed from
-        const int kl = min(kb + (kt + s + D) * Cfg::BK, k_last), ks = min(kb + (kt + s + 1) * Cfg::BK, k_last);
-        a.load(ra[s], kl);
-        b.load(rb[s], kl);
-        __builtin_amdgcn_sched_barrier(0);
-        const char* const stage = smem + (s & 1) * Cfg::STAGE;
-#pragma unroll
-        for (int kk = 0; kk < Cfg::BK / 16; ++kk) {
-          bf16x8 fa[FM], fb[FN];
-#pragma unroll
-          for (int i = 0; i < FM; ++i) fa[i] = any_fragment<Cfg::AKM, Cfg::A_ROW>(stage, wr, i, kk);
-#pragma unroll
-          for (int j = 0; j < FN; ++j) fb[j] = any_fragment<Cfg::BKM, Cfg::B_ROW>(stage + Cfg::A_BYTES, wc, j, kk);
-#pragma unroll
-          for (int i = 0; i < FM; ++i)
-#pragma unroll
-            for (int j = 0; j < FN; ++j) acc[i][j] = MfmaBf16::mma(fa[i], fb[j], acc[i][j]);
-        }
-        char* const to = smem + ((s & 1) ^ 1) * Cfg::STAGE;
-        a.store(ra[(s + 1) % D], ks, ke, to);
-        b.store(rb[(s + 1) % D], ks, ke, to + Cfg::A_BYTES);
-        __syncthreads();
-        __builtin_amdgcn_sched_barrier(0);
-      }
-    }
-  }
 }
 
 }  // namespace vdsl

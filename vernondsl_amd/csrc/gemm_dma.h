@@ -104,7 +104,6 @@ VDSL_DMA_WAIT_CASE(4)
 VDSL_DMA_WAIT_CASE(6)
 VDSL_DMA_WAIT_CASE(8)
 VDSL_DMA_WAIT_CASE(9)
-VDSL_DMA_WAIT_CASE(10)
 VDSL_DMA_WAIT_CASE(12)
 VDSL_DMA_WAIT_CASE(16)
 VDSL_DMA_WAIT_CASE(18)

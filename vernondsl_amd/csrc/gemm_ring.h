@@ -70,11 +70,11 @@ struct RingOperand {
     char* const to = area + wave * C * 1024;
     if (left >= 64) {
 #pragma unroll
-      for (int u = 0; u < C; ++u) __builtin_amdgcn_global_load_lds(from + off[u], (lds_void_t*)(to + u * 1024), 16, 0, 0);
+      for (int u = 0; u < C; ++u) lds_copy16(from + off[u], to + u * 1024);
     } else {
 #pragma unroll
       for (int u = 0; u < C; ++u) {
-        if (k_of[u] < left) __builtin_amdgcn_global_load_lds(from + off[u], (lds_void_t*)(to + u * 1024), 16, 0, 0);
+        if (k_of[u] < left) lds_copy16(from + off[u], to + u * 1024);
         else *reinterpret_cast<u32x4*>(to + u * 1024 + 16 * lane) = u32x4{0u, 0u, 0u, 0u};
       }
     }

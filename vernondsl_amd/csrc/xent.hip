@@ -20,7 +20,6 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "gemm_any.h"
 #include "gemm_ring.h"
 #include "gemm_wide.h"
 #include "rowunit.h"
@@ -178,41 +177,20 @@ __device__ __forceinline__ void count_rows(const int32_t* __restrict__ labels, i
   inv[1] = __int_as_float(k > 0 ? k : 1);
 }
 
-// The main loops of the smaller tiles: gemm_ring.h's where rows are whole 16-byte units (dim % 8 == 0), else
-// gemm_any.h's.  Stages in the ring: as many as leave two blocks a CU (one of 128 x 128).
-template <int BM, int BN, int WGM, int WGN, int NS, bool AKM, bool BKM>
-struct RingLoop : RingConfig<BM, BN, WGM, WGN, NS, AKM, BKM> {
-  using Cfg = RingConfig<BM, BN, WGM, WGN, NS, AKM, BKM>;
-  __device__ static __forceinline__ void run(const uint16_t* a, const uint16_t* b, int m, int n, int, int kb, int ke, int m0, int n0,
-                                             char* smem, f32x16 (&acc)[Cfg::FM][Cfg::FN], int64_t lda, int64_t ldb) {
-    ring_mainloop<Cfg>(a, b, m, n, kb, ke, m0, n0, smem, acc, lda, ldb);
-  }
-};
-template <int BM, int BN, int WGM, int WGN, bool AKM, bool BKM>
-struct AnyLoop : AnyConfig<BM, BN, WGM, WGN, AKM, BKM> {
-  using Cfg = AnyConfig<BM, BN, WGM, WGN, AKM, BKM>;
-  __device__ static __forceinline__ void run(const uint16_t* a, const uint16_t* b, int m, int n, int k, int kb, int ke, int m0, int n0,
-                                             char* smem, f32x16 (&acc)[Cfg::FM][Cfg::FN], int64_t lda, int64_t ldb) {
-    any_mainloop_range<Cfg>(a, b, m, n, k, kb, ke, m0, n0, smem, acc, lda, ldb);
-  }
-};
-template <int BM_, int BN_, int WGM_, int WGN_, int NS>
+// The smaller tiles, of gemm_ring.h.  Stages in the ring: as many as leave two blocks a CU.
+template <int BM_, int BN_, int NS>
 struct Tile {
-  static constexpr int BM = BM_, BN = BN_, WGM = WGM_, WGN = WGN_, NT = 64 * WGM_ * WGN_;
-  template <bool RING, bool AKM, bool BKM>
-  using Loop = std::conditional_t<RING, RingLoop<BM_, BN_, WGM_, WGN_, NS, AKM, BKM>, AnyLoop<BM_, BN_, WGM_, WGN_, AKM, BKM>>;
-  __host__ __device__ static int64_t tiles(int64_t m, int64_t n) { return ((m + BM - 1) / BM) * ((n + BN - 1) / BN); }
+  static constexpr int BM = BM_, BN = BN_, NT = 256;
+  template <bool AKM, bool BKM>
+  using Loop = RingConfig<BM_, BN_, 2, 2, NS, AKM, BKM>;
+  static int64_t tiles(int64_t m, int64_t n) { return ((m + BM - 1) / BM) * ((n + BN - 1) / BN); }
 };
-using Tile64x32 = Tile<64, 32, 2, 1, 6>;    // the logits of up to 32 rows
-using Tile128x32 = Tile<128, 32, 4, 1, 4>;  // their dx
-using Tile64 = Tile<64, 64, 2, 2, 5>;
-using Tile128x64 = Tile<128, 64, 2, 2, 3>;
-using Tile128 = Tile<128, 128, 2, 2, 5>;
+using Tile64 = Tile<64, 64, 5>;
+using Tile128x64 = Tile<128, 64, 3>;
 
-// Products of few tiles, of rows that are no whole stages, or of odd lengths.  The launch has a block more than
-// tiles: the last one counts the rows.
+// The logits on smaller tiles.  The launch has a block more than tiles: the last one counts the rows.
 template <class Cfg, int MODE>
-__global__ __launch_bounds__(Cfg::NT) void xent_logits_any(LogitArgs p, float grad_scale, float* inv) {
+__global__ __launch_bounds__(Cfg::NT) void xent_logits_small(LogitArgs p, float grad_scale, float* inv) {
   __shared__ __attribute__((aligned(1024))) char smem[Cfg::LDS_BYTES];
   const int tiles_m = (p.cols + Cfg::BM - 1) / Cfg::BM, tiles_n = (p.n + Cfg::BN - 1) / Cfg::BN, tiles = tiles_m * tiles_n;
   const int64_t block = block_index();
@@ -223,7 +201,7 @@ __global__ __launch_bounds__(Cfg::NT) void xent_logits_any(LogitArgs p, float gr
   int tm, tn;
   tile_coords(xcd_remap(static_cast<int>(block), tiles), tiles_m, tiles_n, tm, tn);
   f32x16 acc[Cfg::FM][Cfg::FN];
-  Cfg::run(p.w, p.x, p.cols, p.n, p.dim, 0, p.dim, tm * Cfg::BM, tn * Cfg::BN, smem, acc, p.dim, p.dim);
+  ring_mainloop<Cfg>(p.w, p.x, p.cols, p.n, 0, p.dim, tm * Cfg::BM, tn * Cfg::BN, smem, acc, p.dim, p.dim);
   const int wave = threadIdx.x >> 6;
   logits_tile<Cfg::FM, Cfg::FN, MODE>(p, tm * Cfg::BM + wave / Cfg::WGN * Cfg::WTM, tn * Cfg::BN + wave % Cfg::WGN * Cfg::WTN,
                                       [&](int i, int j, int r) { return acc[i][j][r]; });
@@ -240,6 +218,42 @@ __device__ __forceinline__ float block_max_256(float v, float* area) {
   if ((threadIdx.x & 63) == 0) area[threadIdx.x >> 6] = v;
   __syncthreads();
   return fmaxf(fmaxf(area[0], area[1]), fmaxf(area[2], area[3]));
+}
+
+// Rows of x and w of `dim` elements copied in rows of `ld` (a multiple of 8), zeros behind them; a wave per row.
+__global__ __launch_bounds__(256) void xent_layout_kernel(const uint16_t* __restrict__ x, int64_t n, const uint16_t* __restrict__ w,
+                                                          int64_t vocab, int64_t dim, uint16_t* __restrict__ x_out,
+                                                          uint16_t* __restrict__ w_out, int64_t ld) {
+  int64_t row = block_index() * 4 + (threadIdx.x >> 6);
+  if (row >= n + vocab) return;
+  const bool of_x = row < n;
+  if (!of_x) row -= n;
+  const uint16_t* const from = (of_x ? x : w) + row * dim;
+  uint16_t* const to = (of_x ? x_out : w_out) + row * ld;
+#pragma unroll 4
+  for (int64_t c = 8 * static_cast<int64_t>(threadIdx.x & 63); c < ld; c += 512) {
+    // whole units, the row's last moved back to its end (dim >= 8) and shifted into place
+    const UnitAt<8> at(c, dim);
+    u32x4 v = reinterpret_cast<const U32x4At2*>(from + at.c)->v;
+    if (at.skip) {
+      uint16_t e[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) e[j] = static_cast<uint16_t>(v[j / 2] >> (16 * (j & 1)));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t word = 0;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t pick = 0;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) pick = k == 2 * j + h + at.skip ? e[k] : pick;
+          word |= pick << (16 * h);
+        }
+        v[j] = word;
+      }
+    }
+    *reinterpret_cast<u32x4*>(to + c) = v;
+  }
 }
 
 struct RowArgs {
@@ -369,6 +383,17 @@ __global__ __launch_bounds__(256) void xent_zero_kernel(uint16_t* __restrict__ p
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256) p[i] = 0;
 }
 
+// Eight bf16 values, of which the first n (or all) are stored.
+__device__ __forceinline__ void store_eight(uint16_t* to, u32x4 v, int n) {
+  if (n >= 8) {
+    reinterpret_cast<U32x4At2*>(to)->v = v;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < n) to[j] = static_cast<uint16_t>(v[j / 2] >> (16 * (j & 1)));
+  }
+}
+
 // A gradient's product, transposed: out[n][m] = inv sum_k A(m, k) B(n, k), A K-major, so that a lane has
 // neighbouring elements of a row of out.  k may be split, and there may be pieces: then the products go to
 // sum, [split][n][m] in f32, and a last kernel adds the splits.
@@ -396,7 +421,7 @@ __device__ __forceinline__ void grad_tile(const GradArgs& p, int block, char* sm
   const int ke = min(p.k, 64 * static_cast<int>(static_cast<int64_t>(stages) * (split + 1) / p.splits));
   f32x16 acc[Cfg::FM][Cfg::FN];
   if (kb < ke) {  // block-uniform
-    Cfg::run(p.a, p.b, p.m, p.n, p.k, kb, ke, m0, n0, smem, acc, p.lda, p.ldb);
+    ring_mainloop<Cfg>(p.a, p.b, p.m, p.n, kb, ke, m0, n0, smem, acc, p.lda, p.ldb);
   } else {
 #pragma unroll
     for (int i = 0; i < Cfg::FM; ++i)
@@ -409,12 +434,28 @@ __device__ __forceinline__ void grad_tile(const GradArgs& p, int block, char* sm
 #pragma unroll
   for (int j = 0; j < Cfg::FN; ++j) {
     const int row = n0 + wave % Cfg::WGN * Cfg::WTN + 32 * j + static_cast<int>(threadIdx.x & 31);
+    const int col0 = m0 + wave / Cfg::WGN * Cfg::WTM;
+    if (!sum && p.out_dt == VDSL_BF16) {  // the lane of the other half has the row's next four
+      uint16_t* const out = static_cast<uint16_t*>(p.out) + static_cast<int64_t>(row) * p.m;
+#pragma unroll
+      for (int i = 0; i < Cfg::FM; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; q += 2) {
+          uint32_t word[4];
+#pragma unroll
+          for (int h = 0; h < 4; ++h) word[h] = pack_bf16x2(acc[i][j][4 * q + 2 * h] * inv, acc[i][j][4 * q + 2 * h + 1] * inv);
+          const u32x4 eight = wide_exchange(word[0], word[1], word[2], word[3]);
+          const int col = col0 + 32 * i + 8 * (q + half);
+          if (row < p.n && col < p.m) store_eight(out + col, eight, p.m - col);
+        }
+      continue;
+    }
     if (row >= p.n) continue;
 #pragma unroll
     for (int i = 0; i < Cfg::FM; ++i)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const int col = m0 + wave / Cfg::WGN * Cfg::WTM + 32 * i + 8 * q + 4 * half;
+        const int col = col0 + 32 * i + 8 * q + 4 * half;
         const int64_t o = static_cast<int64_t>(row) * p.m + col;
         float v[4] = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
         if (sum) {
@@ -451,12 +492,11 @@ __device__ __forceinline__ void mean_loss(const float* __restrict__ row_loss, in
 
 // Both gradients of a piece in one launch, dx's blocks first (they have the longer sums); loss, if not null:
 // one more block, which forms the mean loss.
-template <class Tx, class Tw, bool RING>
-__global__ __launch_bounds__(Tw::NT) void xent_grads_any(GradArgs dx, GradArgs dw, int64_t dx_blocks, int64_t dw_blocks,
+template <class T>
+__global__ __launch_bounds__(T::NT) void xent_grads_small(GradArgs dx, GradArgs dw, int64_t dx_blocks, int64_t dw_blocks,
                                                             const float* row_loss, float* loss) {
-  using ForDx = typename Tx::template Loop<RING, true, false>;
-  static_assert(Tx::NT == Tw::NT, "one launch");
-  using ForDw = typename Tw::template Loop<RING, true, true>;
+  using ForDx = typename T::template Loop<true, false>;
+  using ForDw = typename T::template Loop<true, true>;
   __shared__ __attribute__((aligned(1024))) char smem[ForDx::LDS_BYTES > ForDw::LDS_BYTES ? ForDx::LDS_BYTES : ForDw::LDS_BYTES];
   const int64_t block = block_index();
   if (block < dx_blocks) grad_tile<ForDx>(dx, static_cast<int>(block), smem);
@@ -496,7 +536,7 @@ __global__ __launch_bounds__(64) void xent_join_kernel(Join dx, Join dw, int64_t
 struct WideGradArgs {
   const uint16_t *a, *b;
   int m, n, k;         // m, n: of out
-  int n_alloc;         // of B, where it is K-major: columns that are allocated
+  int n_alloc;         // of B, where it is K-major: columns that are allocated (of A: lda)
   int64_t lda, ldb;
   float* sum;          // [splits][n][m] f32, the pieces' sum
   bool first, last;    // of the pieces: sum holds nothing yet; the result is whole (never with splits)
@@ -505,6 +545,24 @@ struct WideGradArgs {
   void* out;
   int out_dt;
 };
+
+// Four elements from e on, of which the first n (or all) are the row's, to sum or to out.
+template <class Args>
+__device__ __forceinline__ void store_sum(const Args& p, float* sum, float inv, int64_t e, int n, float (&v)[4]) {
+  if (!p.first) {
+    float before[4];
+    load_some(VDSL_F32, sum, e, n, before);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] += before[j];
+  }
+  if (!p.last) {
+    store_some(VDSL_F32, sum, e, n, v);
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] *= inv;
+  store_some(p.out_dt, p.out, e, n, v);
+}
 
 // WHOLE: the product is all of the sum, rounded to bf16; otherwise any of the forms.
 template <bool BKM, bool WHOLE>
@@ -518,7 +576,7 @@ __global__ __launch_bounds__(WideCfg::NT, 1) void xent_grad_wide(WideGradArgs p)
   const uint16_t *const a = p.a + kb * p.lda, *const b = p.b + (BKM ? kb * p.ldb : kb);
   float* const sum = p.sum + static_cast<int64_t>(blockIdx.y) * p.n * p.m;
   const int cols = BKM ? p.n_alloc : p.n;
-  wide_gemm<true, BKM>(a, b, p.m, cols, ke - kb, p.lda, p.ldb, BKM, smem, [&](const f32x16 (&acc)[4][4], int m0, int n0) {
+  wide_gemm<true, BKM>(a, b, static_cast<int>(p.lda), cols, ke - kb, p.lda, p.ldb, BKM, smem, [&](const f32x16 (&acc)[4][4], int m0, int n0) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int row = n0 + 128 * (wave & 1) + 32 * j + static_cast<int>(threadIdx.x & 31);
@@ -538,22 +596,15 @@ __global__ __launch_bounds__(WideCfg::NT, 1) void xent_grad_wide(WideGradArgs p)
             for (int h = 0; h < 4; ++h) word[h] = pack_bf16x2(v[4 * q + 2 * h] * inv, v[4 * q + 2 * h + 1] * inv);
             const u32x4 eight = wide_exchange(word[0], word[1], word[2], word[3]);
             const int c = 32 * i + 8 * (q + half);
-            if (row < p.n && c0 + c < p.m) *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(p.out) + out + c) = eight;
+            if (row < p.n && c0 + c < p.m) store_eight(static_cast<uint16_t*>(p.out) + out + c, eight, p.m - c0 - c);
           }
         } else {
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             const int c = 32 * i + 8 * q + 4 * half;
             if (row >= p.n || c0 + c >= p.m) continue;
-            f32x4 s = {v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
-            if (!p.first) s += *reinterpret_cast<const f32x4*>(sum + out + c);
-            if (!p.last)
-              *reinterpret_cast<f32x4*>(sum + out + c) = s;
-            else if (p.out_dt == VDSL_F32)
-              *reinterpret_cast<f32x4*>(static_cast<float*>(p.out) + out + c) = s * inv;
-            else
-              *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + out + c) =
-                  make_uint2(pack_bf16x2(s[0] * inv, s[1] * inv), pack_bf16x2(s[2] * inv, s[3] * inv));
+            float four[4] = {v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
+            store_sum(p, sum, inv, out + c, p.m - c0 - c, four);
           }
         }
       }
@@ -564,39 +615,62 @@ __global__ __launch_bounds__(WideCfg::NT, 1) void xent_grad_wide(WideGradArgs p)
 // ---- host ----------------------------------------------------------------------------------------
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-enum Tiling { kTiles64x32, kTiles128x32, kTiles64, kTiles128x64, kTiles128, kTilesWide };
+enum Tiling { kTiles64, kTiles128x64, kTilesWide };
 
-// The tile of an m x n product on gemm_any.h.  A CU takes in operands at about 55 bytes a nanosecond, so a launch
-// lasts as long as its busiest CU's: rounds of tiles over the 256 CUs times the tile's rows and columns.
-// 300 x 5003 x 1000 14.8 us in tiles of 64 x 64 (two rounds).
-Tiling any_tiles(int64_t m, int64_t n) {
-  const auto cost = [&](int64_t bm, int64_t bn) { return ceil_div(ceil_div(m, bm) * ceil_div(n, bn), 256) * (bm + bn); };
-  const int64_t a = cost(64, 64), b = cost(128, 64), c = cost(128, 128);
-  return a <= b && a <= c ? kTiles64 : b <= c ? kTiles128x64 : kTiles128;
-}
-int64_t rows_of(Tiling t) { return t == kTiles64x32 || t == kTiles64 ? 64 : 128; }
-int64_t cols_of(Tiling t) { return t == kTiles64x32 || t == kTiles128x32 ? 32 : t == kTiles128 ? 128 : 64; }
-
-// Whether the products take gemm_wide.h's tiles: whole stages of dim, offsets of 256 rows that fit 32 bits, and
-// tiles for the card's 256 CUs.
-bool wide_runs(int64_t n, int64_t cols, int64_t dim) {
-  return dim % 64 == 0 && dim < (1 << 22) && cols < (1 << 22) && ceil_div(n, 256) * ceil_div(cols, 256) >= 192;
+// go(tile) for one of the smaller tiles.
+template <class Go>
+int on_tile(Tiling t, Go&& go) {
+  return t == kTiles64 ? go(Tile64{}) : go(Tile128x64{});
 }
 
-// Whether the smaller tiles take gemm_ring.h: rows of dim elements are whole 16-byte units, and the offsets of 128
-// rows fit 32 bits (G's rows are whole units of at most a vocabulary).
-bool ring_runs(int64_t dim) { return dim % 8 == 0 && dim < (1 << 23); }
+// Whether a gradient takes 3 2^32 products or more.
+bool many_products(int64_t n, int64_t cols, int64_t dim) { return n * cols >= ceil_div(int64_t{3} << 32, dim); }
+
+// Whether products may take gemm_wide.h's tiles: whole stages of dim, or so many products that laying out the rows
+// in whole stages is worth it; offsets of 256 rows that fit 32 bits.
+bool wide_fits(int64_t n, int64_t cols, int64_t dim) {
+  const bool whole = dim % 64 == 0 || (many_products(n, cols, dim) && 4 * dim >= 3 * (ceil_div(dim, 64) * 64));
+  return whole && dim < (1 << 22) && cols < (1 << 22);
+}
+
+// How many 128 x 64 tiles an m x n product has.
+int64_t small_tiles(int64_t m, int64_t n) { return ceil_div(m, 128) * ceil_div(n, 64); }
+
+// The logits' tiles.  256 x 256 where they use half of the card or more: a CU takes about 1 us for a stage of such a
+// tile on a card that is half idle (1.6 at full power), 0.42 for one of 128 x 64, an eighth of that.  Us of a loss,
+// 256 x 256 and 128 x 64: 2048 rows of 512, 8192 columns (the card full) 26.5, 34.5; 2048 x 1024, 5003 (61%) 33.6,
+// 37.5; 1024 x 1024, 8192 (half) 30.7, 30.0; 512 x 4096, 8192 (a quarter) 73, 43.5.
+// 64 x 64 where the others leave half of the CUs without one (64 x 64 and 128 x 64): 64 x 1000, 5003 (40 tiles)
+// 12.5, 14.5; 128 x 512, 8192 (128) 11.1, 11.9; 300 x 1000, 5003 (200) 16.8, 15.7; 1 x 4096, 32768 (256) 45.5, 43.3.
+Tiling logit_tiles(int64_t n, int64_t cols, int64_t dim) {
+  const int64_t rounds = ceil_div(ceil_div(n, 256) * ceil_div(cols, 256), 256);
+  if (wide_fits(n, cols, dim) && 2 * n * cols > rounds * 256 * 256 * 256) return kTilesWide;
+  return small_tiles(cols, n) <= 128 ? kTiles64 : kTiles128x64;
+}
+
+// The gradients' tiles, of both products.  256 x 256 from 3 2^32 products of a gradient on: they are two launches,
+// join f32 sums where they leave CUs idle and count the rows apart, 40 us.  Us of a call, 256 x 256 and 128 x 64:
+// 128 rows of 4096, 32768 columns 252, 272; 1024 x 2048, 8192 149, 152; 1024 x 1024, 12288 (the bound) 126, 131;
+// 2048 x 1024, 5003 131, 113; 300 x 1024, 32768 146, 137; 64 x 1024, 32768 92, 72.
+// 64 x 64 where two blocks to a CU have two stages of the others each or fewer (64 x 64 and 128 x 64): 16 x 512, 5003
+// 20.3, 22.6; 512 x 256, 1000 17.4, 18.7; 64 x 1000, 5003 28.9, 27.1; 300 x 512, 8192 40.9, 37.3.
+Tiling grad_tiles(int64_t n, int64_t cols, int64_t dim) {
+  if (wide_fits(n, cols, dim) && many_products(n, cols, dim)) return kTilesWide;
+  const int64_t stages = small_tiles(dim, n) * ceil_div(cols, 64) + small_tiles(dim, cols) * ceil_div(n, 64);
+  return stages <= 1024 ? kTiles64 : kTiles128x64;
+}
+int64_t rows_of(Tiling t) { return t == kTiles64 ? 64 : 128; }
 
 // How a call is laid out: the pieces, the tiles and the workspace.
 struct Plan {
   int64_t piece = 0, pieces = 0;  // columns of a piece (the last may have fewer)
-  // of all logits, of a piece's formed again, of dw (and dx where it has no other), of dx
-  Tiling logits = kTiles64, again = kTiles64, grads = kTiles64, dx = kTiles64;
+  Tiling logits = kTiles64, again = kTiles64, grads = kTiles64;  // of all logits, of a piece's formed again, of the gradients
   int64_t group_cols = 0, groups = 0;
   int64_t g_rows = 0, ldg = 0;    // of G; its rows past n are zeros
+  int64_t ld = 0;                 // of x and w: dim, or that of their copies in whole units (stages, for 256 x 256 tiles)
   int splits = 1, dw_splits = 1;  // of the sums over a piece's columns for dx, over the rows for dw
   bool sum = false;               // whether dx is formed by way of f32 sums (dw: where it has splits)
-  size_t at_stats = 0, at_zlabel = 0, at_lse = 0, at_row_loss = 0, at_inv = 0, at_g = 0, at_sum = 0, at_dw_sum = 0, bytes = 0;
+  size_t at_stats = 0, at_zlabel = 0, at_lse = 0, at_row_loss = 0, at_inv = 0, at_g = 0, at_sum = 0, at_dw_sum = 0, at_x = 0, at_w = 0, bytes = 0;
 };
 
 // The splits of the k of an m x n product on 256 x 256 tiles: as many as make its time least, rounds of a block on
@@ -616,37 +690,38 @@ int wide_splits(int64_t n, int64_t m, int64_t k) {
 }
 
 constexpr int64_t kPieceBytes = int64_t{1} << 30;  // of codes, where the caller leaves the piece to the library
+constexpr int64_t kPieceMost = int64_t{1} << 24;   // columns: the offsets of 64 rows of G fit 32 bits
 
 int make_plan(int64_t n, int64_t vocab, int64_t dim, int64_t piece, bool backward, Plan& p) {
   if (n < 0 || vocab < 0 || dim < 0 || piece < 0) return fail(VDSL_ERR_INVALID_ARG, "linear_xent: negative extent");
   if (vocab == 0) return fail(VDSL_ERR_INVALID_ARG, "linear_xent: the vocabulary is empty");
   if (dim < 8) return fail(VDSL_ERR_UNSUPPORTED, "linear_xent: dim must be at least 8");
-  if (n > 0x7fffff00 || vocab > 0x7fffff00 || dim > 0x3fffff00) return fail(VDSL_ERR_UNSUPPORTED, "linear_xent: extents too large");
-  if (!backward) piece = vocab;
-  else if (piece > vocab) piece = vocab;
-  else if (piece == 0) piece = std::max<int64_t>(256, kPieceBytes / 2 / std::max<int64_t>(n, 1));
+  if (n > 0x7fffff00 || vocab > 0x7fffff00 || dim > 0x7fff00) return fail(VDSL_ERR_UNSUPPORTED, "linear_xent: extents too large");
+  if (piece == 0) piece = std::max<int64_t>(256, kPieceBytes / 2 / std::max<int64_t>(n, 1));
+  piece = backward ? std::min({piece, vocab, kPieceMost}) : vocab;
   p.pieces = ceil_div(vocab, std::min(vocab, ceil_div(piece, 256) * 256));
   p.piece = p.pieces == 1 ? vocab : ceil_div(ceil_div(vocab, p.pieces), 256) * 256;
   p.pieces = ceil_div(vocab, p.piece);
-  const bool wide = wide_runs(n, p.piece, dim);
-  const bool few = n <= 32;
-  p.logits = wide ? kTilesWide : few ? kTiles64x32 : any_tiles(vocab, n);
-  p.again = wide ? kTilesWide : few ? kTiles64x32 : any_tiles(p.piece, n);
-  p.grads = wide ? kTilesWide : any_tiles(dim, p.piece);
-  p.dx = few ? kTiles128x32 : p.grads;
-  p.group_cols = wide ? 128 : rows_of(p.logits) / 2;
+  p.logits = logit_tiles(n, vocab, dim);
+  p.again = logit_tiles(n, p.piece, dim);
+  p.grads = grad_tiles(n, p.piece, dim);
+  const bool wide = p.logits == kTilesWide || p.again == kTilesWide || p.grads == kTilesWide;
+  p.ld = wide ? ceil_div(dim, 64) * 64 : ceil_div(dim, 8) * 8;
+  p.group_cols = p.logits == kTilesWide ? 128 : rows_of(p.logits) / 2;
   p.groups = ceil_div(vocab, p.group_cols);  // pieces are whole groups
-  const int64_t unit = wide ? 256 : 8;
+  const int64_t unit = p.grads == kTilesWide ? 256 : 8;
   p.ldg = ceil_div(p.piece, unit) * unit;
-  p.g_rows = wide ? ceil_div(n, 64) * 64 : n;
-  if (wide) {
+  p.g_rows = p.grads == kTilesWide ? ceil_div(n, 64) * 64 : n;
+  if (p.grads == kTilesWide) {
     p.splits = wide_splits(n, dim, p.piece);
     p.dw_splits = wide_splits(p.piece, dim, n);
   } else {
-    // One launch: splits of about as many stages as two blocks a CU come to, five at least.
-    const auto tiles = [&](Tiling t, int64_t rows) { return ceil_div(dim, rows_of(t)) * ceil_div(rows, cols_of(t)); };
+    // One launch: splits of as many stages as two blocks a CU come to, but of 12 or more, since each split's sums are
+    // written and read again (us with 12 and with 5: 16 x 512, 5003 20.3, 22.3; 300 x 1000, 5003 37.6, 39.6; 128 x 512,
+    // 8192 27.8, 33.6).
+    const auto tiles = [&](int64_t rows) { return ceil_div(dim, rows_of(p.grads)) * ceil_div(rows, 64); };
     const int64_t x_stages = ceil_div(p.piece, 64), w_stages = ceil_div(n, 64);
-    const int64_t share = std::max<int64_t>(5, ceil_div(tiles(p.dx, n) * x_stages + tiles(p.grads, p.piece) * w_stages, 512));
+    const int64_t share = std::max<int64_t>(12, ceil_div(tiles(n) * x_stages + tiles(p.piece) * w_stages, 512));
     p.splits = static_cast<int>(std::clamp<int64_t>(ceil_div(x_stages, share), 1, 64));
     p.dw_splits = static_cast<int>(std::clamp<int64_t>(ceil_div(w_stages, share), 1, 64));
   }
@@ -664,6 +739,10 @@ int make_plan(int64_t n, int64_t vocab, int64_t dim, int64_t piece, bool backwar
   p.at_lse = take(n, 4, 1);
   p.at_row_loss = take(n, 4, 1);
   p.at_inv = take(2, 4, 1);
+  if (p.ld != dim) {
+    p.at_x = take(n, p.ld, 2);
+    p.at_w = take(vocab, p.ld, 2);
+  }
   if (backward) {
     p.at_g = take(p.g_rows, p.ldg, 2);
     if (p.sum) p.at_sum = take(n, dim, 4 * p.splits);
@@ -674,44 +753,31 @@ int make_plan(int64_t n, int64_t vocab, int64_t dim, int64_t piece, bool backwar
 }
 
 template <class Cfg, int MODE>
-int launch_logits_on(const LogitArgs& a, float grad_scale, float* inv, hipStream_t s) {
+int launch_logits_small(const LogitArgs& a, float grad_scale, float* inv, hipStream_t s) {
   const int64_t tiles = ceil_div(a.cols, Cfg::BM) * ceil_div(a.n, Cfg::BN);
   if (tiles >= 0x7fffffff) return fail(VDSL_ERR_UNSUPPORTED, "linear_xent: too many tiles");
-  hipLaunchKernelGGL((xent_logits_any<Cfg, MODE>), block_grid(tiles + 1), dim3(Cfg::NT), 0, s, a, grad_scale, inv);
-  return check_launch("xent_logits_any");
-}
-template <class T, int MODE>
-int launch_logits_any(const LogitArgs& a, float grad_scale, float* inv, hipStream_t s) {
-  if (ring_runs(a.dim)) return launch_logits_on<typename T::template Loop<true, false, false>, MODE>(a, grad_scale, inv, s);
-  return launch_logits_on<typename T::template Loop<false, false, false>, MODE>(a, grad_scale, inv, s);
+  hipLaunchKernelGGL((xent_logits_small<Cfg, MODE>), block_grid(tiles + 1), dim3(Cfg::NT), 0, s, a, grad_scale, inv);
+  return check_launch("xent_logits_small");
 }
 
 template <int MODE>
 int launch_logits(const LogitArgs& a, Tiling tiling, float grad_scale, float* inv, hipStream_t s) {
-  switch (tiling) {
-    case kTilesWide:
-      hipLaunchKernelGGL(xent_logits_wide<MODE>, dim3(wide_blocks(ceil_div(a.n, 256) * ceil_div(a.cols, 256))), dim3(WideCfg::NT), 0, s, a);
-      return check_launch("xent_logits_wide");
-    case kTiles128: return launch_logits_any<Tile128, MODE>(a, grad_scale, inv, s);
-    case kTiles128x64: return launch_logits_any<Tile128x64, MODE>(a, grad_scale, inv, s);
-    case kTiles64x32: return launch_logits_any<Tile64x32, MODE>(a, grad_scale, inv, s);
-    default: return launch_logits_any<Tile64, MODE>(a, grad_scale, inv, s);
+  if (tiling != kTilesWide) {
+    return on_tile(tiling, [&](auto tile) {
+      return launch_logits_small<typename decltype(tile)::template Loop<false, false>, MODE>(a, grad_scale, inv, s);
+    });
   }
+  hipLaunchKernelGGL(xent_logits_wide<MODE>, dim3(wide_blocks(ceil_div(a.n, 256) * ceil_div(a.cols, 256))), dim3(WideCfg::NT), 0, s, a);
+  return check_launch("xent_logits_wide");
 }
 
-template <class Tx, class Tw>
-int launch_grads_on(const GradArgs& dx, const GradArgs& dw, const float* row_loss, float* loss, hipStream_t s) {
-  const int64_t x = Tx::tiles(dx.m, dx.n) * dx.splits, w = Tw::tiles(dw.m, dw.n) * dw.splits;
+template <class T>
+int launch_grads_small(const GradArgs& dx, const GradArgs& dw, const float* row_loss, float* loss, hipStream_t s) {
+  const int64_t x = T::tiles(dx.m, dx.n) * dx.splits, w = T::tiles(dw.m, dw.n) * dw.splits;
   if (x > 0x7fffffff || w > 0x7fffffff) return fail(VDSL_ERR_UNSUPPORTED, "linear_xent: too many tiles");
   const dim3 grid = block_grid(x + w + (loss ? 1 : 0));
-  if (ring_runs(dx.m)) hipLaunchKernelGGL((xent_grads_any<Tx, Tw, true>), grid, dim3(Tw::NT), 0, s, dx, dw, x, w, row_loss, loss);
-  else hipLaunchKernelGGL((xent_grads_any<Tx, Tw, false>), grid, dim3(Tw::NT), 0, s, dx, dw, x, w, row_loss, loss);
-  return check_launch("xent_grads_any");
-}
-template <class Tw>
-int launch_grads_any(const GradArgs& dx, const GradArgs& dw, Tiling dx_tiling, const float* row_loss, float* loss, hipStream_t s) {
-  if (dx_tiling == kTiles128x32) return launch_grads_on<Tile128x32, Tw>(dx, dw, row_loss, loss, s);
-  return launch_grads_on<Tw, Tw>(dx, dw, row_loss, loss, s);
+  hipLaunchKernelGGL(xent_grads_small<T>, grid, dim3(T::NT), 0, s, dx, dw, x, w, row_loss, loss);
+  return check_launch("xent_grads_small");
 }
 
 template <bool BKM>
@@ -756,7 +822,7 @@ int run_xent(vdsl_queue q, int64_t n, int64_t dim, int64_t vocab, vdsl_buffer x,
   const int64_t last_piece = (plan.pieces - 1) * plan.piece;
   LogitArgs la{};
   la.x = static_cast<const uint16_t*>(x->ptr);
-  la.w = static_cast<const uint16_t*>(w->ptr);
+  const uint16_t* w_rows = static_cast<const uint16_t*>(w->ptr);
   la.labels = lab;
   la.stats = reinterpret_cast<float2*>(ws + plan.at_stats);
   la.zlabel = reinterpret_cast<float*>(ws + plan.at_zlabel);
@@ -764,10 +830,20 @@ int run_xent(vdsl_queue q, int64_t n, int64_t dim, int64_t vocab, vdsl_buffer x,
   la.lse = reinterpret_cast<const float*>(ws + plan.at_lse);
   la.n = static_cast<int>(n);
   la.cols = la.vocab = static_cast<int>(vocab);
-  la.dim = static_cast<int>(dim);
+  la.dim = static_cast<int>(plan.ld);
   la.groups = static_cast<int>(plan.groups);
   la.ldg = plan.ldg;
   la.g0 = static_cast<int>(last_piece);
+  if (n > 0 && plan.ld != dim) {
+    uint16_t* const x_copy = reinterpret_cast<uint16_t*>(ws + plan.at_x);
+    uint16_t* const w_copy = reinterpret_cast<uint16_t*>(ws + plan.at_w);
+    hipLaunchKernelGGL(xent_layout_kernel, block_grid(ceil_div(n + vocab, 4)), dim3(256), 0, s, la.x, n, w_rows, vocab, dim, x_copy, w_copy,
+                       plan.ld);
+    VDSL_TRY(check_launch("xent_layout_kernel"));
+    la.x = x_copy;
+    w_rows = w_copy;
+  }
+  la.w = w_rows;
   if (n > 0) {
     if (backward) VDSL_TRY(launch_logits<kLogitCodes>(la, plan.logits, grad_scale, inv, s));
     else VDSL_TRY(launch_logits<kLogitStats>(la, plan.logits, grad_scale, inv, s));
@@ -792,7 +868,9 @@ int run_xent(vdsl_queue q, int64_t n, int64_t dim, int64_t vocab, vdsl_buffer x,
     hipLaunchKernelGGL(xent_rows_kernel, block_grid(ra.g_rows), dim3(256), 0, s, ra);
     VDSL_TRY(check_launch("xent_rows_kernel"));
   }
-  if (!backward || n == 0 || plan.grads == kTilesWide) {
+  // (the smaller tiles' launches have blocks for the loss and for the factor of the gradients)
+  const bool mean_apart = !backward || n == 0 || plan.logits == kTilesWide || plan.grads == kTilesWide;
+  if (mean_apart) {
     hipLaunchKernelGGL(xent_mean_kernel, dim3(1), dim3(1024), 0, s, each, lab, n, la.vocab, grad_scale, loss_out, inv);
     VDSL_TRY(check_launch("xent_mean_kernel"));
   }
@@ -805,29 +883,28 @@ int run_xent(vdsl_queue q, int64_t n, int64_t dim, int64_t vocab, vdsl_buffer x,
   float* const sum = plan.sum ? reinterpret_cast<float*>(ws + plan.at_sum) : nullptr;
   float* const dw_sum = plan.dw_splits > 1 ? reinterpret_cast<float*>(ws + plan.at_dw_sum) : nullptr;
   la.g0 = 0;
+  const int out_cols = static_cast<int>(dim);
   // The piece whose codes are held comes first, then those whose logits are formed again.
   for (int64_t t = 0; t < plan.pieces; ++t) {
     const int64_t v0 = last_piece - t * plan.piece;
-    la.w = static_cast<const uint16_t*>(w->ptr) + v0 * dim;
+    la.w = w_rows + v0 * plan.ld;
     la.v0 = static_cast<int>(v0);
     la.cols = static_cast<int>(std::min(plan.piece, vocab - v0));
     const bool last = t == plan.pieces - 1;
     if (t > 0) VDSL_TRY(launch_logits<kLogitGrad>(la, plan.again, grad_scale, inv, s));
     void* const dw_piece = static_cast<char*>(dw->ptr) + v0 * dim * static_cast<int64_t>(dtype_size(dw_dtype));
     if (plan.grads == kTilesWide) {
-      const WideGradArgs for_dx{la.w, g,      la.dim, la.n,   la.cols, 0, dim, plan.ldg, sum, t == 0, last && plan.splits == 1,
+      const WideGradArgs for_dx{la.w, g, out_cols, la.n, la.cols, 0, plan.ld, plan.ldg, sum, t == 0, last && plan.splits == 1,
                                 plan.splits, inv, dx->ptr, dx_dtype};
       VDSL_TRY(launch_grad_wide<false>(for_dx, n, s));
-      const WideGradArgs for_dw{la.x, g,        la.dim, la.cols, la.n, static_cast<int>(plan.ldg), dim, plan.ldg, dw_sum, true, !dw_sum,
+      const WideGradArgs for_dw{la.x, g, out_cols, la.cols, la.n, static_cast<int>(plan.ldg), plan.ld, plan.ldg, dw_sum, true, !dw_sum,
                                 plan.dw_splits, inv, dw_piece, dw_dtype};
       VDSL_TRY(launch_grad_wide<true>(for_dw, plan.ldg, s));
     } else {
-      const GradArgs for_dx{la.w, g, la.dim, la.n, la.cols, dim, plan.ldg, sum, t == 0, plan.splits, inv, dx->ptr, dx_dtype};
-      const GradArgs for_dw{la.x, g, la.dim, la.cols, la.n, dim, plan.ldg, dw_sum, true, plan.dw_splits, inv, dw_piece, dw_dtype};
-      float* const mean = t == 0 ? loss_out : nullptr;
-      if (plan.grads == kTiles128) VDSL_TRY(launch_grads_any<Tile128>(for_dx, for_dw, plan.dx, each, mean, s));
-      else if (plan.grads == kTiles128x64) VDSL_TRY(launch_grads_any<Tile128x64>(for_dx, for_dw, plan.dx, each, mean, s));
-      else VDSL_TRY(launch_grads_any<Tile64>(for_dx, for_dw, plan.dx, each, mean, s));
+      const GradArgs for_dx{la.w, g, out_cols, la.n, la.cols, plan.ld, plan.ldg, sum, t == 0, plan.splits, inv, dx->ptr, dx_dtype};
+      const GradArgs for_dw{la.x, g, out_cols, la.cols, la.n, plan.ld, plan.ldg, dw_sum, true, plan.dw_splits, inv, dw_piece, dw_dtype};
+      float* const mean = t == 0 && !mean_apart ? loss_out : nullptr;
+      VDSL_TRY(on_tile(plan.grads, [&](auto tile) { return launch_grads_small<decltype(tile)>(for_dx, for_dw, each, mean, s); }));
     }
     // a wide dx without splits is whole with its last piece
     const bool join_dx = last && sum && (plan.grads != kTilesWide || plan.splits > 1);

@@ -20,7 +20,7 @@ namespace {
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 // 2^log_l lanes per output row, KU units of U elements each; blockIdx.y: strips of columns.
-template <int TT, int OT, int U, int KU>
+template <int TT, int OT, int U, int KU, bool STREAM>
 __global__ __launch_bounds__(256) void embedding_fwd_kernel(const void* __restrict__ table, const int32_t* __restrict__ ids,
                                                             void* __restrict__ out, int64_t n, int64_t dim, int64_t vocab,
                                                             float scale, int log_l) {
@@ -39,7 +39,7 @@ __global__ __launch_bounds__(256) void embedding_fwd_kernel(const void* __restri
     const UnitAt<U> at(c0 + static_cast<int64_t>(k) * lanes * U, dim);
 #pragma unroll
     for (int j = 0; j < U; ++j) v[k][j] = valid ? v[k][j] * scale : 0.0f;
-    if (at.any()) store_whole<OT, U>(out, i * dim + at.c, v[k]);
+    if (at.any()) store_whole<OT, U, STREAM>(out, i * dim + at.c, v[k]);
   }
 }
 
@@ -55,11 +55,12 @@ __device__ __forceinline__ void clear_places(int2* __restrict__ places, int64_t 
   for (int64_t v = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; v < vocab; v += step) places[v] = make_int2(0, 0);
 }
 
-// Up to kRankTile positions: position i goes to place #{j : id_j < id_i} + #{j < i : id_j = id_i}.  A block
+// Up to 32768 positions.  Of up to kRankTile, position i goes to place #{j : id_j < id_i} + #{j < i : id_j = id_i}.  A block
 // ranks 64 positions, one a lane, its 16 waves a share of the ids each.  Ids are compared as unsigned
-// numbers, so those that are no row come last.  More positions are ranked so in tiles, and a second kernel
-// adds to an element's rank what the other tiles have before it, a binary search in each: 16384 positions
-// 28 us ranked against all ids, 10 so (radix passes 24).
+// numbers, so those that are no row come last.  More are ranked so in tiles, and a second kernel
+// adds to an element's rank what the other tiles have before it, a binary search in each.  Us of a gradient of 256
+// columns, vocabulary 32768, sorted so and by radix passes: n 4096 20.7, 30.9; 16384 22.1, 31.2; 32768 27.4, 34.3; 65536
+// 47.8, 40.3.
 constexpr int kRankTile = 1024;
 
 __global__ __launch_bounds__(1024) void embedding_rank_kernel(const int32_t* __restrict__ ids, int n, uint32_t* __restrict__ sorted,
@@ -361,7 +362,7 @@ __global__ __launch_bounds__(256) void embedding_chunk_kernel(const uint32_t* __
 // most kFewPositions) are searched in LDS.
 constexpr int kFewPositions = 512;
 
-template <int DYT, int U, int NV, bool CHUNKS>
+template <int DYT, int U, int NV, bool CHUNKS, bool STREAM>
 __global__ __launch_bounds__(256) void embedding_bwd_kernel(const uint32_t* __restrict__ sorted, const int32_t* __restrict__ order,
                                                             const void* __restrict__ dy, const int2* __restrict__ places,
                                                             const float* __restrict__ partials, int chunk,
@@ -396,7 +397,7 @@ __global__ __launch_bounds__(256) void embedding_bwd_kernel(const uint32_t* __re
   for (int u = 0; u < NV; ++u) {
 #pragma unroll
     for (int j = 0; j < U; ++j) acc[u][j] *= scale;
-    if (at.any[u]) store_whole<VDSL_F32, U>(dtable, v * dim + at.c[u], acc[u]);
+    if (at.any[u]) store_whole<VDSL_F32, U, STREAM>(dtable, v * dim + at.c[u], acc[u]);
   }
 }
 
@@ -437,23 +438,26 @@ extern "C" int vdsl_op_embedding_fwd(vdsl_queue q, int64_t n, int64_t dim, int64
                        n * dim * static_cast<int64_t>(dtype_size(out_dtype) / 2));
     return check_launch("embedding_zero_kernel");
   }
-  const auto go = [&](auto tt, auto ot, auto unit, auto ku) {
+  const auto go = [&](auto tt, auto ot, auto unit, auto ku, auto stream) {
     constexpr int TT = decltype(tt)::value, OT = decltype(ot)::value, U = decltype(unit)::value, KU = decltype(ku)::value;
     const int64_t units = (dim + U - 1) / U;
     const int l = lanes_log2(units);
     const int64_t bx = (n + (256 >> l) - 1) >> (8 - l), by = (units + (int64_t{KU} << l) - 1) / (int64_t{KU} << l);
     if (by > 65535) return fail(VDSL_ERR_UNSUPPORTED, "embedding_fwd: rows too wide");
-    hipLaunchKernelGGL((embedding_fwd_kernel<TT, OT, U, KU>), block_grid(bx, by), dim3(256), 0, q->stream, table->ptr,
+    hipLaunchKernelGGL((embedding_fwd_kernel<TT, OT, U, KU, decltype(stream)::value>), block_grid(bx, by), dim3(256), 0, q->stream, table->ptr,
                        static_cast<const int32_t*>(ids->ptr), out->ptr, n, dim, vocab, scale, l);
     return check_launch("embedding_fwd_kernel");
   };
-  // A lane takes 4 units where that leaves enough waves to fill the card, so that their loads are in flight together.
-  const bool many = n * dim >= int64_t{1} << 22;
+  // A lane takes 16 bytes of the wider type, or four times that where its loads' time is the longer then: outputs that
+  // pass the caches by.  Us, vocabulary 32768, f32 table and bf16 output, 16 bytes and 64: 4096 x 4096 15.5, 16.0;
+  // 16384 x 4096 73.3, 59.4; bf16 table and f32 output: 16384 x 1024 16.2, 18.6; 16384 x 4096 102.6, 70.9.
   const auto pick = [&](auto tt, auto ot) {
     constexpr int U = decltype(tt)::value == VDSL_BF16 && decltype(ot)::value == VDSL_BF16 ? 8 : 4;
-    if (dim < U) return go(tt, ot, std::integral_constant<int, 1>{}, std::integral_constant<int, 1>{});
-    if (many) return go(tt, ot, std::integral_constant<int, U>{}, std::integral_constant<int, 16 / U>{});
-    return go(tt, ot, std::integral_constant<int, U>{}, std::integral_constant<int, 1>{});
+    using One = std::integral_constant<int, 1>;
+    if (dim < U) return go(tt, ot, One{}, One{}, std::false_type{});
+    const bool large = n * dim * static_cast<int64_t>(dtype_size(out_dtype)) >= kStreamBytes;
+    if (large) return go(tt, ot, std::integral_constant<int, U>{}, std::integral_constant<int, 16 / U>{}, std::true_type{});
+    return go(tt, ot, std::integral_constant<int, U>{}, One{}, std::false_type{});
   };
   using F = std::integral_constant<int, VDSL_F32>;
   using B = std::integral_constant<int, VDSL_BF16>;
@@ -474,11 +478,17 @@ struct GradPlan {
 
 int grad_plan(int64_t n, int64_t vocab, int64_t dim, GradPlan& p) {
   VDSL_TRY(check_extents(n, dim, vocab));
-  p.radix = n > 16384;
+  p.radix = n > 32768;
   p.passes = vocab < 256 ? 1 : vocab < 65536 ? 2 : vocab < (1 << 24) ? 3 : 4;
   p.tile = static_cast<int>(std::max<int64_t>(1024, ((n + 255) / 256 + 1023) / 1024 * 1024));
   p.tiles = (n + p.tile - 1) / p.tile;
-  p.chunk = n <= kFewPositions ? 0 : n <= 32768 ? 16 : n <= 262144 ? 64 : 256;
+  // n / chunk chunks, and up to 2 chunk places of a token outside them.  Us of 512 columns, vocabulary 32768, ids as
+  // frequent as words, in chunks of 16, 32, 64, 128: n 4096 26.9, 31.3, 40.3, 51.8; 16384 36.1, 34.6, 42.5, 59.1; 65536
+  // 93.6, 73.9, 69.3, 88.5; 262144 297, 201, 164, 152.  None at all (1001 columns, vocabulary 5003): n 512 17.5, in
+  // chunks 19.1; 1000 24.9, 20.6.
+  p.chunk = 0;
+  if (n > kFewPositions)
+    for (p.chunk = 16; int64_t{16} * p.chunk * p.chunk < n;) p.chunk *= 2;
   size_t at = 0;
   bool fits = true;
   const auto take = [&](int64_t a, int64_t b) {
@@ -573,7 +583,7 @@ extern "C" int vdsl_op_embedding_bwd(vdsl_queue q, int64_t n, int64_t dim, int64
     const int64_t rows = 256 >> l;
     const dim3 grid = block_grid((vocab + rows - 1) / rows, strips);
     if (!p.chunk) {
-      hipLaunchKernelGGL((embedding_bwd_kernel<DYT, U, NV, false>), grid, dim3(256), 0, s, sorted, order, dy->ptr, nullptr, nullptr, 0,
+      hipLaunchKernelGGL((embedding_bwd_kernel<DYT, U, NV, false, false>), grid, dim3(256), 0, s, sorted, order, dy->ptr, nullptr, nullptr, 0,
                          static_cast<float*>(dtable->ptr), count, dim, vocab, scale, l);
       return check_launch("embedding_bwd_kernel");
     }
@@ -582,7 +592,8 @@ extern "C" int vdsl_op_embedding_bwd(vdsl_queue q, int64_t n, int64_t dim, int64
                        dim3(256), 0, s, sorted, order, dy->ptr, count, dim, vocab, p.chunk, l, static_cast<int>(place_blocks), places,
                        partials);
     VDSL_TRY(check_launch("embedding_chunk_kernel"));
-    hipLaunchKernelGGL((embedding_bwd_kernel<DYT, U, NV, true>), grid, dim3(256), 0, s, sorted, order, dy->ptr, places, partials, p.chunk,
+    const auto rows_kernel = vocab * dim * 4 >= kStreamBytes ? embedding_bwd_kernel<DYT, U, NV, true, true> : embedding_bwd_kernel<DYT, U, NV, true, false>;
+    hipLaunchKernelGGL(rows_kernel, grid, dim3(256), 0, s, sorted, order, dy->ptr, places, partials, p.chunk,
                        static_cast<float*>(dtable->ptr), count, dim, vocab, scale, l);
     return check_launch("embedding_bwd_kernel");
   };

@@ -83,7 +83,7 @@ __device__ __forceinline__ void load_row(const void* __restrict__ p, int64_t row
   }
 }
 
-template <class S, int XT>
+template <class S, int XT, bool STREAM>
 __global__ __launch_bounds__(S::kThreads) void layer_norm_fwd_rows(const void* x, const void* __restrict__ gamma,
                                                                    const void* __restrict__ beta, int param_dt, void* y, int y_dt,
                                                                    float* __restrict__ mean_out, float* __restrict__ rstd_out,
@@ -137,7 +137,7 @@ __global__ __launch_bounds__(S::kThreads) void layer_norm_fwd_rows(const void* x
       float o[U];
 #pragma unroll
       for (int j = 0; j < U; ++j) o[j] = v[k][j] * rstd * ga[k][j] + be[k][j];
-      if (at.any()) store_whole<U>(y_dt, y, row * cols + at.c, o);
+      if (at.any()) store_unit<U, STREAM>(y_dt, y, row * cols + at.c, o);
     }
   }
 }
@@ -187,7 +187,7 @@ __global__ __launch_bounds__(1024) void layer_norm_fwd_stream(const void* x, int
 
 // partials: [gridDim.x][2][cols], a block's sums for dgamma and dbeta over its rows (waves of one block
 // that hold rows of their own meet in LDS, in the order of the waves); null where neither is wanted.
-template <class S, int XT, int DYT>
+template <class S, int XT, int DYT, bool STREAM>
 __global__ __launch_bounds__(S::kThreads) void layer_norm_bwd_rows(const void* dy, const void* __restrict__ x,
                                                                    const void* __restrict__ gamma, int param_dt,
                                                                    const float* __restrict__ mean, const float* __restrict__ rstd,
@@ -197,14 +197,16 @@ __global__ __launch_bounds__(S::kThreads) void layer_norm_bwd_rows(const void* d
   const int t = threadIdx.x % S::kLanes, slot = threadIdx.x / S::kLanes;
   const int64_t step = static_cast<int64_t>(gridDim.x) * S::kRows;
   int64_t row = static_cast<int64_t>(blockIdx.x) * S::kRows + slot;
+  constexpr bool AHEAD = NV * U * S::kThreads < 16384;  // 1024 lanes of 16 columns have no registers for another row
   float ga[NV][U], dg[NV][U], db[NV][U], nx[NV][U], ny[NV][U];
   float nmean = 0.0f, nrstd = 0.0f;
-  if (row < rows) {
-    load_row<S, XT>(x, row, cols, t, nx);
-    load_row<S, DYT>(dy, row, cols, t, ny);
-    nmean = mean[row];
-    nrstd = rstd[row];
-  }
+  const auto load = [&](int64_t at) {
+    load_row<S, XT>(x, at, cols, t, nx);
+    load_row<S, DYT>(dy, at, cols, t, ny);
+    nmean = mean[at];
+    nrstd = rstd[at];
+  };
+  if (AHEAD && row < rows) load(row);
   load_params<S>(gamma, param_dt, cols, t, 1.0f, ga);
 #pragma unroll
   for (int k = 0; k < NV; ++k)
@@ -213,6 +215,7 @@ __global__ __launch_bounds__(S::kThreads) void layer_norm_bwd_rows(const void* d
   const float inv_cols = 1.0f / static_cast<float>(cols);
   int parity = 0;
   for (; row < rows; row += step) {
+    if (!AHEAD) load(row);
     float h[NV][U], d[NV][U];
     const float r = nrstd;
 #pragma unroll
@@ -223,12 +226,7 @@ __global__ __launch_bounds__(S::kThreads) void layer_norm_bwd_rows(const void* d
         d[k][j] = ny[k][j];
       }
     }
-    if (row + step < rows) {
-      load_row<S, XT>(x, row + step, cols, t, nx);
-      load_row<S, DYT>(dy, row + step, cols, t, ny);
-      nmean = mean[row + step];
-      nrstd = rstd[row + step];
-    }
+    if (AHEAD && row + step < rows) load(row + step);
     float s[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
@@ -251,7 +249,7 @@ __global__ __launch_bounds__(S::kThreads) void layer_norm_bwd_rows(const void* d
       float o[U];
 #pragma unroll
       for (int j = 0; j < U; ++j) o[j] = r * ((d[k][j] - m1) - h[k][j] * m2);
-      if (at.any()) store_whole<U>(dx_dt, dx, row * cols + at.c, o);
+      if (at.any()) store_unit<U, STREAM>(dx_dt, dx, row * cols + at.c, o);
     }
   }
   if (!partials) return;
@@ -385,7 +383,18 @@ int row_shape(int64_t cols, Go&& go, Wide&& wide) {
   return wide();
 }
 
-constexpr int64_t kBwdBlocks = 512;  // partial rows at most
+// Blocks of the backward pass, each of which leaves a partial row: so many that a CU has about 32 KiB of rows on their
+// way, 256 to 1024 (us of 256, 512 and 1024, rows of bf16: 65536 x 256 51.2, 35.5, 29.4; 32768 x 2048 168, 107, 81.5;
+// 16384 x 4096 113, 78.0, 94.2; 8192 x 8192 86.1, 90.9, 101; of f32: 16384 x 4096 147, 161, 164), but of four rows
+// or more where there are more than 256 (2048 x 2048, bf16, in 1024 and in 512 blocks 18.8, 14.3; 512 x 8192 in 512 and
+// in 256 22.7, 17.6).
+// together: the rows a block holds at a time; bytes: of a row of x and one of dy.
+int64_t bwd_blocks(int64_t rows, int64_t together, int64_t bytes) {
+  const int64_t most = std::clamp<int64_t>(((int64_t{8} << 20) / (together * bytes) + 128) / 256 * 256, 256, 1024);
+  const int64_t blocks = (rows + together - 1) / together;
+  return blocks <= 256 ? blocks : std::min(most, std::max<int64_t>(256, blocks / 4));
+}
+int64_t bwd_most_blocks(int64_t rows, int64_t cols) { return bwd_blocks(rows, cols <= 1024 ? 4 : 1, 4 * cols); }
 
 bool float_type(int32_t t) { return t == VDSL_F32 || t == VDSL_BF16; }
 
@@ -418,8 +427,10 @@ extern "C" int vdsl_op_layer_norm_fwd(vdsl_queue q, int64_t rows, int64_t cols, 
   const auto rows_kernel = [&](auto shape, auto xt) {
     using S = decltype(shape);
     constexpr int XT = decltype(xt)::value;
-    const int64_t blocks = std::min<int64_t>((rows + S::kRows - 1) / S::kRows, 256 * 2048 / S::kThreads);
-    hipLaunchKernelGGL((layer_norm_fwd_rows<S, XT>), dim3(static_cast<unsigned>(blocks)), dim3(S::kThreads), 0, q->stream, x->ptr,
+    const int64_t blocks = std::min<int64_t>((rows + S::kRows - 1) / S::kRows, 512 * 2048 / S::kThreads);
+    const bool stream = rows * cols * static_cast<int64_t>(dtype_size(y_dtype)) >= kStreamBytes;
+    const auto kernel = stream ? layer_norm_fwd_rows<S, XT, true> : layer_norm_fwd_rows<S, XT, false>;
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(S::kThreads), 0, q->stream, x->ptr,
                        g, b, param_dtype, y->ptr, y_dtype, mo, ro, rows, cols, eps);
     return check_launch("layer_norm_fwd_rows");
   };
@@ -438,7 +449,7 @@ extern "C" int vdsl_op_layer_norm_fwd(vdsl_queue q, int64_t rows, int64_t cols, 
 extern "C" int vdsl_layer_norm_bwd_workspace_bytes(int64_t rows, int64_t cols, size_t* bytes) {
   if (!bytes) return fail(VDSL_ERR_INVALID_ARG, "bytes is null");
   if (rows < 0 || cols < 0) return fail(VDSL_ERR_INVALID_ARG, "negative shape");
-  const size_t n = nbytes(std::min(rows, kBwdBlocks), cols, 8);
+  const size_t n = nbytes(bwd_most_blocks(rows, std::max<int64_t>(cols, 1)), cols, 8);
   if (n == kSizeOverflow) return fail(VDSL_ERR_SHAPE, "layer_norm_bwd workspace size overflows");
   *bytes = n;
   return VDSL_OK;
@@ -478,16 +489,18 @@ extern "C" int vdsl_op_layer_norm_bwd(vdsl_queue q, int64_t rows, int64_t cols, 
   const auto rows_kernel = [&](auto shape, auto xt, auto dyt) {
     using S = decltype(shape);
     constexpr int XT = decltype(xt)::value, DYT = decltype(dyt)::value;
-    const int64_t blocks = std::min<int64_t>((rows + S::kRows - 1) / S::kRows, kBwdBlocks);
+    const int64_t blocks = bwd_blocks(rows, S::kRows, cols * static_cast<int64_t>(dtype_size(x_dtype) + dtype_size(dy_dtype)));
     partial_rows = blocks;
-    hipLaunchKernelGGL((layer_norm_bwd_rows<S, XT, DYT>), dim3(static_cast<unsigned>(blocks)), dim3(S::kThreads), 0, q->stream,
+    const bool stream = rows * cols * static_cast<int64_t>(dtype_size(dx_dtype)) >= kStreamBytes;
+    const auto kernel = stream ? layer_norm_bwd_rows<S, XT, DYT, true> : layer_norm_bwd_rows<S, XT, DYT, false>;
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(S::kThreads), 0, q->stream,
                        dy->ptr, x->ptr, g, param_dtype, mi, ri, dx->ptr, dx_dtype, part, rows, cols);
     return check_launch("layer_norm_bwd_rows");
   };
   const auto wide = [&] {
     if (params) {
       const int64_t strips = (cols + 1023) / 1024;
-      partial_rows = std::min<int64_t>(rows, std::max<int64_t>(1, kBwdBlocks / strips));
+      partial_rows = std::min<int64_t>(bwd_most_blocks(rows, cols), std::max<int64_t>(1, 512 / strips));
       hipLaunchKernelGGL(layer_norm_bwd_columns, dim3(static_cast<unsigned>(strips), static_cast<unsigned>(partial_rows)), dim3(256),
                          0, q->stream, dy->ptr, dy_dtype, x->ptr, x_dtype, mi, ri, part, rows, cols);
       VDSL_TRY(check_launch("layer_norm_bwd_columns"));

@@ -60,7 +60,19 @@ __device__ __forceinline__ void load_whole(const void* __restrict__ p, int64_t e
     }
   }
 }
-template <int DT, int U>
+// Outputs of this many bytes or more pass the caches by: they would drive out what else is there, and whoever reads
+// them next finds little of them.  us of an embedding's lookup and the layer norm that reads it, rows of 4096 in bf16,
+// stores kept and passed by: 64 MiB 44.5, 47.5; 128 MiB 91.7, 88.5; of layer norm's gradient and one that reads it
+// 64.0, 73.5; 129.6, 125.8.
+constexpr int64_t kStreamBytes = int64_t{96} << 20;
+
+// STREAM is the kernels' parameter, since of a plain and a passing store in two branches the compiler makes one plain one.
+template <bool STREAM, class V>
+__device__ __forceinline__ void store_at(V* to, V v) {
+  if constexpr (STREAM) __builtin_nontemporal_store(v, to);
+  else *to = v;
+}
+template <int DT, int U, bool STREAM = false>
 __device__ __forceinline__ void store_whole(void* __restrict__ p, int64_t e, const float (&v)[U]) {
   if constexpr (U == 1) {
     if constexpr (DT == VDSL_F32) static_cast<float*>(p)[e] = v[0];
@@ -69,20 +81,20 @@ __device__ __forceinline__ void store_whole(void* __restrict__ p, int64_t e, con
 #pragma unroll
     for (int h = 0; h < U / 4; ++h) {
       const f32x4 x = {v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]};
-      reinterpret_cast<F32x4At4*>(static_cast<float*>(p) + e + 4 * h)->v = x;
+      store_at<STREAM>(&reinterpret_cast<F32x4At4*>(static_cast<float*>(p) + e + 4 * h)->v, x);
     }
   } else if constexpr (U == 8) {
     const u32x4 x = {pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])};
-    reinterpret_cast<U32x4At2*>(static_cast<uint16_t*>(p) + e)->v = x;
+    store_at<STREAM>(&reinterpret_cast<U32x4At2*>(static_cast<uint16_t*>(p) + e)->v, x);
   } else {
     const u32x2 x = {pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
-    reinterpret_cast<U32x2At2*>(static_cast<uint16_t*>(p) + e)->v = x;
+    store_at<STREAM>(&reinterpret_cast<U32x2At2*>(static_cast<uint16_t*>(p) + e)->v, x);
   }
 }
-template <int U>
-__device__ __forceinline__ void store_whole(int dt, void* __restrict__ p, int64_t e, const float (&v)[U]) {
-  if (dt == VDSL_F32) store_whole<VDSL_F32, U>(p, e, v);
-  else store_whole<VDSL_BF16, U>(p, e, v);
+template <int U, bool STREAM = false>
+__device__ __forceinline__ void store_unit(int dt, void* __restrict__ p, int64_t e, const float (&v)[U]) {
+  if (dt == VDSL_F32) store_whole<VDSL_F32, U, STREAM>(p, e, v);
+  else store_whole<VDSL_BF16, U, STREAM>(p, e, v);
 }
 
 // A lane's unit of U columns from column c on, in a row of at least U: a unit that would pass the row's end
@@ -115,7 +127,7 @@ __device__ __forceinline__ void load_some(int dt, const void* __restrict__ p, in
 }
 __device__ __forceinline__ void store_some(int dt, void* __restrict__ p, int64_t e, int64_t n, const float (&v)[4]) {
   if (n >= 4) {
-    store_whole<4>(dt, p, e, v);
+    store_unit<4>(dt, p, e, v);
   } else {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {

@@ -663,8 +663,8 @@ int vdsl_op_layer_norm_bwd(vdsl_queue q, int64_t rows, int64_t cols, int32_t dy_
  * w BF16 [vocab][dim], f32 accumulate, never stored), lse[i] = log sum_v exp(z[i][v]),
  * row_loss[i] = lse[i] - z[i][labels[i]], 0 where labels[i] (I32 [n]) is outside [0, vocab): such a row
  * does not count; loss (F32 [1]) = sum of row_loss / number of rows that count (0 if none does).
- * row_loss, lse: F32 [n], each may be NULL.  dim >= 8.  A row whose logits hold a NaN or +inf has a NaN
- * lse and loss.  workspace: vdsl_linear_xent_workspace_bytes(n, vocab, dim, 0, 0) bytes. */
+ * row_loss, lse: F32 [n], each may be NULL.  8 <= dim < 2^23.  A row whose logits hold a NaN or +inf, or are
+ * -inf all of them, has a NaN loss and gradient.  workspace: vdsl_linear_xent_workspace_bytes(n, vocab, dim, 0, 0) bytes. */
 int vdsl_linear_xent_workspace_bytes(int64_t n, int64_t vocab, int64_t dim, int64_t piece,
                                      int32_t backward, size_t* bytes);
 int vdsl_op_linear_xent_fwd(vdsl_queue q, int64_t n, int64_t dim, int64_t vocab, vdsl_buffer x,
@@ -672,11 +672,14 @@ int vdsl_op_linear_xent_fwd(vdsl_queue q, int64_t n, int64_t dim, int64_t vocab,
                             vdsl_buffer lse, vdsl_buffer workspace);
 /* The same with the gradients of grad_scale * loss: G = softmax(z) - onehot(label) (0 for a row that
  * does not count), dx (F32 or BF16 [n][dim]) = grad_scale / count * G w and dw (F32 or BF16
- * [vocab][dim], every row written) = grad_scale / count * G^T x.  G is rounded to bf16 for these products,
+ * [vocab][dim], every row written) = grad_scale / count * G^T x (every row of x takes part, those that do
+ * not count with 0: they must be finite).  G is rounded to bf16 for these products,
  * as every gradient that a bf16 GEMM of this library takes; they accumulate in f32 and are rounded once.
  * The vocabulary is worked on in pieces of `piece` columns (rounded up to a multiple of 256, the pieces
- * then made alike): the workspace holds 2 n piece bytes for one of them, and more pieces take more
- * operations (all but one form their logits twice).  piece 0: as many columns as 2 n piece <= 1 GiB allows.
+ * then made alike, of 2^24 columns at most): the workspace holds 2 n piece bytes for one of them, and more
+ * pieces take more operations (all but one form their logits twice).  piece 0: as many columns as
+ * 2 n piece <= 1 GiB allows.  Where dim is no multiple of 8 (of 64, for large products), the workspace also holds
+ * copies of x and w in whole units.
  * The same bits on every call with the same piece.  workspace:
  * vdsl_linear_xent_workspace_bytes(n, vocab, dim, piece, 1) bytes of any contents (two calls that overlap
  * in time need two). */

@@ -252,6 +252,59 @@ int main(void) {
     for (size_t k = 0; k < sizeof bufs / sizeof bufs[0]; ++k) EXPECT_OK(vdsl_buffer_free(bufs[k]));
   }
 
+  /* ---- op class 6: embedding, layer norm, cross entropy over a vocabulary ---- */
+  {
+    const int64_t n = 40, dim = 24, vocab = 300;
+    vdsl_buffer x = alloc(d, (size_t)(n * dim * 2)), w = alloc(d, (size_t)(vocab * dim * 2));
+    vdsl_buffer ids = alloc(d, (size_t)n * 4), dx = alloc(d, (size_t)(n * dim * 4)), dw = alloc(d, (size_t)(vocab * dim * 4));
+    vdsl_buffer mean = alloc(d, (size_t)n * 4), rstd = alloc(d, (size_t)n * 4), loss = alloc(d, 4);
+    int32_t id[40];
+    for (int k = 0; k < 40; ++k) id[k] = 7 * k - 1; /* the first is no row */
+    EXPECT_OK(vdsl_buffer_write(q, ids, 0, id, sizeof id));
+    EXPECT_OK(vdsl_queue_sync(q));
+    fill_bf16(q, w, (size_t)(vocab * dim));
+    EXPECT_OK(vdsl_op_embedding_fwd(q, n, dim, vocab, VDSL_BF16, w, ids, 2.0f, VDSL_BF16, x));
+    EXPECT_ERR(vdsl_op_embedding_fwd(q, n, kHuge, vocab, VDSL_BF16, w, ids, 2.0f, VDSL_BF16, x));
+    EXPECT_ERR(vdsl_op_embedding_fwd(q, n, dim, vocab + 1, VDSL_BF16, w, ids, 2.0f, VDSL_BF16, x));
+    size_t ws = 0;
+    EXPECT_ERR(vdsl_embedding_bwd_workspace_bytes(-1, vocab, dim, &ws));
+    EXPECT_ERR(vdsl_embedding_bwd_workspace_bytes(n, kHuge, dim, &ws));
+    EXPECT_ERR(vdsl_embedding_bwd_workspace_bytes(n, vocab, dim, NULL));
+    EXPECT_OK(vdsl_embedding_bwd_workspace_bytes(n, vocab, dim, &ws));
+    vdsl_buffer we = alloc(d, ws ? ws : 16);
+    EXPECT_OK(vdsl_op_embedding_bwd(q, n, dim, vocab, ids, VDSL_BF16, x, 2.0f, dw, we));
+    EXPECT_ERR(vdsl_op_embedding_bwd(q, n, dim, vocab, ids, VDSL_BF16, x, 2.0f, dw, NULL));
+    EXPECT_ERR(vdsl_op_embedding_bwd(q, n, dim, vocab, ids, VDSL_I8, x, 2.0f, dw, we));
+    EXPECT_OK(vdsl_op_layer_norm_fwd(q, n, dim, VDSL_BF16, x, VDSL_F32, NULL, NULL, 1e-5f, VDSL_F32, dx, mean, rstd));
+    EXPECT_ERR(vdsl_op_layer_norm_fwd(q, n, dim, VDSL_BF16, x, VDSL_F32, NULL, NULL, -1.0f, VDSL_F32, dx, mean, rstd));
+    EXPECT_ERR(vdsl_op_layer_norm_fwd(q, kHuge, dim, VDSL_BF16, x, VDSL_F32, NULL, NULL, 1e-5f, VDSL_F32, dx, mean, rstd));
+    EXPECT_ERR(vdsl_layer_norm_bwd_workspace_bytes(kHuge, kHuge, &ws));
+    EXPECT_OK(vdsl_layer_norm_bwd_workspace_bytes(n, dim, &ws));
+    vdsl_buffer wn = alloc(d, ws ? ws : 16);
+    EXPECT_OK(vdsl_op_layer_norm_bwd(q, n, dim, VDSL_F32, dx, VDSL_BF16, x, VDSL_F32, NULL, mean, rstd, VDSL_F32, dx, mean, NULL, wn));
+    EXPECT_ERR(vdsl_op_layer_norm_bwd(q, n, dim, VDSL_F32, dx, VDSL_BF16, x, VDSL_F32, NULL, mean, rstd, VDSL_F32, dx, mean, NULL, NULL));
+    EXPECT_ERR(vdsl_linear_xent_workspace_bytes(n, 0, dim, 0, 1, &ws));
+    EXPECT_ERR(vdsl_linear_xent_workspace_bytes(n, vocab, dim, -1, 1, &ws));
+    EXPECT_ERR(vdsl_linear_xent_workspace_bytes(n, kHuge, dim, 0, 1, &ws));
+    EXPECT_OK(vdsl_linear_xent_workspace_bytes(n, vocab, dim, INT64_MAX, 1, &ws));
+    EXPECT_OK(vdsl_linear_xent_workspace_bytes(n, vocab, dim, 256, 1, &ws));
+    vdsl_buffer wx = alloc(d, ws);
+    EXPECT_OK(vdsl_op_linear_xent_fwd_bwd(q, n, dim, vocab, x, w, ids, 256, 1.0f, loss, NULL, NULL, VDSL_BF16, dx, VDSL_F32, dw, wx));
+    EXPECT_ERR(vdsl_op_linear_xent_fwd_bwd(q, n, dim, vocab, x, w, ids, 256, 1.0f, loss, NULL, NULL, VDSL_BF16, x, VDSL_F32, dw, wx));
+    EXPECT_ERR(vdsl_op_linear_xent_fwd_bwd(q, n, dim, vocab, x, w, ids, 256, 1.0f, loss, NULL, NULL, VDSL_BF16, dx, VDSL_F32, dw, loss));
+    EXPECT_OK(vdsl_linear_xent_workspace_bytes(n, vocab, dim, 0, 0, &ws));
+    vdsl_buffer wf = alloc(d, ws);
+    EXPECT_OK(vdsl_op_linear_xent_fwd(q, n, dim, vocab, x, w, ids, loss, NULL, NULL, wf));
+    EXPECT_ERR(vdsl_op_linear_xent_fwd(q, n, dim, vocab, x, w, ids, NULL, NULL, NULL, wf));
+    EXPECT_OK(vdsl_queue_sync(q));
+    float out = NAN;
+    EXPECT_OK(vdsl_buffer_read(q, loss, 0, &out, sizeof out));
+    EXPECT_OK(vdsl_queue_sync(q));
+    if (!isfinite(out)) { printf("FAIL linear_xent loss %g\n", out); ++g_fails; }
+    vdsl_buffer bufs[] = {x, w, ids, dx, dw, mean, rstd, loss, we, wn, wx, wf};
+    for (size_t k = 0; k < sizeof bufs / sizeof bufs[0]; ++k) EXPECT_OK(vdsl_buffer_free(bufs[k]));
+  }
+
   /* ---- graphs and events ---- */
   vdsl_graph g = NULL;
   EXPECT_ERR(vdsl_graph_end(q, &g)); /* not recording */

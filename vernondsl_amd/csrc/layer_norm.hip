@@ -394,7 +394,7 @@ int64_t bwd_blocks(int64_t rows, int64_t together, int64_t bytes) {
   const int64_t blocks = (rows + together - 1) / together;
   return blocks <= 256 ? blocks : std::min(most, std::max<int64_t>(256, blocks / 4));
 }
-int64_t bwd_most_blocks(int64_t rows, int64_t cols) { return bwd_blocks(rows, cols <= 1024 ? 4 : 1, 4 * cols); }
+int64_t bwd_most_blocks(int64_t rows, int64_t cols) { return bwd_blocks(rows, cols <= 1024 ? 4 : 1, 4 * std::min<int64_t>(cols, 1 << 24)); }
 
 bool float_type(int32_t t) { return t == VDSL_F32 || t == VDSL_BF16; }
 

@@ -703,8 +703,10 @@ int make_plan(int64_t n, int64_t vocab, int64_t dim, int64_t piece, bool backwar
   p.piece = p.pieces == 1 ? vocab : ceil_div(ceil_div(vocab, p.pieces), 256) * 256;
   p.pieces = ceil_div(vocab, p.piece);
   p.logits = logit_tiles(n, vocab, dim);
-  p.again = logit_tiles(n, p.piece, dim);
-  p.grads = grad_tiles(n, p.piece, dim);
+  if (backward) {
+    p.again = logit_tiles(n, p.piece, dim);
+    p.grads = grad_tiles(n, p.piece, dim);
+  }
   const bool wide = p.logits == kTilesWide || p.again == kTilesWide || p.grads == kTilesWide;
   p.ld = wide ? ceil_div(dim, 64) * 64 : ceil_div(dim, 8) * 8;
   p.group_cols = p.logits == kTilesWide ? 128 : rows_of(p.logits) / 2;
@@ -712,10 +714,10 @@ int make_plan(int64_t n, int64_t vocab, int64_t dim, int64_t piece, bool backwar
   const int64_t unit = p.grads == kTilesWide ? 256 : 8;
   p.ldg = ceil_div(p.piece, unit) * unit;
   p.g_rows = p.grads == kTilesWide ? ceil_div(n, 64) * 64 : n;
-  if (p.grads == kTilesWide) {
+  if (backward && p.grads == kTilesWide) {
     p.splits = wide_splits(n, dim, p.piece);
     p.dw_splits = wide_splits(p.piece, dim, n);
-  } else {
+  } else if (backward) {
     // One launch: splits of as many stages as two blocks a CU come to, but of 12 or more, since each split's sums are
     // written and read again (us with 12 and with 5: 16 x 512, 5003 20.3, 22.3; 300 x 1000, 5003 37.6, 39.6; 128 x 512,
     // 8192 27.8, 33.6).
@@ -725,7 +727,7 @@ int make_plan(int64_t n, int64_t vocab, int64_t dim, int64_t piece, bool backwar
     p.splits = static_cast<int>(std::clamp<int64_t>(ceil_div(x_stages, share), 1, 64));
     p.dw_splits = static_cast<int>(std::clamp<int64_t>(ceil_div(w_stages, share), 1, 64));
   }
-  p.sum = p.pieces > 1 || p.splits > 1;
+  p.sum = p.pieces > 1 || p.splits > 1;  // (forward: one piece, no splits)
   size_t at = 0;
   bool fits = true;
   const auto take = [&](int64_t a, int64_t b, int64_t c) {

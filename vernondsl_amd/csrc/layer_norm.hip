@@ -7,9 +7,11 @@
 //   dgamma_j = sum over rows of dy_j h_j,  dbeta_j = sum over rows of dy_j.
 //
 // All of it in f32, the outputs rounded once to their types.  Both passes are bound by HBM: x (and dy) are
-// read once and held in registers as units of U consecutive elements, y (dx) is written once.  A wave
+// read once and held in registers as units of U consecutive elements, y (dx) is written once: 16384 x 4096 f32 to
+// bf16 70 us (5.8 TB/s), bf16 to bf16 42 (6.4); the backward pass in bf16 78 (5.2, 4.9 of it the second kernel);
+// 300 x 1001 in f32, backward, 9 (two launches).  A wave
 // holds a row of up to 1024 columns, 256 lanes one of up to 4096, 1024 lanes one of up to 16384; wider
-// rows are read again for each step (row_stream kernels).  A block walks over rows and loads the next
+// rows are read again for each step (4096 x 16500 in bf16 103 us, 49 at 16384 columns).  A block walks over rows and loads the next
 // row before it works on the present one, so gamma, beta and, in the backward pass, the sums for dgamma
 // and dbeta stay in its lanes' registers.  Those sums go to a workspace, one row of it per block, and a
 // second kernel adds the blocks' rows in a fixed order: no atomics, the same bits every time.
@@ -197,7 +199,7 @@ __global__ __launch_bounds__(S::kThreads) void layer_norm_bwd_rows(const void* d
   const int t = threadIdx.x % S::kLanes, slot = threadIdx.x / S::kLanes;
   const int64_t step = static_cast<int64_t>(gridDim.x) * S::kRows;
   int64_t row = static_cast<int64_t>(blockIdx.x) * S::kRows + slot;
-  constexpr bool AHEAD = NV * U * S::kThreads < 16384;  // 1024 lanes of 16 columns have no registers for another row
+  constexpr bool AHEAD = NV * U * S::kThreads < 16384;  // 1024 lanes of 16 columns have no registers for another row, or gamma
   float ga[NV][U], dg[NV][U], db[NV][U], nx[NV][U], ny[NV][U];
   float nmean = 0.0f, nrstd = 0.0f;
   const auto load = [&](int64_t at) {
@@ -207,7 +209,7 @@ __global__ __launch_bounds__(S::kThreads) void layer_norm_bwd_rows(const void* d
     nrstd = rstd[at];
   };
   if (AHEAD && row < rows) load(row);
-  load_params<S>(gamma, param_dt, cols, t, 1.0f, ga);
+  if (AHEAD) load_params<S>(gamma, param_dt, cols, t, 1.0f, ga);
 #pragma unroll
   for (int k = 0; k < NV; ++k)
 #pragma unroll
@@ -215,7 +217,11 @@ __global__ __launch_bounds__(S::kThreads) void layer_norm_bwd_rows(const void* d
   const float inv_cols = 1.0f / static_cast<float>(cols);
   int parity = 0;
   for (; row < rows; row += step) {
-    if (!AHEAD) load(row);
+    if (!AHEAD) {
+      asm volatile("" ::: "memory");  // gamma again for each row, not kept through the loop
+      load(row);
+      load_params<S>(gamma, param_dt, cols, t, 1.0f, ga);
+    }
     float h[NV][U], d[NV][U];
     const float r = nrstd;
 #pragma unroll
@@ -383,14 +389,15 @@ int row_shape(int64_t cols, Go&& go, Wide&& wide) {
   return wide();
 }
 
-// Blocks of the backward pass, each of which leaves a partial row: so many that a CU has about 32 KiB of rows on their
-// way, 256 to 1024 (us of 256, 512 and 1024, rows of bf16: 65536 x 256 51.2, 35.5, 29.4; 32768 x 2048 168, 107, 81.5;
-// 16384 x 4096 113, 78.0, 94.2; 8192 x 8192 86.1, 90.9, 101; of f32: 16384 x 4096 147, 161, 164), but of four rows
+// Blocks of the backward pass, each of which leaves a partial row: so many that a CU has 24 to 48 KiB of rows on their
+// way (us of 256, 512 and 1024, rows of bf16: 65536 x 256 51.2, 35.5, 29.4; 32768 x 2048 168, 107, 81.5;
+// 16384 x 4096 113, 78.0, 94.2; 8192 x 8192 86.1, 90.9, 101; of f32: 16384 x 4096 147, 161, 164; x of f32 and dy of
+// bf16: 16384 x 4096 129, 102), but of four rows
 // or more where there are more than 256 (2048 x 2048, bf16, in 1024 and in 512 blocks 18.8, 14.3; 512 x 8192 in 512 and
 // in 256 22.7, 17.6).
 // together: the rows a block holds at a time; bytes: of a row of x and one of dy.
 int64_t bwd_blocks(int64_t rows, int64_t together, int64_t bytes) {
-  const int64_t most = std::clamp<int64_t>(((int64_t{8} << 20) / (together * bytes) + 128) / 256 * 256, 256, 1024);
+  const int64_t most = together * bytes <= 8192 ? 1024 : together * bytes <= 24576 ? 512 : 256;
   const int64_t blocks = (rows + together - 1) / together;
   return blocks <= 256 ? blocks : std::min(most, std::max<int64_t>(256, blocks / 4));
 }

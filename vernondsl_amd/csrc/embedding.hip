@@ -594,7 +594,9 @@ extern "C" int vdsl_op_embedding_bwd(vdsl_queue q, int64_t n, int64_t dim, int64
                        dim3(256), 0, s, sorted, order, dy->ptr, count, dim, vocab, p.chunk, l, static_cast<int>(place_blocks), places,
                        partials);
     VDSL_TRY(check_launch("embedding_chunk_kernel"));
-    const auto rows_kernel = vocab * dim * 4 >= kStreamBytes ? embedding_bwd_kernel<DYT, U, NV, true, true> : embedding_bwd_kernel<DYT, U, NV, true, false>;
+    const auto rows_kernel = vocab * dim * 4 >= kStreamBytes
+                                 ? embedding_bwd_kernel<DYT, U, NV, true, true>
+                                 : embedding_bwd_kernel<DYT, U, NV, true, false>;
     hipLaunchKernelGGL(rows_kernel, grid, dim3(256), 0, s, sorted, order, dy->ptr, places, partials, p.chunk,
                        static_cast<float*>(dtable->ptr), count, dim, vocab, scale, l);
     return check_launch("embedding_bwd_kernel");

@@ -675,9 +675,9 @@ int vdsl_op_linear_xent_fwd(vdsl_queue q, int64_t n, int64_t dim, int64_t vocab,
  * [vocab][dim], every row written) = grad_scale / count * G^T x (every row of x takes part, those that do
  * not count with 0: they must be finite).  G is rounded to bf16 for these products,
  * as every gradient that a bf16 GEMM of this library takes; they accumulate in f32 and are rounded once.
- * The vocabulary is worked on in pieces of `piece` columns (rounded up to a multiple of 256, the pieces
- * then made alike, of 2^24 columns at most): the workspace holds 2 n piece bytes for one of them, and more
- * pieces take more operations (all but one form their logits twice).  piece 0: as many columns as
+ * The vocabulary is worked on in pieces of `piece` columns (4 MiB / (2 n) if that is more, rounded up to a
+ * multiple of 256, the pieces then made alike, of 2^24 columns at most): the workspace holds 2 n piece bytes
+ * for one of them, and more pieces take more operations (all but one form their logits twice).  piece 0: as many columns as
  * 2 n piece <= 1 GiB allows.  Where dim is no multiple of 8 (of 64, for large products), the workspace also holds
  * copies of x and w in whole units.
  * The same bits on every call with the same piece.  workspace:

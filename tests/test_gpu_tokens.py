@@ -492,6 +492,32 @@ def test_linear_xent_gradients_on_256_tiles(q, own, n, dim, vocab, piece, gt):
     check_xent(q, own, *xent_input(np.random.default_rng(n), n, dim, vocab), piece=piece, gt=gt)
 
 
+# smaller tiles in pieces: enough rows that the pieces are not raised (4 MiB); ragged last pieces, dims that are copied
+@pytest.mark.parametrize("n,dim,vocab,piece,gt", [(8300, 64, 700, 256, "bf16"), (4200, 71, 1300, 512, "f32"), (4200, 72, 1030, 512, "bf16"),
+                                                  (9001, 16, 513, 256, "f32")])
+def test_linear_xent_pieces_on_smaller_tiles(q, own, n, dim, vocab, piece, gt):
+    few, whole = (kernels.linear_xent_workspace_bytes(n, vocab, dim, piece=p) for p in (piece, 0))
+    assert few != whole
+    check_xent(q, own, *xent_input(np.random.default_rng(n), n, dim, vocab), piece=piece, gt=gt)
+
+
+def test_linear_xent_rows_without_softmax_in_pieces(q, own):
+    """NaN, +inf and rows of -inf alone in a call of three pieces: their own losses and gradients are NaN, no other's."""
+    n, dim, vocab = 8300, 64, 700
+    r = np.random.default_rng(17)
+    x, w, labels = xent_input(r, n, dim, vocab)
+    labels[:] = np.arange(n) % vocab
+    w[:, 5] = np.abs(w[:, 5]) + 1.0
+    x[7, 5], x[8, 5], x[8000, 3] = -np.inf, np.inf, np.nan
+    tx, tw, tl = own.put(x, "bf16"), own.put(bf16(w), "bf16"), own.put(labels, "i32")
+    loss, each, dx, dw = (own.empty(s, "f32") for s in ((1,), (n,), (n, dim), (vocab, dim)))
+    kernels.linear_xent_fwd_bwd(q, tx, tw, tl, loss, dx, dw, row_loss=each, piece=256,
+                                workspace=own.scratch(kernels.linear_xent_workspace_bytes(n, vocab, dim, piece=256)))
+    bad = np.isin(np.arange(n), (7, 8, 8000))
+    assert np.array_equal(np.isnan(each.numpy(q)), bad)
+    assert np.array_equal(np.isnan(dx.numpy(q)).all(1), bad) and np.array_equal(np.isnan(dx.numpy(q)).any(1), bad)
+
+
 # long sums for the weights' gradient in few tiles
 @pytest.mark.parametrize("n,dim,vocab,piece", [(2000, 72, 300, 0), (1500, 71, 130, 0), (1100, 64, 700, 256)])
 def test_linear_xent_many_rows_few_logits(q, own, n, dim, vocab, piece):

@@ -19,7 +19,7 @@
 //
 // 8192 x 4096, vocabulary 32768, in one piece: logits 1600 to 1720 us on the power-limited card (76% of the cycles in
 // MFMAs, at 1.6 GHz), the rows' pass 188 (537 MB of codes in, as much of G out), dx 1490 to 1580, dw 1560 to 1670.
-// 300 x 1000, 5003: 38 in one piece of five launches, 67 in three pieces of eight.  16 x 512, 5003: logits 5.5, rows 4,
+// 300 x 1000, 5003: 39 in four launches, 67 in three pieces and eight.  16 x 512, 5003: logits 5.5, rows 4,
 // both gradients 8, joining dx's splits 4.
 
 #include <algorithm>

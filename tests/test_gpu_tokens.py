@@ -118,6 +118,8 @@ def skewed(r, n, vocab):
     (1, 1, 1, "skewed"), (1, 8, 300, "skewed"), (5, 3, 2, "skewed"), (300, 1001, 503, "skewed"), (1000, 64, 5003, "skewed"),
     (4099, 20, 65, "skewed"), (257, 40, 4, "one"), (2500, 5, 1, "one"), (2500, 72, 700, "one"), (64, 16, 40, "none"),
     (0, 24, 33, "skewed"), (20000, 33, 3001, "skewed"), (20000, 12, 100000, "skewed"), (17000, 8, 30, "one"), (130, 4100, 10, "skewed"),
+    (1024, 7, 300, "skewed"), (1025, 7, 300, "skewed"), (1024, 64, 3, "one"), (40000, 12, 3001, "skewed"), (33000, 5, 100000, "skewed"),
+    (33000, 4, 200, "skewed"), (33000, 1, 17000000, "skewed"), (270000, 4, 50, "one"),
 ])
 @pytest.mark.parametrize("dt", ["f32", "bf16"])
 def test_embedding_bwd(q, own, n, dim, vocab, ids_of, dt):
@@ -621,6 +623,7 @@ def test_refusals(dev, q, own):
                                        "thinf": ((4, 4), "f32"), "thindw": ((9, 4), "f32")}.items()}
     ro = own.keep(Tensor(dev, (4, 16), "f32", "uniform_constant"))
     ws = own.scratch(1 << 16)
+    many = own.empty((1025,), "i32"), own.empty((1025, 16), "f32")
 
     def status(fn, *a, **kw):
         with pytest.raises(_lib.VdslError) as e:
@@ -642,8 +645,8 @@ def test_refusals(dev, q, own):
     assert status(kernels.embedding_fwd, t["w"], t["ids"], t["bytes"]) == unsupported
     assert status(kernels.embedding_fwd, t["w"], t["ids"], ro) == invalid
     assert status(kernels.embedding_bwd, t["ids"], t["bytes"], t["dw"], workspace=ws) == unsupported
-    assert status(kernels.embedding_bwd, t["ids"], t["f"], t["dw"]) == handle
-    assert status(kernels.embedding_bwd, t["ids"], t["f"], t["dw"], workspace=t["small"]) == shape
+    assert status(kernels.embedding_bwd, *many, t["dw"]) == handle  # (1024 positions need no workspace)
+    assert status(kernels.embedding_bwd, *many, t["dw"], workspace=t["small"]) == shape
     assert status(kernels.layer_norm_fwd, t["x"], None, None, t["bytes"]) == unsupported
     assert status(kernels.layer_norm_fwd, t["x"], None, None, t["f"], eps=-1.0) == invalid
     assert status(kernels.layer_norm_fwd, t["x"], None, None, t["f"], eps=float("nan")) == invalid

@@ -50,16 +50,15 @@ __global__ __launch_bounds__(256) void embedding_zero_kernel(uint16_t* __restric
 }
 
 // ---- positions sorted by token -------------------------------------------------------------------
-// Every row's places [x, y) among the sorted positions, none at first (null: not wanted).
+// Every row's places [x, y) among the sorted positions, none at first.
 __device__ __forceinline__ void clear_places(int2* __restrict__ places, int64_t vocab) {
-  if (!places) return;
   const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.x;
   for (int64_t v = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; v < vocab; v += step) places[v] = make_int2(0, 0);
 }
 
-// Up to 32768 positions.  Of up to kRankTile, position i goes to place #{j : id_j < id_i} + #{j < i : id_j = id_i}.  A block
+// Up to 32768 positions, in tiles of kRankTile.  In a tile position i goes to place #{j : id_j < id_i} + #{j < i : id_j = id_i}.  A block
 // ranks 64 positions, one a lane, its 16 waves a share of the ids each.  Ids are compared as unsigned
-// numbers, so those that are no row come last.  More are ranked so in tiles, and a second kernel
+// numbers, so those that are no row come last.  A second kernel
 // adds to an element's rank what the other tiles have before it, a binary search in each.  Us of a gradient of 256
 // columns, vocabulary 32768, sorted so and by radix passes: n 4096 20.7, 30.9; 16384 22.1, 31.2; 32768 27.4, 34.3; 65536
 // 47.8, 40.3.
@@ -215,17 +214,6 @@ __global__ __launch_bounds__(256) void embedding_radix_kernel(const int32_t* __r
 }
 
 // ---- the rows' sums ------------------------------------------------------------------------------
-// The first of the n sorted places whose token is not below v.
-__device__ __forceinline__ int lower_bound(const uint32_t* sorted, int n, uint32_t v) {
-  int lo = 0, hi = n;
-  while (lo < hi) {
-    const int mid = lo + ((hi - lo) >> 1);
-    if (sorted[mid] < v) lo = mid + 1;
-    else hi = mid;
-  }
-  return lo;
-}
-
 // A wave of the following kernels works on one row at a time (several waves share a wide one), so where a
 // row is and which positions it sums is the same for all of its lanes and stays in scalar registers.
 
@@ -359,48 +347,77 @@ __global__ __launch_bounds__(256) void embedding_chunk_kernel(const uint32_t* __
     if (at.any[u]) store_whole<VDSL_F32, U>(partials, k * dim + at.c[u], acc[u]);
 }
 
-// dtable rows: 2^log_l lanes (64 to 256) to a row, each NV units of U columns; blockIdx.y: strips of columns.  CHUNKS:
-// the rows' places and the chunks' sums come from embedding_chunk_kernel; otherwise the sorted tokens (at
-// most kFewPositions) are searched in LDS.
-constexpr int kFewPositions = 512;
-
-template <int DYT, int U, int NV, bool CHUNKS, bool STREAM>
-__global__ __launch_bounds__(256) void embedding_bwd_kernel(const uint32_t* __restrict__ sorted, const int32_t* __restrict__ order,
-                                                            const void* __restrict__ dy, const int2* __restrict__ places,
-                                                            const float* __restrict__ partials, int chunk,
-                                                            float* __restrict__ dtable, int n, int64_t dim, int64_t vocab,
-                                                            float scale, int log_l) {
-  const int64_t v = (block_index() << (8 - log_l)) + uniform(threadIdx.x >> log_l);
-  int e0 = 0, e1 = 0;
-  if constexpr (CHUNKS) {
-    if (v >= vocab) return;
-    const int2 place = places[v];
-    e0 = place.x;
-    e1 = place.y;
-  } else {
-    __shared__ uint32_t tokens[kFewPositions];
-    for (int e = threadIdx.x; e < n; e += 256) tokens[e] = sorted[e];
-    __syncthreads();
-    if (v >= vocab) return;
-    e0 = uniform(lower_bound(tokens, n, static_cast<uint32_t>(v)));
-    e1 = uniform(lower_bound(tokens, n, static_cast<uint32_t>(v) + 1));
-  }
-  const LaneColumns<U, NV> at(log_l, dim);
-  const auto term = [&](int e) { return order[e]; };
-  float acc[NV][U] = {};
-  if (CHUNKS && e1 - e0 >= 2 * chunk) {  // whole chunks lie inside: the places around them, and their sums between
-    const int k0 = (e0 + chunk - 1) / chunk, k1 = e1 / chunk;
-    add_range<DYT, U, NV, kInFlight<DYT>>(dy, dim, at, e0, k0 * chunk, acc, term);
-    add_range<VDSL_F32, U, NV, 2>(partials, dim, at, k0, k1, acc, [&](int h) { return h; });
-    e0 = k1 * chunk;
-  }
-  add_range<DYT, U, NV, kInFlight<DYT>>(dy, dim, at, e0, e1, acc, term);
+// scale acc as row v of dtable.
+template <int U, int NV, bool STREAM>
+__device__ __forceinline__ void store_row(float* __restrict__ dtable, int64_t v, int64_t dim, const LaneColumns<U, NV>& at, float scale,
+                                          float (&acc)[NV][U]) {
 #pragma unroll
   for (int u = 0; u < NV; ++u) {
 #pragma unroll
     for (int j = 0; j < U; ++j) acc[u][j] *= scale;
     if (at.any[u]) store_whole<VDSL_F32, U, STREAM>(dtable, v * dim + at.c[u], acc[u]);
   }
+}
+
+// dtable rows from the sorted positions: 2^log_l lanes (64 to 256) to a row, each NV units of U columns; blockIdx.y:
+// strips of columns.
+template <int DYT, int U, int NV, bool STREAM>
+__global__ __launch_bounds__(256) void embedding_bwd_kernel(const int32_t* __restrict__ order, const void* __restrict__ dy,
+                                                            const int2* __restrict__ places, const float* __restrict__ partials,
+                                                            int chunk, float* __restrict__ dtable, int64_t dim, int64_t vocab,
+                                                            float scale, int log_l) {
+  const int64_t v = (block_index() << (8 - log_l)) + uniform(threadIdx.x >> log_l);
+  if (v >= vocab) return;
+  const int2 place = places[v];
+  int e0 = place.x;
+  const int e1 = place.y;
+  const LaneColumns<U, NV> at(log_l, dim);
+  const auto term = [&](int e) { return order[e]; };
+  float acc[NV][U] = {};
+  if (e1 - e0 >= 2 * chunk) {  // whole chunks lie inside: the places around them, and their sums between
+    const int k0 = (e0 + chunk - 1) / chunk, k1 = e1 / chunk;
+    add_range<DYT, U, NV, kInFlight<DYT>>(dy, dim, at, e0, k0 * chunk, acc, term);
+    add_range<VDSL_F32, U, NV, 2>(partials, dim, at, k0, k1, acc, [&](int h) { return h; });
+    e0 = k1 * chunk;
+  }
+  add_range<DYT, U, NV, kInFlight<DYT>>(dy, dim, at, e0, e1, acc, term);
+  store_row<U, NV, STREAM>(dtable, v, dim, at, scale, acc);
+}
+
+// The same of few positions, which need no sort: each row's wave looks through all of them.  Us of uniform ids, so and
+// sorted: 300 of 1001 columns, vocabulary 5003 5.8, 11.6; 512 of 64, 32768 8.2, 20.6; 1000 of 1001, 5003 6.4, 13.6; ids as
+// frequent as words: 1000 of 1001, 5003 19.1, 23.5, but 2000 34.4, 26.6.
+constexpr int kFewPositions = 1024;
+
+template <int DYT, int U, int NV>
+__global__ __launch_bounds__(256) void embedding_bwd_few_kernel(const int32_t* __restrict__ ids, const void* __restrict__ dy,
+                                                                float* __restrict__ dtable, int n, int64_t dim, int64_t vocab,
+                                                                float scale, int log_l) {
+  __shared__ int32_t tokens[kFewPositions];
+  __shared__ uint16_t found[4][kFewPositions];
+  for (int e = threadIdx.x; e < (n + 255) / 256 * 256; e += 256) tokens[e] = e < n ? ids[e] : -1;
+  __syncthreads();
+  const int64_t v = (block_index() << (8 - log_l)) + uniform(threadIdx.x >> log_l);
+  if (v >= vocab) return;
+  const int lane = threadIdx.x & 63;
+  uint16_t* const mine = found[uniform(threadIdx.x >> 6)];
+  int count = 0;
+  for (int e0 = 0; e0 < n; e0 += 256) {
+    bool hit[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) hit[k] = tokens[e0 + 64 * k + lane] == static_cast<int32_t>(v);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint64_t hits = __ballot(hit[k]);
+      if (hit[k]) mine[count + __popcll(hits & ((uint64_t{1} << lane) - 1))] = static_cast<uint16_t>(e0 + 64 * k + lane);
+      count += __popcll(hits);
+    }
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  const LaneColumns<U, NV> at(log_l, dim);
+  float acc[NV][U] = {};
+  add_range<DYT, U, NV, kInFlight<DYT>>(dy, dim, at, 0, count, acc, [&](int k) { return static_cast<int>(mine[k]); });
+  store_row<U, NV, false>(dtable, v, dim, at, scale, acc);
 }
 
 bool float_type(int32_t t) { return t == VDSL_F32 || t == VDSL_BF16; }
@@ -486,8 +503,7 @@ int grad_plan(int64_t n, int64_t vocab, int64_t dim, GradPlan& p) {
   p.tiles = (n + p.tile - 1) / p.tile;
   // n / chunk chunks, and up to 2 chunk places of a token outside them.  Us of 512 columns, vocabulary 32768, ids as
   // frequent as words, in chunks of 16, 32, 64, 128: n 4096 26.9, 31.3, 40.3, 51.8; 16384 36.1, 34.6, 42.5, 59.1; 65536
-  // 93.6, 73.9, 69.3, 88.5; 262144 297, 201, 164, 152.  None at all (1001 columns, vocabulary 5003): n 512 17.5, in
-  // chunks 19.1; 1000 24.9, 20.6.
+  // 93.6, 73.9, 69.3, 88.5; 262144 297, 201, 164, 152.
   p.chunk = 0;
   if (n > kFewPositions)
     for (p.chunk = 16; int64_t{16} * p.chunk * p.chunk < n;) p.chunk *= 2;
@@ -499,16 +515,12 @@ int grad_plan(int64_t n, int64_t vocab, int64_t dim, GradPlan& p) {
     else at = (at + 255) / 256 * 256;
     return from;
   };
-  p.sorted = take(n, 4);
-  p.order = take(n, 4);
-  if (n > kRankTile) {
+  if (p.radix) p.hist = take(p.passes * p.tiles, 4 * kDigits);
+  if (p.chunk) {
+    p.sorted = take(n, 4);
+    p.order = take(n, 4);
     p.keys2 = take(n, 4);
     p.order2 = take(n, 4);
-  }
-  if (p.radix) {
-    p.hist = take(p.passes * p.tiles, 4 * kDigits);
-  }
-  if (p.chunk) {
     p.places = take(vocab, 8);
     p.partials = take(n / p.chunk, nbytes(dim, 4) == kSizeOverflow ? -1 : dim * 4);
   }
@@ -568,16 +580,13 @@ extern "C" int vdsl_op_embedding_bwd(vdsl_queue q, int64_t n, int64_t dim, int64
                          k + 1 < p.passes ? h + p.tiles * kDigits : nullptr, second ? keys2 : sorted, second ? order2 : order);
       VDSL_TRY(check_launch("embedding_radix_kernel"));
     }
-  } else if (n) {
+  } else if (p.chunk) {
     const dim3 blocks(static_cast<unsigned>((n + 63) / 64));
-    const bool merge = n > kRankTile;
-    hipLaunchKernelGGL(embedding_rank_kernel, blocks, dim3(1024), 0, s, id, count, merge ? keys2 : sorted, merge ? order2 : order, places,
+    hipLaunchKernelGGL(embedding_rank_kernel, blocks, dim3(1024), 0, s, id, count, keys2, order2, places,
                        vocab);
     VDSL_TRY(check_launch("embedding_rank_kernel"));
-    if (merge) {
-      hipLaunchKernelGGL(embedding_merge_kernel, blocks, dim3(1024), 0, s, keys2, order2, count, sorted, order);
-      VDSL_TRY(check_launch("embedding_merge_kernel"));
-    }
+    hipLaunchKernelGGL(embedding_merge_kernel, blocks, dim3(1024), 0, s, keys2, order2, count, sorted, order);
+    VDSL_TRY(check_launch("embedding_merge_kernel"));
   }
   float* const partials = reinterpret_cast<float*>(ws + p.partials);
   const auto go = [&](auto dyt, auto u, auto units_a_lane) {
@@ -585,9 +594,9 @@ extern "C" int vdsl_op_embedding_bwd(vdsl_queue q, int64_t n, int64_t dim, int64
     const int64_t rows = 256 >> l;
     const dim3 grid = block_grid((vocab + rows - 1) / rows, strips);
     if (!p.chunk) {
-      hipLaunchKernelGGL((embedding_bwd_kernel<DYT, U, NV, false, false>), grid, dim3(256), 0, s, sorted, order, dy->ptr, nullptr, nullptr, 0,
-                         static_cast<float*>(dtable->ptr), count, dim, vocab, scale, l);
-      return check_launch("embedding_bwd_kernel");
+      hipLaunchKernelGGL((embedding_bwd_few_kernel<DYT, U, NV>), grid, dim3(256), 0, s, id, dy->ptr, static_cast<float*>(dtable->ptr), count,
+                         dim, vocab, scale, l);
+      return check_launch("embedding_bwd_few_kernel");
     }
     const int64_t place_blocks = (n + 255) / 256, chunk_blocks = (n / p.chunk + (256 >> l) - 1) >> (8 - l);
     hipLaunchKernelGGL((embedding_chunk_kernel<DYT, U, NV>), dim3(static_cast<unsigned>(place_blocks + chunk_blocks), static_cast<unsigned>(strips)),
@@ -595,10 +604,10 @@ extern "C" int vdsl_op_embedding_bwd(vdsl_queue q, int64_t n, int64_t dim, int64
                        partials);
     VDSL_TRY(check_launch("embedding_chunk_kernel"));
     const auto rows_kernel = vocab * dim * 4 >= kStreamBytes
-                                 ? embedding_bwd_kernel<DYT, U, NV, true, true>
-                                 : embedding_bwd_kernel<DYT, U, NV, true, false>;
-    hipLaunchKernelGGL(rows_kernel, grid, dim3(256), 0, s, sorted, order, dy->ptr, places, partials, p.chunk,
-                       static_cast<float*>(dtable->ptr), count, dim, vocab, scale, l);
+                                 ? embedding_bwd_kernel<DYT, U, NV, true>
+                                 : embedding_bwd_kernel<DYT, U, NV, false>;
+    hipLaunchKernelGGL(rows_kernel, grid, dim3(256), 0, s, order, dy->ptr, places, partials, p.chunk, static_cast<float*>(dtable->ptr),
+                       dim, vocab, scale, l);
     return check_launch("embedding_bwd_kernel");
   };
   const auto pick = [&](auto dyt) {

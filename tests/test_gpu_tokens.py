@@ -289,6 +289,33 @@ def test_layer_norm_bwd(q, own, rows, cols, xt, dyt, dxt):
     assert np.array_equal(alone.numpy(q), dx.numpy(q))
 
 
+@pytest.mark.parametrize("rows,cols", [(1024, 9), (1025, 3), (1040, 700), (1030, 1500), (1030, 3001), (420, 5001), (240, 9000), (130, 16384),
+                                       (1000, 2097), (2000, 513)])
+@pytest.mark.parametrize("t", ["bf16", "f32"])
+def test_layer_norm_bwd_around_partial_rows(q, own, rows, cols, t):
+    """Sizes on both sides of the one that takes partial rows, for each shape of a row."""
+    test_layer_norm_bwd(q, own, rows, cols, t, t, t)
+
+
+def test_layer_norm_bwd_in_place_equals_apart(q, own):
+    """dx over dy's buffer takes partial rows where dx apart does not: the same dx, and sums within their bounds."""
+    r = np.random.default_rng(21)
+    rows, cols = 300, 1001
+    x, dy = norm_input(r, rows, cols, "f32"), r.standard_normal((rows, cols)).astype(np.float32)
+    mean = x.astype(np.float64).mean(1).astype(np.float32)
+    rstd = (1.0 / np.sqrt(x.astype(np.float64).var(1) + 1e-5)).astype(np.float32)
+    args = [own.put(x, "f32"), None, own.put(mean, "f32"), own.put(rstd, "f32")]
+    ws = own.scratch(kernels.layer_norm_bwd_workspace_bytes(rows, cols))
+    tdy, dx = own.put(dy, "f32"), own.empty((rows, cols), "f32")
+    dg, db = ([own.empty((cols,), "f32") for _ in range(2)] for _ in range(2))
+    kernels.layer_norm_bwd(q, tdy, *args, dx, dgamma=dg[0], dbeta=db[0], workspace=ws)
+    kernels.layer_norm_bwd(q, tdy, *args, tdy, dgamma=dg[1], dbeta=db[1], workspace=ws)
+    assert np.array_equal(dx.numpy(q), tdy.numpy(q))
+    h = (x.astype(np.float64) - mean[:, None]) * rstd[:, None]
+    assert np.all(np.abs(get(q, dg[0]) - get(q, dg[1])) <= 2 * ((rows + 8) * U * np.abs(dy * h)).sum(0))
+    assert np.all(np.abs(get(q, db[0]) - get(q, db[1])) <= 2 * ((rows + 4) * U * np.abs(dy)).sum(0))
+
+
 @pytest.mark.parametrize("cols", [90, 3000, 20000])
 def test_layer_norm_bwd_in_place_and_against_differences(q, own, cols):
     """dx over dy's own buffer; dx, dgamma and dbeta against central differences of the 64-bit forward pass

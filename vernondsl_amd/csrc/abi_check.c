@@ -280,8 +280,8 @@ int main(void) {
     EXPECT_ERR(vdsl_layer_norm_bwd_workspace_bytes(kHuge, kHuge, &ws));
     EXPECT_OK(vdsl_layer_norm_bwd_workspace_bytes(n, dim, &ws));
     vdsl_buffer wn = alloc(d, ws ? ws : 16);
-    EXPECT_OK(vdsl_op_layer_norm_bwd(q, n, dim, VDSL_F32, dx, VDSL_BF16, x, VDSL_F32, NULL, mean, rstd, VDSL_F32, dx, mean, NULL, wn));
-    EXPECT_ERR(vdsl_op_layer_norm_bwd(q, n, dim, VDSL_F32, dx, VDSL_BF16, x, VDSL_F32, NULL, mean, rstd, VDSL_F32, dx, mean, NULL, NULL));
+    EXPECT_OK(vdsl_op_layer_norm_bwd(q, n, dim, VDSL_F32, dx, VDSL_BF16, x, VDSL_F32, NULL, mean, rstd, VDSL_F32, dx, dw, NULL, wn));
+    EXPECT_ERR(vdsl_op_layer_norm_bwd(q, n, dim, VDSL_F32, dx, VDSL_BF16, x, VDSL_F32, NULL, mean, rstd, VDSL_F32, dx, dw, NULL, NULL));
     EXPECT_ERR(vdsl_linear_xent_workspace_bytes(n, 0, dim, 0, 1, &ws));
     EXPECT_ERR(vdsl_linear_xent_workspace_bytes(n, vocab, dim, -1, 1, &ws));
     EXPECT_ERR(vdsl_linear_xent_workspace_bytes(n, kHuge, dim, 0, 1, &ws));

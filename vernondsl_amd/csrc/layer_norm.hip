@@ -9,12 +9,13 @@
 // All of it in f32, the outputs rounded once to their types.  Both passes are bound by HBM: x (and dy) are
 // read once and held in registers as units of U consecutive elements, y (dx) is written once: 16384 x 4096 f32 to
 // bf16 70 us (5.8 TB/s), bf16 to bf16 42 (6.4); the backward pass in bf16 78 (5.2, 4.9 of it the second kernel);
-// 300 x 1001 in f32, backward, 9 (two launches).  A wave
+// 300 x 1001 in f32, backward, 5.9.  A wave
 // holds a row of up to 1024 columns, 256 lanes one of up to 4096, 1024 lanes one of up to 16384; wider
 // rows are read again for each step (4096 x 16500 in bf16 103 us, 49 at 16384 columns).  A block walks over rows and loads the next
 // row before it works on the present one, so gamma, beta and, in the backward pass, the sums for dgamma
 // and dbeta stay in its lanes' registers.  Those sums go to a workspace, one row of it per block, and a
-// second kernel adds the blocks' rows in a fixed order: no atomics, the same bits every time.
+// second kernel adds the blocks' rows in a fixed order: no atomics, the same bits every time.  Of few rows,
+// other blocks of the same launch form them.
 
 #include <algorithm>
 #include <type_traits>
@@ -187,17 +188,54 @@ __global__ __launch_bounds__(1024) void layer_norm_fwd_stream(const void* x, int
   }
 }
 
-// partials: [gridDim.x][2][cols], a block's sums for dgamma and dbeta over its rows (waves of one block
-// that hold rows of their own meet in LDS, in the order of the waves); null where neither is wanted.
-template <class S, int XT, int DYT, bool STREAM>
+// dgamma and dbeta of 16 columns from c0 on by one block: a sixteenth of its lanes to a column, their shares of the rows
+// added in f64 in order.
+template <int THREADS, int XT, int DYT>
+__device__ __forceinline__ void column_sums(const void* __restrict__ dy, const void* __restrict__ x, const float* __restrict__ mean,
+                                            const float* __restrict__ rstd, int64_t rows, int64_t cols, int64_t c0,
+                                            float* __restrict__ dgamma, float* __restrict__ dbeta) {
+  constexpr int SLOTS = THREADS / 16;
+  __shared__ float part[SLOTS][2][16];
+  const int column = threadIdx.x & 15, slot = threadIdx.x >> 4;
+  const int64_t c = c0 + column < cols ? c0 + column : cols - 1;
+  float g = 0.0f, b = 0.0f;
+#pragma unroll 8
+  for (int64_t row = slot; row < rows; row += SLOTS) {
+    const float d = load_elem<DYT>(dy, row * cols + c), h = (load_elem<XT>(x, row * cols + c) - mean[row]) * rstd[row];
+    g += d * h;
+    b += d;
+  }
+  part[slot][0][column] = g;
+  part[slot][1][column] = b;
+  __syncthreads();
+  if (threadIdx.x >= 32 || c0 + column >= cols) return;
+  double s = 0.0;
+#pragma unroll 8
+  for (int k = 0; k < SLOTS; ++k) s += part[k][slot][column];
+  float* const out = slot ? dbeta : dgamma;
+  if (out) out[c] = static_cast<float>(s);
+}
+
+// partials: [row_blocks][2][cols], a block's sums for dgamma and dbeta over its rows (waves of one block
+// that hold rows of their own meet in LDS, in the order of the waves); null where neither is wanted.  FEW: no partials, but
+// blocks past row_blocks that form dgamma and dbeta.
+template <class S, int XT, int DYT, bool STREAM, bool FEW>
 __global__ __launch_bounds__(S::kThreads) void layer_norm_bwd_rows(const void* dy, const void* __restrict__ x,
                                                                    const void* __restrict__ gamma, int param_dt,
                                                                    const float* __restrict__ mean, const float* __restrict__ rstd,
                                                                    void* dx, int dx_dt, float* __restrict__ partials, int64_t rows,
-                                                                   int64_t cols) {
+                                                                   int64_t cols, int row_blocks, float* __restrict__ dgamma,
+                                                                   float* __restrict__ dbeta) {
+  if constexpr (FEW) {
+    if (static_cast<int>(blockIdx.x) >= row_blocks) {
+      const int64_t c0 = int64_t{16} * (static_cast<int>(blockIdx.x) - row_blocks);
+      column_sums<S::kThreads, XT, DYT>(dy, x, mean, rstd, rows, cols, c0, dgamma, dbeta);
+      return;
+    }
+  }
   constexpr int U = S::kUnit, NV = S::kUnits;
   const int t = threadIdx.x % S::kLanes, slot = threadIdx.x / S::kLanes;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * S::kRows;
+  const int64_t step = static_cast<int64_t>(row_blocks) * S::kRows;
   int64_t row = static_cast<int64_t>(blockIdx.x) * S::kRows + slot;
   constexpr bool AHEAD = NV * U * S::kThreads < 16384;  // 1024 lanes of 16 columns have no registers for another row, or gamma
   float ga[NV][U], dg[NV][U], db[NV][U], nx[NV][U], ny[NV][U];
@@ -239,8 +277,10 @@ __global__ __launch_bounds__(S::kThreads) void layer_norm_bwd_rows(const void* d
       const UnitAt<U> at((int64_t{k} * S::kLanes + t) * U, cols);
 #pragma unroll
       for (int j = 0; j < U; ++j) {
-        dg[k][j] += d[k][j] * h[k][j];
-        db[k][j] += d[k][j];
+        if (!FEW) {
+          dg[k][j] += d[k][j] * h[k][j];
+          db[k][j] += d[k][j];
+        }
         d[k][j] *= ga[k][j];
         s[0] += j >= at.skip ? d[k][j] : 0.0f;
         s[1] += j >= at.skip ? d[k][j] * h[k][j] : 0.0f;
@@ -258,7 +298,7 @@ __global__ __launch_bounds__(S::kThreads) void layer_norm_bwd_rows(const void* d
       if (at.any()) store_unit<U, STREAM>(dx_dt, dx, row * cols + at.c, o);
     }
   }
-  if (!partials) return;
+  if (FEW || !partials) return;
   if constexpr (S::kRows > 1) {
     __shared__ float sums[S::kRows - 1][2][S::kCols];
     if (slot > 0) {
@@ -389,6 +429,11 @@ int row_shape(int64_t cols, Go&& go, Wide&& wide) {
   return wide();
 }
 
+// Whether dgamma and dbeta are formed by blocks of their own of the one launch, which read x and dy again, instead of by
+// way of partial rows and a second launch.  Us so and by partial rows, bf16: 8 x 4096 5.9, 8.6; 300 x 1001 5.8, 8.1; 1000 x
+// 1024 5.9, 9.5; 256 x 8192 11.6, 15.0; 512 x 4096 7.6, 12.4; 1000 x 4096 18.6, 14.6; 512 x 16384 36.4, 23.8.
+bool few_rows(int64_t rows, int64_t cols) { return rows <= 1024 && cols <= 16384 && rows * cols <= int64_t{1} << 21; }
+
 // Blocks of the backward pass, each of which leaves a partial row: so many that a CU has 24 to 48 KiB of rows on their
 // way (us of 256, 512 and 1024, rows of bf16: 65536 x 256 51.2, 35.5, 29.4; 32768 x 2048 168, 107, 81.5;
 // 16384 x 4096 113, 78.0, 94.2; 8192 x 8192 86.1, 90.9, 101; of f32: 16384 x 4096 147, 161, 164; x of f32 and dy of
@@ -491,6 +536,9 @@ extern "C" int vdsl_op_layer_norm_bwd(vdsl_queue q, int64_t rows, int64_t cols, 
   }
   float* part = params && rows ? static_cast<float*>(workspace->ptr) : nullptr;
   const void* g = gamma ? gamma->ptr : nullptr;
+  float* const dgp = dgamma ? static_cast<float*>(dgamma->ptr) : nullptr;
+  float* const dbp = dbeta ? static_cast<float*>(dbeta->ptr) : nullptr;
+  const bool few = params && few_rows(rows, cols) && dx != dy;  // dy is read beside the writing of dx
   const float* mi = static_cast<const float*>(mean->ptr);
   const float* ri = static_cast<const float*>(rstd->ptr);
   const auto rows_kernel = [&](auto shape, auto xt, auto dyt) {
@@ -498,10 +546,18 @@ extern "C" int vdsl_op_layer_norm_bwd(vdsl_queue q, int64_t rows, int64_t cols, 
     constexpr int XT = decltype(xt)::value, DYT = decltype(dyt)::value;
     const int64_t blocks = bwd_blocks(rows, S::kRows, cols * static_cast<int64_t>(dtype_size(x_dtype) + dtype_size(dy_dtype)));
     partial_rows = blocks;
+    if (few) {
+      const int64_t all = (rows + S::kRows - 1) / S::kRows;
+      hipLaunchKernelGGL((layer_norm_bwd_rows<S, XT, DYT, false, true>), dim3(static_cast<unsigned>(all + (cols + 15) / 16)),
+                         dim3(S::kThreads), 0, q->stream, dy->ptr, x->ptr, g, param_dtype, mi, ri, dx->ptr, dx_dtype, nullptr, rows, cols,
+                         static_cast<int>(all), dgp, dbp);
+      return check_launch("layer_norm_bwd_rows");
+    }
     const bool stream = rows * cols * static_cast<int64_t>(dtype_size(dx_dtype)) >= kStreamBytes;
-    const auto kernel = stream ? layer_norm_bwd_rows<S, XT, DYT, true> : layer_norm_bwd_rows<S, XT, DYT, false>;
+    const auto kernel = stream ? layer_norm_bwd_rows<S, XT, DYT, true, false> : layer_norm_bwd_rows<S, XT, DYT, false, false>;
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(S::kThreads), 0, q->stream,
-                       dy->ptr, x->ptr, g, param_dtype, mi, ri, dx->ptr, dx_dtype, part, rows, cols);
+                       dy->ptr, x->ptr, g, param_dtype, mi, ri, dx->ptr, dx_dtype, part, rows, cols, static_cast<int>(blocks), nullptr,
+                       nullptr);
     return check_launch("layer_norm_bwd_rows");
   };
   const auto wide = [&] {
@@ -527,10 +583,9 @@ extern "C" int vdsl_op_layer_norm_bwd(vdsl_queue q, int64_t rows, int64_t cols, 
     else st = row_shape<8>(cols, [&](auto s) { return rows_kernel(s, B{}, B{}); }, wide);
     VDSL_TRY(st);
   }
-  if (!params) return VDSL_OK;
+  if (!params || (few && rows > 0)) return VDSL_OK;
   const int64_t blocks = (2 * cols + 63) / 64;
   if (blocks > 0x7fffffff) return fail(VDSL_ERR_UNSUPPORTED, "layer_norm_bwd: too many columns");
-  hipLaunchKernelGGL(layer_norm_bwd_finish, block_grid(blocks), dim3(1024), 0, q->stream, part, partial_rows, cols,
-                     dgamma ? static_cast<float*>(dgamma->ptr) : nullptr, dbeta ? static_cast<float*>(dbeta->ptr) : nullptr);
+  hipLaunchKernelGGL(layer_norm_bwd_finish, block_grid(blocks), dim3(1024), 0, q->stream, part, partial_rows, cols, dgp, dbp);
   return check_launch("layer_norm_bwd_finish");
 }

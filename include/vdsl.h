@@ -713,6 +713,12 @@ int vdsl_debug_gemm_config(int32_t config);
  * the tests that cover every plan. */
 int vdsl_debug_w8a8_packed_plan(int32_t cfg, int32_t split);
 
+/* How vdsl_op_linear_xent_fwd_bwd would lay out a call, nothing run: plan[0] the pieces of the vocabulary,
+ * plan[1] the columns of one, plan[2] of the last, which is worked on first; plan[3] the tiles of the gradients'
+ * products (0: 64 x 64, 1: 128 x 64, 2: 256 x 256); plan[4] the splits of dx's sum over a piece's columns, plan[5]
+ * of those the last piece fills; plan[6] the splits of dw's sum over the rows.  Callers are tests. */
+int vdsl_debug_linear_xent_plan(int64_t n, int64_t vocab, int64_t dim, int64_t piece, int64_t* plan);
+
 /* ---- map-chain forms (benchmarks and tests, host-side only) ---------------------------------- */
 /* A map chain (vdsl_op_map_chain, vdsl_op_map_chain_v) runs as a kernel compiled at run time for
  * the chain (hiprtc, for the device's architecture; cached per chain and device, at most 512

@@ -176,6 +176,7 @@ PROTOTYPES = {
                                               _i32, _vp, _vp]),
     "vdsl_debug_fail_alloc_after": (C.c_int, [_i64]),
     "vdsl_debug_gemm_config": (C.c_int, [_i32]),
+    "vdsl_debug_linear_xent_plan": (C.c_int, [_i64, _i64, _i64, _i64, C.POINTER(_i64)]),
     "vdsl_debug_w8a8_packed_plan": (C.c_int, [_i32, _i32]),
 }
 

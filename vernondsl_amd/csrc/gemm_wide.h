@@ -186,7 +186,8 @@ struct WideFragments {
 
 // All tiles of this block: epilogue(acc, m0, n0) for each.  A(m, k) with lda elements between stored rows, B
 // likewise; a K-major operand's M or N a multiple of 8 (of what is allocated).  b_whole: B is K-major, its last stage
-// is allocated whole and holds zeros past K.  K > 0.  smem: WideCfg's bytes.
+// is allocated whole and holds zeros past K.  K > 0: the copies run
+// ahead of the loop and repeat its last stage, which has to be there.  smem: WideCfg's bytes.
 template <bool AKM, bool BKM, class Epilogue>
 __device__ __forceinline__ void wide_gemm(const uint16_t* __restrict__ A, const uint16_t* __restrict__ B, int M, int N, int K,
                                           int64_t lda, int64_t ldb, bool b_whole, char* smem, Epilogue&& epilogue) {

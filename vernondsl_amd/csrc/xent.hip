@@ -546,17 +546,17 @@ struct WideGradArgs {
   int n_alloc;         // of B, where it is K-major: columns that are allocated (of A: lda)
   int64_t lda, ldb;
   float* sum;          // [splits][n][m] f32, the pieces' sum
-  bool first, last;    // of the pieces: sum holds nothing yet; the result is whole (never with splits)
-  int splits;          // of k, blockIdx.y's
+  int held;            // splits of sum that hold something already
+  bool last;           // of the pieces: the result is whole (never with splits)
+  int splits;          // of k, blockIdx.y's: no more than k has stages
   const float* inv;
   void* out;
   int out_dt;
 };
 
 // Four elements from e on, of which the first n (or all) are the row's, to sum or to out.
-template <class Args>
-__device__ __forceinline__ void store_sum(const Args& p, float* sum, float inv, int64_t e, int n, float (&v)[4]) {
-  if (!p.first) {
+__device__ __forceinline__ void store_sum(const WideGradArgs& p, float* sum, float inv, int64_t e, int n, float (&v)[4]) {
+  if (static_cast<int>(blockIdx.y) < p.held) {
     float before[4];
     load_some(VDSL_F32, sum, e, n, before);
 #pragma unroll
@@ -676,6 +676,7 @@ struct Plan {
   int64_t g_rows = 0, ldg = 0;    // of G; its rows past n are zeros
   int64_t ld = 0;                 // of x and w: dim, or that of their copies in whole units (stages, for 256 x 256 tiles)
   int splits = 1, dw_splits = 1;  // of the sums over a piece's columns for dx, over the rows for dw
+  int last_splits = 1;            // of dx's that the last piece fills: it may be a few columns of many pieces' remainder
   bool sum = false;               // whether dx is formed by way of f32 sums (dw: where it has splits)
   size_t at_stats = 0, at_zlabel = 0, at_lse = 0, at_row_loss = 0, at_inv = 0, at_g = 0, at_sum = 0, at_dw_sum = 0, at_x = 0, at_w = 0, bytes = 0;
 };
@@ -730,6 +731,7 @@ int make_plan(int64_t n, int64_t vocab, int64_t dim, int64_t piece, bool backwar
   if (backward && p.grads == kTilesWide) {
     p.splits = wide_splits(n, dim, p.piece);
     p.dw_splits = wide_splits(p.piece, dim, n);
+    p.last_splits = static_cast<int>(std::min<int64_t>(p.splits, ceil_div(vocab - (p.pieces - 1) * p.piece, 64)));
   } else if (backward) {
     // One launch: splits of as many stages as two blocks a CU come to, but of 12 or more, since each split's sums are
     // written and read again (us with 12 and with 5: 16 x 512, 5003 20.3, 22.3; 300 x 1000, 5003 37.6, 39.6; 128 x 512,
@@ -737,7 +739,7 @@ int make_plan(int64_t n, int64_t vocab, int64_t dim, int64_t piece, bool backwar
     const auto tiles = [&](int64_t rows) { return ceil_div(dim, rows_of(p.grads)) * ceil_div(rows, 64); };
     const int64_t x_stages = ceil_div(p.piece, 64), w_stages = ceil_div(n, 64);
     const int64_t share = std::max<int64_t>(12, ceil_div(tiles(n) * x_stages + tiles(p.piece) * w_stages, 512));
-    p.splits = static_cast<int>(std::clamp<int64_t>(ceil_div(x_stages, share), 1, 64));
+    p.splits = p.last_splits = static_cast<int>(std::clamp<int64_t>(ceil_div(x_stages, share), 1, 64));  // (any may be empty)
     p.dw_splits = static_cast<int>(std::clamp<int64_t>(ceil_div(w_stages, share), 1, 64));
   }
   p.sum = p.pieces > 1 || p.splits > 1;  // (forward: one piece, no splits)
@@ -798,7 +800,7 @@ int launch_grads_small(const GradArgs& dx, const GradArgs& dw, const float* row_
 template <bool BKM>
 int launch_grad_wide(const WideGradArgs& a, int64_t n, hipStream_t s) {
   const dim3 grid(wide_blocks(ceil_div(a.m, 256) * ceil_div(n, 256)), static_cast<unsigned>(a.splits));
-  if (a.first && a.last && a.out_dt == VDSL_BF16)
+  if (a.held == 0 && a.last && a.out_dt == VDSL_BF16)
     hipLaunchKernelGGL((xent_grad_wide<BKM, true>), grid, dim3(WideCfg::NT), 0, s, a);
   else
     hipLaunchKernelGGL((xent_grad_wide<BKM, false>), grid, dim3(WideCfg::NT), 0, s, a);
@@ -909,10 +911,12 @@ int run_xent(vdsl_queue q, int64_t n, int64_t dim, int64_t vocab, vdsl_buffer x,
     if (t > 0) VDSL_TRY(launch_logits<kLogitGrad>(la, plan.again, grad_scale, inv, s));
     void* const dw_piece = static_cast<char*>(dw->ptr) + v0 * dim * static_cast<int64_t>(dtype_size(dw_dtype));
     if (plan.grads == kTilesWide) {
-      const WideGradArgs for_dx{la.w, g, out_cols, la.n, la.cols, 0, plan.ld, plan.ldg, sum, t == 0, last && plan.splits == 1,
-                                plan.splits, inv, dx->ptr, dx_dtype};
+      // the last piece comes first and may not fill the splits; those it leaves start with the next piece
+      const int splits = t == 0 ? plan.last_splits : plan.splits, held = t == 0 ? 0 : t == 1 ? plan.last_splits : plan.splits;
+      const WideGradArgs for_dx{la.w, g, out_cols, la.n, la.cols, 0, plan.ld, plan.ldg, sum, held, last && plan.splits == 1,
+                                splits, inv, dx->ptr, dx_dtype};
       VDSL_TRY(launch_grad_wide<false>(for_dx, n, s));
-      const WideGradArgs for_dw{la.x, g, out_cols, la.cols, la.n, static_cast<int>(plan.ldg), plan.ld, plan.ldg, dw_sum, true, !dw_sum,
+      const WideGradArgs for_dw{la.x, g, out_cols, la.cols, la.n, static_cast<int>(plan.ldg), plan.ld, plan.ldg, dw_sum, 0, !dw_sum,
                                 plan.dw_splits, inv, dw_piece, dw_dtype};
       VDSL_TRY(launch_grad_wide<true>(for_dw, plan.ldg, s));
     } else {
@@ -943,6 +947,15 @@ extern "C" int vdsl_linear_xent_workspace_bytes(int64_t n, int64_t vocab, int64_
   Plan plan;
   VDSL_TRY(make_plan(n, vocab, dim, piece, backward != 0, plan));
   *bytes = plan.bytes;
+  return VDSL_OK;
+}
+
+extern "C" int vdsl_debug_linear_xent_plan(int64_t n, int64_t vocab, int64_t dim, int64_t piece, int64_t* plan) {
+  if (!plan) return fail(VDSL_ERR_INVALID_ARG, "plan is null");
+  Plan p;
+  VDSL_TRY(make_plan(n, vocab, dim, piece, true, p));
+  const int64_t values[7] = {p.pieces, p.piece, vocab - (p.pieces - 1) * p.piece, p.grads, p.splits, p.last_splits, p.dw_splits};
+  std::copy(values, values + 7, plan);
   return VDSL_OK;
 }
 

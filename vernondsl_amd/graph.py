@@ -210,6 +210,7 @@ class Graph:
         return loss
 
     def mse_loss(self, y: Value, t: Value, name="loss") -> Value:
+        """The mean of (y - t)^2; t is a constant to backward()."""
         if y.dtype != "f32" or t.dtype != "f32" or y.shape != t.shape:
             raise TypeError("mse_loss takes two f32 tensors of one shape")
         loss = self._value(name, (1,), "f32", requires_grad=y.requires_grad)
@@ -246,7 +247,10 @@ class Graph:
 
     # ---- autodiff --------------------------------------------------------------------------------
     def backward(self, loss: Value) -> dict:
-        """Appends the backward ops of `loss` and returns {param name: f32 gradient Value}."""
+        """Appends the backward ops of `loss` and returns {param name: f32 gradient Value} for every param that the loss
+        depends on through an operand with a rule above, whichever operand that is (a learned position table that is
+        added, a computed weight, table or gain); an mse_loss's target is a constant.  The Value is named grad_<param>
+        in general, but not where it is another value's gradient as well (an operand of add): read it by its own name."""
         if loss.producer is None or loss.producer.kind not in ("mse", "linear_xent"):
             raise ValueError("backward() starts from an mse_loss or a linear_cross_entropy value")
         fwd_ops = list(self.ops)
@@ -259,13 +263,11 @@ class Graph:
         contrib: dict[str, list] = {}  # param name -> its gradient's terms, one per op reading it
         if loss.producer.kind == "linear_xent":
             x, w, _ = loss.producer.inputs
-            dx = self._value(self._fresh("d_" + x.name), x.shape, "f32", "grad")
-            dw = self._value("grad_" + w.name if uses[w.name] == 1 else self._fresh("dterm_" + w.name), w.shape, "f32", "grad")
+            dx, dw = self._term(x, uses), self._term(w, uses)
             loss.producer.outputs += [dx, dw]  # the forward op also emits both gradients
             dx.producer = dw.producer = loss.producer
-            grad[x.name] = ("f32", dx)
-            if w.requires_grad:
-                contrib[w.name] = [dw]
+            self._start(x, ("f32", dx), grad, contrib)
+            self._give(w, ("f32", dw), grad, contrib)
         else:
             y, _ = loss.producer.inputs
             dy = self._value(self._fresh("d_" + y.name), y.shape, "bf16", "grad")
@@ -273,7 +275,7 @@ class Graph:
             self._transposed.add(dy_t.name)
             part = self._value(self._fresh("mse_partials"), (max(1, kernels.mse_partials_count(*y.shape)),), "f32", "scratch")
             loss.producer.outputs += [dy, dy_t, part]  # the forward MSE op also emits dL/dy
-            grad[y.name] = ("bf16", dy, dy_t)
+            self._start(y, ("bf16", dy, dy_t), grad, contrib)
             lin = y.producer
             if (self.fuse_mse and lin is not None and lin.kind == "linear" and lin.attrs["act"] == "none"
                     and uses[y.name] == 1 and lin.attrs.get("packed") is not None and y.dtype == "f32"
@@ -298,23 +300,24 @@ class Graph:
                 continue
             if op.kind == "add":  # d(a + b) passes dL/dy to both operands
                 for x in op.inputs:
-                    if x.requires_grad or (x.producer is not None and x.kind == "activation" and _needs(x, self)):
-                        self._accumulate(grad, x, grad[y.name])
+                    self._give(x, grad[y.name], grad, contrib)
                 continue
             if op.kind == "embedding":
                 table, ids = op.inputs
-                if table.requires_grad:
-                    dt = self._param_term(table, uses, contrib)
+                if self._wants(table):
+                    dt = self._term(table, uses)
                     self._op("embedding_bwd", [ids, grad[y.name][1]], [dt], scale=op.attrs["scale"])
+                    self._give(table, ("f32", dt), grad, contrib)
                 continue
             if op.kind == "layer_norm":
                 x, gamma = op.inputs[:2]
-                dx = self._value(self._fresh("d_" + x.name), x.shape, "f32", "grad")
-                dp = [self._param_term(p, uses, contrib) if p.requires_grad else None for p in op.inputs[1:]]
+                dx = self._term(x, uses)
+                dp = [self._term(p, uses) if self._wants(p) else None for p in op.inputs[1:]]
                 self._op("layer_norm_bwd", [grad[y.name][1], x, gamma, op.outputs[1], op.outputs[2]], [dx] + [d for d in dp if d is not None],
                          dgamma=dp[0], dbeta=dp[1] if len(dp) > 1 else None)
-                if x.requires_grad or (x.producer is not None and x.kind == "activation" and _needs(x, self)):
-                    self._accumulate(grad, x, ("f32", dx))
+                for p, d in zip(op.inputs, [dx] + dp):
+                    if d is not None:
+                        self._give(p, ("f32", d), grad, contrib)
                 continue
             x, w = op.inputs[:2]
             g = grad[y.name]
@@ -343,17 +346,16 @@ class Graph:
                 self._transposed.add(da_t.name)
                 self._op("relu_bwd", [g[1], op.attrs["pre"]], [da, da_t])
                 gb, gt = da, da_t
-            if w.requires_grad:
-                single = uses[w.name] == 1
-                dw = self._value("grad_" + w.name if single else self._fresh("dterm_" + w.name), w.shape, "f32", "grad")
+            if self._wants(w):
+                dw = self._term(w, uses)
                 # dW[out][in] = sum_b g[b][out] x[b][in]: A = g^T [out][B] (K = B contiguous), B = x [B][in];
                 # with k_major_grads A is g as stored ([B][out] = [K][M], trans_a)
                 if self.k_major_grads:
                     self._op("gemm", [gb, x], [dw], trans_a=True, trans_b=False, epi=_lib.EPI_NONE)
                 else:
                     self._op("gemm", [gt, x], [dw], trans_a=False, trans_b=False, epi=_lib.EPI_NONE)
-                contrib.setdefault(w.name, []).append(dw)
-            if x.requires_grad or (x.producer is not None and x.kind == "activation" and _needs(x, self)):
+                self._give(w, ("f32", dw), grad, contrib)
+            if self._wants(x):
                 # dx[B][in] = sum_o g[b][o] W[o][in]: A = g [B][out], B = W stored [out][in] = [K][N].
                 # A param's transpose W^T [in][out] (the NT form's B) is made once by a prepare op
                 # instead of by the GEMM on every step.
@@ -382,15 +384,15 @@ class Graph:
                         self._op("gemm_gelu_bwd", [gb, wt, xp.attrs["pre"]], [da, da_t], packed=packed)
                     grad[x.name] = ("gelu_da", da, da_t)
                 else:
-                    dx = self._value(self._fresh("d_" + x.name), x.shape, "f32", "grad")
+                    dx = self._term(x, uses)
                     if wt is not None:
                         self._op("gemm", [gb, wt], [dx], trans_a=False, trans_b=True, epi=_lib.EPI_NONE)
                     else:
                         self._op("gemm", [gb, w], [dx], trans_a=False, trans_b=False, epi=_lib.EPI_NONE)
-                    self._accumulate(grad, x, ("f32", dx))
+                    self._give(x, ("f32", dx), grad, contrib)
         param_grads = {}
         for name, terms in contrib.items():
-            # a param read by several linear ops (tied weights): the sum of its terms, in the order
+            # a param read by several ops (tied weights): the sum of its terms, in the order
             # backward formed them (the last forward use first), named grad_<param> at the end
             acc = terms[0]
             for k, t in enumerate(terms[1:], 2):
@@ -403,11 +405,34 @@ class Graph:
             self._elide_unread_transposes()
         return param_grads
 
-    def _param_term(self, p: Value, uses: dict, contrib: dict) -> Value:
-        """The f32 value of one op's term of param p's gradient: the gradient itself where no other op reads p."""
-        d = self._value("grad_" + p.name if uses[p.name] == 1 else self._fresh("dterm_" + p.name), p.shape, "f32", "grad")
-        contrib.setdefault(p.name, []).append(d)
-        return d
+    def _wants(self, v: Value) -> bool:
+        """Whether v's gradient is needed: it is a param that takes one, or some such param is upstream of it."""
+        return v.requires_grad or (v.producer is not None and v.kind == "activation" and _needs(v, self))
+
+    def _term(self, v: Value, uses: dict) -> Value:
+        """The f32 value of one op's term of dL/dv: a param's gradient itself where no other op reads the param."""
+        if v.kind == "param" and v.requires_grad:
+            name = "grad_" + v.name if uses[v.name] == 1 else self._fresh("dterm_" + v.name)
+        else:
+            name = self._fresh("d_" + v.name)
+        return self._value(name, v.shape, "f32", "grad")
+
+    def _start(self, v: Value, g: tuple, grad: dict, contrib: dict):
+        """The loss op's gradient of its operand v, from which the rules go on."""
+        if v.kind == "param":
+            self._give(v, g, grad, contrib)
+        else:
+            grad[v.name] = g
+
+    def _give(self, v: Value, g: tuple, grad: dict, contrib: dict):
+        """Hands on the term g of dL/dv that one reader of v gives: a param's terms are kept for their sum, an activation's
+        are added up for its producer's rule; where nothing needs dL/dv it ends here."""
+        if not self._wants(v):
+            return
+        if v.kind == "param":
+            contrib.setdefault(v.name, []).append(g[1] if g[0] == "f32" else self._to_f32(g[1]))
+        else:
+            self._accumulate(grad, v, g)
 
     def _accumulate(self, grad: dict, x: Value, g: tuple):
         """Adds the gradient term g to dL/dx: the first term is kept as it is; a second one (x read

@@ -625,6 +625,8 @@ int vdsl_op_gemm_w8a8_packed_noalloc(vdsl_queue q, int64_t M, int64_t N, int64_t
 /* ========================================================================================== */
 /* Op class 6: what makes an MLP a model of tokens (no reference code): the embedding, layer  */
 /* norm between residual blocks, and the output layer with its cross entropy.                 */
+/* An output or a workspace may share a buffer with another operand only where this says so   */
+/* (VDSL_ERR_INVALID_ARG otherwise); inputs may share one.                                     */
 /* ========================================================================================== */
 /* out[i] = scale * table[ids[i]] (one f32 product per element, rounded once); zeros where ids[i] is
  * outside [0, vocab).  table: F32 or BF16 [vocab][dim]; ids: I32 [n]; out: F32 or BF16 [n][dim]. */

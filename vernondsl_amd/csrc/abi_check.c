@@ -282,11 +282,16 @@ int main(void) {
     vdsl_buffer wn = alloc(d, ws ? ws : 16);
     EXPECT_OK(vdsl_op_layer_norm_bwd(q, n, dim, VDSL_F32, dx, VDSL_BF16, x, VDSL_F32, NULL, mean, rstd, VDSL_F32, dx, dw, NULL, wn));
     EXPECT_ERR(vdsl_op_layer_norm_bwd(q, n, dim, VDSL_F32, dx, VDSL_BF16, x, VDSL_F32, NULL, mean, rstd, VDSL_F32, dx, dw, NULL, NULL));
+    EXPECT_ERR(vdsl_op_layer_norm_bwd(q, n, dim, VDSL_F32, dx, VDSL_BF16, x, VDSL_F32, NULL, mean, rstd, VDSL_F32, dx, dw, dw, wn));
     EXPECT_ERR(vdsl_linear_xent_workspace_bytes(n, 0, dim, 0, 1, &ws));
     EXPECT_ERR(vdsl_linear_xent_workspace_bytes(n, vocab, dim, -1, 1, &ws));
     EXPECT_ERR(vdsl_linear_xent_workspace_bytes(n, kHuge, dim, 0, 1, &ws));
     EXPECT_OK(vdsl_linear_xent_workspace_bytes(n, vocab, dim, INT64_MAX, 1, &ws));
     EXPECT_OK(vdsl_linear_xent_workspace_bytes(n, vocab, dim, 256, 1, &ws));
+    int64_t plan[7];
+    EXPECT_OK(vdsl_debug_linear_xent_plan(n, vocab, dim, 256, plan));
+    EXPECT_ERR(vdsl_debug_linear_xent_plan(n, kHuge, dim, 256, plan));
+    EXPECT_ERR(vdsl_debug_linear_xent_plan(n, vocab, dim, 256, NULL));
     vdsl_buffer wx = alloc(d, ws);
     EXPECT_OK(vdsl_op_linear_xent_fwd_bwd(q, n, dim, vocab, x, w, ids, 256, 1.0f, loss, NULL, NULL, VDSL_BF16, dx, VDSL_F32, dw, wx));
     EXPECT_ERR(vdsl_op_linear_xent_fwd_bwd(q, n, dim, vocab, x, w, ids, 256, 1.0f, loss, NULL, NULL, VDSL_BF16, x, VDSL_F32, dw, wx));

@@ -5,6 +5,7 @@
 #include <stdint.h>
 
 #include <atomic>
+#include <initializer_list>
 #include <string>
 
 #include "fmath.h"
@@ -77,6 +78,10 @@ int enter_queue(vdsl_queue q);
 // Validates `b` (on the queue's device) and that it holds at least `bytes`.  `name` is used in
 // the error message.  If `writable`, rejects UNIFORM_CONSTANT buffers.
 int check_buffer(vdsl_queue q, vdsl_buffer b, size_t bytes, const char* name, bool writable);
+
+// Fails where a buffer that `op` writes (null: not given) is another one that it writes or one of `others`: some of its
+// blocks write while others still read, and two results do not fit one place.
+int check_apart(const char* op, std::initializer_list<vdsl_buffer> written, std::initializer_list<vdsl_buffer> others);
 
 size_t dtype_size(int dtype);
 

@@ -450,7 +450,7 @@ extern "C" int vdsl_op_embedding_fwd(vdsl_queue q, int64_t n, int64_t dim, int64
   VDSL_TRY(check_buffer(q, table, nbytes(vocab, dim, dtype_size(table_dtype)), "table", false));
   VDSL_TRY(check_buffer(q, ids, nbytes(n, 4), "ids", false));
   VDSL_TRY(check_buffer(q, out, nbytes(n, dim, dtype_size(out_dtype)), "out", true));
-  if (out == table) return fail(VDSL_ERR_INVALID_ARG, "embedding_fwd: out must not be the table");
+  VDSL_TRY(check_apart("embedding_fwd", {out}, {table, ids}));
   if (n == 0 || dim == 0) return VDSL_OK;
   if (vocab == 0) {  // no id is a row
     hipLaunchKernelGGL(embedding_zero_kernel, dim3(1024), dim3(256), 0, q->stream, static_cast<uint16_t*>(out->ptr),
@@ -548,7 +548,7 @@ extern "C" int vdsl_op_embedding_bwd(vdsl_queue q, int64_t n, int64_t dim, int64
   VDSL_TRY(check_buffer(q, dy, nbytes(n, dim, dtype_size(dy_dtype)), "dy", false));
   VDSL_TRY(check_buffer(q, dtable, nbytes(vocab, dim, 4), "dtable", true));
   if (p.bytes) VDSL_TRY(check_buffer(q, workspace, p.bytes, "workspace", true));
-  if (dtable == dy) return fail(VDSL_ERR_INVALID_ARG, "embedding_bwd: dtable must not be dy");
+  VDSL_TRY(check_apart("embedding_bwd", {dtable, p.bytes ? workspace : nullptr}, {ids, dy}));
   if (vocab == 0 || dim == 0) return VDSL_OK;
   const hipStream_t s = q->stream;
   // A wave per row of up to 1024 columns (1, 2 or 4 units a lane), 2 or 4 waves for a wider one.

@@ -470,6 +470,8 @@ extern "C" int vdsl_op_layer_norm_fwd(vdsl_queue q, int64_t rows, int64_t cols, 
   if (mean) VDSL_TRY(check_buffer(q, mean, nbytes(rows, 4), "mean", true));
   if (rstd) VDSL_TRY(check_buffer(q, rstd, nbytes(rows, 4), "rstd", true));
   if (x == y && x_dtype != y_dtype) return fail(VDSL_ERR_INVALID_ARG, "in-place layer_norm_fwd needs one dtype");
+  VDSL_TRY(check_apart("layer_norm_fwd", {y, mean, rstd}, {gamma, beta}));
+  VDSL_TRY(check_apart("layer_norm_fwd", {mean, rstd}, {x}));
   if (rows == 0 || cols == 0) return VDSL_OK;
   if (rows > 0x7fffffff) return fail(VDSL_ERR_UNSUPPORTED, "layer_norm_fwd: too many rows");
   const void* g = gamma ? gamma->ptr : nullptr;
@@ -525,15 +527,17 @@ extern "C" int vdsl_op_layer_norm_bwd(vdsl_queue q, int64_t rows, int64_t cols, 
   if (dgamma) VDSL_TRY(check_buffer(q, dgamma, nbytes(cols, 4), "dgamma", true));
   if (dbeta) VDSL_TRY(check_buffer(q, dbeta, nbytes(cols, 4), "dbeta", true));
   if (dx == dy && dx_dtype != dy_dtype) return fail(VDSL_ERR_INVALID_ARG, "in-place layer_norm_bwd needs one dtype");
-  if (dx == x) return fail(VDSL_ERR_INVALID_ARG, "layer_norm_bwd: dx may be dy, not x");
   if (cols == 0) return VDSL_OK;
   if (rows > 0x7fffffff) return fail(VDSL_ERR_UNSUPPORTED, "layer_norm_bwd: too many rows");
   int64_t partial_rows = 0;
+  size_t need = 0;
   if (params) {
-    size_t need = 0;
     VDSL_TRY(vdsl_layer_norm_bwd_workspace_bytes(rows, cols, &need));
     if (need) VDSL_TRY(check_buffer(q, workspace, need, "workspace", true));
   }
+  const vdsl_buffer used = need ? workspace : nullptr;
+  VDSL_TRY(check_apart("layer_norm_bwd", {dx, dgamma, dbeta, used}, {x, gamma, mean, rstd}));
+  VDSL_TRY(check_apart("layer_norm_bwd", {dgamma, dbeta, used}, {dy}));  // dx may be dy
   float* part = params && rows ? static_cast<float*>(workspace->ptr) : nullptr;
   const void* g = gamma ? gamma->ptr : nullptr;
   float* const dgp = dgamma ? static_cast<float*>(dgamma->ptr) : nullptr;

@@ -109,6 +109,17 @@ int check_buffer(vdsl_queue q, vdsl_buffer b, size_t bytes, const char* name, bo
   return VDSL_OK;
 }
 
+int check_apart(const char* op, std::initializer_list<vdsl_buffer> written, std::initializer_list<vdsl_buffer> others) {
+  for (const vdsl_buffer* w = written.begin(); w != written.end(); ++w) {
+    if (!*w) continue;
+    bool shared = false;
+    for (const vdsl_buffer* o = w + 1; o != written.end(); ++o) shared |= *w == *o;
+    for (const vdsl_buffer o : others) shared |= *w == o;
+    if (shared) return fail(VDSL_ERR_INVALID_ARG, std::string(op) + ": an output or the workspace shares a buffer with another operand");
+  }
+  return VDSL_OK;
+}
+
 namespace {
 
 // The library's own device memory, allocated and freed while another queue may be recording on this

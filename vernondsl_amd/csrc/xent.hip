@@ -825,10 +825,9 @@ int run_xent(vdsl_queue q, int64_t n, int64_t dim, int64_t vocab, vdsl_buffer x,
   if (backward) {
     VDSL_TRY(check_buffer(q, dx, nbytes(n, dim, dtype_size(dx_dtype)), "dx", true));
     VDSL_TRY(check_buffer(q, dw, nbytes(vocab, dim, dtype_size(dw_dtype)), "dw", true));
-    if (dx == x || dx == w || dw == x || dw == w || dx == dw)
-      return fail(VDSL_ERR_INVALID_ARG, "linear_xent_fwd_bwd: a gradient must not share a buffer with x, w or the other one");
   }
   VDSL_TRY(check_buffer(q, workspace, plan.bytes, "workspace", true));
+  VDSL_TRY(check_apart("linear_xent", {loss, row_loss, lse, dx, dw, workspace}, {x, w, labels}));
   const hipStream_t s = q->stream;
   char* const ws = static_cast<char*>(workspace->ptr);
   const int32_t* lab = static_cast<const int32_t*>(labels->ptr);

@@ -7,15 +7,20 @@
 
 namespace vdsl {
 
+// (At: the vector with the struct's alignment, for a builtin that takes its address: a member's address would promise
+// the vector's own.)
 struct __attribute__((packed, aligned(2))) U32x4At2 {
   u32x4 v;
+  typedef u32x4 At __attribute__((aligned(2)));
 };
 typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 struct __attribute__((packed, aligned(2))) U32x2At2 {
   u32x2 v;
+  typedef u32x2 At __attribute__((aligned(2)));
 };
 struct __attribute__((packed, aligned(4))) F32x4At4 {
   f32x4 v;
+  typedef f32x4 At __attribute__((aligned(4)));
 };
 
 // A grid of `blocks` blocks of up to 1024 lanes (times y): a launch takes fewer than 2^32 lanes along x, so x holds
@@ -67,10 +72,10 @@ __device__ __forceinline__ void load_whole(const void* __restrict__ p, int64_t e
 constexpr int64_t kStreamBytes = int64_t{96} << 20;
 
 // STREAM is the kernels' parameter, since of a plain and a passing store in two branches the compiler makes one plain one.
-template <bool STREAM, class V>
-__device__ __forceinline__ void store_at(V* to, V v) {
-  if constexpr (STREAM) __builtin_nontemporal_store(v, to);
-  else *to = v;
+template <bool STREAM, class Unit>
+__device__ __forceinline__ void store_at(Unit* to, typename Unit::At v) {
+  if constexpr (STREAM) __builtin_nontemporal_store(v, reinterpret_cast<typename Unit::At*>(to));
+  else to->v = v;
 }
 template <int DT, int U, bool STREAM = false>
 __device__ __forceinline__ void store_whole(void* __restrict__ p, int64_t e, const float (&v)[U]) {
@@ -81,14 +86,14 @@ __device__ __forceinline__ void store_whole(void* __restrict__ p, int64_t e, con
 #pragma unroll
     for (int h = 0; h < U / 4; ++h) {
       const f32x4 x = {v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]};
-      store_at<STREAM>(&reinterpret_cast<F32x4At4*>(static_cast<float*>(p) + e + 4 * h)->v, x);
+      store_at<STREAM>(reinterpret_cast<F32x4At4*>(static_cast<float*>(p) + e + 4 * h), x);
     }
   } else if constexpr (U == 8) {
     const u32x4 x = {pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])};
-    store_at<STREAM>(&reinterpret_cast<U32x4At2*>(static_cast<uint16_t*>(p) + e)->v, x);
+    store_at<STREAM>(reinterpret_cast<U32x4At2*>(static_cast<uint16_t*>(p) + e), x);
   } else {
     const u32x2 x = {pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
-    store_at<STREAM>(&reinterpret_cast<U32x2At2*>(static_cast<uint16_t*>(p) + e)->v, x);
+    store_at<STREAM>(reinterpret_cast<U32x2At2*>(static_cast<uint16_t*>(p) + e), x);
   }
 }
 template <int U, bool STREAM = false>

@@ -364,7 +364,8 @@ __global__ __launch_bounds__(1024) void layer_norm_bwd_stream(const void* dy, in
   }
 }
 
-// The sums for dgamma and dbeta of such rows: block (x, y) takes 1024 columns and the y-th range of rows.
+// The sums for dgamma and dbeta of such rows: block (x, y) takes 1024 columns and every gridDim.y-th row.  The wider the
+// rows, the fewer blocks share them (from 2^18 columns on one takes all), so f32 sums of 64 rows are added up in f64.
 // Runs before layer_norm_bwd_stream, which may overwrite dy.
 __global__ __launch_bounds__(256) void layer_norm_bwd_columns(const void* __restrict__ dy, int dy_dt, const void* __restrict__ x,
                                                               int x_dt, const float* __restrict__ mean,
@@ -372,17 +373,31 @@ __global__ __launch_bounds__(256) void layer_norm_bwd_columns(const void* __rest
                                                               int64_t rows, int64_t cols) {
   const int64_t c = static_cast<int64_t>(blockIdx.x) * 1024 + 4 * threadIdx.x;
   if (c >= cols) return;
-  float dg[4] = {0.0f, 0.0f, 0.0f, 0.0f}, db[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int64_t row = blockIdx.y; row < rows; row += gridDim.y) {
-    float h[4], d[4];
-    load_some(x_dt, x, row * cols + c, cols - c, h);
-    load_some(dy_dt, dy, row * cols + c, cols - c, d);
-    const float m = mean[row], r = rstd[row];
+  double gs[4] = {0.0, 0.0, 0.0, 0.0}, bs[4] = {0.0, 0.0, 0.0, 0.0};
+  for (int64_t row = blockIdx.y; row < rows;) {
+    float dg[4] = {0.0f, 0.0f, 0.0f, 0.0f}, db[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int k = 0; k < 64 && row < rows; ++k, row += gridDim.y) {
+      float h[4], d[4];
+      load_some(x_dt, x, row * cols + c, cols - c, h);
+      load_some(dy_dt, dy, row * cols + c, cols - c, d);
+      const float m = mean[row], r = rstd[row];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        dg[j] += d[j] * ((h[j] - m) * r);
+        db[j] += d[j];
+      }
+    }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      dg[j] += d[j] * ((h[j] - m) * r);
-      db[j] += d[j];
+      gs[j] += dg[j];
+      bs[j] += db[j];
     }
+  }
+  float dg[4], db[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    dg[j] = static_cast<float>(gs[j]);
+    db[j] = static_cast<float>(bs[j]);
   }
   float* const out = partials + static_cast<int64_t>(blockIdx.y) * 2 * cols;
   store_some(VDSL_F32, out, c, cols - c, dg);

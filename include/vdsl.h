@@ -676,7 +676,8 @@ int vdsl_op_linear_xent_fwd(vdsl_queue q, int64_t n, int64_t dim, int64_t vocab,
  * does not count), dx (F32 or BF16 [n][dim]) = grad_scale / count * G w and dw (F32 or BF16
  * [vocab][dim], every row written) = grad_scale / count * G^T x (every row of x takes part, those that do
  * not count with 0: they must be finite).  G is rounded to bf16 for these products,
- * as every gradient that a bf16 GEMM of this library takes; they accumulate in f32 and are rounded once.
+ * as every gradient that a bf16 GEMM of this library takes (1e-3 of the gradients' norm, 1.5e-3 over few
+ * rows); they accumulate in f32 and are rounded once.
  * The vocabulary is worked on in pieces of `piece` columns (4 MiB / (2 n) if that is more, rounded up to a
  * multiple of 256, the pieces then made alike, of 2^24 columns at most): the workspace holds 2 n piece bytes
  * for one of them, and more pieces take more operations (all but one form their logits twice).  piece 0: as many columns as

@@ -7,8 +7,9 @@
 // into f32: 56 us, 6.2 TB/s).  The gradient
 // does not add into the table with atomics, whose order would change its bits from run to run: the
 // positions are sorted by token (stably, so a token's positions ascend), and then every row of dtable is
-// written once, zero or the f32 sum of its terms (16384 positions, 32768 x 4096: sorting 11 us, chunks 8, rows 107 to
-// 112 for 588 MB; 300 positions, 5003 x 1001: 5.8 back to back).
+// written once, zero or the f32 sum of its terms (16384 positions, 32768 x 4096: sorting 11 us, chunks 8, rows 97 to
+// 112 for 588 MB; 300 positions, 5003 x 1001, back to back: 6.2 with uniform ids, 6.8 to 9.2 with ids as frequent as
+// words, whose most frequent token's row is the last one done).
 
 #include <algorithm>
 #include <type_traits>
@@ -386,7 +387,9 @@ __global__ __launch_bounds__(256) void embedding_bwd_kernel(const int32_t* __res
 
 // The same of few positions, which need no sort: each row's wave looks through all of them.  Us of uniform ids, so and
 // sorted: 300 of 1001 columns, vocabulary 5003 5.8, 11.6; 512 of 64, 32768 8.2, 20.6; 1000 of 1001, 5003 6.4, 13.6; ids as
-// frequent as words: 1000 of 1001, 5003 19.1, 23.5, but 2000 34.4, 26.6.
+// frequent as words: 1000 of 1001, 5003 19.1, 23.5, but 2000 34.4, 26.6.  The worst is one token at all positions, whose row one
+// wave sums kInFlight rows at a time: 300 of 1001, 5003 56, 31; 1024 of 1001, 5003 223, 49; 1024 of 4096, 32768 429, 116
+// (uniform 104.5, 104.9).
 constexpr int kFewPositions = 1024;
 
 template <int DYT, int U, int NV>

@@ -692,6 +692,110 @@ int vdsl_op_linear_xent_fwd_bwd(vdsl_queue q, int64_t n, int64_t dim, int64_t vo
                                 int32_t dx_dtype, vdsl_buffer dx, int32_t dw_dtype, vdsl_buffer dw,
                                 vdsl_buffer workspace);
 
+/* ========================================================================================== */
+/* Op class 7: what lets the rows of a sequence see each other (no reference code): rotary    */
+/* positions, attention over packed sequences, and a paged cache with the attention over it.  */
+/* Outputs and workspaces share buffers as in class 6: only where this says so.                */
+/* ========================================================================================== */
+/* Where the heads of a tensor lie in its buffer, in elements: element i of head h of row t at
+ * [first + t * stride + h * dim + i], so q, k and v may be columns of one projection.  Attention takes
+ * first and stride that are multiples of 8, stride at least heads * dim and below 2^24. */
+typedef struct vdsl_heads {
+  int64_t first;
+  int64_t stride;
+} vdsl_heads;
+
+/* y = x [rows][width] with `heads` heads turned by their rows' positions; the other columns are handed on.
+ * Head h of a row takes columns [first + h * dim, first + (h + 1) * dim), h < heads; of these the first rot = 2 * pairs
+ * turn and the others stay.  Pair i is columns (i, i + pairs) of the head, or (2 i, 2 i + 1) if interleaved.  At
+ * position p (I32 [rows], of either sign) its angle is t = 2 pi p (freqs[0][i] + freqs[1][i]) (F32 [2][pairs]: turns
+ * per position and what 32 bits leave of them), and (a, b) becomes magnitude * (a cos t - b sin t, a sin t + b cos t),
+ * with -t if inverse: that is the gradient (dx from dy).  x, y: F32 or BF16; f32 arithmetic, rounded once; y may be x
+ * when the types agree. */
+typedef struct vdsl_rope_params {
+  int64_t rows;
+  int64_t width;
+  int64_t first;
+  int32_t heads;
+  int32_t dim;
+  int32_t pairs;
+  int32_t interleaved;
+  int32_t inverse;
+  float magnitude;
+} vdsl_rope_params;
+int vdsl_op_rope(vdsl_queue q, const vdsl_rope_params* p, int32_t x_dtype, vdsl_buffer x, vdsl_buffer positions,
+                 vdsl_buffer freqs, int32_t y_dtype, vdsl_buffer y);
+
+/* Attention over packed sequences.  Sequence s is rows [starts[s], starts[s + 1]) (I32 [seqs + 1], ascending, of any
+ * lengths, 0 included; values outside [0, n] count as the nearer of the two, and where they do not ascend the results
+ * are unspecified).  Row i of a sequence sees its row j if j <= i or causal is 0.  Head h reads k and v of head
+ * h / (heads / kv_heads) (kv_heads divides heads).  With s[j] = scale * q_i . k_j over the visible j:
+ *   lse[h][i] = log sum_j exp(s[j]),   out[i][h] = sum_j exp(s[j] - lse) v_j
+ * A row of no sequence, or whose scores are -inf all of them, has out 0 and lse -inf.  What a row does not see has no
+ * influence on it, NaN and infinity included.  q, k, v: BF16; scores, sums and statistics are f32, the weights
+ * exp(s[j] - max) are rounded to bf16 for the second product.  out: F32 or BF16 [n][heads * dim], every row written;
+ * lse: F32 [heads][n], or NULL.  dim: a multiple of 8 up to 128.  scale: a positive normal number. */
+typedef struct vdsl_attention_params {
+  int64_t n;
+  int64_t seqs;
+  int32_t heads;
+  int32_t kv_heads;
+  int32_t dim;
+  int32_t causal;
+  float scale;
+  int32_t reserved;   /* 0 */
+  vdsl_heads q, k, v;
+  vdsl_heads dq, dk, dv; /* read by the backward pass only */
+} vdsl_attention_params;
+int vdsl_op_attention_fwd(vdsl_queue q, const vdsl_attention_params* p, vdsl_buffer qs, vdsl_buffer ks, vdsl_buffer vs,
+                          vdsl_buffer starts, int32_t out_dtype, vdsl_buffer out, vdsl_buffer lse);
+/* Its gradient from dout (F32 or BF16 [n][heads * dim]) and the forward pass's out and lse: with
+ * p = exp(s - lse), ds = p * (dout_i . v_j - dout_i . out_i):
+ *   dq_i = scale * sum_j ds k_j,   dk_j = scale * sum_i ds q_i,   dv_j = sum_i p dout_i
+ * (the last two over the rows i that see j and the heads that share j's).  dq, dk, dv: grad_dtype, F32 or BF16, every row
+ * of their heads written (0 for rows of no sequence), columns outside their heads left as they are; they may lie in one
+ * buffer as disjoint columns of one stride.  dout, p and ds are rounded to bf16 for the products, which accumulate in f32.
+ * The same bits on every call.  workspace: vdsl_attention_bwd_workspace_bytes() bytes of any contents (two calls that
+ * overlap in time need two). */
+int vdsl_attention_bwd_workspace_bytes(int64_t n, int64_t seqs, int32_t heads, int32_t kv_heads, int32_t dim, size_t* bytes);
+int vdsl_op_attention_bwd(vdsl_queue q, const vdsl_attention_params* p, int32_t dout_dtype, vdsl_buffer dout, vdsl_buffer qs,
+                          vdsl_buffer ks, vdsl_buffer vs, vdsl_buffer starts, int32_t out_dtype, vdsl_buffer out,
+                          vdsl_buffer lse, int32_t grad_dtype, vdsl_buffer dq, vdsl_buffer dk, vdsl_buffer dv,
+                          vdsl_buffer workspace);
+
+/* A cache of keys and values in pages: k_cache, v_cache BF16 [pages][kv_heads][page][dim] (page a power of two up to
+ * 65536).  Position j of sequence s is slot j % page of page table[s][j / page] (I32 [seqs][table_cols]); an entry outside
+ * [0, pages) is no page: its positions hold nothing.  The new rows of sequence s are [starts[s], starts[s + 1]) (as for
+ * vdsl_op_attention_fwd), m of them; lengths[s] (I32 [seqs]) counts its positions with the new rows: row i of them is
+ * position lengths[s] - m + i.  Positions below 0 or not below table_cols * page hold nothing. */
+typedef struct vdsl_paged_params {
+  int64_t n;
+  int64_t seqs;
+  int64_t pages;
+  int64_t table_cols;
+  int32_t page;
+  int32_t heads;
+  int32_t kv_heads;
+  int32_t dim;
+  float scale;
+  int32_t reserved;   /* 0 */
+  vdsl_heads q, k, v; /* q: read by the attention only, k and v by the append only */
+} vdsl_paged_params;
+/* The new rows' k and v (BF16) into their slots of the cache; rows of no sequence or without a slot are dropped, everything
+ * else in the cache stays.  No two rows may have one slot.  (heads, scale and q are not read.) */
+int vdsl_op_cache_append(vdsl_queue q, const vdsl_paged_params* p, vdsl_buffer ks, vdsl_buffer vs, vdsl_buffer starts,
+                         vdsl_buffer lengths, vdsl_buffer table, vdsl_buffer k_cache, vdsl_buffer v_cache);
+/* Attention of the new rows over the cache, which holds their own keys already: the row at position p sees positions 0 to p.
+ * out, lse, arithmetic and limits as for vdsl_op_attention_fwd; one row a sequence or many.  lengths and table are read on
+ * the device: a recorded call takes what they hold at each replay.  workspace:
+ * vdsl_paged_attention_workspace_bytes() bytes of any contents (two calls that overlap in time need two); it may be NULL
+ * when that is 0. */
+int vdsl_paged_attention_workspace_bytes(int64_t n, int64_t seqs, int32_t heads, int32_t kv_heads, int32_t dim,
+                                         int64_t positions, size_t* bytes); /* positions: table_cols * page */
+int vdsl_op_paged_attention(vdsl_queue q, const vdsl_paged_params* p, vdsl_buffer qs, vdsl_buffer k_cache, vdsl_buffer v_cache,
+                            vdsl_buffer starts, vdsl_buffer lengths, vdsl_buffer table, int32_t out_dtype, vdsl_buffer out,
+                            vdsl_buffer lse, vdsl_buffer workspace);
+
 /* ---- failure injection (tests of error paths, host-side only) ----------------------------- */
 /* After `n` more successful buffer allocations, the next one fails with VDSL_ERR_OUT_OF_MEMORY
  * (n < 0 disables).  While n is 0, queues and recordings get no scratch memory either (which fails

@@ -96,6 +96,27 @@ class MapVInput(C.Structure):
                 ("mat_dim", C.c_int32)]
 
 
+class Heads(C.Structure):
+    _fields_ = [("first", C.c_int64), ("stride", C.c_int64)]
+
+
+class RopeParams(C.Structure):
+    _fields_ = [("rows", C.c_int64), ("width", C.c_int64), ("first", C.c_int64), ("heads", C.c_int32), ("dim", C.c_int32),
+                ("pairs", C.c_int32), ("interleaved", C.c_int32), ("inverse", C.c_int32), ("magnitude", C.c_float)]
+
+
+class AttentionParams(C.Structure):
+    _fields_ = [("n", C.c_int64), ("seqs", C.c_int64), ("heads", C.c_int32), ("kv_heads", C.c_int32), ("dim", C.c_int32),
+                ("causal", C.c_int32), ("scale", C.c_float), ("reserved", C.c_int32), ("q", Heads), ("k", Heads), ("v", Heads),
+                ("dq", Heads), ("dk", Heads), ("dv", Heads)]
+
+
+class PagedParams(C.Structure):
+    _fields_ = [("n", C.c_int64), ("seqs", C.c_int64), ("pages", C.c_int64), ("table_cols", C.c_int64), ("page", C.c_int32),
+                ("heads", C.c_int32), ("kv_heads", C.c_int32), ("dim", C.c_int32), ("scale", C.c_float), ("reserved", C.c_int32),
+                ("q", Heads), ("k", Heads), ("v", Heads)]
+
+
 _vp = C.c_void_p
 _i32 = C.c_int32
 _i64 = C.c_int64
@@ -174,6 +195,14 @@ PROTOTYPES = {
     "vdsl_op_linear_xent_fwd": (C.c_int, [_vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "vdsl_op_linear_xent_fwd_bwd": (C.c_int, [_vp, _i64, _i64, _i64, _vp, _vp, _vp, _i64, C.c_float, _vp, _vp, _vp, _i32, _vp,
                                               _i32, _vp, _vp]),
+    "vdsl_op_rope": (C.c_int, [_vp, C.POINTER(RopeParams), _i32, _vp, _vp, _vp, _i32, _vp]),
+    "vdsl_op_attention_fwd": (C.c_int, [_vp, C.POINTER(AttentionParams), _vp, _vp, _vp, _vp, _i32, _vp, _vp]),
+    "vdsl_attention_bwd_workspace_bytes": (C.c_int, [_i64, _i64, _i32, _i32, _i32, C.POINTER(_sz)]),
+    "vdsl_op_attention_bwd": (C.c_int, [_vp, C.POINTER(AttentionParams), _i32, _vp, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _i32, _vp,
+                                        _vp, _vp, _vp]),
+    "vdsl_op_cache_append": (C.c_int, [_vp, C.POINTER(PagedParams), _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "vdsl_paged_attention_workspace_bytes": (C.c_int, [_i64, _i64, _i32, _i32, _i32, _i64, C.POINTER(_sz)]),
+    "vdsl_op_paged_attention": (C.c_int, [_vp, C.POINTER(PagedParams), _vp, _vp, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _vp]),
     "vdsl_debug_fail_alloc_after": (C.c_int, [_i64]),
     "vdsl_debug_gemm_config": (C.c_int, [_i32]),
     "vdsl_debug_linear_xent_plan": (C.c_int, [_i64, _i64, _i64, _i64, C.POINTER(_i64)]),

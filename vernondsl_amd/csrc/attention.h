@@ -1,0 +1,199 @@
+// What the attention kernels share: sequences and rows, tiles of keys in LDS, fragments.
+//
+// Rows.  A sequence's tokens and the `group` heads that share a kv head make its rows: row r is token r / group, head
+// r % group of the kv head, so a tile of rows shares every key it reads among tokens and heads alike, a few new
+// tokens fill a tile, and a tile's rows see nearly the same keys.  Row tiles do not cross sequences.  Which tile a block has
+// follows from `starts` on the device: piece i of the rows (0: those before the first sequence, 1 .. seqs the sequences,
+// seqs + 1 those behind the last) has the slots from floor(first row of it / tile) + i on, which leaves each piece as
+// many as it needs, so that a grid of floor(all rows / tile) + seqs + 2 slots holds every tile and no pass counts them first.
+//
+// Products.  Scores are formed transposed, S^T = K Q^T: of a 32 x 32 tile a lane then has one row's scores of 16 keys, so
+// the softmax needs one exchange between the wave's halves, and what a lane holds of P^T is its part of the second
+// product's operand as it is, once the sum over keys is taken in the order in which the accumulators have them: step e
+// of 16 keys takes keys 16 e + 8 (j / 4) + 4 (lane / 32) + j % 4 as its elements j of a lane.  V^T comes in that order
+// from transposing LDS reads of 4 neighbouring keys each.
+#pragma once
+
+#include "gemm_dma.h"
+#include "rowunit.h"
+
+namespace vdsl {
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+__device__ __forceinline__ float neg_inf() { return -__builtin_inff(); }
+
+// The largest i in [0, count) with below(i), for a `below` that holds from 0 up to some i; every lane of the wave asks the
+// same.  64 places at a time: one round trip for up to 64, two for 4096.
+template <class Below>
+__device__ __forceinline__ int64_t wave_search(int64_t count, Below&& below) {
+  const int lane = threadIdx.x & 63;
+  int64_t lo = 0, hi = count;
+  while (hi - lo > 1) {
+    const int64_t step = (hi - lo + 63) / 64, at = lo + lane * step;
+    const uint64_t yes = __ballot(at < hi && below(at));
+    const int n = yes ? __popcll(yes) : 1;  // place lo is below
+    const int64_t from = lo + (n - 1) * step;
+    hi = from + step < hi ? from + step : hi;
+    lo = from;
+  }
+  return lo;
+}
+
+struct Sequences {
+  const int32_t* starts;
+  int64_t n, seqs;
+  // Row token i of the seqs + 3 borders of the pieces.
+  __device__ __forceinline__ int64_t border(int64_t i) const {
+    if (i == 0) return 0;
+    if (i > seqs + 1) return n;
+    const int64_t s = starts[i - 1];
+    return s < 0 ? 0 : s > n ? n : s;
+  }
+};
+
+struct RowTile {
+  int64_t seq;    // -1: rows of no sequence
+  int64_t token;  // the piece's first token
+  int len;        // its tokens
+  int row;        // the tile's first row in the piece
+  bool any;       // whether it has one
+};
+template <int LOG_TILE>
+__device__ __forceinline__ RowTile row_tile(const Sequences& s, int group, int64_t slot) {
+  const int64_t i = wave_search(s.seqs + 2, [&](int64_t p) { return ((s.border(p) * group) >> LOG_TILE) + p <= slot; });
+  RowTile t;
+  t.token = s.border(i);
+  const int64_t len = s.border(i + 1) - t.token;
+  t.len = len > 0 ? static_cast<int>(len) : 0;
+  t.seq = i >= 1 && i <= s.seqs ? i - 1 : -1;
+  const int64_t row = (slot - ((t.token * group) >> LOG_TILE) - i) << LOG_TILE;
+  t.any = row >= 0 && row < static_cast<int64_t>(t.len) * group;
+  t.row = t.any ? static_cast<int>(row) : 0;
+  return t;
+}
+inline int64_t row_slots(int64_t n, int64_t seqs, int64_t group, int log_tile) { return ((n * group) >> log_tile) + seqs + 2; }
+
+// ---- tiles of key rows in LDS ---------------------------------------------------------------------
+// DP: a head's columns, a multiple of 32 (those past dim are zeros).  A row takes PITCH bytes in 16-byte chunks, chunk c
+// in place c ^ swz(row).  Read as rows, 16 neighbouring rows are read at one chunk together: swz puts them into 16 bank
+// groups.  Read as columns, 64 bytes of each of 4 neighbouring rows: swz puts them into the four quarters of the banks.
+template <int DP>
+struct TileShape {
+  static constexpr int PITCH = DP <= 64 ? 128 : 256;
+  static constexpr int CPR = PITCH / 16;
+  static __device__ __forceinline__ int swz(int row) {
+    return PITCH == 256 ? ((row & 3) << 2) | ((row >> 2) & 3) : (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
+  }
+};
+
+// The fragment of rows row0 .. + 31, k-step kk (16 columns): element j of lane l is column 16 kk + 8 (l / 32) + j of row
+// row0 + l % 32.  row0 is a multiple of 32.
+template <int DP>
+__device__ __forceinline__ bf16x8 rows_fragment(const char* area, int row0, int kk) {
+  using T = TileShape<DP>;
+  const int lane = threadIdx.x & 63;
+  return *reinterpret_cast<const bf16x8*>(area + row0 * T::PITCH + (lane & 31) * T::PITCH +
+                                          (((2 * kk + (lane >> 5)) ^ T::swz(lane & 31)) << 4));
+}
+// The fragment of columns col0 .. + 31 over the 16 rows from row0 on: element j of lane l is column col0 + l % 32 of row
+// row0 + 8 (j / 4) + 4 (l / 32) + j % 4.  row0 is a multiple of 16, col0 of 32.
+template <int DP>
+__device__ __forceinline__ bf16x8 cols_fragment(const char* area, int row0, int col0) {
+  using T = TileShape<DP>;
+  const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
+  const int r = 4 * (g >> 1) + (i >> 2);
+  const int chunk = (col0 / 8 + 2 * (g & 1) + ((i & 3) >> 1)) ^ T::swz(r);
+  const char* const p = area + row0 * T::PITCH + r * T::PITCH + (i & 1) * 8;
+  // 8 rows further swz has the other bit 1
+  const i16x4_t lo = lds_read_tr16(p + (chunk << 4)), hi = lds_read_tr16(p + 8 * T::PITCH + ((chunk ^ 2) << 4));
+  return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+// The values of lanes l % 32 and l % 32 + 32, in every lane.
+__device__ __forceinline__ f32x2_t both_halves(float v) {
+  const uint32_t b = __builtin_bit_cast(uint32_t, v);
+  const auto r = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+  const uint32_t lo = r[0], hi = r[1];  // (a bit cast of r[1] itself takes element 0)
+  return f32x2_t{__builtin_bit_cast(float, lo), __builtin_bit_cast(float, hi)};
+}
+__device__ __forceinline__ float halves_max(float v) {
+  const f32x2_t r = both_halves(v);
+  return fmaxf(r[0], r[1]);
+}
+__device__ __forceinline__ float halves_sum(float v) {
+  const f32x2_t r = both_halves(v);
+  return r[0] + r[1];
+}
+
+// Registers 8 e .. 8 e + 7 of a score tile as the operand of a step over its 16 keys.
+__device__ __forceinline__ bf16x8 weights_fragment(const f32x16& s, int e) {
+  const u32x4 w = {pack_bf16x2(s[8 * e], s[8 * e + 1]), pack_bf16x2(s[8 * e + 2], s[8 * e + 3]),
+                   pack_bf16x2(s[8 * e + 4], s[8 * e + 5]), pack_bf16x2(s[8 * e + 6], s[8 * e + 7])};
+  return __builtin_bit_cast(bf16x8, w);
+}
+
+// Sets a bit of each of x's eight elements that is no finite number (bit 15 of its half word).
+__device__ __forceinline__ uint32_t not_finite(const bf16x8& x) {
+  const u32x4 w = __builtin_bit_cast(u32x4, x);
+  uint32_t f = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) f |= (w[j] & 0x7F807F80u) + 0x00800080u;
+  return f & 0x80008000u;
+}
+
+// One of a step's 16 places alone, the others zero: of both operands it leaves the product's terms of that one.
+__device__ __forceinline__ bf16x8 only_place(const bf16x8& x, int place) {
+  const int half = (threadIdx.x & 63) >> 5;
+  const u32x4 w = __builtin_bit_cast(u32x4, x);
+  u32x4 r;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int k0 = 8 * (j / 2) + 4 * half + 2 * (j % 2);
+    r[j] = (k0 == place ? w[j] & 0xFFFFu : 0u) | (k0 + 1 == place ? w[j] & 0xFFFF0000u : 0u);
+  }
+  return __builtin_bit_cast(bf16x8, r);
+}
+
+// acc += the product of 16 rows of a tile, read as columns, with weights w, where some lanes do not see some of these rows and
+// an element is no finite number: 0 times it would be NaN for every lane.  Place by place, and each lane takes those that
+// it sees: from lo on, below hi, and set in valid.
+template <int DP>
+__device__ __forceinline__ void add_seen(f32x16 (&acc)[DP / 32], const char* area, int row0, const bf16x8& w, int lo, int hi, uint32_t valid) {
+#pragma unroll 1
+  for (int place = 0; place < 16; ++place) {
+    const bf16x8 b = only_place(w, place);
+    const bool in = place >= lo && place < hi && ((valid >> place) & 1);
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) {
+      const f32x16 t = MfmaBf16::mma(only_place(cols_fragment<DP>(area, row0, 32 * d), place), b, MfmaBf16::zero());
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[d][r] += in ? t[r] : 0.0f;
+    }
+  }
+}
+// Whether a tile's rows row0 .. + 16 steps - 1 hold an element that is no finite number.
+template <int DP>
+__device__ __forceinline__ bool any_not_finite(const char* area, int row0, int steps) {
+  uint32_t f = 0;
+  for (int e = 0; e < steps; ++e)
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) f |= not_finite(cols_fragment<DP>(area, row0 + 16 * e, 32 * d));
+  return __any(f != 0);
+}
+
+// r / group for r below 2^31.
+struct Divider {
+  uint32_t by, mul;
+  int shift;
+  __device__ __forceinline__ int operator()(int r) const {
+    return by == 1 ? r : static_cast<int>(__umulhi(static_cast<uint32_t>(r), mul) >> shift);
+  }
+};
+// With 2^l >= group, mul = ceil(2^(31 + l) / group) < 2^32 gives floor(r mul / 2^(31 + l)) = floor(r / group).
+inline Divider divider(int group) {
+  int l = 0;
+  while ((int64_t{1} << l) < group) ++l;
+  return {static_cast<uint32_t>(group), l ? static_cast<uint32_t>(((uint64_t{1} << (31 + l)) + group - 1) / group) : 0u, l - 1};
+}
+
+}  // namespace vdsl

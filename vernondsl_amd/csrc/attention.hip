@@ -1,0 +1,688 @@
+// Attention forward: over packed sequences, and of new rows over a paged cache; and the append to that cache.
+//
+// For a row's scores s over the keys it sees: m = max s, p = exp2(c (s - m)), l = sum p, out = sum p v / l, with
+// c = scale log2 e; one pass over the keys, tile by tile, with m, l and the unnormalised output carried along and
+// rescaled where m grows.  m may lag behind the maximum by a factor of 2^8 in p (bf16 and f32 hold that without loss), so
+// most tiles rescale nothing.  See attention.h for rows, tiles and the order of keys in the products.
+#include <algorithm>
+#include <cmath>
+
+#include "attention.h"
+
+namespace vdsl {
+namespace {
+
+struct AttentionArgs {
+  const uint16_t *q, *k, *v;
+  int64_t q_stride, k_stride, v_stride;
+  Sequences seqs;
+  const int32_t *lengths, *table;  // paged
+  void* out;
+  float* lse;
+  float* parts;  // of splits: the unnormalised outputs, f32 [splits][kv_heads][n * group][dim]
+  float2* stats; // and m c and l, [splits][kv_heads][n * group]
+  int heads, kv_heads, group, dim, causal, out_dtype;
+  float scale;
+  int64_t pages;
+  int table_cols, page_shift;
+  int splits, blocks;
+};
+
+constexpr float kLag = 8.0f;  // by how much m may lag, in powers of two
+
+// Keys of one sequence and kv head, as tiles of KT rows for copies of NW waves.
+template <int DP, int KT, int NW, bool PAGED>
+struct KeySource {
+  using T = TileShape<DP>;
+  static constexpr int C = KT * T::PITCH / 1024 / NW;  // copies of a wave for a tile's keys, and as many for its values
+  const char *k, *v;       // packed: of the sequence's first key; paged: the caches
+  uint32_t k_row, v_row;   // packed: bytes from a key to the next
+  int keys, head, kv_heads, dim, table_cols, shift;
+  int64_t pages;
+  const int32_t* table;    // the sequence's pages
+  int row_of[C], chunk[C];
+
+  __device__ __forceinline__ void lanes(int wave) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int u = 0; u < C; ++u) {
+      row_of[u] = (wave * C + u) * (64 / T::CPR) + lane / T::CPR;
+      chunk[u] = lane % T::CPR ^ T::swz(row_of[u]);
+    }
+  }
+  // Paged: this lane's entry of the page table for key j0 + lane (-1: none), loaded a tile before it is used.
+  __device__ __forceinline__ int entry(int j0) const {
+    const int j = j0 + (threadIdx.x & 63);
+    int e = -1;
+    if (j < keys) {
+      e = table[j >> shift];
+      if (static_cast<uint32_t>(e) >= static_cast<uint64_t>(pages)) e = -1;
+    }
+    return e;
+  }
+  // Tile j0 to the slot at `to` (its keys, then its values).  Keys past the last one repeat it, keys without a page take
+  // page 0: they are masked.
+  __device__ __forceinline__ void copy(int j0, int entries, char* to, int wave) const {
+    const int dc = dim / 8;
+    if constexpr (!PAGED) {
+      const char* const kb = k + static_cast<int64_t>(j0) * k_row;
+      const char* const vb = v + static_cast<int64_t>(j0) * v_row;
+      const int last = keys - 1 - j0;
+#pragma unroll
+      for (int u = 0; u < C; ++u) {
+        const uint32_t r = min(row_of[u], last);
+        if (chunk[u] >= dc) continue;
+        lds_copy16(kb + r * k_row + 16 * chunk[u], to + (wave * C + u) * 1024);
+        lds_copy16(vb + r * v_row + 16 * chunk[u], to + KT * T::PITCH + (wave * C + u) * 1024);
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < C; ++u) {
+        const int r = min(row_of[u], keys - 1 - j0);
+        const int e = max(__shfl(entries, r, 64), 0);
+        const int64_t at = ((static_cast<int64_t>(e) * kv_heads + head) << shift) + ((j0 + r) & ((1 << shift) - 1));
+        if (chunk[u] >= dc) continue;
+        lds_copy16(k + at * k_row + 16 * chunk[u], to + (wave * C + u) * 1024);
+        lds_copy16(v + at * v_row + 16 * chunk[u], to + KT * T::PITCH + (wave * C + u) * 1024);
+      }
+    }
+  }
+};
+
+// What a block's rows see, and where they are.
+struct RowsAt {
+  int64_t token;  // of row 0 of the piece
+  int len, rows;  // tokens and rows of the piece
+  int keys;       // of its sequence
+  int before;     // keys before its first token (negative: its first tokens have none)
+  __device__ __forceinline__ int sees(int row, int group, int causal) const {
+    const int pos = before + row / group;
+    return causal ? min(max(pos + 1, 0), keys) : keys;
+  }
+};
+template <bool PAGED>
+__device__ __forceinline__ RowsAt rows_at(const AttentionArgs& a, const RowTile& t) {
+  RowsAt r;
+  r.token = t.token;
+  r.len = t.len;
+  r.rows = t.len * a.group;
+  r.keys = t.len;
+  r.before = 0;
+  if constexpr (PAGED) {
+    if (t.seq >= 0) {
+      const int64_t have = a.lengths[t.seq], room = static_cast<int64_t>(a.table_cols) << a.page_shift;
+      const int64_t before = have - t.len;
+      r.keys = static_cast<int>(have < 0 || a.pages == 0 ? 0 : have < room ? have : room);
+      r.before = static_cast<int>(before < -0x7fffffff ? -0x7fffffff : before);
+    }
+  }
+  if (t.seq < 0) r.keys = 0;
+  return r;
+}
+
+// The state of a wave's QT tiles of 32 rows: this lane has row lane % 32 of each and, of its 32 x (16 DP / 32) outputs,
+// o[c][d][r] of column 32 d + 8 (r / 4) + 4 (lane / 32) + r % 4.
+template <int DP, int QT>
+struct RowState {
+  f32x16 o[QT][DP / 32];
+  float m[QT], l[QT];  // m in powers of two (times c); l: this half's share
+
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int c = 0; c < QT; ++c) {
+      m[c] = neg_inf();
+      l[c] = 0.0f;
+#pragma unroll
+      for (int d = 0; d < DP / 32; ++d) o[c][d] = MfmaBf16::zero();
+    }
+  }
+  // s: the scores of row tile c over KS x 32 keys, those that are not seen -inf; they become p.
+  template <int KS>
+  __device__ __forceinline__ void weigh(f32x16 (&s)[KS], int c, float scale2) {
+    float top = s[0][0];
+#pragma unroll
+    for (int t = 0; t < KS; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[t][r]);
+    top = halves_max(top) * scale2;
+    if (__any(top > m[c] + kLag)) {
+      const float now = fmaxf(m[c], top);
+      const float by = now == neg_inf() ? 1.0f : __builtin_amdgcn_exp2f(m[c] - now);
+      m[c] = now;
+      l[c] *= by;
+#pragma unroll
+      for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[c][d][r] *= by;
+    }
+    const float at = m[c] == neg_inf() ? 0.0f : m[c];
+    float sum = 0.0f;
+#pragma unroll
+    for (int t = 0; t < KS; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[t][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][r], scale2, -at));
+        sum += s[t][r];
+      }
+    l[c] += sum;
+  }
+};
+
+// Hides what a row does not see of a tile of KS x 32 keys.  sees: of the row, less the tile's first key.
+template <int KS>
+__device__ __forceinline__ void hide(f32x16 (&s)[KS], int sees, uint64_t valid) {
+  const int half = 4 * ((threadIdx.x & 63) >> 5);
+  const uint64_t mine = valid >> half;
+#pragma unroll
+  for (int t = 0; t < KS; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int j = 32 * t + 8 * (r / 4) + r % 4;
+      if (!(j < sees - half) || !((mine >> j) & 1)) s[t][r] = neg_inf();
+    }
+}
+
+// The rows' outputs (or their parts of split `split`) from a wave's state.
+template <int DP, int QT>
+__device__ __forceinline__ void store_rows(const AttentionArgs& a, RowState<DP, QT>& st, const RowsAt& at, int row0, int kv, int split) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int c = 0; c < QT; ++c) {
+    const int row = row0 + 32 * c + (lane & 31);
+    const float l = halves_sum(st.l[c]);
+    if (row >= at.rows) continue;
+    const int64_t token = at.token + row / a.group;
+    const int head = kv * a.group + row % a.group;
+    float by;
+    int64_t base;
+    if (a.splits > 1) {
+      const int64_t place = (static_cast<int64_t>(split) * a.kv_heads + kv) * a.seqs.n * a.group + at.token * a.group + row;
+      if (lane < 32) a.stats[place] = make_float2(st.m[c], l);
+      if (st.m[c] == neg_inf()) continue;  // not read
+      by = 1.0f;
+      base = place * a.dim;
+    } else {
+      if (a.lse && lane < 32)
+        a.lse[head * a.seqs.n + token] = st.m[c] == neg_inf() ? neg_inf() : (st.m[c] + __builtin_amdgcn_logf(l)) * kLn2;
+      by = st.m[c] == neg_inf() ? 0.0f : 1.0f / l;
+      base = (token * a.heads + head) * a.dim;
+    }
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int col = 32 * d + 8 * g + 4 * (lane >> 5);
+        if (col >= a.dim) continue;
+        float v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = st.o[c][d][4 * g + j] * by;
+        if (a.splits > 1) store_whole<VDSL_F32, 4>(a.parts, base + col, v);
+        else store_unit<4>(a.out_dtype, a.out, base + col, v);
+      }
+  }
+}
+
+// Rows of no sequence, or that see no key: out 0, lse -inf.
+__device__ __forceinline__ void store_none(const AttentionArgs& a, const RowsAt& at, int row0, int rows, int kv, int split) {
+  rows = min(rows, at.rows - row0);
+  if (a.splits > 1) {
+    const int64_t place = (static_cast<int64_t>(split) * a.kv_heads + kv) * a.seqs.n * a.group + at.token * a.group + row0;
+    for (int r = threadIdx.x; r < rows; r += blockDim.x) a.stats[place + r] = make_float2(neg_inf(), 0.0f);
+    return;
+  }
+  const float none[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  const int per = a.dim / 4;
+  for (int u = threadIdx.x; u < rows * per; u += blockDim.x) {
+    const int row = row0 + u / per;
+    const int64_t token = at.token + row / a.group;
+    const int head = kv * a.group + row % a.group;
+    store_unit<4>(a.out_dtype, a.out, (token * a.heads + head) * a.dim + 4 * (u % per), none);
+    if (a.lse && u % per == 0) a.lse[head * a.seqs.n + token] = neg_inf();
+  }
+}
+
+// A wave's QT tiles of rows as the operand Q^T: element j of lane l is column 16 kk + 8 (l / 32) + j.
+template <int DP, int QT>
+__device__ __forceinline__ void load_rows(const AttentionArgs& a, const RowsAt& at, int row0, int kv, bf16x8 (&f)[QT][DP / 16]) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int c = 0; c < QT; ++c) {
+    const int row = min(row0 + 32 * c + (lane & 31), at.rows - 1);
+    const uint16_t* const p = a.q + (at.token + row / a.group) * a.q_stride + static_cast<int64_t>(kv * a.group + row % a.group) * a.dim;
+#pragma unroll
+    for (int kk = 0; kk < DP / 16; ++kk) {
+      const int col = 16 * kk + 8 * (lane >> 5);
+      u32x4 w = {0u, 0u, 0u, 0u};
+      if (col < a.dim) w = *reinterpret_cast<const u32x4*>(p + col);
+      f[c][kk] = __builtin_bit_cast(bf16x8, w);
+    }
+  }
+}
+
+template <bool PAGED, class Source>
+__device__ __forceinline__ void open_keys(const AttentionArgs& a, const RowTile& t, const RowsAt& at, int kv, Source& src) {
+  src.keys = at.keys;
+  src.head = kv;
+  src.kv_heads = a.kv_heads;
+  src.dim = a.dim;
+  src.table_cols = a.table_cols;
+  src.shift = a.page_shift;
+  src.pages = a.pages;
+  if constexpr (PAGED) {
+    src.k = reinterpret_cast<const char*>(a.k);
+    src.v = reinterpret_cast<const char*>(a.v);
+    src.k_row = src.v_row = 2 * a.dim;
+    src.table = a.table + (t.seq < 0 ? 0 : t.seq) * a.table_cols;
+  } else {
+    src.k = reinterpret_cast<const char*>(a.k + at.token * a.k_stride + static_cast<int64_t>(kv) * a.dim);
+    src.v = reinterpret_cast<const char*>(a.v + at.token * a.v_stride + static_cast<int64_t>(kv) * a.dim);
+    src.k_row = static_cast<uint32_t>(2 * a.k_stride);
+    src.v_row = static_cast<uint32_t>(2 * a.v_stride);
+  }
+}
+
+// The block's place: kv head, row slot and split.  Blocks that are dispatched together (to the XCDs in turn) have
+// different kv heads, so that an XCD reads few heads' keys where there are 8 or more; the last rows, which see most, first.
+struct Place {
+  int kv, split;
+  int64_t slot;
+  __device__ __forceinline__ Place(const AttentionArgs& a) {
+    int b = static_cast<int>(blockIdx.x);
+    kv = b % a.kv_heads;
+    b /= a.kv_heads;
+    split = b % a.splits;
+    slot = a.blocks - 1 - b / a.splits;
+  }
+};
+
+// Four waves of QT x 32 rows each, sharing tiles of 64 keys through a ring of NS slots.
+template <int DP, int QT, bool PAGED>
+__global__ __launch_bounds__(256, QT == 1 ? 2 : 1) void attention_rows(AttentionArgs a) {
+  constexpr int KT = 64, KS = KT / 32, NS = QT == 1 ? 2 : 4, ROWS = 128 * QT;
+  using T = TileShape<DP>;
+  constexpr int SLOT = 2 * KT * T::PITCH;
+  __shared__ __attribute__((aligned(1024))) char smem[NS * SLOT];
+  const Place place(a);
+  const RowTile tile = row_tile<QT == 1 ? 7 : 8>(a.seqs, a.group, place.slot);
+  if (!tile.any) return;
+  const RowsAt at = rows_at<PAGED>(a, tile);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int last_row = min(tile.row + ROWS, at.rows) - 1;
+  const int sees_most = at.sees(last_row, a.group, a.causal);
+  // the split's share of the block's tiles of keys
+  const int tiles = (sees_most + KT - 1) / KT;
+  const int share = (tiles + a.splits - 1) / a.splits;
+  const int first = place.split * share, end = min(first + share, tiles);
+  if (first >= end) {
+    store_none(a, at, tile.row, ROWS, place.kv, place.split);
+    return;
+  }
+  KeySource<DP, KT, 4, PAGED> src;
+  open_keys<PAGED>(a, tile, at, place.kv, src);
+  src.lanes(wave);
+  if (2 * a.dim < T::PITCH) {  // columns past dim are never copied
+    for (int i = threadIdx.x; i < NS * SLOT / 16; i += 256) reinterpret_cast<u32x4*>(smem)[i] = u32x4{0u, 0u, 0u, 0u};
+    __syncthreads();
+  }
+  uint64_t valid[NS];  // paged: which keys of a slot's tile hold something
+  int entries = -1;
+  const auto fetch = [&](int t, int slot) {
+    if constexpr (PAGED) valid[slot] = __ballot(entries >= 0);
+    src.copy(t * KT, entries, smem + slot * SLOT, wave);
+  };
+#pragma unroll
+  for (int t = 0; t < NS - 1; ++t) {
+    valid[t] = ~0ull;
+    if constexpr (PAGED) entries = src.entry(min(first + t, end - 1) * KT);
+    fetch(min(first + t, end - 1), t);
+  }
+  valid[NS - 1] = ~0ull;
+  if constexpr (PAGED) entries = src.entry(min(first + NS - 1, end - 1) * KT);
+
+  const int row0 = tile.row + wave * 32 * QT;
+  const bool mine = row0 < at.rows;
+  const float scale2 = a.scale * kLog2e;
+  bf16x8 qf[QT][DP / 16];
+  RowState<DP, QT> st;
+  st.clear();
+  int sees[QT];
+#pragma unroll
+  for (int c = 0; c < QT; ++c) sees[c] = at.sees(min(row0 + 32 * c + (lane & 31), at.rows - 1), a.group, a.causal);
+  load_rows<DP, QT>(a, at, mine ? row0 : 0, place.kv, qf);
+  // of the wave's rows: the fewest and the most keys that one sees
+  const int fewest = __builtin_amdgcn_readfirstlane(at.sees(min(row0, at.rows - 1), a.group, a.causal));
+  const int most = mine ? at.sees(min(row0 + 32 * QT, at.rows) - 1, a.group, a.causal) : 0;
+
+  for (int t0 = first; t0 < end; t0 += NS) {
+#pragma unroll
+    for (int slot = 0; slot < NS; ++slot) {
+      const int t = t0 + slot;
+      if (t >= end) break;
+      // copies of the tiles behind t stay in flight
+      if constexpr (PAGED) dma_wait<0>();
+      else dma_wait<(NS - 2) * 2 * KeySource<DP, KT, 4, PAGED>::C>();
+      dma_barrier();
+      {
+        constexpr int ahead = NS - 1;
+        const int to = (slot + ahead) % NS;
+        fetch(min(t + ahead, end - 1), to);  // past the end the last tile again, so that the waits count the same
+        if constexpr (PAGED) entries = src.entry(min(t + NS, end - 1) * KT);
+      }
+      const int j0 = t * KT;
+      if (j0 >= most) continue;
+      const char* const keys = smem + slot * SLOT;
+      const char* const values = keys + KT * T::PITCH;
+      f32x16 s[QT][KS];
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+#pragma unroll
+        for (int c = 0; c < QT; ++c) s[c][k] = MfmaBf16::zero();
+#pragma unroll
+        for (int kk = 0; kk < DP / 16; ++kk) {
+          const bf16x8 f = rows_fragment<DP>(keys, 32 * k, kk);
+#pragma unroll
+          for (int c = 0; c < QT; ++c) s[c][k] = MfmaBf16::mma(f, qf[c][kk], s[c][k]);
+        }
+      }
+      const bool masked = j0 + KT > fewest || (PAGED && valid[slot] != ~0ull);
+      if (masked) {
+#pragma unroll
+        for (int c = 0; c < QT; ++c) hide(s[c], sees[c] - j0, valid[slot]);
+      }
+#pragma unroll
+      for (int c = 0; c < QT; ++c) st.weigh(s[c], c, scale2);
+      if (masked && any_not_finite<DP>(values, 0, 2 * KS)) {
+#pragma unroll
+        for (int e = 0; e < 2 * KS; ++e)
+#pragma unroll
+          for (int c = 0; c < QT; ++c)
+            add_seen<DP>(st.o[c], values, 16 * e, weights_fragment(s[c][e / 2], e % 2), 0, sees[c] - j0 - 16 * e,
+                         static_cast<uint32_t>(valid[slot] >> (16 * e)) & 0xFFFFu);
+        continue;
+      }
+#pragma unroll
+      for (int e = 0; e < 2 * KS; ++e) {
+        bf16x8 w[QT];
+#pragma unroll
+        for (int c = 0; c < QT; ++c) w[c] = weights_fragment(s[c][e / 2], e % 2);
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) {
+          const bf16x8 f = cols_fragment<DP>(values, 16 * e, 32 * d);
+#pragma unroll
+          for (int c = 0; c < QT; ++c) st.o[c][d] = MfmaBf16::mma(f, w[c], st.o[c][d]);
+        }
+      }
+    }
+  }
+  dma_wait<0>();
+  if (mine) store_rows(a, st, at, row0, place.kv, place.split);
+}
+
+// Joins the splits: with M = max m, out = sum 2^(m - M) o / sum 2^(m - M) l.  32 lanes a row.
+__global__ __launch_bounds__(256) void attention_join(AttentionArgs a) {
+  const int64_t rows = a.seqs.n * a.group, all = rows * a.kv_heads;
+  const int64_t r = block_index() * 8 + (threadIdx.x >> 5);
+  if (r >= all) return;
+  const int kv = static_cast<int>(r / rows);
+  const int64_t token = r % rows / a.group;
+  const int head = kv * a.group + static_cast<int>(r % rows % a.group);
+  float m = neg_inf();
+  for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.stats[s * all + r].x);
+  const int col = 4 * (threadIdx.x & 31);
+  float v[4] = {0.0f, 0.0f, 0.0f, 0.0f}, l = 0.0f;
+  for (int s = 0; s < a.splits; ++s) {
+    const float2 st = a.stats[s * all + r];
+    if (st.x == neg_inf()) continue;
+    const float by = __builtin_amdgcn_exp2f(st.x - m);
+    l += by * st.y;
+    if (col >= a.dim) continue;
+    float o[4];
+    load_whole<VDSL_F32, 4>(a.parts, (s * all + r) * a.dim + col, o);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] += by * o[j];
+  }
+  const bool none = m == neg_inf();
+  if (a.lse && col == 0) a.lse[head * a.seqs.n + token] = none ? neg_inf() : (m + __builtin_amdgcn_logf(l)) * kLn2;
+  if (col >= a.dim) return;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = none ? 0.0f : v[j] / l;
+  store_unit<4>(a.out_dtype, a.out, (token * a.heads + head) * a.dim + col, v);
+}
+
+// A block per new row: its keys and values of all kv heads into their slots.
+__global__ __launch_bounds__(256) void cache_append_rows(AttentionArgs a, uint16_t* __restrict__ k_cache, uint16_t* __restrict__ v_cache) {
+  const int64_t row = block_index();
+  if (row >= a.seqs.n) return;
+  const int64_t i = wave_search(a.seqs.seqs + 2, [&](int64_t p) { return a.seqs.border(p) <= row; });
+  if (i < 1 || i > a.seqs.seqs) return;
+  const int64_t pos = a.lengths[i - 1] - (a.seqs.border(i + 1) - row);
+  if (pos < 0 || pos >= (static_cast<int64_t>(a.table_cols) << a.page_shift)) return;
+  const int64_t page = a.table[(i - 1) * a.table_cols + (pos >> a.page_shift)];
+  if (page < 0 || page >= a.pages) return;
+  const int per = a.dim / 8, slot = static_cast<int>(pos) & ((1 << a.page_shift) - 1);
+  for (int u = threadIdx.x; u < 2 * a.kv_heads * per; u += 256) {
+    const bool is_v = u >= a.kv_heads * per;
+    const int x = is_v ? u - a.kv_heads * per : u;
+    const int64_t to = ((((page * a.kv_heads + x / per) << a.page_shift) + slot) * per + x % per) * 8;
+    const uint16_t* const from = is_v ? a.v + row * a.v_stride : a.k + row * a.k_stride;
+    *reinterpret_cast<u32x4*>((is_v ? v_cache : k_cache) + to) = *reinterpret_cast<const u32x4*>(from + 8 * x);
+  }
+}
+
+bool float_type(int32_t t) { return t == VDSL_F32 || t == VDSL_BF16; }
+
+template <bool PAGED>
+int launch_rows(vdsl_queue q, AttentionArgs& a, int qt) {
+  const int log_tile = qt == 1 ? 7 : 8;
+  const int64_t slots = row_slots(a.seqs.n, a.seqs.seqs, a.group, log_tile);
+  const int64_t blocks = slots * a.kv_heads * a.splits;
+  if (slots > 0x7fffffff || blocks > 0x7fffff) return fail(VDSL_ERR_UNSUPPORTED, "attention: too many rows");
+  a.blocks = static_cast<int>(slots);
+  const auto go = [&](auto kernel, const char* name) {
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, q->stream, a);
+    return check_launch(name);
+  };
+  if (a.dim <= 64) return go(qt == 1 ? attention_rows<64, 1, PAGED> : attention_rows<64, 2, PAGED>, "attention_rows");
+  if (a.dim <= 96) return go(qt == 1 ? attention_rows<96, 1, PAGED> : attention_rows<96, 2, PAGED>, "attention_rows");
+  return go(qt == 1 ? attention_rows<128, 1, PAGED> : attention_rows<128, 2, PAGED>, "attention_rows");
+}
+
+}  // namespace
+
+// Checks shared by the attention ops.
+int attention_check_shape(const char* op, int64_t n, int64_t seqs, int32_t heads, int32_t kv_heads, int32_t dim) {
+  const std::string name = op;
+  if (n < 0 || seqs < 0 || heads < 0 || kv_heads < 0 || dim < 0) return fail(VDSL_ERR_INVALID_ARG, name + ": negative shape");
+  if (heads == 0 || kv_heads == 0 || heads % kv_heads) return fail(VDSL_ERR_INVALID_ARG, name + ": kv_heads must divide heads");
+  if (dim == 0 || dim % 8 || dim > 128) return fail(VDSL_ERR_UNSUPPORTED, name + ": dim must be a multiple of 8 up to 128");
+  if (heads > 65535 || n > 0x7f000000 / heads || seqs > 0x3fffffff) return fail(VDSL_ERR_UNSUPPORTED, name + ": too many rows");
+  return VDSL_OK;
+}
+int attention_check_scale(const char* op, float scale) {
+  if (!(scale > 0.0f) || !std::isnormal(scale) || !std::isfinite(scale * kLog2e))
+    return fail(VDSL_ERR_INVALID_ARG, std::string(op) + ": scale must be a positive normal number");
+  return VDSL_OK;
+}
+// The bytes of a buffer that holds n rows of `heads` heads laid out as h says, and whether h can be used.
+int attention_check_heads(const char* op, const char* name, const vdsl_heads& h, int64_t n, int32_t heads, int32_t dim, size_t elem,
+                          size_t* bytes) {
+  const std::string where = std::string(op) + ": " + name;
+  if (h.first < 0 || h.stride < 0) return fail(VDSL_ERR_INVALID_ARG, where + ": negative first or stride");
+  const int64_t width = static_cast<int64_t>(heads) * dim;
+  if (h.first % 8 || h.stride % 8) return fail(VDSL_ERR_UNSUPPORTED, where + ": first and stride must be multiples of 8");
+  if (h.stride < width) return fail(VDSL_ERR_SHAPE, where + ": stride is less than the heads' columns");
+  if (h.stride >= (1 << 24)) return fail(VDSL_ERR_UNSUPPORTED, where + ": stride of 2^24 or more");
+  if (h.first > (int64_t{1} << 60)) return fail(VDSL_ERR_SHAPE, where + ": first is past any buffer");
+  *bytes = n == 0 ? 0 : nbytes(h.first + (n - 1) * h.stride + width, static_cast<int64_t>(elem));
+  return VDSL_OK;
+}
+
+}  // namespace vdsl
+
+using namespace vdsl;
+
+extern "C" int vdsl_op_attention_fwd(vdsl_queue q, const vdsl_attention_params* p, vdsl_buffer qs, vdsl_buffer ks, vdsl_buffer vs,
+                                     vdsl_buffer starts, int32_t out_dtype, vdsl_buffer out, vdsl_buffer lse) {
+  VDSL_TRY(enter_queue(q));
+  if (!p) return fail(VDSL_ERR_INVALID_ARG, "params is null");
+  const char* const op = "attention_fwd";
+  VDSL_TRY(attention_check_shape(op, p->n, p->seqs, p->heads, p->kv_heads, p->dim));
+  VDSL_TRY(attention_check_scale(op, p->scale));
+  if (!float_type(out_dtype)) return fail(VDSL_ERR_UNSUPPORTED, "attention_fwd stores f32 and bf16");
+  size_t qb, kb, vb;
+  VDSL_TRY(attention_check_heads(op, "q", p->q, p->n, p->heads, p->dim, 2, &qb));
+  VDSL_TRY(attention_check_heads(op, "k", p->k, p->n, p->kv_heads, p->dim, 2, &kb));
+  VDSL_TRY(attention_check_heads(op, "v", p->v, p->n, p->kv_heads, p->dim, 2, &vb));
+  VDSL_TRY(check_buffer(q, qs, qb, "q", false));
+  VDSL_TRY(check_buffer(q, ks, kb, "k", false));
+  VDSL_TRY(check_buffer(q, vs, vb, "v", false));
+  VDSL_TRY(check_buffer(q, starts, nbytes(p->seqs + 1, 4), "starts", false));
+  VDSL_TRY(check_buffer(q, out, nbytes(p->n, static_cast<int64_t>(p->heads) * p->dim, dtype_size(out_dtype)), "out", true));
+  if (lse) VDSL_TRY(check_buffer(q, lse, nbytes(p->n, p->heads, 4), "lse", true));
+  VDSL_TRY(check_apart(op, {out, lse}, {qs, ks, vs, starts}));
+  if (p->n == 0) return VDSL_OK;
+  AttentionArgs a = {};
+  a.q = static_cast<const uint16_t*>(qs->ptr) + p->q.first;
+  a.k = static_cast<const uint16_t*>(ks->ptr) + p->k.first;
+  a.v = static_cast<const uint16_t*>(vs->ptr) + p->v.first;
+  a.q_stride = p->q.stride;
+  a.k_stride = p->k.stride;
+  a.v_stride = p->v.stride;
+  a.seqs = {static_cast<const int32_t*>(starts->ptr), p->n, p->seqs};
+  a.out = out->ptr;
+  a.out_dtype = out_dtype;
+  a.lse = lse ? static_cast<float*>(lse->ptr) : nullptr;
+  a.heads = p->heads;
+  a.kv_heads = p->kv_heads;
+  a.group = p->heads / p->kv_heads;
+  a.dim = p->dim;
+  a.causal = p->causal != 0;
+  a.scale = p->scale;
+  a.splits = 1;
+  const int64_t rows = p->n * a.group * a.kv_heads;
+  return launch_rows<false>(q, a, rows >= 256 * 256 ? 2 : 1);
+}
+
+namespace vdsl {
+namespace {
+struct PagedPlan {
+  int qt, splits;
+};
+PagedPlan paged_plan(int64_t n, int64_t seqs, int32_t heads, int32_t kv_heads, int64_t positions) {
+  const int64_t group = heads / kv_heads;
+  const int64_t blocks = std::max<int64_t>(1, (n * group / 128 + std::min(seqs, n)) * kv_heads);
+  PagedPlan plan = {1, 1};
+  while (blocks * plan.splits < 512 && plan.splits < 32 && positions > 256 * plan.splits) plan.splits *= 2;
+  return plan;
+}
+int paged_check(const char* op, const vdsl_paged_params* p) {
+  if (!p) return fail(VDSL_ERR_INVALID_ARG, "params is null");
+  VDSL_TRY(attention_check_shape(op, p->n, p->seqs, p->heads, p->kv_heads, p->dim));
+  if (p->pages < 0 || p->table_cols < 0 || p->page <= 0) return fail(VDSL_ERR_INVALID_ARG, std::string(op) + ": negative shape or no page size");
+  if ((p->page & (p->page - 1)) || p->page > 65536) return fail(VDSL_ERR_UNSUPPORTED, std::string(op) + ": page must be a power of two up to 65536");
+  if (p->pages > 0x7fffffff || p->table_cols > 0x7fffffff / p->page)
+    return fail(VDSL_ERR_UNSUPPORTED, std::string(op) + ": 2^31 positions a sequence or more");
+  return VDSL_OK;
+}
+AttentionArgs paged_args(const vdsl_paged_params* p, vdsl_buffer starts, vdsl_buffer lengths, vdsl_buffer table) {
+  AttentionArgs a = {};
+  a.seqs = {static_cast<const int32_t*>(starts->ptr), p->n, p->seqs};
+  a.lengths = static_cast<const int32_t*>(lengths->ptr);
+  a.table = static_cast<const int32_t*>(table->ptr);
+  a.heads = p->heads;
+  a.kv_heads = p->kv_heads;
+  a.group = p->heads / p->kv_heads;
+  a.dim = p->dim;
+  a.causal = 1;
+  a.scale = p->scale;
+  a.pages = p->pages;
+  a.table_cols = static_cast<int>(p->table_cols);
+  a.page_shift = __builtin_ctz(static_cast<unsigned>(p->page));
+  a.splits = 1;
+  return a;
+}
+size_t cache_bytes(const vdsl_paged_params* p) {
+  return nbytes(p->pages, static_cast<int64_t>(p->kv_heads) * p->page, static_cast<int64_t>(p->dim) * 2);
+}
+}  // namespace
+}  // namespace vdsl
+
+extern "C" int vdsl_op_cache_append(vdsl_queue q, const vdsl_paged_params* p, vdsl_buffer ks, vdsl_buffer vs, vdsl_buffer starts,
+                                    vdsl_buffer lengths, vdsl_buffer table, vdsl_buffer k_cache, vdsl_buffer v_cache) {
+  VDSL_TRY(enter_queue(q));
+  const char* const op = "cache_append";
+  VDSL_TRY(paged_check(op, p));
+  size_t kb, vb;
+  VDSL_TRY(attention_check_heads(op, "k", p->k, p->n, p->kv_heads, p->dim, 2, &kb));
+  VDSL_TRY(attention_check_heads(op, "v", p->v, p->n, p->kv_heads, p->dim, 2, &vb));
+  VDSL_TRY(check_buffer(q, ks, kb, "k", false));
+  VDSL_TRY(check_buffer(q, vs, vb, "v", false));
+  VDSL_TRY(check_buffer(q, starts, nbytes(p->seqs + 1, 4), "starts", false));
+  VDSL_TRY(check_buffer(q, lengths, nbytes(p->seqs, 4), "lengths", false));
+  VDSL_TRY(check_buffer(q, table, nbytes(p->seqs, p->table_cols, 4), "table", false));
+  VDSL_TRY(check_buffer(q, k_cache, cache_bytes(p), "k_cache", true));
+  VDSL_TRY(check_buffer(q, v_cache, cache_bytes(p), "v_cache", true));
+  VDSL_TRY(check_apart(op, {k_cache, v_cache}, {ks, vs, starts, lengths, table}));
+  if (p->n == 0 || p->seqs == 0) return VDSL_OK;
+  AttentionArgs a = paged_args(p, starts, lengths, table);
+  a.k = static_cast<const uint16_t*>(ks->ptr) + p->k.first;
+  a.v = static_cast<const uint16_t*>(vs->ptr) + p->v.first;
+  a.k_stride = p->k.stride;
+  a.v_stride = p->v.stride;
+  hipLaunchKernelGGL(cache_append_rows, block_grid(p->n), dim3(256), 0, q->stream, a, static_cast<uint16_t*>(k_cache->ptr),
+                     static_cast<uint16_t*>(v_cache->ptr));
+  return check_launch("cache_append_rows");
+}
+
+extern "C" int vdsl_paged_attention_workspace_bytes(int64_t n, int64_t seqs, int32_t heads, int32_t kv_heads, int32_t dim,
+                                                    int64_t positions, size_t* bytes) {
+  if (!bytes) return fail(VDSL_ERR_INVALID_ARG, "bytes is null");
+  VDSL_TRY(attention_check_shape("paged_attention", n, seqs, heads, kv_heads, dim));
+  if (positions < 0) return fail(VDSL_ERR_INVALID_ARG, "negative shape");
+  const int splits = paged_plan(n, seqs, heads, kv_heads, positions).splits;
+  *bytes = splits == 1 ? 0 : nbytes(n * heads, splits, 8 + 4 * static_cast<int64_t>(dim));
+  return VDSL_OK;
+}
+
+extern "C" int vdsl_op_paged_attention(vdsl_queue q, const vdsl_paged_params* p, vdsl_buffer qs, vdsl_buffer k_cache,
+                                       vdsl_buffer v_cache, vdsl_buffer starts, vdsl_buffer lengths, vdsl_buffer table,
+                                       int32_t out_dtype, vdsl_buffer out, vdsl_buffer lse, vdsl_buffer workspace) {
+  VDSL_TRY(enter_queue(q));
+  const char* const op = "paged_attention";
+  VDSL_TRY(paged_check(op, p));
+  VDSL_TRY(attention_check_scale(op, p->scale));
+  if (!float_type(out_dtype)) return fail(VDSL_ERR_UNSUPPORTED, "paged_attention stores f32 and bf16");
+  size_t qb, need;
+  VDSL_TRY(attention_check_heads(op, "q", p->q, p->n, p->heads, p->dim, 2, &qb));
+  VDSL_TRY(check_buffer(q, qs, qb, "q", false));
+  VDSL_TRY(check_buffer(q, k_cache, cache_bytes(p), "k_cache", false));
+  VDSL_TRY(check_buffer(q, v_cache, cache_bytes(p), "v_cache", false));
+  VDSL_TRY(check_buffer(q, starts, nbytes(p->seqs + 1, 4), "starts", false));
+  VDSL_TRY(check_buffer(q, lengths, nbytes(p->seqs, 4), "lengths", false));
+  VDSL_TRY(check_buffer(q, table, nbytes(p->seqs, p->table_cols, 4), "table", false));
+  VDSL_TRY(check_buffer(q, out, nbytes(p->n, static_cast<int64_t>(p->heads) * p->dim, dtype_size(out_dtype)), "out", true));
+  if (lse) VDSL_TRY(check_buffer(q, lse, nbytes(p->n, p->heads, 4), "lse", true));
+  const int64_t positions = p->table_cols * p->page;
+  VDSL_TRY(vdsl_paged_attention_workspace_bytes(p->n, p->seqs, p->heads, p->kv_heads, p->dim, positions, &need));
+  if (need) VDSL_TRY(check_buffer(q, workspace, need, "workspace", true));
+  VDSL_TRY(check_apart(op, {out, lse, need ? workspace : nullptr}, {qs, k_cache, v_cache, starts, lengths, table}));
+  if (p->n == 0) return VDSL_OK;
+  AttentionArgs a = paged_args(p, starts, lengths, table);
+  a.q = static_cast<const uint16_t*>(qs->ptr) + p->q.first;
+  a.k = static_cast<const uint16_t*>(k_cache->ptr);
+  a.v = static_cast<const uint16_t*>(v_cache->ptr);
+  a.q_stride = p->q.stride;
+  a.out = out->ptr;
+  a.out_dtype = out_dtype;
+  a.lse = lse ? static_cast<float*>(lse->ptr) : nullptr;
+  const PagedPlan plan = paged_plan(p->n, p->seqs, p->heads, p->kv_heads, positions);
+  a.splits = plan.splits;
+  if (plan.splits > 1) {
+    a.parts = static_cast<float*>(workspace->ptr);
+    a.stats = reinterpret_cast<float2*>(a.parts + static_cast<int64_t>(plan.splits) * p->n * p->heads * p->dim);
+  }
+  VDSL_TRY(launch_rows<true>(q, a, plan.qt));
+  if (plan.splits == 1) return VDSL_OK;
+  hipLaunchKernelGGL(attention_join, block_grid((p->n * p->heads + 7) / 8), dim3(256), 0, q->stream, a);
+  return check_launch("attention_join");
+}

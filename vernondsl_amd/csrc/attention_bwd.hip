@@ -1,0 +1,481 @@
+// The gradient of attention over packed sequences.  With p = exp2(c s - lse log2 e) formed again from q, k and lse,
+// dp = dout v, delta = dout out and ds = p (dp - delta):
+//   dq = scale ds k (rows' own sum over keys),   dk = scale ds^T q and dv = p^T dout (keys' own sums over rows and heads)
+// Three launches: delta of each row; dk and dv, a wave holding 32 keys and walking over the rows that see them; dq, a
+// wave holding its rows and walking over the keys they see.  Each sum belongs to one wave and is taken in one order, so
+// nothing is added atomically and the bits are the same on every call; the price is that s and dp are formed twice (7
+// products where 5 would do).  See attention.h for rows, tiles and the order of the products' sums.
+#include <algorithm>
+
+#include "attention.h"
+
+namespace vdsl {
+
+int attention_check_shape(const char* op, int64_t n, int64_t seqs, int32_t heads, int32_t kv_heads, int32_t dim);
+int attention_check_scale(const char* op, float scale);
+int attention_check_heads(const char* op, const char* name, const vdsl_heads& h, int64_t n, int32_t heads, int32_t dim, size_t elem,
+                          size_t* bytes);
+
+namespace {
+
+struct GradArgs {
+  const uint16_t *q, *k, *v, *dout;  // dout: bf16
+  int64_t q_stride, k_stride, v_stride, dout_stride;
+  Sequences seqs;
+  const float2* rows;  // lse log2 e and delta, [kv_heads][n * group]
+  void *dq, *dk, *dv;
+  int64_t dq_first, dq_stride, dk_first, dk_stride, dv_first, dv_stride;
+  int heads, kv_heads, group, dim, causal, grad_dtype;
+  float scale;
+  Divider token_of;
+  int blocks;
+};
+
+// Rows' lse and delta, and dout in bf16 where it is f32.  32 lanes a row.
+__global__ __launch_bounds__(256) void attention_bwd_rows(const void* __restrict__ dout, int dout_dtype, const void* __restrict__ out,
+                                                          int out_dtype, const float* __restrict__ lse, int64_t n, int heads, int group,
+                                                          int dim, uint16_t* __restrict__ copy, float2* __restrict__ rows) {
+  const int64_t r = block_index() * 8 + (threadIdx.x >> 5);
+  if (r >= n * heads) return;
+  const int64_t token = r / heads;
+  const int head = static_cast<int>(r % heads), col = 4 * (threadIdx.x & 31);
+  float sum = 0.0f;
+  if (col < dim) {
+    float d[4], o[4];
+    load_some(dout_dtype, dout, r * dim + col, 4, d);
+    load_some(out_dtype, out, r * dim + col, 4, o);
+    if (copy) {
+      store_whole<VDSL_BF16, 4>(copy, r * dim + col, d);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) d[j] = bf16_to_f32(f32_to_bf16(d[j]));
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sum += d[j] * o[j];
+  }
+#pragma unroll
+  for (int m = 16; m >= 1; m >>= 1) sum += __shfl_xor(sum, m, 64);
+  if (col != 0) return;
+  const float l = lse[head * n + token];
+  const float2 v = make_float2(l == neg_inf() ? __builtin_inff() : l * kLog2e, sum);  // no score of such a row has a weight
+  rows[static_cast<int64_t>(head / group) * n * group + token * group + head % group] = v;
+}
+
+// 32 rows of this lane's wave as an operand (element j of lane l: column 16 kk + 8 (l / 32) + j of row l % 32), from
+// the lane's own row at p.
+template <int DP>
+__device__ __forceinline__ void load_operand(const uint16_t* p, int dim, bf16x8 (&f)[DP / 16]) {
+#pragma unroll
+  for (int kk = 0; kk < DP / 16; ++kk) {
+    const int col = 16 * kk + 8 * ((threadIdx.x & 63) >> 5);
+    u32x4 w = {0u, 0u, 0u, 0u};
+    if (col < dim) w = *reinterpret_cast<const u32x4*>(p + col);
+    f[kk] = __builtin_bit_cast(bf16x8, w);
+  }
+}
+// acc (columns x rows: this lane has columns 32 d + 8 g + 4 (l / 32) + j of its own row) times `by` to element e of `to`.
+template <int DP>
+__device__ __forceinline__ void store_gradient(const f32x16 (&acc)[DP / 32], float by, int dtype, void* to, int64_t e, int dim) {
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int col = 32 * d + 8 * g + 4 * ((threadIdx.x & 63) >> 5);
+      if (col >= dim) continue;
+      float v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = acc[d][4 * g + j] * by;
+      store_unit<4>(dtype, to, e + col, v);
+    }
+}
+__device__ __forceinline__ void store_zeros(int dtype, void* to, int64_t e, int cols) {
+  const float none[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int c = 0; c < cols; c += 4) store_unit<4>(dtype, to, e + c, none);
+}
+
+// Tiles of TR rows of two operands for copies of four waves.
+template <int DP, int TR>
+struct PairCopies {
+  using T = TileShape<DP>;
+  static constexpr int C = TR * T::PITCH / 1024 / 4, SLOT = 2 * TR * T::PITCH;
+  int row_of[C], chunk[C];
+  __device__ __forceinline__ PairCopies(int wave) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int u = 0; u < C; ++u) {
+      row_of[u] = (wave * C + u) * (64 / T::CPR) + lane / T::CPR;
+      chunk[u] = lane % T::CPR ^ T::swz(row_of[u]);
+    }
+  }
+  // at(row of the tile, which operand): that row's first byte
+  template <class At>
+  __device__ __forceinline__ void operator()(char* to, int wave, int dim, At&& at) const {
+#pragma unroll
+    for (int u = 0; u < C; ++u) {
+      if (chunk[u] >= dim / 8) continue;
+      lds_copy16(at(row_of[u], 0) + 16 * chunk[u], to + (wave * C + u) * 1024);
+      lds_copy16(at(row_of[u], 1) + 16 * chunk[u], to + TR * T::PITCH + (wave * C + u) * 1024);
+    }
+  }
+};
+
+// dk and dv: four waves of 32 keys each, walking over tiles of 64 rows.
+template <int DP>
+__global__ __launch_bounds__(256, 1) void attention_bwd_keys(GradArgs a) {
+  constexpr int TR = 64, NS = 4;
+  using T = TileShape<DP>;
+  using Copies = PairCopies<DP, TR>;
+  __shared__ __attribute__((aligned(1024))) char smem[NS * Copies::SLOT];
+  __shared__ float2 stat[NS][TR];
+  int b = static_cast<int>(blockIdx.x);
+  const int kv = b % a.kv_heads;
+  const RowTile tile = row_tile<7>(a.seqs, 1, b / a.kv_heads);
+  if (!tile.any) return;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+  const int key = tile.row + 32 * wave + (lane & 31);
+  const int64_t head_col = static_cast<int64_t>(kv) * a.dim;
+  if (tile.seq < 0) {
+    if (key < tile.len && half == 0) {
+      store_zeros(a.grad_dtype, a.dk, a.dk_first + (tile.token + key) * a.dk_stride + head_col, a.dim);
+      store_zeros(a.grad_dtype, a.dv, a.dv_first + (tile.token + key) * a.dv_stride + head_col, a.dim);
+    }
+    return;
+  }
+  const Copies copies(wave);
+  if (2 * a.dim < T::PITCH) {
+    for (int i = threadIdx.x; i < NS * Copies::SLOT / 16; i += 256) reinterpret_cast<u32x4*>(smem)[i] = u32x4{0u, 0u, 0u, 0u};
+    __syncthreads();
+  }
+  const int64_t token = tile.token + min(key, tile.len - 1);
+  bf16x8 kf[DP / 16], vf[DP / 16];
+  load_operand<DP>(a.k + token * a.k_stride + head_col, a.dim, kf);
+  load_operand<DP>(a.v + token * a.v_stride + head_col, a.dim, vf);
+  const int rows = tile.len * a.group;
+  const int first = a.causal ? tile.row * a.group / TR : 0, end = (rows + TR - 1) / TR;
+  const char* const qp = reinterpret_cast<const char*>(a.q + tile.token * a.q_stride + head_col * a.group);
+  const char* const dp = reinterpret_cast<const char*>(a.dout + tile.token * a.dout_stride + head_col * a.group);
+  const float2* const sp = a.rows + (static_cast<int64_t>(kv) * a.seqs.n + tile.token) * a.group;
+  float2 next;
+  const auto fetch = [&](int t, int slot) {
+    copies(smem + slot * Copies::SLOT, wave, a.dim, [&](int r, int which) {
+      const int row = min(t * TR + r, rows - 1), i = a.token_of(row);
+      const int64_t col = static_cast<int64_t>(row - i * a.group) * a.dim;
+      return which == 0 ? qp + 2 * (i * a.q_stride + col) : dp + 2 * (i * a.dout_stride + col);
+    });
+  };
+#pragma unroll
+  for (int t = 0; t < NS - 1; ++t) {
+    fetch(min(first + t, end - 1), t);
+    if (threadIdx.x < TR) stat[t][threadIdx.x] = sp[min(min(first + t, end - 1) * TR + static_cast<int>(threadIdx.x), rows - 1)];
+  }
+  f32x16 dk[DP / 32], dv[DP / 32];
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d) dk[d] = dv[d] = MfmaBf16::zero();
+  const float scale2 = a.scale * kLog2e;
+  const int sees_from = a.causal ? key * a.group : 0;  // the key's first row
+  const int wave_first = a.causal ? (tile.row + 32 * wave) * a.group : 0, wave_all = a.causal ? (tile.row + 32 * wave + 31) * a.group : 0;
+  for (int t0 = first; t0 < end; t0 += NS) {
+#pragma unroll
+    for (int slot = 0; slot < NS; ++slot) {
+      const int t = t0 + slot;
+      if (t >= end) break;
+      const int ahead = min(t + NS - 1, end - 1), to = (slot + NS - 1) % NS;
+      dma_wait<0>();
+      __syncthreads();
+      if (threadIdx.x < TR) next = sp[min(ahead * TR + static_cast<int>(threadIdx.x), rows - 1)];
+      fetch(ahead, to);
+      const char* const qs = smem + slot * Copies::SLOT;
+      const char* const ds = qs + TR * T::PITCH;
+      if ((t + 1) * TR > wave_first) {
+#pragma unroll
+        for (int u = 0; u < TR / 32; ++u) {
+          const int r0 = t * TR + 32 * u;
+          f32x16 s = MfmaBf16::zero(), p = MfmaBf16::zero();
+#pragma unroll
+          for (int kk = 0; kk < DP / 16; ++kk) {
+            s = MfmaBf16::mma(rows_fragment<DP>(qs, 32 * u, kk), kf[kk], s);
+            p = MfmaBf16::mma(rows_fragment<DP>(ds, 32 * u, kk), vf[kk], p);
+          }
+          const bool masked = r0 < wave_all || r0 + 32 > rows;
+          const int lo = sees_from - r0, hi = rows - r0;
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int r = 8 * g + 4 * half + j;
+              const float2 st = stat[slot][32 * u + r];
+              float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * g + j], scale2, -st.x));
+              float d = w * (p[4 * g + j] - st.y);
+              if (masked && !(r >= lo && r < hi)) w = d = 0.0f;
+              s[4 * g + j] = w;
+              p[4 * g + j] = d;
+            }
+          }
+          if (masked && (any_not_finite<DP>(qs, 32 * u, 2) || any_not_finite<DP>(ds, 32 * u, 2))) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              add_seen<DP>(dv, ds, 32 * u + 16 * e, weights_fragment(s, e), lo - 16 * e, hi - 16 * e, 0xFFFFu);
+              add_seen<DP>(dk, qs, 32 * u + 16 * e, weights_fragment(p, e), lo - 16 * e, hi - 16 * e, 0xFFFFu);
+            }
+            continue;
+          }
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const bf16x8 w = weights_fragment(s, e), d = weights_fragment(p, e);
+#pragma unroll
+            for (int x = 0; x < DP / 32; ++x) {
+              dv[x] = MfmaBf16::mma(cols_fragment<DP>(ds, 32 * u + 16 * e, 32 * x), w, dv[x]);
+              dk[x] = MfmaBf16::mma(cols_fragment<DP>(qs, 32 * u + 16 * e, 32 * x), d, dk[x]);
+            }
+          }
+        }
+      }
+      if (threadIdx.x < TR) stat[to][threadIdx.x] = next;
+    }
+  }
+  dma_wait<0>();
+  if (key < tile.len) {
+    store_gradient<DP>(dk, a.scale, a.grad_dtype, a.dk, a.dk_first + token * a.dk_stride + head_col, a.dim);
+    store_gradient<DP>(dv, 1.0f, a.grad_dtype, a.dv, a.dv_first + token * a.dv_stride + head_col, a.dim);
+  }
+}
+
+// dq: four waves of QT x 32 rows each, walking over tiles of 64 keys.
+template <int DP, int QT>
+__global__ __launch_bounds__(256, 1) void attention_bwd_queries(GradArgs a) {
+  constexpr int KT = 64, NS = 4, ROWS = 128 * QT;
+  using T = TileShape<DP>;
+  using Copies = PairCopies<DP, KT>;
+  __shared__ __attribute__((aligned(1024))) char smem[NS * Copies::SLOT];
+  int b = static_cast<int>(blockIdx.x);
+  const int kv = b % a.kv_heads;
+  const RowTile tile = row_tile<QT == 1 ? 7 : 8>(a.seqs, a.group, a.blocks - 1 - b / a.kv_heads);
+  if (!tile.any) return;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int rows = tile.len * a.group, row0 = tile.row + 32 * QT * wave;
+  const int64_t head_col = static_cast<int64_t>(kv) * a.dim;
+  const auto dq_at = [&](int row) {
+    const int i = a.token_of(row);
+    return a.dq_first + (tile.token + i) * a.dq_stride + head_col * a.group + static_cast<int64_t>(row - i * a.group) * a.dim;
+  };
+  if (tile.seq < 0) {
+    for (int row = tile.row + static_cast<int>(threadIdx.x); row < min(tile.row + ROWS, rows); row += 256)
+      store_zeros(a.grad_dtype, a.dq, dq_at(row), a.dim);
+    return;
+  }
+  const Copies copies(wave);
+  if (2 * a.dim < T::PITCH) {
+    for (int i = threadIdx.x; i < NS * Copies::SLOT / 16; i += 256) reinterpret_cast<u32x4*>(smem)[i] = u32x4{0u, 0u, 0u, 0u};
+    __syncthreads();
+  }
+  const auto sees = [&](int row) { return a.causal ? a.token_of(row) + 1 : tile.len; };
+  const int end = (sees(min(tile.row + ROWS, rows) - 1) + KT - 1) / KT;
+  const char* const kp = reinterpret_cast<const char*>(a.k + tile.token * a.k_stride + head_col);
+  const char* const vp = reinterpret_cast<const char*>(a.v + tile.token * a.v_stride + head_col);
+  const auto fetch = [&](int t, int slot) {
+    copies(smem + slot * Copies::SLOT, wave, a.dim, [&](int r, int which) {
+      const int64_t i = min(t * KT + r, tile.len - 1);
+      return which == 0 ? kp + 2 * i * a.k_stride : vp + 2 * i * a.v_stride;
+    });
+  };
+#pragma unroll
+  for (int t = 0; t < NS - 1; ++t) fetch(min(t, end - 1), t);
+  bf16x8 qf[QT][DP / 16], df[QT][DP / 16];
+  float2 st[QT];
+  int seen[QT];
+  f32x16 dq[QT][DP / 32];
+#pragma unroll
+  for (int c = 0; c < QT; ++c) {
+    const int row = min(row0 + 32 * c + (lane & 31), rows - 1), i = a.token_of(row);
+    const int64_t col = head_col * a.group + static_cast<int64_t>(row - i * a.group) * a.dim;
+    load_operand<DP>(a.q + (tile.token + i) * a.q_stride + col, a.dim, qf[c]);
+    load_operand<DP>(a.dout + (tile.token + i) * a.dout_stride + col, a.dim, df[c]);
+    st[c] = a.rows[(static_cast<int64_t>(kv) * a.seqs.n + tile.token) * a.group + row];
+    seen[c] = sees(row);
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) dq[c][d] = MfmaBf16::zero();
+  }
+  const float scale2 = a.scale * kLog2e;
+  const bool mine = row0 < rows;
+  const int fewest = sees(min(row0, rows - 1)), most = mine ? sees(min(row0 + 32 * QT, rows) - 1) : 0;
+  for (int t0 = 0; t0 < end; t0 += NS) {
+#pragma unroll
+    for (int slot = 0; slot < NS; ++slot) {
+      const int t = t0 + slot;
+      if (t >= end) break;
+      dma_wait<(NS - 2) * 2 * Copies::C>();
+      dma_barrier();
+      fetch(min(t + NS - 1, end - 1), (slot + NS - 1) % NS);
+      const char* const ks = smem + slot * Copies::SLOT;
+      const char* const vs = ks + KT * T::PITCH;
+#pragma unroll
+      for (int u = 0; u < KT / 32; ++u) {
+        const int j0 = t * KT + 32 * u;
+        if (j0 >= most) continue;
+        f32x16 s[QT], p[QT];
+#pragma unroll
+        for (int c = 0; c < QT; ++c) s[c] = p[c] = MfmaBf16::zero();
+#pragma unroll
+        for (int kk = 0; kk < DP / 16; ++kk) {
+          const bf16x8 kf = rows_fragment<DP>(ks, 32 * u, kk), vf = rows_fragment<DP>(vs, 32 * u, kk);
+#pragma unroll
+          for (int c = 0; c < QT; ++c) {
+            s[c] = MfmaBf16::mma(kf, qf[c][kk], s[c]);
+            p[c] = MfmaBf16::mma(vf, df[c][kk], p[c]);
+          }
+        }
+        const bool masked = j0 + 32 > fewest;
+#pragma unroll
+        for (int c = 0; c < QT; ++c) {
+          const int hi = seen[c] - j0 - 4 * (lane >> 5);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[c][r], scale2, -st[c].x));
+            p[c][r] = w * (p[c][r] - st[c].y);
+            if (masked && !(8 * (r / 4) + r % 4 < hi)) p[c][r] = 0.0f;
+          }
+        }
+        if (masked && any_not_finite<DP>(ks, 32 * u, 2)) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int c = 0; c < QT; ++c)
+              add_seen<DP>(dq[c], ks, 32 * u + 16 * e, weights_fragment(p[c], e), 0, seen[c] - j0 - 16 * e, 0xFFFFu);
+          continue;
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          bf16x8 w[QT];
+#pragma unroll
+          for (int c = 0; c < QT; ++c) w[c] = weights_fragment(p[c], e);
+#pragma unroll
+          for (int d = 0; d < DP / 32; ++d) {
+            const bf16x8 f = cols_fragment<DP>(ks, 32 * u + 16 * e, 32 * d);
+#pragma unroll
+            for (int c = 0; c < QT; ++c) dq[c][d] = MfmaBf16::mma(f, w[c], dq[c][d]);
+          }
+        }
+      }
+    }
+  }
+  dma_wait<0>();
+#pragma unroll
+  for (int c = 0; c < QT; ++c) {
+    const int row = row0 + 32 * c + (lane & 31);
+    if (row < rows) store_gradient<DP>(dq[c], a.scale, a.grad_dtype, a.dq, dq_at(row), a.dim);
+  }
+}
+
+bool float_type(int32_t t) { return t == VDSL_F32 || t == VDSL_BF16; }
+
+// Whether two of the gradients, as columns of one buffer, have no element in common.
+bool apart(const vdsl_heads& x, int64_t x_width, const vdsl_heads& y, int64_t y_width) {
+  if (x.stride != y.stride) return false;
+  if (x.first + x_width > x.stride || y.first + y_width > y.stride) return false;
+  return x.first + x_width <= y.first || y.first + y_width <= x.first;
+}
+
+}  // namespace
+}  // namespace vdsl
+
+using namespace vdsl;
+
+// The rows' lse and delta, then a copy of dout in bf16.
+extern "C" int vdsl_attention_bwd_workspace_bytes(int64_t n, int64_t seqs, int32_t heads, int32_t kv_heads, int32_t dim, size_t* bytes) {
+  if (!bytes) return fail(VDSL_ERR_INVALID_ARG, "bytes is null");
+  VDSL_TRY(attention_check_shape("attention_bwd", n, seqs, heads, kv_heads, dim));
+  *bytes = nbytes(n, heads, 8 + 2 * static_cast<int64_t>(dim));
+  return VDSL_OK;
+}
+
+extern "C" int vdsl_op_attention_bwd(vdsl_queue q, const vdsl_attention_params* p, int32_t dout_dtype, vdsl_buffer dout, vdsl_buffer qs,
+                                     vdsl_buffer ks, vdsl_buffer vs, vdsl_buffer starts, int32_t out_dtype, vdsl_buffer out,
+                                     vdsl_buffer lse, int32_t grad_dtype, vdsl_buffer dq, vdsl_buffer dk, vdsl_buffer dv,
+                                     vdsl_buffer workspace) {
+  VDSL_TRY(enter_queue(q));
+  if (!p) return fail(VDSL_ERR_INVALID_ARG, "params is null");
+  const char* const op = "attention_bwd";
+  VDSL_TRY(attention_check_shape(op, p->n, p->seqs, p->heads, p->kv_heads, p->dim));
+  VDSL_TRY(attention_check_scale(op, p->scale));
+  if (!float_type(dout_dtype) || !float_type(out_dtype) || !float_type(grad_dtype))
+    return fail(VDSL_ERR_UNSUPPORTED, "attention_bwd supports f32 and bf16");
+  const size_t elem = dtype_size(grad_dtype);
+  size_t qb, kb, vb, dqb, dkb, dvb, need;
+  VDSL_TRY(attention_check_heads(op, "q", p->q, p->n, p->heads, p->dim, 2, &qb));
+  VDSL_TRY(attention_check_heads(op, "k", p->k, p->n, p->kv_heads, p->dim, 2, &kb));
+  VDSL_TRY(attention_check_heads(op, "v", p->v, p->n, p->kv_heads, p->dim, 2, &vb));
+  VDSL_TRY(attention_check_heads(op, "dq", p->dq, p->n, p->heads, p->dim, elem, &dqb));
+  VDSL_TRY(attention_check_heads(op, "dk", p->dk, p->n, p->kv_heads, p->dim, elem, &dkb));
+  VDSL_TRY(attention_check_heads(op, "dv", p->dv, p->n, p->kv_heads, p->dim, elem, &dvb));
+  const int64_t width = static_cast<int64_t>(p->heads) * p->dim, kv_width = static_cast<int64_t>(p->kv_heads) * p->dim;
+  VDSL_TRY(check_buffer(q, dout, nbytes(p->n, width, dtype_size(dout_dtype)), "dout", false));
+  VDSL_TRY(check_buffer(q, qs, qb, "q", false));
+  VDSL_TRY(check_buffer(q, ks, kb, "k", false));
+  VDSL_TRY(check_buffer(q, vs, vb, "v", false));
+  VDSL_TRY(check_buffer(q, starts, nbytes(p->seqs + 1, 4), "starts", false));
+  VDSL_TRY(check_buffer(q, out, nbytes(p->n, width, dtype_size(out_dtype)), "out", false));
+  VDSL_TRY(check_buffer(q, lse, nbytes(p->n, p->heads, 4), "lse", false));
+  VDSL_TRY(check_buffer(q, dq, dqb, "dq", true));
+  VDSL_TRY(check_buffer(q, dk, dkb, "dk", true));
+  VDSL_TRY(check_buffer(q, dv, dvb, "dv", true));
+  VDSL_TRY(vdsl_attention_bwd_workspace_bytes(p->n, p->seqs, p->heads, p->kv_heads, p->dim, &need));
+  VDSL_TRY(check_buffer(q, workspace, need, "workspace", true));
+  for (const vdsl_buffer w : {dq, dk, dv}) VDSL_TRY(check_apart(op, {w, workspace}, {dout, qs, ks, vs, starts, out, lse}));
+  if ((dq == dk && !apart(p->dq, width, p->dk, kv_width)) || (dq == dv && !apart(p->dq, width, p->dv, kv_width)) ||
+      (dk == dv && !apart(p->dk, kv_width, p->dv, kv_width)))
+    return fail(VDSL_ERR_INVALID_ARG, "attention_bwd: gradients in one buffer must be disjoint columns of one stride");
+  if (p->n == 0) return VDSL_OK;
+  const int group = p->heads / p->kv_heads;
+  float2* const rows = static_cast<float2*>(workspace->ptr);
+  uint16_t* const copy = dout_dtype == VDSL_F32 ? reinterpret_cast<uint16_t*>(rows + p->n * p->heads) : nullptr;
+  GradArgs a = {};
+  a.q = static_cast<const uint16_t*>(qs->ptr) + p->q.first;
+  a.k = static_cast<const uint16_t*>(ks->ptr) + p->k.first;
+  a.v = static_cast<const uint16_t*>(vs->ptr) + p->v.first;
+  a.dout = copy ? copy : static_cast<const uint16_t*>(dout->ptr);
+  a.q_stride = p->q.stride;
+  a.k_stride = p->k.stride;
+  a.v_stride = p->v.stride;
+  a.dout_stride = width;
+  a.seqs = {static_cast<const int32_t*>(starts->ptr), p->n, p->seqs};
+  a.rows = rows;
+  a.dq = dq->ptr;
+  a.dk = dk->ptr;
+  a.dv = dv->ptr;
+  a.dq_first = p->dq.first;
+  a.dq_stride = p->dq.stride;
+  a.dk_first = p->dk.first;
+  a.dk_stride = p->dk.stride;
+  a.dv_first = p->dv.first;
+  a.dv_stride = p->dv.stride;
+  a.heads = p->heads;
+  a.kv_heads = p->kv_heads;
+  a.group = group;
+  a.dim = p->dim;
+  a.causal = p->causal != 0;
+  a.grad_dtype = grad_dtype;
+  a.scale = p->scale;
+  a.token_of = divider(group);
+  hipLaunchKernelGGL(attention_bwd_rows, block_grid((p->n * p->heads + 7) / 8), dim3(256), 0, q->stream, dout->ptr, dout_dtype,
+                     out->ptr, out_dtype, static_cast<const float*>(lse->ptr), p->n, p->heads, group, p->dim, copy, rows);
+  VDSL_TRY(check_launch("attention_bwd_rows"));
+  const int64_t key_slots = row_slots(p->n, p->seqs, 1, 7);
+  const int qt = p->n * p->heads >= 256 * 256 ? 2 : 1;
+  const int64_t row_slots_ = row_slots(p->n, p->seqs, group, qt == 1 ? 7 : 8);
+  if (std::max(key_slots, row_slots_) * p->kv_heads > 0x7fffff) return fail(VDSL_ERR_UNSUPPORTED, "attention_bwd: too many rows");
+  const auto go = [&](auto kernel, int64_t slots, const char* name) {
+    a.blocks = static_cast<int>(slots);
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(slots * p->kv_heads)), dim3(256), 0, q->stream, a);
+    return check_launch(name);
+  };
+  const char *const keys = "attention_bwd_keys", *const queries = "attention_bwd_queries";
+  if (p->dim <= 64) {
+    VDSL_TRY(go(attention_bwd_keys<64>, key_slots, keys));
+    return go(qt == 1 ? attention_bwd_queries<64, 1> : attention_bwd_queries<64, 2>, row_slots_, queries);
+  }
+  if (p->dim <= 96) {
+    VDSL_TRY(go(attention_bwd_keys<96>, key_slots, keys));
+    return go(qt == 1 ? attention_bwd_queries<96, 1> : attention_bwd_queries<96, 2>, row_slots_, queries);
+  }
+  VDSL_TRY(go(attention_bwd_keys<128>, key_slots, keys));
+  return go(qt == 1 ? attention_bwd_queries<128, 1> : attention_bwd_queries<128, 2>, row_slots_, queries);
+}

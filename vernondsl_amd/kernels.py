@@ -6,6 +6,9 @@ ABI checks buffer sizes again), then enqueues the op on `q` and returns without 
 from __future__ import annotations
 
 import ctypes as C
+from typing import NamedTuple
+
+import numpy as np
 
 from . import _lib
 from ._lib import call
@@ -513,3 +516,193 @@ def linear_xent_fwd_bwd(q: Queue, x: Tensor, w: Tensor, labels: Tensor, loss: Te
         raise ValueError(f"dw: shape {dw.shape}, expected {(vocab, dim)}")
     call("vdsl_op_linear_xent_fwd_bwd", q.handle, n, dim, vocab, x.handle, w.handle, labels.handle, piece, grad_scale, loss.handle,
          _h(row_loss), _h(lse), dx.dtype, dx.handle, dw.dtype, dw.handle, _h(workspace))
+
+
+# ---- op class 7: what lets the rows of a sequence see each other ---------------------------------------
+class Heads(NamedTuple):
+    """Heads in the columns of a tensor [rows][width]: head h is columns [first + h * dim, first + (h + 1) * dim).  A tensor
+    [rows][heads][dim] stands for all of its columns wherever the calls below take Heads."""
+    tensor: Tensor
+    heads: int
+    dim: int
+    first: int = 0
+
+
+def _heads(x, name) -> Heads:
+    if isinstance(x, Heads):
+        if len(x.tensor.shape) != 2:
+            raise ValueError(f"{name}: Heads are columns of a tensor [rows][width], got shape {x.tensor.shape}")
+        if x.first < 0 or x.heads < 0 or x.dim < 0 or x.first + x.heads * x.dim > x.tensor.shape[1]:
+            raise ValueError(f"{name}: columns {x.first} to {x.first + x.heads * x.dim} of a tensor of width {x.tensor.shape[1]}")
+        return x
+    if len(x.shape) != 3:
+        raise ValueError(f"{name}: shape {x.shape}, expected [rows][heads][dim] or Heads of [rows][width]")
+    return Heads(x, x.shape[1], x.shape[2])
+
+
+def _layout(x: Heads) -> _lib.Heads:
+    return _lib.Heads(x.first, x.tensor.numel // x.tensor.shape[0] if x.tensor.shape[0] else x.heads * x.dim)
+
+
+def rope_frequencies(rot: int, base: float = 10000.0, factor: float = 1.0, trained: int = 0, kind: str = "ramp") -> np.ndarray:
+    """The frequencies of rope's rot / 2 pairs, f32 [2][rot / 2]: turns per position (base^(-2 i / rot) / 2 pi, formed in 64
+    bits) and what 32 bits leave of them.  factor > 1 stretches them for contexts that much longer than the trained ones:
+    kind "linear" divides every frequency by it; "base" raises the base to base * factor^(rot / (rot - 2)), which leaves the
+    fastest pair and divides the slowest one; "ramp" (YaRN, Peng et al. 2023) divides the pairs that turn less than once
+    over the `trained` positions, keeps those that turn more than 32 times, and goes from one to the other linearly between
+    (its magnitude is 0.1 log(factor) + 1)."""
+    if rot < 0 or rot % 2:
+        raise ValueError(f"rope_frequencies: rot {rot} is not an even number of columns")
+    if not (base > 1.0 and factor >= 1.0 and np.isfinite(base) and np.isfinite(factor)):
+        raise ValueError("rope_frequencies: base must be above 1 and factor at least 1")
+    i = np.arange(rot // 2, dtype=np.float64)
+    if kind == "base" and factor > 1.0:
+        if rot <= 2:
+            raise ValueError("rope_frequencies: kind 'base' needs two pairs or more")
+        base = base * factor ** (rot / (rot - 2.0))
+    f = base ** (-2.0 * i / max(rot, 1))
+    if kind == "linear":
+        f = f / factor
+    elif kind == "ramp":
+        if factor > 1.0:
+            if trained <= 0:
+                raise ValueError("rope_frequencies: kind 'ramp' needs the number of trained positions")
+            pair = [rot * np.log(trained / (2.0 * np.pi * turns)) / (2.0 * np.log(base)) for turns in (32.0, 1.0)]
+            lo, hi = max(0.0, np.floor(pair[0])), min(rot - 1.0, np.ceil(pair[1]))
+            ramp = np.clip((i - lo) / max(hi - lo, 0.001), 0.0, 1.0)
+            f = f * (1.0 - ramp) + f / factor * ramp
+    elif kind != "base":
+        raise ValueError(f"rope_frequencies: unknown kind {kind!r}")
+    turns = f / (2.0 * np.pi)
+    hi = turns.astype(np.float32)
+    return np.stack([hi, (turns - hi).astype(np.float32)])
+
+
+def rope(q: Queue, x: Tensor, positions: Tensor, freqs: Tensor, y: Tensor, heads: int, dim: int, first: int = 0,
+         interleaved: bool = False, inverse: bool = False, magnitude: float = 1.0):
+    """y = x [rows][width] with `heads` heads of `dim` columns, from column `first` on, turned by positions (i32 [rows]): the first
+    2 * pairs columns of each, freqs f32 [2][pairs] (rope_frequencies); the other columns are handed on.  Pairs are columns
+    (i, i + pairs), or (2 i, 2 i + 1) if interleaved.  inverse: the gradient, dx from dy.  y may be x (one dtype)."""
+    rows, width = x.shape
+    if y.shape != (rows, width):
+        raise ValueError(f"y: shape {y.shape}, expected {(rows, width)}")
+    _expect(positions, (rows,), "i32", "positions")
+    _expect(freqs, (2, freqs.shape[-1]), "f32", "freqs")
+    p = _lib.RopeParams(rows, width, first, heads, dim, freqs.shape[1], int(bool(interleaved)), int(bool(inverse)), magnitude)
+    call("vdsl_op_rope", q.handle, C.byref(p), x.dtype, x.handle, positions.handle, freqs.handle, y.dtype, y.handle)
+
+
+def _attention_operands(qh, k, v, starts, out, lse, scale):
+    qh, k, v = _heads(qh, "q"), _heads(k, "k"), _heads(v, "v")
+    n, dim = qh.tensor.shape[0], qh.dim
+    for x, name in ((qh, "q"), (k, "k"), (v, "v")):
+        if x.tensor.dtype != _lib.BF16:
+            raise ValueError(f"{name}: dtype {x.tensor.dtype}, expected bf16")
+        if x.tensor.shape[0] != n or x.dim != dim or (x is not qh and x.heads != k.heads):
+            raise ValueError(f"{name}: {x.tensor.shape[0]} rows of {x.heads} heads of {x.dim} beside q's {n} rows of {dim}")
+    _expect(starts, (starts.numel,), "i32", "starts")
+    if starts.numel < 1:
+        raise ValueError("starts: needs the number of sequences + 1 elements")
+    if out.numel != n * qh.heads * dim or out.shape[0] != n:
+        raise ValueError(f"out: shape {out.shape}, expected {(n, qh.heads * dim)}")
+    _expect(lse, (qh.heads, n), "f32", "lse")
+    return qh, k, v, float(dim) ** -0.5 if scale is None and dim else scale
+
+
+def attention_fwd(q: Queue, qh, k, v, starts: Tensor, out: Tensor, lse=None, causal: bool = True, scale=None):
+    """out [n][heads * dim] (f32 or bf16) = softmax(scale q k^T) v over packed sequences: rows starts[s] to starts[s + 1] (i32
+    [seqs + 1]) see each other, earlier ones only if causal.  q, k, v: bf16 Heads, or tensors [n][heads][dim]; kv heads divide
+    the heads.  scale: 1 / sqrt(dim) if None.  lse (f32 [heads][n], optional): log of the scores' exponentials' sum, kept for
+    attention_bwd.  Rows of no sequence get 0, lse -inf."""
+    qh, k, v, scale = _attention_operands(qh, k, v, starts, out, lse, scale)
+    p = _lib.AttentionParams(qh.tensor.shape[0], starts.numel - 1, qh.heads, k.heads, qh.dim, int(bool(causal)), scale, 0,
+                             _layout(qh), _layout(k), _layout(v))
+    call("vdsl_op_attention_fwd", q.handle, C.byref(p), qh.tensor.handle, k.tensor.handle, v.tensor.handle, starts.handle, out.dtype,
+         out.handle, _h(lse))
+
+
+def attention_bwd_workspace_bytes(n, seqs, heads, kv_heads, dim) -> int:
+    b = C.c_size_t()
+    call("vdsl_attention_bwd_workspace_bytes", n, seqs, heads, kv_heads, dim, C.byref(b))
+    return b.value
+
+
+def attention_bwd(q: Queue, dout: Tensor, qh, k, v, starts: Tensor, out: Tensor, lse: Tensor, dq, dk, dv, causal: bool = True,
+                  scale=None, workspace=None):
+    """The gradients dq, dk, dv (Heads or tensors [n][heads][dim], all f32 or all bf16; disjoint columns of one tensor if they
+    like) of attention_fwd from dout [n][heads * dim] (f32 or bf16) and the forward pass's out and lse.  workspace:
+    attention_bwd_workspace_bytes(n, seqs, heads, kv_heads, dim) bytes."""
+    qh, k, v, scale = _attention_operands(qh, k, v, starts, out, lse, scale)
+    n = qh.tensor.shape[0]
+    if dout.numel != out.numel or dout.shape[0] != n:
+        raise ValueError(f"dout: shape {dout.shape}, expected {out.shape}")
+    grads = [_heads(g, name) for g, name in ((dq, "dq"), (dk, "dk"), (dv, "dv"))]
+    for g, x, name in zip(grads, (qh, k, v), ("dq", "dk", "dv")):
+        if (g.tensor.shape[0], g.heads, g.dim) != (n, x.heads, x.dim):
+            raise ValueError(f"{name}: {g.tensor.shape[0]} rows of {g.heads} heads of {g.dim}, expected {n} rows of {x.heads} heads of {x.dim}")
+        if g.tensor.dtype != grads[0].tensor.dtype:
+            raise ValueError("dq, dk and dv must be of one dtype")
+    p = _lib.AttentionParams(n, starts.numel - 1, qh.heads, k.heads, qh.dim, int(bool(causal)), scale, 0, _layout(qh), _layout(k), _layout(v),
+                             *(_layout(g) for g in grads))
+    call("vdsl_op_attention_bwd", q.handle, C.byref(p), dout.dtype, dout.handle, qh.tensor.handle, k.tensor.handle, v.tensor.handle,
+         starts.handle, out.dtype, out.handle, _h(lse), grads[0].tensor.dtype, *(g.tensor.handle for g in grads), _h(workspace))
+
+
+def _paged_params(n, dim, kv_heads, heads, scale, starts, lengths, table, k_cache, v_cache):
+    """starts, lengths and table against the caches [pages][kv_heads][page][dim]; the params without layouts."""
+    if len(k_cache.shape) != 4 or k_cache.shape[1] != kv_heads or k_cache.shape[3] != dim:
+        raise ValueError(f"k_cache: shape {k_cache.shape}, expected [pages][{kv_heads}][page][{dim}]")
+    _expect(k_cache, k_cache.shape, "bf16", "k_cache")
+    _expect(v_cache, k_cache.shape, "bf16", "v_cache")
+    (seqs,) = lengths.shape
+    _expect(starts, (seqs + 1,), "i32", "starts")
+    _expect(lengths, (seqs,), "i32", "lengths")
+    if len(table.shape) != 2:
+        raise ValueError(f"table: shape {table.shape}, expected [seqs][pages of a sequence]")
+    _expect(table, (seqs, table.shape[1]), "i32", "table")
+    return _lib.PagedParams(n, seqs, k_cache.shape[0], table.shape[1], k_cache.shape[2], heads, kv_heads, dim, scale, 0)
+
+
+def cache_append(q: Queue, k, v, starts: Tensor, lengths: Tensor, table: Tensor, k_cache: Tensor, v_cache: Tensor):
+    """The new rows' k and v (bf16 Heads or tensors [n][kv_heads][dim]) into their slots of the paged caches (bf16
+    [pages][kv_heads][page][dim], page a power of two): row i of the m new rows starts[s] to starts[s + 1] of sequence s is
+    position p = lengths[s] - m + i, slot p % page of page table[s][p / page] (i32; lengths counts the new rows).  Rows without
+    a page are dropped."""
+    k, v = _heads(k, "k"), _heads(v, "v")
+    n = k.tensor.shape[0]
+    for x, name in ((k, "k"), (v, "v")):
+        if x.tensor.dtype != _lib.BF16:
+            raise ValueError(f"{name}: dtype {x.tensor.dtype}, expected bf16")
+    if (v.tensor.shape[0], v.heads, v.dim) != (n, k.heads, k.dim):
+        raise ValueError(f"v: {v.tensor.shape[0]} rows of {v.heads} heads of {v.dim}, expected {n} rows of {k.heads} heads of {k.dim}")
+    p = _paged_params(n, k.dim, k.heads, k.heads, 1.0, starts, lengths, table, k_cache, v_cache)
+    p.k, p.v = _layout(k), _layout(v)
+    call("vdsl_op_cache_append", q.handle, C.byref(p), k.tensor.handle, v.tensor.handle, starts.handle, lengths.handle, table.handle,
+         k_cache.handle, v_cache.handle)
+
+
+def paged_attention_workspace_bytes(n, seqs, heads, kv_heads, dim, positions) -> int:
+    """positions: those that a row of the page table has room for (its pages times the page size)."""
+    b = C.c_size_t()
+    call("vdsl_paged_attention_workspace_bytes", n, seqs, heads, kv_heads, dim, positions, C.byref(b))
+    return b.value
+
+
+def paged_attention(q: Queue, qh, k_cache: Tensor, v_cache: Tensor, starts: Tensor, lengths: Tensor, table: Tensor, out: Tensor, lse=None,
+                    scale=None, workspace=None):
+    """Attention of new rows over a paged cache that holds their own keys already (cache_append): the row at position p sees
+    positions 0 to p of its sequence.  qh: bf16 Heads or a tensor [n][heads][dim]; out [n][heads * dim], lse and scale as
+    for attention_fwd.  workspace: paged_attention_workspace_bytes(...) bytes, None where that is 0."""
+    qh = _heads(qh, "q")
+    n, dim = qh.tensor.shape[0], qh.dim
+    if qh.tensor.dtype != _lib.BF16:
+        raise ValueError(f"q: dtype {qh.tensor.dtype}, expected bf16")
+    if out.numel != n * qh.heads * dim or out.shape[0] != n:
+        raise ValueError(f"out: shape {out.shape}, expected {(n, qh.heads * dim)}")
+    _expect(lse, (qh.heads, n), "f32", "lse")
+    kv_heads = k_cache.shape[1] if len(k_cache.shape) == 4 else 0
+    p = _paged_params(n, dim, kv_heads, qh.heads, float(dim) ** -0.5 if scale is None and dim else scale, starts, lengths, table, k_cache,
+                      v_cache)
+    p.q = _layout(qh)
+    call("vdsl_op_paged_attention", q.handle, C.byref(p), qh.tensor.handle, k_cache.handle, v_cache.handle, starts.handle, lengths.handle,
+         table.handle, out.dtype, out.handle, _h(lse), _h(workspace))

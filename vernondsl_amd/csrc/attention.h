@@ -141,44 +141,54 @@ __device__ __forceinline__ uint32_t not_finite(const bf16x8& x) {
   return f & 0x80008000u;
 }
 
-// One of a step's 16 places alone, the others zero: of both operands it leaves the product's terms of that one.
-__device__ __forceinline__ bf16x8 only_place(const bf16x8& x, int place) {
-  const int half = (threadIdx.x & 63) >> 5;
-  const u32x4 w = __builtin_bit_cast(u32x4, x);
-  u32x4 r;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int k0 = 8 * (j / 2) + 4 * half + 2 * (j % 2);
-    r[j] = (k0 == place ? w[j] & 0xFFFFu : 0u) | (k0 + 1 == place ? w[j] & 0xFFFF0000u : 0u);
-  }
-  return __builtin_bit_cast(bf16x8, r);
-}
-
-// acc += the product of 16 rows of a tile, read as columns, with weights w, where some lanes do not see some of these rows and
-// an element is no finite number: 0 times it would be NaN for every lane.  Place by place, and each lane takes those that
-// it sees: from lo on, below hi, and set in valid.
-template <int DP>
-__device__ __forceinline__ void add_seen(f32x16 (&acc)[DP / 32], const char* area, int row0, const bf16x8& w, int lo, int hi, uint32_t valid) {
-#pragma unroll 1
-  for (int place = 0; place < 16; ++place) {
-    const bf16x8 b = only_place(w, place);
-    const bool in = place >= lo && place < hi && ((valid >> place) & 1);
-#pragma unroll
-    for (int d = 0; d < DP / 32; ++d) {
-      const f32x16 t = MfmaBf16::mma(only_place(cols_fragment<DP>(area, row0, 32 * d), place), b, MfmaBf16::zero());
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc[d][r] += in ? t[r] : 0.0f;
-    }
-  }
-}
+// What a row does not see has weight 0, and 0 times NaN or infinity would spoil it in the products.  Keys (rows) that are
+// not there are zeros in LDS; those of the sequence that only some rows of a tile see are looked through, and from the
+// first tile that holds an element that is no finite number on, such tiles are left out and added at the end key by
+// key, each lane taking what it sees: by half_dot and add_row.
 // Whether a tile's rows row0 .. + 16 steps - 1 hold an element that is no finite number.
 template <int DP>
 __device__ __forceinline__ bool any_not_finite(const char* area, int row0, int steps) {
   uint32_t f = 0;
+#pragma unroll 1
   for (int e = 0; e < steps; ++e)
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d) f |= not_finite(cols_fragment<DP>(area, row0 + 16 * e, 32 * d));
   return __any(f != 0);
+}
+
+// This half's share of the product of the lane's row, held as an operand, and the row at p (the same for all lanes).
+template <int DP>
+__device__ __forceinline__ float half_dot(const bf16x8 (&f)[DP / 16], const uint16_t* p, int dim) {
+  float sum = 0.0f;
+#pragma unroll
+  for (int kk = 0; kk < DP / 16; ++kk) {
+    const int col = 16 * kk + 8 * ((threadIdx.x & 63) >> 5);
+    if (col >= dim) continue;
+    const u32x4 x = *reinterpret_cast<const u32x4*>(p + col), y = __builtin_bit_cast(u32x4, f[kk]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      sum = __builtin_fmaf(__uint_as_float(x[j] << 16), __uint_as_float(y[j] << 16), sum);
+      sum = __builtin_fmaf(__uint_as_float(x[j] & 0xFFFF0000u), __uint_as_float(y[j] & 0xFFFF0000u), sum);
+    }
+  }
+  return sum;
+}
+// acc += w times the row at p, columns 32 d + 8 g + 4 (l / 32) + j.
+template <int DP>
+__device__ __forceinline__ void add_row(f32x16 (&acc)[DP / 32], float w, const uint16_t* p, int dim) {
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int col = 32 * d + 8 * g + 4 * ((threadIdx.x & 63) >> 5);
+      if (col >= dim) continue;
+      const u32x2 x = *reinterpret_cast<const u32x2*>(p + col);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        acc[d][4 * g + 2 * j] = __builtin_fmaf(w, __uint_as_float(x[j] << 16), acc[d][4 * g + 2 * j]);
+        acc[d][4 * g + 2 * j + 1] = __builtin_fmaf(w, __uint_as_float(x[j] & 0xFFFF0000u), acc[d][4 * g + 2 * j + 1]);
+      }
+    }
 }
 
 // r / group for r below 2^31.

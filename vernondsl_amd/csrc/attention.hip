@@ -60,30 +60,45 @@ struct KeySource {
     }
     return e;
   }
-  // Tile j0 to the slot at `to` (its keys, then its values).  Keys past the last one repeat it, keys without a page take
-  // page 0: they are masked.
+  // Paged: key j's place among the caches' rows, in page e.
+  __device__ __forceinline__ int64_t place(int e, int j) const {
+    return ((static_cast<int64_t>(e) * kv_heads + head) << shift) + (j & ((1 << shift) - 1));
+  }
+  // The first element of key j's row of k (of v), j the same for all lanes, of a page that is one.
+  __device__ __forceinline__ const uint16_t* row(const char* base, uint32_t bytes, int j) const {
+    const int64_t at = PAGED ? place(table[j >> shift], j) : j;
+    return reinterpret_cast<const uint16_t*>(base + at * bytes);
+  }
+  // Tile j0 to the slot at `to` (its keys, then its values); keys past the last one and without a page are zeros there.
   __device__ __forceinline__ void copy(int j0, int entries, char* to, int wave) const {
-    const int dc = dim / 8;
-    if constexpr (!PAGED) {
-      const char* const kb = k + static_cast<int64_t>(j0) * k_row;
-      const char* const vb = v + static_cast<int64_t>(j0) * v_row;
-      const int last = keys - 1 - j0;
+    const int dc = dim / 8, last = keys - 1 - j0;
+    const bool whole = PAGED ? __all(entries >= 0) : last >= KT - 1;
 #pragma unroll
-      for (int u = 0; u < C; ++u) {
-        const uint32_t r = min(row_of[u], last);
-        if (chunk[u] >= dc) continue;
-        lds_copy16(kb + r * k_row + 16 * chunk[u], to + (wave * C + u) * 1024);
-        lds_copy16(vb + r * v_row + 16 * chunk[u], to + KT * T::PITCH + (wave * C + u) * 1024);
+    for (int u = 0; u < C; ++u) {
+      char* const kt = to + (wave * C + u) * 1024;
+      char* const vt = kt + KT * T::PITCH;
+      int64_t at = 0;
+      bool there = true;
+      if constexpr (PAGED) {
+        const int e = __shfl(entries, row_of[u], 64);
+        there = e >= 0;
+        at = place(e, j0 + row_of[u]);
+      } else {
+        there = row_of[u] <= last;
       }
-    } else {
-#pragma unroll
-      for (int u = 0; u < C; ++u) {
-        const int r = min(row_of[u], keys - 1 - j0);
-        const int e = max(__shfl(entries, r, 64), 0);
-        const int64_t at = ((static_cast<int64_t>(e) * kv_heads + head) << shift) + ((j0 + r) & ((1 << shift) - 1));
-        if (chunk[u] >= dc) continue;
-        lds_copy16(k + at * k_row + 16 * chunk[u], to + (wave * C + u) * 1024);
-        lds_copy16(v + at * v_row + 16 * chunk[u], to + KT * T::PITCH + (wave * C + u) * 1024);
+      if (chunk[u] >= dc) continue;
+      if (whole || there) {
+        if constexpr (PAGED) {
+          lds_copy16(k + at * k_row + 16 * chunk[u], kt);
+          lds_copy16(v + at * v_row + 16 * chunk[u], vt);
+        } else {
+          lds_copy16(k + static_cast<int64_t>(j0) * k_row + (static_cast<uint32_t>(row_of[u]) * k_row + 16 * chunk[u]), kt);
+          lds_copy16(v + static_cast<int64_t>(j0) * v_row + (static_cast<uint32_t>(row_of[u]) * v_row + 16 * chunk[u]), vt);
+        }
+      } else {
+        const int lane = threadIdx.x & 63;
+        *reinterpret_cast<u32x4*>(kt + 16 * lane) = u32x4{0u, 0u, 0u, 0u};
+        *reinterpret_cast<u32x4*>(vt + 16 * lane) = u32x4{0u, 0u, 0u, 0u};
       }
     }
   }
@@ -324,19 +339,25 @@ __global__ __launch_bounds__(256, QT == 1 ? 2 : 1) void attention_rows(Attention
     for (int i = threadIdx.x; i < NS * SLOT / 16; i += 256) reinterpret_cast<u32x4*>(smem)[i] = u32x4{0u, 0u, 0u, 0u};
     __syncthreads();
   }
-  uint64_t valid[NS];  // paged: which keys of a slot's tile hold something
+  // Paged: which keys of a tile hold something (bits of the tiles in flight, the next one to be used last), and this lane's
+  // entry of the page table for the tile that is copied next.
+  uint64_t valid[NS];
   int entries = -1;
+#pragma unroll
+  for (int t = 0; t < NS; ++t) valid[t] = ~0ull;
   const auto fetch = [&](int t, int slot) {
-    if constexpr (PAGED) valid[slot] = __ballot(entries >= 0);
+    if constexpr (PAGED) {
+#pragma unroll
+      for (int i = NS - 1; i > 0; --i) valid[i] = valid[i - 1];
+      valid[0] = __ballot(entries >= 0);
+    }
     src.copy(t * KT, entries, smem + slot * SLOT, wave);
   };
 #pragma unroll
   for (int t = 0; t < NS - 1; ++t) {
-    valid[t] = ~0ull;
     if constexpr (PAGED) entries = src.entry(min(first + t, end - 1) * KT);
     fetch(min(first + t, end - 1), t);
   }
-  valid[NS - 1] = ~0ull;
   if constexpr (PAGED) entries = src.entry(min(first + NS - 1, end - 1) * KT);
 
   const int row0 = tile.row + wave * 32 * QT;
@@ -353,68 +374,70 @@ __global__ __launch_bounds__(256, QT == 1 ? 2 : 1) void attention_rows(Attention
   const int fewest = __builtin_amdgcn_readfirstlane(at.sees(min(row0, at.rows - 1), a.group, a.causal));
   const int most = mine ? at.sees(min(row0 + 32 * QT, at.rows) - 1, a.group, a.causal) : 0;
 
-  for (int t0 = first; t0 < end; t0 += NS) {
+  int slot = 0, left_out = 0x7fffffff;
+#pragma unroll 1
+  for (int t = first; t < end; ++t) {
+    // copies of the tiles behind t stay in flight
+    if constexpr (PAGED) dma_wait<0>();
+    else dma_wait<(NS - 2) * 2 * KeySource<DP, KT, 4, PAGED>::C>();
+    dma_barrier();
+    // past the end the last tile again, so that the waits count the same
+    fetch(min(t + NS - 1, end - 1), slot == 0 ? NS - 1 : slot - 1);
+    if constexpr (PAGED) entries = src.entry(min(t + NS, end - 1) * KT);
+    const char* const keys = smem + slot * SLOT;
+    const char* const values = keys + KT * T::PITCH;
+    slot = slot + 1 == NS ? 0 : slot + 1;
+    const int j0 = t * KT;
+    if (j0 >= most) continue;
+    f32x16 s[QT][KS];
 #pragma unroll
-    for (int slot = 0; slot < NS; ++slot) {
-      const int t = t0 + slot;
-      if (t >= end) break;
-      // copies of the tiles behind t stay in flight
-      if constexpr (PAGED) dma_wait<0>();
-      else dma_wait<(NS - 2) * 2 * KeySource<DP, KT, 4, PAGED>::C>();
-      dma_barrier();
-      {
-        constexpr int ahead = NS - 1;
-        const int to = (slot + ahead) % NS;
-        fetch(min(t + ahead, end - 1), to);  // past the end the last tile again, so that the waits count the same
-        if constexpr (PAGED) entries = src.entry(min(t + NS, end - 1) * KT);
-      }
-      const int j0 = t * KT;
-      if (j0 >= most) continue;
-      const char* const keys = smem + slot * SLOT;
-      const char* const values = keys + KT * T::PITCH;
-      f32x16 s[QT][KS];
+    for (int k = 0; k < KS; ++k) {
 #pragma unroll
-      for (int k = 0; k < KS; ++k) {
+      for (int c = 0; c < QT; ++c) s[c][k] = MfmaBf16::zero();
 #pragma unroll
-        for (int c = 0; c < QT; ++c) s[c][k] = MfmaBf16::zero();
+      for (int kk = 0; kk < DP / 16; ++kk) {
+        const bf16x8 f = rows_fragment<DP>(keys, 32 * k, kk);
 #pragma unroll
-        for (int kk = 0; kk < DP / 16; ++kk) {
-          const bf16x8 f = rows_fragment<DP>(keys, 32 * k, kk);
-#pragma unroll
-          for (int c = 0; c < QT; ++c) s[c][k] = MfmaBf16::mma(f, qf[c][kk], s[c][k]);
-        }
-      }
-      const bool masked = j0 + KT > fewest || (PAGED && valid[slot] != ~0ull);
-      if (masked) {
-#pragma unroll
-        for (int c = 0; c < QT; ++c) hide(s[c], sees[c] - j0, valid[slot]);
-      }
-#pragma unroll
-      for (int c = 0; c < QT; ++c) st.weigh(s[c], c, scale2);
-      if (masked && any_not_finite<DP>(values, 0, 2 * KS)) {
-#pragma unroll
-        for (int e = 0; e < 2 * KS; ++e)
-#pragma unroll
-          for (int c = 0; c < QT; ++c)
-            add_seen<DP>(st.o[c], values, 16 * e, weights_fragment(s[c][e / 2], e % 2), 0, sees[c] - j0 - 16 * e,
-                         static_cast<uint32_t>(valid[slot] >> (16 * e)) & 0xFFFFu);
-        continue;
-      }
-#pragma unroll
-      for (int e = 0; e < 2 * KS; ++e) {
-        bf16x8 w[QT];
-#pragma unroll
-        for (int c = 0; c < QT; ++c) w[c] = weights_fragment(s[c][e / 2], e % 2);
-#pragma unroll
-        for (int d = 0; d < DP / 32; ++d) {
-          const bf16x8 f = cols_fragment<DP>(values, 16 * e, 32 * d);
-#pragma unroll
-          for (int c = 0; c < QT; ++c) st.o[c][d] = MfmaBf16::mma(f, w[c], st.o[c][d]);
-        }
+        for (int c = 0; c < QT; ++c) s[c][k] = MfmaBf16::mma(f, qf[c][kk], s[c][k]);
       }
     }
+    const uint64_t there = valid[NS - 1];
+    const bool masked = j0 + KT > fewest || (PAGED && there != ~0ull);
+    if (masked) {
+#pragma unroll
+      for (int c = 0; c < QT; ++c) hide(s[c], sees[c] - j0, there);
+    }
+    bf16x8 w[QT][2 * KS];
+#pragma unroll
+    for (int c = 0; c < QT; ++c) {
+      st.weigh(s[c], c, scale2);
+#pragma unroll
+      for (int e = 0; e < 2 * KS; ++e) w[c][e] = weights_fragment(s[c][e / 2], e % 2);
+    }
+    // some rows do not see some of these keys
+    if (a.causal && j0 + KT > fewest && (j0 >= left_out || any_not_finite<DP>(values, 0, 2 * KS))) {
+      left_out = min(left_out, j0);
+      continue;
+    }
+#pragma unroll
+    for (int e = 0; e < 2 * KS; ++e)
+#pragma unroll
+      for (int d = 0; d < DP / 32; ++d) {
+        const bf16x8 f = cols_fragment<DP>(values, 16 * e, 32 * d);
+#pragma unroll
+        for (int c = 0; c < QT; ++c) st.o[c][d] = MfmaBf16::mma(f, w[c][e], st.o[c][d]);
+      }
   }
   dma_wait<0>();
+#pragma unroll 1
+  for (int j = left_out; j < min(most, end * KT); ++j) {
+    if (PAGED && static_cast<uint32_t>(src.table[j >> src.shift]) >= static_cast<uint64_t>(a.pages)) continue;
+#pragma unroll
+    for (int c = 0; c < QT; ++c) {
+      const float s = halves_sum(half_dot<DP>(qf[c], src.row(src.k, src.k_row, j), a.dim));
+      if (j < sees[c]) add_row<DP>(st.o[c], __builtin_amdgcn_exp2f(__builtin_fmaf(s, scale2, -(st.m[c] == neg_inf() ? 0.0f : st.m[c]))), src.row(src.v, src.v_row, j), a.dim);
+    }
+  }
   if (mine) store_rows(a, st, at, row0, place.kv, place.split);
 }
 

@@ -106,14 +106,22 @@ struct PairCopies {
       chunk[u] = lane % T::CPR ^ T::swz(row_of[u]);
     }
   }
-  // at(row of the tile, which operand): that row's first byte
+  // Rows 0 .. last of a tile; those behind are zeros.  at(row of the tile, which operand): that row's first byte.
   template <class At>
-  __device__ __forceinline__ void operator()(char* to, int wave, int dim, At&& at) const {
+  __device__ __forceinline__ void operator()(char* to, int wave, int dim, int last, At&& at) const {
 #pragma unroll
     for (int u = 0; u < C; ++u) {
       if (chunk[u] >= dim / 8) continue;
-      lds_copy16(at(row_of[u], 0) + 16 * chunk[u], to + (wave * C + u) * 1024);
-      lds_copy16(at(row_of[u], 1) + 16 * chunk[u], to + TR * T::PITCH + (wave * C + u) * 1024);
+      char* const first = to + (wave * C + u) * 1024;
+      char* const second = first + TR * T::PITCH;
+      if (last >= TR - 1 || row_of[u] <= last) {
+        lds_copy16(at(row_of[u], 0) + 16 * chunk[u], first);
+        lds_copy16(at(row_of[u], 1) + 16 * chunk[u], second);
+      } else {
+        const int lane = threadIdx.x & 63;
+        *reinterpret_cast<u32x4*>(first + 16 * lane) = u32x4{0u, 0u, 0u, 0u};
+        *reinterpret_cast<u32x4*>(second + 16 * lane) = u32x4{0u, 0u, 0u, 0u};
+      }
     }
   }
 };
@@ -156,8 +164,8 @@ __global__ __launch_bounds__(256, 1) void attention_bwd_keys(GradArgs a) {
   const float2* const sp = a.rows + (static_cast<int64_t>(kv) * a.seqs.n + tile.token) * a.group;
   float2 next;
   const auto fetch = [&](int t, int slot) {
-    copies(smem + slot * Copies::SLOT, wave, a.dim, [&](int r, int which) {
-      const int row = min(t * TR + r, rows - 1), i = a.token_of(row);
+    copies(smem + slot * Copies::SLOT, wave, a.dim, rows - 1 - t * TR, [&](int r, int which) {
+      const int row = t * TR + r, i = a.token_of(row);
       const int64_t col = static_cast<int64_t>(row - i * a.group) * a.dim;
       return which == 0 ? qp + 2 * (i * a.q_stride + col) : dp + 2 * (i * a.dout_stride + col);
     });
@@ -173,66 +181,73 @@ __global__ __launch_bounds__(256, 1) void attention_bwd_keys(GradArgs a) {
   const float scale2 = a.scale * kLog2e;
   const int sees_from = a.causal ? key * a.group : 0;  // the key's first row
   const int wave_first = a.causal ? (tile.row + 32 * wave) * a.group : 0, wave_all = a.causal ? (tile.row + 32 * wave + 31) * a.group : 0;
-  for (int t0 = first; t0 < end; t0 += NS) {
+  int slot = 0, left_out = 0x7fffffff;
+#pragma unroll 1
+  for (int t = first; t < end; ++t) {
+    const int ahead = min(t + NS - 1, end - 1), to = slot == 0 ? NS - 1 : slot - 1;
+    dma_wait<0>();
+    __syncthreads();
+    if (threadIdx.x < TR) next = sp[min(ahead * TR + static_cast<int>(threadIdx.x), rows - 1)];
+    fetch(ahead, to);
+    const char* const qs = smem + slot * Copies::SLOT;
+    const char* const ds = qs + TR * T::PITCH;
+    const float2* const stats = stat[slot];
+    slot = slot + 1 == NS ? 0 : slot + 1;
+    if ((t + 1) * TR > wave_first) {
+#pragma unroll 1
+      for (int u = 0; u < TR / 32; ++u) {
+        const int r0 = t * TR + 32 * u;
+        f32x16 s = MfmaBf16::zero(), p = MfmaBf16::zero();
 #pragma unroll
-    for (int slot = 0; slot < NS; ++slot) {
-      const int t = t0 + slot;
-      if (t >= end) break;
-      const int ahead = min(t + NS - 1, end - 1), to = (slot + NS - 1) % NS;
-      dma_wait<0>();
-      __syncthreads();
-      if (threadIdx.x < TR) next = sp[min(ahead * TR + static_cast<int>(threadIdx.x), rows - 1)];
-      fetch(ahead, to);
-      const char* const qs = smem + slot * Copies::SLOT;
-      const char* const ds = qs + TR * T::PITCH;
-      if ((t + 1) * TR > wave_first) {
+        for (int kk = 0; kk < DP / 16; ++kk) {
+          s = MfmaBf16::mma(rows_fragment<DP>(qs, 32 * u, kk), kf[kk], s);
+          p = MfmaBf16::mma(rows_fragment<DP>(ds, 32 * u, kk), vf[kk], p);
+        }
+        const bool masked = r0 < wave_all || r0 + 32 > rows;
+        const int lo = sees_from - r0, hi = rows - r0;
 #pragma unroll
-        for (int u = 0; u < TR / 32; ++u) {
-          const int r0 = t * TR + 32 * u;
-          f32x16 s = MfmaBf16::zero(), p = MfmaBf16::zero();
+        for (int g = 0; g < 4; ++g) {
 #pragma unroll
-          for (int kk = 0; kk < DP / 16; ++kk) {
-            s = MfmaBf16::mma(rows_fragment<DP>(qs, 32 * u, kk), kf[kk], s);
-            p = MfmaBf16::mma(rows_fragment<DP>(ds, 32 * u, kk), vf[kk], p);
-          }
-          const bool masked = r0 < wave_all || r0 + 32 > rows;
-          const int lo = sees_from - r0, hi = rows - r0;
-#pragma unroll
-          for (int g = 0; g < 4; ++g) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const int r = 8 * g + 4 * half + j;
-              const float2 st = stat[slot][32 * u + r];
-              float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * g + j], scale2, -st.x));
-              float d = w * (p[4 * g + j] - st.y);
-              if (masked && !(r >= lo && r < hi)) w = d = 0.0f;
-              s[4 * g + j] = w;
-              p[4 * g + j] = d;
-            }
-          }
-          if (masked && (any_not_finite<DP>(qs, 32 * u, 2) || any_not_finite<DP>(ds, 32 * u, 2))) {
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              add_seen<DP>(dv, ds, 32 * u + 16 * e, weights_fragment(s, e), lo - 16 * e, hi - 16 * e, 0xFFFFu);
-              add_seen<DP>(dk, qs, 32 * u + 16 * e, weights_fragment(p, e), lo - 16 * e, hi - 16 * e, 0xFFFFu);
-            }
-            continue;
-          }
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const bf16x8 w = weights_fragment(s, e), d = weights_fragment(p, e);
-#pragma unroll
-            for (int x = 0; x < DP / 32; ++x) {
-              dv[x] = MfmaBf16::mma(cols_fragment<DP>(ds, 32 * u + 16 * e, 32 * x), w, dv[x]);
-              dk[x] = MfmaBf16::mma(cols_fragment<DP>(qs, 32 * u + 16 * e, 32 * x), d, dk[x]);
-            }
+          for (int j = 0; j < 4; ++j) {
+            const int r = 8 * g + 4 * half + j;
+            const float2 st = stats[32 * u + r];
+            float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * g + j], scale2, -st.x));
+            float d = w * (p[4 * g + j] - st.y);
+            if (masked && !(r >= lo && r < hi)) w = d = 0.0f;
+            s[4 * g + j] = w;
+            p[4 * g + j] = d;
           }
         }
+        const bf16x8 w[2] = {weights_fragment(s, 0), weights_fragment(s, 1)}, d[2] = {weights_fragment(p, 0), weights_fragment(p, 1)};
+        // some keys are not seen by some of these rows
+        if (r0 < wave_all && (r0 >= left_out || any_not_finite<DP>(qs, 32 * u, 2) || any_not_finite<DP>(ds, 32 * u, 2))) {
+          left_out = min(left_out, r0);
+          continue;
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int x = 0; x < DP / 32; ++x) {
+            dv[x] = MfmaBf16::mma(cols_fragment<DP>(ds, 32 * u + 16 * e, 32 * x), w[e], dv[x]);
+            dk[x] = MfmaBf16::mma(cols_fragment<DP>(qs, 32 * u + 16 * e, 32 * x), d[e], dk[x]);
+          }
       }
-      if (threadIdx.x < TR) stat[to][threadIdx.x] = next;
     }
+    if (threadIdx.x < TR) stat[to][threadIdx.x] = next;
   }
   dma_wait<0>();
+#pragma unroll 1
+  for (int r = left_out; r < min((wave_all + 31) & ~31, rows); ++r) {
+    const int i = a.token_of(r);
+    const int64_t col = static_cast<int64_t>(r - i * a.group) * a.dim;
+    const uint16_t* const qr = reinterpret_cast<const uint16_t*>(qp) + i * a.q_stride + col;
+    const uint16_t* const dr = reinterpret_cast<const uint16_t*>(dp) + i * a.dout_stride + col;
+    const float s = halves_sum(half_dot<DP>(kf, qr, a.dim)), p = halves_sum(half_dot<DP>(vf, dr, a.dim));
+    if (r < sees_from) continue;
+    const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s, scale2, -sp[r].x));
+    add_row<DP>(dv, w, dr, a.dim);
+    add_row<DP>(dk, w * (p - sp[r].y), qr, a.dim);
+  }
   if (key < tile.len) {
     store_gradient<DP>(dk, a.scale, a.grad_dtype, a.dk, a.dk_first + token * a.dk_stride + head_col, a.dim);
     store_gradient<DP>(dv, 1.0f, a.grad_dtype, a.dv, a.dv_first + token * a.dv_stride + head_col, a.dim);
@@ -241,8 +256,8 @@ __global__ __launch_bounds__(256, 1) void attention_bwd_keys(GradArgs a) {
 
 // dq: four waves of QT x 32 rows each, walking over tiles of 64 keys.
 template <int DP, int QT>
-__global__ __launch_bounds__(256, 1) void attention_bwd_queries(GradArgs a) {
-  constexpr int KT = 64, NS = 4, ROWS = 128 * QT;
+__global__ __launch_bounds__(256, QT == 1 ? 2 : 1) void attention_bwd_queries(GradArgs a) {
+  constexpr int KT = 64, NS = QT == 1 ? 2 : 4, ROWS = 128 * QT;
   using T = TileShape<DP>;
   using Copies = PairCopies<DP, KT>;
   __shared__ __attribute__((aligned(1024))) char smem[NS * Copies::SLOT];
@@ -272,8 +287,8 @@ __global__ __launch_bounds__(256, 1) void attention_bwd_queries(GradArgs a) {
   const char* const kp = reinterpret_cast<const char*>(a.k + tile.token * a.k_stride + head_col);
   const char* const vp = reinterpret_cast<const char*>(a.v + tile.token * a.v_stride + head_col);
   const auto fetch = [&](int t, int slot) {
-    copies(smem + slot * Copies::SLOT, wave, a.dim, [&](int r, int which) {
-      const int64_t i = min(t * KT + r, tile.len - 1);
+    copies(smem + slot * Copies::SLOT, wave, a.dim, tile.len - 1 - t * KT, [&](int r, int which) {
+      const int64_t i = t * KT + r;
       return which == 0 ? kp + 2 * i * a.k_stride : vp + 2 * i * a.v_stride;
     });
   };
@@ -297,67 +312,72 @@ __global__ __launch_bounds__(256, 1) void attention_bwd_queries(GradArgs a) {
   const float scale2 = a.scale * kLog2e;
   const bool mine = row0 < rows;
   const int fewest = sees(min(row0, rows - 1)), most = mine ? sees(min(row0 + 32 * QT, rows) - 1) : 0;
-  for (int t0 = 0; t0 < end; t0 += NS) {
+  int slot = 0, left_out = 0x7fffffff;
+#pragma unroll 1
+  for (int t = 0; t < end; ++t) {
+    dma_wait<(NS - 2) * 2 * Copies::C>();
+    dma_barrier();
+    fetch(min(t + NS - 1, end - 1), slot == 0 ? NS - 1 : slot - 1);
+    const char* const ks = smem + slot * Copies::SLOT;
+    const char* const vs = ks + KT * T::PITCH;
+    slot = slot + 1 == NS ? 0 : slot + 1;
+#pragma unroll 1
+    for (int u = 0; u < KT / 32; ++u) {
+      const int j0 = t * KT + 32 * u;
+      if (j0 >= most) break;
+      f32x16 s[QT], p[QT];
 #pragma unroll
-    for (int slot = 0; slot < NS; ++slot) {
-      const int t = t0 + slot;
-      if (t >= end) break;
-      dma_wait<(NS - 2) * 2 * Copies::C>();
-      dma_barrier();
-      fetch(min(t + NS - 1, end - 1), (slot + NS - 1) % NS);
-      const char* const ks = smem + slot * Copies::SLOT;
-      const char* const vs = ks + KT * T::PITCH;
+      for (int c = 0; c < QT; ++c) s[c] = p[c] = MfmaBf16::zero();
 #pragma unroll
-      for (int u = 0; u < KT / 32; ++u) {
-        const int j0 = t * KT + 32 * u;
-        if (j0 >= most) continue;
-        f32x16 s[QT], p[QT];
-#pragma unroll
-        for (int c = 0; c < QT; ++c) s[c] = p[c] = MfmaBf16::zero();
-#pragma unroll
-        for (int kk = 0; kk < DP / 16; ++kk) {
-          const bf16x8 kf = rows_fragment<DP>(ks, 32 * u, kk), vf = rows_fragment<DP>(vs, 32 * u, kk);
-#pragma unroll
-          for (int c = 0; c < QT; ++c) {
-            s[c] = MfmaBf16::mma(kf, qf[c][kk], s[c]);
-            p[c] = MfmaBf16::mma(vf, df[c][kk], p[c]);
-          }
-        }
-        const bool masked = j0 + 32 > fewest;
+      for (int kk = 0; kk < DP / 16; ++kk) {
+        const bf16x8 kf = rows_fragment<DP>(ks, 32 * u, kk), vf = rows_fragment<DP>(vs, 32 * u, kk);
 #pragma unroll
         for (int c = 0; c < QT; ++c) {
-          const int hi = seen[c] - j0 - 4 * (lane >> 5);
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[c][r], scale2, -st[c].x));
-            p[c][r] = w * (p[c][r] - st[c].y);
-            if (masked && !(8 * (r / 4) + r % 4 < hi)) p[c][r] = 0.0f;
-          }
-        }
-        if (masked && any_not_finite<DP>(ks, 32 * u, 2)) {
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-#pragma unroll
-            for (int c = 0; c < QT; ++c)
-              add_seen<DP>(dq[c], ks, 32 * u + 16 * e, weights_fragment(p[c], e), 0, seen[c] - j0 - 16 * e, 0xFFFFu);
-          continue;
-        }
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          bf16x8 w[QT];
-#pragma unroll
-          for (int c = 0; c < QT; ++c) w[c] = weights_fragment(p[c], e);
-#pragma unroll
-          for (int d = 0; d < DP / 32; ++d) {
-            const bf16x8 f = cols_fragment<DP>(ks, 32 * u + 16 * e, 32 * d);
-#pragma unroll
-            for (int c = 0; c < QT; ++c) dq[c][d] = MfmaBf16::mma(f, w[c], dq[c][d]);
-          }
+          s[c] = MfmaBf16::mma(kf, qf[c][kk], s[c]);
+          p[c] = MfmaBf16::mma(vf, df[c][kk], p[c]);
         }
       }
+      const bool masked = j0 + 32 > fewest;
+      bf16x8 w[QT][2];
+#pragma unroll
+      for (int c = 0; c < QT; ++c) {
+        const int hi = seen[c] - j0 - 4 * (lane >> 5);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[c][r], scale2, -st[c].x));
+          p[c][r] = e * (p[c][r] - st[c].y);
+          if (masked && !(8 * (r / 4) + r % 4 < hi)) p[c][r] = 0.0f;
+        }
+        w[c][0] = weights_fragment(p[c], 0);
+        w[c][1] = weights_fragment(p[c], 1);
+      }
+      // some rows do not see some of these keys
+      if (a.causal && masked && (j0 >= left_out || any_not_finite<DP>(ks, 32 * u, 2))) {
+        left_out = min(left_out, j0);
+        continue;
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) {
+          const bf16x8 f = cols_fragment<DP>(ks, 32 * u + 16 * e, 32 * d);
+#pragma unroll
+          for (int c = 0; c < QT; ++c) dq[c][d] = MfmaBf16::mma(f, w[c][e], dq[c][d]);
+        }
     }
   }
   dma_wait<0>();
+#pragma unroll 1
+  for (int j = left_out; j < most; ++j) {
+    const uint16_t* const kr = reinterpret_cast<const uint16_t*>(kp) + j * a.k_stride;
+    const uint16_t* const vr = reinterpret_cast<const uint16_t*>(vp) + j * a.v_stride;
+#pragma unroll
+    for (int c = 0; c < QT; ++c) {
+      const float s = halves_sum(half_dot<DP>(qf[c], kr, a.dim)), p = halves_sum(half_dot<DP>(df[c], vr, a.dim));
+      if (j >= seen[c]) continue;
+      add_row<DP>(dq[c], __builtin_amdgcn_exp2f(__builtin_fmaf(s, scale2, -st[c].x)) * (p - st[c].y), kr, a.dim);
+    }
+  }
 #pragma unroll
   for (int c = 0; c < QT; ++c) {
     const int row = row0 + 32 * c + (lane & 31);
@@ -459,7 +479,7 @@ extern "C" int vdsl_op_attention_bwd(vdsl_queue q, const vdsl_attention_params* 
                      out->ptr, out_dtype, static_cast<const float*>(lse->ptr), p->n, p->heads, group, p->dim, copy, rows);
   VDSL_TRY(check_launch("attention_bwd_rows"));
   const int64_t key_slots = row_slots(p->n, p->seqs, 1, 7);
-  const int qt = p->n * p->heads >= 256 * 256 ? 2 : 1;
+  const int qt = p->dim <= 64 && p->n * p->heads >= 256 * 256 ? 2 : 1;
   const int64_t row_slots_ = row_slots(p->n, p->seqs, group, qt == 1 ? 7 : 8);
   if (std::max(key_slots, row_slots_) * p->kv_heads > 0x7fffff) return fail(VDSL_ERR_UNSUPPORTED, "attention_bwd: too many rows");
   const auto go = [&](auto kernel, int64_t slots, const char* name) {
@@ -474,8 +494,8 @@ extern "C" int vdsl_op_attention_bwd(vdsl_queue q, const vdsl_attention_params* 
   }
   if (p->dim <= 96) {
     VDSL_TRY(go(attention_bwd_keys<96>, key_slots, keys));
-    return go(qt == 1 ? attention_bwd_queries<96, 1> : attention_bwd_queries<96, 2>, row_slots_, queries);
+    return go(attention_bwd_queries<96, 1>, row_slots_, queries);
   }
   VDSL_TRY(go(attention_bwd_keys<128>, key_slots, keys));
-  return go(qt == 1 ? attention_bwd_queries<128, 1> : attention_bwd_queries<128, 2>, row_slots_, queries);
+  return go(attention_bwd_queries<128, 1>, row_slots_, queries);
 }

@@ -734,7 +734,7 @@ int vdsl_op_rope(vdsl_queue q, const vdsl_rope_params* p, int32_t x_dtype, vdsl_
  * A row of no sequence, or whose scores are -inf all of them, has out 0 and lse -inf.  What a row does not see has no
  * influence on it, NaN and infinity included.  q, k, v: BF16; scores, sums and statistics are f32, the weights
  * exp(s[j] - max) are rounded to bf16 for the second product.  out: F32 or BF16 [n][heads * dim], every row written;
- * lse: F32 [heads][n], or NULL.  dim: a multiple of 8 up to 128.  scale: a positive normal number. */
+ * lse: F32 [heads][n], or NULL.  dim: a multiple of 8 up to 128.  scale: from 2^-100 to 2^100. */
 typedef struct vdsl_attention_params {
   int64_t n;
   int64_t seqs;

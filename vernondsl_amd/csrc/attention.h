@@ -109,6 +109,19 @@ __device__ __forceinline__ bf16x8 cols_fragment(const char* area, int row0, int 
   return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
+// 32 rows of this lane's wave as an operand (element j of lane l: column 16 kk + 8 (l / 32) + j of row l % 32), from
+// the lane's own row at p.
+template <int DP>
+__device__ __forceinline__ void load_operand(const uint16_t* p, int dim, bf16x8 (&f)[DP / 16]) {
+#pragma unroll
+  for (int kk = 0; kk < DP / 16; ++kk) {
+    const int col = 16 * kk + 8 * ((threadIdx.x & 63) >> 5);
+    u32x4 w = {0u, 0u, 0u, 0u};
+    if (col < dim) w = *reinterpret_cast<const u32x4*>(p + col);
+    f[kk] = __builtin_bit_cast(bf16x8, w);
+  }
+}
+
 // The values of lanes l % 32 and l % 32 + 32, in every lane.
 __device__ __forceinline__ f32x2_t both_halves(float v) {
   const uint32_t b = __builtin_bit_cast(uint32_t, v);

@@ -135,42 +135,39 @@ __device__ __forceinline__ RowsAt rows_at(const AttentionArgs& a, const RowTile&
   return r;
 }
 
-// The state of a wave's QT tiles of 32 rows: this lane has row lane % 32 of each and, of its 32 x (16 DP / 32) outputs,
-// o[c][d][r] of column 32 d + 8 (r / 4) + 4 (lane / 32) + r % 4.
-template <int DP, int QT>
+// The state of a wave's 32 rows: this lane has row lane % 32 and, of its outputs, o[d][r] of column
+// 32 d + 8 (r / 4) + 4 (lane / 32) + r % 4.
+template <int DP>
 struct RowState {
-  f32x16 o[QT][DP / 32];
-  float m[QT], l[QT];  // m in powers of two (times c); l: this half's share
+  f32x16 o[DP / 32];
+  float m, l;  // m in powers of two (times c); l: this half's share
 
   __device__ __forceinline__ void clear() {
+    m = neg_inf();
+    l = 0.0f;
 #pragma unroll
-    for (int c = 0; c < QT; ++c) {
-      m[c] = neg_inf();
-      l[c] = 0.0f;
-#pragma unroll
-      for (int d = 0; d < DP / 32; ++d) o[c][d] = MfmaBf16::zero();
-    }
+    for (int d = 0; d < DP / 32; ++d) o[d] = MfmaBf16::zero();
   }
-  // s: the scores of row tile c over KS x 32 keys, those that are not seen -inf; they become p.
+  // s: the rows' scores over KS x 32 keys, those that are not seen -inf; they become p.
   template <int KS>
-  __device__ __forceinline__ void weigh(f32x16 (&s)[KS], int c, float scale2) {
+  __device__ __forceinline__ void weigh(f32x16 (&s)[KS], float scale2) {
     float top = s[0][0];
 #pragma unroll
     for (int t = 0; t < KS; ++t)
 #pragma unroll
       for (int r = 0; r < 16; ++r) top = fmaxf(top, s[t][r]);
     top = halves_max(top) * scale2;
-    if (__any(top > m[c] + kLag)) {
-      const float now = fmaxf(m[c], top);
-      const float by = now == neg_inf() ? 1.0f : __builtin_amdgcn_exp2f(m[c] - now);
-      m[c] = now;
-      l[c] *= by;
+    if (__any(top > m + kLag)) {
+      const float now = fmaxf(m, top);
+      const float by = now == neg_inf() ? 1.0f : __builtin_amdgcn_exp2f(m - now);
+      m = now;
+      l *= by;
 #pragma unroll
       for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) o[c][d][r] *= by;
+        for (int r = 0; r < 16; ++r) o[d][r] *= by;
     }
-    const float at = m[c] == neg_inf() ? 0.0f : m[c];
+    const float at = m == neg_inf() ? 0.0f : m;
     float sum = 0.0f;
 #pragma unroll
     for (int t = 0; t < KS; ++t)
@@ -179,7 +176,7 @@ struct RowState {
         s[t][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][r], scale2, -at));
         sum += s[t][r];
       }
-    l[c] += sum;
+    l += sum;
   }
 };
 
@@ -198,43 +195,39 @@ __device__ __forceinline__ void hide(f32x16 (&s)[KS], int sees, uint64_t valid) 
 }
 
 // The rows' outputs (or their parts of split `split`) from a wave's state.
-template <int DP, int QT>
-__device__ __forceinline__ void store_rows(const AttentionArgs& a, RowState<DP, QT>& st, const RowsAt& at, int row0, int kv, int split) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int c = 0; c < QT; ++c) {
-    const int row = row0 + 32 * c + (lane & 31);
-    const float l = halves_sum(st.l[c]);
-    if (row >= at.rows) continue;
-    const int64_t token = at.token + row / a.group;
-    const int head = kv * a.group + row % a.group;
-    float by;
-    int64_t base;
-    if (a.splits > 1) {
-      const int64_t place = (static_cast<int64_t>(split) * a.kv_heads + kv) * a.seqs.n * a.group + at.token * a.group + row;
-      if (lane < 32) a.stats[place] = make_float2(st.m[c], l);
-      if (st.m[c] == neg_inf()) continue;  // not read
-      by = 1.0f;
-      base = place * a.dim;
-    } else {
-      if (a.lse && lane < 32)
-        a.lse[head * a.seqs.n + token] = st.m[c] == neg_inf() ? neg_inf() : (st.m[c] + __builtin_amdgcn_logf(l)) * kLn2;
-      by = st.m[c] == neg_inf() ? 0.0f : 1.0f / l;
-      base = (token * a.heads + head) * a.dim;
-    }
-#pragma unroll
-    for (int d = 0; d < DP / 32; ++d)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int col = 32 * d + 8 * g + 4 * (lane >> 5);
-        if (col >= a.dim) continue;
-        float v[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = st.o[c][d][4 * g + j] * by;
-        if (a.splits > 1) store_whole<VDSL_F32, 4>(a.parts, base + col, v);
-        else store_unit<4>(a.out_dtype, a.out, base + col, v);
-      }
+template <int DP>
+__device__ __forceinline__ void store_rows(const AttentionArgs& a, RowState<DP>& st, const RowsAt& at, int row0, int kv, int split) {
+  const int lane = threadIdx.x & 63, row = row0 + (lane & 31);
+  const float l = halves_sum(st.l);
+  if (row >= at.rows) return;
+  const int64_t token = at.token + row / a.group;
+  const int head = kv * a.group + row % a.group;
+  float by;
+  int64_t base;
+  if (a.splits > 1) {
+    const int64_t place = (static_cast<int64_t>(split) * a.kv_heads + kv) * a.seqs.n * a.group + at.token * a.group + row;
+    if (lane < 32) a.stats[place] = make_float2(st.m, l);
+    if (st.m == neg_inf()) return;  // not read
+    by = 1.0f;
+    base = place * a.dim;
+  } else {
+    if (a.lse && lane < 32)
+      a.lse[head * a.seqs.n + token] = st.m == neg_inf() ? neg_inf() : (st.m + __builtin_amdgcn_logf(l)) * kLn2;
+    by = st.m == neg_inf() ? 0.0f : 1.0f / l;
+    base = (token * a.heads + head) * a.dim;
   }
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int col = 32 * d + 8 * g + 4 * (lane >> 5);
+      if (col >= a.dim) continue;
+      float v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = st.o[d][4 * g + j] * by;
+      if (a.splits > 1) store_whole<VDSL_F32, 4>(a.parts, base + col, v);
+      else store_unit<4>(a.out_dtype, a.out, base + col, v);
+    }
 }
 
 // Rows of no sequence, or that see no key: out 0, lse -inf.
@@ -253,24 +246,6 @@ __device__ __forceinline__ void store_none(const AttentionArgs& a, const RowsAt&
     const int head = kv * a.group + row % a.group;
     store_unit<4>(a.out_dtype, a.out, (token * a.heads + head) * a.dim + 4 * (u % per), none);
     if (a.lse && u % per == 0) a.lse[head * a.seqs.n + token] = neg_inf();
-  }
-}
-
-// A wave's QT tiles of rows as the operand Q^T: element j of lane l is column 16 kk + 8 (l / 32) + j.
-template <int DP, int QT>
-__device__ __forceinline__ void load_rows(const AttentionArgs& a, const RowsAt& at, int row0, int kv, bf16x8 (&f)[QT][DP / 16]) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int c = 0; c < QT; ++c) {
-    const int row = min(row0 + 32 * c + (lane & 31), at.rows - 1);
-    const uint16_t* const p = a.q + (at.token + row / a.group) * a.q_stride + static_cast<int64_t>(kv * a.group + row % a.group) * a.dim;
-#pragma unroll
-    for (int kk = 0; kk < DP / 16; ++kk) {
-      const int col = 16 * kk + 8 * (lane >> 5);
-      u32x4 w = {0u, 0u, 0u, 0u};
-      if (col < a.dim) w = *reinterpret_cast<const u32x4*>(p + col);
-      f[c][kk] = __builtin_bit_cast(bf16x8, w);
-    }
   }
 }
 
@@ -310,15 +285,16 @@ struct Place {
   }
 };
 
-// Four waves of QT x 32 rows each, sharing tiles of 64 keys through a ring of NS slots.
-template <int DP, int QT, bool PAGED>
-__global__ __launch_bounds__(256, QT == 1 ? 2 : 1) void attention_rows(AttentionArgs a) {
-  constexpr int KT = 64, KS = KT / 32, NS = QT == 1 ? 2 : 4, ROWS = 128 * QT;
+// Four waves of 32 rows each, sharing tiles of 64 keys through two slots of LDS; two blocks to a CU, so that a SIMD has
+// one wave's exponentials beside another's products.
+template <int DP, bool PAGED>
+__global__ __launch_bounds__(256, 2) void attention_rows(AttentionArgs a) {
+  constexpr int KT = 64, KS = KT / 32, NS = 2, ROWS = 128;
   using T = TileShape<DP>;
   constexpr int SLOT = 2 * KT * T::PITCH;
   __shared__ __attribute__((aligned(1024))) char smem[NS * SLOT];
   const Place place(a);
-  const RowTile tile = row_tile<QT == 1 ? 7 : 8>(a.seqs, a.group, place.slot);
+  const RowTile tile = row_tile<7>(a.seqs, a.group, place.slot);
   if (!tile.any) return;
   const RowsAt at = rows_at<PAGED>(a, tile);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -341,79 +317,59 @@ __global__ __launch_bounds__(256, QT == 1 ? 2 : 1) void attention_rows(Attention
   }
   // Paged: which keys of a tile hold something (bits of the tiles in flight, the next one to be used last), and this lane's
   // entry of the page table for the tile that is copied next.
-  uint64_t valid[NS];
+  uint64_t valid[NS] = {~0ull, ~0ull};
   int entries = -1;
-#pragma unroll
-  for (int t = 0; t < NS; ++t) valid[t] = ~0ull;
   const auto fetch = [&](int t, int slot) {
     if constexpr (PAGED) {
-#pragma unroll
-      for (int i = NS - 1; i > 0; --i) valid[i] = valid[i - 1];
+      valid[1] = valid[0];
       valid[0] = __ballot(entries >= 0);
     }
     src.copy(t * KT, entries, smem + slot * SLOT, wave);
   };
-#pragma unroll
-  for (int t = 0; t < NS - 1; ++t) {
-    if constexpr (PAGED) entries = src.entry(min(first + t, end - 1) * KT);
-    fetch(min(first + t, end - 1), t);
-  }
-  if constexpr (PAGED) entries = src.entry(min(first + NS - 1, end - 1) * KT);
+  if constexpr (PAGED) entries = src.entry(first * KT);
+  fetch(first, 0);
+  if constexpr (PAGED) entries = src.entry(min(first + 1, end - 1) * KT);
 
-  const int row0 = tile.row + wave * 32 * QT;
+  const int row0 = tile.row + wave * 32;
   const bool mine = row0 < at.rows;
   const float scale2 = a.scale * kLog2e;
-  bf16x8 qf[QT][DP / 16];
-  RowState<DP, QT> st;
+  const int row = min(row0 + (lane & 31), at.rows - 1), sees = at.sees(row, a.group, a.causal);
+  bf16x8 qf[DP / 16];
+  load_operand<DP>(a.q + (at.token + row / a.group) * a.q_stride + static_cast<int64_t>(place.kv * a.group + row % a.group) * a.dim, a.dim, qf);
+  RowState<DP> st;
   st.clear();
-  int sees[QT];
-#pragma unroll
-  for (int c = 0; c < QT; ++c) sees[c] = at.sees(min(row0 + 32 * c + (lane & 31), at.rows - 1), a.group, a.causal);
-  load_rows<DP, QT>(a, at, mine ? row0 : 0, place.kv, qf);
   // of the wave's rows: the fewest and the most keys that one sees
   const int fewest = __builtin_amdgcn_readfirstlane(at.sees(min(row0, at.rows - 1), a.group, a.causal));
-  const int most = mine ? at.sees(min(row0 + 32 * QT, at.rows) - 1, a.group, a.causal) : 0;
-
+  const int most = mine ? at.sees(min(row0 + 32, at.rows) - 1, a.group, a.causal) : 0;
   int slot = 0, left_out = 0x7fffffff;
 #pragma unroll 1
   for (int t = first; t < end; ++t) {
-    // copies of the tiles behind t stay in flight
-    if constexpr (PAGED) dma_wait<0>();
-    else dma_wait<(NS - 2) * 2 * KeySource<DP, KT, 4, PAGED>::C>();
+    dma_wait<0>();
     dma_barrier();
-    // past the end the last tile again, so that the waits count the same
-    fetch(min(t + NS - 1, end - 1), slot == 0 ? NS - 1 : slot - 1);
-    if constexpr (PAGED) entries = src.entry(min(t + NS, end - 1) * KT);
+    if (t + 1 < end) {
+      fetch(t + 1, slot ^ 1);
+      if constexpr (PAGED) entries = src.entry(min(t + 2, end - 1) * KT);
+    } else if constexpr (PAGED) {
+      valid[1] = valid[0];
+    }
     const char* const keys = smem + slot * SLOT;
     const char* const values = keys + KT * T::PITCH;
-    slot = slot + 1 == NS ? 0 : slot + 1;
+    slot ^= 1;
     const int j0 = t * KT;
     if (j0 >= most) continue;
-    f32x16 s[QT][KS];
+    f32x16 s[KS];
 #pragma unroll
     for (int k = 0; k < KS; ++k) {
+      s[k] = MfmaBf16::zero();
 #pragma unroll
-      for (int c = 0; c < QT; ++c) s[c][k] = MfmaBf16::zero();
-#pragma unroll
-      for (int kk = 0; kk < DP / 16; ++kk) {
-        const bf16x8 f = rows_fragment<DP>(keys, 32 * k, kk);
-#pragma unroll
-        for (int c = 0; c < QT; ++c) s[c][k] = MfmaBf16::mma(f, qf[c][kk], s[c][k]);
-      }
+      for (int kk = 0; kk < DP / 16; ++kk) s[k] = MfmaBf16::mma(rows_fragment<DP>(keys, 32 * k, kk), qf[kk], s[k]);
     }
-    const uint64_t there = valid[NS - 1];
-    const bool masked = j0 + KT > fewest || (PAGED && there != ~0ull);
-    if (masked) {
+    const uint64_t there = valid[1];
+    if (j0 + KT > fewest || (PAGED && there != ~0ull)) hide(s, sees - j0, there);
+    st.weigh(s, scale2);
+    bf16x8 w[2 * KS];
 #pragma unroll
-      for (int c = 0; c < QT; ++c) hide(s[c], sees[c] - j0, there);
-    }
-    bf16x8 w[QT][2 * KS];
-#pragma unroll
-    for (int c = 0; c < QT; ++c) {
-      st.weigh(s[c], c, scale2);
-#pragma unroll
-      for (int e = 0; e < 2 * KS; ++e) w[c][e] = weights_fragment(s[c][e / 2], e % 2);
-    }
+    for (int e = 0; e < 2 * KS; ++e) w[e] = weights_fragment(s[e / 2], e % 2);
     // some rows do not see some of these keys
     if (a.causal && j0 + KT > fewest && (j0 >= left_out || any_not_finite<DP>(values, 0, 2 * KS))) {
       left_out = min(left_out, j0);
@@ -422,23 +378,17 @@ __global__ __launch_bounds__(256, QT == 1 ? 2 : 1) void attention_rows(Attention
 #pragma unroll
     for (int e = 0; e < 2 * KS; ++e)
 #pragma unroll
-      for (int d = 0; d < DP / 32; ++d) {
-        const bf16x8 f = cols_fragment<DP>(values, 16 * e, 32 * d);
-#pragma unroll
-        for (int c = 0; c < QT; ++c) st.o[c][d] = MfmaBf16::mma(f, w[c][e], st.o[c][d]);
-      }
+      for (int d = 0; d < DP / 32; ++d) st.o[d] = MfmaBf16::mma(cols_fragment<DP>(values, 16 * e, 32 * d), w[e], st.o[d]);
   }
-  dma_wait<0>();
 #pragma unroll 1
   for (int j = left_out; j < min(most, end * KT); ++j) {
     if (PAGED && static_cast<uint32_t>(src.table[j >> src.shift]) >= static_cast<uint64_t>(a.pages)) continue;
-#pragma unroll
-    for (int c = 0; c < QT; ++c) {
-      const float s = halves_sum(half_dot<DP>(qf[c], src.row(src.k, src.k_row, j), a.dim));
-      if (j < sees[c]) add_row<DP>(st.o[c], __builtin_amdgcn_exp2f(__builtin_fmaf(s, scale2, -(st.m[c] == neg_inf() ? 0.0f : st.m[c]))), src.row(src.v, src.v_row, j), a.dim);
-    }
+    const float s = halves_sum(half_dot<DP>(qf, src.row(src.k, src.k_row, j), a.dim));
+    if (j >= sees) continue;
+    const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s, scale2, -(st.m == neg_inf() ? 0.0f : st.m)));
+    add_row<DP>(st.o, w, src.row(src.v, src.v_row, j), a.dim);
   }
-  if (mine) store_rows(a, st, at, row0, place.kv, place.split);
+  if (mine) store_rows<DP>(a, st, at, row0, place.kv, place.split);
 }
 
 // Joins the splits: with M = max m, out = sum 2^(m - M) o / sum 2^(m - M) l.  32 lanes a row.
@@ -495,19 +445,14 @@ __global__ __launch_bounds__(256) void cache_append_rows(AttentionArgs a, uint16
 bool float_type(int32_t t) { return t == VDSL_F32 || t == VDSL_BF16; }
 
 template <bool PAGED>
-int launch_rows(vdsl_queue q, AttentionArgs& a, int qt) {
-  const int log_tile = qt == 1 ? 7 : 8;
-  const int64_t slots = row_slots(a.seqs.n, a.seqs.seqs, a.group, log_tile);
+int launch_rows(vdsl_queue q, AttentionArgs& a) {
+  const int64_t slots = row_slots(a.seqs.n, a.seqs.seqs, a.group, 7);
   const int64_t blocks = slots * a.kv_heads * a.splits;
   if (slots > 0x7fffffff || blocks > 0x7fffff) return fail(VDSL_ERR_UNSUPPORTED, "attention: too many rows");
   a.blocks = static_cast<int>(slots);
-  const auto go = [&](auto kernel, const char* name) {
-    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, q->stream, a);
-    return check_launch(name);
-  };
-  if (a.dim <= 64) return go(qt == 1 ? attention_rows<64, 1, PAGED> : attention_rows<64, 2, PAGED>, "attention_rows");
-  if (a.dim <= 96) return go(qt == 1 ? attention_rows<96, 1, PAGED> : attention_rows<96, 2, PAGED>, "attention_rows");
-  return go(qt == 1 ? attention_rows<128, 1, PAGED> : attention_rows<128, 2, PAGED>, "attention_rows");
+  const auto kernel = a.dim <= 64 ? attention_rows<64, PAGED> : a.dim <= 96 ? attention_rows<96, PAGED> : attention_rows<128, PAGED>;
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, q->stream, a);
+  return check_launch("attention_rows");
 }
 
 }  // namespace
@@ -522,8 +467,8 @@ int attention_check_shape(const char* op, int64_t n, int64_t seqs, int32_t heads
   return VDSL_OK;
 }
 int attention_check_scale(const char* op, float scale) {
-  if (!(scale > 0.0f) || !std::isnormal(scale) || !std::isfinite(scale * kLog2e))
-    return fail(VDSL_ERR_INVALID_ARG, std::string(op) + ": scale must be a positive normal number");
+  if (!(scale >= 0x1p-100f && scale <= 0x1p100f))
+    return fail(VDSL_ERR_INVALID_ARG, std::string(op) + ": scale must be between 2^-100 and 2^100");
   return VDSL_OK;
 }
 // The bytes of a buffer that holds n rows of `heads` heads laid out as h says, and whether h can be used.
@@ -582,21 +527,18 @@ extern "C" int vdsl_op_attention_fwd(vdsl_queue q, const vdsl_attention_params* 
   a.causal = p->causal != 0;
   a.scale = p->scale;
   a.splits = 1;
-  const int64_t rows = p->n * a.group * a.kv_heads;
-  return launch_rows<false>(q, a, rows >= 256 * 256 ? 2 : 1);
+  return launch_rows<false>(q, a);
 }
 
 namespace vdsl {
 namespace {
-struct PagedPlan {
-  int qt, splits;
-};
-PagedPlan paged_plan(int64_t n, int64_t seqs, int32_t heads, int32_t kv_heads, int64_t positions) {
+// Splits of the keys: as many as make two blocks a CU, of 256 positions at least.
+int paged_splits(int64_t n, int64_t seqs, int32_t heads, int32_t kv_heads, int64_t positions) {
   const int64_t group = heads / kv_heads;
   const int64_t blocks = std::max<int64_t>(1, (n * group / 128 + std::min(seqs, n)) * kv_heads);
-  PagedPlan plan = {1, 1};
-  while (blocks * plan.splits < 512 && plan.splits < 32 && positions > 256 * plan.splits) plan.splits *= 2;
-  return plan;
+  int splits = 1;
+  while (blocks * splits < 512 && splits < 32 && positions > 256 * splits) splits *= 2;
+  return splits;
 }
 int paged_check(const char* op, const vdsl_paged_params* p) {
   if (!p) return fail(VDSL_ERR_INVALID_ARG, "params is null");
@@ -662,7 +604,7 @@ extern "C" int vdsl_paged_attention_workspace_bytes(int64_t n, int64_t seqs, int
   if (!bytes) return fail(VDSL_ERR_INVALID_ARG, "bytes is null");
   VDSL_TRY(attention_check_shape("paged_attention", n, seqs, heads, kv_heads, dim));
   if (positions < 0) return fail(VDSL_ERR_INVALID_ARG, "negative shape");
-  const int splits = paged_plan(n, seqs, heads, kv_heads, positions).splits;
+  const int splits = paged_splits(n, seqs, heads, kv_heads, positions);
   *bytes = splits == 1 ? 0 : nbytes(n * heads, splits, 8 + 4 * static_cast<int64_t>(dim));
   return VDSL_OK;
 }
@@ -698,14 +640,13 @@ extern "C" int vdsl_op_paged_attention(vdsl_queue q, const vdsl_paged_params* p,
   a.out = out->ptr;
   a.out_dtype = out_dtype;
   a.lse = lse ? static_cast<float*>(lse->ptr) : nullptr;
-  const PagedPlan plan = paged_plan(p->n, p->seqs, p->heads, p->kv_heads, positions);
-  a.splits = plan.splits;
-  if (plan.splits > 1) {
+  a.splits = paged_splits(p->n, p->seqs, p->heads, p->kv_heads, positions);
+  if (a.splits > 1) {
     a.parts = static_cast<float*>(workspace->ptr);
-    a.stats = reinterpret_cast<float2*>(a.parts + static_cast<int64_t>(plan.splits) * p->n * p->heads * p->dim);
+    a.stats = reinterpret_cast<float2*>(a.parts + static_cast<int64_t>(a.splits) * p->n * p->heads * p->dim);
   }
-  VDSL_TRY(launch_rows<true>(q, a, plan.qt));
-  if (plan.splits == 1) return VDSL_OK;
+  VDSL_TRY(launch_rows<true>(q, a));
+  if (a.splits == 1) return VDSL_OK;
   hipLaunchKernelGGL(attention_join, block_grid((p->n * p->heads + 7) / 8), dim3(256), 0, q->stream, a);
   return check_launch("attention_join");
 }

@@ -22,7 +22,7 @@ struct GradArgs {
   const uint16_t *q, *k, *v, *dout;  // dout: bf16
   int64_t q_stride, k_stride, v_stride, dout_stride;
   Sequences seqs;
-  const float2* rows;  // lse log2 e and delta, [kv_heads][n * group]
+  const float* rows;  // -lse / scale, then -delta, each [kv_heads][n * group]
   void *dq, *dk, *dv;
   int64_t dq_first, dq_stride, dk_first, dk_stride, dv_first, dv_stride;
   int heads, kv_heads, group, dim, causal, grad_dtype;
@@ -31,10 +31,10 @@ struct GradArgs {
   int blocks;
 };
 
-// Rows' lse and delta, and dout in bf16 where it is f32.  32 lanes a row.
+// What a row's scores and dp start from, -lse / scale and -delta, and dout in bf16 where it is f32.  32 lanes a row.
 __global__ __launch_bounds__(256) void attention_bwd_rows(const void* __restrict__ dout, int dout_dtype, const void* __restrict__ out,
                                                           int out_dtype, const float* __restrict__ lse, int64_t n, int heads, int group,
-                                                          int dim, uint16_t* __restrict__ copy, float2* __restrict__ rows) {
+                                                          int dim, float scale, uint16_t* __restrict__ copy, float* __restrict__ rows) {
   const int64_t r = block_index() * 8 + (threadIdx.x >> 5);
   if (r >= n * heads) return;
   const int64_t token = r / heads;
@@ -56,22 +56,11 @@ __global__ __launch_bounds__(256) void attention_bwd_rows(const void* __restrict
   for (int m = 16; m >= 1; m >>= 1) sum += __shfl_xor(sum, m, 64);
   if (col != 0) return;
   const float l = lse[head * n + token];
-  const float2 v = make_float2(l == neg_inf() ? __builtin_inff() : l * kLog2e, sum);  // no score of such a row has a weight
-  rows[static_cast<int64_t>(head / group) * n * group + token * group + head % group] = v;
+  float* const to = rows + static_cast<int64_t>(head / group) * n * group + token * group + head % group;
+  *to = l == neg_inf() ? neg_inf() : -l / scale;  // no score of such a row has a weight
+  to[n * heads] = -sum;
 }
 
-// 32 rows of this lane's wave as an operand (element j of lane l: column 16 kk + 8 (l / 32) + j of row l % 32), from
-// the lane's own row at p.
-template <int DP>
-__device__ __forceinline__ void load_operand(const uint16_t* p, int dim, bf16x8 (&f)[DP / 16]) {
-#pragma unroll
-  for (int kk = 0; kk < DP / 16; ++kk) {
-    const int col = 16 * kk + 8 * ((threadIdx.x & 63) >> 5);
-    u32x4 w = {0u, 0u, 0u, 0u};
-    if (col < dim) w = *reinterpret_cast<const u32x4*>(p + col);
-    f[kk] = __builtin_bit_cast(bf16x8, w);
-  }
-}
 // acc (columns x rows: this lane has columns 32 d + 8 g + 4 (l / 32) + j of its own row) times `by` to element e of `to`.
 template <int DP>
 __device__ __forceinline__ void store_gradient(const f32x16 (&acc)[DP / 32], float by, int dtype, void* to, int64_t e, int dim) {
@@ -92,11 +81,11 @@ __device__ __forceinline__ void store_zeros(int dtype, void* to, int64_t e, int 
   for (int c = 0; c < cols; c += 4) store_unit<4>(dtype, to, e + c, none);
 }
 
-// Tiles of TR rows of two operands for copies of four waves.
-template <int DP, int TR>
+// Tiles of TR rows of two operands for copies of NW waves.
+template <int DP, int TR, int NW>
 struct PairCopies {
   using T = TileShape<DP>;
-  static constexpr int C = TR * T::PITCH / 1024 / 4, SLOT = 2 * TR * T::PITCH;
+  static constexpr int C = TR * T::PITCH / 1024 / NW, SLOT = 2 * TR * T::PITCH;
   int row_of[C], chunk[C];
   __device__ __forceinline__ PairCopies(int wave) {
     const int lane = threadIdx.x & 63;
@@ -109,16 +98,25 @@ struct PairCopies {
   // Rows 0 .. last of a tile; those behind are zeros.  at(row of the tile, which operand): that row's first byte.
   template <class At>
   __device__ __forceinline__ void operator()(char* to, int wave, int dim, int last, At&& at) const {
+    if (last >= TR - 1) {
 #pragma unroll
+      for (int u = 0; u < C; ++u) {
+        if (chunk[u] >= dim / 8) continue;
+        lds_copy16(at(row_of[u], 0) + 16 * chunk[u], to + (wave * C + u) * 1024);
+        lds_copy16(at(row_of[u], 1) + 16 * chunk[u], to + TR * T::PITCH + (wave * C + u) * 1024);
+      }
+      return;
+    }
+#pragma unroll 1
     for (int u = 0; u < C; ++u) {
-      if (chunk[u] >= dim / 8) continue;
+      const int lane = threadIdx.x & 63, row = (wave * C + u) * (64 / T::CPR) + lane / T::CPR, c = lane % T::CPR ^ T::swz(row);
+      if (c >= dim / 8) continue;
       char* const first = to + (wave * C + u) * 1024;
       char* const second = first + TR * T::PITCH;
-      if (last >= TR - 1 || row_of[u] <= last) {
-        lds_copy16(at(row_of[u], 0) + 16 * chunk[u], first);
-        lds_copy16(at(row_of[u], 1) + 16 * chunk[u], second);
+      if (row <= last) {
+        lds_copy16(at(row, 0) + 16 * c, first);
+        lds_copy16(at(row, 1) + 16 * c, second);
       } else {
-        const int lane = threadIdx.x & 63;
         *reinterpret_cast<u32x4*>(first + 16 * lane) = u32x4{0u, 0u, 0u, 0u};
         *reinterpret_cast<u32x4*>(second + 16 * lane) = u32x4{0u, 0u, 0u, 0u};
       }
@@ -126,17 +124,17 @@ struct PairCopies {
   }
 };
 
-// dk and dv: four waves of 32 keys each, walking over tiles of 64 rows.
-template <int DP>
-__global__ __launch_bounds__(256, 1) void attention_bwd_keys(GradArgs a) {
-  constexpr int TR = 64, NS = 4;
+// dk and dv: eight waves of 32 keys each, walking over tiles of 64 rows.
+template <int DP, int NW>
+__global__ __launch_bounds__(64 * NW, NW / 4) void attention_bwd_keys(GradArgs a) {
+  constexpr int TR = 64;
   using T = TileShape<DP>;
-  using Copies = PairCopies<DP, TR>;
-  __shared__ __attribute__((aligned(1024))) char smem[NS * Copies::SLOT];
-  __shared__ float2 stat[NS][TR];
+  using Copies = PairCopies<DP, TR, NW>;
+  __shared__ __attribute__((aligned(1024))) char smem[2 * Copies::SLOT];
+  __shared__ __attribute__((aligned(16))) float start[2][2][TR];  // what the rows' scores and dp start from
   int b = static_cast<int>(blockIdx.x);
   const int kv = b % a.kv_heads;
-  const RowTile tile = row_tile<7>(a.seqs, 1, b / a.kv_heads);
+  const RowTile tile = row_tile<NW == 4 ? 7 : 8>(a.seqs, 1, b / a.kv_heads);
   if (!tile.any) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
   const int key = tile.row + 32 * wave + (lane & 31);
@@ -150,7 +148,7 @@ __global__ __launch_bounds__(256, 1) void attention_bwd_keys(GradArgs a) {
   }
   const Copies copies(wave);
   if (2 * a.dim < T::PITCH) {
-    for (int i = threadIdx.x; i < NS * Copies::SLOT / 16; i += 256) reinterpret_cast<u32x4*>(smem)[i] = u32x4{0u, 0u, 0u, 0u};
+    for (int i = threadIdx.x; i < 2 * Copies::SLOT / 16; i += 64 * NW) reinterpret_cast<u32x4*>(smem)[i] = u32x4{0u, 0u, 0u, 0u};
     __syncthreads();
   }
   const int64_t token = tile.token + min(key, tile.len - 1);
@@ -161,8 +159,12 @@ __global__ __launch_bounds__(256, 1) void attention_bwd_keys(GradArgs a) {
   const int first = a.causal ? tile.row * a.group / TR : 0, end = (rows + TR - 1) / TR;
   const char* const qp = reinterpret_cast<const char*>(a.q + tile.token * a.q_stride + head_col * a.group);
   const char* const dp = reinterpret_cast<const char*>(a.dout + tile.token * a.dout_stride + head_col * a.group);
-  const float2* const sp = a.rows + (static_cast<int64_t>(kv) * a.seqs.n + tile.token) * a.group;
-  float2 next;
+  const float* const sp = a.rows + (static_cast<int64_t>(kv) * a.seqs.n + tile.token) * a.group;
+  const int64_t delta_at = a.seqs.n * a.heads;
+  const auto start_of = [&](int t) {  // of the lane's row and which of the two
+    return sp[(threadIdx.x / TR) * delta_at + min(t * TR + static_cast<int>(threadIdx.x % TR), rows - 1)];
+  };
+  float next = 0.0f;
   const auto fetch = [&](int t, int slot) {
     copies(smem + slot * Copies::SLOT, wave, a.dim, rows - 1 - t * TR, [&](int r, int which) {
       const int row = t * TR + r, i = a.token_of(row);
@@ -170,11 +172,8 @@ __global__ __launch_bounds__(256, 1) void attention_bwd_keys(GradArgs a) {
       return which == 0 ? qp + 2 * (i * a.q_stride + col) : dp + 2 * (i * a.dout_stride + col);
     });
   };
-#pragma unroll
-  for (int t = 0; t < NS - 1; ++t) {
-    fetch(min(first + t, end - 1), t);
-    if (threadIdx.x < TR) stat[t][threadIdx.x] = sp[min(min(first + t, end - 1) * TR + static_cast<int>(threadIdx.x), rows - 1)];
-  }
+  fetch(first, 0);
+  if (threadIdx.x < 2 * TR) start[0][threadIdx.x / TR][threadIdx.x % TR] = start_of(first);
   f32x16 dk[DP / 32], dv[DP / 32];
 #pragma unroll
   for (int d = 0; d < DP / 32; ++d) dk[d] = dv[d] = MfmaBf16::zero();
@@ -184,20 +183,29 @@ __global__ __launch_bounds__(256, 1) void attention_bwd_keys(GradArgs a) {
   int slot = 0, left_out = 0x7fffffff;
 #pragma unroll 1
   for (int t = first; t < end; ++t) {
-    const int ahead = min(t + NS - 1, end - 1), to = slot == 0 ? NS - 1 : slot - 1;
     dma_wait<0>();
     __syncthreads();
-    if (threadIdx.x < TR) next = sp[min(ahead * TR + static_cast<int>(threadIdx.x), rows - 1)];
-    fetch(ahead, to);
+    if (t + 1 < end) {
+      if (threadIdx.x < 2 * TR) next = start_of(t + 1);
+      fetch(t + 1, slot ^ 1);
+    }
     const char* const qs = smem + slot * Copies::SLOT;
     const char* const ds = qs + TR * T::PITCH;
-    const float2* const stats = stat[slot];
-    slot = slot + 1 == NS ? 0 : slot + 1;
     if ((t + 1) * TR > wave_first) {
 #pragma unroll 1
       for (int u = 0; u < TR / 32; ++u) {
         const int r0 = t * TR + 32 * u;
-        f32x16 s = MfmaBf16::zero(), p = MfmaBf16::zero();
+        f32x16 s, p;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const f32x4 x = *reinterpret_cast<const f32x4*>(&start[slot][0][32 * u + 8 * g + 4 * half]);
+          const f32x4 y = *reinterpret_cast<const f32x4*>(&start[slot][1][32 * u + 8 * g + 4 * half]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            s[4 * g + j] = x[j];
+            p[4 * g + j] = y[j];
+          }
+        }
 #pragma unroll
         for (int kk = 0; kk < DP / 16; ++kk) {
           s = MfmaBf16::mma(rows_fragment<DP>(qs, 32 * u, kk), kf[kk], s);
@@ -206,16 +214,17 @@ __global__ __launch_bounds__(256, 1) void attention_bwd_keys(GradArgs a) {
         const bool masked = r0 < wave_all || r0 + 32 > rows;
         const int lo = sees_from - r0, hi = rows - r0;
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
+        for (int i = 0; i < 16; ++i) {
+          s[i] = __builtin_amdgcn_exp2f(s[i] * scale2);
+          p[i] *= s[i];
+        }
+        if (masked) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int r = 8 * g + 4 * half + j;
-            const float2 st = stats[32 * u + r];
-            float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * g + j], scale2, -st.x));
-            float d = w * (p[4 * g + j] - st.y);
-            if (masked && !(r >= lo && r < hi)) w = d = 0.0f;
-            s[4 * g + j] = w;
-            p[4 * g + j] = d;
+          for (int i = 0; i < 16; ++i) {
+            const int r = 8 * (i / 4) + 4 * half + i % 4;
+            const bool in = r >= lo && r < hi;
+            s[i] = in ? s[i] : 0.0f;
+            p[i] = in ? p[i] : 0.0f;
           }
         }
         const bf16x8 w[2] = {weights_fragment(s, 0), weights_fragment(s, 1)}, d[2] = {weights_fragment(p, 0), weights_fragment(p, 1)};
@@ -233,9 +242,9 @@ __global__ __launch_bounds__(256, 1) void attention_bwd_keys(GradArgs a) {
           }
       }
     }
-    if (threadIdx.x < TR) stat[to][threadIdx.x] = next;
+    slot ^= 1;
+    if (t + 1 < end && threadIdx.x < 2 * TR) start[slot][threadIdx.x / TR][threadIdx.x % TR] = next;
   }
-  dma_wait<0>();
 #pragma unroll 1
   for (int r = left_out; r < min((wave_all + 31) & ~31, rows); ++r) {
     const int i = a.token_of(r);
@@ -244,9 +253,9 @@ __global__ __launch_bounds__(256, 1) void attention_bwd_keys(GradArgs a) {
     const uint16_t* const dr = reinterpret_cast<const uint16_t*>(dp) + i * a.dout_stride + col;
     const float s = halves_sum(half_dot<DP>(kf, qr, a.dim)), p = halves_sum(half_dot<DP>(vf, dr, a.dim));
     if (r < sees_from) continue;
-    const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s, scale2, -sp[r].x));
+    const float w = __builtin_amdgcn_exp2f((s + sp[r]) * scale2);
     add_row<DP>(dv, w, dr, a.dim);
-    add_row<DP>(dk, w * (p - sp[r].y), qr, a.dim);
+    add_row<DP>(dk, w * (p + sp[delta_at + r]), qr, a.dim);
   }
   if (key < tile.len) {
     store_gradient<DP>(dk, a.scale, a.grad_dtype, a.dk, a.dk_first + token * a.dk_stride + head_col, a.dim);
@@ -254,19 +263,19 @@ __global__ __launch_bounds__(256, 1) void attention_bwd_keys(GradArgs a) {
   }
 }
 
-// dq: four waves of QT x 32 rows each, walking over tiles of 64 keys.
-template <int DP, int QT>
-__global__ __launch_bounds__(256, QT == 1 ? 2 : 1) void attention_bwd_queries(GradArgs a) {
-  constexpr int KT = 64, NS = QT == 1 ? 2 : 4, ROWS = 128 * QT;
+// dq: four waves of 32 rows each, walking over tiles of 64 keys.
+template <int DP>
+__global__ __launch_bounds__(256, 2) void attention_bwd_queries(GradArgs a) {
+  constexpr int KT = 64, ROWS = 128;
   using T = TileShape<DP>;
-  using Copies = PairCopies<DP, KT>;
-  __shared__ __attribute__((aligned(1024))) char smem[NS * Copies::SLOT];
+  using Copies = PairCopies<DP, KT, 4>;
+  __shared__ __attribute__((aligned(1024))) char smem[2 * Copies::SLOT];
   int b = static_cast<int>(blockIdx.x);
   const int kv = b % a.kv_heads;
-  const RowTile tile = row_tile<QT == 1 ? 7 : 8>(a.seqs, a.group, a.blocks - 1 - b / a.kv_heads);
+  const RowTile tile = row_tile<7>(a.seqs, a.group, a.blocks - 1 - b / a.kv_heads);
   if (!tile.any) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int rows = tile.len * a.group, row0 = tile.row + 32 * QT * wave;
+  const int rows = tile.len * a.group, row0 = tile.row + 32 * wave;
   const int64_t head_col = static_cast<int64_t>(kv) * a.dim;
   const auto dq_at = [&](int row) {
     const int i = a.token_of(row);
@@ -279,7 +288,7 @@ __global__ __launch_bounds__(256, QT == 1 ? 2 : 1) void attention_bwd_queries(Gr
   }
   const Copies copies(wave);
   if (2 * a.dim < T::PITCH) {
-    for (int i = threadIdx.x; i < NS * Copies::SLOT / 16; i += 256) reinterpret_cast<u32x4*>(smem)[i] = u32x4{0u, 0u, 0u, 0u};
+    for (int i = threadIdx.x; i < 2 * Copies::SLOT / 16; i += 256) reinterpret_cast<u32x4*>(smem)[i] = u32x4{0u, 0u, 0u, 0u};
     __syncthreads();
   }
   const auto sees = [&](int row) { return a.causal ? a.token_of(row) + 1 : tile.len; };
@@ -292,64 +301,49 @@ __global__ __launch_bounds__(256, QT == 1 ? 2 : 1) void attention_bwd_queries(Gr
       return which == 0 ? kp + 2 * i * a.k_stride : vp + 2 * i * a.v_stride;
     });
   };
-#pragma unroll
-  for (int t = 0; t < NS - 1; ++t) fetch(min(t, end - 1), t);
-  bf16x8 qf[QT][DP / 16], df[QT][DP / 16];
-  float2 st[QT];
-  int seen[QT];
-  f32x16 dq[QT][DP / 32];
-#pragma unroll
-  for (int c = 0; c < QT; ++c) {
-    const int row = min(row0 + 32 * c + (lane & 31), rows - 1), i = a.token_of(row);
-    const int64_t col = head_col * a.group + static_cast<int64_t>(row - i * a.group) * a.dim;
-    load_operand<DP>(a.q + (tile.token + i) * a.q_stride + col, a.dim, qf[c]);
-    load_operand<DP>(a.dout + (tile.token + i) * a.dout_stride + col, a.dim, df[c]);
-    st[c] = a.rows[(static_cast<int64_t>(kv) * a.seqs.n + tile.token) * a.group + row];
-    seen[c] = sees(row);
-#pragma unroll
-    for (int d = 0; d < DP / 32; ++d) dq[c][d] = MfmaBf16::zero();
-  }
-  const float scale2 = a.scale * kLog2e;
+  fetch(0, 0);
   const bool mine = row0 < rows;
-  const int fewest = sees(min(row0, rows - 1)), most = mine ? sees(min(row0 + 32 * QT, rows) - 1) : 0;
+  const int row = min(row0 + (lane & 31), rows - 1), seen = sees(row);
+  bf16x8 qf[DP / 16], df[DP / 16];
+  {
+    const int i = a.token_of(row);
+    const int64_t col = head_col * a.group + static_cast<int64_t>(row - i * a.group) * a.dim;
+    load_operand<DP>(a.q + (tile.token + i) * a.q_stride + col, a.dim, qf);
+    load_operand<DP>(a.dout + (tile.token + i) * a.dout_stride + col, a.dim, df);
+  }
+  const float* const start = a.rows + (static_cast<int64_t>(kv) * a.seqs.n + tile.token) * a.group + row;
+  const float score0 = *start, dp0 = start[a.seqs.n * a.heads];
+  f32x16 dq[DP / 32];
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d) dq[d] = MfmaBf16::zero();
+  const float scale2 = a.scale * kLog2e;
+  const int fewest = sees(min(row0, rows - 1)), most = mine ? sees(min(row0 + 32, rows) - 1) : 0;
   int slot = 0, left_out = 0x7fffffff;
 #pragma unroll 1
   for (int t = 0; t < end; ++t) {
-    dma_wait<(NS - 2) * 2 * Copies::C>();
+    dma_wait<0>();
     dma_barrier();
-    fetch(min(t + NS - 1, end - 1), slot == 0 ? NS - 1 : slot - 1);
+    if (t + 1 < end) fetch(t + 1, slot ^ 1);
     const char* const ks = smem + slot * Copies::SLOT;
     const char* const vs = ks + KT * T::PITCH;
-    slot = slot + 1 == NS ? 0 : slot + 1;
+    slot ^= 1;
 #pragma unroll 1
     for (int u = 0; u < KT / 32; ++u) {
       const int j0 = t * KT + 32 * u;
       if (j0 >= most) break;
-      f32x16 s[QT], p[QT];
-#pragma unroll
-      for (int c = 0; c < QT; ++c) s[c] = p[c] = MfmaBf16::zero();
+      f32x16 s = MfmaBf16::zero(), p = MfmaBf16::zero();
 #pragma unroll
       for (int kk = 0; kk < DP / 16; ++kk) {
-        const bf16x8 kf = rows_fragment<DP>(ks, 32 * u, kk), vf = rows_fragment<DP>(vs, 32 * u, kk);
-#pragma unroll
-        for (int c = 0; c < QT; ++c) {
-          s[c] = MfmaBf16::mma(kf, qf[c][kk], s[c]);
-          p[c] = MfmaBf16::mma(vf, df[c][kk], p[c]);
-        }
+        s = MfmaBf16::mma(rows_fragment<DP>(ks, 32 * u, kk), qf[kk], s);
+        p = MfmaBf16::mma(rows_fragment<DP>(vs, 32 * u, kk), df[kk], p);
       }
       const bool masked = j0 + 32 > fewest;
-      bf16x8 w[QT][2];
+      const int hi = seen - j0 - 4 * (lane >> 5);
 #pragma unroll
-      for (int c = 0; c < QT; ++c) {
-        const int hi = seen[c] - j0 - 4 * (lane >> 5);
+      for (int r = 0; r < 16; ++r) p[r] = __builtin_amdgcn_exp2f((s[r] + score0) * scale2) * (p[r] + dp0);
+      if (masked) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[c][r], scale2, -st[c].x));
-          p[c][r] = e * (p[c][r] - st[c].y);
-          if (masked && !(8 * (r / 4) + r % 4 < hi)) p[c][r] = 0.0f;
-        }
-        w[c][0] = weights_fragment(p[c], 0);
-        w[c][1] = weights_fragment(p[c], 1);
+        for (int r = 0; r < 16; ++r) p[r] = 8 * (r / 4) + r % 4 < hi ? p[r] : 0.0f;
       }
       // some rows do not see some of these keys
       if (a.causal && masked && (j0 >= left_out || any_not_finite<DP>(ks, 32 * u, 2))) {
@@ -357,32 +351,22 @@ __global__ __launch_bounds__(256, QT == 1 ? 2 : 1) void attention_bwd_queries(Gr
         continue;
       }
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
+      for (int e = 0; e < 2; ++e) {
+        const bf16x8 w = weights_fragment(p, e);
 #pragma unroll
-        for (int d = 0; d < DP / 32; ++d) {
-          const bf16x8 f = cols_fragment<DP>(ks, 32 * u + 16 * e, 32 * d);
-#pragma unroll
-          for (int c = 0; c < QT; ++c) dq[c][d] = MfmaBf16::mma(f, w[c][e], dq[c][d]);
-        }
+        for (int d = 0; d < DP / 32; ++d) dq[d] = MfmaBf16::mma(cols_fragment<DP>(ks, 32 * u + 16 * e, 32 * d), w, dq[d]);
+      }
     }
   }
-  dma_wait<0>();
 #pragma unroll 1
   for (int j = left_out; j < most; ++j) {
     const uint16_t* const kr = reinterpret_cast<const uint16_t*>(kp) + j * a.k_stride;
     const uint16_t* const vr = reinterpret_cast<const uint16_t*>(vp) + j * a.v_stride;
-#pragma unroll
-    for (int c = 0; c < QT; ++c) {
-      const float s = halves_sum(half_dot<DP>(qf[c], kr, a.dim)), p = halves_sum(half_dot<DP>(df[c], vr, a.dim));
-      if (j >= seen[c]) continue;
-      add_row<DP>(dq[c], __builtin_amdgcn_exp2f(__builtin_fmaf(s, scale2, -st[c].x)) * (p - st[c].y), kr, a.dim);
-    }
+    const float s = halves_sum(half_dot<DP>(qf, kr, a.dim)), p = halves_sum(half_dot<DP>(df, vr, a.dim));
+    if (j >= seen) continue;
+    add_row<DP>(dq, __builtin_amdgcn_exp2f((s + score0) * scale2) * (p + dp0), kr, a.dim);
   }
-#pragma unroll
-  for (int c = 0; c < QT; ++c) {
-    const int row = row0 + 32 * c + (lane & 31);
-    if (row < rows) store_gradient<DP>(dq[c], a.scale, a.grad_dtype, a.dq, dq_at(row), a.dim);
-  }
+  if (row0 + (lane & 31) < rows) store_gradient<DP>(dq, a.scale, a.grad_dtype, a.dq, dq_at(row), a.dim);
 }
 
 bool float_type(int32_t t) { return t == VDSL_F32 || t == VDSL_BF16; }
@@ -399,7 +383,7 @@ bool apart(const vdsl_heads& x, int64_t x_width, const vdsl_heads& y, int64_t y_
 
 using namespace vdsl;
 
-// The rows' lse and delta, then a copy of dout in bf16.
+// What the rows' scores and dp start from, then a copy of dout in bf16.
 extern "C" int vdsl_attention_bwd_workspace_bytes(int64_t n, int64_t seqs, int32_t heads, int32_t kv_heads, int32_t dim, size_t* bytes) {
   if (!bytes) return fail(VDSL_ERR_INVALID_ARG, "bytes is null");
   VDSL_TRY(attention_check_shape("attention_bwd", n, seqs, heads, kv_heads, dim));
@@ -445,8 +429,8 @@ extern "C" int vdsl_op_attention_bwd(vdsl_queue q, const vdsl_attention_params* 
     return fail(VDSL_ERR_INVALID_ARG, "attention_bwd: gradients in one buffer must be disjoint columns of one stride");
   if (p->n == 0) return VDSL_OK;
   const int group = p->heads / p->kv_heads;
-  float2* const rows = static_cast<float2*>(workspace->ptr);
-  uint16_t* const copy = dout_dtype == VDSL_F32 ? reinterpret_cast<uint16_t*>(rows + p->n * p->heads) : nullptr;
+  float* const rows = static_cast<float*>(workspace->ptr);
+  uint16_t* const copy = dout_dtype == VDSL_F32 ? reinterpret_cast<uint16_t*>(rows + 2 * p->n * p->heads) : nullptr;
   GradArgs a = {};
   a.q = static_cast<const uint16_t*>(qs->ptr) + p->q.first;
   a.k = static_cast<const uint16_t*>(ks->ptr) + p->k.first;
@@ -476,26 +460,18 @@ extern "C" int vdsl_op_attention_bwd(vdsl_queue q, const vdsl_attention_params* 
   a.scale = p->scale;
   a.token_of = divider(group);
   hipLaunchKernelGGL(attention_bwd_rows, block_grid((p->n * p->heads + 7) / 8), dim3(256), 0, q->stream, dout->ptr, dout_dtype,
-                     out->ptr, out_dtype, static_cast<const float*>(lse->ptr), p->n, p->heads, group, p->dim, copy, rows);
+                     out->ptr, out_dtype, static_cast<const float*>(lse->ptr), p->n, p->heads, group, p->dim, p->scale, copy, rows);
   VDSL_TRY(check_launch("attention_bwd_rows"));
-  const int64_t key_slots = row_slots(p->n, p->seqs, 1, 7);
-  const int qt = p->dim <= 64 && p->n * p->heads >= 256 * 256 ? 2 : 1;
-  const int64_t row_slots_ = row_slots(p->n, p->seqs, group, qt == 1 ? 7 : 8);
-  if (std::max(key_slots, row_slots_) * p->kv_heads > 0x7fffff) return fail(VDSL_ERR_UNSUPPORTED, "attention_bwd: too many rows");
-  const auto go = [&](auto kernel, int64_t slots, const char* name) {
+  const int64_t key_slots = row_slots(p->n, p->seqs, 1, p->dim <= 96 ? 8 : 7);
+  const int64_t query_slots = row_slots(p->n, p->seqs, group, 7);
+  if (std::max(key_slots, query_slots) * p->kv_heads > 0x7fffff) return fail(VDSL_ERR_UNSUPPORTED, "attention_bwd: too many rows");
+  const auto go = [&](auto kernel, unsigned lanes, int64_t slots, const char* name) {
     a.blocks = static_cast<int>(slots);
-    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(slots * p->kv_heads)), dim3(256), 0, q->stream, a);
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(slots * p->kv_heads)), dim3(lanes), 0, q->stream, a);
     return check_launch(name);
   };
-  const char *const keys = "attention_bwd_keys", *const queries = "attention_bwd_queries";
-  if (p->dim <= 64) {
-    VDSL_TRY(go(attention_bwd_keys<64>, key_slots, keys));
-    return go(qt == 1 ? attention_bwd_queries<64, 1> : attention_bwd_queries<64, 2>, row_slots_, queries);
-  }
-  if (p->dim <= 96) {
-    VDSL_TRY(go(attention_bwd_keys<96>, key_slots, keys));
-    return go(attention_bwd_queries<96, 1>, row_slots_, queries);
-  }
-  VDSL_TRY(go(attention_bwd_keys<128>, key_slots, keys));
-  return go(attention_bwd_queries<128, 1>, row_slots_, queries);
+  const auto keys = p->dim <= 64 ? attention_bwd_keys<64, 8> : p->dim <= 96 ? attention_bwd_keys<96, 8> : attention_bwd_keys<128, 4>;
+  const auto queries = p->dim <= 64 ? attention_bwd_queries<64> : p->dim <= 96 ? attention_bwd_queries<96> : attention_bwd_queries<128>;
+  VDSL_TRY(go(keys, p->dim <= 96 ? 512 : 256, key_slots, "attention_bwd_keys"));
+  return go(queries, 256, query_slots, "attention_bwd_queries");
 }

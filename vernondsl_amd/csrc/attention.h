@@ -145,31 +145,32 @@ __device__ __forceinline__ bf16x8 weights_fragment(const f32x16& s, int e) {
   return __builtin_bit_cast(bf16x8, w);
 }
 
-// Sets a bit of each of x's eight elements that is no finite number (bit 15 of its half word).
-__device__ __forceinline__ uint32_t not_finite(const bf16x8& x) {
-  const u32x4 w = __builtin_bit_cast(u32x4, x);
-  uint32_t f = 0;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) f |= (w[j] & 0x7F807F80u) + 0x00800080u;
-  return f & 0x80008000u;
-}
-
 // What a row does not see has weight 0, and 0 times NaN or infinity would spoil it in the products.  Keys (rows) that are
 // not there are zeros in LDS; those of the sequence that only some rows of a tile see are looked through, and from the
 // first tile that holds an element that is no finite number on, such tiles are left out and added at the end key by
 // key, each lane taking what it sees: by half_dot and add_row.
-// Whether a tile's rows row0 .. + 16 steps - 1 hold an element that is no finite number.
+// Whether a tile's rows 0 .. 16 steps - 1 hold an element that is no finite number.
 template <int DP>
-__device__ __forceinline__ bool any_not_finite(const char* area, int row0, int steps) {
-  uint32_t f = 0;
+__device__ __forceinline__ bool any_not_finite(const char* area, int steps) {
+  typedef short i16x2 __attribute__((ext_vector_type(2)));
+  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+  i16x2 above = {0, 0};  // as integers, those from +inf on are the largest signed ones, those from -inf on the largest of all
+  u16x2 below = {0, 0};
 #pragma unroll 1
   for (int e = 0; e < steps; ++e)
 #pragma unroll
-    for (int d = 0; d < DP / 32; ++d) f |= not_finite(cols_fragment<DP>(area, row0 + 16 * e, 32 * d));
-  return __any(f != 0);
+    for (int d = 0; d < DP / 32; ++d) {
+      const u32x4 w = __builtin_bit_cast(u32x4, cols_fragment<DP>(area, 16 * e, 32 * d));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        above = __builtin_elementwise_max(above, __builtin_bit_cast(i16x2, w[j]));
+        below = __builtin_elementwise_max(below, __builtin_bit_cast(u16x2, w[j]));
+      }
+    }
+  return __any(above[0] >= 0x7F80 || above[1] >= 0x7F80 || below[0] >= 0xFF80 || below[1] >= 0xFF80);
 }
-
-// This half's share of the product of the lane's row, held as an operand, and the row at p (the same for all lanes).
+// This half's share of the product of the lane's row, held as an operand, and the row at p (the same for all lanes).  (The
+// scheduling barriers, here and below: this is rare, and loads side by side would take registers from the main loops.)
 template <int DP>
 __device__ __forceinline__ float half_dot(const bf16x8 (&f)[DP / 16], const uint16_t* p, int dim) {
   float sum = 0.0f;
@@ -183,6 +184,7 @@ __device__ __forceinline__ float half_dot(const bf16x8 (&f)[DP / 16], const uint
       sum = __builtin_fmaf(__uint_as_float(x[j] << 16), __uint_as_float(y[j] << 16), sum);
       sum = __builtin_fmaf(__uint_as_float(x[j] & 0xFFFF0000u), __uint_as_float(y[j] & 0xFFFF0000u), sum);
     }
+    __builtin_amdgcn_sched_barrier(0);
   }
   return sum;
 }
@@ -194,15 +196,25 @@ __device__ __forceinline__ void add_row(f32x16 (&acc)[DP / 32], float w, const u
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const int col = 32 * d + 8 * g + 4 * ((threadIdx.x & 63) >> 5);
-      if (col >= dim) continue;
-      const u32x2 x = *reinterpret_cast<const u32x2*>(p + col);
+      const u32x2 x = *reinterpret_cast<const u32x2*>(p + min(col, dim - 4));  // columns past dim are not stored
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         acc[d][4 * g + 2 * j] = __builtin_fmaf(w, __uint_as_float(x[j] << 16), acc[d][4 * g + 2 * j]);
         acc[d][4 * g + 2 * j + 1] = __builtin_fmaf(w, __uint_as_float(x[j] & 0xFFFF0000u), acc[d][4 * g + 2 * j + 1]);
       }
+      __builtin_amdgcn_sched_barrier(0);
     }
 }
+
+// Copies 4 bytes a lane straight to LDS, lane l's to l + 4 l.
+__device__ __forceinline__ void lds_copy4(const char* g, char* l) { __builtin_amdgcn_global_load_lds(g, (lds_void_t*)l, 4, 0, 0); }
+
+// Waits of the counts of copies that gemm_dma.h has none for.
+#define VDSL_DMA_WAIT_CASE(n) \
+  template <> __device__ __forceinline__ void dma_wait<n>() { __builtin_amdgcn_s_waitcnt(((n) & 0xF) | (((n) >> 4) << 14) | (0x7 << 4)); }
+VDSL_DMA_WAIT_CASE(5)
+VDSL_DMA_WAIT_CASE(10)
+#undef VDSL_DMA_WAIT_CASE
 
 // r / group for r below 2^31.
 struct Divider {

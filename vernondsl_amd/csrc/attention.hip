@@ -371,7 +371,7 @@ __global__ __launch_bounds__(256, 2) void attention_rows(AttentionArgs a) {
 #pragma unroll
     for (int e = 0; e < 2 * KS; ++e) w[e] = weights_fragment(s[e / 2], e % 2);
     // some rows do not see some of these keys
-    if (a.causal && j0 + KT > fewest && (j0 >= left_out || any_not_finite<DP>(values, 0, 2 * KS))) {
+    if (a.causal && j0 + KT > fewest && (j0 >= left_out || any_not_finite<DP>(values, 2 * KS))) {
       left_out = min(left_out, j0);
       continue;
     }

@@ -124,23 +124,30 @@ struct PairCopies {
   }
 };
 
-// dk and dv: eight waves of 32 keys each, walking over tiles of 64 rows.
-template <int DP, int NW>
-__global__ __launch_bounds__(64 * NW, NW / 4) void attention_bwd_keys(GradArgs a) {
-  constexpr int TR = 64;
+// dk and dv: a block has 128 keys and walks over tiles of 64 rows through a ring of three slots of LDS.  Each 32 keys have two waves, one
+// for each half of a tile's rows, which add up their sums at the end; both are on one SIMD, and the first has priority
+// there, so that its exponentials come beside the other's products.  To leave both their registers, wide heads'
+// values are an operand read from LDS (V_LDS).
+template <int DP>
+__global__ __launch_bounds__(512, 2) void attention_bwd_keys(GradArgs a) {
+  constexpr int TR = 64, NW = 8;
+  constexpr bool V_LDS = DP > 96;
   using T = TileShape<DP>;
   using Copies = PairCopies<DP, TR, NW>;
-  __shared__ __attribute__((aligned(1024))) char smem[2 * Copies::SLOT];
-  __shared__ __attribute__((aligned(16))) float start[2][2][TR];  // what the rows' scores and dp start from
+  constexpr int SUMS = 4 * 32 * DP * 4;  // one gradient's sums of four waves
+  constexpr int NS = 3, AREA = NS * Copies::SLOT + (V_LDS ? 128 * T::PITCH : 0);
+  __shared__ __attribute__((aligned(1024))) char smem[AREA > SUMS ? AREA : SUMS];
+  __shared__ __attribute__((aligned(16))) float starts[NW][NS][2][32];  // what the rows' scores and dp start from, a copy a wave
   int b = static_cast<int>(blockIdx.x);
   const int kv = b % a.kv_heads;
-  const RowTile tile = row_tile<NW == 4 ? 7 : 8>(a.seqs, 1, b / a.kv_heads);
+  const RowTile tile = row_tile<7>(a.seqs, 1, b / a.kv_heads);
   if (!tile.any) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
-  const int key = tile.row + 32 * wave + (lane & 31);
+  const int part = wave >> 2;  // of a tile's rows
+  const int key0 = tile.row + 32 * (wave & 3), key = key0 + (lane & 31);
   const int64_t head_col = static_cast<int64_t>(kv) * a.dim;
   if (tile.seq < 0) {
-    if (key < tile.len && half == 0) {
+    if (key < tile.len && half == 0 && part == 0) {
       store_zeros(a.grad_dtype, a.dk, a.dk_first + (tile.token + key) * a.dk_stride + head_col, a.dim);
       store_zeros(a.grad_dtype, a.dv, a.dv_first + (tile.token + key) * a.dv_stride + head_col, a.dim);
     }
@@ -148,116 +155,156 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void attention_bwd_keys(GradArgs a
   }
   const Copies copies(wave);
   if (2 * a.dim < T::PITCH) {
-    for (int i = threadIdx.x; i < 2 * Copies::SLOT / 16; i += 64 * NW) reinterpret_cast<u32x4*>(smem)[i] = u32x4{0u, 0u, 0u, 0u};
+    for (int i = threadIdx.x; i < NS * Copies::SLOT / 16; i += 512) reinterpret_cast<u32x4*>(smem)[i] = u32x4{0u, 0u, 0u, 0u};
     __syncthreads();
   }
   const int64_t token = tile.token + min(key, tile.len - 1);
   bf16x8 kf[DP / 16], vf[DP / 16];
   load_operand<DP>(a.k + token * a.k_stride + head_col, a.dim, kf);
   load_operand<DP>(a.v + token * a.v_stride + head_col, a.dim, vf);
+  char* const values = smem + NS * Copies::SLOT + (wave & 3) * 32 * T::PITCH;  // both waves write the same
+  if constexpr (V_LDS) {
+#pragma unroll
+    for (int kk = 0; kk < DP / 16; ++kk)
+      *reinterpret_cast<bf16x8*>(values + (lane & 31) * T::PITCH + (((2 * kk + half) ^ T::swz(lane & 31)) << 4)) = vf[kk];
+  }
   const int rows = tile.len * a.group;
   const int first = a.causal ? tile.row * a.group / TR : 0, end = (rows + TR - 1) / TR;
   const char* const qp = reinterpret_cast<const char*>(a.q + tile.token * a.q_stride + head_col * a.group);
   const char* const dp = reinterpret_cast<const char*>(a.dout + tile.token * a.dout_stride + head_col * a.group);
   const float* const sp = a.rows + (static_cast<int64_t>(kv) * a.seqs.n + tile.token) * a.group;
   const int64_t delta_at = a.seqs.n * a.heads;
-  const auto start_of = [&](int t) {  // of the lane's row and which of the two
-    return sp[(threadIdx.x / TR) * delta_at + min(t * TR + static_cast<int>(threadIdx.x % TR), rows - 1)];
-  };
-  float next = 0.0f;
+  // The copies of tile t.
   const auto fetch = [&](int t, int slot) {
-    copies(smem + slot * Copies::SLOT, wave, a.dim, rows - 1 - t * TR, [&](int r, int which) {
+    const int last = rows - 1 - t * TR;
+    copies(smem + slot * Copies::SLOT, wave, a.dim, last, [&](int r, int which) {
       const int row = t * TR + r, i = a.token_of(row);
       const int64_t col = static_cast<int64_t>(row - i * a.group) * a.dim;
       return which == 0 ? qp + 2 * (i * a.q_stride + col) : dp + 2 * (i * a.dout_stride + col);
     });
+    float* const to = starts[wave][slot][0];
+    const int r = 32 * part + (lane & 31);
+    // rows that are not there: no weight
+    if (r <= last) lds_copy4(reinterpret_cast<const char*>(sp + (half ? delta_at : 0) + t * TR + r), reinterpret_cast<char*>(to));
+    else to[lane] = half ? 0.0f : neg_inf();
   };
-  fetch(first, 0);
-  if (threadIdx.x < 2 * TR) start[0][threadIdx.x / TR][threadIdx.x % TR] = start_of(first);
   f32x16 dk[DP / 32], dv[DP / 32];
 #pragma unroll
   for (int d = 0; d < DP / 32; ++d) dk[d] = dv[d] = MfmaBf16::zero();
   const float scale2 = a.scale * kLog2e;
   const int sees_from = a.causal ? key * a.group : 0;  // the key's first row
-  const int wave_first = a.causal ? (tile.row + 32 * wave) * a.group : 0, wave_all = a.causal ? (tile.row + 32 * wave + 31) * a.group : 0;
-  int slot = 0, left_out = 0x7fffffff;
+  // the first row that sees one of the wave's keys, and the first that sees all of them
+  const int one_seen = a.causal ? key0 * a.group : 0, all_seen = a.causal ? (key0 + 31) * a.group : 0;
+  int left_out = 0;  // rows before this one
+  // All blocks begin with the last rows, which they all see, and so read the same rows at about the same time.
+  fetch(end - 1, 0);
+  if (end - 2 >= first) fetch(end - 2, 1);
+  int slot = 0;
+  if (part == 0) __builtin_amdgcn_s_setprio(1);
 #pragma unroll 1
-  for (int t = first; t < end; ++t) {
-    dma_wait<0>();
-    __syncthreads();
-    if (t + 1 < end) {
-      if (threadIdx.x < 2 * TR) next = start_of(t + 1);
-      fetch(t + 1, slot ^ 1);
-    }
-    const char* const qs = smem + slot * Copies::SLOT;
+  for (int t = end - 1; t >= first; --t) {
+    // the next tile, which is whole, may be on its way; every wave has left the one before
+    if (t > first) dma_wait<2 * Copies::C + 1>();
+    else dma_wait<0>();
+    dma_barrier();
+    if (t - 2 >= first) fetch(t - 2, slot == 0 ? 2 : slot - 1);
+    const char* const qs = smem + slot * Copies::SLOT + part * 32 * T::PITCH;
     const char* const ds = qs + TR * T::PITCH;
-    if ((t + 1) * TR > wave_first) {
-#pragma unroll 1
-      for (int u = 0; u < TR / 32; ++u) {
-        const int r0 = t * TR + 32 * u;
-        f32x16 s, p;
+    const float* const x = starts[wave][slot][0] + 4 * half;
+    slot = slot == 2 ? 0 : slot + 1;
+    const int r0 = t * TR + 32 * part;
+    if (r0 + 32 <= one_seen || r0 >= rows) continue;
+    f32x16 s, p;
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const f32x4 x = *reinterpret_cast<const f32x4*>(&start[slot][0][32 * u + 8 * g + 4 * half]);
-          const f32x4 y = *reinterpret_cast<const f32x4*>(&start[slot][1][32 * u + 8 * g + 4 * half]);
+    for (int g = 0; g < 4; ++g) {
+      const f32x4 s0 = *reinterpret_cast<const f32x4*>(x + 8 * g), p0 = *reinterpret_cast<const f32x4*>(x + 32 + 8 * g);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            s[4 * g + j] = x[j];
-            p[4 * g + j] = y[j];
-          }
-        }
-#pragma unroll
-        for (int kk = 0; kk < DP / 16; ++kk) {
-          s = MfmaBf16::mma(rows_fragment<DP>(qs, 32 * u, kk), kf[kk], s);
-          p = MfmaBf16::mma(rows_fragment<DP>(ds, 32 * u, kk), vf[kk], p);
-        }
-        const bool masked = r0 < wave_all || r0 + 32 > rows;
-        const int lo = sees_from - r0, hi = rows - r0;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          s[i] = __builtin_amdgcn_exp2f(s[i] * scale2);
-          p[i] *= s[i];
-        }
-        if (masked) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int r = 8 * (i / 4) + 4 * half + i % 4;
-            const bool in = r >= lo && r < hi;
-            s[i] = in ? s[i] : 0.0f;
-            p[i] = in ? p[i] : 0.0f;
-          }
-        }
-        const bf16x8 w[2] = {weights_fragment(s, 0), weights_fragment(s, 1)}, d[2] = {weights_fragment(p, 0), weights_fragment(p, 1)};
-        // some keys are not seen by some of these rows
-        if (r0 < wave_all && (r0 >= left_out || any_not_finite<DP>(qs, 32 * u, 2) || any_not_finite<DP>(ds, 32 * u, 2))) {
-          left_out = min(left_out, r0);
-          continue;
-        }
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-#pragma unroll
-          for (int x = 0; x < DP / 32; ++x) {
-            dv[x] = MfmaBf16::mma(cols_fragment<DP>(ds, 32 * u + 16 * e, 32 * x), w[e], dv[x]);
-            dk[x] = MfmaBf16::mma(cols_fragment<DP>(qs, 32 * u + 16 * e, 32 * x), d[e], dk[x]);
-          }
+      for (int j = 0; j < 4; ++j) {
+        s[4 * g + j] = s0[j];
+        p[4 * g + j] = p0[j];
       }
     }
-    slot ^= 1;
-    if (t + 1 < end && threadIdx.x < 2 * TR) start[slot][threadIdx.x / TR][threadIdx.x % TR] = next;
+#pragma unroll
+    for (int kk = 0; kk < DP / 16; ++kk) {
+      s = MfmaBf16::mma(rows_fragment<DP>(qs, 0, kk), kf[kk], s);
+      p = MfmaBf16::mma(rows_fragment<DP>(ds, 0, kk), V_LDS ? rows_fragment<DP>(values, 0, kk) : vf[kk], p);
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      s[i] = __builtin_amdgcn_exp2f(s[i] * scale2);
+      p[i] *= s[i];
+    }
+    if (r0 < all_seen) {
+      const int lo = sees_from - r0;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const bool in = 8 * (i / 4) + 4 * half + i % 4 >= lo;
+        s[i] = in ? s[i] : 0.0f;
+        p[i] = in ? p[i] : 0.0f;
+      }
+      // some rows do not see some of these keys
+      if (left_out > 0 || any_not_finite<DP>(qs, 2) || any_not_finite<DP>(ds, 2)) {
+        left_out = max(left_out, r0 + 32);
+        continue;
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const bf16x8 wf = weights_fragment(s, e), df = weights_fragment(p, e);
+#pragma unroll
+      for (int d = 0; d < DP / 32; ++d) {
+        dv[d] = MfmaBf16::mma(cols_fragment<DP>(ds, 16 * e, 32 * d), wf, dv[d]);
+        dk[d] = MfmaBf16::mma(cols_fragment<DP>(qs, 16 * e, 32 * d), df, dk[d]);
+      }
+    }
   }
+  __builtin_amdgcn_s_setprio(0);
 #pragma unroll 1
-  for (int r = left_out; r < min((wave_all + 31) & ~31, rows); ++r) {
+  for (int r = one_seen; r < min(left_out, rows); ++r) {
+    if (((r >> 5) & 1) != part) continue;
     const int i = a.token_of(r);
     const int64_t col = static_cast<int64_t>(r - i * a.group) * a.dim;
     const uint16_t* const qr = reinterpret_cast<const uint16_t*>(qp) + i * a.q_stride + col;
     const uint16_t* const dr = reinterpret_cast<const uint16_t*>(dp) + i * a.dout_stride + col;
-    const float s = halves_sum(half_dot<DP>(kf, qr, a.dim)), p = halves_sum(half_dot<DP>(vf, dr, a.dim));
+    float pr;
+    if constexpr (V_LDS) {
+      load_operand<DP>(a.v + token * a.v_stride + head_col, a.dim, vf);
+      pr = halves_sum(half_dot<DP>(vf, dr, a.dim));
+    } else {
+      pr = halves_sum(half_dot<DP>(vf, dr, a.dim));
+    }
+    const float sr = halves_sum(half_dot<DP>(kf, qr, a.dim));
     if (r < sees_from) continue;
-    const float w = __builtin_amdgcn_exp2f((s + sp[r]) * scale2);
+    const float w = __builtin_amdgcn_exp2f((sr + sp[r]) * scale2);
     add_row<DP>(dv, w, dr, a.dim);
-    add_row<DP>(dk, w * (p + sp[delta_at + r]), qr, a.dim);
+    add_row<DP>(dk, w * (pr + sp[delta_at + r]), qr, a.dim);
   }
-  if (key < tile.len) {
+  // the second halves' sums by way of LDS, one gradient after the other
+  float* const sums = reinterpret_cast<float*>(smem) + (wave & 3) * DP * 32 + lane * 4;
+  const auto join = [&](f32x16 (&acc)[DP / 32]) {
+    __syncthreads();
+    if (part == 1) {
+#pragma unroll
+      for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<f32x4*>(sums + (4 * d + g) * 256) = f32x4{acc[d][4 * g], acc[d][4 * g + 1], acc[d][4 * g + 2], acc[d][4 * g + 3]};
+    }
+    __syncthreads();
+    if (part == 0) {
+#pragma unroll
+      for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const f32x4 v = *reinterpret_cast<const f32x4*>(sums + (4 * d + g) * 256);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[d][4 * g + j] += v[j];
+        }
+    }
+  };
+  join(dk);
+  join(dv);
+  if (part == 0 && key < tile.len) {
     store_gradient<DP>(dk, a.scale, a.grad_dtype, a.dk, a.dk_first + token * a.dk_stride + head_col, a.dim);
     store_gradient<DP>(dv, 1.0f, a.grad_dtype, a.dv, a.dv_first + token * a.dv_stride + head_col, a.dim);
   }
@@ -346,7 +393,7 @@ __global__ __launch_bounds__(256, 2) void attention_bwd_queries(GradArgs a) {
         for (int r = 0; r < 16; ++r) p[r] = 8 * (r / 4) + r % 4 < hi ? p[r] : 0.0f;
       }
       // some rows do not see some of these keys
-      if (a.causal && masked && (j0 >= left_out || any_not_finite<DP>(ks, 32 * u, 2))) {
+      if (a.causal && masked && (j0 >= left_out || any_not_finite<DP>(ks + 32 * u * T::PITCH, 2))) {
         left_out = min(left_out, j0);
         continue;
       }
@@ -462,7 +509,7 @@ extern "C" int vdsl_op_attention_bwd(vdsl_queue q, const vdsl_attention_params* 
   hipLaunchKernelGGL(attention_bwd_rows, block_grid((p->n * p->heads + 7) / 8), dim3(256), 0, q->stream, dout->ptr, dout_dtype,
                      out->ptr, out_dtype, static_cast<const float*>(lse->ptr), p->n, p->heads, group, p->dim, p->scale, copy, rows);
   VDSL_TRY(check_launch("attention_bwd_rows"));
-  const int64_t key_slots = row_slots(p->n, p->seqs, 1, p->dim <= 96 ? 8 : 7);
+  const int64_t key_slots = row_slots(p->n, p->seqs, 1, 7);
   const int64_t query_slots = row_slots(p->n, p->seqs, group, 7);
   if (std::max(key_slots, query_slots) * p->kv_heads > 0x7fffff) return fail(VDSL_ERR_UNSUPPORTED, "attention_bwd: too many rows");
   const auto go = [&](auto kernel, unsigned lanes, int64_t slots, const char* name) {
@@ -470,8 +517,8 @@ extern "C" int vdsl_op_attention_bwd(vdsl_queue q, const vdsl_attention_params* 
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(slots * p->kv_heads)), dim3(lanes), 0, q->stream, a);
     return check_launch(name);
   };
-  const auto keys = p->dim <= 64 ? attention_bwd_keys<64, 8> : p->dim <= 96 ? attention_bwd_keys<96, 8> : attention_bwd_keys<128, 4>;
+  const auto keys = p->dim <= 64 ? attention_bwd_keys<64> : p->dim <= 96 ? attention_bwd_keys<96> : attention_bwd_keys<128>;
   const auto queries = p->dim <= 64 ? attention_bwd_queries<64> : p->dim <= 96 ? attention_bwd_queries<96> : attention_bwd_queries<128>;
-  VDSL_TRY(go(keys, p->dim <= 96 ? 512 : 256, key_slots, "attention_bwd_keys"));
+  VDSL_TRY(go(keys, 512, key_slots, "attention_bwd_keys"));
   return go(queries, 256, query_slots, "attention_bwd_queries");
 }

@@ -126,7 +126,7 @@ __device__ __forceinline__ void load_operand(const uint16_t* p, int dim, bf16x8 
 __device__ __forceinline__ f32x2_t both_halves(float v) {
   const uint32_t b = __builtin_bit_cast(uint32_t, v);
   const auto r = __builtin_amdgcn_permlane32_swap(b, b, false, false);
-  const uint32_t lo = r[0], hi = r[1];  // (a bit cast of r[1] itself takes element 0)
+  const uint32_t lo = r[0], hi = r[1];  // (a bit cast of a vector's element itself takes element 0)
   return f32x2_t{__builtin_bit_cast(float, lo), __builtin_bit_cast(float, hi)};
 }
 __device__ __forceinline__ float halves_max(float v) {
@@ -163,8 +163,9 @@ __device__ __forceinline__ bool any_not_finite(const char* area, int steps) {
       const u32x4 w = __builtin_bit_cast(u32x4, cols_fragment<DP>(area, 16 * e, 32 * d));
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        above = __builtin_elementwise_max(above, __builtin_bit_cast(i16x2, w[j]));
-        below = __builtin_elementwise_max(below, __builtin_bit_cast(u16x2, w[j]));
+        const uint32_t x = w[j];
+        above = __builtin_elementwise_max(above, __builtin_bit_cast(i16x2, x));
+        below = __builtin_elementwise_max(below, __builtin_bit_cast(u16x2, x));
       }
     }
   return __any(above[0] >= 0x7F80 || above[1] >= 0x7F80 || below[0] >= 0xFF80 || below[1] >= 0xFF80);

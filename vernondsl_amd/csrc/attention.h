@@ -149,15 +149,15 @@ __device__ __forceinline__ bf16x8 weights_fragment(const f32x16& s, int e) {
 // not there are zeros in LDS; those of the sequence that only some rows of a tile see are looked through, and from the
 // first tile that holds an element that is no finite number on, such tiles are left out and added at the end key by
 // key, each lane taking what it sees: by half_dot and add_row.
-// Whether a tile's rows 0 .. 16 steps - 1 hold an element that is no finite number.
+// Whether 32 rows of a tile hold an element that is no finite number.
 template <int DP>
-__device__ __forceinline__ bool any_not_finite(const char* area, int steps) {
+__device__ __forceinline__ bool any_not_finite(const char* area) {
   typedef short i16x2 __attribute__((ext_vector_type(2)));
   typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
   i16x2 above = {0, 0};  // as integers, those from +inf on are the largest signed ones, those from -inf on the largest of all
   u16x2 below = {0, 0};
-#pragma unroll 1
-  for (int e = 0; e < steps; ++e)
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d) {
       const u32x4 w = __builtin_bit_cast(u32x4, cols_fragment<DP>(area, 16 * e, 32 * d));
@@ -169,6 +169,13 @@ __device__ __forceinline__ bool any_not_finite(const char* area, int steps) {
       }
     }
   return __any(above[0] >= 0x7F80 || above[1] >= 0x7F80 || below[0] >= 0xFF80 || below[1] >= 0xFF80);
+}
+// Whether a lane of the wave has a value that is no finite number.
+__device__ __forceinline__ bool any_not_finite(const f32x16& v) {
+  float z = 0.0f;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) z = __builtin_fmaf(v[r], 0.0f, z);
+  return __any(z != z);
 }
 // This half's share of the product of the lane's row, held as an operand, and the row at p (the same for all lanes).  (The
 // scheduling barriers, here and below: this is rare, and loads side by side would take registers from the main loops.)

@@ -341,9 +341,9 @@ __global__ __launch_bounds__(256, 2) void attention_rows(AttentionArgs a) {
   // of the wave's rows: the fewest and the most keys that one sees
   const int fewest = __builtin_amdgcn_readfirstlane(at.sees(min(row0, at.rows - 1), a.group, a.causal));
   const int most = mine ? at.sees(min(row0 + 32, at.rows) - 1, a.group, a.causal) : 0;
-  int slot = 0, left_out = 0x7fffffff;
-#pragma unroll 1
-  for (int t = first; t < end; ++t) {
+  int slot = 0, t = first;
+  // The tile t is there and every wave has left the one before, whose slot the next one goes to.
+  const auto enter = [&]() {
     dma_wait<0>();
     dma_barrier();
     if (t + 1 < end) {
@@ -352,11 +352,14 @@ __global__ __launch_bounds__(256, 2) void attention_rows(AttentionArgs a) {
     } else if constexpr (PAGED) {
       valid[1] = valid[0];
     }
+  };
+  // tiles that all of the wave's rows see all of
+#pragma unroll 1
+  for (const int whole = min(end, fewest / KT); t < whole; ++t) {
+    enter();
     const char* const keys = smem + slot * SLOT;
     const char* const values = keys + KT * T::PITCH;
     slot ^= 1;
-    const int j0 = t * KT;
-    if (j0 >= most) continue;
     f32x16 s[KS];
 #pragma unroll
     for (int k = 0; k < KS; ++k) {
@@ -364,21 +367,43 @@ __global__ __launch_bounds__(256, 2) void attention_rows(AttentionArgs a) {
 #pragma unroll
       for (int kk = 0; kk < DP / 16; ++kk) s[k] = MfmaBf16::mma(rows_fragment<DP>(keys, 32 * k, kk), qf[kk], s[k]);
     }
-    const uint64_t there = valid[1];
-    if (j0 + KT > fewest || (PAGED && there != ~0ull)) hide(s, sees - j0, there);
+    if (PAGED && valid[1] != ~0ull) hide(s, KT, valid[1]);
     st.weigh(s, scale2);
-    bf16x8 w[2 * KS];
 #pragma unroll
-    for (int e = 0; e < 2 * KS; ++e) w[e] = weights_fragment(s[e / 2], e % 2);
-    // some rows do not see some of these keys
-    if (a.causal && j0 + KT > fewest && (j0 >= left_out || any_not_finite<DP>(values, 2 * KS))) {
-      left_out = min(left_out, j0);
-      continue;
+    for (int e = 0; e < 2 * KS; ++e) {
+      const bf16x8 w = weights_fragment(s[e / 2], e % 2);
+#pragma unroll
+      for (int d = 0; d < DP / 32; ++d) st.o[d] = MfmaBf16::mma(cols_fragment<DP>(values, 16 * e, 32 * d), w, st.o[d]);
     }
+  }
+  // the others, 32 keys at a time
+  int left_out = 0x7fffffff;
+#pragma unroll 1
+  for (; t < end; ++t) {
+    enter();
+    const char* const keys = smem + slot * SLOT;
+    const char* const values = keys + KT * T::PITCH;
+    slot ^= 1;
+#pragma unroll 1
+    for (int k = 0; k < KS; ++k) {
+      const int j0 = t * KT + 32 * k;
+      if (j0 >= most) break;
+      f32x16 s[1] = {MfmaBf16::zero()};
 #pragma unroll
-    for (int e = 0; e < 2 * KS; ++e)
+      for (int kk = 0; kk < DP / 16; ++kk) s[0] = MfmaBf16::mma(rows_fragment<DP>(keys, 32 * k, kk), qf[kk], s[0]);
+      hide(s, sees - j0, valid[1] >> (32 * k));
+      st.weigh(s, scale2);
+      if (a.causal && (j0 >= left_out || any_not_finite<DP>(values + 32 * k * T::PITCH))) {
+        left_out = min(left_out, j0);
+        continue;
+      }
 #pragma unroll
-      for (int d = 0; d < DP / 32; ++d) st.o[d] = MfmaBf16::mma(cols_fragment<DP>(values, 16 * e, 32 * d), w[e], st.o[d]);
+      for (int e = 0; e < 2; ++e) {
+        const bf16x8 w = weights_fragment(s[0], e);
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) st.o[d] = MfmaBf16::mma(cols_fragment<DP>(values, 32 * k + 16 * e, 32 * d), w, st.o[d]);
+      }
+    }
   }
 #pragma unroll 1
   for (int j = left_out; j < min(most, end * KT); ++j) {

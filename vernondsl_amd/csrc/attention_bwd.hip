@@ -1,7 +1,7 @@
 // The gradient of attention over packed sequences.  With p = exp2(c s - lse log2 e) formed again from q, k and lse,
 // dp = dout v, delta = dout out and ds = p (dp - delta):
 //   dq = scale ds k (rows' own sum over keys),   dk = scale ds^T q and dv = p^T dout (keys' own sums over rows and heads)
-// Three launches: delta of each row; dk and dv, a wave holding 32 keys and walking over the rows that see them; dq, a
+// The launches: delta of each row; dk and dv, a wave holding 32 keys and walking over the rows that see them; dq, a
 // wave holding its rows and walking over the keys they see.  Each sum belongs to one wave and is taken in one order, so
 // nothing is added atomically and the bits are the same on every call; the price is that s and dp are formed twice (7
 // products where 5 would do).  See attention.h for rows, tiles and the order of the products' sums.
@@ -22,6 +22,7 @@ struct GradArgs {
   const uint16_t *q, *k, *v, *dout;  // dout: bf16
   int64_t q_stride, k_stride, v_stride, dout_stride;
   Sequences seqs;
+  int* left_out;      // by the waves of attention_bwd_keys
   const float* rows;  // -lse / scale, then -delta, each [kv_heads][n * group]
   void *dq, *dk, *dv;
   int64_t dq_first, dq_stride, dk_first, dk_stride, dv_first, dv_stride;
@@ -141,12 +142,16 @@ __global__ __launch_bounds__(512, 2) void attention_bwd_keys(GradArgs a) {
   int b = static_cast<int>(blockIdx.x);
   const int kv = b % a.kv_heads;
   const RowTile tile = row_tile<7>(a.seqs, 1, b / a.kv_heads);
-  if (!tile.any) return;
+  if (!tile.any) {
+    if (threadIdx.x < NW) a.left_out[blockIdx.x * NW + threadIdx.x] = 0;
+    return;
+  }
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
   const int part = wave >> 2;  // of a tile's rows
   const int key0 = tile.row + 32 * (wave & 3), key = key0 + (lane & 31);
   const int64_t head_col = static_cast<int64_t>(kv) * a.dim;
   if (tile.seq < 0) {
+    if (lane == 0) a.left_out[blockIdx.x * NW + wave] = 0;
     if (key < tile.len && half == 0 && part == 0) {
       store_zeros(a.grad_dtype, a.dk, a.dk_first + (tile.token + key) * a.dk_stride + head_col, a.dim);
       store_zeros(a.grad_dtype, a.dv, a.dv_first + (tile.token + key) * a.dv_stride + head_col, a.dim);
@@ -186,7 +191,7 @@ __global__ __launch_bounds__(512, 2) void attention_bwd_keys(GradArgs a) {
     const int r = 32 * part + (lane & 31);
     // rows that are not there: no weight
     if (r <= last) lds_copy4(reinterpret_cast<const char*>(sp + (half ? delta_at : 0) + t * TR + r), reinterpret_cast<char*>(to));
-    else to[lane] = half ? 0.0f : neg_inf();
+    else to[lane] = half ? 0.0f : -3e38f;
   };
   f32x16 dk[DP / 32], dv[DP / 32];
 #pragma unroll
@@ -195,7 +200,7 @@ __global__ __launch_bounds__(512, 2) void attention_bwd_keys(GradArgs a) {
   const int sees_from = a.causal ? key * a.group : 0;  // the key's first row
   // the first row that sees one of the wave's keys, and the first that sees all of them
   const int one_seen = a.causal ? key0 * a.group : 0, all_seen = a.causal ? (key0 + 31) * a.group : 0;
-  int left_out = 0;  // rows before this one
+  int left_out = 0;  // rows before this one: attention_bwd_left_out adds them
   // All blocks begin with the last rows, which they all see, and so read the same rows at about the same time.
   fetch(end - 1, 0);
   if (end - 2 >= first) fetch(end - 2, 1);
@@ -229,6 +234,9 @@ __global__ __launch_bounds__(512, 2) void attention_bwd_keys(GradArgs a) {
       s = MfmaBf16::mma(rows_fragment<DP>(qs, 0, kk), kf[kk], s);
       p = MfmaBf16::mma(rows_fragment<DP>(ds, 0, kk), V_LDS ? rows_fragment<DP>(values, 0, kk) : vf[kk], p);
     }
+    // a row whose q or dout holds an element that is no finite number has no finite score or dp with any key
+    bool leave = false;
+    if (r0 < all_seen) leave = left_out > 0 || any_not_finite(s) || any_not_finite(p);
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       s[i] = __builtin_amdgcn_exp2f(s[i] * scale2);
@@ -242,8 +250,7 @@ __global__ __launch_bounds__(512, 2) void attention_bwd_keys(GradArgs a) {
         s[i] = in ? s[i] : 0.0f;
         p[i] = in ? p[i] : 0.0f;
       }
-      // some rows do not see some of these keys
-      if (left_out > 0 || any_not_finite<DP>(qs, 2) || any_not_finite<DP>(ds, 2)) {
+      if (leave) {
         left_out = max(left_out, r0 + 32);
         continue;
       }
@@ -259,26 +266,7 @@ __global__ __launch_bounds__(512, 2) void attention_bwd_keys(GradArgs a) {
     }
   }
   __builtin_amdgcn_s_setprio(0);
-#pragma unroll 1
-  for (int r = one_seen; r < min(left_out, rows); ++r) {
-    if (((r >> 5) & 1) != part) continue;
-    const int i = a.token_of(r);
-    const int64_t col = static_cast<int64_t>(r - i * a.group) * a.dim;
-    const uint16_t* const qr = reinterpret_cast<const uint16_t*>(qp) + i * a.q_stride + col;
-    const uint16_t* const dr = reinterpret_cast<const uint16_t*>(dp) + i * a.dout_stride + col;
-    float pr;
-    if constexpr (V_LDS) {
-      load_operand<DP>(a.v + token * a.v_stride + head_col, a.dim, vf);
-      pr = halves_sum(half_dot<DP>(vf, dr, a.dim));
-    } else {
-      pr = halves_sum(half_dot<DP>(vf, dr, a.dim));
-    }
-    const float sr = halves_sum(half_dot<DP>(kf, qr, a.dim));
-    if (r < sees_from) continue;
-    const float w = __builtin_amdgcn_exp2f((sr + sp[r]) * scale2);
-    add_row<DP>(dv, w, dr, a.dim);
-    add_row<DP>(dk, w * (pr + sp[delta_at + r]), qr, a.dim);
-  }
+  if (lane == 0) a.left_out[blockIdx.x * NW + wave] = left_out;
   // the second halves' sums by way of LDS, one gradient after the other
   float* const sums = reinterpret_cast<float*>(smem) + (wave & 3) * DP * 32 + lane * 4;
   const auto join = [&](f32x16 (&acc)[DP / 32]) {
@@ -308,6 +296,65 @@ __global__ __launch_bounds__(512, 2) void attention_bwd_keys(GradArgs a) {
     store_gradient<DP>(dk, a.scale, a.grad_dtype, a.dk, a.dk_first + token * a.dk_stride + head_col, a.dim);
     store_gradient<DP>(dv, 1.0f, a.grad_dtype, a.dv, a.dv_first + token * a.dv_stride + head_col, a.dim);
   }
+}
+
+// The rows that a block of attention_bwd_keys left out, added to what it stored (so of bf16 gradients rounded once more): row by
+// row, each lane taking what its key is seen by.  (A launch of its own, whose blocks mostly find nothing: as a part of
+// that kernel it took the registers of its loop.)
+template <int DP>
+__global__ __launch_bounds__(256) void attention_bwd_left_out(GradArgs a) {
+  const int place = static_cast<int>(blockIdx.x);
+  const int* const flags = a.left_out + 8 * place;
+  int any = 0;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) any |= flags[w];
+  if (any == 0) return;
+  const int kv = place % a.kv_heads;
+  const RowTile tile = row_tile<7>(a.seqs, 1, place / a.kv_heads);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int key0 = tile.row + 32 * wave, key = key0 + (lane & 31);
+  const int64_t head_col = static_cast<int64_t>(kv) * a.dim, token = tile.token + min(key, tile.len - 1);
+  bf16x8 kf[DP / 16], vf[DP / 16];
+  load_operand<DP>(a.k + token * a.k_stride + head_col, a.dim, kf);
+  load_operand<DP>(a.v + token * a.v_stride + head_col, a.dim, vf);
+  f32x16 dk[DP / 32], dv[DP / 32];
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d) dk[d] = dv[d] = MfmaBf16::zero();
+  const uint16_t* const qp = a.q + tile.token * a.q_stride + head_col * a.group;
+  const uint16_t* const dp = a.dout + tile.token * a.dout_stride + head_col * a.group;
+  const float* const sp = a.rows + (static_cast<int64_t>(kv) * a.seqs.n + tile.token) * a.group;
+  const float scale2 = a.scale * kLog2e;
+  const int end = min(max(flags[wave], flags[wave + 4]), tile.len * a.group);
+#pragma unroll 1
+  for (int r = key0 * a.group; r < end; ++r) {
+    if (r >= flags[wave + 4 * ((r >> 5) & 1)]) continue;
+    const int i = a.token_of(r);
+    const int64_t col = static_cast<int64_t>(r - i * a.group) * a.dim;
+    const uint16_t* const qr = qp + i * a.q_stride + col;
+    const uint16_t* const dr = dp + i * a.dout_stride + col;
+    const float sr = halves_sum(half_dot<DP>(kf, qr, a.dim)), pr = halves_sum(half_dot<DP>(vf, dr, a.dim));
+    if (r < key * a.group) continue;
+    const float w = __builtin_amdgcn_exp2f((sr + sp[r]) * scale2);
+    add_row<DP>(dv, w, dr, a.dim);
+    add_row<DP>(dk, w * (pr + sp[a.seqs.n * a.heads + r]), qr, a.dim);
+  }
+  if (key >= tile.len) return;
+  const auto add = [&](const f32x16 (&acc)[DP / 32], float by, void* to, int64_t e) {
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int c = 32 * d + 8 * g + 4 * (lane >> 5);
+        if (c >= a.dim) continue;
+        float v[4];
+        load_some(a.grad_dtype, to, e + c, 4, v);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] += acc[d][4 * g + j] * by;
+        store_some(a.grad_dtype, to, e + c, 4, v);
+      }
+  };
+  add(dk, a.scale, a.dk, a.dk_first + token * a.dk_stride + head_col);
+  add(dv, 1.0f, a.dv, a.dv_first + token * a.dv_stride + head_col);
 }
 
 // dq: four waves of 32 rows each, walking over tiles of 64 keys.
@@ -365,44 +412,59 @@ __global__ __launch_bounds__(256, 2) void attention_bwd_queries(GradArgs a) {
   for (int d = 0; d < DP / 32; ++d) dq[d] = MfmaBf16::zero();
   const float scale2 = a.scale * kLog2e;
   const int fewest = sees(min(row0, rows - 1)), most = mine ? sees(min(row0 + 32, rows) - 1) : 0;
-  int slot = 0, left_out = 0x7fffffff;
-#pragma unroll 1
-  for (int t = 0; t < end; ++t) {
+  int slot = 0, t = 0, left_out = 0x7fffffff;
+  const auto enter = [&]() {
     dma_wait<0>();
     dma_barrier();
     if (t + 1 < end) fetch(t + 1, slot ^ 1);
+  };
+  // ds of 32 keys; odd: whether to say if a key holds an element that is no finite number, which has no finite score then
+  const auto form = [&](const char* ks, bool* odd) {
+    f32x16 s = MfmaBf16::zero(), p = MfmaBf16::zero();
+#pragma unroll
+    for (int kk = 0; kk < DP / 16; ++kk) {
+      s = MfmaBf16::mma(rows_fragment<DP>(ks, 0, kk), qf[kk], s);
+      p = MfmaBf16::mma(rows_fragment<DP>(ks + KT * T::PITCH, 0, kk), df[kk], p);
+    }
+    if (odd) *odd = any_not_finite(s);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) p[r] = __builtin_amdgcn_exp2f((s[r] + score0) * scale2) * (p[r] + dp0);
+    return p;
+  };
+  const auto add = [&](const char* ks, const f32x16& ds) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const bf16x8 w = weights_fragment(ds, e);
+#pragma unroll
+      for (int d = 0; d < DP / 32; ++d) dq[d] = MfmaBf16::mma(cols_fragment<DP>(ks, 16 * e, 32 * d), w, dq[d]);
+    }
+  };
+  // tiles that all of the wave's rows see all of
+#pragma unroll 1
+  for (const int whole = min(end, fewest / KT); t < whole; ++t) {
+    enter();
     const char* const ks = smem + slot * Copies::SLOT;
-    const char* const vs = ks + KT * T::PITCH;
     slot ^= 1;
 #pragma unroll 1
-    for (int u = 0; u < KT / 32; ++u) {
-      const int j0 = t * KT + 32 * u;
+    for (int u = 0; u < KT / 32; ++u) add(ks + 32 * u * T::PITCH, form(ks + 32 * u * T::PITCH, nullptr));
+  }
+  // the others
+#pragma unroll 1
+  for (; t < end; ++t) {
+    enter();
+    const char* ks = smem + slot * Copies::SLOT;
+    slot ^= 1;
+#pragma unroll 1
+    for (int u = 0; u < KT / 32; ++u, ks += 32 * T::PITCH) {
+      const int j0 = t * KT + 32 * u, hi = seen - j0 - 4 * (lane >> 5);
       if (j0 >= most) break;
-      f32x16 s = MfmaBf16::zero(), p = MfmaBf16::zero();
+      bool odd;
+      f32x16 p = form(ks, &odd);
 #pragma unroll
-      for (int kk = 0; kk < DP / 16; ++kk) {
-        s = MfmaBf16::mma(rows_fragment<DP>(ks, 32 * u, kk), qf[kk], s);
-        p = MfmaBf16::mma(rows_fragment<DP>(vs, 32 * u, kk), df[kk], p);
-      }
-      const bool masked = j0 + 32 > fewest;
-      const int hi = seen - j0 - 4 * (lane >> 5);
-#pragma unroll
-      for (int r = 0; r < 16; ++r) p[r] = __builtin_amdgcn_exp2f((s[r] + score0) * scale2) * (p[r] + dp0);
-      if (masked) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) p[r] = 8 * (r / 4) + r % 4 < hi ? p[r] : 0.0f;
-      }
+      for (int r = 0; r < 16; ++r) p[r] = 8 * (r / 4) + r % 4 < hi ? p[r] : 0.0f;
       // some rows do not see some of these keys
-      if (a.causal && masked && (j0 >= left_out || any_not_finite<DP>(ks + 32 * u * T::PITCH, 2))) {
-        left_out = min(left_out, j0);
-        continue;
-      }
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const bf16x8 w = weights_fragment(p, e);
-#pragma unroll
-        for (int d = 0; d < DP / 32; ++d) dq[d] = MfmaBf16::mma(cols_fragment<DP>(ks, 32 * u + 16 * e, 32 * d), w, dq[d]);
-      }
+      if (a.causal && (j0 >= left_out || odd)) left_out = min(left_out, j0);
+      else add(ks, p);
     }
   }
 #pragma unroll 1
@@ -430,11 +492,15 @@ bool apart(const vdsl_heads& x, int64_t x_width, const vdsl_heads& y, int64_t y_
 
 using namespace vdsl;
 
-// What the rows' scores and dp start from, then a copy of dout in bf16.
+// What the rows' scores and dp start from, what attention_bwd_keys left out, a copy of dout in bf16.
 extern "C" int vdsl_attention_bwd_workspace_bytes(int64_t n, int64_t seqs, int32_t heads, int32_t kv_heads, int32_t dim, size_t* bytes) {
   if (!bytes) return fail(VDSL_ERR_INVALID_ARG, "bytes is null");
   VDSL_TRY(attention_check_shape("attention_bwd", n, seqs, heads, kv_heads, dim));
-  *bytes = nbytes(n, heads, 8 + 2 * static_cast<int64_t>(dim));
+  // a multiple of 16 bytes before the copy
+  const size_t flags = nbytes(row_slots(n, seqs, 1, 7), kv_heads, 32), rows = nbytes(n, heads, 8 + 2 * static_cast<int64_t>(dim));
+  if (flags == kSizeOverflow || rows == kSizeOverflow || rows + flags + 16 < rows)
+    return fail(VDSL_ERR_SHAPE, "attention_bwd workspace size overflows");
+  *bytes = rows + flags + 16;
   return VDSL_OK;
 }
 
@@ -477,7 +543,10 @@ extern "C" int vdsl_op_attention_bwd(vdsl_queue q, const vdsl_attention_params* 
   if (p->n == 0) return VDSL_OK;
   const int group = p->heads / p->kv_heads;
   float* const rows = static_cast<float*>(workspace->ptr);
-  uint16_t* const copy = dout_dtype == VDSL_F32 ? reinterpret_cast<uint16_t*>(rows + 2 * p->n * p->heads) : nullptr;
+  const int64_t key_slots = row_slots(p->n, p->seqs, 1, 7), query_slots = row_slots(p->n, p->seqs, group, 7);
+  if (std::max(key_slots, query_slots) * p->kv_heads > 0x3fffff) return fail(VDSL_ERR_UNSUPPORTED, "attention_bwd: too many rows");
+  const int64_t flags_at = 2 * p->n * p->heads, copy_at = (flags_at + 8 * key_slots * p->kv_heads + 3) & ~int64_t{3};
+  uint16_t* const copy = dout_dtype == VDSL_F32 ? reinterpret_cast<uint16_t*>(rows + copy_at) : nullptr;
   GradArgs a = {};
   a.q = static_cast<const uint16_t*>(qs->ptr) + p->q.first;
   a.k = static_cast<const uint16_t*>(ks->ptr) + p->k.first;
@@ -489,6 +558,7 @@ extern "C" int vdsl_op_attention_bwd(vdsl_queue q, const vdsl_attention_params* 
   a.dout_stride = width;
   a.seqs = {static_cast<const int32_t*>(starts->ptr), p->n, p->seqs};
   a.rows = rows;
+  a.left_out = reinterpret_cast<int*>(rows + flags_at);
   a.dq = dq->ptr;
   a.dk = dk->ptr;
   a.dv = dv->ptr;
@@ -509,16 +579,15 @@ extern "C" int vdsl_op_attention_bwd(vdsl_queue q, const vdsl_attention_params* 
   hipLaunchKernelGGL(attention_bwd_rows, block_grid((p->n * p->heads + 7) / 8), dim3(256), 0, q->stream, dout->ptr, dout_dtype,
                      out->ptr, out_dtype, static_cast<const float*>(lse->ptr), p->n, p->heads, group, p->dim, p->scale, copy, rows);
   VDSL_TRY(check_launch("attention_bwd_rows"));
-  const int64_t key_slots = row_slots(p->n, p->seqs, 1, 7);
-  const int64_t query_slots = row_slots(p->n, p->seqs, group, 7);
-  if (std::max(key_slots, query_slots) * p->kv_heads > 0x7fffff) return fail(VDSL_ERR_UNSUPPORTED, "attention_bwd: too many rows");
   const auto go = [&](auto kernel, unsigned lanes, int64_t slots, const char* name) {
-    a.blocks = static_cast<int>(slots);
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(slots * p->kv_heads)), dim3(lanes), 0, q->stream, a);
     return check_launch(name);
   };
+  a.blocks = static_cast<int>(query_slots);
   const auto keys = p->dim <= 64 ? attention_bwd_keys<64> : p->dim <= 96 ? attention_bwd_keys<96> : attention_bwd_keys<128>;
   const auto queries = p->dim <= 64 ? attention_bwd_queries<64> : p->dim <= 96 ? attention_bwd_queries<96> : attention_bwd_queries<128>;
+  const auto rest = p->dim <= 64 ? attention_bwd_left_out<64> : p->dim <= 96 ? attention_bwd_left_out<96> : attention_bwd_left_out<128>;
   VDSL_TRY(go(keys, 512, key_slots, "attention_bwd_keys"));
+  if (p->causal) VDSL_TRY(go(rest, 256, key_slots, "attention_bwd_left_out"));
   return go(queries, 256, query_slots, "attention_bwd_queries");
 }

@@ -416,28 +416,195 @@ __global__ __launch_bounds__(256, 2) void attention_rows(AttentionArgs a) {
   if (mine) store_rows<DP>(a, st, at, row0, place.kv, place.split);
 }
 
-// Joins the splits: with M = max m, out = sum 2^(m - M) o / sum 2^(m - M) l.  32 lanes a row.
+// Few rows: a block is one wave with 32 rows and a split of the keys, in tiles of 32 through two slots of LDS of its own, so
+// that nothing waits for another wave.  What bounds it is the cache's bytes: five such blocks to a CU keep 80 KiB of them
+// on their way.  Pages of 16 positions or more: the halves of a tile lie in one page each, so a copy's address is a scalar
+// and an offset that a lane keeps.
+template <int DP>
+__global__ __launch_bounds__(64, 2) void attention_few(AttentionArgs a) {
+  constexpr int KT = 32;
+  using T = TileShape<DP>;
+  constexpr int SLOT = 2 * KT * T::PITCH, C = KT * T::PITCH / 1024;  // copies of a tile's keys, and of its values
+  __shared__ __attribute__((aligned(1024))) char smem[2 * SLOT];
+  const Place place(a);
+  const RowTile tile = row_tile<5>(a.seqs, a.group, place.slot);
+  if (!tile.any) return;
+  const RowsAt at = rows_at<true>(a, tile);
+  const int lane = threadIdx.x;
+  const int last_row = min(tile.row + 32, at.rows) - 1;
+  const int most = at.sees(last_row, a.group, 1), fewest = at.sees(tile.row, a.group, 1);
+  const int tiles = (most + KT - 1) / KT;
+  const int share = (tiles + a.splits - 1) / a.splits;
+  const int first = place.split * share, end = min(first + share, tiles);
+  if (first >= end) {
+    store_none(a, at, tile.row, 32, place.kv, place.split);
+    return;
+  }
+  if (2 * a.dim < T::PITCH) {  // columns past dim are never copied
+    for (int i = lane; i < 2 * SLOT / 16; i += 64) reinterpret_cast<u32x4*>(smem)[i] = u32x4{0u, 0u, 0u, 0u};
+  }
+  // as constant memory: scalar loads, which no copy is waited for with
+  typedef const __attribute__((address_space(4))) int32_t* ScalarTable;
+  const int64_t seq = tile.seq < 0 ? 0 : tile.seq;
+  const ScalarTable table = (ScalarTable)(reinterpret_cast<uint64_t>(a.table)) +
+                            (static_cast<int64_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(seq))) * a.table_cols);
+  const uint32_t row_bytes = 2 * static_cast<uint32_t>(a.dim);
+  uint32_t off[C / 2];
+#pragma unroll
+  for (int u = 0; u < C / 2; ++u) {
+    const int r = u * (64 / T::CPR) + lane / T::CPR, c = lane % T::CPR ^ T::swz(r);
+    off[u] = c < a.dim / 8 ? static_cast<uint32_t>(r) * row_bytes + 16u * static_cast<uint32_t>(c) : ~0u;
+  }
+  const bool all = 2 * a.dim == T::PITCH;
+  // The pages of a tile's halves.
+  const auto entry = [&](int t, int half) {
+    const int j = __builtin_amdgcn_readfirstlane(t * KT + 16 * half);
+    if (j >= most) return -1;
+    const int e = table[j >> a.page_shift];
+    return static_cast<uint32_t>(e) < static_cast<uint64_t>(a.pages) ? e : -1;
+  };
+  int page0 = entry(first, 0), page1 = entry(first, 1);
+  uint32_t valid = 0u, valid_next = 0u;  // which keys of the tile and of the next one hold something
+  const auto fetch = [&](int t, int slot) {
+    const int now[2] = {page0, page1};
+    if (t + 1 < end) {
+      page0 = entry(t + 1, 0);
+      page1 = entry(t + 1, 1);
+    }
+    valid = valid_next;
+    valid_next = (now[0] >= 0 ? 0xFFFFu : 0u) | (now[1] >= 0 ? 0xFFFF0000u : 0u);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      char* const to = smem + slot * SLOT + h * 16 * T::PITCH;
+      if (now[h] >= 0) {
+        const int64_t row = ((static_cast<int64_t>(now[h]) * a.kv_heads + place.kv) << a.page_shift) +
+                            ((t * KT + 16 * h) & ((1 << a.page_shift) - 1));
+        const char* const k = reinterpret_cast<const char*>(a.k) + row * row_bytes;
+        const char* const v = reinterpret_cast<const char*>(a.v) + row * row_bytes;
+        if (all) {
+#pragma unroll
+          for (int u = 0; u < C / 2; ++u) {
+            lds_copy16(k + off[u], to + u * 1024);
+            lds_copy16(v + off[u], to + KT * T::PITCH + u * 1024);
+          }
+        } else {
+#pragma unroll
+          for (int u = 0; u < C / 2; ++u) {
+            if (off[u] == ~0u) continue;
+            lds_copy16(k + off[u], to + u * 1024);
+            lds_copy16(v + off[u], to + KT * T::PITCH + u * 1024);
+          }
+        }
+      } else {
+        // masked, and zero times them has to be zero
+        for (int i = lane; i < 16 * T::CPR; i += 64) {
+          reinterpret_cast<u32x4*>(to)[i] = u32x4{0u, 0u, 0u, 0u};
+          reinterpret_cast<u32x4*>(to + KT * T::PITCH)[i] = u32x4{0u, 0u, 0u, 0u};
+        }
+      }
+    }
+  };
+  fetch(first, 0);
+  const float scale2 = a.scale * kLog2e;
+  const int row = min(tile.row + (lane & 31), at.rows - 1), sees = at.sees(row, a.group, 1);
+  bf16x8 qf[DP / 16];
+  load_operand<DP>(a.q + (at.token + row / a.group) * a.q_stride + static_cast<int64_t>(place.kv * a.group + row % a.group) * a.dim, a.dim, qf);
+  RowState<DP> st;
+  st.clear();
+  int slot = 0, left_out = 0x7fffffff;
+#pragma unroll 1
+  for (int t = first; t < end; ++t) {
+    const char* const keys = smem + slot * SLOT;
+    const char* const values = keys + KT * T::PITCH;
+    slot ^= 1;
+    if (t + 1 < end) {
+      fetch(t + 1, slot);
+      // these may be on their way, if they are as many as those of a whole tile
+      if (valid_next == ~0u) dma_wait<2 * C>();
+      else dma_wait<0>();
+    } else {
+      valid = valid_next;
+      dma_wait<0>();
+    }
+    asm volatile("" ::: "memory");
+    const int j0 = t * KT;
+    if (j0 + KT > most) {  // what lies behind the sequence in its last page is masked too
+      for (int i = lane; i < KT * T::CPR; i += 64)
+        if (i / T::CPR >= most - j0) reinterpret_cast<u32x4*>(smem + (slot ^ 1) * SLOT + KT * T::PITCH)[i] = u32x4{0u, 0u, 0u, 0u};
+      asm volatile("" ::: "memory");
+    }
+    f32x16 s[1] = {MfmaBf16::zero()};
+#pragma unroll
+    for (int kk = 0; kk < DP / 16; ++kk) s[0] = MfmaBf16::mma(rows_fragment<DP>(keys, 0, kk), qf[kk], s[0]);
+    if (j0 + KT > fewest || valid != ~0u) hide(s, sees - j0, valid);
+    st.weigh(s, scale2);
+    // some rows do not see some of these keys
+    if (j0 + KT > fewest && fewest < most && (j0 >= left_out || any_not_finite<DP>(values))) {
+      left_out = min(left_out, j0);
+      continue;
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const bf16x8 w = weights_fragment(s[0], e);
+#pragma unroll
+      for (int d = 0; d < DP / 32; ++d) st.o[d] = MfmaBf16::mma(cols_fragment<DP>(values, 16 * e, 32 * d), w, st.o[d]);
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the slot has been read when the copies after the next one's go to it
+  }
+  // key j's row of a cache, j the same for all lanes, of a page that is one
+  const auto key_row = [&](const uint16_t* cache, int j) {
+    const int64_t r = ((static_cast<int64_t>(table[j >> a.page_shift]) * a.kv_heads + place.kv) << a.page_shift) + (j & ((1 << a.page_shift) - 1));
+    return cache + r * a.dim;
+  };
+#pragma unroll 1
+  for (int j = left_out; j < min(most, end * KT); ++j) {
+    if (static_cast<uint32_t>(table[j >> a.page_shift]) >= static_cast<uint64_t>(a.pages)) continue;
+    const float s = halves_sum(half_dot<DP>(qf, key_row(a.k, j), a.dim));
+    if (j >= sees) continue;
+    const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s, scale2, -(st.m == neg_inf() ? 0.0f : st.m)));
+    add_row<DP>(st.o, w, key_row(a.v, j), a.dim);
+  }
+  store_rows<DP>(a, st, at, tile.row, place.kv, place.split);
+}
+
+// Joins the splits: with M = max m, out = sum 2^(m - M) o / sum 2^(m - M) l.  A block has one row, each of its groups of 32 lanes
+// a share of the splits.
 __global__ __launch_bounds__(256) void attention_join(AttentionArgs a) {
+  __shared__ float sums[8][4][32], heads_l[8];
   const int64_t rows = a.seqs.n * a.group, all = rows * a.kv_heads;
-  const int64_t r = block_index() * 8 + (threadIdx.x >> 5);
+  const int64_t r = block_index();
   if (r >= all) return;
   const int kv = static_cast<int>(r / rows);
   const int64_t token = r % rows / a.group;
   const int head = kv * a.group + static_cast<int>(r % rows % a.group);
+  const int group = threadIdx.x >> 5, groups = blockDim.x >> 5, lane = threadIdx.x & 31, col = 4 * lane;
   float m = neg_inf();
-  for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.stats[s * all + r].x);
-  const int col = 4 * (threadIdx.x & 31);
+  for (int s = lane; s < a.splits; s += 32) m = fmaxf(m, a.stats[s * all + r].x);
+#pragma unroll
+  for (int i = 16; i >= 1; i >>= 1) m = fmaxf(m, __shfl_xor(m, i, 64));
   float v[4] = {0.0f, 0.0f, 0.0f, 0.0f}, l = 0.0f;
-  for (int s = 0; s < a.splits; ++s) {
+#pragma unroll 4
+  for (int s = group; s < a.splits; s += groups) {
     const float2 st = a.stats[s * all + r];
-    if (st.x == neg_inf()) continue;
-    const float by = __builtin_amdgcn_exp2f(st.x - m);
+    float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    const bool some = st.x != neg_inf();
+    if (some && col < a.dim) load_whole<VDSL_F32, 4>(a.parts, (s * all + r) * a.dim + col, o);
+    const float by = some ? __builtin_amdgcn_exp2f(st.x - m) : 0.0f;
     l += by * st.y;
-    if (col >= a.dim) continue;
-    float o[4];
-    load_whole<VDSL_F32, 4>(a.parts, (s * all + r) * a.dim + col, o);
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] += by * o[j];
+  }
+  if (groups > 1) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sums[group][j][lane] = v[j];
+    if (lane == 0) heads_l[group] = l;
+    __syncthreads();
+    if (group > 0) return;
+    for (int g = 1; g < groups; ++g) {
+      l += heads_l[g];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] += sums[g][j][lane];
+    }
   }
   const bool none = m == neg_inf();
   if (a.lse && col == 0) a.lse[head * a.seqs.n + token] = none ? neg_inf() : (m + __builtin_amdgcn_logf(l)) * kLn2;
@@ -469,15 +636,20 @@ __global__ __launch_bounds__(256) void cache_append_rows(AttentionArgs a, uint16
 
 bool float_type(int32_t t) { return t == VDSL_F32 || t == VDSL_BF16; }
 
+// `lanes` to a block, tiles of 2^log_tile rows.
+template <class Kernel>
+int launch_rows(vdsl_queue q, AttentionArgs& a, Kernel kernel, unsigned lanes, int log_tile, const char* name) {
+  const int64_t slots = row_slots(a.seqs.n, a.seqs.seqs, a.group, log_tile);
+  const int64_t blocks = slots * a.kv_heads * a.splits;
+  if (slots > 0x7fffffff || blocks > 0xffffff) return fail(VDSL_ERR_UNSUPPORTED, "attention: too many rows");
+  a.blocks = static_cast<int>(slots);
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(lanes), 0, q->stream, a);
+  return check_launch(name);
+}
 template <bool PAGED>
 int launch_rows(vdsl_queue q, AttentionArgs& a) {
-  const int64_t slots = row_slots(a.seqs.n, a.seqs.seqs, a.group, 7);
-  const int64_t blocks = slots * a.kv_heads * a.splits;
-  if (slots > 0x7fffffff || blocks > 0x7fffff) return fail(VDSL_ERR_UNSUPPORTED, "attention: too many rows");
-  a.blocks = static_cast<int>(slots);
-  const auto kernel = a.dim <= 64 ? attention_rows<64, PAGED> : a.dim <= 96 ? attention_rows<96, PAGED> : attention_rows<128, PAGED>;
-  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, q->stream, a);
-  return check_launch("attention_rows");
+  return launch_rows(q, a, a.dim <= 64 ? attention_rows<64, PAGED> : a.dim <= 96 ? attention_rows<96, PAGED> : attention_rows<128, PAGED>, 256, 7,
+                     "attention_rows");
 }
 
 }  // namespace
@@ -557,13 +729,21 @@ extern "C" int vdsl_op_attention_fwd(vdsl_queue q, const vdsl_attention_params* 
 
 namespace vdsl {
 namespace {
-// Splits of the keys: as many as make two blocks a CU, of 256 positions at least.
-int paged_splits(int64_t n, int64_t seqs, int32_t heads, int32_t kv_heads, int64_t positions) {
-  const int64_t group = heads / kv_heads;
-  const int64_t blocks = std::max<int64_t>(1, (n * group / 128 + std::min(seqs, n)) * kv_heads);
-  int splits = 1;
-  while (blocks * splits < 512 && splits < 32 && positions > 256 * splits) splits *= 2;
-  return splits;
+// How the rows' keys are split.  few: attention_few, where a sequence has up to 32 rows on average and pages are whole halves
+// of its tiles.
+struct PagedPlan {
+  bool few;
+  int splits;
+};
+PagedPlan paged_plan(int64_t n, int64_t seqs, int32_t heads, int32_t kv_heads, int64_t positions, int32_t page) {
+  const int64_t group = heads / kv_heads, with_rows = std::max<int64_t>(1, std::min(seqs, n));
+  PagedPlan plan = {n * group <= 32 * with_rows && page >= 16, 1};
+  const int64_t tiles = (n * group / (plan.few ? 32 : 128) + with_rows) * kv_heads;
+  // blocks: those of attention_few four times what the card holds, since sequences differ in length; attention_rows two a CU
+  const int64_t want = plan.few ? 5120 : 512, least = plan.few ? 64 : 256;
+  const int64_t splits = std::min<int64_t>({(want + tiles - 1) / tiles, positions / least, 256});
+  plan.splits = static_cast<int>(std::max<int64_t>(1, splits));
+  return plan;
 }
 int paged_check(const char* op, const vdsl_paged_params* p) {
   if (!p) return fail(VDSL_ERR_INVALID_ARG, "params is null");
@@ -629,7 +809,8 @@ extern "C" int vdsl_paged_attention_workspace_bytes(int64_t n, int64_t seqs, int
   if (!bytes) return fail(VDSL_ERR_INVALID_ARG, "bytes is null");
   VDSL_TRY(attention_check_shape("paged_attention", n, seqs, heads, kv_heads, dim));
   if (positions < 0) return fail(VDSL_ERR_INVALID_ARG, "negative shape");
-  const int splits = paged_splits(n, seqs, heads, kv_heads, positions);
+  // of either form
+  const int splits = std::max(paged_plan(n, seqs, heads, kv_heads, positions, 16).splits, paged_plan(n, seqs, heads, kv_heads, positions, 1).splits);
   *bytes = splits == 1 ? 0 : nbytes(n * heads, splits, 8 + 4 * static_cast<int64_t>(dim));
   return VDSL_OK;
 }
@@ -665,13 +846,18 @@ extern "C" int vdsl_op_paged_attention(vdsl_queue q, const vdsl_paged_params* p,
   a.out = out->ptr;
   a.out_dtype = out_dtype;
   a.lse = lse ? static_cast<float*>(lse->ptr) : nullptr;
-  a.splits = paged_splits(p->n, p->seqs, p->heads, p->kv_heads, positions);
+  const PagedPlan plan = paged_plan(p->n, p->seqs, p->heads, p->kv_heads, positions, p->page);
+  a.splits = plan.splits;
   if (a.splits > 1) {
     a.parts = static_cast<float*>(workspace->ptr);
     a.stats = reinterpret_cast<float2*>(a.parts + static_cast<int64_t>(a.splits) * p->n * p->heads * p->dim);
   }
-  VDSL_TRY(launch_rows<true>(q, a));
+  if (plan.few)
+    VDSL_TRY(launch_rows(q, a, a.dim <= 64 ? attention_few<64> : a.dim <= 96 ? attention_few<96> : attention_few<128>, 64, 5, "attention_few"));
+  else
+    VDSL_TRY(launch_rows<true>(q, a));
   if (a.splits == 1) return VDSL_OK;
-  hipLaunchKernelGGL(attention_join, block_grid((p->n * p->heads + 7) / 8), dim3(256), 0, q->stream, a);
+  const unsigned lanes = a.splits <= 4 ? 32 : a.splits <= 32 ? 128 : 256;
+  hipLaunchKernelGGL(attention_join, block_grid(p->n * p->heads), dim3(lanes), 0, q->stream, a);
   return check_launch("attention_join");
 }

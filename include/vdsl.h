@@ -763,8 +763,8 @@ int vdsl_op_attention_bwd(vdsl_queue q, const vdsl_attention_params* p, int32_t 
                           vdsl_buffer lse, int32_t grad_dtype, vdsl_buffer dq, vdsl_buffer dk, vdsl_buffer dv,
                           vdsl_buffer workspace);
 
-/* A cache of keys and values in pages: k_cache, v_cache BF16 [pages][kv_heads][page][dim] (page a power of two up to
- * 65536).  Position j of sequence s is slot j % page of page table[s][j / page] (I32 [seqs][table_cols]); an entry outside
+/* A cache of keys and values in pages: k_cache, v_cache BF16 [pages][kv_heads][page][dim] (page a power of two from 16
+ * to 65536).  Position j of sequence s is slot j % page of page table[s][j / page] (I32 [seqs][table_cols]); an entry outside
  * [0, pages) is no page: its positions hold nothing.  The new rows of sequence s are [starts[s], starts[s + 1]) (as for
  * vdsl_op_attention_fwd), m of them; lengths[s] (I32 [seqs]) counts its positions with the new rows: row i of them is
  * position lengths[s] - m + i.  Positions below 0 or not below table_cols * page hold nothing. */

@@ -169,9 +169,9 @@ def test_extreme_scores(q, own):
 
 
 # page, table's columns, lengths, new rows, heads, kv heads, dim, rows behind
-CACHES = [(16, 4, [20, 64, 1], [1, 1, 1], 4, 2, 64, 0), (1, 40, [40, 7, 0], [1, 1, 0], 2, 1, 128, 2), (64, 3, [130, 192, 64, 65], [1, 0, 1, 1], 8, 1, 80, 1),
+CACHES = [(16, 4, [20, 64, 1], [1, 1, 1], 4, 2, 64, 0), (16, 40, [40, 7, 0], [1, 1, 0], 2, 1, 128, 2), (64, 3, [130, 192, 64, 65], [1, 0, 1, 1], 8, 1, 80, 1),
           (16, 20, [300, 17], [40, 17], 4, 4, 128, 0), (256, 8, [2000, 1000, 5], [130, 1, 5], 8, 2, 128, 3), (32, 64, [2048], [1], 32, 8, 128, 0),
-          (8, 30, [200, 100], [200, 3], 6, 2, 40, 0), (64, 64, [4000, 3000], [600, 2], 16, 2, 96, 0), (16, 64, [1000] * 40, [1] * 40, 8, 2, 64, 0),
+          (32, 30, [200, 100], [200, 3], 6, 2, 40, 0), (64, 64, [4000, 3000], [600, 2], 16, 2, 96, 0), (16, 64, [1000] * 40, [1] * 40, 8, 2, 64, 0),
           (65536, 1, [700], [9], 1, 1, 8, 0)]
 
 
@@ -428,18 +428,19 @@ def test_refusals(dev, q, own):
     fwd(k=t["v"])  # inputs may share
     bwd(dq=kernels.Heads(over, heads, dim), dk=kernels.Heads(over, kv, dim, heads * dim), dv=kernels.Heads(over, kv, dim, (heads + kv) * dim))
 
-    kc, vc = own.put(np.ones((4, kv, 8, dim)), "bf16"), own.put(np.ones((4, kv, 8, dim)), "bf16")
+    kc, vc = own.put(np.ones((4, kv, 16, dim)), "bf16"), own.put(np.ones((4, kv, 16, dim)), "bf16")
     table, lengths = own.put(np.zeros((1, 4)), "i32"), own.put(np.array([n]), "i32")
-    need = kernels.paged_attention_workspace_bytes(n, 1, heads, kv, dim, 32)
+    need = kernels.paged_attention_workspace_bytes(n, 1, heads, kv, dim, 64)
     pws = own.scratch(need)
-    refused(UNSUPPORTED, kernels.cache_append, q, t["k"], t["v"], starts, lengths, table, own.put(np.ones((4, kv, 12, dim)), "bf16"),
-            own.put(np.ones((4, kv, 12, dim)), "bf16"))
+    for page in (24, 8, 1):  # no power of two, less than 16
+        refused(UNSUPPORTED, kernels.cache_append, q, t["k"], t["v"], starts, lengths, table, own.put(np.ones((4, kv, page, dim)), "bf16"),
+                own.put(np.ones((4, kv, page, dim)), "bf16"))
     refused(INVALID, kernels.cache_append, q, t["k"], t["v"], starts, lengths, table, kc, kc)
     refused(INVALID, kernels.paged_attention, q, t["q"], kc, vc, starts, lengths, table, t["q"].view((n, heads * dim)), workspace=pws)
     with pytest.raises(ValueError):
         kernels.cache_append(q, t["k"], t["v"], starts, lengths, own.put(np.zeros((2, 4)), "i32"), kc, vc)
     with pytest.raises(ValueError):
-        kernels.paged_attention(q, t["q"], kc, own.put(np.ones((4, kv, 16, dim)), "bf16"), starts, lengths, table, out, workspace=pws)
+        kernels.paged_attention(q, t["q"], kc, own.put(np.ones((4, kv, 32, dim)), "bf16"), starts, lengths, table, out, workspace=pws)
 
     x, y, pos = own.put(np.ones((4, 32)), "f32"), own.empty((4, 32), "bf16"), own.put(np.zeros(4), "i32")
     f = own.put(kernels.rope_frequencies(16), "f32")

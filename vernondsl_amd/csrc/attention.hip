@@ -30,75 +30,81 @@ struct AttentionArgs {
 
 constexpr float kLag = 8.0f;  // by how much m may lag, in powers of two
 
-// Keys of one sequence and kv head, as tiles of KT rows for copies of NW waves.
-template <int DP, int KT, int NW, bool PAGED>
+// Keys of one sequence and kv head, copied 16 at a time by one wave: from a scalar address and an offset that a lane keeps.
+// Paged: 16 positions lie in one page, whose entry in the table is read as constant memory, by a scalar load, so that no
+// copy is waited for with it.
+template <int DP, bool PAGED>
 struct KeySource {
   using T = TileShape<DP>;
-  static constexpr int C = KT * T::PITCH / 1024 / NW;  // copies of a wave for a tile's keys, and as many for its values
-  const char *k, *v;       // packed: of the sequence's first key; paged: the caches
-  uint32_t k_row, v_row;   // packed: bytes from a key to the next
-  int keys, head, kv_heads, dim, table_cols, shift;
-  int64_t pages;
-  const int32_t* table;    // the sequence's pages
-  int row_of[C], chunk[C];
+  typedef const __attribute__((address_space(4))) int32_t* ScalarTable;
+  static constexpr int C = 16 * T::PITCH / 1024;  // copies for 16 keys, and as many for their values
+  const char *k, *v;      // packed: of the sequence's first key; paged: of the caches
+  uint32_t k_row, v_row;  // bytes from a key to the next
+  uint32_t k_off[C], v_off[C];
+  int keys, head, kv_heads, shift;
+  uint32_t pages;
+  ScalarTable table;      // the sequence's pages
+  bool all;               // a head fills a row of LDS
 
-  __device__ __forceinline__ void lanes(int wave) {
+  __device__ __forceinline__ KeySource(const AttentionArgs& a, const RowTile& t, int sequence_keys, int kv)
+      : keys(sequence_keys), head(kv), kv_heads(a.kv_heads), shift(a.page_shift), pages(static_cast<uint32_t>(a.pages)), all(2 * a.dim == T::PITCH) {
+    if constexpr (PAGED) {
+      k = reinterpret_cast<const char*>(a.k);
+      v = reinterpret_cast<const char*>(a.v);
+      k_row = v_row = 2 * a.dim;
+      const int seq = __builtin_amdgcn_readfirstlane(static_cast<int>(t.seq < 0 ? 0 : t.seq));
+      table = (ScalarTable)(reinterpret_cast<uint64_t>(a.table)) + static_cast<int64_t>(seq) * a.table_cols;
+    } else {
+      k = reinterpret_cast<const char*>(a.k + t.token * a.k_stride + static_cast<int64_t>(kv) * a.dim);
+      v = reinterpret_cast<const char*>(a.v + t.token * a.v_stride + static_cast<int64_t>(kv) * a.dim);
+      k_row = static_cast<uint32_t>(2 * a.k_stride);
+      v_row = static_cast<uint32_t>(2 * a.v_stride);
+    }
     const int lane = threadIdx.x & 63;
 #pragma unroll
     for (int u = 0; u < C; ++u) {
-      row_of[u] = (wave * C + u) * (64 / T::CPR) + lane / T::CPR;
-      chunk[u] = lane % T::CPR ^ T::swz(row_of[u]);
+      const int r = u * (64 / T::CPR) + lane / T::CPR, c = lane % T::CPR ^ T::swz(r);
+      k_off[u] = c < a.dim / 8 ? static_cast<uint32_t>(r) * k_row + 16u * static_cast<uint32_t>(c) : ~0u;
+      v_off[u] = c < a.dim / 8 ? static_cast<uint32_t>(r) * v_row + 16u * static_cast<uint32_t>(c) : ~0u;
     }
   }
-  // Paged: this lane's entry of the page table for key j0 + lane (-1: none), loaded a tile before it is used.
-  __device__ __forceinline__ int entry(int j0) const {
-    const int j = j0 + (threadIdx.x & 63);
-    int e = -1;
-    if (j < keys) {
-      e = table[j >> shift];
-      if (static_cast<uint32_t>(e) >= static_cast<uint64_t>(pages)) e = -1;
+  // The page of keys j .. j + 15 (j the same for all lanes): -1 for none.  (Packed: 0.)
+  __device__ __forceinline__ int page(int j) const {
+    if (j >= keys) return -1;
+    if constexpr (!PAGED) return 0;
+    const int e = table[__builtin_amdgcn_readfirstlane(j) >> shift];
+    return static_cast<uint32_t>(e) < pages ? e : -1;
+  }
+  // How many of keys j .. j + 15 hold something, as that many bits.
+  __device__ __forceinline__ uint32_t there(int j, int e) const { return e < 0 ? 0u : keys - j >= 16 ? 0xFFFFu : (1u << (keys - j)) - 1u; }
+  // Key j's row of the keys or values at `base`, in page e.
+  __device__ __forceinline__ const char* row(const char* base, uint32_t bytes, int j, int e) const {
+    const int64_t at = PAGED ? ((static_cast<int64_t>(e) * kv_heads + head) << shift) + (j & ((1 << shift) - 1)) : j;
+    return base + at * bytes;
+  }
+  // Keys j .. j + 15 of page e to kt, their values to vt; those that hold nothing are zeros there.
+  __device__ __forceinline__ void copy(int j, int e, char* kt, char* vt) const {
+    const int last = e < 0 ? -1 : keys - 1 - j;
+    const char* const kb = row(k, k_row, j, e);
+    const char* const vb = row(v, v_row, j, e);
+    if (last >= 15 && all) {
+#pragma unroll
+      for (int u = 0; u < C; ++u) {
+        lds_copy16(kb + k_off[u], kt + u * 1024);
+        lds_copy16(vb + v_off[u], vt + u * 1024);
+      }
+      return;
     }
-    return e;
-  }
-  // Paged: key j's place among the caches' rows, in page e.
-  __device__ __forceinline__ int64_t place(int e, int j) const {
-    return ((static_cast<int64_t>(e) * kv_heads + head) << shift) + (j & ((1 << shift) - 1));
-  }
-  // The first element of key j's row of k (of v), j the same for all lanes, of a page that is one.
-  __device__ __forceinline__ const uint16_t* row(const char* base, uint32_t bytes, int j) const {
-    const int64_t at = PAGED ? place(table[j >> shift], j) : j;
-    return reinterpret_cast<const uint16_t*>(base + at * bytes);
-  }
-  // Tile j0 to the slot at `to` (its keys, then its values); keys past the last one and without a page are zeros there.
-  __device__ __forceinline__ void copy(int j0, int entries, char* to, int wave) const {
-    const int dc = dim / 8, last = keys - 1 - j0;
-    const bool whole = PAGED ? __all(entries >= 0) : last >= KT - 1;
+    const int lane = threadIdx.x & 63;
 #pragma unroll
     for (int u = 0; u < C; ++u) {
-      char* const kt = to + (wave * C + u) * 1024;
-      char* const vt = kt + KT * T::PITCH;
-      int64_t at = 0;
-      bool there = true;
-      if constexpr (PAGED) {
-        const int e = __shfl(entries, row_of[u], 64);
-        there = e >= 0;
-        at = place(e, j0 + row_of[u]);
+      if (k_off[u] == ~0u) continue;
+      if (u * (64 / T::CPR) + lane / T::CPR <= last) {
+        lds_copy16(kb + k_off[u], kt + u * 1024);
+        lds_copy16(vb + v_off[u], vt + u * 1024);
       } else {
-        there = row_of[u] <= last;
-      }
-      if (chunk[u] >= dc) continue;
-      if (whole || there) {
-        if constexpr (PAGED) {
-          lds_copy16(k + at * k_row + 16 * chunk[u], kt);
-          lds_copy16(v + at * v_row + 16 * chunk[u], vt);
-        } else {
-          lds_copy16(k + static_cast<int64_t>(j0) * k_row + (static_cast<uint32_t>(row_of[u]) * k_row + 16 * chunk[u]), kt);
-          lds_copy16(v + static_cast<int64_t>(j0) * v_row + (static_cast<uint32_t>(row_of[u]) * v_row + 16 * chunk[u]), vt);
-        }
-      } else {
-        const int lane = threadIdx.x & 63;
-        *reinterpret_cast<u32x4*>(kt + 16 * lane) = u32x4{0u, 0u, 0u, 0u};
-        *reinterpret_cast<u32x4*>(vt + 16 * lane) = u32x4{0u, 0u, 0u, 0u};
+        *reinterpret_cast<u32x4*>(kt + u * 1024 + 16 * lane) = u32x4{0u, 0u, 0u, 0u};
+        *reinterpret_cast<u32x4*>(vt + u * 1024 + 16 * lane) = u32x4{0u, 0u, 0u, 0u};
       }
     }
   }
@@ -249,28 +255,6 @@ __device__ __forceinline__ void store_none(const AttentionArgs& a, const RowsAt&
   }
 }
 
-template <bool PAGED, class Source>
-__device__ __forceinline__ void open_keys(const AttentionArgs& a, const RowTile& t, const RowsAt& at, int kv, Source& src) {
-  src.keys = at.keys;
-  src.head = kv;
-  src.kv_heads = a.kv_heads;
-  src.dim = a.dim;
-  src.table_cols = a.table_cols;
-  src.shift = a.page_shift;
-  src.pages = a.pages;
-  if constexpr (PAGED) {
-    src.k = reinterpret_cast<const char*>(a.k);
-    src.v = reinterpret_cast<const char*>(a.v);
-    src.k_row = src.v_row = 2 * a.dim;
-    src.table = a.table + (t.seq < 0 ? 0 : t.seq) * a.table_cols;
-  } else {
-    src.k = reinterpret_cast<const char*>(a.k + at.token * a.k_stride + static_cast<int64_t>(kv) * a.dim);
-    src.v = reinterpret_cast<const char*>(a.v + at.token * a.v_stride + static_cast<int64_t>(kv) * a.dim);
-    src.k_row = static_cast<uint32_t>(2 * a.k_stride);
-    src.v_row = static_cast<uint32_t>(2 * a.v_stride);
-  }
-}
-
 // The block's place: kv head, row slot and split.  Blocks that are dispatched together (to the XCDs in turn) have
 // different kv heads, so that an XCD reads few heads' keys where there are 8 or more; the last rows, which see most, first.
 struct Place {
@@ -308,27 +292,38 @@ __global__ __launch_bounds__(256, 2) void attention_rows(AttentionArgs a) {
     store_none(a, at, tile.row, ROWS, place.kv, place.split);
     return;
   }
-  KeySource<DP, KT, 4, PAGED> src;
-  open_keys<PAGED>(a, tile, at, place.kv, src);
-  src.lanes(wave);
+  const KeySource<DP, PAGED> src(a, tile, at.keys, place.kv);
   if (2 * a.dim < T::PITCH) {  // columns past dim are never copied
     for (int i = threadIdx.x; i < NS * SLOT / 16; i += 256) reinterpret_cast<u32x4*>(smem)[i] = u32x4{0u, 0u, 0u, 0u};
     __syncthreads();
   }
-  // Paged: which keys of a tile hold something (bits of the tiles in flight, the next one to be used last), and this lane's
-  // entry of the page table for the tile that is copied next.
-  uint64_t valid[NS] = {~0ull, ~0ull};
-  int entries = -1;
-  const auto fetch = [&](int t, int slot) {
-    if constexpr (PAGED) {
-      valid[1] = valid[0];
-      valid[0] = __ballot(entries >= 0);
-    }
-    src.copy(t * KT, entries, smem + slot * SLOT, wave);
+  // Paged: which keys of the tile and of the next one hold something, and the pages of that one.
+  uint64_t valid = ~0ull, valid_next = ~0ull;
+  int pages[4] = {0, 0, 0, 0};
+  const auto look = [&](int t) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) pages[i] = src.page(t * KT + 16 * i);
   };
-  if constexpr (PAGED) entries = src.entry(first * KT);
+  // Tile t to a slot, 16 keys by each wave.
+  const auto fetch = [&](int t, int slot) {
+    int e = 0;
+    valid = valid_next;
+    if constexpr (PAGED) {
+      valid_next = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        valid_next |= static_cast<uint64_t>(src.there(t * KT + 16 * i, pages[i])) << (16 * i);
+        if (wave == i) e = pages[i];
+      }
+      if (t + 1 < end) look(t + 1);
+    } else if (t * KT + 16 * wave >= at.keys) {
+      e = -1;
+    }
+    char* const to = smem + slot * SLOT + wave * 16 * T::PITCH;
+    src.copy(t * KT + 16 * wave, e, to, to + KT * T::PITCH);
+  };
+  if constexpr (PAGED) look(first);
   fetch(first, 0);
-  if constexpr (PAGED) entries = src.entry(min(first + 1, end - 1) * KT);
 
   const int row0 = tile.row + wave * 32;
   const bool mine = row0 < at.rows;
@@ -346,12 +341,8 @@ __global__ __launch_bounds__(256, 2) void attention_rows(AttentionArgs a) {
   const auto enter = [&]() {
     dma_wait<0>();
     dma_barrier();
-    if (t + 1 < end) {
-      fetch(t + 1, slot ^ 1);
-      if constexpr (PAGED) entries = src.entry(min(t + 2, end - 1) * KT);
-    } else if constexpr (PAGED) {
-      valid[1] = valid[0];
-    }
+    if (t + 1 < end) fetch(t + 1, slot ^ 1);
+    else valid = valid_next;
   };
   // tiles that all of the wave's rows see all of
 #pragma unroll 1
@@ -367,7 +358,7 @@ __global__ __launch_bounds__(256, 2) void attention_rows(AttentionArgs a) {
 #pragma unroll
       for (int kk = 0; kk < DP / 16; ++kk) s[k] = MfmaBf16::mma(rows_fragment<DP>(keys, 32 * k, kk), qf[kk], s[k]);
     }
-    if (PAGED && valid[1] != ~0ull) hide(s, KT, valid[1]);
+    if (PAGED && valid != ~0ull) hide(s, KT, valid);
     st.weigh(s, scale2);
 #pragma unroll
     for (int e = 0; e < 2 * KS; ++e) {
@@ -391,7 +382,7 @@ __global__ __launch_bounds__(256, 2) void attention_rows(AttentionArgs a) {
       f32x16 s[1] = {MfmaBf16::zero()};
 #pragma unroll
       for (int kk = 0; kk < DP / 16; ++kk) s[0] = MfmaBf16::mma(rows_fragment<DP>(keys, 32 * k, kk), qf[kk], s[0]);
-      hide(s, sees - j0, valid[1] >> (32 * k));
+      hide(s, sees - j0, PAGED ? valid >> (32 * k) : ~0ull);
       st.weigh(s, scale2);
       if (a.causal && (j0 >= left_out || any_not_finite<DP>(values + 32 * k * T::PITCH))) {
         left_out = min(left_out, j0);
@@ -407,24 +398,24 @@ __global__ __launch_bounds__(256, 2) void attention_rows(AttentionArgs a) {
   }
 #pragma unroll 1
   for (int j = left_out; j < min(most, end * KT); ++j) {
-    if (PAGED && static_cast<uint32_t>(src.table[j >> src.shift]) >= static_cast<uint64_t>(a.pages)) continue;
-    const float s = halves_sum(half_dot<DP>(qf, src.row(src.k, src.k_row, j), a.dim));
+    const int e = src.page(j);
+    if (e < 0) continue;
+    const float s = halves_sum(half_dot<DP>(qf, reinterpret_cast<const uint16_t*>(src.row(src.k, src.k_row, j, e)), a.dim));
     if (j >= sees) continue;
     const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s, scale2, -(st.m == neg_inf() ? 0.0f : st.m)));
-    add_row<DP>(st.o, w, src.row(src.v, src.v_row, j), a.dim);
+    add_row<DP>(st.o, w, reinterpret_cast<const uint16_t*>(src.row(src.v, src.v_row, j, e)), a.dim);
   }
   if (mine) store_rows<DP>(a, st, at, row0, place.kv, place.split);
 }
 
 // Few rows: a block is one wave with 32 rows and a split of the keys, in tiles of 32 through two slots of LDS of its own, so
 // that nothing waits for another wave.  What bounds it is the cache's bytes: five such blocks to a CU keep 80 KiB of them
-// on their way.  Pages of 16 positions or more: the halves of a tile lie in one page each, so a copy's address is a scalar
-// and an offset that a lane keeps.
+// on their way.
 template <int DP>
 __global__ __launch_bounds__(64, 2) void attention_few(AttentionArgs a) {
   constexpr int KT = 32;
   using T = TileShape<DP>;
-  constexpr int SLOT = 2 * KT * T::PITCH, C = KT * T::PITCH / 1024;  // copies of a tile's keys, and of its values
+  constexpr int SLOT = 2 * KT * T::PITCH;
   __shared__ __attribute__((aligned(1024))) char smem[2 * SLOT];
   const Place place(a);
   const RowTile tile = row_tile<5>(a.seqs, a.group, place.slot);
@@ -443,66 +434,20 @@ __global__ __launch_bounds__(64, 2) void attention_few(AttentionArgs a) {
   if (2 * a.dim < T::PITCH) {  // columns past dim are never copied
     for (int i = lane; i < 2 * SLOT / 16; i += 64) reinterpret_cast<u32x4*>(smem)[i] = u32x4{0u, 0u, 0u, 0u};
   }
-  // as constant memory: scalar loads, which no copy is waited for with
-  typedef const __attribute__((address_space(4))) int32_t* ScalarTable;
-  const int64_t seq = tile.seq < 0 ? 0 : tile.seq;
-  const ScalarTable table = (ScalarTable)(reinterpret_cast<uint64_t>(a.table)) +
-                            (static_cast<int64_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(seq))) * a.table_cols);
-  const uint32_t row_bytes = 2 * static_cast<uint32_t>(a.dim);
-  uint32_t off[C / 2];
-#pragma unroll
-  for (int u = 0; u < C / 2; ++u) {
-    const int r = u * (64 / T::CPR) + lane / T::CPR, c = lane % T::CPR ^ T::swz(r);
-    off[u] = c < a.dim / 8 ? static_cast<uint32_t>(r) * row_bytes + 16u * static_cast<uint32_t>(c) : ~0u;
-  }
-  const bool all = 2 * a.dim == T::PITCH;
-  // The pages of a tile's halves.
-  const auto entry = [&](int t, int half) {
-    const int j = __builtin_amdgcn_readfirstlane(t * KT + 16 * half);
-    if (j >= most) return -1;
-    const int e = table[j >> a.page_shift];
-    return static_cast<uint32_t>(e) < static_cast<uint64_t>(a.pages) ? e : -1;
-  };
-  int page0 = entry(first, 0), page1 = entry(first, 1);
+  const KeySource<DP, true> src(a, tile, most, place.kv);
+  int page0 = src.page(first * KT), page1 = src.page(first * KT + 16);
   uint32_t valid = 0u, valid_next = 0u;  // which keys of the tile and of the next one hold something
   const auto fetch = [&](int t, int slot) {
-    const int now[2] = {page0, page1};
+    const int e0 = page0, e1 = page1, j = t * KT;
     if (t + 1 < end) {
-      page0 = entry(t + 1, 0);
-      page1 = entry(t + 1, 1);
+      page0 = src.page(j + KT);
+      page1 = src.page(j + KT + 16);
     }
     valid = valid_next;
-    valid_next = (now[0] >= 0 ? 0xFFFFu : 0u) | (now[1] >= 0 ? 0xFFFF0000u : 0u);
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      char* const to = smem + slot * SLOT + h * 16 * T::PITCH;
-      if (now[h] >= 0) {
-        const int64_t row = ((static_cast<int64_t>(now[h]) * a.kv_heads + place.kv) << a.page_shift) +
-                            ((t * KT + 16 * h) & ((1 << a.page_shift) - 1));
-        const char* const k = reinterpret_cast<const char*>(a.k) + row * row_bytes;
-        const char* const v = reinterpret_cast<const char*>(a.v) + row * row_bytes;
-        if (all) {
-#pragma unroll
-          for (int u = 0; u < C / 2; ++u) {
-            lds_copy16(k + off[u], to + u * 1024);
-            lds_copy16(v + off[u], to + KT * T::PITCH + u * 1024);
-          }
-        } else {
-#pragma unroll
-          for (int u = 0; u < C / 2; ++u) {
-            if (off[u] == ~0u) continue;
-            lds_copy16(k + off[u], to + u * 1024);
-            lds_copy16(v + off[u], to + KT * T::PITCH + u * 1024);
-          }
-        }
-      } else {
-        // masked, and zero times them has to be zero
-        for (int i = lane; i < 16 * T::CPR; i += 64) {
-          reinterpret_cast<u32x4*>(to)[i] = u32x4{0u, 0u, 0u, 0u};
-          reinterpret_cast<u32x4*>(to + KT * T::PITCH)[i] = u32x4{0u, 0u, 0u, 0u};
-        }
-      }
-    }
+    valid_next = src.there(j, e0) | src.there(j + 16, e1) << 16;
+    char* const to = smem + slot * SLOT;
+    src.copy(j, e0, to, to + KT * T::PITCH);
+    src.copy(j + 16, e1, to + 16 * T::PITCH, to + (KT + 16) * T::PITCH);
   };
   fetch(first, 0);
   const float scale2 = a.scale * kLog2e;
@@ -520,7 +465,7 @@ __global__ __launch_bounds__(64, 2) void attention_few(AttentionArgs a) {
     if (t + 1 < end) {
       fetch(t + 1, slot);
       // these may be on their way, if they are as many as those of a whole tile
-      if (valid_next == ~0u) dma_wait<2 * C>();
+      if (valid_next == ~0u) dma_wait<4 * KeySource<DP, true>::C>();
       else dma_wait<0>();
     } else {
       valid = valid_next;
@@ -528,11 +473,6 @@ __global__ __launch_bounds__(64, 2) void attention_few(AttentionArgs a) {
     }
     asm volatile("" ::: "memory");
     const int j0 = t * KT;
-    if (j0 + KT > most) {  // what lies behind the sequence in its last page is masked too
-      for (int i = lane; i < KT * T::CPR; i += 64)
-        if (i / T::CPR >= most - j0) reinterpret_cast<u32x4*>(smem + (slot ^ 1) * SLOT + KT * T::PITCH)[i] = u32x4{0u, 0u, 0u, 0u};
-      asm volatile("" ::: "memory");
-    }
     f32x16 s[1] = {MfmaBf16::zero()};
 #pragma unroll
     for (int kk = 0; kk < DP / 16; ++kk) s[0] = MfmaBf16::mma(rows_fragment<DP>(keys, 0, kk), qf[kk], s[0]);
@@ -551,18 +491,14 @@ __global__ __launch_bounds__(64, 2) void attention_few(AttentionArgs a) {
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the slot has been read when the copies after the next one's go to it
   }
-  // key j's row of a cache, j the same for all lanes, of a page that is one
-  const auto key_row = [&](const uint16_t* cache, int j) {
-    const int64_t r = ((static_cast<int64_t>(table[j >> a.page_shift]) * a.kv_heads + place.kv) << a.page_shift) + (j & ((1 << a.page_shift) - 1));
-    return cache + r * a.dim;
-  };
 #pragma unroll 1
   for (int j = left_out; j < min(most, end * KT); ++j) {
-    if (static_cast<uint32_t>(table[j >> a.page_shift]) >= static_cast<uint64_t>(a.pages)) continue;
-    const float s = halves_sum(half_dot<DP>(qf, key_row(a.k, j), a.dim));
+    const int e = src.page(j);
+    if (e < 0) continue;
+    const float s = halves_sum(half_dot<DP>(qf, reinterpret_cast<const uint16_t*>(src.row(src.k, src.k_row, j, e)), a.dim));
     if (j >= sees) continue;
     const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s, scale2, -(st.m == neg_inf() ? 0.0f : st.m)));
-    add_row<DP>(st.o, w, key_row(a.v, j), a.dim);
+    add_row<DP>(st.o, w, reinterpret_cast<const uint16_t*>(src.row(src.v, src.v_row, j, e)), a.dim);
   }
   store_rows<DP>(a, st, at, tile.row, place.kv, place.split);
 }
@@ -729,15 +665,14 @@ extern "C" int vdsl_op_attention_fwd(vdsl_queue q, const vdsl_attention_params* 
 
 namespace vdsl {
 namespace {
-// How the rows' keys are split.  few: attention_few, where a sequence has up to 32 rows on average and pages are whole halves
-// of its tiles.
+// How the rows' keys are split.  few: attention_few, where a sequence has up to 32 rows on average.
 struct PagedPlan {
   bool few;
   int splits;
 };
-PagedPlan paged_plan(int64_t n, int64_t seqs, int32_t heads, int32_t kv_heads, int64_t positions, int32_t page) {
+PagedPlan paged_plan(int64_t n, int64_t seqs, int32_t heads, int32_t kv_heads, int64_t positions) {
   const int64_t group = heads / kv_heads, with_rows = std::max<int64_t>(1, std::min(seqs, n));
-  PagedPlan plan = {n * group <= 32 * with_rows && page >= 16, 1};
+  PagedPlan plan = {n * group <= 32 * with_rows, 1};
   const int64_t tiles = (n * group / (plan.few ? 32 : 128) + with_rows) * kv_heads;
   // blocks: those of attention_few four times what the card holds, since sequences differ in length; attention_rows two a CU
   const int64_t want = plan.few ? 5120 : 512, least = plan.few ? 64 : 256;
@@ -749,7 +684,8 @@ int paged_check(const char* op, const vdsl_paged_params* p) {
   if (!p) return fail(VDSL_ERR_INVALID_ARG, "params is null");
   VDSL_TRY(attention_check_shape(op, p->n, p->seqs, p->heads, p->kv_heads, p->dim));
   if (p->pages < 0 || p->table_cols < 0 || p->page <= 0) return fail(VDSL_ERR_INVALID_ARG, std::string(op) + ": negative shape or no page size");
-  if ((p->page & (p->page - 1)) || p->page > 65536) return fail(VDSL_ERR_UNSUPPORTED, std::string(op) + ": page must be a power of two up to 65536");
+  if ((p->page & (p->page - 1)) || p->page < 16 || p->page > 65536)
+    return fail(VDSL_ERR_UNSUPPORTED, std::string(op) + ": page must be a power of two from 16 to 65536");
   if (p->pages > 0x7fffffff || p->table_cols > 0x7fffffff / p->page)
     return fail(VDSL_ERR_UNSUPPORTED, std::string(op) + ": 2^31 positions a sequence or more");
   return VDSL_OK;
@@ -809,8 +745,7 @@ extern "C" int vdsl_paged_attention_workspace_bytes(int64_t n, int64_t seqs, int
   if (!bytes) return fail(VDSL_ERR_INVALID_ARG, "bytes is null");
   VDSL_TRY(attention_check_shape("paged_attention", n, seqs, heads, kv_heads, dim));
   if (positions < 0) return fail(VDSL_ERR_INVALID_ARG, "negative shape");
-  // of either form
-  const int splits = std::max(paged_plan(n, seqs, heads, kv_heads, positions, 16).splits, paged_plan(n, seqs, heads, kv_heads, positions, 1).splits);
+  const int splits = paged_plan(n, seqs, heads, kv_heads, positions).splits;
   *bytes = splits == 1 ? 0 : nbytes(n * heads, splits, 8 + 4 * static_cast<int64_t>(dim));
   return VDSL_OK;
 }
@@ -846,7 +781,7 @@ extern "C" int vdsl_op_paged_attention(vdsl_queue q, const vdsl_paged_params* p,
   a.out = out->ptr;
   a.out_dtype = out_dtype;
   a.lse = lse ? static_cast<float*>(lse->ptr) : nullptr;
-  const PagedPlan plan = paged_plan(p->n, p->seqs, p->heads, p->kv_heads, positions, p->page);
+  const PagedPlan plan = paged_plan(p->n, p->seqs, p->heads, p->kv_heads, positions);
   a.splits = plan.splits;
   if (a.splits > 1) {
     a.parts = static_cast<float*>(workspace->ptr);

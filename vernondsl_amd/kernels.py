@@ -665,7 +665,7 @@ def _paged_params(n, dim, kv_heads, heads, scale, starts, lengths, table, k_cach
 
 def cache_append(q: Queue, k, v, starts: Tensor, lengths: Tensor, table: Tensor, k_cache: Tensor, v_cache: Tensor):
     """The new rows' k and v (bf16 Heads or tensors [n][kv_heads][dim]) into their slots of the paged caches (bf16
-    [pages][kv_heads][page][dim], page a power of two): row i of the m new rows starts[s] to starts[s + 1] of sequence s is
+    [pages][kv_heads][page][dim], page a power of two from 16 on): row i of the m new rows starts[s] to starts[s + 1] of sequence s is
     position p = lengths[s] - m + i, slot p % page of page table[s][p / page] (i32; lengths counts the new rows).  Rows without
     a page are dropped."""
     k, v = _heads(k, "k"), _heads(v, "v")

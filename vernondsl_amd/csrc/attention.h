@@ -122,6 +122,52 @@ __device__ __forceinline__ void load_operand(const uint16_t* p, int dim, bf16x8 
   }
 }
 
+// A wave's copies of ROWS rows of two operands to LDS: from scalar addresses and offsets that a lane keeps.
+template <int DP, int ROWS>
+struct RowCopies {
+  using T = TileShape<DP>;
+  static constexpr int C = ROWS * T::PITCH / 1024;  // copies of an operand
+  static_assert(C * 1024 == ROWS * T::PITCH, "a wave copies 1 KiB at a time");
+  uint32_t a_off[C], b_off[C];  // ~0: a column past the head's
+  bool all;                     // a head fills a row of LDS
+
+  static __device__ __forceinline__ int row_of(int u) { return u * (64 / T::CPR) + static_cast<int>(threadIdx.x & 63) / T::CPR; }
+  // at_a, at_b: bytes from the operand's first row to row r; row0: the place of that one in its tile.
+  template <class AtA, class AtB>
+  __device__ __forceinline__ void offsets(int row0, int dim, AtA&& at_a, AtB&& at_b) {
+    all = 2 * dim == T::PITCH;
+#pragma unroll
+    for (int u = 0; u < C; ++u) {
+      const int r = row_of(u), c = static_cast<int>(threadIdx.x & 63) % T::CPR ^ T::swz(row0 + r);
+      a_off[u] = c < dim / 8 ? at_a(r) + 16u * static_cast<uint32_t>(c) : ~0u;
+      b_off[u] = c < dim / 8 ? at_b(r) + 16u * static_cast<uint32_t>(c) : ~0u;
+    }
+  }
+  // Rows 0 .. last; those behind are zeros.
+  __device__ __forceinline__ void copy(const char* a, const char* b, int last, char* to_a, char* to_b) const {
+    if (last >= ROWS - 1 && all) {
+#pragma unroll
+      for (int u = 0; u < C; ++u) {
+        lds_copy16(a + a_off[u], to_a + u * 1024);
+        lds_copy16(b + b_off[u], to_b + u * 1024);
+      }
+      return;
+    }
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int u = 0; u < C; ++u) {
+      if (a_off[u] == ~0u) continue;
+      if (row_of(u) <= last) {
+        lds_copy16(a + a_off[u], to_a + u * 1024);
+        lds_copy16(b + b_off[u], to_b + u * 1024);
+      } else {
+        *reinterpret_cast<u32x4*>(to_a + u * 1024 + 16 * lane) = u32x4{0u, 0u, 0u, 0u};
+        *reinterpret_cast<u32x4*>(to_b + u * 1024 + 16 * lane) = u32x4{0u, 0u, 0u, 0u};
+      }
+    }
+  }
+};
+
 // The values of lanes l % 32 and l % 32 + 32, in every lane.
 __device__ __forceinline__ f32x2_t both_halves(float v) {
   const uint32_t b = __builtin_bit_cast(uint32_t, v);

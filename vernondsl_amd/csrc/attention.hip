@@ -37,17 +37,16 @@ template <int DP, bool PAGED>
 struct KeySource {
   using T = TileShape<DP>;
   typedef const __attribute__((address_space(4))) int32_t* ScalarTable;
-  static constexpr int C = 16 * T::PITCH / 1024;  // copies for 16 keys, and as many for their values
+  static constexpr int C = RowCopies<DP, 16>::C;  // copies for 16 keys, and as many for their values
   const char *k, *v;      // packed: of the sequence's first key; paged: of the caches
   uint32_t k_row, v_row;  // bytes from a key to the next
-  uint32_t k_off[C], v_off[C];
+  RowCopies<DP, 16> copies;
   int keys, head, kv_heads, shift;
   uint32_t pages;
   ScalarTable table;      // the sequence's pages
-  bool all;               // a head fills a row of LDS
 
   __device__ __forceinline__ KeySource(const AttentionArgs& a, const RowTile& t, int sequence_keys, int kv)
-      : keys(sequence_keys), head(kv), kv_heads(a.kv_heads), shift(a.page_shift), pages(static_cast<uint32_t>(a.pages)), all(2 * a.dim == T::PITCH) {
+      : keys(sequence_keys), head(kv), kv_heads(a.kv_heads), shift(a.page_shift), pages(static_cast<uint32_t>(a.pages)) {
     if constexpr (PAGED) {
       k = reinterpret_cast<const char*>(a.k);
       v = reinterpret_cast<const char*>(a.v);
@@ -60,13 +59,7 @@ struct KeySource {
       k_row = static_cast<uint32_t>(2 * a.k_stride);
       v_row = static_cast<uint32_t>(2 * a.v_stride);
     }
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int u = 0; u < C; ++u) {
-      const int r = u * (64 / T::CPR) + lane / T::CPR, c = lane % T::CPR ^ T::swz(r);
-      k_off[u] = c < a.dim / 8 ? static_cast<uint32_t>(r) * k_row + 16u * static_cast<uint32_t>(c) : ~0u;
-      v_off[u] = c < a.dim / 8 ? static_cast<uint32_t>(r) * v_row + 16u * static_cast<uint32_t>(c) : ~0u;
-    }
+    copies.offsets(0, a.dim, [&](int r) { return static_cast<uint32_t>(r) * k_row; }, [&](int r) { return static_cast<uint32_t>(r) * v_row; });
   }
   // The page of keys j .. j + 15 (j the same for all lanes): -1 for none.  (Packed: 0.)
   __device__ __forceinline__ int page(int j) const {
@@ -84,29 +77,7 @@ struct KeySource {
   }
   // Keys j .. j + 15 of page e to kt, their values to vt; those that hold nothing are zeros there.
   __device__ __forceinline__ void copy(int j, int e, char* kt, char* vt) const {
-    const int last = e < 0 ? -1 : keys - 1 - j;
-    const char* const kb = row(k, k_row, j, e);
-    const char* const vb = row(v, v_row, j, e);
-    if (last >= 15 && all) {
-#pragma unroll
-      for (int u = 0; u < C; ++u) {
-        lds_copy16(kb + k_off[u], kt + u * 1024);
-        lds_copy16(vb + v_off[u], vt + u * 1024);
-      }
-      return;
-    }
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int u = 0; u < C; ++u) {
-      if (k_off[u] == ~0u) continue;
-      if (u * (64 / T::CPR) + lane / T::CPR <= last) {
-        lds_copy16(kb + k_off[u], kt + u * 1024);
-        lds_copy16(vb + v_off[u], vt + u * 1024);
-      } else {
-        *reinterpret_cast<u32x4*>(kt + u * 1024 + 16 * lane) = u32x4{0u, 0u, 0u, 0u};
-        *reinterpret_cast<u32x4*>(vt + u * 1024 + 16 * lane) = u32x4{0u, 0u, 0u, 0u};
-      }
-    }
+    copies.copy(row(k, k_row, j, e), row(v, v_row, j, e), e < 0 ? -1 : keys - 1 - j, kt, vt);
   }
 };
 

@@ -82,49 +82,6 @@ __device__ __forceinline__ void store_zeros(int dtype, void* to, int64_t e, int 
   for (int c = 0; c < cols; c += 4) store_unit<4>(dtype, to, e + c, none);
 }
 
-// Tiles of TR rows of two operands for copies of NW waves.
-template <int DP, int TR, int NW>
-struct PairCopies {
-  using T = TileShape<DP>;
-  static constexpr int C = TR * T::PITCH / 1024 / NW, SLOT = 2 * TR * T::PITCH;
-  int row_of[C], chunk[C];
-  __device__ __forceinline__ PairCopies(int wave) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int u = 0; u < C; ++u) {
-      row_of[u] = (wave * C + u) * (64 / T::CPR) + lane / T::CPR;
-      chunk[u] = lane % T::CPR ^ T::swz(row_of[u]);
-    }
-  }
-  // Rows 0 .. last of a tile; those behind are zeros.  at(row of the tile, which operand): that row's first byte.
-  template <class At>
-  __device__ __forceinline__ void operator()(char* to, int wave, int dim, int last, At&& at) const {
-    if (last >= TR - 1) {
-#pragma unroll
-      for (int u = 0; u < C; ++u) {
-        if (chunk[u] >= dim / 8) continue;
-        lds_copy16(at(row_of[u], 0) + 16 * chunk[u], to + (wave * C + u) * 1024);
-        lds_copy16(at(row_of[u], 1) + 16 * chunk[u], to + TR * T::PITCH + (wave * C + u) * 1024);
-      }
-      return;
-    }
-#pragma unroll 1
-    for (int u = 0; u < C; ++u) {
-      const int lane = threadIdx.x & 63, row = (wave * C + u) * (64 / T::CPR) + lane / T::CPR, c = lane % T::CPR ^ T::swz(row);
-      if (c >= dim / 8) continue;
-      char* const first = to + (wave * C + u) * 1024;
-      char* const second = first + TR * T::PITCH;
-      if (row <= last) {
-        lds_copy16(at(row, 0) + 16 * c, first);
-        lds_copy16(at(row, 1) + 16 * c, second);
-      } else {
-        *reinterpret_cast<u32x4*>(first + 16 * lane) = u32x4{0u, 0u, 0u, 0u};
-        *reinterpret_cast<u32x4*>(second + 16 * lane) = u32x4{0u, 0u, 0u, 0u};
-      }
-    }
-  }
-};
-
 // dk and dv: a block has 128 keys and walks over tiles of 64 rows through a ring of three slots of LDS.  Each 32 keys have two waves, one
 // for each half of a tile's rows, which add up their sums at the end; both are on one SIMD, and the first has priority
 // there, so that its exponentials come beside the other's products.  To leave both their registers, wide heads'
@@ -134,9 +91,9 @@ __global__ __launch_bounds__(512, 2) void attention_bwd_keys(GradArgs a) {
   constexpr int TR = 64, NW = 8;
   constexpr bool V_LDS = DP > 96;
   using T = TileShape<DP>;
-  using Copies = PairCopies<DP, TR, NW>;
+  using Copies = RowCopies<DP, 8>;  // of a tile's rows by each wave
   constexpr int SUMS = 4 * 32 * DP * 4;  // one gradient's sums of four waves
-  constexpr int NS = 3, AREA = NS * Copies::SLOT + (V_LDS ? 128 * T::PITCH : 0);
+  constexpr int NS = 3, SLOT = 2 * TR * T::PITCH, AREA = NS * SLOT + (V_LDS ? 128 * T::PITCH : 0);
   __shared__ __attribute__((aligned(1024))) char smem[AREA > SUMS ? AREA : SUMS];
   __shared__ __attribute__((aligned(16))) float starts[NW][NS][2][32];  // what the rows' scores and dp start from, a copy a wave
   int b = static_cast<int>(blockIdx.x);
@@ -158,16 +115,15 @@ __global__ __launch_bounds__(512, 2) void attention_bwd_keys(GradArgs a) {
     }
     return;
   }
-  const Copies copies(wave);
   if (2 * a.dim < T::PITCH) {
-    for (int i = threadIdx.x; i < NS * Copies::SLOT / 16; i += 512) reinterpret_cast<u32x4*>(smem)[i] = u32x4{0u, 0u, 0u, 0u};
+    for (int i = threadIdx.x; i < NS * SLOT / 16; i += 512) reinterpret_cast<u32x4*>(smem)[i] = u32x4{0u, 0u, 0u, 0u};
     __syncthreads();
   }
   const int64_t token = tile.token + min(key, tile.len - 1);
   bf16x8 kf[DP / 16], vf[DP / 16];
   load_operand<DP>(a.k + token * a.k_stride + head_col, a.dim, kf);
   load_operand<DP>(a.v + token * a.v_stride + head_col, a.dim, vf);
-  char* const values = smem + NS * Copies::SLOT + (wave & 3) * 32 * T::PITCH;  // both waves write the same
+  char* const values = smem + NS * SLOT + (wave & 3) * 32 * T::PITCH;  // both waves write the same
   if constexpr (V_LDS) {
 #pragma unroll
     for (int kk = 0; kk < DP / 16; ++kk)
@@ -179,14 +135,22 @@ __global__ __launch_bounds__(512, 2) void attention_bwd_keys(GradArgs a) {
   const char* const dp = reinterpret_cast<const char*>(a.dout + tile.token * a.dout_stride + head_col * a.group);
   const float* const sp = a.rows + (static_cast<int64_t>(kv) * a.seqs.n + tile.token) * a.group;
   const int64_t delta_at = a.seqs.n * a.heads;
-  // The copies of tile t.
+  // The copies of tile t.  Their offsets are the same for all tiles if 8 rows are whole tokens.
+  Copies copies;
+  const auto offsets = [&](int row0, int token0) {
+    const auto at = [&](int r, int64_t stride) {
+      const int i = a.token_of(row0 + r);
+      return 2u * (static_cast<uint32_t>(i - token0) * static_cast<uint32_t>(stride) + static_cast<uint32_t>((row0 + r - i * a.group) * a.dim));
+    };
+    copies.offsets(8 * wave, a.dim, [&](int r) { return at(r, a.q_stride); }, [&](int r) { return at(r, a.dout_stride); });
+  };
+  const bool whole_tokens = 8 % a.group == 0;
+  if (whole_tokens) offsets(0, 0);
   const auto fetch = [&](int t, int slot) {
-    const int last = rows - 1 - t * TR;
-    copies(smem + slot * Copies::SLOT, wave, a.dim, last, [&](int r, int which) {
-      const int row = t * TR + r, i = a.token_of(row);
-      const int64_t col = static_cast<int64_t>(row - i * a.group) * a.dim;
-      return which == 0 ? qp + 2 * (i * a.q_stride + col) : dp + 2 * (i * a.dout_stride + col);
-    });
+    const int last = rows - 1 - t * TR, row0 = t * TR + 8 * wave, token0 = a.token_of(row0);
+    if (!whole_tokens) offsets(row0, token0);
+    char* const area = smem + slot * SLOT + 8 * wave * T::PITCH;
+    copies.copy(qp + 2 * (token0 * a.q_stride), dp + 2 * (token0 * a.dout_stride), last - 8 * wave, area, area + TR * T::PITCH);
     float* const to = starts[wave][slot][0];
     const int r = 32 * part + (lane & 31);
     // rows that are not there: no weight
@@ -213,7 +177,7 @@ __global__ __launch_bounds__(512, 2) void attention_bwd_keys(GradArgs a) {
     else dma_wait<0>();
     dma_barrier();
     if (t - 2 >= first) fetch(t - 2, slot == 0 ? 2 : slot - 1);
-    const char* const qs = smem + slot * Copies::SLOT + part * 32 * T::PITCH;
+    const char* const qs = smem + slot * SLOT + part * 32 * T::PITCH;
     const char* const ds = qs + TR * T::PITCH;
     const float* const x = starts[wave][slot][0] + 4 * half;
     slot = slot == 2 ? 0 : slot + 1;
@@ -362,8 +326,9 @@ template <int DP>
 __global__ __launch_bounds__(256, 2) void attention_bwd_queries(GradArgs a) {
   constexpr int KT = 64, ROWS = 128;
   using T = TileShape<DP>;
-  using Copies = PairCopies<DP, KT, 4>;
-  __shared__ __attribute__((aligned(1024))) char smem[2 * Copies::SLOT];
+  using Copies = RowCopies<DP, 16>;  // of a tile's keys by each wave
+  constexpr int SLOT = 2 * KT * T::PITCH;
+  __shared__ __attribute__((aligned(1024))) char smem[2 * SLOT];
   int b = static_cast<int>(blockIdx.x);
   const int kv = b % a.kv_heads;
   const RowTile tile = row_tile<7>(a.seqs, a.group, a.blocks - 1 - b / a.kv_heads);
@@ -380,20 +345,21 @@ __global__ __launch_bounds__(256, 2) void attention_bwd_queries(GradArgs a) {
       store_zeros(a.grad_dtype, a.dq, dq_at(row), a.dim);
     return;
   }
-  const Copies copies(wave);
   if (2 * a.dim < T::PITCH) {
-    for (int i = threadIdx.x; i < 2 * Copies::SLOT / 16; i += 256) reinterpret_cast<u32x4*>(smem)[i] = u32x4{0u, 0u, 0u, 0u};
+    for (int i = threadIdx.x; i < 2 * SLOT / 16; i += 256) reinterpret_cast<u32x4*>(smem)[i] = u32x4{0u, 0u, 0u, 0u};
     __syncthreads();
   }
   const auto sees = [&](int row) { return a.causal ? a.token_of(row) + 1 : tile.len; };
   const int end = (sees(min(tile.row + ROWS, rows) - 1) + KT - 1) / KT;
   const char* const kp = reinterpret_cast<const char*>(a.k + tile.token * a.k_stride + head_col);
   const char* const vp = reinterpret_cast<const char*>(a.v + tile.token * a.v_stride + head_col);
+  Copies copies;
+  copies.offsets(0, a.dim, [&](int r) { return 2u * static_cast<uint32_t>(r) * static_cast<uint32_t>(a.k_stride); },
+                 [&](int r) { return 2u * static_cast<uint32_t>(r) * static_cast<uint32_t>(a.v_stride); });
   const auto fetch = [&](int t, int slot) {
-    copies(smem + slot * Copies::SLOT, wave, a.dim, tile.len - 1 - t * KT, [&](int r, int which) {
-      const int64_t i = t * KT + r;
-      return which == 0 ? kp + 2 * i * a.k_stride : vp + 2 * i * a.v_stride;
-    });
+    const int j = t * KT + 16 * wave;
+    char* const area = smem + slot * SLOT + 16 * wave * T::PITCH;
+    copies.copy(kp + 2 * (j * a.k_stride), vp + 2 * (j * a.v_stride), tile.len - 1 - j, area, area + KT * T::PITCH);
   };
   fetch(0, 0);
   const bool mine = row0 < rows;
@@ -443,7 +409,7 @@ __global__ __launch_bounds__(256, 2) void attention_bwd_queries(GradArgs a) {
 #pragma unroll 1
   for (const int whole = min(end, fewest / KT); t < whole; ++t) {
     enter();
-    const char* const ks = smem + slot * Copies::SLOT;
+    const char* const ks = smem + slot * SLOT;
     slot ^= 1;
 #pragma unroll 1
     for (int u = 0; u < KT / 32; ++u) add(ks + 32 * u * T::PITCH, form(ks + 32 * u * T::PITCH, nullptr));
@@ -452,7 +418,7 @@ __global__ __launch_bounds__(256, 2) void attention_bwd_queries(GradArgs a) {
 #pragma unroll 1
   for (; t < end; ++t) {
     enter();
-    const char* ks = smem + slot * Copies::SLOT;
+    const char* ks = smem + slot * SLOT;
     slot ^= 1;
 #pragma unroll 1
     for (int u = 0; u < KT / 32; ++u, ks += 32 * T::PITCH) {

@@ -32,29 +32,32 @@ struct GradArgs {
   int blocks;
 };
 
-// What a row's scores and dp start from, -lse / scale and -delta, and dout in bf16 where it is f32.  32 lanes a row.
+// What a row's scores and dp start from, -lse / scale and -delta, and dout in bf16 where it is f32.  16 lanes a row of one head.
 __global__ __launch_bounds__(256) void attention_bwd_rows(const void* __restrict__ dout, int dout_dtype, const void* __restrict__ out,
                                                           int out_dtype, const float* __restrict__ lse, int64_t n, int heads, int group,
                                                           int dim, float scale, uint16_t* __restrict__ copy, float* __restrict__ rows) {
-  const int64_t r = block_index() * 8 + (threadIdx.x >> 5);
+  const int64_t r = block_index() * 16 + (threadIdx.x >> 4);
   if (r >= n * heads) return;
   const int64_t token = r / heads;
-  const int head = static_cast<int>(r % heads), col = 4 * (threadIdx.x & 31);
+  const int head = static_cast<int>(r % heads), col = 8 * (threadIdx.x & 15);
   float sum = 0.0f;
   if (col < dim) {
-    float d[4], o[4];
-    load_some(dout_dtype, dout, r * dim + col, 4, d);
-    load_some(out_dtype, out, r * dim + col, 4, o);
-    if (copy) {
-      store_whole<VDSL_BF16, 4>(copy, r * dim + col, d);
+    float d[8], o[8];
+    if (dout_dtype == VDSL_F32) {
+      load_whole<VDSL_F32, 8>(dout, r * dim + col, d);
+      store_whole<VDSL_BF16, 8>(copy, r * dim + col, d);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) d[j] = bf16_to_f32(f32_to_bf16(d[j]));
+      for (int j = 0; j < 8; ++j) d[j] = bf16_to_f32(f32_to_bf16(d[j]));
+    } else {
+      load_whole<VDSL_BF16, 8>(dout, r * dim + col, d);
     }
+    if (out_dtype == VDSL_F32) load_whole<VDSL_F32, 8>(out, r * dim + col, o);
+    else load_whole<VDSL_BF16, 8>(out, r * dim + col, o);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) sum += d[j] * o[j];
+    for (int j = 0; j < 8; ++j) sum += d[j] * o[j];
   }
 #pragma unroll
-  for (int m = 16; m >= 1; m >>= 1) sum += __shfl_xor(sum, m, 64);
+  for (int m = 8; m >= 1; m >>= 1) sum += __shfl_xor(sum, m, 64);
   if (col != 0) return;
   const float l = lse[head * n + token];
   float* const to = rows + static_cast<int64_t>(head / group) * n * group + token * group + head % group;
@@ -542,7 +545,7 @@ extern "C" int vdsl_op_attention_bwd(vdsl_queue q, const vdsl_attention_params* 
   a.grad_dtype = grad_dtype;
   a.scale = p->scale;
   a.token_of = divider(group);
-  hipLaunchKernelGGL(attention_bwd_rows, block_grid((p->n * p->heads + 7) / 8), dim3(256), 0, q->stream, dout->ptr, dout_dtype,
+  hipLaunchKernelGGL(attention_bwd_rows, block_grid((p->n * p->heads + 15) / 16), dim3(256), 0, q->stream, dout->ptr, dout_dtype,
                      out->ptr, out_dtype, static_cast<const float*>(lse->ptr), p->n, p->heads, group, p->dim, p->scale, copy, rows);
   VDSL_TRY(check_launch("attention_bwd_rows"));
   const auto go = [&](auto kernel, unsigned lanes, int64_t slots, const char* name) {

@@ -24,6 +24,8 @@ Backward rules (y = act(x W^T), W stored [out][in]):
     y = a + b: dL/da = dL/db = dL/dy.
     embedding: dL/dtable = the sum of dL/dy over each row's tokens (vdsl_op_embedding_bwd).
     layer_norm: dL/dx, dL/dgamma, dL/dbeta from dL/dy (f32 or bf16), x and the forward pass's mean and rstd.
+    rope: dL/dx = the inverse rotation of dL/dy; attention: dL/dq, dL/dk, dL/dv from dL/dout, q, k, v and the forward pass's
+    out and lse (vdsl_op_attention_bwd).  paged_attention serves: it updates its caches and has no gradient.
     linear_cross_entropy (the output layer with its loss, logits never stored): dL/dx and dL/dW from the
     loss op itself (vdsl_op_linear_xent_fwd_bwd); W may be the embedding's table (tied weights).
     A value read by several ops (a residual input, a weight tied across layers): dL/dv is the f32
@@ -196,6 +198,68 @@ class Graph:
         self._op("layer_norm", [x, gamma] + ([beta] if beta is not None else []), [y, mean, rstd], eps=float(eps))
         return y
 
+    def rope(self, x: Value, positions: Value, freqs: Value, heads: int, dim: int, first: int = 0, interleaved: bool = False,
+             magnitude: float = 1.0, out_dtype: str | None = None, name=None) -> Value:
+        """x [rows][width] with `heads` heads of `dim` columns from column `first` on turned by positions (i32 [rows]): the first
+        2 * pairs columns of each, freqs f32 [2][pairs] (kernels.rope_frequencies); the other columns are handed on."""
+        out_dtype = out_dtype or x.dtype
+        if x.dtype not in ("f32", "bf16") or out_dtype not in ("f32", "bf16"):
+            raise TypeError("rope takes and stores f32 and bf16 tensors")
+        if len(x.shape) != 2 or positions.shape != x.shape[:1] or positions.dtype != "i32":
+            raise TypeError("rope takes x [rows][width] and i32 positions [rows]")
+        if freqs.dtype != "f32" or len(freqs.shape) != 2 or freqs.shape[0] != 2 or 2 * freqs.shape[1] > dim:
+            raise TypeError(f"rope: freqs {freqs.shape} must be f32 [2][pairs] with 2 * pairs up to {dim}")
+        if first < 0 or heads < 0 or first + heads * dim > x.shape[1]:
+            raise ValueError(f"rope: {heads} heads of {dim} from column {first} on do not fit {x.shape[1]} columns")
+        y = self._value(name or self._fresh("rope"), x.shape, out_dtype, requires_grad=x.requires_grad)
+        self._op("rope", [x, positions, freqs], [y], heads=int(heads), dim=int(dim), first=int(first), interleaved=bool(interleaved),
+                 magnitude=float(magnitude), inverse=False)
+        return y
+
+    @staticmethod
+    def _head_dim(qkv: Value, heads: int, kv_heads: int) -> int:
+        if qkv.dtype != "bf16" or len(qkv.shape) != 2:
+            raise TypeError("attention takes a bf16 projection [rows][(heads + 2 kv_heads) dim]: q, then k, then v")
+        if heads < 1 or kv_heads < 1 or heads % kv_heads or qkv.shape[1] % (heads + 2 * kv_heads):
+            raise ValueError(f"attention: {heads} heads and {kv_heads} kv heads do not fit {qkv.shape[1]} columns")
+        return qkv.shape[1] // (heads + 2 * kv_heads)
+
+    def attention(self, qkv: Value, starts: Value, heads: int, kv_heads: int, causal: bool = True, scale: float | None = None,
+                  out_dtype: str = "bf16", name=None) -> Value:
+        """[rows][heads * dim]: softmax(scale q k^T) v within each sequence, rows starts[s] to starts[s + 1] (i32 [seqs + 1]), of q, k
+        and v as columns of qkv [rows][(heads + 2 kv_heads) * dim] bf16; 0 in rows of no sequence."""
+        dim = self._head_dim(qkv, heads, kv_heads)
+        if starts.dtype != "i32" or len(starts.shape) != 1 or starts.shape[0] < 1:
+            raise TypeError("attention takes i32 starts [seqs + 1]")
+        if out_dtype not in ("f32", "bf16"):
+            raise TypeError("attention stores f32 or bf16")
+        y = self._value(name or self._fresh("attention"), (qkv.shape[0], heads * dim), out_dtype, requires_grad=qkv.requires_grad)
+        lse = self._value(self._fresh("lse"), (heads, qkv.shape[0]), "f32")  # kept for the backward pass
+        self._op("attention", [qkv, starts], [y, lse], heads=heads, kv_heads=kv_heads, dim=dim, causal=bool(causal), scale=scale)
+        return y
+
+    def paged_attention(self, qkv: Value, k_cache: Value, v_cache: Value, starts: Value, lengths: Value, table: Value, heads: int,
+                        scale: float | None = None, out_dtype: str = "bf16", name=None) -> Value:
+        """The new rows' k and v into their slots of the paged caches (bf16 [pages][kv_heads][page][dim], updated in place), then
+        attention of the rows over them: the row at position p sees positions 0 to p of its sequence.  lengths (i32 [seqs]) counts
+        a sequence's positions with the new rows, table (i32 [seqs][pages of a sequence]) says where they lie."""
+        if len(k_cache.shape) != 4 or v_cache.shape != k_cache.shape or (k_cache.dtype, v_cache.dtype) != ("bf16", "bf16"):
+            raise TypeError("paged_attention takes bf16 caches [pages][kv_heads][page][dim]")
+        kv_heads = k_cache.shape[1]
+        dim = self._head_dim(qkv, heads, kv_heads)
+        if dim != k_cache.shape[3]:
+            raise ValueError(f"paged_attention: heads of {dim} columns and a cache of {k_cache.shape[3]}")
+        seqs = lengths.shape[0]
+        if {starts.dtype, lengths.dtype, table.dtype} != {"i32"} or starts.shape != (seqs + 1,) or len(table.shape) != 2 or table.shape[0] != seqs:
+            raise TypeError("paged_attention takes i32 starts [seqs + 1], lengths [seqs] and table [seqs][pages of a sequence]")
+        if out_dtype not in ("f32", "bf16"):
+            raise TypeError("attention stores f32 or bf16")
+        y = self._value(name or self._fresh("paged_attention"), (qkv.shape[0], heads * dim), out_dtype)
+        attrs = dict(heads=heads, kv_heads=kv_heads, dim=dim, scale=scale)
+        self._op("cache_append", [qkv, k_cache, v_cache, starts, lengths, table], [], **attrs)
+        self._op("paged_attention", [qkv, k_cache, v_cache, starts, lengths, table], [y], **attrs)
+        return y
+
     def linear_cross_entropy(self, x: Value, w: Value, labels: Value, piece: int = 0, name="loss") -> Value:
         """The output layer over a vocabulary and its softmax cross entropy, without storing the logits: the mean over
         the rows whose label is in [0, vocab) of logsumexp(x W^T) - (x W^T)[label].  x [n][dim] and w [vocab][dim] bf16,
@@ -293,7 +357,7 @@ class Graph:
         for op in reversed(fwd_ops):
             if op.kind in ("mse", "linear_xent"):
                 continue
-            if op.kind not in ("linear", "linear_mse", "add", "embedding", "layer_norm"):
+            if op.kind not in ("linear", "linear_mse", "add", "embedding", "layer_norm", "rope", "attention"):
                 raise NotImplementedError(f"no backward rule for {op.kind}")
             y = op.outputs[0]
             if y.name not in grad:
@@ -318,6 +382,20 @@ class Graph:
                 for p, d in zip(op.inputs, [dx] + dp):
                     if d is not None:
                         self._give(p, ("f32", d), grad, contrib)
+                continue
+            if op.kind == "rope":
+                x, positions, freqs = op.inputs
+                if self._wants(x):
+                    dx = self._term(x, uses)
+                    self._op("rope", [grad[y.name][1], positions, freqs], [dx], **{**op.attrs, "inverse": True})
+                    self._give(x, ("f32", dx), grad, contrib)
+                continue
+            if op.kind == "attention":
+                qkv, starts = op.inputs
+                if self._wants(qkv):
+                    d = self._term(qkv, uses)
+                    self._op("attention_bwd", [grad[y.name][1], qkv, starts, *op.outputs], [d], **op.attrs)
+                    self._give(qkv, ("f32", d), grad, contrib)
                 continue
             x, w = op.inputs[:2]
             g = grad[y.name]
@@ -531,6 +609,13 @@ class Executable:
                 ws = max(ws, kernels.embedding_bwd_workspace_bytes(op.inputs[0].shape[0], *op.outputs[0].shape))
             if op.kind == "layer_norm_bwd":
                 ws = max(ws, kernels.layer_norm_bwd_workspace_bytes(*op.inputs[1].shape))
+            if op.kind == "attention_bwd":
+                n, a = op.inputs[0].shape[0], op.attrs
+                ws = max(ws, kernels.attention_bwd_workspace_bytes(n, op.inputs[2].shape[0] - 1, a["heads"], a["kv_heads"], a["dim"]))
+            if op.kind == "paged_attention":
+                qkv, cache, _, _, lengths, table = op.inputs
+                ws = max(ws, kernels.paged_attention_workspace_bytes(qkv.shape[0], lengths.shape[0], op.attrs["heads"], op.attrs["kv_heads"],
+                                                                     op.attrs["dim"], table.shape[1] * cache.shape[2]))
             if op.kind == "linear_xent":
                 (n, dim), vocab, backward = op.inputs[0].shape, op.inputs[1].shape[0], len(op.outputs) > 1
                 ws = max(ws, kernels.linear_xent_workspace_bytes(n, vocab, dim, op.attrs["piece"] if backward else 0, backward))
@@ -624,7 +709,7 @@ class Executable:
         return f"{op.kind} {'x'.join(map(str, ins[0].shape))}"
 
     def op_flops(self, op: Op) -> int:
-        """2 M N K for a GEMM op (multiply-adds of its main loop), 0 otherwise."""
+        """2 M N K for a GEMM op (multiply-adds of its main loop), 0 otherwise (attention's depend on its sequences)."""
         ins = op.inputs
         if op.kind in ("linear", "gemm_gelu_bwd", "gemm_mul_bwd", "linear_mse"):
             return 2 * ins[0].shape[0] * ins[0].shape[1] * ins[1].shape[0]
@@ -680,6 +765,22 @@ class Executable:
         elif op.kind == "layer_norm_bwd":
             dp = [None if op.attrs[k] is None else T[op.attrs[k].name] for k in ("dgamma", "dbeta")]
             kernels.layer_norm_bwd(q, *ins, outs[0], *dp, workspace=self.workspace)
+        elif op.kind == "rope":
+            a = op.attrs
+            kernels.rope(q, *ins, outs[0], a["heads"], a["dim"], a["first"], a["interleaved"], a["inverse"], a["magnitude"])
+        elif op.kind == "attention":
+            kernels.attention_fwd(q, *self._qkv(op, ins[0]), ins[1], outs[0], lse=outs[1], causal=op.attrs["causal"], scale=op.attrs["scale"])
+        elif op.kind == "attention_bwd":
+            dout, qkv, starts, out, lse = ins
+            kernels.attention_bwd(q, dout, *self._qkv(op, qkv), starts, out, lse, *self._qkv(op, outs[0]), causal=op.attrs["causal"],
+                                  scale=op.attrs["scale"], workspace=self.workspace)
+        elif op.kind == "cache_append":
+            qkv, k_cache, v_cache, starts, lengths, table = ins
+            kernels.cache_append(q, *self._qkv(op, qkv)[1:], starts, lengths, table, k_cache, v_cache)
+        elif op.kind == "paged_attention":
+            qkv, k_cache, v_cache, starts, lengths, table = ins
+            kernels.paged_attention(q, self._qkv(op, qkv)[0], k_cache, v_cache, starts, lengths, table, outs[0], scale=op.attrs["scale"],
+                                    workspace=self.workspace)
         elif op.kind == "gelu_bwd":
             kernels.gelu_bwd(q, ins[0], ins[1], outs[0], outs[1])
         elif op.kind == "relu_bwd":
@@ -703,6 +804,12 @@ class Executable:
                                      self.workspace)
         else:
             raise NotImplementedError(op.kind)
+
+    @staticmethod
+    def _qkv(op: Op, t: Tensor) -> list:
+        """q, k and v (or their gradients) as columns of one tensor."""
+        h, kv, dim = op.attrs["heads"], op.attrs["kv_heads"], op.attrs["dim"]
+        return [kernels.Heads(t, n, dim, at * dim) for n, at in ((h, 0), (kv, h), (kv, h + kv))]
 
     def capture(self, q: Queue) -> "Step":
         """Records one run() into a hipGraph and returns it as a Step (.launch(q), .destroy()).
@@ -798,3 +905,58 @@ def token_mlp_train_graph(tokens=2048, vocab=32768, dim=1024, hidden=4096, layer
     loss = g.linear_cross_entropy(norm(h, "norm_out"), out, labels, piece)
     grads = g.backward(loss)
     return g, grads
+
+
+def _transformer(g: Graph, ids: Value, positions: Value, freqs: Value, vocab: int, dim: int, heads: int, kv_heads: int, head_dim: int,
+                 hidden: int, layers: int, attend):
+    """Embedding (scaled by sqrt(dim)), `layers` blocks of [h + W_o attention(rope(W_qkv norm(h)))] and [h + W_down gelu(W_up norm(h))],
+    and the last norm; attend(qkv, layer): the attention.  Returns the embedding's table and the normed rows."""
+    def norm(x, name):
+        return g.layer_norm(x, g.param(name + "_gamma", (dim,), "f32"), g.param(name + "_beta", (dim,), "f32"))
+
+    table = g.param("E", (vocab, dim), "bf16")
+    h = g.embedding(table, ids, scale=float(dim) ** 0.5, out_dtype="f32")
+    for k in range(layers):
+        w = g.param(f"W{k}_qkv", ((heads + 2 * kv_heads) * head_dim, dim), "bf16")
+        qkv = g.rope(g.linear(norm(h, f"norm{k}a"), w, out_dtype="bf16"), positions, freqs, heads + kv_heads, head_dim)
+        h = g.add(h, g.linear(attend(qkv, k), g.param(f"W{k}_o", (dim, heads * head_dim), "bf16"), out_dtype="f32"))
+        u = g.linear(norm(h, f"norm{k}b"), g.param(f"W{k}_up", (hidden, dim), "bf16"), act="gelu")
+        h = g.add(h, g.linear(u, g.param(f"W{k}_down", (dim, hidden), "bf16"), out_dtype="f32"))
+    return table, norm(h, "norm_out")
+
+
+def token_transformer_train_graph(tokens=2048, seqs=4, vocab=32768, dim=1024, heads=8, kv_heads=2, head_dim=128, hidden=4096, layers=2, tied=True,
+                                  piece=0):
+    """A training step of a model of tokens that see the earlier ones of their sequence: token_mlp_train_graph with an attention
+    before each MLP.  Inputs: ids, labels and positions (i32 [tokens]), starts (i32 [seqs + 1]: the packed sequences), freqs (f32
+    [2][pairs], kernels.rope_frequencies(head_dim))."""
+    g = Graph(prepare_transposes=True, fuse_gelu_backward=True, pack_weights=True, store_gelu_deriv=True, k_major_grads=True)
+    ids, labels, positions = (g.input(n, (tokens,), "i32") for n in ("ids", "labels", "positions"))
+    starts, freqs = g.input("starts", (seqs + 1,), "i32"), g.input("freqs", (2, head_dim // 2), "f32")
+    table, h = _transformer(g, ids, positions, freqs, vocab, dim, heads, kv_heads, head_dim, hidden, layers,
+                            lambda qkv, k: g.attention(qkv, starts, heads, kv_heads))
+    out = table if tied else g.param("W_out", (vocab, dim), "bf16")
+    loss = g.linear_cross_entropy(h, out, labels, piece)
+    grads = g.backward(loss)
+    return g, grads
+
+
+def token_transformer_serve_graph(rows=64, seqs=8, pages=64, page=64, pages_per_seq=8, vocab=32768, dim=1024, heads=8, kv_heads=2, head_dim=128,
+                                  hidden=4096, layers=2, tied=True):
+    """A serving step of the same model, on the same weights: up to `rows` new tokens of up to `seqs` sequences, chunks of prompts
+    and single tokens alike, over paged caches.  Inputs: ids and positions (i32 [rows]; -1 for rows without a token), starts (i32
+    [seqs + 1]: which of them are a sequence's), lengths (i32 [seqs]: a sequence's positions with the new ones), table (i32
+    [seqs][pages_per_seq]), freqs, and per layer k_cache{k} and v_cache{k}, which the step updates.  Output: logits f32
+    [rows][vocab]."""
+    g = Graph(pack_weights=True)
+    ids, positions = g.input("ids", (rows,), "i32"), g.input("positions", (rows,), "i32")
+    starts, lengths = g.input("starts", (seqs + 1,), "i32"), g.input("lengths", (seqs,), "i32")
+    pages_of, freqs = g.input("table", (seqs, pages_per_seq), "i32"), g.input("freqs", (2, head_dim // 2), "f32")
+
+    def attend(qkv, k):
+        caches = [g.input(f"{n}_cache{k}", (pages, kv_heads, page, head_dim), "bf16") for n in "kv"]
+        return g.paged_attention(qkv, *caches, starts, lengths, pages_of, heads)
+
+    table, h = _transformer(g, ids, positions, freqs, vocab, dim, heads, kv_heads, head_dim, hidden, layers, attend)
+    g.linear(h, table if tied else g.param("W_out", (vocab, dim), "bf16"), out_dtype="f32", name="logits")
+    return g

@@ -474,45 +474,48 @@ __global__ __launch_bounds__(64, 2) void attention_few(AttentionArgs a) {
   store_rows<DP>(a, st, at, tile.row, place.kv, place.split);
 }
 
-// Joins the splits: with M = max m, out = sum 2^(m - M) o / sum 2^(m - M) l.  A block has one row, each of its groups of 32 lanes
-// a share of the splits.
+// Joins the splits: with M = max m, out = sum 2^(m - M) o / sum 2^(m - M) l.  A block's eight groups of 32 lanes have 8 / SHARES rows,
+// each row's groups a share of its splits.
+template <int SHARES>
 __global__ __launch_bounds__(256) void attention_join(AttentionArgs a) {
-  __shared__ float sums[8][4][32], heads_l[8];
+  __shared__ float sums[8][5][32];
   const int64_t rows = a.seqs.n * a.group, all = rows * a.kv_heads;
-  const int64_t r = block_index();
-  if (r >= all) return;
-  const int kv = static_cast<int>(r / rows);
-  const int64_t token = r % rows / a.group;
-  const int head = kv * a.group + static_cast<int>(r % rows % a.group);
-  const int group = threadIdx.x >> 5, groups = blockDim.x >> 5, lane = threadIdx.x & 31, col = 4 * lane;
+  const int group = threadIdx.x >> 5, lane = threadIdx.x & 31, col = 4 * lane, part = group % SHARES;
+  const int64_t r = block_index() * (8 / SHARES) + group / SHARES;
+  if (SHARES == 1 && r >= all) return;
+  const int64_t row = r < all ? r : all - 1;
   float m = neg_inf();
-  for (int s = lane; s < a.splits; s += 32) m = fmaxf(m, a.stats[s * all + r].x);
+  for (int s = lane; s < a.splits; s += 32) m = fmaxf(m, a.stats[s * all + row].x);
 #pragma unroll
   for (int i = 16; i >= 1; i >>= 1) m = fmaxf(m, __shfl_xor(m, i, 64));
   float v[4] = {0.0f, 0.0f, 0.0f, 0.0f}, l = 0.0f;
 #pragma unroll 4
-  for (int s = group; s < a.splits; s += groups) {
-    const float2 st = a.stats[s * all + r];
+  for (int s = part; s < a.splits; s += SHARES) {
+    const float2 st = a.stats[s * all + row];
     float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     const bool some = st.x != neg_inf();
-    if (some && col < a.dim) load_whole<VDSL_F32, 4>(a.parts, (s * all + r) * a.dim + col, o);
+    if (some && col < a.dim) load_whole<VDSL_F32, 4>(a.parts, (s * all + row) * a.dim + col, o);
     const float by = some ? __builtin_amdgcn_exp2f(st.x - m) : 0.0f;
     l += by * st.y;
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] += by * o[j];
   }
-  if (groups > 1) {
+  if constexpr (SHARES > 1) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) sums[group][j][lane] = v[j];
-    if (lane == 0) heads_l[group] = l;
+    sums[group][4][lane] = l;
     __syncthreads();
-    if (group > 0) return;
-    for (int g = 1; g < groups; ++g) {
-      l += heads_l[g];
+    if (part > 0 || r >= all) return;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] += sums[g][j][lane];
+    for (int g = 1; g < SHARES; ++g) {
+      l += sums[group + g][4][lane];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] += sums[group + g][j][lane];
     }
   }
+  const int kv = static_cast<int>(r / rows);
+  const int64_t token = r % rows / a.group;
+  const int head = kv * a.group + static_cast<int>(r % rows % a.group);
   const bool none = m == neg_inf();
   if (a.lse && col == 0) a.lse[head * a.seqs.n + token] = none ? neg_inf() : (m + __builtin_amdgcn_logf(l)) * kLn2;
   if (col >= a.dim) return;
@@ -645,9 +648,13 @@ PagedPlan paged_plan(int64_t n, int64_t seqs, int32_t heads, int32_t kv_heads, i
   const int64_t group = heads / kv_heads, with_rows = std::max<int64_t>(1, std::min(seqs, n));
   PagedPlan plan = {n * group <= 32 * with_rows, 1};
   const int64_t tiles = (n * group / (plan.few ? 32 : 128) + with_rows) * kv_heads;
-  // blocks: those of attention_few four times what the card holds, since sequences differ in length; attention_rows two a CU
-  const int64_t want = plan.few ? 5120 : 512, least = plan.few ? 64 : 256;
-  const int64_t splits = std::min<int64_t>({(want + tiles - 1) / tiles, positions / least, 256});
+  const auto split = [&](int64_t blocks, int64_t least) { return std::min<int64_t>({(blocks + tiles - 1) / tiles, positions / least, 256}); };
+  // attention_few: two rounds of the blocks the card holds, of 64 positions at least, or eight rounds, which sequences of
+  // different lengths are better spread over, of 1024.  us with 2560, 5120 and 10240 blocks of 64 positions at least (32 / 8
+  // heads of 128 unless said): 64 sequences of up to 16384 positions 482, 470, 462; 16 of 4096, 8 / 8 heads 37.3, 42.3, 51.2;
+  // 8 of 1000 (15 splits) 14.5 all, of 128 positions at least 15.3.  attention_rows: four rounds; 1024 rows over 16384 positions with 512,
+  // 1024 and 1536 blocks 266, 257, 257.
+  const int64_t splits = plan.few ? std::max(split(2560, 64), split(10240, 1024)) : split(1024, 256);
   plan.splits = static_cast<int>(std::max<int64_t>(1, splits));
   return plan;
 }
@@ -763,7 +770,8 @@ extern "C" int vdsl_op_paged_attention(vdsl_queue q, const vdsl_paged_params* p,
   else
     VDSL_TRY(launch_rows<true>(q, a));
   if (a.splits == 1) return VDSL_OK;
-  const unsigned lanes = a.splits <= 4 ? 32 : a.splits <= 32 ? 128 : 256;
-  hipLaunchKernelGGL(attention_join, block_grid(p->n * p->heads), dim3(lanes), 0, q->stream, a);
+  const int shares = a.splits <= 8 ? 1 : a.splits <= 64 ? 4 : 8;
+  const auto join = shares == 1 ? attention_join<1> : shares == 4 ? attention_join<4> : attention_join<8>;
+  hipLaunchKernelGGL(join, block_grid((p->n * p->heads + 8 / shares - 1) / (8 / shares)), dim3(256), 0, q->stream, a);
   return check_launch("attention_join");
 }

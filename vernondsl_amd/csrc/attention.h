@@ -184,6 +184,18 @@ __device__ __forceinline__ float halves_sum(float v) {
   return r[0] + r[1];
 }
 
+// Asks the scheduler for READS LDS reads, then MFMAS times a product and PER reads, so that a fragment is read some products
+// before the one that takes it (left alone it is read right before, and each product waits for its own).
+template <int READS, int MFMAS, int PER>
+__device__ __forceinline__ void reads_ahead() {
+  __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+#pragma unroll
+  for (int i = 0; i < MFMAS; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, PER, 0);
+  }
+}
+
 // Registers 8 e .. 8 e + 7 of a score tile as the operand of a step over its 16 keys.
 __device__ __forceinline__ bf16x8 weights_fragment(const f32x16& s, int e) {
   const u32x4 w = {pack_bf16x2(s[8 * e], s[8 * e + 1]), pack_bf16x2(s[8 * e + 2], s[8 * e + 3]),

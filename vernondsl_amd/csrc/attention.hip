@@ -324,11 +324,12 @@ __global__ __launch_bounds__(256, 2) void attention_rows(AttentionArgs a) {
     slot ^= 1;
     f32x16 s[KS];
 #pragma unroll
-    for (int k = 0; k < KS; ++k) {
-      s[k] = MfmaBf16::zero();
+    for (int k = 0; k < KS; ++k) s[k] = MfmaBf16::zero();
 #pragma unroll
-      for (int kk = 0; kk < DP / 16; ++kk) s[k] = MfmaBf16::mma(rows_fragment<DP>(keys, 32 * k, kk), qf[kk], s[k]);
-    }
+    for (int kk = 0; kk < DP / 16; ++kk)
+#pragma unroll
+      for (int k = 0; k < KS; ++k) s[k] = MfmaBf16::mma(rows_fragment<DP>(keys, 32 * k, kk), qf[kk], s[k]);
+    reads_ahead<6, KS * DP / 16, 1>();
     if (PAGED && valid != ~0ull) hide(s, KT, valid);
     st.weigh(s, scale2);
 #pragma unroll

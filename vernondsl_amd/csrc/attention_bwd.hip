@@ -201,6 +201,8 @@ __global__ __launch_bounds__(512, 2) void attention_bwd_keys(GradArgs a) {
       s = MfmaBf16::mma(rows_fragment<DP>(qs, 0, kk), kf[kk], s);
       p = MfmaBf16::mma(rows_fragment<DP>(ds, 0, kk), V_LDS ? rows_fragment<DP>(values, 0, kk) : vf[kk], p);
     }
+    if constexpr (V_LDS) reads_ahead<14, DP / 8, 2>();  // the first 8 are of what they start from
+    else reads_ahead<12, DP / 8, 1>();
     // a row whose q or dout holds an element that is no finite number has no finite score or dp with any key
     bool leave = false;
     if (r0 < all_seen) leave = left_out > 0 || any_not_finite(s) || any_not_finite(p);
@@ -395,6 +397,7 @@ __global__ __launch_bounds__(256, 2) void attention_bwd_queries(GradArgs a) {
       s = MfmaBf16::mma(rows_fragment<DP>(ks, 0, kk), qf[kk], s);
       p = MfmaBf16::mma(rows_fragment<DP>(ks + KT * T::PITCH, 0, kk), df[kk], p);
     }
+    reads_ahead<4, DP / 8, 1>();
     if (odd) *odd = any_not_finite(s);
 #pragma unroll
     for (int r = 0; r < 16; ++r) p[r] = __builtin_amdgcn_exp2f((s[r] + score0) * scale2) * (p[r] + dp0);

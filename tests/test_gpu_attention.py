@@ -61,7 +61,9 @@ PACKED = [([1], 0, 0, 1, 1, 8, True), ([2, 0, 1], 1, 2, 2, 1, 16, True), ([33], 
           ([127, 0, 130, 1], 2, 5, 6, 2, 80, True), ([300], 0, 0, 5, 1, 128, True), ([257, 31], 0, 0, 4, 4, 40, True),
           ([129, 70], 3, 0, 8, 1, 96, True), ([200, 0, 56], 0, 7, 2, 2, 128, False), ([1, 1, 1, 1, 1], 0, 0, 4, 2, 64, False),
           ([513], 0, 0, 2, 1, 104, False), ([0, 0], 0, 9, 2, 1, 64, True), ([90] * 70, 0, 0, 2, 2, 32, True),
-          ([4200], 0, 0, 16, 2, 64, True), ([2300, 2000], 0, 11, 16, 4, 128, True), ([4100], 0, 0, 16, 2, 88, False)]
+          ([4200], 0, 0, 16, 2, 64, True), ([2300, 2000], 0, 11, 16, 4, 128, True), ([4100], 0, 0, 16, 2, 88, False),
+          # as above, with so many kv heads that the gradient's blocks have 128 keys
+          ([1100], 0, 0, 32, 32, 8, True), ([1000, 50], 0, 3, 40, 40, 128, True), ([500, 0, 600], 2, 0, 64, 32, 64, True), ([700], 0, 0, 32, 32, 96, False)]
 
 
 @pytest.mark.parametrize("lengths,front,back,heads,kv,dim,causal", PACKED)
@@ -116,7 +118,7 @@ def test_packed(q, own, lengths, front, back, heads, kv, dim, causal):
 
 
 @pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
-@pytest.mark.parametrize("dim,heads,kv,n,at", [(64, 2, 1, 200, 70), (128, 4, 2, 333, 150), (80, 1, 1, 100, 99)])
+@pytest.mark.parametrize("dim,heads,kv,n,at", [(64, 2, 1, 200, 70), (128, 4, 2, 333, 150), (80, 1, 1, 100, 99), (64, 40, 40, 900, 400), (128, 72, 36, 1000, 530)])
 def test_what_is_not_seen_has_no_influence(q, own, dim, heads, kv, n, at, bad):
     """Rows from `at` on hold NaN or infinities: the rows before have the outputs that they would have alone, and their dq too;
     rows before `at` whose q and dout are so leave the gradients of the keys from `at` on alone."""

@@ -23,6 +23,7 @@ struct GradArgs {
   int64_t q_stride, k_stride, v_stride, dout_stride;
   Sequences seqs;
   int* left_out;      // by the waves of attention_bwd_keys
+  int key_log;        // log2 of the keys of one of its blocks
   const float* rows;  // -lse / scale, then -delta, each [kv_heads][n * group]
   void *dq, *dk, *dv;
   int64_t dq_first, dq_stride, dk_first, dk_stride, dv_first, dv_stride;
@@ -85,30 +86,31 @@ __device__ __forceinline__ void store_zeros(int dtype, void* to, int64_t e, int 
   for (int c = 0; c < cols; c += 4) store_unit<4>(dtype, to, e + c, none);
 }
 
-// dk and dv: a block has 128 keys and walks over tiles of 64 rows through a ring of three slots of LDS.  Each 32 keys have two waves, one
-// for each half of a tile's rows, which add up their sums at the end; both are on one SIMD, and the first has priority
-// there, so that its exponentials come beside the other's products.  To leave both their registers, wide heads'
-// values are an operand read from LDS (V_LDS).
-template <int DP>
+// dk and dv: a block has KEYS keys and walks over tiles of rows through a ring of two or three slots of LDS.  Each 32 keys
+// have 8 / (KEYS / 32) waves, one for each 32 rows of a tile, which add up their sums at the end.  Two waves share a SIMD,
+// and one has priority there, so that its exponentials come beside the other's products.  To leave both their
+// registers, wide heads' values are an operand read from LDS (V_LDS).
+template <int DP, int KEYS>
 __global__ __launch_bounds__(512, 2) void attention_bwd_keys(GradArgs a) {
-  constexpr int TR = 64, NW = 8;
+  constexpr int NW = 8, GROUPS = KEYS / 32, PARTS = NW / GROUPS, TR = 32 * PARTS;
   constexpr bool V_LDS = DP > 96;
   using T = TileShape<DP>;
-  using Copies = RowCopies<DP, 8>;  // of a tile's rows by each wave
-  constexpr int SUMS = 4 * 32 * DP * 4;  // one gradient's sums of four waves
-  constexpr int NS = 3, SLOT = 2 * TR * T::PITCH, AREA = NS * SLOT + (V_LDS ? 128 * T::PITCH : 0);
+  constexpr int CR = TR / NW;  // of a tile's rows a wave copies
+  using Copies = RowCopies<DP, CR>;
+  constexpr int SUMS = (NW - GROUPS) * 32 * DP * 4;  // one gradient's sums of all but the first parts
+  constexpr int NS = PARTS == 2 ? 3 : 2, SLOT = 2 * TR * T::PITCH, AREA = NS * SLOT + (V_LDS ? KEYS * T::PITCH : 0);
   __shared__ __attribute__((aligned(1024))) char smem[AREA > SUMS ? AREA : SUMS];
   __shared__ __attribute__((aligned(16))) float starts[NW][NS][2][32];  // what the rows' scores and dp start from, a copy a wave
   int b = static_cast<int>(blockIdx.x);
   const int kv = b % a.kv_heads;
-  const RowTile tile = row_tile<7>(a.seqs, 1, b / a.kv_heads);
+  const RowTile tile = row_tile<KEYS == 128 ? 7 : 6>(a.seqs, 1, b / a.kv_heads);
   if (!tile.any) {
     if (threadIdx.x < NW) a.left_out[blockIdx.x * NW + threadIdx.x] = 0;
     return;
   }
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
-  const int part = wave >> 2;  // of a tile's rows
-  const int key0 = tile.row + 32 * (wave & 3), key = key0 + (lane & 31);
+  const int part = wave / GROUPS;  // of a tile's rows
+  const int key0 = tile.row + 32 * (wave % GROUPS), key = key0 + (lane & 31);
   const int64_t head_col = static_cast<int64_t>(kv) * a.dim;
   if (tile.seq < 0) {
     if (lane == 0) a.left_out[blockIdx.x * NW + wave] = 0;
@@ -126,7 +128,7 @@ __global__ __launch_bounds__(512, 2) void attention_bwd_keys(GradArgs a) {
   bf16x8 kf[DP / 16], vf[DP / 16];
   load_operand<DP>(a.k + token * a.k_stride + head_col, a.dim, kf);
   load_operand<DP>(a.v + token * a.v_stride + head_col, a.dim, vf);
-  char* const values = smem + NS * SLOT + (wave & 3) * 32 * T::PITCH;  // both waves write the same
+  char* const values = smem + NS * SLOT + wave % GROUPS * 32 * T::PITCH;  // all parts write the same
   if constexpr (V_LDS) {
 #pragma unroll
     for (int kk = 0; kk < DP / 16; ++kk)
@@ -138,22 +140,22 @@ __global__ __launch_bounds__(512, 2) void attention_bwd_keys(GradArgs a) {
   const char* const dp = reinterpret_cast<const char*>(a.dout + tile.token * a.dout_stride + head_col * a.group);
   const float* const sp = a.rows + (static_cast<int64_t>(kv) * a.seqs.n + tile.token) * a.group;
   const int64_t delta_at = a.seqs.n * a.heads;
-  // The copies of tile t.  Their offsets are the same for all tiles if 8 rows are whole tokens.
+  // The copies of tile t.  Their offsets are the same for all tiles if a wave's rows are whole tokens.
   Copies copies;
   const auto offsets = [&](int row0, int token0) {
     const auto at = [&](int r, int64_t stride) {
       const int i = a.token_of(row0 + r);
       return 2u * (static_cast<uint32_t>(i - token0) * static_cast<uint32_t>(stride) + static_cast<uint32_t>((row0 + r - i * a.group) * a.dim));
     };
-    copies.offsets(8 * wave, a.dim, [&](int r) { return at(r, a.q_stride); }, [&](int r) { return at(r, a.dout_stride); });
+    copies.offsets(CR * wave, a.dim, [&](int r) { return at(r, a.q_stride); }, [&](int r) { return at(r, a.dout_stride); });
   };
-  const bool whole_tokens = 8 % a.group == 0;
+  const bool whole_tokens = CR % a.group == 0;
   if (whole_tokens) offsets(0, 0);
   const auto fetch = [&](int t, int slot) {
-    const int last = rows - 1 - t * TR, row0 = t * TR + 8 * wave, token0 = a.token_of(row0);
+    const int last = rows - 1 - t * TR, row0 = t * TR + CR * wave, token0 = a.token_of(row0);
     if (!whole_tokens) offsets(row0, token0);
-    char* const area = smem + slot * SLOT + 8 * wave * T::PITCH;
-    copies.copy(qp + 2 * (token0 * a.q_stride), dp + 2 * (token0 * a.dout_stride), last - 8 * wave, area, area + TR * T::PITCH);
+    char* const area = smem + slot * SLOT + CR * wave * T::PITCH;
+    copies.copy(qp + 2 * (token0 * a.q_stride), dp + 2 * (token0 * a.dout_stride), last - CR * wave, area, area + TR * T::PITCH);
     float* const to = starts[wave][slot][0];
     const int r = 32 * part + (lane & 31);
     // rows that are not there: no weight
@@ -170,20 +172,20 @@ __global__ __launch_bounds__(512, 2) void attention_bwd_keys(GradArgs a) {
   int left_out = 0;  // rows before this one: attention_bwd_left_out adds them
   // All blocks begin with the last rows, which they all see, and so read the same rows at about the same time.
   fetch(end - 1, 0);
-  if (end - 2 >= first) fetch(end - 2, 1);
+  if (NS == 3 && end - 2 >= first) fetch(end - 2, 1);
   int slot = 0;
-  if (part == 0) __builtin_amdgcn_s_setprio(1);
+  if (wave < 4) __builtin_amdgcn_s_setprio(1);
 #pragma unroll 1
   for (int t = end - 1; t >= first; --t) {
-    // the next tile, which is whole, may be on its way; every wave has left the one before
-    if (t > first) dma_wait<2 * Copies::C + 1>();
+    // Every wave has left the tile before.  Of three slots, the next tile, which is whole, may be on its way.
+    if (NS == 3 && t > first) dma_wait<2 * Copies::C + 1>();
     else dma_wait<0>();
     dma_barrier();
-    if (t - 2 >= first) fetch(t - 2, slot == 0 ? 2 : slot - 1);
+    if (t - (NS - 1) >= first) fetch(t - (NS - 1), slot == 0 ? NS - 1 : slot - 1);
     const char* const qs = smem + slot * SLOT + part * 32 * T::PITCH;
     const char* const ds = qs + TR * T::PITCH;
     const float* const x = starts[wave][slot][0] + 4 * half;
-    slot = slot == 2 ? 0 : slot + 1;
+    slot = slot == NS - 1 ? 0 : slot + 1;
     const int r0 = t * TR + 32 * part;
     if (r0 + 32 <= one_seen || r0 >= rows) continue;
     f32x16 s, p;
@@ -236,27 +238,29 @@ __global__ __launch_bounds__(512, 2) void attention_bwd_keys(GradArgs a) {
   }
   __builtin_amdgcn_s_setprio(0);
   if (lane == 0) a.left_out[blockIdx.x * NW + wave] = left_out;
-  // the second halves' sums by way of LDS, one gradient after the other
-  float* const sums = reinterpret_cast<float*>(smem) + (wave & 3) * DP * 32 + lane * 4;
+  // the other parts' sums by way of LDS, one gradient after the other
+  float* const sums = reinterpret_cast<float*>(smem) + lane * 4;
   const auto join = [&](f32x16 (&acc)[DP / 32]) {
     __syncthreads();
-    if (part == 1) {
+    if (part != 0) {
 #pragma unroll
       for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
         for (int g = 0; g < 4; ++g)
-          *reinterpret_cast<f32x4*>(sums + (4 * d + g) * 256) = f32x4{acc[d][4 * g], acc[d][4 * g + 1], acc[d][4 * g + 2], acc[d][4 * g + 3]};
+          *reinterpret_cast<f32x4*>(sums + (wave - GROUPS) * DP * 32 + (4 * d + g) * 256) = f32x4{acc[d][4 * g], acc[d][4 * g + 1], acc[d][4 * g + 2], acc[d][4 * g + 3]};
     }
     __syncthreads();
     if (part == 0) {
 #pragma unroll
-      for (int d = 0; d < DP / 32; ++d)
+      for (int o = 0; o < PARTS - 1; ++o)
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const f32x4 v = *reinterpret_cast<const f32x4*>(sums + (4 * d + g) * 256);
+        for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) acc[d][4 * g + j] += v[j];
-        }
+          for (int g = 0; g < 4; ++g) {
+            const f32x4 v = *reinterpret_cast<const f32x4*>(sums + (wave + o * GROUPS) * DP * 32 + (4 * d + g) * 256);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[d][4 * g + j] += v[j];
+          }
     }
   };
   join(dk);
@@ -279,8 +283,10 @@ __global__ __launch_bounds__(256) void attention_bwd_left_out(GradArgs a) {
   for (int w = 0; w < 8; ++w) any |= flags[w];
   if (any == 0) return;
   const int kv = place % a.kv_heads;
-  const RowTile tile = row_tile<7>(a.seqs, 1, place / a.kv_heads);
+  const RowTile tile = a.key_log == 7 ? row_tile<7>(a.seqs, 1, place / a.kv_heads) : row_tile<6>(a.seqs, 1, place / a.kv_heads);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int groups = 1 << (a.key_log - 5), parts = 8 / groups;
+  if (wave >= groups) return;
   const int key0 = tile.row + 32 * wave, key = key0 + (lane & 31);
   const int64_t head_col = static_cast<int64_t>(kv) * a.dim, token = tile.token + min(key, tile.len - 1);
   bf16x8 kf[DP / 16], vf[DP / 16];
@@ -293,10 +299,12 @@ __global__ __launch_bounds__(256) void attention_bwd_left_out(GradArgs a) {
   const uint16_t* const dp = a.dout + tile.token * a.dout_stride + head_col * a.group;
   const float* const sp = a.rows + (static_cast<int64_t>(kv) * a.seqs.n + tile.token) * a.group;
   const float scale2 = a.scale * kLog2e;
-  const int end = min(max(flags[wave], flags[wave + 4]), tile.len * a.group);
+  int end = 0;
+  for (int p = 0; p < parts; ++p) end = max(end, flags[wave + groups * p]);
+  end = min(end, tile.len * a.group);
 #pragma unroll 1
   for (int r = key0 * a.group; r < end; ++r) {
-    if (r >= flags[wave + 4 * ((r >> 5) & 1)]) continue;
+    if (r >= flags[wave + groups * ((r >> 5) & (parts - 1))]) continue;
     const int i = a.token_of(r);
     const int64_t col = static_cast<int64_t>(r - i * a.group) * a.dim;
     const uint16_t* const qr = qp + i * a.q_stride + col;
@@ -450,6 +458,13 @@ __global__ __launch_bounds__(256, 2) void attention_bwd_queries(GradArgs a) {
   if (row0 + (lane & 31) < rows) store_gradient<DP>(dq, a.scale, a.grad_dtype, a.dq, dq_at(row), a.dim);
 }
 
+// 128 keys a block, or 64 in twice the blocks, each half as long, where 128 would leave CUs idle (full attention) or wait for the
+// blocks of the first keys, which the most rows see (causal).  32 heads of 128 over 8: causal, one sequence of 1024 rows 164 us by
+// 128 keys and 124 by 64, 2048: 309 and 238, 4096: 684 and 571, 8192: 1820 and 2040; full, 4096: 893 and 1042.
+int key_tile_log(int64_t n, int64_t kv_heads, bool causal) {
+  return ((n + 127) >> 7) * kv_heads <= (causal ? 256 : 128) ? 6 : 7;
+}
+
 bool float_type(int32_t t) { return t == VDSL_F32 || t == VDSL_BF16; }
 
 // Whether two of the gradients, as columns of one buffer, have no element in common.
@@ -469,7 +484,7 @@ extern "C" int vdsl_attention_bwd_workspace_bytes(int64_t n, int64_t seqs, int32
   if (!bytes) return fail(VDSL_ERR_INVALID_ARG, "bytes is null");
   VDSL_TRY(attention_check_shape("attention_bwd", n, seqs, heads, kv_heads, dim));
   // a multiple of 16 bytes before the copy
-  const size_t flags = nbytes(row_slots(n, seqs, 1, 7), kv_heads, 32), rows = nbytes(n, heads, 8 + 2 * static_cast<int64_t>(dim));
+  const size_t flags = nbytes(row_slots(n, seqs, 1, 6), kv_heads, 32), rows = nbytes(n, heads, 8 + 2 * static_cast<int64_t>(dim));
   if (flags == kSizeOverflow || rows == kSizeOverflow || rows + flags + 16 < rows)
     return fail(VDSL_ERR_SHAPE, "attention_bwd workspace size overflows");
   *bytes = rows + flags + 16;
@@ -515,7 +530,8 @@ extern "C" int vdsl_op_attention_bwd(vdsl_queue q, const vdsl_attention_params* 
   if (p->n == 0) return VDSL_OK;
   const int group = p->heads / p->kv_heads;
   float* const rows = static_cast<float*>(workspace->ptr);
-  const int64_t key_slots = row_slots(p->n, p->seqs, 1, 7), query_slots = row_slots(p->n, p->seqs, group, 7);
+  const int key_log = key_tile_log(p->n, p->kv_heads, p->causal != 0);
+  const int64_t key_slots = row_slots(p->n, p->seqs, 1, key_log), query_slots = row_slots(p->n, p->seqs, group, 7);
   if (std::max(key_slots, query_slots) * p->kv_heads > 0x3fffff) return fail(VDSL_ERR_UNSUPPORTED, "attention_bwd: too many rows");
   const int64_t flags_at = 2 * p->n * p->heads, copy_at = (flags_at + 8 * key_slots * p->kv_heads + 3) & ~int64_t{3};
   uint16_t* const copy = dout_dtype == VDSL_F32 ? reinterpret_cast<uint16_t*>(rows + copy_at) : nullptr;
@@ -530,6 +546,7 @@ extern "C" int vdsl_op_attention_bwd(vdsl_queue q, const vdsl_attention_params* 
   a.dout_stride = width;
   a.seqs = {static_cast<const int32_t*>(starts->ptr), p->n, p->seqs};
   a.rows = rows;
+  a.key_log = key_log;
   a.left_out = reinterpret_cast<int*>(rows + flags_at);
   a.dq = dq->ptr;
   a.dk = dk->ptr;
@@ -556,7 +573,8 @@ extern "C" int vdsl_op_attention_bwd(vdsl_queue q, const vdsl_attention_params* 
     return check_launch(name);
   };
   a.blocks = static_cast<int>(query_slots);
-  const auto keys = p->dim <= 64 ? attention_bwd_keys<64> : p->dim <= 96 ? attention_bwd_keys<96> : attention_bwd_keys<128>;
+  const auto keys = a.key_log == 7 ? (p->dim <= 64 ? attention_bwd_keys<64, 128> : p->dim <= 96 ? attention_bwd_keys<96, 128> : attention_bwd_keys<128, 128>)
+                                   : (p->dim <= 64 ? attention_bwd_keys<64, 64> : p->dim <= 96 ? attention_bwd_keys<96, 64> : attention_bwd_keys<128, 64>);
   const auto queries = p->dim <= 64 ? attention_bwd_queries<64> : p->dim <= 96 ? attention_bwd_queries<96> : attention_bwd_queries<128>;
   const auto rest = p->dim <= 64 ? attention_bwd_left_out<64> : p->dim <= 96 ? attention_bwd_left_out<96> : attention_bwd_left_out<128>;
   VDSL_TRY(go(keys, 512, key_slots, "attention_bwd_keys"));

@@ -755,6 +755,7 @@ int vdsl_op_attention_fwd(vdsl_queue q, const vdsl_attention_params* p, vdsl_buf
  * (the last two over the rows i that see j and the heads that share j's).  dq, dk, dv: grad_dtype, F32 or BF16, every row
  * of their heads written (0 for rows of no sequence), columns outside their heads left as they are; they may lie in one
  * buffer as disjoint columns of one stride.  dout, p and ds are rounded to bf16 for the products, which accumulate in f32.
+ * (Where some rows of q or dout hold NaN or infinities, bf16 gradients of the keys just behind them may be rounded twice.)
  * The same bits on every call.  workspace: vdsl_attention_bwd_workspace_bytes() bytes of any contents (two calls that
  * overlap in time need two). */
 int vdsl_attention_bwd_workspace_bytes(int64_t n, int64_t seqs, int32_t heads, int32_t kv_heads, int32_t dim, size_t* bytes);
@@ -767,7 +768,8 @@ int vdsl_op_attention_bwd(vdsl_queue q, const vdsl_attention_params* p, int32_t 
  * to 65536).  Position j of sequence s is slot j % page of page table[s][j / page] (I32 [seqs][table_cols]); an entry outside
  * [0, pages) is no page: its positions hold nothing.  The new rows of sequence s are [starts[s], starts[s + 1]) (as for
  * vdsl_op_attention_fwd), m of them; lengths[s] (I32 [seqs]) counts its positions with the new rows: row i of them is
- * position lengths[s] - m + i.  Positions below 0 or not below table_cols * page hold nothing. */
+ * position lengths[s] - m + i.  Positions below 0 or not below table_cols * page hold nothing.
+ * table_cols * page: up to 2^31 - 2^16. */
 typedef struct vdsl_paged_params {
   int64_t n;
   int64_t seqs;
@@ -782,7 +784,7 @@ typedef struct vdsl_paged_params {
   vdsl_heads q, k, v; /* q: read by the attention only, k and v by the append only */
 } vdsl_paged_params;
 /* The new rows' k and v (BF16) into their slots of the cache; rows of no sequence or without a slot are dropped, everything
- * else in the cache stays.  No two rows may have one slot.  (heads, scale and q are not read.) */
+ * else in the cache stays.  No two rows may have one slot.  (scale and q are not read; heads is any multiple of kv_heads.) */
 int vdsl_op_cache_append(vdsl_queue q, const vdsl_paged_params* p, vdsl_buffer ks, vdsl_buffer vs, vdsl_buffer starts,
                          vdsl_buffer lengths, vdsl_buffer table, vdsl_buffer k_cache, vdsl_buffer v_cache);
 /* Attention of the new rows over the cache, which holds their own keys already: the row at position p sees positions 0 to p.

@@ -170,6 +170,46 @@ def test_extreme_scores(q, own):
     assert not get(q, out).any() and np.isneginf(get(q, lse)).all()
 
 
+def test_nan_is_handed_on(q, own):
+    """A row whose q is NaN, in one head: NaN for that row and head alone, and for the gradients that it has a part in."""
+    n, heads, kv, dim, bad = 150, 4, 2, 64, 70
+    a, b, c = projection(np.random.default_rng(7), n, heads, kv, dim)
+    a[bad, 1] = np.nan
+    starts = own.put(starts_of([n]), "i32")
+    x = [own.put(y, "bf16") for y in (a, b, c)]
+    out, lse = own.empty((n, heads * dim), "f32"), own.empty((heads, n), "f32")
+    kernels.attention_fwd(q, *x, starts, out, lse=lse)
+    hit = np.zeros((n, heads), bool)
+    hit[bad, 1] = True
+
+    def of_that_row_only(n=n, hit=hit):
+        found = get(q, out).reshape(n, heads, dim)
+        assert np.isnan(found[hit]).all() and np.isfinite(found[~hit]).all()
+        assert np.array_equal(np.isnan(get(q, lse)).T, hit) and np.isfinite(get(q, lse).T[~hit]).all()
+
+    of_that_row_only()
+    g = [own.empty((n, h, dim), "f32") for h in (heads, kv, kv)]
+    kernels.attention_bwd(q, own.put(np.ones((n, heads * dim)), "bf16"), *x, starts, out, lse, *g,
+                          workspace=own.scratch(kernels.attention_bwd_workspace_bytes(n, 1, heads, kv, dim)))
+    dq, dk, dv = (get(q, y) for y in g)
+    assert np.isnan(dq[hit]).all() and np.isfinite(dq[~hit]).all()
+    for d in (dk, dv):
+        assert np.isnan(d[:bad + 1, 0]).all() and np.isfinite(d[bad + 1:]).all() and np.isfinite(d[:, 1]).all()
+
+    page = 16
+    for rows, keys, cols in ((3, 30, 2), (3, 1900, 120), (100, 200, 13), (100, 1900, 120)):  # of few rows and many, whole and split
+        kc, vc = (own.put(y, "bf16") for y in make_cache(np.random.default_rng(8), cols, kv, page, dim))
+        out, lse = own.empty((rows, heads * dim), "f32"), own.empty((heads, rows), "f32")
+        y = a[bad - 1:bad - 1 + rows]  # row 1 is the one
+        need = kernels.paged_attention_workspace_bytes(rows, 1, heads, kv, dim, cols * page)
+        assert (need > 0) == (keys == 1900)
+        kernels.paged_attention(q, own.put(np.concatenate([y, a[:rows - len(y)]]), "bf16"), kc, vc, own.put(starts_of([rows]), "i32"),
+                                own.put(np.array([keys]), "i32"), own.put(np.arange(cols)[None], "i32"), out, lse=lse, workspace=own.scratch(max(4, need)))
+        hit = np.zeros((rows, heads), bool)
+        hit[1, 1] = True
+        of_that_row_only(rows, hit)
+
+
 # page, table's columns, lengths, new rows, heads, kv heads, dim, rows behind
 CACHES = [(16, 4, [20, 64, 1], [1, 1, 1], 4, 2, 64, 0), (16, 40, [40, 7, 0], [1, 1, 0], 2, 1, 128, 2), (64, 3, [130, 192, 64, 65], [1, 0, 1, 1], 8, 1, 80, 1),
           (16, 20, [300, 17], [40, 17], 4, 4, 128, 0), (256, 8, [2000, 1000, 5], [130, 1, 5], 8, 2, 128, 3), (32, 64, [2048], [1], 32, 8, 128, 0),

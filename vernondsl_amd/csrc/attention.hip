@@ -183,14 +183,15 @@ __device__ __forceinline__ void store_rows(const AttentionArgs& a, RowState<DP>&
   int64_t base;
   if (a.splits > 1) {
     const int64_t place = (static_cast<int64_t>(split) * a.kv_heads + kv) * a.seqs.n * a.group + at.token * a.group + row;
-    if (lane < 32) a.stats[place] = make_float2(st.m, l);
-    if (st.m == neg_inf()) return;  // not read
+    // scores that are NaN all of them leave m as it was: the join has to see them
+    if (lane < 32) a.stats[place] = make_float2(st.m == neg_inf() && l != 0.0f ? l : st.m, l);
+    if (l == 0.0f) return;  // not read
     by = 1.0f;
     base = place * a.dim;
   } else {
     if (a.lse && lane < 32)
-      a.lse[head * a.seqs.n + token] = st.m == neg_inf() ? neg_inf() : (st.m + __builtin_amdgcn_logf(l)) * kLn2;
-    by = st.m == neg_inf() ? 0.0f : 1.0f / l;
+      a.lse[head * a.seqs.n + token] = l == 0.0f ? neg_inf() : (st.m + __builtin_amdgcn_logf(l)) * kLn2;
+    by = l == 0.0f ? 0.0f : 1.0f / l;  // 0: nothing seen, or scores of -inf (the largest score has p >= 1)
     base = (token * a.heads + head) * a.dim;
   }
 #pragma unroll
@@ -405,6 +406,7 @@ __global__ __launch_bounds__(64, 2) void attention_few(AttentionArgs a) {
   }
   if (2 * a.dim < T::PITCH) {  // columns past dim are never copied
     for (int i = lane; i < 2 * SLOT / 16; i += 64) reinterpret_cast<u32x4*>(smem)[i] = u32x4{0u, 0u, 0u, 0u};
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   }
   const KeySource<DP, true> src(a, tile, most, place.kv);
   int page0 = src.page(first * KT), page1 = src.page(first * KT + 16);
@@ -517,7 +519,7 @@ __global__ __launch_bounds__(256) void attention_join(AttentionArgs a) {
   const int kv = static_cast<int>(r / rows);
   const int64_t token = r % rows / a.group;
   const int head = kv * a.group + static_cast<int>(r % rows % a.group);
-  const bool none = m == neg_inf();
+  const bool none = l == 0.0f;
   if (a.lse && col == 0) a.lse[head * a.seqs.n + token] = none ? neg_inf() : (m + __builtin_amdgcn_logf(l)) * kLn2;
   if (col >= a.dim) return;
 #pragma unroll
@@ -665,8 +667,8 @@ int paged_check(const char* op, const vdsl_paged_params* p) {
   if (p->pages < 0 || p->table_cols < 0 || p->page <= 0) return fail(VDSL_ERR_INVALID_ARG, std::string(op) + ": negative shape or no page size");
   if ((p->page & (p->page - 1)) || p->page < 16 || p->page > 65536)
     return fail(VDSL_ERR_UNSUPPORTED, std::string(op) + ": page must be a power of two from 16 to 65536");
-  if (p->pages > 0x7fffffff || p->table_cols > 0x7fffffff / p->page)
-    return fail(VDSL_ERR_UNSUPPORTED, std::string(op) + ": 2^31 positions a sequence or more");
+  if (p->pages > 0x7fffffff || p->table_cols > 0x7fff0000 / p->page)  // a tile further is still below 2^31
+    return fail(VDSL_ERR_UNSUPPORTED, std::string(op) + ": more than 2^31 - 2^16 positions a sequence");
   return VDSL_OK;
 }
 AttentionArgs paged_args(const vdsl_paged_params* p, vdsl_buffer starts, vdsl_buffer lengths, vdsl_buffer table) {

@@ -1,5 +1,7 @@
 """Attention over packed sequences and over a paged cache, the append to it, and rotary positions on the device against
 attention64's plain forms in 64 bits, at the lengths, layouts and masks where they can go wrong."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
@@ -287,6 +289,41 @@ def test_pages_that_are_none(q, own, rows):
     check(get(q, lse), want_lse, el, "lse")
     check(get(q, out).reshape(n, heads, dim), want, eo + rounding("f32", want), "out")
     assert not get(q, out)[rows:2 * rows].any()  # a sequence without a page
+
+
+def test_nothing_there(q, own):
+    """No rows, no sequences, no pages, a table without columns: nothing read, every row written."""
+    n, heads, kv, dim = 5, 2, 1, 16
+    x, one = own.put(np.ones((n, heads, dim)), "bf16"), own.put(np.zeros(2), "i32")
+    at = _lib.Heads(0, heads * dim), _lib.Heads(0, kv * dim)
+    k = own.put(np.ones((n, kv, dim)), "bf16")
+
+    def paged(rows, seqs, pages, cols):
+        return _lib.PagedParams(rows, seqs, pages, cols, 16, heads, kv, dim, 0.25, 0, at[0], at[1], at[1])
+
+    lengths, table = own.put(np.full(2, 30), "i32"), own.put(np.zeros(4), "i32")
+    cache = [own.put(np.full((1, kv, 16, dim), 3.0), "bf16") for _ in range(2)]
+    for rows, seqs in ((0, 0), (0, 1), (n, 0)):
+        out, lse = own.empty((n, heads * dim), "f32"), own.empty((heads, n), "f32")
+        p = _lib.AttentionParams(rows, seqs, heads, kv, dim, 1, 0.25, 0, at[0], at[1], at[1], at[0], at[1], at[1])
+        _lib.call("vdsl_op_attention_fwd", q.handle, C.byref(p), x.handle, k.handle, k.handle, one.handle, 0, out.handle, lse.handle)
+        assert np.array_equal(get(q, out)[:rows], np.zeros((rows, heads * dim))) and np.isnan(get(q, out)[rows:]).all()
+        assert np.isneginf(get(q, lse)).all() if rows else np.isnan(get(q, lse)).all()
+        g = [own.empty((n, h, dim), "f32") for h in (heads, kv, kv)]
+        ws = own.scratch(kernels.attention_bwd_workspace_bytes(rows, seqs, heads, kv, dim))
+        _lib.call("vdsl_op_attention_bwd", q.handle, C.byref(p), 1, x.handle, x.handle, k.handle, k.handle, one.handle, 0, out.handle,
+                  lse.handle, 0, g[0].handle, g[1].handle, g[2].handle, ws.handle)
+        assert all(not get(q, y)[:rows].any() and np.isnan(get(q, y)[rows:]).all() for y in g)
+    starts = own.put(starts_of([n]), "i32")
+    for rows, seqs, pages, cols in ((0, 1, 1, 4), (n, 0, 1, 4), (n, 1, 0, 4), (n, 1, 1, 0)):
+        p, out = paged(rows, seqs, pages, cols), own.empty((n, heads * dim), "f32")
+        need = kernels.paged_attention_workspace_bytes(rows, seqs, heads, kv, dim, cols * 16)
+        _lib.call("vdsl_op_cache_append", q.handle, C.byref(p), k.handle, k.handle, starts.handle, lengths.handle, table.handle,
+                  cache[0].handle, cache[1].handle)
+        assert all((get(q, y) == 3.0).all() for y in cache)
+        _lib.call("vdsl_op_paged_attention", q.handle, C.byref(p), x.handle, cache[0].handle, cache[1].handle, starts.handle,
+                  lengths.handle, table.handle, 0, out.handle, None, own.scratch(max(4, need)).handle)
+        assert not get(q, out)[:rows].any() and np.isnan(get(q, out)[rows:]).all()
 
 
 def test_cache_past_32_bits(dev, q, own):

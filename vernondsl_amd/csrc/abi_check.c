@@ -309,6 +309,107 @@ int main(void) {
     for (size_t k = 0; k < sizeof bufs / sizeof bufs[0]; ++k) EXPECT_OK(vdsl_buffer_free(bufs[k]));
   }
 
+  /* ---- op class 7: rotary positions, attention over packed sequences, a paged cache ---- */
+  {
+    const int64_t n = 20, heads = 4, kv = 2, dim = 16, width = (heads + 2 * kv) * dim, pages = 4, page = 16;
+    vdsl_buffer x = alloc(d, (size_t)(n * width * 2)), y = alloc(d, (size_t)(n * width * 2)), dx = alloc(d, (size_t)(n * width * 2));
+    vdsl_buffer ints = alloc(d, 256), freqs = alloc(d, 64), out = alloc(d, (size_t)(n * heads * dim * 4)), lse = alloc(d, (size_t)(n * heads * 4));
+    vdsl_buffer dout = alloc(d, (size_t)(n * heads * dim * 2)), kc = alloc(d, (size_t)(pages * kv * page * dim * 2));
+    vdsl_buffer vc = alloc(d, (size_t)(pages * kv * page * dim * 2)), lengths = alloc(d, 8), table = alloc(d, 16);
+    int32_t id[64], starts[3] = {0, 7, 20}, have[2] = {7, 30}, tab[4] = {2, -1, 0, 3}; /* the first sequence has one page */
+    for (int k = 0; k < 64; ++k) id[k] = k;
+    vdsl_buffer st = alloc(d, sizeof starts);
+    EXPECT_OK(vdsl_buffer_write(q, ints, 0, id, sizeof id));
+    EXPECT_OK(vdsl_buffer_write(q, st, 0, starts, sizeof starts));
+    EXPECT_OK(vdsl_buffer_write(q, lengths, 0, have, sizeof have));
+    EXPECT_OK(vdsl_buffer_write(q, table, 0, tab, sizeof tab));
+    EXPECT_OK(vdsl_queue_sync(q));
+    fill_bf16(q, x, (size_t)(n * width));
+    fill_bf16(q, dout, (size_t)(n * heads * dim));
+    fill_bf16(q, kc, (size_t)(pages * kv * page * dim));
+    fill_bf16(q, vc, (size_t)(pages * kv * page * dim));
+    fill_f32(q, freqs, 16, 0.01f);
+    vdsl_rope_params r = {n, width, 0, (int32_t)(heads + kv), (int32_t)dim, (int32_t)dim / 2, 0, 0, 1.0f};
+    EXPECT_OK(vdsl_op_rope(q, &r, VDSL_BF16, x, ints, freqs, VDSL_BF16, y));
+    EXPECT_OK(vdsl_op_rope(q, &r, VDSL_BF16, y, ints, freqs, VDSL_BF16, y));
+    EXPECT_ERR(vdsl_op_rope(q, NULL, VDSL_BF16, x, ints, freqs, VDSL_BF16, y));
+    EXPECT_ERR(vdsl_op_rope(q, &r, VDSL_F32, x, ints, freqs, VDSL_BF16, y));  /* x is one of bf16's size */
+    EXPECT_ERR(vdsl_op_rope(q, &r, VDSL_BF16, x, ints, y, VDSL_BF16, y));
+    vdsl_rope_params r2 = r;
+    r2.pairs = (int32_t)dim / 2 + 1;
+    EXPECT_ERR(vdsl_op_rope(q, &r2, VDSL_BF16, x, ints, freqs, VDSL_BF16, y));
+    r2 = r, r2.first = 3 * dim;
+    EXPECT_ERR(vdsl_op_rope(q, &r2, VDSL_BF16, x, ints, freqs, VDSL_BF16, y));
+    r2 = r, r2.rows = kHuge;
+    EXPECT_ERR(vdsl_op_rope(q, &r2, VDSL_BF16, x, ints, freqs, VDSL_BF16, y));
+
+    const vdsl_heads hq = {0, width}, hk = {heads * dim, width}, hv = {(heads + kv) * dim, width};
+    const vdsl_attention_params a = {n, 2, (int32_t)heads, (int32_t)kv, (int32_t)dim, 1, 0.25f, 0, hq, hk, hv, hq, hk, hv};
+    EXPECT_OK(vdsl_op_attention_fwd(q, &a, y, y, y, st, VDSL_F32, out, lse));
+    EXPECT_OK(vdsl_op_attention_fwd(q, &a, y, y, y, st, VDSL_BF16, out, NULL));
+    EXPECT_OK(vdsl_op_attention_fwd(q, &a, y, y, y, st, VDSL_F32, out, lse));
+    EXPECT_ERR(vdsl_op_attention_fwd(q, NULL, y, y, y, st, VDSL_F32, out, lse));
+    EXPECT_ERR(vdsl_op_attention_fwd(NULL, &a, y, y, y, st, VDSL_F32, out, lse));
+    EXPECT_ERR(vdsl_op_attention_fwd(q, &a, y, y, y, st, VDSL_I8, out, lse));
+    EXPECT_ERR(vdsl_op_attention_fwd(q, &a, y, y, y, st, VDSL_F32, lse, lse));
+    EXPECT_ERR(vdsl_op_attention_fwd(q, &a, y, NULL, y, st, VDSL_F32, out, lse));
+    vdsl_attention_params a2 = a;
+    a2.n = n + 1;
+    EXPECT_ERR(vdsl_op_attention_fwd(q, &a2, y, y, y, st, VDSL_F32, out, lse));
+    a2.n = kHuge;
+    EXPECT_ERR(vdsl_op_attention_fwd(q, &a2, y, y, y, st, VDSL_F32, out, lse));
+    a2 = a, a2.seqs = 3;
+    EXPECT_ERR(vdsl_op_attention_fwd(q, &a2, y, y, y, st, VDSL_F32, out, lse));
+    a2 = a, a2.v.first = hv.first + 8;
+    EXPECT_ERR(vdsl_op_attention_fwd(q, &a2, y, y, y, st, VDSL_F32, out, lse)); /* past the end */
+    a2 = a, a2.v.first = kHuge;
+    EXPECT_ERR(vdsl_op_attention_fwd(q, &a2, y, y, y, st, VDSL_F32, out, lse));
+    a2 = a, a2.k.stride = kv * dim - 8;
+    EXPECT_ERR(vdsl_op_attention_fwd(q, &a2, y, y, y, st, VDSL_F32, out, lse));
+    a2 = a, a2.scale = NAN;
+    EXPECT_ERR(vdsl_op_attention_fwd(q, &a2, y, y, y, st, VDSL_F32, out, lse));
+    size_t ws = 0;
+    EXPECT_ERR(vdsl_attention_bwd_workspace_bytes(n, 2, 4, 3, 16, &ws));
+    EXPECT_ERR(vdsl_attention_bwd_workspace_bytes(kHuge, 2, 4, 2, 16, &ws));
+    EXPECT_ERR(vdsl_attention_bwd_workspace_bytes(n, 2, 4, 2, 16, NULL));
+    EXPECT_OK(vdsl_attention_bwd_workspace_bytes(n, 2, 4, 2, 16, &ws));
+    vdsl_buffer wb = alloc(d, ws), little = alloc(d, ws - 4);
+    EXPECT_OK(vdsl_op_attention_bwd(q, &a, VDSL_BF16, dout, y, y, y, st, VDSL_F32, out, lse, VDSL_BF16, dx, dx, dx, wb));
+    EXPECT_ERR(vdsl_op_attention_bwd(q, &a, VDSL_BF16, dout, y, y, y, st, VDSL_F32, out, lse, VDSL_BF16, dx, dx, dx, little));
+    EXPECT_ERR(vdsl_op_attention_bwd(q, &a, VDSL_BF16, dout, y, y, y, st, VDSL_F32, out, lse, VDSL_F32, dx, dx, dx, wb));
+    EXPECT_ERR(vdsl_op_attention_bwd(q, &a, VDSL_BF16, dout, y, y, y, st, VDSL_F32, out, lse, VDSL_BF16, dx, y, dx, wb));
+    a2 = a, a2.dk.first = dim;
+    EXPECT_ERR(vdsl_op_attention_bwd(q, &a2, VDSL_BF16, dout, y, y, y, st, VDSL_F32, out, lse, VDSL_BF16, dx, dx, dx, wb));
+
+    const vdsl_paged_params c7 = {n, 2, pages, 2, (int32_t)page, (int32_t)heads, (int32_t)kv, (int32_t)dim, 0.25f, 0, hq, hk, hv};
+    EXPECT_OK(vdsl_op_cache_append(q, &c7, y, y, st, lengths, table, kc, vc));
+    EXPECT_ERR(vdsl_op_cache_append(q, &c7, y, y, st, lengths, table, kc, kc));
+    EXPECT_ERR(vdsl_op_cache_append(q, NULL, y, y, st, lengths, table, kc, vc));
+    EXPECT_ERR(vdsl_paged_attention_workspace_bytes(n, 2, 4, 2, 16, -1, &ws));
+    EXPECT_ERR(vdsl_paged_attention_workspace_bytes(n, 2, 4, 2, 16, 32, NULL));
+    EXPECT_OK(vdsl_paged_attention_workspace_bytes(n, 2, 4, 2, 16, INT64_MAX, &ws));
+    EXPECT_OK(vdsl_paged_attention_workspace_bytes(n, 2, 4, 2, 16, 32, &ws));
+    EXPECT_OK(vdsl_op_paged_attention(q, &c7, y, kc, vc, st, lengths, table, VDSL_F32, out, lse, ws ? wb : NULL));
+    vdsl_paged_params c2 = c7;
+    c2.page = 8;
+    EXPECT_ERR(vdsl_op_paged_attention(q, &c2, y, kc, vc, st, lengths, table, VDSL_F32, out, lse, wb));
+    c2 = c7, c2.pages = pages + 1;
+    EXPECT_ERR(vdsl_op_paged_attention(q, &c2, y, kc, vc, st, lengths, table, VDSL_F32, out, lse, wb));
+    c2 = c7, c2.table_cols = INT64_MAX;
+    EXPECT_ERR(vdsl_op_paged_attention(q, &c2, y, kc, vc, st, lengths, table, VDSL_F32, out, lse, wb));
+    c2 = c7, c2.seqs = 3;
+    EXPECT_ERR(vdsl_op_paged_attention(q, &c2, y, kc, vc, st, lengths, table, VDSL_F32, out, lse, wb));
+    EXPECT_ERR(vdsl_op_paged_attention(q, &c7, y, kc, vc, st, lengths, table, VDSL_F32, y, lse, wb));
+    EXPECT_OK(vdsl_queue_sync(q));
+    float got[80];
+    EXPECT_OK(vdsl_buffer_read(q, lse, 0, got, sizeof got));
+    EXPECT_OK(vdsl_queue_sync(q));
+    for (int k = 0; k < 80; ++k)
+      if (!isfinite(got[k])) { printf("FAIL paged_attention lse %d: %g\n", k, got[k]); ++g_fails; break; }
+    vdsl_buffer bufs[] = {x, y, dx, ints, freqs, out, lse, dout, kc, vc, lengths, table, st, wb, little};
+    for (size_t k = 0; k < sizeof bufs / sizeof bufs[0]; ++k) EXPECT_OK(vdsl_buffer_free(bufs[k]));
+  }
+
   /* ---- graphs and events ---- */
   vdsl_graph g = NULL;
   EXPECT_ERR(vdsl_graph_end(q, &g)); /* not recording */

@@ -65,7 +65,9 @@ PACKED = [([1], 0, 0, 1, 1, 8, True), ([2, 0, 1], 1, 2, 2, 1, 16, True), ([33], 
           ([513], 0, 0, 2, 1, 104, False), ([0, 0], 0, 9, 2, 1, 64, True), ([90] * 70, 0, 0, 2, 2, 32, True),
           ([4200], 0, 0, 16, 2, 64, True), ([2300, 2000], 0, 11, 16, 4, 128, True), ([4100], 0, 0, 16, 2, 88, False),
           # as above, with so many kv heads that the gradient's blocks have 128 keys
-          ([1100], 0, 0, 32, 32, 8, True), ([1000, 50], 0, 3, 40, 40, 128, True), ([500, 0, 600], 2, 0, 64, 32, 64, True), ([700], 0, 0, 32, 32, 96, False)]
+          ([1100], 0, 0, 32, 32, 8, True), ([1000, 50], 0, 3, 40, 40, 128, True), ([500, 0, 600], 2, 0, 64, 32, 64, True), ([700], 0, 0, 32, 32, 96, False),
+          # few kv heads that many share, whose rows the gradient splits
+          ([700], 0, 5, 64, 1, 128, True), ([40, 900, 3], 1, 0, 12, 2, 72, False)]
 
 
 @pytest.mark.parametrize("lengths,front,back,heads,kv,dim,causal", PACKED)
@@ -120,7 +122,7 @@ def test_packed(q, own, lengths, front, back, heads, kv, dim, causal):
 
 
 @pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
-@pytest.mark.parametrize("dim,heads,kv,n,at", [(64, 2, 1, 200, 70), (128, 4, 2, 333, 150), (80, 1, 1, 100, 99), (64, 40, 40, 900, 400), (128, 72, 36, 1000, 530)])
+@pytest.mark.parametrize("dim,heads,kv,n,at", [(64, 2, 1, 200, 70), (128, 4, 2, 333, 150), (80, 1, 1, 100, 99), (64, 40, 40, 900, 400), (128, 72, 36, 1000, 530), (128, 16, 1, 400, 130)])
 def test_what_is_not_seen_has_no_influence(q, own, dim, heads, kv, n, at, bad):
     """Rows from `at` on hold NaN or infinities: the rows before have the outputs that they would have alone, and their dq too;
     rows before `at` whose q and dout are so leave the gradients of the keys from `at` on alone."""

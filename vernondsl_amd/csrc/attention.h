@@ -122,6 +122,13 @@ __device__ __forceinline__ void load_operand(const uint16_t* p, int dim, bf16x8 
   }
 }
 
+// threadIdx.x where what follows from it is to be formed there and not kept through a loop.
+__device__ __forceinline__ int late_thread() {
+  int t = threadIdx.x;
+  asm volatile("" : "+v"(t));
+  return t;
+}
+
 // A wave's copies of ROWS rows of two operands to LDS: from scalar addresses and offsets that a lane keeps.
 template <int DP, int ROWS>
 struct RowCopies {
@@ -153,7 +160,7 @@ struct RowCopies {
       }
       return;
     }
-    const int lane = threadIdx.x & 63;
+    const int lane = late_thread() & 63;
 #pragma unroll
     for (int u = 0; u < C; ++u) {
       if (a_off[u] == ~0u) continue;
@@ -235,6 +242,15 @@ __device__ __forceinline__ bool any_not_finite(const f32x16& v) {
   for (int r = 0; r < 16; ++r) z = __builtin_fmaf(v[r], 0.0f, z);
   return __any(z != z);
 }
+// sum plus the product of 8 bf16 elements each.
+__device__ __forceinline__ float dot8(u32x4 x, u32x4 y, float sum) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    sum = __builtin_fmaf(__uint_as_float(x[j] << 16), __uint_as_float(y[j] << 16), sum);
+    sum = __builtin_fmaf(__uint_as_float(x[j] & 0xFFFF0000u), __uint_as_float(y[j] & 0xFFFF0000u), sum);
+  }
+  return sum;
+}
 // This half's share of the product of the lane's row, held as an operand, and the row at p (the same for all lanes).  (The
 // scheduling barriers, here and below: this is rare, and loads side by side would take registers from the main loops.)
 template <int DP>
@@ -244,12 +260,7 @@ __device__ __forceinline__ float half_dot(const bf16x8 (&f)[DP / 16], const uint
   for (int kk = 0; kk < DP / 16; ++kk) {
     const int col = 16 * kk + 8 * ((threadIdx.x & 63) >> 5);
     if (col >= dim) continue;
-    const u32x4 x = *reinterpret_cast<const u32x4*>(p + col), y = __builtin_bit_cast(u32x4, f[kk]);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      sum = __builtin_fmaf(__uint_as_float(x[j] << 16), __uint_as_float(y[j] << 16), sum);
-      sum = __builtin_fmaf(__uint_as_float(x[j] & 0xFFFF0000u), __uint_as_float(y[j] & 0xFFFF0000u), sum);
-    }
+    sum = dot8(*reinterpret_cast<const u32x4*>(p + col), __builtin_bit_cast(u32x4, f[kk]), sum);
     __builtin_amdgcn_sched_barrier(0);
   }
   return sum;

@@ -22,16 +22,28 @@ struct GradArgs {
   const uint16_t *q, *k, *v, *dout;  // dout: bf16
   int64_t q_stride, k_stride, v_stride, dout_stride;
   Sequences seqs;
-  int* left_out;      // by the waves of attention_bwd_keys
-  int key_log;        // log2 of the keys of one of its blocks
+  int* left_out;      // rows, by each wave of the keys' blocks
+  float* parts;       // of splits: dk and dv, f32 [splits][2][kv_heads][n][dim]
+  int key_log;        // log2 of the keys of a block
+  int key_splits;     // of the rows that see them
   const float* rows;  // -lse / scale, then -delta, each [kv_heads][n * group]
   void *dq, *dk, *dv;
   int64_t dq_first, dq_stride, dk_first, dk_stride, dv_first, dv_stride;
   int heads, kv_heads, group, dim, causal, grad_dtype;
   float scale;
   Divider token_of;
-  int blocks;
+  int blocks;      // row slots of attention_bwd_queries
+  int key_blocks;  // attention_bwd_both's blocks that are of keys
 };
+
+// The kernel's arguments, read again: what only the end of a kernel takes would hold scalar registers through its main loop, which
+// has none to spare.
+__device__ __forceinline__ const GradArgs& late_args() {
+  typedef const __attribute__((address_space(4))) GradArgs* Args;
+  Args p = (Args)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const GradArgs*)p;
+}
 
 // What a row's scores and dp start from, -lse / scale and -delta, and dout in bf16 where it is f32.  16 lanes a row of one head.
 __global__ __launch_bounds__(256) void attention_bwd_rows(const void* __restrict__ dout, int dout_dtype, const void* __restrict__ out,
@@ -66,20 +78,39 @@ __global__ __launch_bounds__(256) void attention_bwd_rows(const void* __restrict
   to[n * heads] = -sum;
 }
 
-// acc (columns x rows: this lane has columns 32 d + 8 g + 4 (l / 32) + j of its own row) times `by` to element e of `to`.
+// The sums of a block's waves by way of LDS, so that whole rows are stored and by code of a few lines (an unrolled store of what a lane
+// has reads as many instructions as the main loop, which short calls wait for).  Of its 32 x DP sums (column 32 d + 8 g +
+// 4 (l / 32) + j of row l % 32) a wave leaves 4 columns in a place of 528 bytes.  Then 32 * GROUPS rows of `by` times the sums of
+// PARTS waves, w, w + GROUPS, ..: at(row) is the element of its column 0, less than 0 for none.
 template <int DP>
-__device__ __forceinline__ void store_gradient(const f32x16 (&acc)[DP / 32], float by, int dtype, void* to, int64_t e, int dim) {
+constexpr int kSumBytes = DP / 4 * 528;
+template <int DP, int GROUPS, int PARTS, class At>
+__device__ __forceinline__ void store_sums(const f32x16 (&acc)[DP / 32], float by, int dim, int dtype, void* to, char* smem, At&& at) {
+  const int thread = late_thread(), lane = thread & 63, wave = thread >> 6;
+  __syncthreads();
+  char* const mine = smem + wave * kSumBytes<DP> + (lane >> 5) * 528 + (lane & 31) * 16;
 #pragma unroll
   for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int col = 32 * d + 8 * g + 4 * ((threadIdx.x & 63) >> 5);
-      if (col >= dim) continue;
-      float v[4];
+    for (int g = 0; g < 4; ++g)
+      *reinterpret_cast<f32x4*>(mine + (4 * d + g) * 1056) = f32x4{acc[d][4 * g], acc[d][4 * g + 1], acc[d][4 * g + 2], acc[d][4 * g + 3]};
+  __syncthreads();
+#pragma unroll 1
+  for (int u = thread; u < 32 * GROUPS * (DP / 4); u += 64 * GROUPS * PARTS) {
+    const int row = u / (DP / 4), c = u % (DP / 4);
+    const int64_t e = at(row);
+    if (4 * c >= dim || e < 0) continue;
+    const char* const from = smem + (row >> 5) * kSumBytes<DP> + c * 528 + (row & 31) * 16;
+    f32x4 v = *reinterpret_cast<const f32x4*>(from);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = acc[d][4 * g + j] * by;
-      store_unit<4>(dtype, to, e + col, v);
+    for (int o = 1; o < PARTS; ++o) {
+      const f32x4 x = *reinterpret_cast<const f32x4*>(from + o * GROUPS * kSumBytes<DP>);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] += x[j];
     }
+    const float w[4] = {v[0] * by, v[1] * by, v[2] * by, v[3] * by};
+    store_unit<4>(dtype, to, e + 4 * c, w);
+  }
 }
 __device__ __forceinline__ void store_zeros(int dtype, void* to, int64_t e, int cols) {
   const float none[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -90,22 +121,38 @@ __device__ __forceinline__ void store_zeros(int dtype, void* to, int64_t e, int 
 // have 8 / (KEYS / 32) waves, one for each 32 rows of a tile, which add up their sums at the end.  Two waves share a SIMD,
 // and one has priority there, so that its exponentials come beside the other's products.  To leave both their
 // registers, wide heads' values are an operand read from LDS (V_LDS).
+// The tiles of TR rows that see a block's keys, and how many of them a split has.
+struct RowShare {
+  int first, end, tiles;
+  __device__ __forceinline__ RowShare(const GradArgs& a, const RowTile& t, int TR)
+      : first(a.causal ? t.row * a.group / TR : 0), end((t.len * a.group + TR - 1) / TR), tiles((end - first + a.key_splits - 1) / a.key_splits) {}
+};
 template <int DP, int KEYS>
-__global__ __launch_bounds__(512, 2) void attention_bwd_keys(GradArgs a) {
-  constexpr int NW = 8, GROUPS = KEYS / 32, PARTS = NW / GROUPS, TR = 32 * PARTS;
-  constexpr bool V_LDS = DP > 96;
+struct KeysShape {
+  static constexpr int NW = 8, GROUPS = KEYS / 32, PARTS = NW / GROUPS, TR = 32 * PARTS;
+  static constexpr bool V_LDS = DP > 96;
+  static constexpr int SUMS = NW * kSumBytes<DP>;
+  static constexpr int NS = PARTS == 2 ? 3 : 2, SLOT = 2 * TR * TileShape<DP>::PITCH;
+  static constexpr int TILES = NS * SLOT + (V_LDS ? KEYS * TileShape<DP>::PITCH : 0), AREA = TILES > SUMS ? TILES : SUMS;
+  static constexpr int BYTES = AREA + NW * NS * 2 * 32 * 4;
+};
+template <int DP, int KEYS>
+__device__ __forceinline__ void keys_block(const GradArgs& a, int b, char* smem) {
+  using S = KeysShape<DP, KEYS>;
+  constexpr int NW = S::NW, GROUPS = S::GROUPS, PARTS = S::PARTS, TR = S::TR, NS = S::NS, SLOT = S::SLOT;
+  constexpr bool V_LDS = S::V_LDS;
   using T = TileShape<DP>;
   constexpr int CR = TR / NW;  // of a tile's rows a wave copies
   using Copies = RowCopies<DP, CR>;
-  constexpr int SUMS = (NW - GROUPS) * 32 * DP * 4;  // one gradient's sums of all but the first parts
-  constexpr int NS = PARTS == 2 ? 3 : 2, SLOT = 2 * TR * T::PITCH, AREA = NS * SLOT + (V_LDS ? KEYS * T::PITCH : 0);
-  __shared__ __attribute__((aligned(1024))) char smem[AREA > SUMS ? AREA : SUMS];
-  __shared__ __attribute__((aligned(16))) float starts[NW][NS][2][32];  // what the rows' scores and dp start from, a copy a wave
-  int b = static_cast<int>(blockIdx.x);
+  // what the rows' scores and dp start from, a copy a wave: [NS][2][32] each
+  float* const starts = reinterpret_cast<float*>(smem + S::AREA) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * (NS * 64);
+  int* const left_out_to = a.left_out + b * NW;
   const int kv = b % a.kv_heads;
-  const RowTile tile = row_tile<KEYS == 128 ? 7 : 6>(a.seqs, 1, b / a.kv_heads);
+  b /= a.kv_heads;
+  const int split = b % a.key_splits;
+  const RowTile tile = row_tile<KEYS == 128 ? 7 : 6>(a.seqs, 1, b / a.key_splits);
   if (!tile.any) {
-    if (threadIdx.x < NW) a.left_out[blockIdx.x * NW + threadIdx.x] = 0;
+    if (threadIdx.x < NW) left_out_to[threadIdx.x] = 0;
     return;
   }
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
@@ -113,8 +160,8 @@ __global__ __launch_bounds__(512, 2) void attention_bwd_keys(GradArgs a) {
   const int key0 = tile.row + 32 * (wave % GROUPS), key = key0 + (lane & 31);
   const int64_t head_col = static_cast<int64_t>(kv) * a.dim;
   if (tile.seq < 0) {
-    if (lane == 0) a.left_out[blockIdx.x * NW + wave] = 0;
-    if (key < tile.len && half == 0 && part == 0) {
+    if (lane == 0) left_out_to[wave] = 0;
+    if (key < tile.len && half == 0 && part == 0 && split == 0) {
       store_zeros(a.grad_dtype, a.dk, a.dk_first + (tile.token + key) * a.dk_stride + head_col, a.dim);
       store_zeros(a.grad_dtype, a.dv, a.dv_first + (tile.token + key) * a.dv_stride + head_col, a.dim);
     }
@@ -135,7 +182,8 @@ __global__ __launch_bounds__(512, 2) void attention_bwd_keys(GradArgs a) {
       *reinterpret_cast<bf16x8*>(values + (lane & 31) * T::PITCH + (((2 * kk + half) ^ T::swz(lane & 31)) << 4)) = vf[kk];
   }
   const int rows = tile.len * a.group;
-  const int first = a.causal ? tile.row * a.group / TR : 0, end = (rows + TR - 1) / TR;
+  const RowShare share(a, tile, TR);
+  const int first = share.first + split * share.tiles, end = min(first + share.tiles, share.end);
   const char* const qp = reinterpret_cast<const char*>(a.q + tile.token * a.q_stride + head_col * a.group);
   const char* const dp = reinterpret_cast<const char*>(a.dout + tile.token * a.dout_stride + head_col * a.group);
   const float* const sp = a.rows + (static_cast<int64_t>(kv) * a.seqs.n + tile.token) * a.group;
@@ -156,7 +204,7 @@ __global__ __launch_bounds__(512, 2) void attention_bwd_keys(GradArgs a) {
     if (!whole_tokens) offsets(row0, token0);
     char* const area = smem + slot * SLOT + CR * wave * T::PITCH;
     copies.copy(qp + 2 * (token0 * a.q_stride), dp + 2 * (token0 * a.dout_stride), last - CR * wave, area, area + TR * T::PITCH);
-    float* const to = starts[wave][slot][0];
+    float* const to = starts + 64 * slot;
     const int r = 32 * part + (lane & 31);
     // rows that are not there: no weight
     if (r <= last) lds_copy4(reinterpret_cast<const char*>(sp + (half ? delta_at : 0) + t * TR + r), reinterpret_cast<char*>(to));
@@ -171,7 +219,7 @@ __global__ __launch_bounds__(512, 2) void attention_bwd_keys(GradArgs a) {
   const int one_seen = a.causal ? key0 * a.group : 0, all_seen = a.causal ? (key0 + 31) * a.group : 0;
   int left_out = 0;  // rows before this one: attention_bwd_left_out adds them
   // All blocks begin with the last rows, which they all see, and so read the same rows at about the same time.
-  fetch(end - 1, 0);
+  if (end > first) fetch(end - 1, 0);
   if (NS == 3 && end - 2 >= first) fetch(end - 2, 1);
   int slot = 0;
   if (wave < 4) __builtin_amdgcn_s_setprio(1);
@@ -184,7 +232,7 @@ __global__ __launch_bounds__(512, 2) void attention_bwd_keys(GradArgs a) {
     if (t - (NS - 1) >= first) fetch(t - (NS - 1), slot == 0 ? NS - 1 : slot - 1);
     const char* const qs = smem + slot * SLOT + part * 32 * T::PITCH;
     const char* const ds = qs + TR * T::PITCH;
-    const float* const x = starts[wave][slot][0] + 4 * half;
+    const float* const x = starts + 64 * slot + 4 * half;
     slot = slot == NS - 1 ? 0 : slot + 1;
     const int r0 = t * TR + 32 * part;
     if (r0 + 32 <= one_seen || r0 >= rows) continue;
@@ -237,129 +285,157 @@ __global__ __launch_bounds__(512, 2) void attention_bwd_keys(GradArgs a) {
     }
   }
   __builtin_amdgcn_s_setprio(0);
-  if (lane == 0) a.left_out[blockIdx.x * NW + wave] = left_out;
-  // the other parts' sums by way of LDS, one gradient after the other
-  float* const sums = reinterpret_cast<float*>(smem) + lane * 4;
-  const auto join = [&](f32x16 (&acc)[DP / 32]) {
-    __syncthreads();
-    if (part != 0) {
-#pragma unroll
-      for (int d = 0; d < DP / 32; ++d)
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-          *reinterpret_cast<f32x4*>(sums + (wave - GROUPS) * DP * 32 + (4 * d + g) * 256) = f32x4{acc[d][4 * g], acc[d][4 * g + 1], acc[d][4 * g + 2], acc[d][4 * g + 3]};
-    }
-    __syncthreads();
-    if (part == 0) {
-#pragma unroll
-      for (int o = 0; o < PARTS - 1; ++o)
-#pragma unroll
-        for (int d = 0; d < DP / 32; ++d)
-#pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const f32x4 v = *reinterpret_cast<const f32x4*>(sums + (wave + o * GROUPS) * DP * 32 + (4 * d + g) * 256);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) acc[d][4 * g + j] += v[j];
-          }
-    }
+  if ((late_thread() & 63) == 0) left_out_to[wave] = left_out;
+  const GradArgs& z = late_args();
+  const bool whole = z.key_splits == 1;
+  const int place = static_cast<int>(blockIdx.x), kv_head = place % z.kv_heads, row_split = place / z.kv_heads % z.key_splits;
+  const auto store = [&](const f32x16 (&acc)[DP / 32], float by, void* to, int64_t first, int64_t stride, int which) {
+    const int64_t e = whole ? first + static_cast<int64_t>(kv_head) * z.dim : ((2 * row_split + which) * z.kv_heads + kv_head) * z.seqs.n * z.dim;
+    const int64_t step = whole ? stride : z.dim;
+    store_sums<DP, GROUPS, PARTS>(acc, by, z.dim, whole ? z.grad_dtype : static_cast<int>(VDSL_F32), whole ? to : z.parts, smem,
+                                  [&](int r) { return tile.row + r < tile.len ? e + (tile.token + tile.row + r) * step : -1; });
   };
-  join(dk);
-  join(dv);
-  if (part == 0 && key < tile.len) {
-    store_gradient<DP>(dk, a.scale, a.grad_dtype, a.dk, a.dk_first + token * a.dk_stride + head_col, a.dim);
-    store_gradient<DP>(dv, 1.0f, a.grad_dtype, a.dv, a.dv_first + token * a.dv_stride + head_col, a.dim);
-  }
+  store(dk, z.scale, z.dk, z.dk_first, z.dk_stride, 0);
+  store(dv, 1.0f, z.dv, z.dv_first, z.dv_stride, 1);
 }
 
-// The rows that a block of attention_bwd_keys left out, added to what it stored (so of bf16 gradients rounded once more): row by
-// row, each lane taking what its key is seen by.  (A launch of its own, whose blocks mostly find nothing: as a part of
-// that kernel it took the registers of its loop.)
 template <int DP>
-__global__ __launch_bounds__(256) void attention_bwd_left_out(GradArgs a) {
-  const int place = static_cast<int>(blockIdx.x);
-  const int* const flags = a.left_out + 8 * place;
+__global__ __launch_bounds__(512, 2) void attention_bwd_keys(GradArgs a) {
+  __shared__ __attribute__((aligned(1024))) char smem[KeysShape<DP, 128>::BYTES];
+  keys_block<DP, 128>(a, static_cast<int>(blockIdx.x), smem);
+}
+
+// What the keys' blocks leave.  Their splits' sums, if they have more than one, in order; then the rows that they left out, added
+// row by row to what is stored (so bf16 gradients are rounded once more), each lane taking what its key is seen by, 32 columns of
+// the gradients at a time.  (A launch of its own, whose blocks mostly find no such rows: as a part of the keys' kernel it took
+// the registers of its loop.)
+constexpr int kSumBlocks = 16;
+__global__ __launch_bounds__(256) void attention_bwd_finish(GradArgs a) {
+  const int sums = a.key_splits > 1 ? kSumBlocks : 1;  // blocks that share a tile's sums
+  const int place = static_cast<int>(blockIdx.x) / sums, sum_block = static_cast<int>(blockIdx.x) % sums;
+  const int kv = place % a.kv_heads, slot = place / a.kv_heads;
+  const int64_t split_step = 8 * a.kv_heads;  // from a split's flags to the next one's
+  const int* const flags = a.left_out + slot * a.key_splits * split_step + 8 * kv;
   int any = 0;
+  for (int s = 0; s < a.key_splits; ++s)
 #pragma unroll
-  for (int w = 0; w < 8; ++w) any |= flags[w];
-  if (any == 0) return;
-  const int kv = place % a.kv_heads;
-  const RowTile tile = a.key_log == 7 ? row_tile<7>(a.seqs, 1, place / a.kv_heads) : row_tile<6>(a.seqs, 1, place / a.kv_heads);
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    for (int w = 0; w < 8; ++w) any |= flags[s * split_step + w];
+  // one block that has them all where rows were left out, which come after the sums
+  if (any == 0 ? a.key_splits == 1 : sum_block > 0) return;
+  const int lanes = any == 0 ? 256 * sums : 256;
+  const RowTile tile = a.key_log == 7 ? row_tile<7>(a.seqs, 1, slot) : row_tile<6>(a.seqs, 1, slot);
+  if (!tile.any || tile.seq < 0) return;
+  const int64_t head_col = static_cast<int64_t>(kv) * a.dim;
+  if (a.key_splits > 1) {
+    const int per = a.dim / 4, units = min(1 << a.key_log, tile.len - tile.row) * per;
+    const int64_t other = a.kv_heads * a.seqs.n * a.dim;
+    for (int u = 256 * sum_block + threadIdx.x; u < 2 * units; u += lanes) {
+      const bool is_v = u >= units;
+      const int x = is_v ? u - units : u;
+      const int64_t token = tile.token + tile.row + x / per;
+      const int col = 4 * (x % per);
+      const float* from = a.parts + (kv * a.seqs.n + token) * a.dim + col + (is_v ? other : 0);
+      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+      for (int s = 0; s < a.key_splits; ++s, from += 2 * other) {
+        const f32x4 v = *reinterpret_cast<const f32x4*>(from);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum[j] += v[j];
+      }
+      if (is_v) store_unit<4>(a.grad_dtype, a.dv, a.dv_first + token * a.dv_stride + head_col + col, sum);
+      else store_unit<4>(a.grad_dtype, a.dk, a.dk_first + token * a.dk_stride + head_col + col, sum);
+    }
+    if (any == 0) return;
+    __syncthreads();
+  }
+  const int lane = threadIdx.x & 63, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int groups = 1 << (a.key_log - 5), parts = 8 / groups;
   if (wave >= groups) return;
   const int key0 = tile.row + 32 * wave, key = key0 + (lane & 31);
-  const int64_t head_col = static_cast<int64_t>(kv) * a.dim, token = tile.token + min(key, tile.len - 1);
-  bf16x8 kf[DP / 16], vf[DP / 16];
-  load_operand<DP>(a.k + token * a.k_stride + head_col, a.dim, kf);
-  load_operand<DP>(a.v + token * a.v_stride + head_col, a.dim, vf);
-  f32x16 dk[DP / 32], dv[DP / 32];
-#pragma unroll
-  for (int d = 0; d < DP / 32; ++d) dk[d] = dv[d] = MfmaBf16::zero();
+  const int64_t token = tile.token + min(key, tile.len - 1);
+  const uint16_t* const kp = a.k + token * a.k_stride + head_col;
+  const uint16_t* const vp = a.v + token * a.v_stride + head_col;
   const uint16_t* const qp = a.q + tile.token * a.q_stride + head_col * a.group;
   const uint16_t* const dp = a.dout + tile.token * a.dout_stride + head_col * a.group;
   const float* const sp = a.rows + (static_cast<int64_t>(kv) * a.seqs.n + tile.token) * a.group;
   const float scale2 = a.scale * kLog2e;
   int end = 0;
-  for (int p = 0; p < parts; ++p) end = max(end, flags[wave + groups * p]);
+  for (int s = 0; s < a.key_splits; ++s)
+    for (int p = 0; p < parts; ++p) end = max(end, flags[s * split_step + wave + groups * p]);
   end = min(end, tile.len * a.group);
+  const int tile_rows = 32 * parts;
+  const RowShare share(a, tile, tile_rows);
 #pragma unroll 1
-  for (int r = key0 * a.group; r < end; ++r) {
-    if (r >= flags[wave + groups * ((r >> 5) & (parts - 1))]) continue;
-    const int i = a.token_of(r);
-    const int64_t col = static_cast<int64_t>(r - i * a.group) * a.dim;
-    const uint16_t* const qr = qp + i * a.q_stride + col;
-    const uint16_t* const dr = dp + i * a.dout_stride + col;
-    const float sr = halves_sum(half_dot<DP>(kf, qr, a.dim)), pr = halves_sum(half_dot<DP>(vf, dr, a.dim));
-    if (r < key * a.group) continue;
-    const float w = __builtin_amdgcn_exp2f((sr + sp[r]) * scale2);
-    add_row<DP>(dv, w, dr, a.dim);
-    add_row<DP>(dk, w * (pr + sp[a.seqs.n * a.heads + r]), qr, a.dim);
-  }
-  if (key >= tile.len) return;
-  const auto add = [&](const f32x16 (&acc)[DP / 32], float by, void* to, int64_t e) {
-#pragma unroll
-    for (int d = 0; d < DP / 32; ++d)
+  for (int c0 = 0; c0 < a.dim; c0 += 32) {
+    f32x16 dk[1] = {MfmaBf16::zero()}, dv[1] = {MfmaBf16::zero()};
+#pragma unroll 1
+    for (int r = key0 * a.group; r < end; ++r) {
+      if (r >= flags[(r / tile_rows - share.first) / share.tiles * split_step + wave + groups * ((r >> 5) & (parts - 1))]) continue;
+      const int i = a.token_of(r);
+      const int64_t head = static_cast<int64_t>(r - i * a.group) * a.dim;
+      const uint16_t* const qr = qp + i * a.q_stride + head;
+      const uint16_t* const dr = dp + i * a.dout_stride + head;
+      float sr = 0.0f, pr = 0.0f;
+#pragma unroll 1
+      for (int col = 8 * half; col < a.dim; col += 16) {
+        sr = dot8(*reinterpret_cast<const u32x4*>(kp + col), *reinterpret_cast<const u32x4*>(qr + col), sr);
+        pr = dot8(*reinterpret_cast<const u32x4*>(vp + col), *reinterpret_cast<const u32x4*>(dr + col), pr);
+      }
+      sr = halves_sum(sr);
+      pr = halves_sum(pr);
+      if (r < key * a.group) continue;
+      const float w = __builtin_amdgcn_exp2f((sr + sp[r]) * scale2);
+      add_row<32>(dv, w, dr + c0, a.dim - c0);
+      add_row<32>(dk, w * (pr + sp[a.seqs.n * a.heads + r]), qr + c0, a.dim - c0);
+    }
+    if (key >= tile.len) continue;
+    const auto add = [&](const f32x16& acc, float by, void* to, int64_t e) {
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const int c = 32 * d + 8 * g + 4 * (lane >> 5);
+        const int c = c0 + 8 * g + 4 * half;
         if (c >= a.dim) continue;
         float v[4];
         load_some(a.grad_dtype, to, e + c, 4, v);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] += acc[d][4 * g + j] * by;
+        for (int j = 0; j < 4; ++j) v[j] += acc[4 * g + j] * by;
         store_some(a.grad_dtype, to, e + c, 4, v);
       }
-  };
-  add(dk, a.scale, a.dk, a.dk_first + token * a.dk_stride + head_col);
-  add(dv, 1.0f, a.dv, a.dv_first + token * a.dv_stride + head_col);
+    };
+    add(dk[0], a.scale, a.dk, a.dk_first + token * a.dk_stride + head_col);
+    add(dv[0], 1.0f, a.dv, a.dv_first + token * a.dv_stride + head_col);
+  }
 }
 
-// dq: four waves of 32 rows each, walking over tiles of 64 keys.
+// dq: a block has 128 rows and walks over tiles of 64 keys.  32 rows have NW / 4 waves, of which each takes its share of a
+// tile's keys; they add up their sums at the end.
 template <int DP>
-__global__ __launch_bounds__(256, 2) void attention_bwd_queries(GradArgs a) {
-  constexpr int KT = 64, ROWS = 128;
+constexpr int kQueriesTiles = 2 * 2 * 64 * TileShape<DP>::PITCH;
+template <int DP, int NW>
+constexpr int kQueriesBytes = kQueriesTiles<DP> > NW * kSumBytes<DP> ? kQueriesTiles<DP> : NW * kSumBytes<DP>;
+template <int DP, int NW>
+__device__ __forceinline__ void queries_block(const GradArgs& a, int b, char* smem) {
+  constexpr int KT = 64, ROWS = 128, CK = KT / NW, PARTS = NW / 4;
   using T = TileShape<DP>;
-  using Copies = RowCopies<DP, 16>;  // of a tile's keys by each wave
+  using Copies = RowCopies<DP, CK>;  // of a tile's keys by each wave
   constexpr int SLOT = 2 * KT * T::PITCH;
-  __shared__ __attribute__((aligned(1024))) char smem[2 * SLOT];
-  int b = static_cast<int>(blockIdx.x);
   const int kv = b % a.kv_heads;
   const RowTile tile = row_tile<7>(a.seqs, a.group, a.blocks - 1 - b / a.kv_heads);
   if (!tile.any) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int rows = tile.len * a.group, row0 = tile.row + 32 * wave;
+  const int part = wave >> 2;  // of a tile's keys
+  const int rows = tile.len * a.group, row0 = tile.row + 32 * (wave & 3);
   const int64_t head_col = static_cast<int64_t>(kv) * a.dim;
-  const auto dq_at = [&](int row) {
-    const int i = a.token_of(row);
-    return a.dq_first + (tile.token + i) * a.dq_stride + head_col * a.group + static_cast<int64_t>(row - i * a.group) * a.dim;
+  const auto dq_at = [&tile](const GradArgs& z, int64_t first, int row) {
+    const int i = z.token_of(row);
+    return first + (tile.token + i) * z.dq_stride + static_cast<int64_t>(row - i * z.group) * z.dim;
   };
   if (tile.seq < 0) {
-    for (int row = tile.row + static_cast<int>(threadIdx.x); row < min(tile.row + ROWS, rows); row += 256)
-      store_zeros(a.grad_dtype, a.dq, dq_at(row), a.dim);
+    for (int row = tile.row + static_cast<int>(threadIdx.x); row < min(tile.row + ROWS, rows); row += 64 * NW)
+      store_zeros(a.grad_dtype, a.dq, dq_at(a, a.dq_first + head_col * a.group, row), a.dim);
     return;
   }
   if (2 * a.dim < T::PITCH) {
-    for (int i = threadIdx.x; i < 2 * SLOT / 16; i += 256) reinterpret_cast<u32x4*>(smem)[i] = u32x4{0u, 0u, 0u, 0u};
+    for (int i = threadIdx.x; i < 2 * SLOT / 16; i += 64 * NW) reinterpret_cast<u32x4*>(smem)[i] = u32x4{0u, 0u, 0u, 0u};
     __syncthreads();
   }
   const auto sees = [&](int row) { return a.causal ? a.token_of(row) + 1 : tile.len; };
@@ -367,11 +443,11 @@ __global__ __launch_bounds__(256, 2) void attention_bwd_queries(GradArgs a) {
   const char* const kp = reinterpret_cast<const char*>(a.k + tile.token * a.k_stride + head_col);
   const char* const vp = reinterpret_cast<const char*>(a.v + tile.token * a.v_stride + head_col);
   Copies copies;
-  copies.offsets(0, a.dim, [&](int r) { return 2u * static_cast<uint32_t>(r) * static_cast<uint32_t>(a.k_stride); },
+  copies.offsets(CK * wave, a.dim, [&](int r) { return 2u * static_cast<uint32_t>(r) * static_cast<uint32_t>(a.k_stride); },
                  [&](int r) { return 2u * static_cast<uint32_t>(r) * static_cast<uint32_t>(a.v_stride); });
   const auto fetch = [&](int t, int slot) {
-    const int j = t * KT + 16 * wave;
-    char* const area = smem + slot * SLOT + 16 * wave * T::PITCH;
+    const int j = t * KT + CK * wave;
+    char* const area = smem + slot * SLOT + CK * wave * T::PITCH;
     copies.copy(kp + 2 * (j * a.k_stride), vp + 2 * (j * a.v_stride), tile.len - 1 - j, area, area + KT * T::PITCH);
   };
   fetch(0, 0);
@@ -426,16 +502,16 @@ __global__ __launch_bounds__(256, 2) void attention_bwd_queries(GradArgs a) {
     const char* const ks = smem + slot * SLOT;
     slot ^= 1;
 #pragma unroll 1
-    for (int u = 0; u < KT / 32; ++u) add(ks + 32 * u * T::PITCH, form(ks + 32 * u * T::PITCH, nullptr));
+    for (int u = part; u < KT / 32; u += PARTS) add(ks + 32 * u * T::PITCH, form(ks + 32 * u * T::PITCH, nullptr));
   }
   // the others
 #pragma unroll 1
   for (; t < end; ++t) {
     enter();
-    const char* ks = smem + slot * SLOT;
+    const char* ks = smem + slot * SLOT + part * 32 * T::PITCH;
     slot ^= 1;
 #pragma unroll 1
-    for (int u = 0; u < KT / 32; ++u, ks += 32 * T::PITCH) {
+    for (int u = part; u < KT / 32; u += PARTS, ks += PARTS * 32 * T::PITCH) {
       const int j0 = t * KT + 32 * u, hi = seen - j0 - 4 * (lane >> 5);
       if (j0 >= most) break;
       bool odd;
@@ -449,13 +525,33 @@ __global__ __launch_bounds__(256, 2) void attention_bwd_queries(GradArgs a) {
   }
 #pragma unroll 1
   for (int j = left_out; j < most; ++j) {
+    if (PARTS == 2 && ((j >> 5) & 1) != part) continue;
     const uint16_t* const kr = reinterpret_cast<const uint16_t*>(kp) + j * a.k_stride;
     const uint16_t* const vr = reinterpret_cast<const uint16_t*>(vp) + j * a.v_stride;
     const float s = halves_sum(half_dot<DP>(qf, kr, a.dim)), p = halves_sum(half_dot<DP>(df, vr, a.dim));
     if (j >= seen) continue;
     add_row<DP>(dq, __builtin_amdgcn_exp2f((s + score0) * scale2) * (p + dp0), kr, a.dim);
   }
-  if (row0 + (lane & 31) < rows) store_gradient<DP>(dq, a.scale, a.grad_dtype, a.dq, dq_at(row), a.dim);
+  const GradArgs& z = late_args();
+  const int64_t first = z.dq_first + static_cast<int64_t>((static_cast<int>(blockIdx.x) - (PARTS == 2 ? z.key_blocks : 0)) % z.kv_heads) * z.group * z.dim;
+  store_sums<DP, 4, PARTS>(dq, z.scale, z.dim, z.grad_dtype, z.dq, smem,
+                           [&](int r) { return tile.row + r < rows ? dq_at(z, first, tile.row + r) : -1; });
+}
+template <int DP>
+__global__ __launch_bounds__(256, 2) void attention_bwd_queries(GradArgs a) {
+  __shared__ __attribute__((aligned(1024))) char smem[kQueriesBytes<DP, 4>];
+  queries_block<DP, 4>(a, static_cast<int>(blockIdx.x), smem);
+}
+
+// Both in one launch, side by side, where the card holds all their blocks at once.
+template <int DP>
+__global__ __launch_bounds__(512, 2) void attention_bwd_both(GradArgs a) {
+  constexpr int BYTES = KeysShape<DP, 64>::BYTES;
+  static_assert(BYTES >= kQueriesBytes<DP, 8>, "one area for either");
+  __shared__ __attribute__((aligned(1024))) char smem[BYTES];
+  const int b = static_cast<int>(blockIdx.x);
+  if (b < a.key_blocks) keys_block<DP, 64>(a, b, smem);
+  else queries_block<DP, 8>(a, b - a.key_blocks, smem);
 }
 
 // 128 keys a block, or 64 in twice the blocks, each half as long, where 128 would leave CUs idle (full attention) or wait for the
@@ -463,6 +559,21 @@ __global__ __launch_bounds__(256, 2) void attention_bwd_queries(GradArgs a) {
 // 128 keys and 124 by 64, 2048: 309 and 238, 4096: 684 and 571, 8192: 1820 and 2040; full, 4096: 893 and 1042.
 int key_tile_log(int64_t n, int64_t kv_heads, bool causal) {
   return ((n + 127) >> 7) * kv_heads <= (causal ? 256 : 128) ? 6 : 7;
+}
+// Splits of the rows that see a block's 64 keys, where those blocks are few: so many that the longest block (a tile of 128 rows takes it
+// about 2 us, and its start and end as long as five) times the rounds of the card's 256 CUs is least.  us with 1 split, as many as
+// make 256 blocks, and these: 1000 rows, 8 heads of 128 over 2 74, 52, 38; 2048 136, 74, 74; 1024 over 8 each 34, 55, 34; 8192, 8
+// over 1 986, 554, 554; 32 over 8: 512 47, 44, 44, 1024 78, 66, 66.
+int key_splits(int64_t n, int64_t seqs, int64_t heads, int64_t kv_heads) {
+  const int64_t with_rows = std::max<int64_t>(1, std::min(seqs, n)), tiles = n * (heads / kv_heads) / 128 / with_rows;
+  const int64_t most = std::min({256 / std::max<int64_t>(1, ((n + 63) >> 6) * kv_heads), tiles, int64_t{8}});
+  int64_t best = 1, least = INT64_MAX;
+  for (int64_t s = 1; s <= most; ++s) {
+    const int64_t blocks = (row_slots(n, seqs, 1, 6) * s + row_slots(n, seqs, heads / kv_heads, 7)) * kv_heads;
+    const int64_t takes = (blocks + 255) / 256 * (5 * s + tiles) * 840 / s;  // 840: a multiple of 1 .. 8
+    if (takes < least) best = s, least = takes;
+  }
+  return static_cast<int>(best);
 }
 
 bool float_type(int32_t t) { return t == VDSL_F32 || t == VDSL_BF16; }
@@ -479,15 +590,17 @@ bool apart(const vdsl_heads& x, int64_t x_width, const vdsl_heads& y, int64_t y_
 
 using namespace vdsl;
 
-// What the rows' scores and dp start from, what attention_bwd_keys left out, a copy of dout in bf16.
+// What the rows' scores and dp start from, what the keys' blocks left out, a copy of dout in bf16, splits' sums.
 extern "C" int vdsl_attention_bwd_workspace_bytes(int64_t n, int64_t seqs, int32_t heads, int32_t kv_heads, int32_t dim, size_t* bytes) {
   if (!bytes) return fail(VDSL_ERR_INVALID_ARG, "bytes is null");
   VDSL_TRY(attention_check_shape("attention_bwd", n, seqs, heads, kv_heads, dim));
   // a multiple of 16 bytes before the copy
-  const size_t flags = nbytes(row_slots(n, seqs, 1, 6), kv_heads, 32), rows = nbytes(n, heads, 8 + 2 * static_cast<int64_t>(dim));
-  if (flags == kSizeOverflow || rows == kSizeOverflow || rows + flags + 16 < rows)
+  const int splits = key_splits(n, seqs, heads, kv_heads);
+  const size_t flags = nbytes(row_slots(n, seqs, 1, 6), kv_heads, 32 * splits), rows = nbytes(n, heads, 8 + 2 * static_cast<int64_t>(dim));
+  const size_t parts = splits == 1 ? 0 : nbytes(n, static_cast<int64_t>(kv_heads) * dim, 8 * splits);
+  if (flags == kSizeOverflow || rows == kSizeOverflow || parts == kSizeOverflow || rows + flags + 32 < rows || rows + flags + 32 + parts < parts)
     return fail(VDSL_ERR_SHAPE, "attention_bwd workspace size overflows");
-  *bytes = rows + flags + 16;
+  *bytes = rows + flags + parts + 32;
   return VDSL_OK;
 }
 
@@ -531,9 +644,10 @@ extern "C" int vdsl_op_attention_bwd(vdsl_queue q, const vdsl_attention_params* 
   const int group = p->heads / p->kv_heads;
   float* const rows = static_cast<float*>(workspace->ptr);
   const int key_log = key_tile_log(p->n, p->kv_heads, p->causal != 0);
+  const int splits = key_log == 6 ? key_splits(p->n, p->seqs, p->heads, p->kv_heads) : 1;
   const int64_t key_slots = row_slots(p->n, p->seqs, 1, key_log), query_slots = row_slots(p->n, p->seqs, group, 7);
-  if (std::max(key_slots, query_slots) * p->kv_heads > 0x3fffff) return fail(VDSL_ERR_UNSUPPORTED, "attention_bwd: too many rows");
-  const int64_t flags_at = 2 * p->n * p->heads, copy_at = (flags_at + 8 * key_slots * p->kv_heads + 3) & ~int64_t{3};
+  if (std::max(key_slots * splits, query_slots) * p->kv_heads > 0x3fffff) return fail(VDSL_ERR_UNSUPPORTED, "attention_bwd: too many rows");
+  const int64_t flags_at = 2 * p->n * p->heads, copy_at = (flags_at + 8 * key_slots * splits * p->kv_heads + 3) & ~int64_t{3};
   uint16_t* const copy = dout_dtype == VDSL_F32 ? reinterpret_cast<uint16_t*>(rows + copy_at) : nullptr;
   GradArgs a = {};
   a.q = static_cast<const uint16_t*>(qs->ptr) + p->q.first;
@@ -547,6 +661,8 @@ extern "C" int vdsl_op_attention_bwd(vdsl_queue q, const vdsl_attention_params* 
   a.seqs = {static_cast<const int32_t*>(starts->ptr), p->n, p->seqs};
   a.rows = rows;
   a.key_log = key_log;
+  a.key_splits = splits;
+  a.parts = rows + ((copy_at + (copy ? p->n * width / 2 : 0) + 3) & ~int64_t{3});
   a.left_out = reinterpret_cast<int*>(rows + flags_at);
   a.dq = dq->ptr;
   a.dk = dk->ptr;
@@ -568,16 +684,23 @@ extern "C" int vdsl_op_attention_bwd(vdsl_queue q, const vdsl_attention_params* 
   hipLaunchKernelGGL(attention_bwd_rows, block_grid((p->n * p->heads + 15) / 16), dim3(256), 0, q->stream, dout->ptr, dout_dtype,
                      out->ptr, out_dtype, static_cast<const float*>(lse->ptr), p->n, p->heads, group, p->dim, p->scale, copy, rows);
   VDSL_TRY(check_launch("attention_bwd_rows"));
-  const auto go = [&](auto kernel, unsigned lanes, int64_t slots, const char* name) {
-    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(slots * p->kv_heads)), dim3(lanes), 0, q->stream, a);
+  const auto go = [&](auto kernel, unsigned lanes, int64_t blocks, const char* name) {
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(lanes), 0, q->stream, a);
     return check_launch(name);
   };
+  const int64_t tiles = key_slots * p->kv_heads, key_blocks = tiles * splits, query_blocks = query_slots * p->kv_heads;
+  const auto pick = [&](auto of64, auto of96, auto of128) { return p->dim <= 64 ? of64 : p->dim <= 96 ? of96 : of128; };
+  const auto finish = [&]() -> int {
+    if (!p->causal && splits == 1) return VDSL_OK;
+    return go(attention_bwd_finish, 256, splits > 1 ? kSumBlocks * tiles : tiles, "attention_bwd_finish");
+  };
   a.blocks = static_cast<int>(query_slots);
-  const auto keys = a.key_log == 7 ? (p->dim <= 64 ? attention_bwd_keys<64, 128> : p->dim <= 96 ? attention_bwd_keys<96, 128> : attention_bwd_keys<128, 128>)
-                                   : (p->dim <= 64 ? attention_bwd_keys<64, 64> : p->dim <= 96 ? attention_bwd_keys<96, 64> : attention_bwd_keys<128, 64>);
-  const auto queries = p->dim <= 64 ? attention_bwd_queries<64> : p->dim <= 96 ? attention_bwd_queries<96> : attention_bwd_queries<128>;
-  const auto rest = p->dim <= 64 ? attention_bwd_left_out<64> : p->dim <= 96 ? attention_bwd_left_out<96> : attention_bwd_left_out<128>;
-  VDSL_TRY(go(keys, 512, key_slots, "attention_bwd_keys"));
-  if (p->causal) VDSL_TRY(go(rest, 256, key_slots, "attention_bwd_left_out"));
-  return go(queries, 256, query_slots, "attention_bwd_queries");
+  a.key_blocks = static_cast<int>(key_blocks);
+  if (key_log == 6) {
+    VDSL_TRY(go(pick(attention_bwd_both<64>, attention_bwd_both<96>, attention_bwd_both<128>), 512, key_blocks + query_blocks, "attention_bwd_both"));
+    return finish();
+  }
+  VDSL_TRY(go(pick(attention_bwd_keys<64>, attention_bwd_keys<96>, attention_bwd_keys<128>), 512, key_blocks, "attention_bwd_keys"));
+  VDSL_TRY(finish());
+  return go(pick(attention_bwd_queries<64>, attention_bwd_queries<96>, attention_bwd_queries<128>), 256, query_blocks, "attention_bwd_queries");
 }

@@ -283,6 +283,46 @@ __device__ __forceinline__ void add_row(f32x16 (&acc)[DP / 32], float w, const u
     }
 }
 
+// The sums of a block's waves by way of LDS, so that whole rows are stored and by code of a few lines (an unrolled store of what a lane
+// has reads as many instructions as the main loop, which short calls wait for).  Of its 32 x DP sums (column 32 d + 8 g +
+// 4 (l / 32) + j of row l % 32) a wave leaves 4 columns in a place of 528 bytes.  Then 32 * GROUPS rows of `by` times the sums of
+// PARTS waves, w, w + GROUPS, ..: at(row) is the element of its column 0, less than 0 for none.
+template <int DP>
+constexpr int kSumBytes = DP / 4 * 528;
+template <int DP, int GROUPS, int PARTS, class At>
+__device__ __forceinline__ void store_sums(const f32x16 (&acc)[DP / 32], float by, int dim, int dtype, void* to, char* smem, At&& at) {
+  const int thread = late_thread(), lane = thread & 63, wave = thread >> 6;
+  __syncthreads();
+  char* const mine = smem + wave * kSumBytes<DP> + (lane >> 5) * 528 + (lane & 31) * 16;
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      *reinterpret_cast<f32x4*>(mine + (4 * d + g) * 1056) = f32x4{acc[d][4 * g], acc[d][4 * g + 1], acc[d][4 * g + 2], acc[d][4 * g + 3]};
+  __syncthreads();
+#pragma unroll 1
+  for (int u = thread; u < 32 * GROUPS * (DP / 8); u += 64 * GROUPS * PARTS) {
+    const int row = u / (DP / 8), c = u % (DP / 8);
+    const int64_t e = at(row);
+    if (8 * c >= dim || e < 0) continue;
+    const char* const from = smem + (row >> 5) * kSumBytes<DP> + c * 1056 + (row & 31) * 16;
+    float v[8] = {};
+#pragma unroll
+    for (int o = 0; o < PARTS; ++o) {
+      const f32x4 x = *reinterpret_cast<const f32x4*>(from + o * GROUPS * kSumBytes<DP>);
+      const f32x4 y = *reinterpret_cast<const f32x4*>(from + o * GROUPS * kSumBytes<DP> + 528);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        v[j] += x[j];
+        v[4 + j] += y[j];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] *= by;
+    store_unit<8>(dtype, to, e + 8 * c, v);
+  }
+}
+
 // Copies 4 bytes a lane straight to LDS, lane l's to l + 4 l.
 __device__ __forceinline__ void lds_copy4(const char* g, char* l) { __builtin_amdgcn_global_load_lds(g, (lds_void_t*)l, 4, 0, 0); }
 

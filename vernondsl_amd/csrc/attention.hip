@@ -26,6 +26,7 @@ struct AttentionArgs {
   int64_t pages;
   int table_cols, page_shift;
   int splits, blocks;
+  Divider token_of;
 };
 
 constexpr float kLag = 8.0f;  // by how much m may lag, in powers of two
@@ -241,16 +242,22 @@ struct Place {
   }
 };
 
-// Four waves of 32 rows each, sharing tiles of 64 keys through two slots of LDS; two blocks to a CU, so that a SIMD has
-// one wave's exponentials beside another's products.
-template <int DP, bool PAGED>
-__global__ __launch_bounds__(256, 2) void attention_rows(AttentionArgs a) {
-  constexpr int KT = 64, KS = KT / 32, NS = 2, ROWS = 128;
+// Waves of 32 rows each, sharing tiles of keys through two slots of LDS.  PARTS 1: four waves and tiles of 64 keys, two blocks to a
+// CU, so that a SIMD has one wave's exponentials beside another's products.  PARTS 4: two times 32 rows with four waves each, which
+// take 32 keys each of a tile of 128 and join what they have at the end.
+// What bounds it: the matrix units are busy 54% of the cycles and the vector units 50%, the two waves of a SIMD only partly beside
+// each other; the reads of LDS (32 KB for 32 products, by each wave) take as long as the products.  64 rows a wave would
+// halve those, but leave a SIMD one wave: 3020 us where this took 2300.  16384 rows, 32 heads of 128 over 8, causal: 2070 us, 1063
+// TFLOP/s (the library's product of 8192^3: 1360).
+template <int DP, bool PAGED, int PARTS>
+__global__ __launch_bounds__(PARTS == 1 ? 256 : 512, 2) void attention_rows(AttentionArgs a) {
+  static_assert(PARTS == 1 || !PAGED, "a paged cache's keys are split among blocks");
+  constexpr int NW = PARTS == 1 ? 4 : 8, GROUPS = NW / PARTS, ROWS = 32 * GROUPS, KT = 16 * NW, KW = KT / PARTS, KS = KW / 32, NS = 2;
   using T = TileShape<DP>;
-  constexpr int SLOT = 2 * KT * T::PITCH;
-  __shared__ __attribute__((aligned(1024))) char smem[NS * SLOT];
+  constexpr int SLOT = 2 * KT * T::PITCH, SUMS = PARTS == 1 ? 0 : NW * kSumBytes<DP>, AREA = NS * SLOT > SUMS ? NS * SLOT : SUMS;
+  __shared__ __attribute__((aligned(1024))) char smem[AREA];
   const Place place(a);
-  const RowTile tile = row_tile<7>(a.seqs, a.group, place.slot);
+  const RowTile tile = row_tile<GROUPS == 4 ? 7 : 6>(a.seqs, a.group, place.slot);
   if (!tile.any) return;
   const RowsAt at = rows_at<PAGED>(a, tile);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -266,7 +273,7 @@ __global__ __launch_bounds__(256, 2) void attention_rows(AttentionArgs a) {
   }
   const KeySource<DP, PAGED> src(a, tile, at.keys, place.kv);
   if (2 * a.dim < T::PITCH) {  // columns past dim are never copied
-    for (int i = threadIdx.x; i < NS * SLOT / 16; i += 256) reinterpret_cast<u32x4*>(smem)[i] = u32x4{0u, 0u, 0u, 0u};
+    for (int i = threadIdx.x; i < NS * SLOT / 16; i += 64 * NW) reinterpret_cast<u32x4*>(smem)[i] = u32x4{0u, 0u, 0u, 0u};
     __syncthreads();
   }
   // Paged: which keys of the tile and of the next one hold something, and the pages of that one.
@@ -297,7 +304,7 @@ __global__ __launch_bounds__(256, 2) void attention_rows(AttentionArgs a) {
   if constexpr (PAGED) look(first);
   fetch(first, 0);
 
-  const int row0 = tile.row + wave * 32;
+  const int part = wave / GROUPS, row0 = tile.row + wave % GROUPS * 32;  // the wave's keys of a tile, its rows
   const bool mine = row0 < at.rows;
   const float scale2 = a.scale * kLog2e;
   const int row = min(row0 + (lane & 31), at.rows - 1), sees = at.sees(row, a.group, a.causal);
@@ -320,7 +327,7 @@ __global__ __launch_bounds__(256, 2) void attention_rows(AttentionArgs a) {
 #pragma unroll 1
   for (const int whole = min(end, fewest / KT); t < whole; ++t) {
     enter();
-    const char* const keys = smem + slot * SLOT;
+    const char* const keys = smem + slot * SLOT + part * KW * T::PITCH;
     const char* const values = keys + KT * T::PITCH;
     slot ^= 1;
     f32x16 s[KS];
@@ -331,7 +338,7 @@ __global__ __launch_bounds__(256, 2) void attention_rows(AttentionArgs a) {
 #pragma unroll
       for (int k = 0; k < KS; ++k) s[k] = MfmaBf16::mma(rows_fragment<DP>(keys, 32 * k, kk), qf[kk], s[k]);
     reads_ahead<6, KS * DP / 16, 1>();
-    if (PAGED && valid != ~0ull) hide(s, KT, valid);
+    if (PAGED && valid != ~0ull) hide(s, KW, valid);
     st.weigh(s, scale2);
 #pragma unroll
     for (int e = 0; e < 2 * KS; ++e) {
@@ -345,12 +352,12 @@ __global__ __launch_bounds__(256, 2) void attention_rows(AttentionArgs a) {
 #pragma unroll 1
   for (; t < end; ++t) {
     enter();
-    const char* const keys = smem + slot * SLOT;
+    const char* const keys = smem + slot * SLOT + part * KW * T::PITCH;
     const char* const values = keys + KT * T::PITCH;
     slot ^= 1;
 #pragma unroll 1
     for (int k = 0; k < KS; ++k) {
-      const int j0 = t * KT + 32 * k;
+      const int j0 = t * KT + part * KW + 32 * k;
       if (j0 >= most) break;
       f32x16 s[1] = {MfmaBf16::zero()};
 #pragma unroll
@@ -372,13 +379,43 @@ __global__ __launch_bounds__(256, 2) void attention_rows(AttentionArgs a) {
 #pragma unroll 1
   for (int j = left_out; j < min(most, end * KT); ++j) {
     const int e = src.page(j);
-    if (e < 0) continue;
+    if (e < 0 || (PARTS > 1 && j % KT / KW != part)) continue;
     const float s = halves_sum(half_dot<DP>(qf, reinterpret_cast<const uint16_t*>(src.row(src.k, src.k_row, j, e)), a.dim));
     if (j >= sees) continue;
     const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s, scale2, -(st.m == neg_inf() ? 0.0f : st.m)));
     add_row<DP>(st.o, w, reinterpret_cast<const uint16_t*>(src.row(src.v, src.v_row, j, e)), a.dim);
   }
-  if (mine) store_rows<DP>(a, st, at, row0, place.kv, place.split);
+  if constexpr (PARTS == 1) {
+    if (mine) store_rows<DP>(a, st, at, row0, place.kv, place.split);
+  } else {
+    // the parts joined as attention_join does it
+    float2* const stats = reinterpret_cast<float2*>(smem);  // [waves][32]
+    const float l = halves_sum(st.l);
+    __syncthreads();
+    if (lane < 32) stats[32 * wave + lane] = make_float2(st.m, l);
+    __syncthreads();
+    float m = neg_inf(), sum = 0.0f;
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p) m = fmaxf(m, stats[32 * (wave % GROUPS + p * GROUPS) + (lane & 31)].x);
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p) {
+      const float2 of = stats[32 * (wave % GROUPS + p * GROUPS) + (lane & 31)];
+      sum += (of.x == neg_inf() ? 0.0f : __builtin_amdgcn_exp2f(of.x - m)) * of.y;
+    }
+    const float by = sum == 0.0f || st.m == neg_inf() ? sum : __builtin_amdgcn_exp2f(st.m - m) / sum;
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) st.o[d][i] *= by;
+    const int row = row0 + (lane & 31);
+    if (a.lse && part == 0 && lane < 32 && row < at.rows)
+      a.lse[(place.kv * a.group + row % a.group) * a.seqs.n + at.token + row / a.group] = sum == 0.0f ? neg_inf() : (m + __builtin_amdgcn_logf(sum)) * kLn2;
+    store_sums<DP, GROUPS, PARTS>(st.o, 1.0f, a.dim, a.out_dtype, a.out, smem, [&](int r) {
+      const int x = tile.row + r;
+      const int i = a.token_of(x);
+      return x < at.rows ? ((at.token + i) * a.heads + place.kv * a.group + x - i * a.group) * a.dim : -1;
+    });
+  }
 }
 
 // Few rows: a block is one wave with 32 rows and a split of the keys, in tiles of 32 through two slots of LDS of its own, so
@@ -559,10 +596,10 @@ int launch_rows(vdsl_queue q, AttentionArgs& a, Kernel kernel, unsigned lanes, i
   hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(lanes), 0, q->stream, a);
   return check_launch(name);
 }
-template <bool PAGED>
+template <bool PAGED, int PARTS>
 int launch_rows(vdsl_queue q, AttentionArgs& a) {
-  return launch_rows(q, a, a.dim <= 64 ? attention_rows<64, PAGED> : a.dim <= 96 ? attention_rows<96, PAGED> : attention_rows<128, PAGED>, 256, 7,
-                     "attention_rows");
+  return launch_rows(q, a, a.dim <= 64 ? attention_rows<64, PAGED, PARTS> : a.dim <= 96 ? attention_rows<96, PAGED, PARTS> : attention_rows<128, PAGED, PARTS>,
+                     PARTS == 1 ? 256 : 512, PARTS == 4 ? 6 : 7, "attention_rows");
 }
 
 }  // namespace
@@ -637,7 +674,12 @@ extern "C" int vdsl_op_attention_fwd(vdsl_queue q, const vdsl_attention_params* 
   a.causal = p->causal != 0;
   a.scale = p->scale;
   a.splits = 1;
-  return launch_rows<false>(q, a);
+  a.token_of = divider(a.group);
+  // Blocks of 128 rows that are few, walking over many keys one after the other, become blocks of 64 with four parts of the keys.
+  // us, heads of 128: 1024 rows of 8 over 8 heads (64 blocks) 26 and 17, 2048 of 8 over 2 (128) 42 and 26, 1024 of 32 over 8 (256)
+  // 25.8 and 25.6, 2048 of these (512) 52 and 67; 90 rows of 8 over 2 (6) 8.3 and 8.4.
+  if (((p->n * a.group + 127) >> 7) * p->kv_heads <= 192) return launch_rows<false, 4>(q, a);
+  return launch_rows<false, 1>(q, a);
 }
 
 namespace vdsl {
@@ -771,7 +813,7 @@ extern "C" int vdsl_op_paged_attention(vdsl_queue q, const vdsl_paged_params* p,
   if (plan.few)
     VDSL_TRY(launch_rows(q, a, a.dim <= 64 ? attention_few<64> : a.dim <= 96 ? attention_few<96> : attention_few<128>, 64, 5, "attention_few"));
   else
-    VDSL_TRY(launch_rows<true>(q, a));
+    VDSL_TRY((launch_rows<true, 1>(q, a)));
   if (a.splits == 1) return VDSL_OK;
   const int shares = a.splits <= 8 ? 1 : a.splits <= 64 ? 4 : 8;
   const auto join = shares == 1 ? attention_join<1> : shares == 4 ? attention_join<4> : attention_join<8>;

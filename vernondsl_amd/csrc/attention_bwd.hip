@@ -78,40 +78,6 @@ __global__ __launch_bounds__(256) void attention_bwd_rows(const void* __restrict
   to[n * heads] = -sum;
 }
 
-// The sums of a block's waves by way of LDS, so that whole rows are stored and by code of a few lines (an unrolled store of what a lane
-// has reads as many instructions as the main loop, which short calls wait for).  Of its 32 x DP sums (column 32 d + 8 g +
-// 4 (l / 32) + j of row l % 32) a wave leaves 4 columns in a place of 528 bytes.  Then 32 * GROUPS rows of `by` times the sums of
-// PARTS waves, w, w + GROUPS, ..: at(row) is the element of its column 0, less than 0 for none.
-template <int DP>
-constexpr int kSumBytes = DP / 4 * 528;
-template <int DP, int GROUPS, int PARTS, class At>
-__device__ __forceinline__ void store_sums(const f32x16 (&acc)[DP / 32], float by, int dim, int dtype, void* to, char* smem, At&& at) {
-  const int thread = late_thread(), lane = thread & 63, wave = thread >> 6;
-  __syncthreads();
-  char* const mine = smem + wave * kSumBytes<DP> + (lane >> 5) * 528 + (lane & 31) * 16;
-#pragma unroll
-  for (int d = 0; d < DP / 32; ++d)
-#pragma unroll
-    for (int g = 0; g < 4; ++g)
-      *reinterpret_cast<f32x4*>(mine + (4 * d + g) * 1056) = f32x4{acc[d][4 * g], acc[d][4 * g + 1], acc[d][4 * g + 2], acc[d][4 * g + 3]};
-  __syncthreads();
-#pragma unroll 1
-  for (int u = thread; u < 32 * GROUPS * (DP / 4); u += 64 * GROUPS * PARTS) {
-    const int row = u / (DP / 4), c = u % (DP / 4);
-    const int64_t e = at(row);
-    if (4 * c >= dim || e < 0) continue;
-    const char* const from = smem + (row >> 5) * kSumBytes<DP> + c * 528 + (row & 31) * 16;
-    f32x4 v = *reinterpret_cast<const f32x4*>(from);
-#pragma unroll
-    for (int o = 1; o < PARTS; ++o) {
-      const f32x4 x = *reinterpret_cast<const f32x4*>(from + o * GROUPS * kSumBytes<DP>);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] += x[j];
-    }
-    const float w[4] = {v[0] * by, v[1] * by, v[2] * by, v[3] * by};
-    store_unit<4>(dtype, to, e + 4 * c, w);
-  }
-}
 __device__ __forceinline__ void store_zeros(int dtype, void* to, int64_t e, int cols) {
   const float none[4] = {0.0f, 0.0f, 0.0f, 0.0f};
   for (int c = 0; c < cols; c += 4) store_unit<4>(dtype, to, e + c, none);

@@ -67,7 +67,9 @@ PACKED = [([1], 0, 0, 1, 1, 8, True), ([2, 0, 1], 1, 2, 2, 1, 16, True), ([33], 
           # as above, with so many kv heads that the gradient's blocks have 128 keys
           ([1100], 0, 0, 32, 32, 8, True), ([1000, 50], 0, 3, 40, 40, 128, True), ([500, 0, 600], 2, 0, 64, 32, 64, True), ([700], 0, 0, 32, 32, 96, False),
           # few kv heads that many share, whose rows the gradient splits
-          ([700], 0, 5, 64, 1, 128, True), ([40, 900, 3], 1, 0, 12, 2, 72, False)]
+          ([700], 0, 5, 64, 1, 128, True), ([40, 900, 3], 1, 0, 12, 2, 72, False),
+          # more sequences than a wave's lanes hold, at both sides of it
+          ([3, 0] * 62 + [17], 2, 3, 4, 2, 16, True), ([3, 0] * 63, 0, 3, 4, 2, 16, True), ([2] * 300, 1, 0, 2, 1, 8, False)]
 
 
 @pytest.mark.parametrize("lengths,front,back,heads,kv,dim,causal", PACKED)

@@ -51,6 +51,26 @@ struct Sequences {
   }
 };
 
+// The last piece i with below(i, its first token), which holds for 0, and its first token and the next one's.  Up to 125 sequences
+// take one trip to memory: their borders stay with the lanes, two each.
+struct Piece {
+  int64_t i, token, next;
+};
+template <class Below>
+__device__ __forceinline__ Piece find_piece(const Sequences& s, Below&& below) {
+  if (s.seqs <= 125) {
+    const int lane = threadIdx.x & 63, count = static_cast<int>(s.seqs) + 2;
+    const int first = static_cast<int>(s.border(lane)), second = static_cast<int>(s.border(lane + 64));
+    const uint64_t of_first = __ballot(lane < count && below(int64_t{lane}, int64_t{first}));
+    const uint64_t of_second = __ballot(lane + 64 < count && below(int64_t{lane} + 64, int64_t{second}));
+    const int i = __popcll(of_first) + __popcll(of_second) - 1;
+    const auto at = [&](int x) { return x < 64 ? __builtin_amdgcn_readlane(first, x) : __builtin_amdgcn_readlane(second, x - 64); };
+    return {i, at(i), at(i + 1)};
+  }
+  const int64_t i = wave_search(s.seqs + 2, [&](int64_t p) { return below(p, s.border(p)); });
+  return {i, s.border(i), s.border(i + 1)};
+}
+
 struct RowTile {
   int64_t seq;    // -1: rows of no sequence
   int64_t token;  // the piece's first token
@@ -60,13 +80,13 @@ struct RowTile {
 };
 template <int LOG_TILE>
 __device__ __forceinline__ RowTile row_tile(const Sequences& s, int group, int64_t slot) {
-  const int64_t i = wave_search(s.seqs + 2, [&](int64_t p) { return ((s.border(p) * group) >> LOG_TILE) + p <= slot; });
+  const Piece piece = find_piece(s, [&](int64_t p, int64_t border) { return ((border * group) >> LOG_TILE) + p <= slot; });
   RowTile t;
-  t.token = s.border(i);
-  const int64_t len = s.border(i + 1) - t.token;
+  t.token = piece.token;
+  const int64_t len = piece.next - t.token;
   t.len = len > 0 ? static_cast<int>(len) : 0;
-  t.seq = i >= 1 && i <= s.seqs ? i - 1 : -1;
-  const int64_t row = (slot - ((t.token * group) >> LOG_TILE) - i) << LOG_TILE;
+  t.seq = piece.i >= 1 && piece.i <= s.seqs ? piece.i - 1 : -1;
+  const int64_t row = (slot - ((t.token * group) >> LOG_TILE) - piece.i) << LOG_TILE;
   t.any = row >= 0 && row < static_cast<int64_t>(t.len) * group;
   t.row = t.any ? static_cast<int>(row) : 0;
   return t;

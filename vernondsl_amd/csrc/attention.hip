@@ -568,9 +568,10 @@ __global__ __launch_bounds__(256) void attention_join(AttentionArgs a) {
 __global__ __launch_bounds__(256) void cache_append_rows(AttentionArgs a, uint16_t* __restrict__ k_cache, uint16_t* __restrict__ v_cache) {
   const int64_t row = block_index();
   if (row >= a.seqs.n) return;
-  const int64_t i = wave_search(a.seqs.seqs + 2, [&](int64_t p) { return a.seqs.border(p) <= row; });
+  const Piece piece = find_piece(a.seqs, [&](int64_t, int64_t border) { return border <= row; });
+  const int64_t i = piece.i;
   if (i < 1 || i > a.seqs.seqs) return;
-  const int64_t pos = a.lengths[i - 1] - (a.seqs.border(i + 1) - row);
+  const int64_t pos = a.lengths[i - 1] - (piece.next - row);
   if (pos < 0 || pos >= (static_cast<int64_t>(a.table_cols) << a.page_shift)) return;
   const int64_t page = a.table[(i - 1) * a.table_cols + (pos >> a.page_shift)];
   if (page < 0 || page >= a.pages) return;

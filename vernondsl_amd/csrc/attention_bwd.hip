@@ -137,16 +137,6 @@ __device__ __forceinline__ void keys_block(const GradArgs& a, int b, char* smem)
     for (int i = threadIdx.x; i < NS * SLOT / 16; i += 512) reinterpret_cast<u32x4*>(smem)[i] = u32x4{0u, 0u, 0u, 0u};
     __syncthreads();
   }
-  const int64_t token = tile.token + min(key, tile.len - 1);
-  bf16x8 kf[DP / 16], vf[DP / 16];
-  load_operand<DP>(a.k + token * a.k_stride + head_col, a.dim, kf);
-  load_operand<DP>(a.v + token * a.v_stride + head_col, a.dim, vf);
-  char* const values = smem + NS * SLOT + wave % GROUPS * 32 * T::PITCH;  // all parts write the same
-  if constexpr (V_LDS) {
-#pragma unroll
-    for (int kk = 0; kk < DP / 16; ++kk)
-      *reinterpret_cast<bf16x8*>(values + (lane & 31) * T::PITCH + (((2 * kk + half) ^ T::swz(lane & 31)) << 4)) = vf[kk];
-  }
   const int rows = tile.len * a.group;
   const RowShare share(a, tile, TR);
   const int first = share.first + split * share.tiles, end = min(first + share.tiles, share.end);
@@ -187,6 +177,16 @@ __device__ __forceinline__ void keys_block(const GradArgs& a, int b, char* smem)
   // All blocks begin with the last rows, which they all see, and so read the same rows at about the same time.
   if (end > first) fetch(end - 1, 0);
   if (NS == 3 && end - 2 >= first) fetch(end - 2, 1);
+  const int64_t token = tile.token + min(key, tile.len - 1);
+  bf16x8 kf[DP / 16], vf[DP / 16];
+  load_operand<DP>(a.k + token * a.k_stride + head_col, a.dim, kf);
+  load_operand<DP>(a.v + token * a.v_stride + head_col, a.dim, vf);
+  char* const values = smem + NS * SLOT + wave % GROUPS * 32 * T::PITCH;  // all parts write the same
+  if constexpr (V_LDS) {
+#pragma unroll
+    for (int kk = 0; kk < DP / 16; ++kk)
+      *reinterpret_cast<bf16x8*>(values + (lane & 31) * T::PITCH + (((2 * kk + half) ^ T::swz(lane & 31)) << 4)) = vf[kk];
+  }
   int slot = 0;
   if (wave < 4) __builtin_amdgcn_s_setprio(1);
 #pragma unroll 1

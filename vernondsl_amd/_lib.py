@@ -195,14 +195,14 @@ PROTOTYPES = {
     "vdsl_op_linear_xent_fwd": (C.c_int, [_vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "vdsl_op_linear_xent_fwd_bwd": (C.c_int, [_vp, _i64, _i64, _i64, _vp, _vp, _vp, _i64, C.c_float, _vp, _vp, _vp, _i32, _vp,
                                               _i32, _vp, _vp]),
-    "vdsl_op_rope": (C.c_int, [_vp, C.POINTER(RopeParams), _i32, _vp, _vp, _vp, _i32, _vp]),
-    "vdsl_op_attention_fwd": (C.c_int, [_vp, C.POINTER(AttentionParams), _vp, _vp, _vp, _vp, _i32, _vp, _vp]),
+    "vdsl_op_rope": (C.c_int, [_vp, _vp, _i32, _vp, _vp, _vp, _i32, _vp]),
+    "vdsl_op_attention_fwd": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i32, _vp, _vp]),
     "vdsl_attention_bwd_workspace_bytes": (C.c_int, [_i64, _i64, _i32, _i32, _i32, C.POINTER(_sz)]),
-    "vdsl_op_attention_bwd": (C.c_int, [_vp, C.POINTER(AttentionParams), _i32, _vp, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _i32, _vp,
+    "vdsl_op_attention_bwd": (C.c_int, [_vp, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _i32, _vp,
                                         _vp, _vp, _vp]),
-    "vdsl_op_cache_append": (C.c_int, [_vp, C.POINTER(PagedParams), _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "vdsl_op_cache_append": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "vdsl_paged_attention_workspace_bytes": (C.c_int, [_i64, _i64, _i32, _i32, _i32, _i64, C.POINTER(_sz)]),
-    "vdsl_op_paged_attention": (C.c_int, [_vp, C.POINTER(PagedParams), _vp, _vp, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _vp]),
+    "vdsl_op_paged_attention": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _vp]),
     "vdsl_debug_fail_alloc_after": (C.c_int, [_i64]),
     "vdsl_debug_gemm_config": (C.c_int, [_i32]),
     "vdsl_debug_linear_xent_plan": (C.c_int, [_i64, _i64, _i64, _i64, C.POINTER(_i64)]),

@@ -1,10 +1,13 @@
 // The gradient of attention over packed sequences.  With p = exp2(c s - lse log2 e) formed again from q, k and lse,
 // dp = dout v, delta = dout out and ds = p (dp - delta):
 //   dq = scale ds k (rows' own sum over keys),   dk = scale ds^T q and dv = p^T dout (keys' own sums over rows and heads)
-// The launches: delta of each row; dk and dv, a wave holding 32 keys and walking over the rows that see them; dq, a
-// wave holding its rows and walking over the keys they see.  Each sum belongs to one wave and is taken in one order, so
-// nothing is added atomically and the bits are the same on every call; the price is that s and dp are formed twice (7
-// products where 5 would do).  See attention.h for rows, tiles and the order of the products' sums.
+// The launches: delta of each row; dk and dv, waves holding 32 keys and walking over the rows that see them; what those leave
+// (attention_bwd_finish); dq, waves holding their rows and walking over the keys they see.  Where the keys' blocks are
+// few, keys and rows have one launch.  Every sum is taken in one order, so nothing is added atomically and the bits are
+// the same on every call; the price is that s and dp are formed twice (7 products where 5 would do).  See attention.h for rows,
+// tiles and the order of the products' sums.
+// 8192 rows of two sequences, 32 heads of 128 over 8, causal, 707 GFLOP by five products: 1050 us, of which rows 30, keys 632 (four
+// products, 640 TFLOP/s), what they leave 5, queries 410 (three, 740 TFLOP/s).
 #include <algorithm>
 
 #include "attention.h"
@@ -45,7 +48,8 @@ __device__ __forceinline__ const GradArgs& late_args() {
   return *(const GradArgs*)p;
 }
 
-// What a row's scores and dp start from, -lse / scale and -delta, and dout in bf16 where it is f32.  16 lanes a row of one head.
+// What a row's scores and dp start from, -lse / scale and -delta, and dout in bf16 where it is f32.  16 lanes a row of one head, 16
+// bytes each (8 bytes: 44 us where this takes 30, at 4.5 TB/s).
 __global__ __launch_bounds__(256) void attention_bwd_rows(const void* __restrict__ dout, int dout_dtype, const void* __restrict__ out,
                                                           int out_dtype, const float* __restrict__ lse, int64_t n, int heads, int group,
                                                           int dim, float scale, uint16_t* __restrict__ copy, float* __restrict__ rows) {
@@ -77,22 +81,24 @@ __global__ __launch_bounds__(256) void attention_bwd_rows(const void* __restrict
   *to = l == neg_inf() ? neg_inf() : -l / scale;  // no score of such a row has a weight
   to[n * heads] = -sum;
 }
-
 __device__ __forceinline__ void store_zeros(int dtype, void* to, int64_t e, int cols) {
   const float none[4] = {0.0f, 0.0f, 0.0f, 0.0f};
   for (int c = 0; c < cols; c += 4) store_unit<4>(dtype, to, e + c, none);
 }
 
-// dk and dv: a block has KEYS keys and walks over tiles of rows through a ring of two or three slots of LDS.  Each 32 keys
-// have 8 / (KEYS / 32) waves, one for each 32 rows of a tile, which add up their sums at the end.  Two waves share a SIMD,
-// and one has priority there, so that its exponentials come beside the other's products.  To leave both their
-// registers, wide heads' values are an operand read from LDS (V_LDS).
 // The tiles of TR rows that see a block's keys, and how many of them a split has.
 struct RowShare {
   int first, end, tiles;
   __device__ __forceinline__ RowShare(const GradArgs& a, const RowTile& t, int TR)
       : first(a.causal ? t.row * a.group / TR : 0), end((t.len * a.group + TR - 1) / TR), tiles((end - first + a.key_splits - 1) / a.key_splits) {}
 };
+// dk and dv: a block has KEYS keys and walks over tiles of rows through a ring of two or three slots of LDS.  Each 32 keys
+// have 8 / (KEYS / 32) waves, one for each 32 rows of a tile, which add up their sums at the end.  Two waves share a SIMD,
+// and one has priority there, so that its exponentials come beside the other's products.  To leave both their
+// registers, wide heads' values are an operand read from LDS (V_LDS).
+// Bounded by both: the products at the clock that they leave, and the reads of LDS that feed them (a wave's 32 products take 40 KB, so a
+// CU's eight 2560 cycles of LDS for 2048 of the matrix units).  Rows from the last to the first: all blocks begin with rows that
+// they all see, and so read the same ones at about the same time (1287 us for the whole gradient before, 1165 with it).
 template <int DP, int KEYS>
 struct KeysShape {
   static constexpr int NW = 8, GROUPS = KEYS / 32, PARTS = NW / GROUPS, TR = 32 * PARTS;
@@ -273,8 +279,8 @@ __global__ __launch_bounds__(512, 2) void attention_bwd_keys(GradArgs a) {
 
 // What the keys' blocks leave.  Their splits' sums, if they have more than one, in order; then the rows that they left out, added
 // row by row to what is stored (so bf16 gradients are rounded once more), each lane taking what its key is seen by, 32 columns of
-// the gradients at a time.  (A launch of its own, whose blocks mostly find no such rows: as a part of the keys' kernel it took
-// the registers of its loop.)
+// the gradients at a time.  (A launch of its own, 3 to 5 us, whose blocks mostly find no such rows: as a part of the keys' kernel it took
+// the registers of its loop.)  kSumBlocks: one to four units a lane; fewer wait for one load after the other.
 constexpr int kSumBlocks = 16;
 __global__ __launch_bounds__(256) void attention_bwd_finish(GradArgs a) {
   const int sums = a.key_splits > 1 ? kSumBlocks : 1;  // blocks that share a tile's sums
@@ -373,7 +379,7 @@ __global__ __launch_bounds__(256) void attention_bwd_finish(GradArgs a) {
 }
 
 // dq: a block has 128 rows and walks over tiles of 64 keys.  32 rows have NW / 4 waves, of which each takes its share of a
-// tile's keys; they add up their sums at the end.
+// tile's keys; they add up their sums at the end.  Bounded as the forward pass is.
 template <int DP>
 constexpr int kQueriesTiles = 2 * 2 * 64 * TileShape<DP>::PITCH;
 template <int DP, int NW>
@@ -509,7 +515,8 @@ __global__ __launch_bounds__(256, 2) void attention_bwd_queries(GradArgs a) {
   queries_block<DP, 4>(a, static_cast<int>(blockIdx.x), smem);
 }
 
-// Both in one launch, side by side, where the card holds all their blocks at once.
+// Both in one launch, side by side: the keys' blocks first, which are the longer ones.  293 rows of 6 heads of 80 over 2: 27 us in two
+// launches, 18 in one.
 template <int DP>
 __global__ __launch_bounds__(512, 2) void attention_bwd_both(GradArgs a) {
   constexpr int BYTES = KeysShape<DP, 64>::BYTES;
@@ -521,8 +528,9 @@ __global__ __launch_bounds__(512, 2) void attention_bwd_both(GradArgs a) {
 }
 
 // 128 keys a block, or 64 in twice the blocks, each half as long, where 128 would leave CUs idle (full attention) or wait for the
-// blocks of the first keys, which the most rows see (causal).  32 heads of 128 over 8: causal, one sequence of 1024 rows 164 us by
-// 128 keys and 124 by 64, 2048: 309 and 238, 4096: 684 and 571, 8192: 1820 and 2040; full, 4096: 893 and 1042.
+// blocks of the first keys, which the most rows see (causal).  Whole gradients, 32 heads of 128 over 8: causal, one sequence of 1024
+// rows 164 us by 128 keys and 66 by 64 with the queries in the same launch, 2048: 309 and 158, 4096: 684 and 534, 8192: 1820
+// and (a launch each) 2040; full, 4096: 893 and 1042.
 int key_tile_log(int64_t n, int64_t kv_heads, bool causal) {
   return ((n + 127) >> 7) * kv_heads <= (causal ? 256 : 128) ? 6 : 7;
 }

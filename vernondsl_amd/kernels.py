@@ -6,6 +6,7 @@ ABI checks buffer sizes again), then enqueues the op on `q` and returns without 
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from typing import NamedTuple
 
 import numpy as np
@@ -528,20 +529,33 @@ class Heads(NamedTuple):
     first: int = 0
 
 
-def _heads(x, name) -> Heads:
+def _columns(x, name):
+    """Heads, or a tensor [rows][heads][dim], as (tensor, heads, dim, first, elements of a row)."""
     if isinstance(x, Heads):
-        if len(x.tensor.shape) != 2:
-            raise ValueError(f"{name}: Heads are columns of a tensor [rows][width], got shape {x.tensor.shape}")
-        if x.first < 0 or x.heads < 0 or x.dim < 0 or x.first + x.heads * x.dim > x.tensor.shape[1]:
-            raise ValueError(f"{name}: columns {x.first} to {x.first + x.heads * x.dim} of a tensor of width {x.tensor.shape[1]}")
-        return x
+        t, heads, dim, first = x
+        if len(t.shape) != 2:
+            raise ValueError(f"{name}: Heads are columns of a tensor [rows][width], got shape {t.shape}")
+        width = t.shape[1]
+        if first < 0 or heads < 0 or dim < 0 or first + heads * dim > width:
+            raise ValueError(f"{name}: columns {first} to {first + heads * dim} of a tensor of width {width}")
+        return t, heads, dim, first, width
     if len(x.shape) != 3:
         raise ValueError(f"{name}: shape {x.shape}, expected [rows][heads][dim] or Heads of [rows][width]")
-    return Heads(x, x.shape[1], x.shape[2])
+    _, heads, dim = x.shape
+    return x, heads, dim, 0, heads * dim
 
 
-def _layout(x: Heads) -> _lib.Heads:
-    return _lib.Heads(x.first, x.tensor.numel // x.tensor.shape[0] if x.tensor.shape[0] else x.heads * x.dim)
+# The params of the calls below as the bytes of their C structs (ctypes structs take as long to fill as a launch takes).
+_ROPE_PARAMS = struct.Struct("=qqqiiiiif")
+_ATTENTION_PARAMS = struct.Struct("=qqiiiifi12q")
+_PAGED_PARAMS = struct.Struct("=qqqqiiiifi6q")
+
+
+def _pack(params: struct.Struct, *values) -> bytes:
+    try:
+        return params.pack(*values)
+    except (struct.error, OverflowError) as e:
+        raise ValueError(f"{values}: {e}") from None
 
 
 def rope_frequencies(rot: int, base: float = 10000.0, factor: float = 1.0, trained: int = 0, kind: str = "ramp") -> np.ndarray:
@@ -588,25 +602,29 @@ def rope(q: Queue, x: Tensor, positions: Tensor, freqs: Tensor, y: Tensor, heads
         raise ValueError(f"y: shape {y.shape}, expected {(rows, width)}")
     _expect(positions, (rows,), "i32", "positions")
     _expect(freqs, (2, freqs.shape[-1]), "f32", "freqs")
-    p = _lib.RopeParams(rows, width, first, heads, dim, freqs.shape[1], int(bool(interleaved)), int(bool(inverse)), magnitude)
-    call("vdsl_op_rope", q.handle, C.byref(p), x.dtype, x.handle, positions.handle, freqs.handle, y.dtype, y.handle)
+    p = _pack(_ROPE_PARAMS, rows, width, first, heads, dim, freqs.shape[1], bool(interleaved), bool(inverse), magnitude)
+    call("vdsl_op_rope", q.handle, p, x.dtype, x.handle, positions.handle, freqs.handle, y.dtype, y.handle)
 
 
 def _attention_operands(qh, k, v, starts, out, lse, scale):
-    qh, k, v = _heads(qh, "q"), _heads(k, "k"), _heads(v, "v")
-    n, dim = qh.tensor.shape[0], qh.dim
-    for x, name in ((qh, "q"), (k, "k"), (v, "v")):
-        if x.tensor.dtype != _lib.BF16:
-            raise ValueError(f"{name}: dtype {x.tensor.dtype}, expected bf16")
-        if x.tensor.shape[0] != n or x.dim != dim or (x is not qh and x.heads != k.heads):
-            raise ValueError(f"{name}: {x.tensor.shape[0]} rows of {x.heads} heads of {x.dim} beside q's {n} rows of {dim}")
-    _expect(starts, (starts.numel,), "i32", "starts")
-    if starts.numel < 1:
-        raise ValueError("starts: needs the number of sequences + 1 elements")
-    if out.numel != n * qh.heads * dim or out.shape[0] != n:
-        raise ValueError(f"out: shape {out.shape}, expected {(n, qh.heads * dim)}")
-    _expect(lse, (qh.heads, n), "f32", "lse")
-    return qh, k, v, float(dim) ** -0.5 if scale is None and dim else scale
+    """q, k and v as _columns gives them, checked against each other, and the scale."""
+    qt, heads, dim, _, _ = qc = _columns(qh, "q")
+    kt, kv_heads, _, _, _ = kc = _columns(k, "k")
+    vc = _columns(v, "v")
+    n = qt.shape[0]
+    for name, (t, of, columns, _, _), expected in (("q", qc, heads), ("k", kc, kv_heads), ("v", vc, kv_heads)):
+        if t.dtype != _lib.BF16:
+            raise ValueError(f"{name}: dtype {t.dtype}, expected bf16")
+        if t.shape[0] != n or columns != dim or of != expected:
+            raise ValueError(f"{name}: {t.shape[0]} rows of {of} heads of {columns}, expected {n} rows of {expected} heads of {dim}")
+    if len(starts.shape) != 1 or starts.numel < 1:
+        raise ValueError(f"starts: shape {starts.shape}, expected one more element than there are sequences")
+    if starts.dtype != _lib.I32:
+        raise ValueError(f"starts: dtype {starts.dtype}, expected i32")
+    if out.numel != n * heads * dim or out.shape[0] != n:
+        raise ValueError(f"out: shape {out.shape}, expected {(n, heads * dim)}")
+    _expect(lse, (heads, n), "f32", "lse")
+    return qc, kc, vc, float(dim) ** -0.5 if scale is None and dim else scale
 
 
 def attention_fwd(q: Queue, qh, k, v, starts: Tensor, out: Tensor, lse=None, causal: bool = True, scale=None):
@@ -614,11 +632,11 @@ def attention_fwd(q: Queue, qh, k, v, starts: Tensor, out: Tensor, lse=None, cau
     [seqs + 1]) see each other, earlier ones only if causal.  q, k, v: bf16 Heads, or tensors [n][heads][dim]; kv heads divide
     the heads.  scale: 1 / sqrt(dim) if None.  lse (f32 [heads][n], optional): log of the scores' exponentials' sum, kept for
     attention_bwd.  Rows of no sequence get 0, lse -inf."""
-    qh, k, v, scale = _attention_operands(qh, k, v, starts, out, lse, scale)
-    p = _lib.AttentionParams(qh.tensor.shape[0], starts.numel - 1, qh.heads, k.heads, qh.dim, int(bool(causal)), scale, 0,
-                             _layout(qh), _layout(k), _layout(v))
-    call("vdsl_op_attention_fwd", q.handle, C.byref(p), qh.tensor.handle, k.tensor.handle, v.tensor.handle, starts.handle, out.dtype,
-         out.handle, _h(lse))
+    qc, kc, vc, scale = _attention_operands(qh, k, v, starts, out, lse, scale)
+    qt, kt, vt = qc[0], kc[0], vc[0]
+    p = _pack(_ATTENTION_PARAMS, qt.shape[0], starts.numel - 1, qc[1], kc[1], qc[2], bool(causal), scale, 0, *qc[3:], *kc[3:], *vc[3:],
+              0, 0, 0, 0, 0, 0)
+    call("vdsl_op_attention_fwd", q.handle, p, qt.handle, kt.handle, vt.handle, starts.handle, out.dtype, out.handle, _h(lse))
 
 
 def attention_bwd_workspace_bytes(n, seqs, heads, kv_heads, dim) -> int:
@@ -632,35 +650,39 @@ def attention_bwd(q: Queue, dout: Tensor, qh, k, v, starts: Tensor, out: Tensor,
     """The gradients dq, dk, dv (Heads or tensors [n][heads][dim], all f32 or all bf16; disjoint columns of one tensor if they
     like) of attention_fwd from dout [n][heads * dim] (f32 or bf16) and the forward pass's out and lse.  workspace:
     attention_bwd_workspace_bytes(n, seqs, heads, kv_heads, dim) bytes."""
-    qh, k, v, scale = _attention_operands(qh, k, v, starts, out, lse, scale)
-    n = qh.tensor.shape[0]
+    qc, kc, vc, scale = _attention_operands(qh, k, v, starts, out, lse, scale)
+    qt, kt, vt = qc[0], kc[0], vc[0]
+    n = qt.shape[0]
     if dout.numel != out.numel or dout.shape[0] != n:
         raise ValueError(f"dout: shape {dout.shape}, expected {out.shape}")
-    grads = [_heads(g, name) for g, name in ((dq, "dq"), (dk, "dk"), (dv, "dv"))]
-    for g, x, name in zip(grads, (qh, k, v), ("dq", "dk", "dv")):
-        if (g.tensor.shape[0], g.heads, g.dim) != (n, x.heads, x.dim):
-            raise ValueError(f"{name}: {g.tensor.shape[0]} rows of {g.heads} heads of {g.dim}, expected {n} rows of {x.heads} heads of {x.dim}")
-        if g.tensor.dtype != grads[0].tensor.dtype:
+    dqc, dkc, dvc = _columns(dq, "dq"), _columns(dk, "dk"), _columns(dv, "dv")
+    dtype = dqc[0].dtype
+    for name, (t, of, columns, _, _), x in (("dq", dqc, qc), ("dk", dkc, kc), ("dv", dvc, vc)):
+        if t.shape[0] != n or of != x[1] or columns != x[2]:
+            raise ValueError(f"{name}: {t.shape[0]} rows of {of} heads of {columns}, expected {n} rows of {x[1]} heads of {x[2]}")
+        if t.dtype != dtype:
             raise ValueError("dq, dk and dv must be of one dtype")
-    p = _lib.AttentionParams(n, starts.numel - 1, qh.heads, k.heads, qh.dim, int(bool(causal)), scale, 0, _layout(qh), _layout(k), _layout(v),
-                             *(_layout(g) for g in grads))
-    call("vdsl_op_attention_bwd", q.handle, C.byref(p), dout.dtype, dout.handle, qh.tensor.handle, k.tensor.handle, v.tensor.handle,
-         starts.handle, out.dtype, out.handle, _h(lse), grads[0].tensor.dtype, *(g.tensor.handle for g in grads), _h(workspace))
+    p = _pack(_ATTENTION_PARAMS, n, starts.numel - 1, qc[1], kc[1], qc[2], bool(causal), scale, 0, *qc[3:], *kc[3:], *vc[3:],
+              *dqc[3:], *dkc[3:], *dvc[3:])
+    call("vdsl_op_attention_bwd", q.handle, p, dout.dtype, dout.handle, qt.handle, kt.handle, vt.handle, starts.handle, out.dtype,
+         out.handle, _h(lse), dtype, dqc[0].handle, dkc[0].handle, dvc[0].handle, _h(workspace))
 
 
-def _paged_params(n, dim, kv_heads, heads, scale, starts, lengths, table, k_cache, v_cache):
-    """starts, lengths and table against the caches [pages][kv_heads][page][dim]; the params without layouts."""
-    if len(k_cache.shape) != 4 or k_cache.shape[1] != kv_heads or k_cache.shape[3] != dim:
-        raise ValueError(f"k_cache: shape {k_cache.shape}, expected [pages][{kv_heads}][page][{dim}]")
-    _expect(k_cache, k_cache.shape, "bf16", "k_cache")
-    _expect(v_cache, k_cache.shape, "bf16", "v_cache")
+def _paged_params(n, dim, kv_heads, heads, scale, starts, lengths, table, k_cache, v_cache, *layouts):
+    """starts, lengths and table against the caches [pages][kv_heads][page][dim]; the params, with first and stride of q, k and v."""
+    shape = k_cache.shape
+    if len(shape) != 4 or shape[1] != kv_heads or shape[3] != dim:
+        raise ValueError(f"k_cache: shape {shape}, expected [pages][{kv_heads}][page][{dim}]")
+    if k_cache.dtype != _lib.BF16:
+        raise ValueError(f"k_cache: dtype {k_cache.dtype}, expected bf16")
+    _expect(v_cache, shape, "bf16", "v_cache")
     (seqs,) = lengths.shape
     _expect(starts, (seqs + 1,), "i32", "starts")
     _expect(lengths, (seqs,), "i32", "lengths")
     if len(table.shape) != 2:
         raise ValueError(f"table: shape {table.shape}, expected [seqs][pages of a sequence]")
     _expect(table, (seqs, table.shape[1]), "i32", "table")
-    return _lib.PagedParams(n, seqs, k_cache.shape[0], table.shape[1], k_cache.shape[2], heads, kv_heads, dim, scale, 0)
+    return _pack(_PAGED_PARAMS, n, seqs, shape[0], table.shape[1], shape[2], heads, kv_heads, dim, scale, 0, *layouts)
 
 
 def cache_append(q: Queue, k, v, starts: Tensor, lengths: Tensor, table: Tensor, k_cache: Tensor, v_cache: Tensor):
@@ -668,17 +690,16 @@ def cache_append(q: Queue, k, v, starts: Tensor, lengths: Tensor, table: Tensor,
     [pages][kv_heads][page][dim], page a power of two from 16 on): row i of the m new rows starts[s] to starts[s + 1] of sequence s is
     position p = lengths[s] - m + i, slot p % page of page table[s][p / page] (i32; lengths counts the new rows).  Rows without
     a page are dropped."""
-    k, v = _heads(k, "k"), _heads(v, "v")
-    n = k.tensor.shape[0]
-    for x, name in ((k, "k"), (v, "v")):
-        if x.tensor.dtype != _lib.BF16:
-            raise ValueError(f"{name}: dtype {x.tensor.dtype}, expected bf16")
-    if (v.tensor.shape[0], v.heads, v.dim) != (n, k.heads, k.dim):
-        raise ValueError(f"v: {v.tensor.shape[0]} rows of {v.heads} heads of {v.dim}, expected {n} rows of {k.heads} heads of {k.dim}")
-    p = _paged_params(n, k.dim, k.heads, k.heads, 1.0, starts, lengths, table, k_cache, v_cache)
-    p.k, p.v = _layout(k), _layout(v)
-    call("vdsl_op_cache_append", q.handle, C.byref(p), k.tensor.handle, v.tensor.handle, starts.handle, lengths.handle, table.handle,
-         k_cache.handle, v_cache.handle)
+    kt, heads, dim, k_first, k_stride = _columns(k, "k")
+    vt, v_heads, v_dim, v_first, v_stride = _columns(v, "v")
+    n = kt.shape[0]
+    for t, name in ((kt, "k"), (vt, "v")):
+        if t.dtype != _lib.BF16:
+            raise ValueError(f"{name}: dtype {t.dtype}, expected bf16")
+    if vt.shape[0] != n or v_heads != heads or v_dim != dim:
+        raise ValueError(f"v: {vt.shape[0]} rows of {v_heads} heads of {v_dim}, expected {n} rows of {heads} heads of {dim}")
+    p = _paged_params(n, dim, heads, heads, 1.0, starts, lengths, table, k_cache, v_cache, 0, 0, k_first, k_stride, v_first, v_stride)
+    call("vdsl_op_cache_append", q.handle, p, kt.handle, vt.handle, starts.handle, lengths.handle, table.handle, k_cache.handle, v_cache.handle)
 
 
 def paged_attention_workspace_bytes(n, seqs, heads, kv_heads, dim, positions) -> int:
@@ -693,16 +714,15 @@ def paged_attention(q: Queue, qh, k_cache: Tensor, v_cache: Tensor, starts: Tens
     """Attention of new rows over a paged cache that holds their own keys already (cache_append): the row at position p sees
     positions 0 to p of its sequence.  qh: bf16 Heads or a tensor [n][heads][dim]; out [n][heads * dim], lse and scale as
     for attention_fwd.  workspace: paged_attention_workspace_bytes(...) bytes, None where that is 0."""
-    qh = _heads(qh, "q")
-    n, dim = qh.tensor.shape[0], qh.dim
-    if qh.tensor.dtype != _lib.BF16:
-        raise ValueError(f"q: dtype {qh.tensor.dtype}, expected bf16")
-    if out.numel != n * qh.heads * dim or out.shape[0] != n:
-        raise ValueError(f"out: shape {out.shape}, expected {(n, qh.heads * dim)}")
-    _expect(lse, (qh.heads, n), "f32", "lse")
+    qt, heads, dim, first, stride = _columns(qh, "q")
+    n = qt.shape[0]
+    if qt.dtype != _lib.BF16:
+        raise ValueError(f"q: dtype {qt.dtype}, expected bf16")
+    if out.numel != n * heads * dim or out.shape[0] != n:
+        raise ValueError(f"out: shape {out.shape}, expected {(n, heads * dim)}")
+    _expect(lse, (heads, n), "f32", "lse")
     kv_heads = k_cache.shape[1] if len(k_cache.shape) == 4 else 0
-    p = _paged_params(n, dim, kv_heads, qh.heads, float(dim) ** -0.5 if scale is None and dim else scale, starts, lengths, table, k_cache,
-                      v_cache)
-    p.q = _layout(qh)
-    call("vdsl_op_paged_attention", q.handle, C.byref(p), qh.tensor.handle, k_cache.handle, v_cache.handle, starts.handle, lengths.handle,
+    p = _paged_params(n, dim, kv_heads, heads, float(dim) ** -0.5 if scale is None and dim else scale, starts, lengths, table, k_cache,
+                      v_cache, first, stride, 0, 0, 0, 0)
+    call("vdsl_op_paged_attention", q.handle, p, qt.handle, k_cache.handle, v_cache.handle, starts.handle, lengths.handle,
          table.handle, out.dtype, out.handle, _h(lse), _h(workspace))

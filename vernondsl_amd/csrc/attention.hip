@@ -245,10 +245,10 @@ struct Place {
 // Waves of 32 rows each, sharing tiles of keys through two slots of LDS.  PARTS 1: four waves and tiles of 64 keys, two blocks to a
 // CU, so that a SIMD has one wave's exponentials beside another's products.  PARTS 4: two times 32 rows with four waves each, which
 // take 32 keys each of a tile of 128 and join what they have at the end.
-// What bounds it: the matrix units are busy 54% of the cycles and the vector units 50%, the two waves of a SIMD only partly beside
-// each other; the reads of LDS (32 KB for 32 products, by each wave) take as long as the products.  64 rows a wave would
-// halve those, but leave a SIMD one wave: 3020 us where this took 2300.  16384 rows, 32 heads of 128 over 8, causal: 2070 us, 1063
-// TFLOP/s (the library's product of 8192^3: 1360).
+// What bounds it: the matrix units are busy 52% of the cycles and the vector units 49%, so the two waves of a SIMD are seldom beside
+// each other in what they do; LDS is active 26%, without bank conflicts.  64 rows a wave would halve its reads, but leave a SIMD
+// one wave: 3020 us where this took 2300.  16384 rows, 32 heads of 128 over 8, causal: 2070 us, 1061 TFLOP/s (the library's product
+// of 8192^3: 1360).
 template <int DP, bool PAGED, int PARTS>
 __global__ __launch_bounds__(PARTS == 1 ? 256 : 512, 2) void attention_rows(AttentionArgs a) {
   static_assert(PARTS == 1 || !PAGED, "a paged cache's keys are split among blocks");

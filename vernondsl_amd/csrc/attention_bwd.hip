@@ -96,9 +96,10 @@ struct RowShare {
 // have 8 / (KEYS / 32) waves, one for each 32 rows of a tile, which add up their sums at the end.  Two waves share a SIMD,
 // and one has priority there, so that its exponentials come beside the other's products.  To leave both their
 // registers, wide heads' values are an operand read from LDS (V_LDS).
-// Bounded by both: the products at the clock that they leave, and the reads of LDS that feed them (a wave's 32 products take 40 KB, so a
-// CU's eight 2560 cycles of LDS for 2048 of the matrix units).  Rows from the last to the first: all blocks begin with rows that
-// they all see, and so read the same ones at about the same time (1287 us for the whole gradient before, 1165 with it).
+// Bounded by the eight waves' turns at products and exponentials (a tile of 64 rows takes a block 2 us; its products 0.85 at 2.4 GHz) and
+// by the longest block, of the first keys (300 tiles where the mean CU has 272, at 8192 rows of two sequences).  Rows from the last to the first:
+// all blocks begin with rows that they all see, and so read the same ones at about the same time (1287 us for the whole
+// gradient before, 1165 with it).
 template <int DP, int KEYS>
 struct KeysShape {
   static constexpr int NW = 8, GROUPS = KEYS / 32, PARTS = NW / GROUPS, TR = 32 * PARTS;

@@ -6,8 +6,8 @@
 // few, keys and rows have one launch.  Every sum is taken in one order, so nothing is added atomically and the bits are
 // the same on every call; the price is that s and dp are formed twice (7 products where 5 would do).  See attention.h for rows,
 // tiles and the order of the products' sums.
-// 8192 rows of two sequences, 32 heads of 128 over 8, causal, 707 GFLOP by five products: 1050 us, of which rows 30, keys 632 (four
-// products, 640 TFLOP/s), what they leave 5, queries 410 (three, 740 TFLOP/s).
+// 8192 rows of two sequences, 32 heads of 128 over 8, causal, 707 GFLOP by five products: 1020 us, of which rows 30, keys 605 (four
+// products, 670 TFLOP/s), what they leave 5, queries 410 (three, 740 TFLOP/s).
 #include <algorithm>
 
 #include "attention.h"
@@ -93,9 +93,8 @@ struct RowShare {
       : first(a.causal ? t.row * a.group / TR : 0), end((t.len * a.group + TR - 1) / TR), tiles((end - first + a.key_splits - 1) / a.key_splits) {}
 };
 // dk and dv: a block has KEYS keys and walks over tiles of rows through a ring of two or three slots of LDS.  Each 32 keys
-// have 8 / (KEYS / 32) waves, one for each 32 rows of a tile, which add up their sums at the end.  Two waves share a SIMD,
-// and one has priority there, so that its exponentials come beside the other's products.  To leave both their
-// registers, wide heads' values are an operand read from LDS (V_LDS).
+// have 8 / (KEYS / 32) waves, one for each 32 rows of a tile, which add up their sums at the end.  Two waves share a SIMD.  To
+// leave both their registers, wide heads' values are an operand read from LDS (V_LDS).
 // Bounded by the eight waves' turns at products and exponentials (a tile of 64 rows takes a block 2 us; its products 0.85 at 2.4 GHz) and
 // by the longest block, of the first keys (300 tiles where the mean CU has 272, at 8192 rows of two sequences).  Rows from the last to the first:
 // all blocks begin with rows that they all see, and so read the same ones at about the same time (1287 us for the whole
@@ -195,7 +194,6 @@ __device__ __forceinline__ void keys_block(const GradArgs& a, int b, char* smem)
       *reinterpret_cast<bf16x8*>(values + (lane & 31) * T::PITCH + (((2 * kk + half) ^ T::swz(lane & 31)) << 4)) = vf[kk];
   }
   int slot = 0;
-  if (wave < 4) __builtin_amdgcn_s_setprio(1);
 #pragma unroll 1
   for (int t = end - 1; t >= first; --t) {
     // Every wave has left the tile before.  Of three slots, the next tile, which is whole, may be on its way.
@@ -256,8 +254,8 @@ __device__ __forceinline__ void keys_block(const GradArgs& a, int b, char* smem)
         dk[d] = MfmaBf16::mma(cols_fragment<DP>(qs, 16 * e, 32 * d), df, dk[d]);
       }
     }
+    reads_ahead<4, DP / 8, 2>();  // the whole gradient 1046 us without, 1019 with these, 1049 with two more
   }
-  __builtin_amdgcn_s_setprio(0);
   if ((late_thread() & 63) == 0) left_out_to[wave] = left_out;
   const GradArgs& z = late_args();
   const bool whole = z.key_splits == 1;

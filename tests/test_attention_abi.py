@@ -60,3 +60,28 @@ def test_no_queue(call, params, operands):
     fn = getattr(_lib.lib, call)
     assert len(fn.argtypes) == 2 + operands
     assert fn(None, C.byref(params()), *[0 if t is C.c_int32 else None for t in fn.argtypes[2:]]) != 0
+
+
+def flat(struct):
+    """A ctypes struct's values in order."""
+    out = []
+    for name, kind in struct._fields_:
+        value = getattr(struct, name)
+        out += flat(value) if issubclass(kind, C.Structure) else [value]
+    return out
+
+
+@pytest.mark.parametrize("packed,struct", [(kernels._ROPE_PARAMS, _lib.RopeParams), (kernels._ATTENTION_PARAMS, _lib.AttentionParams),
+                                           (kernels._PAGED_PARAMS, _lib.PagedParams)])
+def test_packed_params(packed, struct):
+    raw = bytes((7 * i + 1) % 113 for i in range(C.sizeof(struct)))
+    x = struct.from_buffer_copy(raw)
+    assert kernels._pack(packed, *flat(x)) == bytes(x) == raw
+
+
+def test_params_that_do_not_fit():
+    fine = [1, 1, 1, 1, 8, 1, 1.0, 0] + [0] * 12
+    kernels._pack(kernels._ATTENTION_PARAMS, *fine)
+    for at, value in ((0, 1 << 63), (2, 1 << 31), (6, 1e39), (6, None)):
+        with pytest.raises(ValueError):
+            kernels._pack(kernels._ATTENTION_PARAMS, *(value if i == at else x for i, x in enumerate(fine)))

@@ -731,8 +731,9 @@ int vdsl_op_rope(vdsl_queue q, const vdsl_rope_params* p, int32_t x_dtype, vdsl_
  * are unspecified).  Row i of a sequence sees its row j if j <= i or causal is 0.  Head h reads k and v of head
  * h / (heads / kv_heads) (kv_heads divides heads).  With s[j] = scale * q_i . k_j over the visible j:
  *   lse[h][i] = log sum_j exp(s[j]),   out[i][h] = sum_j exp(s[j] - lse) v_j
- * A row of no sequence, or whose scores are -inf all of them, has out 0 and lse -inf.  What a row does not see has no
- * influence on it, NaN and infinity included.  q, k, v: BF16; scores, sums and statistics are f32, the weights
+ * A row of no sequence, or whose scores are -inf all of them, has out 0 and lse -inf, whatever its values hold.  What a row
+ * does not see has no influence on it, NaN and infinity included.  (What it sees with score -inf has weight 0: where its value is
+ * no finite number, the row's may be NaN, as 0 times it is, or not.)  q, k, v: BF16; scores, sums and statistics are f32, the weights
  * exp(s[j] - max) are rounded to bf16 for the second product.  out: F32 or BF16 [n][heads * dim], every row written;
  * lse: F32 [heads][n], or NULL.  dim: a multiple of 8 up to 128.  scale: from 2^-100 to 2^100. */
 typedef struct vdsl_attention_params {

@@ -168,9 +168,8 @@ __device__ __forceinline__ void keys_block(const GradArgs& a, int b, char* smem)
     copies.copy(qp + 2 * (token0 * a.q_stride), dp + 2 * (token0 * a.dout_stride), last - CR * wave, area, area + TR * T::PITCH);
     float* const to = starts + 64 * slot;
     const int r = 32 * part + (lane & 31);
-    // rows that are not there: no weight
     if (r <= last) lds_copy4(reinterpret_cast<const char*>(sp + (half ? delta_at : 0) + t * TR + r), reinterpret_cast<char*>(to));
-    else to[lane] = half ? 0.0f : -3e38f;
+    else to[lane] = 0.0f;  // rows that are not there
   };
   f32x16 dk[DP / 32], dv[DP / 32];
 #pragma unroll
@@ -232,11 +231,12 @@ __device__ __forceinline__ void keys_block(const GradArgs& a, int b, char* smem)
       s[i] = __builtin_amdgcn_exp2f(s[i] * scale2);
       p[i] *= s[i];
     }
-    if (r0 < all_seen) {
-      const int lo = sees_from - r0;
+    // what does not see the key, and rows that are not there: by selection, since 0 times a key of infinity is NaN
+    if (r0 < all_seen || rows < r0 + 32) {
+      const int lo = sees_from - r0, count = rows - sees_from;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const bool in = 8 * (i / 4) + 4 * half + i % 4 >= lo;
+        const bool in = static_cast<uint32_t>(8 * (i / 4) + 4 * half + i % 4 - lo) < static_cast<uint32_t>(count);
         s[i] = in ? s[i] : 0.0f;
         p[i] = in ? p[i] : 0.0f;
       }

@@ -758,7 +758,7 @@ int vdsl_op_attention_fwd(vdsl_queue q, const vdsl_attention_params* p, vdsl_buf
  * buffer as disjoint columns of one stride.  dout, p and ds are rounded to bf16 for the products, which accumulate in f32.
  * (Where some rows of q or dout hold NaN or infinities, bf16 gradients of the keys just behind them may be rounded twice.)
  * The same bits on every call.  workspace: vdsl_attention_bwd_workspace_bytes() bytes of any contents (two calls that
- * overlap in time need two). */
+ * overlap in time need two); never fewer for more rows or sequences, so that one for the largest batch serves all. */
 int vdsl_attention_bwd_workspace_bytes(int64_t n, int64_t seqs, int32_t heads, int32_t kv_heads, int32_t dim, size_t* bytes);
 int vdsl_op_attention_bwd(vdsl_queue q, const vdsl_attention_params* p, int32_t dout_dtype, vdsl_buffer dout, vdsl_buffer qs,
                           vdsl_buffer ks, vdsl_buffer vs, vdsl_buffer starts, int32_t out_dtype, vdsl_buffer out,

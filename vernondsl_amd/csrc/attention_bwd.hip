@@ -537,13 +537,14 @@ int key_tile_log(int64_t n, int64_t kv_heads, bool causal) {
 // about 2 us, and its start and end as long as five) times the rounds of the card's 256 CUs is least.  us with 1 split, as many as
 // make 256 blocks, and these: 1000 rows, 8 heads of 128 over 2 74, 52, 38; 2048 136, 74, 74; 1024 over 8 each 34, 55, 34; 8192, 8
 // over 1 986, 554, 554; 32 over 8: 512 47, 44, 44, 1024 78, 66, 66.
+constexpr int64_t kMostKeySplits = 8;
 int key_splits(int64_t n, int64_t seqs, int64_t heads, int64_t kv_heads) {
   const int64_t with_rows = std::max<int64_t>(1, std::min(seqs, n)), tiles = n * (heads / kv_heads) / 128 / with_rows;
-  const int64_t most = std::min({256 / std::max<int64_t>(1, ((n + 63) >> 6) * kv_heads), tiles, int64_t{8}});
+  const int64_t most = std::min({256 / std::max<int64_t>(1, ((n + 63) >> 6) * kv_heads), tiles, kMostKeySplits});
   int64_t best = 1, least = INT64_MAX;
   for (int64_t s = 1; s <= most; ++s) {
     const int64_t blocks = (row_slots(n, seqs, 1, 6) * s + row_slots(n, seqs, heads / kv_heads, 7)) * kv_heads;
-    const int64_t takes = (blocks + 255) / 256 * (5 * s + tiles) * 840 / s;  // 840: a multiple of 1 .. 8
+    const int64_t takes = (blocks + 255) / 256 * (5 * s + tiles) * 840 / s;  // 840: a multiple of 1 .. kMostKeySplits
     if (takes < least) best = s, least = takes;
   }
   return static_cast<int>(best);
@@ -567,10 +568,18 @@ using namespace vdsl;
 extern "C" int vdsl_attention_bwd_workspace_bytes(int64_t n, int64_t seqs, int32_t heads, int32_t kv_heads, int32_t dim, size_t* bytes) {
   if (!bytes) return fail(VDSL_ERR_INVALID_ARG, "bytes is null");
   VDSL_TRY(attention_check_shape("attention_bwd", n, seqs, heads, kv_heads, dim));
+  // The most that a call of up to so many rows and sequences takes, so that a batch of fewer rows, which may be split more, fits too:
+  // key_splits gives s splits to 256 / (kv_heads * s) tiles of 64 keys at most, and to 128 * s of a sequence's rows at least.
+  int64_t slots = row_slots(n, seqs, 1, 6), split_rows = 0;
+  for (int64_t s = 2; s <= kMostKeySplits; ++s) {
+    const int64_t with = std::min(n, 256 / (kv_heads * s) * 64);
+    if (with * (heads / kv_heads) / 128 < s) continue;
+    slots = std::max(slots, row_slots(with, seqs, 1, 6) * s);
+    split_rows = std::max(split_rows, with * s);
+  }
   // a multiple of 16 bytes before the copy
-  const int splits = key_splits(n, seqs, heads, kv_heads);
-  const size_t flags = nbytes(row_slots(n, seqs, 1, 6), kv_heads, 32 * splits), rows = nbytes(n, heads, 8 + 2 * static_cast<int64_t>(dim));
-  const size_t parts = splits == 1 ? 0 : nbytes(n, static_cast<int64_t>(kv_heads) * dim, 8 * splits);
+  const size_t flags = nbytes(slots, kv_heads, 32), rows = nbytes(n, heads, 8 + 2 * static_cast<int64_t>(dim));
+  const size_t parts = nbytes(split_rows, static_cast<int64_t>(kv_heads) * dim, 8);
   if (flags == kSizeOverflow || rows == kSizeOverflow || parts == kSizeOverflow || rows + flags + 32 < rows || rows + flags + 32 + parts < parts)
     return fail(VDSL_ERR_SHAPE, "attention_bwd workspace size overflows");
   *bytes = rows + flags + parts + 32;

@@ -640,6 +640,7 @@ def attention_fwd(q: Queue, qh, k, v, starts: Tensor, out: Tensor, lse=None, cau
 
 
 def attention_bwd_workspace_bytes(n, seqs, heads, kv_heads, dim) -> int:
+    """Never less for more rows or sequences: a workspace for the largest batch serves smaller ones."""
     b = C.c_size_t()
     call("vdsl_attention_bwd_workspace_bytes", n, seqs, heads, kv_heads, dim, C.byref(b))
     return b.value

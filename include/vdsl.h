@@ -790,9 +790,10 @@ int vdsl_op_cache_append(vdsl_queue q, const vdsl_paged_params* p, vdsl_buffer k
                          vdsl_buffer lengths, vdsl_buffer table, vdsl_buffer k_cache, vdsl_buffer v_cache);
 /* Attention of the new rows over the cache, which holds their own keys already: the row at position p sees positions 0 to p.
  * out, lse, arithmetic and limits as for vdsl_op_attention_fwd; one row a sequence or many.  lengths and table are read on
- * the device: a recorded call takes what they hold at each replay.  workspace:
- * vdsl_paged_attention_workspace_bytes() bytes of any contents (two calls that overlap in time need two); it may be NULL
- * when that is 0. */
+ * the device: a recorded call takes what they hold at each replay.  workspace: any contents (two calls that overlap in time
+ * need two); with vdsl_paged_attention_workspace_bytes() bytes the positions are split into as many parts as is fastest, with
+ * fewer, or NULL, into as many as fit (more time, the sums in another order).  That size may be larger for fewer rows: one
+ * workspace for calls of several sizes is the largest of theirs. */
 int vdsl_paged_attention_workspace_bytes(int64_t n, int64_t seqs, int32_t heads, int32_t kv_heads, int32_t dim,
                                          int64_t positions, size_t* bytes); /* positions: table_cols * page */
 int vdsl_op_paged_attention(vdsl_queue q, const vdsl_paged_params* p, vdsl_buffer qs, vdsl_buffer k_cache, vdsl_buffer v_cache,

@@ -709,6 +709,9 @@ PagedPlan paged_plan(int64_t n, int64_t seqs, int32_t heads, int32_t kv_heads, i
   plan.splits = static_cast<int>(std::max<int64_t>(1, splits));
   return plan;
 }
+// What a split leaves in the workspace.  A call has as many as its workspace holds, so that one made for the most rows, which may have
+// fewer splits, serves any.
+size_t split_bytes(int64_t n, int64_t heads, int64_t dim) { return nbytes(n, heads, 8 + 4 * dim); }
 int paged_check(const char* op, const vdsl_paged_params* p) {
   if (!p) return fail(VDSL_ERR_INVALID_ARG, "params is null");
   VDSL_TRY(attention_check_shape(op, p->n, p->seqs, p->heads, p->kv_heads, p->dim));
@@ -775,7 +778,7 @@ extern "C" int vdsl_paged_attention_workspace_bytes(int64_t n, int64_t seqs, int
   VDSL_TRY(attention_check_shape("paged_attention", n, seqs, heads, kv_heads, dim));
   if (positions < 0) return fail(VDSL_ERR_INVALID_ARG, "negative shape");
   const int splits = paged_plan(n, seqs, heads, kv_heads, positions).splits;
-  *bytes = splits == 1 ? 0 : nbytes(n * heads, splits, 8 + 4 * static_cast<int64_t>(dim));
+  *bytes = splits == 1 ? 0 : splits * split_bytes(n, heads, dim);
   return VDSL_OK;
 }
 
@@ -787,7 +790,7 @@ extern "C" int vdsl_op_paged_attention(vdsl_queue q, const vdsl_paged_params* p,
   VDSL_TRY(paged_check(op, p));
   VDSL_TRY(attention_check_scale(op, p->scale));
   if (!float_type(out_dtype)) return fail(VDSL_ERR_UNSUPPORTED, "paged_attention stores f32 and bf16");
-  size_t qb, need;
+  size_t qb;
   VDSL_TRY(attention_check_heads(op, "q", p->q, p->n, p->heads, p->dim, 2, &qb));
   VDSL_TRY(check_buffer(q, qs, qb, "q", false));
   VDSL_TRY(check_buffer(q, k_cache, cache_bytes(p), "k_cache", false));
@@ -797,10 +800,14 @@ extern "C" int vdsl_op_paged_attention(vdsl_queue q, const vdsl_paged_params* p,
   VDSL_TRY(check_buffer(q, table, nbytes(p->seqs, p->table_cols, 4), "table", false));
   VDSL_TRY(check_buffer(q, out, nbytes(p->n, static_cast<int64_t>(p->heads) * p->dim, dtype_size(out_dtype)), "out", true));
   if (lse) VDSL_TRY(check_buffer(q, lse, nbytes(p->n, p->heads, 4), "lse", true));
-  const int64_t positions = p->table_cols * p->page;
-  VDSL_TRY(vdsl_paged_attention_workspace_bytes(p->n, p->seqs, p->heads, p->kv_heads, p->dim, positions, &need));
-  if (need) VDSL_TRY(check_buffer(q, workspace, need, "workspace", true));
-  VDSL_TRY(check_apart(op, {out, lse, need ? workspace : nullptr}, {qs, k_cache, v_cache, starts, lengths, table}));
+  PagedPlan plan = paged_plan(p->n, p->seqs, p->heads, p->kv_heads, p->table_cols * p->page);
+  if (plan.splits == 1) workspace = nullptr;
+  if (workspace) {
+    VDSL_TRY(check_buffer(q, workspace, 0, "workspace", true));
+    plan.splits = static_cast<int>(std::min<size_t>(plan.splits, workspace->bytes / std::max<size_t>(1, split_bytes(p->n, p->heads, p->dim))));
+  }
+  if (!workspace || plan.splits == 0) plan.splits = 1;
+  VDSL_TRY(check_apart(op, {out, lse, workspace}, {qs, k_cache, v_cache, starts, lengths, table}));
   if (p->n == 0) return VDSL_OK;
   AttentionArgs a = paged_args(p, starts, lengths, table);
   a.q = static_cast<const uint16_t*>(qs->ptr) + p->q.first;
@@ -810,7 +817,6 @@ extern "C" int vdsl_op_paged_attention(vdsl_queue q, const vdsl_paged_params* p,
   a.out = out->ptr;
   a.out_dtype = out_dtype;
   a.lse = lse ? static_cast<float*>(lse->ptr) : nullptr;
-  const PagedPlan plan = paged_plan(p->n, p->seqs, p->heads, p->kv_heads, positions);
   a.splits = plan.splits;
   if (a.splits > 1) {
     a.parts = static_cast<float*>(workspace->ptr);

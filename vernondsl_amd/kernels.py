@@ -704,7 +704,8 @@ def cache_append(q: Queue, k, v, starts: Tensor, lengths: Tensor, table: Tensor,
 
 
 def paged_attention_workspace_bytes(n, seqs, heads, kv_heads, dim, positions) -> int:
-    """positions: those that a row of the page table has room for (its pages times the page size)."""
+    """positions: those that a row of the page table has room for (its pages times the page size).  May be more for fewer rows, which
+    are split into more parts: one workspace for calls of several sizes is the largest of theirs."""
     b = C.c_size_t()
     call("vdsl_paged_attention_workspace_bytes", n, seqs, heads, kv_heads, dim, positions, C.byref(b))
     return b.value
@@ -714,7 +715,8 @@ def paged_attention(q: Queue, qh, k_cache: Tensor, v_cache: Tensor, starts: Tens
                     scale=None, workspace=None):
     """Attention of new rows over a paged cache that holds their own keys already (cache_append): the row at position p sees
     positions 0 to p of its sequence.  qh: bf16 Heads or a tensor [n][heads][dim]; out [n][heads * dim], lse and scale as
-    for attention_fwd.  workspace: paged_attention_workspace_bytes(...) bytes, None where that is 0."""
+    for attention_fwd.  workspace: paged_attention_workspace_bytes(...) bytes; with fewer, or None, the positions are split into as
+    many parts as fit, which takes longer."""
     qt, heads, dim, first, stride = _columns(qh, "q")
     n = qt.shape[0]
     if qt.dtype != _lib.BF16:

@@ -735,7 +735,8 @@ int vdsl_op_rope(vdsl_queue q, const vdsl_rope_params* p, int32_t x_dtype, vdsl_
  * does not see has no influence on it, NaN and infinity included.  (What it sees with score -inf has weight 0: where its value is
  * no finite number, the row's may be NaN, as 0 times it is, or not.)  q, k, v: BF16; scores, sums and statistics are f32, the weights
  * exp(s[j] - max) are rounded to bf16 for the second product.  out: F32 or BF16 [n][heads * dim], every row written;
- * lse: F32 [heads][n], or NULL.  dim: a multiple of 8 up to 128.  scale: from 2^-100 to 2^100. */
+ * lse: F32 [heads][n], or NULL.  dim: a multiple of 8 up to 128.  scale: from 2^-100 to 2^100.  heads: up to 65535;
+ * n * heads up to 2^31 - 2^24; n * heads / 128 + (seqs + 2) * kv_heads below 2^24, for the gradient 2^22 - 2^10. */
 typedef struct vdsl_attention_params {
   int64_t n;
   int64_t seqs;

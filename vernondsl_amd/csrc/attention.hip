@@ -592,12 +592,15 @@ __global__ __launch_bounds__(256) void cache_append_rows(AttentionArgs a, uint16
 
 bool float_type(int32_t t) { return t == VDSL_F32 || t == VDSL_BF16; }
 
+// A launch's blocks of `lanes` lanes: fewer than 2^32 lanes.
+constexpr int64_t most_blocks(int64_t lanes) { return 0xffffffff / lanes; }
+
 // `lanes` to a block, tiles of 2^log_tile rows.
 template <class Kernel>
 int launch_rows(vdsl_queue q, AttentionArgs& a, Kernel kernel, unsigned lanes, int log_tile, const char* name) {
   const int64_t slots = row_slots(a.seqs.n, a.seqs.seqs, a.group, log_tile);
   const int64_t blocks = slots * a.kv_heads * a.splits;
-  if (slots > 0x7fffffff || blocks > 0xffffff) return fail(VDSL_ERR_UNSUPPORTED, "attention: too many rows");
+  if (blocks > most_blocks(lanes)) return fail(VDSL_ERR_UNSUPPORTED, "attention: too many rows or sequences");
   a.blocks = static_cast<int>(slots);
   hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(lanes), 0, q->stream, a);
   return check_launch(name);
@@ -684,7 +687,9 @@ extern "C" int vdsl_op_attention_fwd(vdsl_queue q, const vdsl_attention_params* 
   // Blocks of 128 rows that are few, walking over many keys one after the other, become blocks of 64 with four parts of the keys.
   // us, heads of 128: 1024 rows of 8 over 8 heads (64 blocks) 26 and 17, 2048 of 8 over 2 (128) 42 and 26, 1024 of 32 over 8 (256)
   // 25.8 and 25.6, 2048 of these (512) 52 and 67; 90 rows of 8 over 2 (6) 8.3 and 8.4.
-  if (((p->n * a.group + 127) >> 7) * p->kv_heads <= 192) return launch_rows<false, 4>(q, a);
+  // (Many empty sequences can be more blocks than a launch of 512 lanes each takes.)
+  if (((p->n * a.group + 127) >> 7) * p->kv_heads <= 192 && row_slots(p->n, p->seqs, a.group, 6) * p->kv_heads <= most_blocks(512))
+    return launch_rows<false, 4>(q, a);
   return launch_rows<false, 1>(q, a);
 }
 
@@ -705,7 +710,8 @@ PagedPlan paged_plan(int64_t n, int64_t seqs, int32_t heads, int32_t kv_heads, i
   // heads of 128 unless said): 64 sequences of up to 16384 positions 482, 470, 462; 16 of 4096, 8 / 8 heads 37.3, 42.3, 51.2;
   // 8 of 1000 (15 splits) 14.5 all, of 128 positions at least 15.3.  attention_rows: four rounds; 1024 rows over 16384 positions with 512,
   // 1024 and 1536 blocks 266, 257, 257.
-  const int64_t splits = plan.few ? std::max(split(2560, 64), split(10240, 1024)) : split(1024, 256);
+  const int64_t fit = most_blocks(plan.few ? 64 : 256) / (row_slots(n, seqs, group, plan.few ? 5 : 7) * kv_heads);  // in a launch
+  const int64_t splits = std::min(fit, plan.few ? std::max(split(2560, 64), split(10240, 1024)) : split(1024, 256));
   plan.splits = static_cast<int>(std::max<int64_t>(1, splits));
   return plan;
 }

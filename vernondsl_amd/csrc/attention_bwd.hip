@@ -36,7 +36,7 @@ struct GradArgs {
   float scale;
   Divider token_of;
   int blocks;      // row slots of attention_bwd_queries
-  int key_blocks;  // attention_bwd_both's blocks that are of keys
+  int key_blocks;  // blocks of keys
 };
 
 // The kernel's arguments, read again: what only the end of a kernel takes would hold scalar registers through its main loop, which
@@ -283,7 +283,8 @@ __global__ __launch_bounds__(512, 2) void attention_bwd_keys(GradArgs a) {
 constexpr int kSumBlocks = 16;
 __global__ __launch_bounds__(256) void attention_bwd_finish(GradArgs a) {
   const int sums = a.key_splits > 1 ? kSumBlocks : 1;  // blocks that share a tile's sums
-  const int place = static_cast<int>(blockIdx.x) / sums, sum_block = static_cast<int>(blockIdx.x) % sums;
+  const int block = static_cast<int>(block_index()), place = block / sums, sum_block = block % sums;
+  if (place >= a.key_blocks / a.key_splits) return;
   const int kv = place % a.kv_heads, slot = place / a.kv_heads;
   const int64_t split_step = 8 * a.kv_heads;  // from a split's flags to the next one's
   const int* const flags = a.left_out + slot * a.key_splits * split_step + 8 * kv;
@@ -538,9 +539,11 @@ int key_tile_log(int64_t n, int64_t kv_heads, bool causal) {
 // make 256 blocks, and these: 1000 rows, 8 heads of 128 over 2 74, 52, 38; 2048 136, 74, 74; 1024 over 8 each 34, 55, 34; 8192, 8
 // over 1 986, 554, 554; 32 over 8: 512 47, 44, 44, 1024 78, 66, 66.
 constexpr int64_t kMostKeySplits = 8;
+constexpr int64_t kMostBlocks = 0x3fffff;  // of keys, and of rows: both in one launch of 512 lanes each are fewer than 2^32 lanes
 int key_splits(int64_t n, int64_t seqs, int64_t heads, int64_t kv_heads) {
   const int64_t with_rows = std::max<int64_t>(1, std::min(seqs, n)), tiles = n * (heads / kv_heads) / 128 / with_rows;
-  const int64_t most = std::min({256 / std::max<int64_t>(1, ((n + 63) >> 6) * kv_heads), tiles, kMostKeySplits});
+  const int64_t most = std::min({256 / std::max<int64_t>(1, ((n + 63) >> 6) * kv_heads), tiles, kMostKeySplits,
+                                 kMostBlocks / (row_slots(n, seqs, 1, 6) * kv_heads)});
   int64_t best = 1, least = INT64_MAX;
   for (int64_t s = 1; s <= most; ++s) {
     const int64_t blocks = (row_slots(n, seqs, 1, 6) * s + row_slots(n, seqs, heads / kv_heads, 7)) * kv_heads;
@@ -628,7 +631,8 @@ extern "C" int vdsl_op_attention_bwd(vdsl_queue q, const vdsl_attention_params* 
   const int key_log = key_tile_log(p->n, p->kv_heads, p->causal != 0);
   const int splits = key_log == 6 ? key_splits(p->n, p->seqs, p->heads, p->kv_heads) : 1;
   const int64_t key_slots = row_slots(p->n, p->seqs, 1, key_log), query_slots = row_slots(p->n, p->seqs, group, 7);
-  if (std::max(key_slots * splits, query_slots) * p->kv_heads > 0x3fffff) return fail(VDSL_ERR_UNSUPPORTED, "attention_bwd: too many rows");
+  if (std::max(key_slots * splits, query_slots) * p->kv_heads > kMostBlocks)
+    return fail(VDSL_ERR_UNSUPPORTED, "attention_bwd: too many rows or sequences");
   const int64_t flags_at = 2 * p->n * p->heads, copy_at = (flags_at + 8 * key_slots * splits * p->kv_heads + 3) & ~int64_t{3};
   uint16_t* const copy = dout_dtype == VDSL_F32 ? reinterpret_cast<uint16_t*>(rows + copy_at) : nullptr;
   GradArgs a = {};
@@ -674,7 +678,8 @@ extern "C" int vdsl_op_attention_bwd(vdsl_queue q, const vdsl_attention_params* 
   const auto pick = [&](auto of64, auto of96, auto of128) { return p->dim <= 64 ? of64 : p->dim <= 96 ? of96 : of128; };
   const auto finish = [&]() -> int {
     if (!p->causal && splits == 1) return VDSL_OK;
-    return go(attention_bwd_finish, 256, splits > 1 ? kSumBlocks * tiles : tiles, "attention_bwd_finish");
+    hipLaunchKernelGGL(attention_bwd_finish, block_grid(splits > 1 ? kSumBlocks * tiles : tiles), dim3(256), 0, q->stream, a);
+    return check_launch("attention_bwd_finish");
   };
   a.blocks = static_cast<int>(query_slots);
   a.key_blocks = static_cast<int>(key_blocks);

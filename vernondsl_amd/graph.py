@@ -313,7 +313,8 @@ class Graph:
     def backward(self, loss: Value) -> dict:
         """Appends the backward ops of `loss` and returns {param name: f32 gradient Value} for every param that the loss
         depends on through an operand with a rule above, whichever operand that is (a learned position table that is
-        added, a computed weight, table or gain); an mse_loss's target is a constant.  The Value is named grad_<param>
+        added, a computed weight, table or gain); an mse_loss's target is a constant.  Ops without a rule (int8 layers, paged
+        attention) may stand beside what the loss depends on, not in it.  The Value is named grad_<param>
         in general, but not where it is another value's gradient as well (an operand of add): read it by its own name."""
         if loss.producer is None or loss.producer.kind not in ("mse", "linear_xent"):
             raise ValueError("backward() starts from an mse_loss or a linear_cross_entropy value")
@@ -357,11 +358,11 @@ class Graph:
         for op in reversed(fwd_ops):
             if op.kind in ("mse", "linear_xent"):
                 continue
-            if op.kind not in ("linear", "linear_mse", "add", "embedding", "layer_norm", "rope", "attention"):
-                raise NotImplementedError(f"no backward rule for {op.kind}")
-            y = op.outputs[0]
-            if y.name not in grad:
+            if not any(v.name in grad for v in op.outputs):  # the loss does not depend on it
                 continue
+            y = op.outputs[0]
+            if op.kind not in ("linear", "linear_mse", "add", "embedding", "layer_norm", "rope", "attention") or y.name not in grad:
+                raise NotImplementedError(f"no backward rule for {op.kind}")
             if op.kind == "add":  # d(a + b) passes dL/dy to both operands
                 for x in op.inputs:
                     self._give(x, grad[y.name], grad, contrib)

@@ -346,12 +346,9 @@ __device__ __forceinline__ void store_sums(const f32x16 (&acc)[DP / 32], float b
 // Copies 4 bytes a lane straight to LDS, lane l's to l + 4 l.
 __device__ __forceinline__ void lds_copy4(const char* g, char* l) { __builtin_amdgcn_global_load_lds(g, (lds_void_t*)l, 4, 0, 0); }
 
-// Waits of the counts of copies that gemm_dma.h has none for.
-#define VDSL_DMA_WAIT_CASE(n) \
-  template <> __device__ __forceinline__ void dma_wait<n>() { __builtin_amdgcn_s_waitcnt(((n) & 0xF) | (((n) >> 4) << 14) | (0x7 << 4)); }
-VDSL_DMA_WAIT_CASE(5)
-VDSL_DMA_WAIT_CASE(10)
-#undef VDSL_DMA_WAIT_CASE
+// A wait for all but the last 5 copies, a count that gemm_dma.h has none for.
+template <>
+__device__ __forceinline__ void dma_wait<5>() { __builtin_amdgcn_s_waitcnt(5 | (0x7 << 4)); }
 
 // r / group for r below 2^31.
 struct Divider {

@@ -85,7 +85,7 @@ struct KeySource {
 // What a block's rows see, and where they are.
 struct RowsAt {
   int64_t token;  // of row 0 of the piece
-  int len, rows;  // tokens and rows of the piece
+  int rows;       // of the piece
   int keys;       // of its sequence
   int before;     // keys before its first token (negative: its first tokens have none)
   __device__ __forceinline__ int sees(int row, int group, int causal) const {
@@ -97,7 +97,6 @@ template <bool PAGED>
 __device__ __forceinline__ RowsAt rows_at(const AttentionArgs& a, const RowTile& t) {
   RowsAt r;
   r.token = t.token;
-  r.len = t.len;
   r.rows = t.len * a.group;
   r.keys = t.len;
   r.before = 0;
@@ -590,8 +589,6 @@ __global__ __launch_bounds__(256) void cache_append_rows(AttentionArgs a, uint16
     *reinterpret_cast<u32x4*>((is_v ? v_cache : k_cache) + to) = *reinterpret_cast<const u32x4*>(from + 8 * x);
   }
 }
-
-bool float_type(int32_t t) { return t == VDSL_F32 || t == VDSL_BF16; }
 
 // A launch's blocks of `lanes` lanes: fewer than 2^32 lanes.
 constexpr int64_t most_blocks(int64_t lanes) { return 0xffffffff / lanes; }

@@ -553,8 +553,6 @@ int key_splits(int64_t n, int64_t seqs, int64_t heads, int64_t kv_heads) {
   return static_cast<int>(best);
 }
 
-bool float_type(int32_t t) { return t == VDSL_F32 || t == VDSL_BF16; }
-
 // Whether two of the gradients, as columns of one buffer, have no element in common.
 bool apart(const vdsl_heads& x, int64_t x_width, const vdsl_heads& y, int64_t y_width) {
   if (x.stride != y.stride) return false;

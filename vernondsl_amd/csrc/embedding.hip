@@ -423,8 +423,6 @@ __global__ __launch_bounds__(256) void embedding_bwd_few_kernel(const int32_t* _
   store_row<U, NV, false>(dtable, v, dim, at, scale, acc);
 }
 
-bool float_type(int32_t t) { return t == VDSL_F32 || t == VDSL_BF16; }
-
 // log2 of the lanes that share a row of `units` units: a power of two from 16 to 256.
 int lanes_log2(int64_t units) {
   int l = 4;

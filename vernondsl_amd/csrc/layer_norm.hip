@@ -466,8 +466,6 @@ int64_t bwd_blocks(int64_t rows, int64_t together, int64_t bytes) {
 }
 int64_t bwd_most_blocks(int64_t rows, int64_t cols) { return bwd_blocks(rows, cols <= 1024 ? 4 : 1, 4 * std::min<int64_t>(cols, 1 << 24)); }
 
-bool float_type(int32_t t) { return t == VDSL_F32 || t == VDSL_BF16; }
-
 }  // namespace
 }  // namespace vdsl
 

@@ -112,8 +112,6 @@ __global__ __launch_bounds__(256) void rope_rows(RopeArgs p) {
   }
 }
 
-bool float_type(int32_t t) { return t == VDSL_F32 || t == VDSL_BF16; }
-
 }  // namespace
 }  // namespace vdsl
 

@@ -23,6 +23,9 @@ struct __attribute__((packed, aligned(4))) F32x4At4 {
   typedef f32x4 At __attribute__((aligned(4)));
 };
 
+// The types that rows may have.
+inline bool float_type(int32_t t) { return t == VDSL_F32 || t == VDSL_BF16; }
+
 // A grid of `blocks` blocks of up to 1024 lanes (times y): a launch takes fewer than 2^32 lanes along x, so x holds
 // 2^21 blocks and z what that leaves.  The last of z may hold more: a kernel returns from those past its own.
 inline dim3 block_grid(int64_t blocks, int64_t y = 1) {

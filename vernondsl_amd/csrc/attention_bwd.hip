@@ -221,8 +221,7 @@ __device__ __forceinline__ void keys_block(const GradArgs& a, int b, char* smem)
       s = MfmaBf16::mma(rows_fragment<DP>(qs, 0, kk), kf[kk], s);
       p = MfmaBf16::mma(rows_fragment<DP>(ds, 0, kk), V_LDS ? rows_fragment<DP>(values, 0, kk) : vf[kk], p);
     }
-    if constexpr (V_LDS) reads_ahead<14, DP / 8, 2>();  // the first 8 are of what they start from
-    else reads_ahead<12, DP / 8, 1>();
+    if constexpr (!V_LDS) reads_ahead<12, DP / 8, 1>();  // the first 8 are of what they start from.  (V_LDS has no registers for it.)
     // a row whose q or dout holds an element that is no finite number has no finite score or dp with any key
     bool leave = false;
     if (r0 < all_seen) leave = left_out > 0 || any_not_finite(s) || any_not_finite(p);

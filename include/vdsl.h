@@ -756,7 +756,8 @@ int vdsl_op_attention_fwd(vdsl_queue q, const vdsl_attention_params* p, vdsl_buf
  *   dq_i = scale * sum_j ds k_j,   dk_j = scale * sum_i ds q_i,   dv_j = sum_i p dout_i
  * (the last two over the rows i that see j and the heads that share j's).  dq, dk, dv: grad_dtype, F32 or BF16, every row
  * of their heads written (0 for rows of no sequence), columns outside their heads left as they are; they may lie in one
- * buffer as disjoint columns of one stride.  dout, p and ds are rounded to bf16 for the products, which accumulate in f32.
+ * buffer as disjoint columns of one stride.  dout, p and ds are rounded to bf16 for the products, which accumulate in f32;
+ * dout_i . out_i takes dout as rounded too, so that it is the mean of the dout_i . v_j that it is taken from.
  * (Where some rows of q or dout hold NaN or infinities, bf16 gradients of the keys just behind them may be rounded twice.)
  * The same bits on every call.  workspace: vdsl_attention_bwd_workspace_bytes() bytes of any contents (two calls that
  * overlap in time need two); never fewer for more rows or sequences, so that one for the largest batch serves all. */
@@ -794,7 +795,8 @@ int vdsl_op_cache_append(vdsl_queue q, const vdsl_paged_params* p, vdsl_buffer k
  * the device: a recorded call takes what they hold at each replay.  workspace: any contents (two calls that overlap in time
  * need two); with vdsl_paged_attention_workspace_bytes() bytes the positions are split into as many parts as is fastest, with
  * fewer, or NULL, into as many as fit (more time, the sums in another order).  That size may be larger for fewer rows: one
- * workspace for calls of several sizes is the largest of theirs. */
+ * workspace for calls of several sizes is the largest of theirs.  (A table with room for many more positions than the sequences
+ * have takes more time, too.) */
 int vdsl_paged_attention_workspace_bytes(int64_t n, int64_t seqs, int32_t heads, int32_t kv_heads, int32_t dim,
                                          int64_t positions, size_t* bytes); /* positions: table_cols * page */
 int vdsl_op_paged_attention(vdsl_queue q, const vdsl_paged_params* p, vdsl_buffer qs, vdsl_buffer k_cache, vdsl_buffer v_cache,

@@ -231,7 +231,8 @@ __device__ __forceinline__ void store_none(const AttentionArgs& a, const RowsAt&
 }
 
 // The block's place: kv head, row slot and split.  Blocks that are dispatched together (to the XCDs in turn) have
-// different kv heads, so that an XCD reads few heads' keys where there are 8 or more; the last rows, which see most, first.
+// different kv heads, so that an XCD reads few heads' keys where there are 8 or more; the last rows first, which see most of their
+// sequence.
 struct Place {
   int kv, split;
   int64_t slot;
@@ -247,7 +248,7 @@ struct Place {
 // Waves of 32 rows each, sharing tiles of keys through two slots of LDS.  PARTS 1: four waves and tiles of 64 keys, two blocks to a
 // CU, so that a SIMD has one wave's exponentials beside another's products.  PARTS 4: two times 32 rows with four waves each, which
 // take 32 keys each of a tile of 128 and join what they have at the end.
-// What bounds it: the matrix units are busy 52% of the cycles and the vector units 49%, so the two waves of a SIMD are seldom beside
+// What bounds it: the matrix units are busy 54% of the cycles and the vector units 50%, so the two waves of a SIMD are seldom beside
 // each other in what they do; LDS is active 26%, without bank conflicts.  64 rows a wave would halve its reads, but leave a SIMD
 // one wave: 3020 us where this took 2300.  16384 rows, 32 heads of 128 over 8, causal: 2070 us, 1061 TFLOP/s (the library's product
 // of 8192^3: 1360).
@@ -422,8 +423,9 @@ __global__ __launch_bounds__(PARTS == 1 ? 256 : 512, 2) void attention_rows(Atte
 }
 
 // Few rows: a block is one wave with 32 rows and a split of the keys, in tiles of 32 through two slots of LDS of its own, so
-// that nothing waits for another wave.  What bounds it is the cache's bytes: five such blocks to a CU keep 80 KiB of them
-// on their way.  64 sequences of up to 16384 positions, 32 heads of 128 over 8 (2.7 GB): 460-500 us, 5.4-5.9 TB/s, where blocks of
+// that nothing waits for another wave.  What bounds it is the cache's bytes: five such blocks to a CU have up to 80 KiB of them on their
+// way, each from a tile's start to its second products (the compiler takes the transposing reads for readers of what the copies
+// write, and waits for all of them there).  64 sequences of up to 16384 positions, 32 heads of 128 over 8 (2.7 GB): 460-500 us, 5.4-5.9 TB/s, where blocks of
 // attention_rows had 645; a copy of 2 GiB moves 4.9.
 template <int DP>
 __global__ __launch_bounds__(64, 2) void attention_few(AttentionArgs a) {
@@ -693,7 +695,9 @@ extern "C" int vdsl_op_attention_fwd(vdsl_queue q, const vdsl_attention_params* 
 
 namespace vdsl {
 namespace {
-// How the rows' keys are split.  few: attention_few, where a sequence has up to 32 rows on average.
+// How the rows' keys are split.  few: attention_few, where a sequence has up to 32 rows on average.  (One form for a batch, by its
+// sizes alone: 63 single tokens over 8192 positions take 376 us and a chunk of 512 rows 97, both in one call 487; that chunk alone among
+// 63 empty sequences, with which the average is 8 rows, 190.)
 struct PagedPlan {
   bool few;
   int splits;
@@ -703,8 +707,11 @@ PagedPlan paged_plan(int64_t n, int64_t seqs, int32_t heads, int32_t kv_heads, i
   PagedPlan plan = {n * group <= 32 * with_rows, 1};
   const int64_t tiles = (n * group / (plan.few ? 32 : 128) + with_rows) * kv_heads;
   const auto split = [&](int64_t blocks, int64_t least) { return std::min<int64_t>({(blocks + tiles - 1) / tiles, positions / least, 256}); };
-  // attention_few: two rounds of the blocks the card holds, of 64 positions at least, or eight rounds, which sequences of
-  // different lengths are better spread over, of 1024.  us with 2560, 5120 and 10240 blocks of 64 positions at least (32 / 8
+  // attention_few: two rounds of the blocks the card holds, of 64 positions of the table's room at least, or eight rounds, which
+  // sequences of different lengths are better spread over, of 1024.  The lengths are on the device: a table of more room than they take
+  // makes empty splits, which cost their blocks and the join: 8 single tokens over 1000 positions 15 us with room for 1008, 21 for
+  // 16384, 29 for 131072.  (Two tiles a split at least in the kernel: 19 and 28 there, but 12.3 for 12.1 and 18.5 for 17.5 of
+  // sequences of 500.)  us with 2560, 5120 and 10240 blocks of 64 positions at least (32 / 8
   // heads of 128 unless said): 64 sequences of up to 16384 positions 482, 470, 462; 16 of 4096, 8 / 8 heads 37.3, 42.3, 51.2;
   // 8 of 1000 (15 splits) 14.5 all, of 128 positions at least 15.3.  attention_rows: four rounds; 1024 rows over 16384 positions with 512,
   // 1024 and 1536 blocks 266, 257, 257.

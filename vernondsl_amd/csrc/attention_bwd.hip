@@ -6,8 +6,8 @@
 // few, keys and rows have one launch.  Every sum is taken in one order, so nothing is added atomically and the bits are
 // the same on every call; the price is that s and dp are formed twice (7 products where 5 would do).  See attention.h for rows,
 // tiles and the order of the products' sums.
-// 8192 rows of two sequences, 32 heads of 128 over 8, causal, 707 GFLOP by five products: 1020 us, of which rows 30, keys 605 (four
-// products, 670 TFLOP/s), what they leave 5, queries 410 (three, 740 TFLOP/s).
+// 8192 rows of two sequences, 32 heads of 128 over 8, causal, 707 GFLOP by five products: 1005 us, of which rows 30, keys 580 (four
+// products, 700 TFLOP/s), what they leave 5, queries 390 (three, 780 TFLOP/s).
 #include <algorithm>
 
 #include "attention.h"
@@ -195,7 +195,9 @@ __device__ __forceinline__ void keys_block(const GradArgs& a, int b, char* smem)
   int slot = 0;
 #pragma unroll 1
   for (int t = end - 1; t >= first; --t) {
-    // Every wave has left the tile before.  Of three slots, the next tile, which is whole, may be on its way.
+    // Every wave has left the tile before.  Of three slots, the next tile, which is whole, may be on its way, and those issued
+    // below until this tile's second products (where the compiler waits for all copies: it takes the transposing reads for readers of
+    // what they write).
     if (NS == 3 && t > first) dma_wait<2 * Copies::C + 1>();
     else dma_wait<0>();
     dma_barrier();

@@ -4,7 +4,8 @@
 //
 // A block has one row.  Its angles depend on the pair alone, so they are made once a row and shared through LDS by all
 // heads (one sine and cosine per row and pair, whatever the number of heads); the rest is a copy at memory rate, which bounds
-// it: 16384 rows of 48 heads of 128, of which 40 turn, f32 to bf16 (604 MB) take 107 us, 5.6 TB/s; 8 rows a launch.  The turns
+// it: 16384 rows of 48 heads of 128, of which 40 turn, f32 to bf16 (604 MB) take 107 us, 5.6 TB/s; 8 rows a launch.  Pairs and widths
+// that are no multiples of 4 move single elements: 48 heads of 126 in bf16, 63 pairs each, 3.7 TB/s where heads of 128 have 5.6.  The turns
 // p f are formed in f64: at p = 2^20 a product in f32 would hold its fraction to 2^-4 only.  They leave as a
 // fraction of a turn in [-1/2, 1/2], of which f32 sine and cosine are good to their last place.
 #include <algorithm>

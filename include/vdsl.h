@@ -735,7 +735,8 @@ int vdsl_op_rope(vdsl_queue q, const vdsl_rope_params* p, int32_t x_dtype, vdsl_
  * does not see has no influence on it, NaN and infinity included.  (What it sees with score -inf has weight 0: where its value is
  * no finite number, the row's may be NaN, as 0 times it is, or not.)  q, k, v: BF16; scores, sums and statistics are f32, the weights
  * exp(s[j] - max) are rounded to bf16 for the second product.  out: F32 or BF16 [n][heads * dim], every row written;
- * lse: F32 [heads][n], or NULL.  dim: a multiple of 8 up to 128.  scale: from 2^-100 to 2^100.  heads: up to 65535;
+ * lse: F32 [heads][n], or NULL.  dim: a multiple of 8 up to 128.  scale: from 2^-100 to 2^100, scores up to
+ * 2^30 in magnitude (past that f32 holds the maximum too coarsely: out may be 0 or NaN).  heads: up to 65535;
  * n * heads up to 2^31 - 2^24; n * heads / 128 + (seqs + 2) * kv_heads below 2^24, for the gradient 2^22 - 2^10. */
 typedef struct vdsl_attention_params {
   int64_t n;
@@ -759,6 +760,7 @@ int vdsl_op_attention_fwd(vdsl_queue q, const vdsl_attention_params* p, vdsl_buf
  * buffer as disjoint columns of one stride.  dout, p and ds are rounded to bf16 for the products, which accumulate in f32;
  * dout_i . out_i takes dout as rounded too, so that it is the mean of the dout_i . v_j that it is taken from.
  * (Where some rows of q or dout hold NaN or infinities, bf16 gradients of the keys just behind them may be rounded twice.)
+ * p is formed from lse as f32 holds it, so its relative error grows with the scores, as 2^-22 of them.
  * The same bits on every call.  workspace: vdsl_attention_bwd_workspace_bytes() bytes of any contents (two calls that
  * overlap in time need two); never fewer for more rows or sequences, so that one for the largest batch serves all. */
 int vdsl_attention_bwd_workspace_bytes(int64_t n, int64_t seqs, int32_t heads, int32_t kv_heads, int32_t dim, size_t* bytes);

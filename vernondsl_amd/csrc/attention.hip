@@ -2,9 +2,9 @@
 //
 // For a row's scores s over the keys it sees: m = max s, p = exp2(c (s - m)), l = sum p, out = sum p v / l, with
 // c = scale log2 e; one pass over the keys, tile by tile, with m, l and the unnormalised output carried along and
-// rescaled where m grows.  The exponent is one fma, c s - m, whose m = c max s is off by up to 2^-25 of itself: the same factor for all
-// of a row's p, which drops out; it stays within f32 for scores up to 2^30.  m may lag behind the maximum by a factor of 2^8 in p (bf16 and f32 hold that without loss), so
-// most tiles rescale nothing.  See attention.h for rows, tiles and the order of keys in the products.
+// rescaled where m grows.  The exponent is one fma, c s - m, whose m = c max s is off by up to 2^-25 of itself: the same factor
+// for all of a row's p, which drops out; it stays within f32 for scores up to 2^30.  m may lag behind the maximum by a factor of
+// 2^8 in p (bf16 and f32 hold that without loss), so most tiles rescale nothing.  See attention.h for rows, tiles and the order of keys in the products.
 #include <algorithm>
 #include <cmath>
 
